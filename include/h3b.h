@@ -41,7 +41,8 @@ enum h3b_dtype {
   H3B_FP16 = 1,
   H3B_FP32 = 2,
   H3B_FP8_E4M3 = 3, /* float8_e4m3fn group scales (raw bytes) */
-  H3B_INT32 = 4     /* int32 accumulator output (parity dump) */
+  H3B_INT32 = 4,    /* int32 accumulator output (parity dump); int32 positions */
+  H3B_INT64 = 5     /* int64 positions */
 };
 
 enum h3b_quant_mode {
@@ -128,6 +129,67 @@ int h3b_gate_residual(void* x, int x_dtype, int64_t ldx, const void* other, int6
 int h3b_attn_merge(float* acc, float* acc_lse, const void* o, int64_t o_head_stride, int64_t o_query_stride, int o_dtype,
                    const float* lse, int64_t heads, int64_t queries, int head_dim, int first, void* out, int64_t ldo,
                    void* stream);
+
+/* Rotary embedding of q and k from positions on several axes (time, height, width), out of place (no reference
+ * counterpart as one operator: rope_angles and the rotation of norm_rope_, layout.py:265-273, 348-355, without the norm
+ * and without cos / sin tables).
+ *   theta[b, s, j] = pos[b, s, axis(j)] * inv_freq[j],  j < F = sum(sections), axis(j) the section that holds j
+ *   pair j: channels (j, j + F) H3B_PAIR_HALF, (2 j, 2 j + 1) H3B_PAIR_ADJACENT; channels >= 2 F are copied
+ *   (a, b) -> (a cos - b sin, a sin + b cos) in fp32, one rounding;  inverse != 0: by -theta (the gradient's direction)
+ *   q, k       one of them may be null; S tokens (0 is valid) of `heads` heads, strides in elements, channels contiguous;
+ *              any stride and alignment (16-byte aligned rows are faster); y must not overlap x
+ *   pos        [B, S, n_axes] of pos_dtype (fp32, int32, int64), axes contiguous, strides in elements (0: shared)
+ *   inv_freq   DEVICE fp32 [F];  sections: HOST int32 [n_axes], n_axes <= H3B_MAX_AXES, 2 F <= head_dim <= 1024 */
+#define H3B_MAX_AXES 8
+enum h3b_rope_pairing { H3B_PAIR_HALF = 0, H3B_PAIR_ADJACENT = 1 };
+typedef struct h3b_rope_operand {
+  const void* x;
+  void* y;
+  const void* pos;
+  int64_t S, x_stride_b, x_stride_s, x_stride_h, y_stride_b, y_stride_s, y_stride_h, pos_stride_b, pos_stride_s;
+  int32_t heads;
+} h3b_rope_operand;
+int h3b_rope_axes(const h3b_rope_operand* q, const h3b_rope_operand* k, int x_dtype, int64_t B, int head_dim,
+                  const float* inv_freq, const int32_t* sections, int n_axes, int pos_dtype, int pairing, int inverse,
+                  void* stream);
+
+/* Cross attention: softmax attention of q over another stream's k and v (no reference counterpart: the reference's
+ * attention is one stream's own, model.py:196-228).  s_ij = scale q_i . k_j + bias_j,  o_i = sum_j softmax_j(s_ij) v_j.
+ *   q, o       [B, Sq, Hq, head_dim];  k, v: [B, Sk, Hkv, head_dim] of dtype (bf16 or fp16); Hq a multiple of Hkv (query
+ *              head h reads key head h / (Hq / Hkv)); strides in elements, multiples of 8, channels contiguous, every
+ *              tensor 16-byte aligned; head_dim a multiple of 8, at most 128; scale > 0
+ *   kv_lens    optional DEVICE int32 [B]: only keys j < kv_lens[b] take part
+ *   mask       optional DEVICE key mask, rows ldm elements apart (0: shared): H3B_MASK_BOOL uint8 [B, Sk], 0 leaves the
+ *              key out; H3B_MASK_BIAS fp32 [B, Sk] added to the scaled scores, -inf leaves the key out.  The largest bias
+ *              in use of a batch entry is taken off all of them first: the softmax does not change, and `lse` is that of
+ *              the scores so shifted
+ *   lse        optional fp32 [B, Hq, Sq]: natural log of sum_j exp(s_ij)
+ * A query without keys (Sk = 0, kv_lens 0, all masked) gets o = 0 and lse = -inf.  What keys that are left out hold (NaN
+ * and infinities too) never reaches a result.  Products take operands of dtype and add up in fp32; softmax and sums are
+ * fp32; the probabilities are rounded to dtype for the second product.
+ * workspace >= h3b_cross_attention_workspace_bytes(..., backward = 0), 256-byte aligned (may be null when that is 0). */
+enum h3b_mask_kind { H3B_MASK_NONE = 0, H3B_MASK_BOOL = 1, H3B_MASK_BIAS = 2 };
+typedef struct h3b_attn_tensor {
+  void* ptr;
+  int64_t stride_b, stride_s, stride_h;
+} h3b_attn_tensor;
+size_t h3b_cross_attention_workspace_bytes(int64_t B, int64_t Sq, int64_t Sk, int Hq, int Hkv, int head_dim, int mask_kind,
+                                           int backward);
+int h3b_cross_attention(const h3b_attn_tensor* q, const h3b_attn_tensor* k, const h3b_attn_tensor* v,
+                        const h3b_attn_tensor* o, int dtype, int64_t B, int64_t Sq, int64_t Sk, int Hq, int Hkv,
+                        int head_dim, float scale, const int32_t* kv_lens, const void* mask, int mask_kind, int64_t ldm,
+                        float* lse, void* workspace, size_t ws_bytes, void* stream);
+
+/* Gradients of h3b_cross_attention's o with respect to q, k and v; o and lse are the forward's, the other arguments the
+ * same.  grad_o, dq: as q; dk, dv: as k.  Shared heads add up; keys that are left out get zero gradients.  Every sum has a
+ * fixed order (no atomics): the same call gives the same bits.  The mask has no gradient.
+ * workspace >= h3b_cross_attention_workspace_bytes(..., backward = 1). */
+int h3b_cross_attention_backward(const h3b_attn_tensor* grad_o, const h3b_attn_tensor* q, const h3b_attn_tensor* k,
+                                 const h3b_attn_tensor* v, const h3b_attn_tensor* o, const float* lse,
+                                 const h3b_attn_tensor* dq, const h3b_attn_tensor* dk, const h3b_attn_tensor* dv, int dtype,
+                                 int64_t B, int64_t Sq, int64_t Sk, int Hq, int Hkv, int head_dim, float scale,
+                                 const int32_t* kv_lens, const void* mask, int mask_kind, int64_t ldm, void* workspace,
+                                 size_t ws_bytes, void* stream);
 
 /* int4 codebook indices + group scales -> the exact int8 grid [N, K] (row stride ldg bytes).
  * Replaces decode_int8_grid / _decode_rows / _pair_lut (qlinear.py:157-204).

@@ -19,7 +19,10 @@ NOALLOC_SCRATCH_BYTES = 16 << 20  # H3B_NOALLOC_SCRATCH_BYTES
 
 # enum h3b_status / h3b_dtype / h3b_quant_mode
 OK, ERR_ARG, ERR_CUDA, ERR_UNSUPPORTED, ERR_DEVICE = 0, 1, 2, 3, 4
-BF16, FP16, FP32, FP8_E4M3, INT32 = 0, 1, 2, 3, 4
+BF16, FP16, FP32, FP8_E4M3, INT32, INT64 = 0, 1, 2, 3, 4, 5
+PAIRING = {"half": 0, "adjacent": 1}  # enum h3b_rope_pairing
+MASK_NONE, MASK_BOOL, MASK_BIAS = 0, 1, 2  # enum h3b_mask_kind
+MAX_AXES = 8  # H3B_MAX_AXES
 QMODE = {"ck": 0, "eager": 1}
 COPY_DIRECT, COPY_STAGED, COPY_PAGEABLE = 0, 1, 2
 
@@ -32,6 +35,23 @@ _lib: Optional[ctypes.CDLL] = None
 _load_error: Optional[str] = None
 
 _c_void_p, _i64, _int, _sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t
+
+
+class RopeOperand(ctypes.Structure):
+    """struct h3b_rope_operand"""
+
+    _fields_ = [("x", _c_void_p), ("y", _c_void_p), ("pos", _c_void_p),
+                *[(n, _i64) for n in ("S", "x_stride_b", "x_stride_s", "x_stride_h", "y_stride_b", "y_stride_s",
+                                      "y_stride_h", "pos_stride_b", "pos_stride_s")], ("heads", ctypes.c_int32)]
+
+
+class AttnTensor(ctypes.Structure):
+    """struct h3b_attn_tensor"""
+
+    _fields_ = [("ptr", _c_void_p), ("stride_b", _i64), ("stride_s", _i64), ("stride_h", _i64)]
+
+
+_rope_p, _attn_p = ctypes.POINTER(RopeOperand), ctypes.POINTER(AttnTensor)
 _SIGNATURES = {
     "h3b_version": ([], _int),
     "h3b_last_error": ([], ctypes.c_char_p),
@@ -47,6 +67,13 @@ _SIGNATURES = {
                            _c_void_p, _c_void_p], _int),
     "h3b_attn_merge": ([_c_void_p, _c_void_p, _c_void_p, _i64, _i64, _int, _c_void_p, _i64, _i64, _int, _int, _c_void_p, _i64,
                         _c_void_p], _int),
+    "h3b_rope_axes": ([_rope_p, _rope_p, _int, _i64, _int, _c_void_p, _c_void_p, _int, _int, _int, _int, _c_void_p], _int),
+    "h3b_cross_attention_workspace_bytes": ([_i64, _i64, _i64, _int, _int, _int, _int, _int], _sz),
+    "h3b_cross_attention": ([_attn_p] * 4 + [_int, _i64, _i64, _i64, _int, _int, _int, ctypes.c_float, _c_void_p, _c_void_p,
+                                             _int, _i64, _c_void_p, _c_void_p, _sz, _c_void_p], _int),
+    "h3b_cross_attention_backward": ([_attn_p] * 5 + [_c_void_p] + [_attn_p] * 3 +
+                                     [_int, _i64, _i64, _i64, _int, _int, _int, ctypes.c_float, _c_void_p, _c_void_p, _int,
+                                      _i64, _c_void_p, _sz, _c_void_p], _int),
     "h3b_w4a8_gemm_decodes_in_kernel": ([_i64, _i64, _i64, _c_void_p, _i64, _int, _int], _int),
     "h3b_decode_grid": ([_c_void_p, _i64, _i64, _i64, _c_void_p, _int, _i64, _c_void_p, _int, _c_void_p, _i64, _c_void_p], _int),
     "h3b_int8_gemm_s32": ([_c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _i64, _c_void_p, _i64, _c_void_p], _int),

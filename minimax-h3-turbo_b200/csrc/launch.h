@@ -4,6 +4,8 @@
 // Translation units (compiled in parallel, linked into one library without relocatable device code):
 //   k_act.cu      rotate + quantise (rotq.cuh), RMSNorm + modulation (rmsmod.cuh), q/k norm + RoPE (rope.cuh),
 //                 attention merge (attn_merge.cuh)
+//   k_rope_axes.cu  rotary embedding from positions on several axes (rope_axes.cuh)
+//   k_cross.cu    cross attention and its gradients (cross_attn.cuh)
 //   k_decode.cu   int4 -> int8 grid decode (decode.cuh)
 //   k_gemm.cu     int8 GEMM + epilogue, 1-CTA and CTA-pair kernels (gemm_sm100.cuh)
 //   k_w4.cu       dispatch of the decode-in-producer W4A8 GEMM for few M tiles (gemm_w4.cuh), instantiated per group
@@ -61,6 +63,18 @@ int qk_norm_rope_launch(void* q, int64_t ldq, void* k, int64_t ldk, int x_dtype,
 int attn_merge_launch(float* acc, float* acc_lse, const void* o, int64_t o_sh, int64_t o_sq, const float* lse, int64_t H,
                       int64_t Q, int D, int first, void* out, int64_t ldo, cudaStream_t st);
 
+// ---- k_rope_axes.cu
+int rope_axes_launch(const h3b_rope_operand* q, const h3b_rope_operand* k, int x_dtype, int64_t B, int D,
+                     const float* inv_freq, const int32_t* sections, int axes, int pos_dtype, int pairing, int inverse,
+                     cudaStream_t st);
+
+// ---- k_cross.cu
+size_t cross_workspace(int64_t B, int64_t Sq, int64_t Sk, int Hq, int Hkv, int D, int mask_kind, bool backward);
+// t: q, k, v, o, and for the backward pass do, dq, dk, dv
+int cross_launch(const h3b_attn_tensor* t, int dtype, int64_t B, int64_t Sq, int64_t Sk, int Hq, int Hkv, int D, float scale,
+                 const int32_t* kv_lens, const void* mask, int mask_kind, int64_t ldm, float* lse, void* ws, bool backward,
+                 cudaStream_t st);
+
 // ---- k_decode.cu
 int decode_launch(const void* q4, int64_t N, int64_t K, int64_t ldq4, const void* s_rel, int s_dtype, int64_t lds,
                   const float* codebook, int group, int8_t* grid, int64_t ldg, cudaStream_t st);
@@ -87,5 +101,6 @@ cudaError_t device_error_w4_fp8(unsigned* v, int clear);
 cudaError_t device_error_w4_fp16(unsigned* v, int clear);
 cudaError_t device_error_w4_bf16(unsigned* v, int clear);
 cudaError_t device_error_w4_fp32(unsigned* v, int clear);
+cudaError_t device_error_cross(unsigned* v, int clear);
 
 }  // namespace h3b

@@ -1,5 +1,6 @@
 // libh3b.so: the C ABI declared in include/h3b.h, argument validation and error state, the block streamer and the
 // wait self-test.  The kernels live in the k_*.cu translation units (launch.h lists what each exports).
+#include <cmath>
 #include <cstdio>
 #include <mutex>
 #include <string>
@@ -261,6 +262,106 @@ int h3b_attn_merge(float* acc, float* acc_lse, const void* o, int64_t o_head_str
   if (out && ldo < heads * head_dim) return fail(H3B_ERR_ARG, "attn_merge: output row stride below heads * head_dim");
   return attn_merge_launch(acc, acc_lse, o, o_head_stride, o_query_stride, lse, heads, queries, head_dim, first, out, ldo,
                            static_cast<cudaStream_t>(stream));
+}
+
+static int check_rope_operand(const h3b_rope_operand* o, const char* name) {
+  if (!o) return H3B_OK;
+  if (o->S < 0 || o->heads < 1) return fail(H3B_ERR_ARG, std::string("rope_axes: ") + name + " needs S >= 0 and heads >= 1");
+  if (o->S > 0 && (!o->x || !o->y || !o->pos)) return fail(H3B_ERR_ARG, std::string("rope_axes: ") + name + ": null tensor");
+  return H3B_OK;
+}
+
+int h3b_rope_axes(const h3b_rope_operand* q, const h3b_rope_operand* k, int x_dtype, int64_t B, int head_dim,
+                  const float* inv_freq, const int32_t* sections, int n_axes, int pos_dtype, int pairing, int inverse,
+                  void* stream) {
+  if (!q && !k) return fail(H3B_ERR_ARG, "rope_axes: q and k are both null");
+  if (!is_act(x_dtype)) return fail(H3B_ERR_ARG, "rope_axes: q/k dtype must be bf16, fp16 or fp32");
+  if (pos_dtype != H3B_FP32 && pos_dtype != H3B_INT32 && pos_dtype != H3B_INT64)
+    return fail(H3B_ERR_ARG, "rope_axes: positions must be fp32, int32 or int64");
+  if (pairing != H3B_PAIR_HALF && pairing != H3B_PAIR_ADJACENT) return fail(H3B_ERR_ARG, "rope_axes: pairing must be half or adjacent");
+  if (n_axes < 1 || n_axes > H3B_MAX_AXES || !sections) return fail(H3B_ERR_ARG, "rope_axes: 1 to " + std::to_string(H3B_MAX_AXES) + " axes");
+  int64_t pairs = 0;
+  for (int a = 0; a < n_axes; ++a) {
+    if (sections[a] < 0) return fail(H3B_ERR_ARG, "rope_axes: a section is negative");
+    pairs += sections[a];
+  }
+  if (B < 0 || head_dim < 1 || pairs < 1 || 2 * pairs > head_dim || head_dim > 1024)
+    return fail(H3B_ERR_ARG, "rope_axes: the sections must sum to 1 .. head_dim / 2 pairs, head_dim <= 1024");
+  int rc = check_rope_operand(q, "q");
+  if (!rc) rc = check_rope_operand(k, "k");
+  if (rc) return rc;
+  if (!inv_freq) return fail(H3B_ERR_ARG, "rope_axes: null inv_freq");
+  if (B == 0) return H3B_OK;
+  const h3b_rope_operand* qq = q && q->S > 0 ? q : nullptr;
+  const h3b_rope_operand* kk = k && k->S > 0 ? k : nullptr;
+  if (!qq && !kk) return H3B_OK;
+  return rope_axes_launch(qq, kk, x_dtype, B, head_dim, inv_freq, sections, n_axes, pos_dtype, pairing, inverse,
+                          static_cast<cudaStream_t>(stream));
+}
+
+static int check_cross(const h3b_attn_tensor* const* t, const bool* key_side, int n, int dtype, int64_t B, int64_t Sq,
+                       int64_t Sk, int Hq, int Hkv, int D, float scale, const void* mask, int mask_kind, int64_t ldm,
+                       const void* ws, size_t ws_bytes, bool backward) {
+  if (dtype != H3B_BF16 && dtype != H3B_FP16) return fail(H3B_ERR_ARG, "cross_attention: q, k and v must be bf16 or fp16");
+  if (B < 0 || Sq < 0 || Sk < 0 || Hq < 1 || Hkv < 1) return fail(H3B_ERR_ARG, "cross_attention: negative size or no heads");
+  if (Hq % Hkv || Hq / Hkv > 128) return fail(H3B_ERR_ARG, "cross_attention: query heads must be 1 to 128 times the key heads");
+  if (D < 8 || D > 128 || D % 8) return fail(H3B_ERR_ARG, "cross_attention: head_dim must be a multiple of 8, at most 128");
+  if (!(scale > 0.f) || !(scale < INFINITY)) return fail(H3B_ERR_ARG, "cross_attention: scale must be positive and finite");
+  if (Sq > 0x7FFFFF00 || Sk > 0x7FFFFF00 || B > 65535 || Hq > 65535)
+    return fail(H3B_ERR_UNSUPPORTED, "cross_attention: at most 2^31 rows, 65535 batch entries and heads");
+  if (mask_kind != H3B_MASK_NONE && mask_kind != H3B_MASK_BOOL && mask_kind != H3B_MASK_BIAS)
+    return fail(H3B_ERR_ARG, "cross_attention: unknown mask kind");
+  if (mask_kind != H3B_MASK_NONE && B > 0 && Sk > 0 && (!mask || ldm < 0)) return fail(H3B_ERR_ARG, "cross_attention: the mask is missing");
+  for (int i = 0; i < n; ++i) {
+    if (!t[i]) return fail(H3B_ERR_ARG, "cross_attention: a tensor is missing");
+    if (B == 0 || (key_side[i] ? Sk : Sq) == 0) continue;
+    if (!t[i]->ptr || !aligned(t[i]->ptr, 16) || t[i]->stride_b % 8 || t[i]->stride_s % 8 || t[i]->stride_h % 8 ||
+        t[i]->stride_b < 0 || t[i]->stride_s < 0 || t[i]->stride_h < 0)
+      return fail(H3B_ERR_ARG, "cross_attention: tensors must be 16-byte aligned with strides that are multiples of 8 elements");
+  }
+  const size_t need = cross_workspace(B, Sq, Sk, Hq, Hkv, D, mask_kind, backward);
+  if (need > 0 && (!ws || ws_bytes < need || !aligned(ws, 256)))
+    return fail(H3B_ERR_ARG, "cross_attention: workspace must be 256-byte aligned and hold " + std::to_string(need) + " bytes");
+  return H3B_OK;
+}
+
+size_t h3b_cross_attention_workspace_bytes(int64_t B, int64_t Sq, int64_t Sk, int Hq, int Hkv, int head_dim, int mask_kind,
+                                           int backward) {
+  if (B <= 0 || Sq < 0 || Sk < 0 || Hq < 1 || Hkv < 1 || head_dim < 1) return 0;
+  return cross_workspace(B, Sq, Sk, Hq, Hkv, head_dim, mask_kind, backward != 0);
+}
+
+int h3b_cross_attention(const h3b_attn_tensor* q, const h3b_attn_tensor* k, const h3b_attn_tensor* v,
+                        const h3b_attn_tensor* o, int dtype, int64_t B, int64_t Sq, int64_t Sk, int Hq, int Hkv,
+                        int head_dim, float scale, const int32_t* kv_lens, const void* mask, int mask_kind, int64_t ldm,
+                        float* lse, void* workspace, size_t ws_bytes, void* stream) {
+  const h3b_attn_tensor* t[4] = {q, k, v, o};
+  const bool key_side[4] = {false, true, true, false};
+  const int rc = check_cross(t, key_side, 4, dtype, B, Sq, Sk, Hq, Hkv, head_dim, scale, mask, mask_kind, ldm, workspace,
+                             ws_bytes, false);
+  if (rc) return rc;
+  if (B == 0 || Sq == 0) return H3B_OK;
+  const h3b_attn_tensor all[4] = {*q, *k, *v, *o};
+  return cross_launch(all, dtype, B, Sq, Sk, Hq, Hkv, head_dim, scale, kv_lens, mask, Sk > 0 ? mask_kind : H3B_MASK_NONE, ldm,
+                      lse, workspace, false, static_cast<cudaStream_t>(stream));
+}
+
+int h3b_cross_attention_backward(const h3b_attn_tensor* grad_o, const h3b_attn_tensor* q, const h3b_attn_tensor* k,
+                                 const h3b_attn_tensor* v, const h3b_attn_tensor* o, const float* lse,
+                                 const h3b_attn_tensor* dq, const h3b_attn_tensor* dk, const h3b_attn_tensor* dv, int dtype,
+                                 int64_t B, int64_t Sq, int64_t Sk, int Hq, int Hkv, int head_dim, float scale,
+                                 const int32_t* kv_lens, const void* mask, int mask_kind, int64_t ldm, void* workspace,
+                                 size_t ws_bytes, void* stream) {
+  const h3b_attn_tensor* t[8] = {q, k, v, o, grad_o, dq, dk, dv};
+  const bool key_side[8] = {false, true, true, false, false, false, true, true};
+  const int rc = check_cross(t, key_side, 8, dtype, B, Sq, Sk, Hq, Hkv, head_dim, scale, mask, mask_kind, ldm, workspace,
+                             ws_bytes, true);
+  if (rc) return rc;
+  if (B == 0 || (Sq == 0 && Sk == 0)) return H3B_OK;
+  if (Sq > 0 && !lse) return fail(H3B_ERR_ARG, "cross_attention_backward: lse is missing");
+  const h3b_attn_tensor all[8] = {*q, *k, *v, *o, *grad_o, *dq, *dk, *dv};
+  return cross_launch(all, dtype, B, Sq, Sk, Hq, Hkv, head_dim, scale, kv_lens, mask, Sk > 0 ? mask_kind : H3B_MASK_NONE, ldm,
+                      const_cast<float*>(lse), workspace, true, static_cast<cudaStream_t>(stream));
 }
 
 int h3b_decode_grid(const void* q4, int64_t N, int64_t K, int64_t ldq4, const void* s_rel, int s_dtype, int64_t lds,
@@ -568,7 +669,8 @@ int h3b_device_error(int clear) {
   if (e != cudaSuccess) return -static_cast<int>(cuda_fail(e, "cudaDeviceSynchronize"));
   cudaError_t (*const units[])(unsigned*, int) = {device_error_abi, device_error_act, device_error_decode,
                                                   device_error_gemm, device_error_w4, device_error_w4_fp8,
-                                                  device_error_w4_fp16, device_error_w4_bf16, device_error_w4_fp32};
+                                                  device_error_w4_fp16, device_error_w4_bf16, device_error_w4_fp32,
+                                                  device_error_cross};
   for (auto unit : units) {
     unsigned u = 0;
     e = unit(&u, clear);

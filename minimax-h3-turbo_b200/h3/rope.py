@@ -4,10 +4,14 @@
 reference's "torch" form of comfy_kitchen's fused op (rms_norm_fused_order, layout.py:309-326, then the fp32 rotation):
 impl "auto", "b200", "ck" and "torch" all mean that kernel.  ComfyUI's portable "eager" formula (other roundings) is not
 built, and neither is a CPU or fp32 path: such calls raise RuntimeError.
+
+`rope_axes` is the rotary embedding alone, from positions on several axes instead of cos/sin tables: out of place, for q
+and k of different lengths and head counts, bf16/fp16/fp32, in both directions (kernel `h3b_rope_axes`).
 """
 from __future__ import annotations
 
-from typing import Optional
+import ctypes
+from typing import Optional, Sequence, Tuple
 
 import torch
 
@@ -63,3 +67,102 @@ def norm_rope_(q: torch.Tensor, k: torch.Tensor, wq: torch.Tensor, wk: torch.Ten
         raise RuntimeError("the fused q/k norm+RoPE kernel needs bf16/fp16 CUDA tensors with head_dim 32/64/128/256 "
                            "(there is no CPU or fp32 path)")
     _fused(q, k, wq, wk, eps, cos, sin)
+
+
+# ------------------------------------------------------------------------------------------- rotary from positions
+_POS_CODES = {torch.float32: _lib.FP32, torch.int32: _lib.INT32, torch.int64: _lib.INT64}
+
+
+def _rope_operand(x: torch.Tensor, pos: torch.Tensor, axes: int, name: str):
+    """(struct, output, tensors to keep) of one side, x [B, S, heads, D] or [S, heads, D]."""
+    if x.dim() not in (3, 4):
+        raise ValueError(f"{name} must be [B, S, heads, D] or [S, heads, D], got {tuple(x.shape)}")
+    x4 = x if x.dim() == 4 else x.unsqueeze(0)
+    b, s, h, d = x4.shape
+    if pos is None or pos.device != x.device or pos.dtype not in _POS_CODES:
+        raise ValueError(f"{name}: positions must be fp32, int32 or int64 on {x.device}")
+    if pos.dim() == 2:
+        pos = pos.unsqueeze(0)
+    if pos.dim() != 3 or pos.shape[0] not in (1, b) or pos.shape[1] != s or pos.shape[2] != axes:
+        raise ValueError(f"{name}: positions must be [{s}, {axes}] or [{b}, {s}, {axes}], got {tuple(pos.shape)}")
+    if x4.stride(3) != 1 and d > 1:
+        x4 = x4.contiguous()
+    if pos.stride(2) != 1 and axes > 1:
+        pos = pos.contiguous()
+    y = torch.empty(b, s, h, d, dtype=x.dtype, device=x.device)
+    st = tuple(v if n > 1 else 0 for n, v in zip(x4.shape, x4.stride()))
+    op = _lib.RopeOperand(x4.data_ptr(), y.data_ptr(), pos.data_ptr(), s, st[0], st[1], st[2], s * h * d, h * d, d,
+                          pos.stride(0) if pos.shape[0] > 1 else 0, pos.stride(1), h)
+    return op, y.view(x.shape), (x4, pos)
+
+
+def _rope_axes(q, k, q_pos, k_pos, inv_freq, sections, pairing, inverse):
+    ref = q if q is not None else k
+    if not ref.is_cuda or (k is not None and not k.is_cuda):
+        raise RuntimeError("rope_axes: CUDA tensors only (there is no CPU path)")
+    code = _lib.act_code(ref.dtype)
+    if inv_freq.dim() != 1 or inv_freq.device != ref.device:
+        raise ValueError(f"rope_axes: inv_freq must be 1-D on {ref.device}")
+    n = inv_freq.shape[0]
+    axes = q_pos if q is not None else k_pos
+    axes = axes.shape[-1] if axes is not None and axes.dim() in (2, 3) else 0
+    if sections is None:  # every axis turns by all the frequencies, axis after axis
+        sections, inv_freq = (n,) * axes, inv_freq.repeat(axes)
+    if len(sections) != axes or sum(sections) != inv_freq.shape[0]:
+        raise ValueError(f"rope_axes: {axes} axes with {inv_freq.shape[0]} frequencies do not match sections {tuple(sections)}")
+    inv_freq = inv_freq.to(torch.float32).contiguous()
+    if q is not None and k is not None and (k.dtype != q.dtype or k.device != q.device or k.dim() != q.dim() or
+                                            k.shape[-1] != q.shape[-1] or (q.dim() == 4 and k.shape[0] != q.shape[0])):
+        raise ValueError(f"rope_axes: q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} do not match")
+    if q is not None and k is not None and k_pos is not None and k_pos.dtype != q_pos.dtype:
+        raise ValueError("rope_axes: positions of q and k must have one dtype")
+    oq = _rope_operand(q, q_pos, axes, "q") if q is not None else None
+    ok = _rope_operand(k, k_pos, axes, "k") if k is not None else None
+    pos = (oq or ok)[2][1]
+    b = ref.shape[0] if ref.dim() == 4 else 1
+    by = ctypes.byref
+    dev = ref.device
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().h3b_rope_axes(by(oq[0]) if oq else None, by(ok[0]) if ok else None, code, b, ref.shape[-1],
+                                            inv_freq.data_ptr(), (ctypes.c_int32 * max(1, axes))(*sections), axes,
+                                            _POS_CODES[pos.dtype], _lib.PAIRING[pairing], int(inverse),
+                                            _lib.stream_ptr(dev)), "rope_axes")
+    return (oq[1] if oq else None), (ok[1] if ok else None)
+
+
+class _RopeAxes(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_pos, k_pos, inv_freq, sections, pairing, inverse):
+        ctx.save_for_backward(q_pos, k_pos, inv_freq)
+        ctx.rest = (sections, pairing, inverse)
+        return _rope_axes(q, k, q_pos, k_pos, inv_freq, sections, pairing, inverse)
+
+    @staticmethod
+    def backward(ctx, gq, gk):
+        (q_pos, k_pos, inv_freq), (sections, pairing, inverse) = ctx.saved_tensors, ctx.rest
+        if gq is None and gk is None:
+            return (None,) * 8
+        dq, dk = _rope_axes(gq, gk, q_pos, k_pos, inv_freq, sections, pairing, not inverse)
+        return dq, dk, None, None, None, None, None, None
+
+
+def rope_axes(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions: Optional[torch.Tensor],
+              inv_freq: torch.Tensor, sections: Optional[Sequence[int]] = None, *,
+              k_positions: Optional[torch.Tensor] = None, pairing: str = "half", inverse: bool = False
+              ) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """Rotary embedding from positions on several axes (time, height, width), out of place -> (q', k').
+
+    q, k: [B, S, heads, D] or [S, heads, D], one of them may be None; lengths and head counts may differ.  positions:
+    [S, A] or [B, S, A] fp32, int32 or int64 for q (and for k, unless k_positions gives k's own).  Pair j of a head turns by
+    positions[axis(j)] * inv_freq[j]: sections (n_0, ..., n_{A-1}) deals the sum(sections) frequencies out to the axes in
+    order; None lets every axis turn by all of inv_freq, as rope_angles does.  pairing "half": channels (j, j + F), F the
+    number of pairs, as norm_rope_ rotates; "adjacent": (2j, 2j + 1).  Channels >= 2 F are copied.  inverse=True turns back:
+    the gradient's direction.  bf16, fp16 or fp32 (rounded once); differentiable in q and k."""
+    if q is None and k is None:
+        raise ValueError("rope_axes: q and k are both None")
+    if pairing not in _lib.PAIRING:
+        raise ValueError(f"pairing must be 'half' or 'adjacent', got {pairing!r}")
+    k_positions = positions if k_positions is None else k_positions
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k)):
+        return _RopeAxes.apply(q, k, positions, k_positions, inv_freq, sections, pairing, inverse)
+    return _rope_axes(q, k, positions, k_positions, inv_freq, sections, pairing, inverse)
