@@ -1,15 +1,6 @@
-// Cross attention: softmax attention of one stream's queries over another stream's keys and values, and its gradients.
-//
-//   s_ij = scale q_i . k_j + bias_j          bias_j: 0, the additive key bias (less its largest value), -inf if masked
-//   p_ij = exp(s_ij - lse_i),  lse_i = log sum_j exp(s_ij),  o_i = sum_j p_ij v_j;   no key left: o_i = 0, lse_i = -inf
-//   backward, with g = dL/do:  delta_i = g_i . o_i,  ds_ij = p_ij (g_i . v_j - delta_i)
-//     dv_j = sum_i p_ij g_i,  dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i
-//   Hq / Hkv query heads share a key head; their gradients add up in dk and dv.
-//
-// Simple kernels, everything in fp32: four lanes own a row (32 channels each), the other side's rows are staged in
-// shared memory 32 at a time, and every lane keeps its row's operands and sums in registers.
-#include "h3b_common.cuh"
-#include "launch.h"
+// Cross attention: the gradients, simple kernels in fp32 (four lanes own a row, 32 channels each; the other side's rows are
+// staged in shared memory 32 at a time), and the host side of both directions.
+#include "cross_fwd.cuh"
 
 namespace h3b {
 
@@ -17,19 +8,7 @@ constexpr int CA_ROWS = 32;      // rows a CTA owns
 constexpr int CA_TILE = 32;      // rows of the other side staged at a time
 constexpr int CA_LANES = 4;      // lanes per row
 constexpr int CA_CH = 32;        // channels per lane
-constexpr float CA_LOG2E = 1.4426950408889634f, CA_LN2 = 0.6931471805599453f;
 constexpr int CA_MAXD = CA_LANES * CA_CH;
-
-struct CrossParams {
-  h3b_attn_tensor q, k, v, o, go, dq, dk, dv;
-  float* lse;    // [B, Hq, Sq]
-  float* delta;  // [B, Hq, Sq]
-  const int32_t* kv_lens;  // [B] keys in use, or null: all
-  const float* bias2;      // [B, Skp] what is added to the scores, in units of log2; or null
-  int64_t Sq, Sk, Skp;
-  int B, Hq, Hkv, G, D;
-  float scale, scale2;  // scale2 = scale log2(e)
-};
 
 template <typename T>
 __device__ __forceinline__ float ca_f(T v) {
@@ -45,50 +24,6 @@ __device__ __forceinline__ T ca_t(float v) {
 template <typename T>
 __device__ __forceinline__ const T* ca_row(const h3b_attn_tensor& t, int b, int64_t s, int h) {
   return static_cast<const T*>(t.ptr) + b * t.stride_b + s * t.stride_s + h * t.stride_h;
-}
-
-__device__ __forceinline__ int64_t ca_len(const int32_t* lens, int b, int64_t Sk) {
-  if (!lens) return Sk;
-  const int64_t n = lens[b];
-  return n < 0 ? 0 : n > Sk ? Sk : n;
-}
-
-// One CTA per batch entry turns a key mask into what the kernels add to the scores: bias2[j] = log2(e) (bias_j - top),
-// top the largest bias in use (softmax does not change, and an entry whose keys all carry a large negative value keeps
-// its scores' digits and its log-sum-exp), -inf for keys that are out; and the number of keys up to the last one in use.
-constexpr int CA_PREP = 1024;
-__device__ __forceinline__ float ca_mask_value(const void* mask, int kind, int64_t i) {
-  return kind == H3B_MASK_BOOL ? (static_cast<const uint8_t*>(mask)[i] ? 0.f : -INFINITY) : static_cast<const float*>(mask)[i];
-}
-__global__ void __launch_bounds__(CA_PREP) cross_mask_kernel(const void* mask, int kind, int64_t ldm, const int32_t* kv_lens,
-                                                             int64_t Sk, int64_t Skp, float* bias2, int32_t* lens) {
-  __shared__ float top_s[CA_PREP / 32];
-  __shared__ int last_s[CA_PREP / 32];
-  const int b = blockIdx.x, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int64_t len = ca_len(kv_lens, b, Sk);
-  float top = -INFINITY;
-  int last = 0;
-  for (int64_t j = threadIdx.x; j < len; j += CA_PREP) {
-    const float v = ca_mask_value(mask, kind, b * ldm + j);
-    if (v != -INFINITY) last = static_cast<int>(j) + 1;
-    top = fmaxf(top, v);
-  }
-  for (int o = 16; o; o >>= 1) {
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
-  }
-  if (lane == 0) top_s[w] = top, last_s[w] = last;
-  __syncthreads();
-  top = top_s[lane], last = last_s[lane];
-  for (int o = 16; o; o >>= 1) {
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
-  }
-  if (threadIdx.x == 0) lens[b] = last;
-  for (int64_t j = threadIdx.x; j < Skp; j += CA_PREP) {
-    const float v = j < len ? ca_mask_value(mask, kind, b * ldm + j) : -INFINITY;
-    bias2[b * Skp + j] = v == -INFINITY ? v : (v - top) * CA_LOG2E;
-  }
 }
 
 // stage rows [s0, s0 + CA_TILE) of head h as fp32 [CA_TILE][CA_MAXD] (zero outside the tensor)
@@ -125,11 +60,11 @@ __device__ __forceinline__ float ca_dot(const float (&x)[CA_CH], const float* ro
   return s;
 }
 
-// MODE 0: forward.  MODE 1: dq and delta.  grid (row tiles of Sq, Hq, B)
+// dq and delta.  grid (row tiles of Sq, Hq, B)
 __device__ __forceinline__ float ca_bias(const CrossParams& P, int b, int64_t j, int64_t len) {
   return j >= len ? -INFINITY : P.bias2 ? P.bias2[b * P.Skp + j] : 0.f;
 }
-template <typename T, int MODE>
+template <typename T>
 __global__ void __launch_bounds__(CA_ROWS* CA_LANES) cross_rows_kernel(const CrossParams P) {
   __shared__ float ks[CA_TILE][CA_MAXD], vs[CA_TILE][CA_MAXD];
   __shared__ float bias[CA_TILE];
@@ -137,21 +72,18 @@ __global__ void __launch_bounds__(CA_ROWS* CA_LANES) cross_rows_kernel(const Cro
   const int64_t row = static_cast<int64_t>(blockIdx.x) * CA_ROWS + threadIdx.x / CA_LANES;
   const bool valid = row < P.Sq;
   const int64_t len = ca_len(P.kv_lens, b, P.Sk), stat = (static_cast<int64_t>(b) * P.Hq + h) * P.Sq + row;
-  float q[CA_CH], acc[CA_CH] = {}, g[CA_CH];
+  float q[CA_CH], acc[CA_CH] = {}, g[CA_CH], o[CA_CH];
   ca_own<T>(q, P.q, b, row, valid, h, P.D, sub);
-  float m = -INFINITY, l = 0.f, lse = INFINITY, delta = 0.f;
-  if constexpr (MODE == 1) {
-    float o[CA_CH];
-    ca_own<T>(g, P.go, b, row, valid, h, P.D, sub);
-    ca_own<T>(o, P.o, b, row, valid, h, P.D, sub);
+  float lse = INFINITY, delta = 0.f;
+  ca_own<T>(g, P.go, b, row, valid, h, P.D, sub);
+  ca_own<T>(o, P.o, b, row, valid, h, P.D, sub);
 #pragma unroll
-    for (int i = 0; i < CA_CH; ++i) delta = fmaf(g[i], o[i], delta);
-    delta += __shfl_xor_sync(0xffffffffu, delta, 1);
-    delta += __shfl_xor_sync(0xffffffffu, delta, 2);
-    if (valid) lse = P.lse[stat] * CA_LOG2E;
-    if (lse == -INFINITY) lse = INFINITY;  // a row without keys: every p is 0
-    if (valid && sub == 0) P.delta[stat] = delta;
-  }
+  for (int i = 0; i < CA_CH; ++i) delta = fmaf(g[i], o[i], delta);
+  delta += __shfl_xor_sync(0xffffffffu, delta, 1);
+  delta += __shfl_xor_sync(0xffffffffu, delta, 2);
+  if (valid) lse = P.lse[stat] * CA_LOG2E;
+  if (lse == -INFINITY) lse = INFINITY;  // a row without keys: every p is 0
+  if (valid && sub == 0) P.delta[stat] = delta;
   for (int64_t j0 = 0; j0 < len; j0 += CA_TILE) {
     __syncthreads();
     ca_stage<T>(ks, P.k, b, j0, len, hk, P.D);
@@ -162,26 +94,12 @@ __global__ void __launch_bounds__(CA_ROWS* CA_LANES) cross_rows_kernel(const Cro
       const float bj = bias[j];
       if (bj == -INFINITY) continue;  // what a masked key holds is never looked at
       const float s = fmaf(ca_dot(q, ks[j], sub), P.scale2, bj);
-      if constexpr (MODE == 0) {
-        const float mn = fmaxf(m, s), corr = exp2f(m - mn), p = exp2f(s - mn);
-        l = fmaf(l, corr, p);
-        m = mn;
+      const float ds = exp2f(s - lse) * (ca_dot(g, vs[j], sub) - delta);
 #pragma unroll
-        for (int i = 0; i < CA_CH; ++i) acc[i] = fmaf(acc[i], corr, p * vs[j][sub + CA_LANES * i]);
-      } else {
-        const float ds = exp2f(s - lse) * (ca_dot(g, vs[j], sub) - delta);
-#pragma unroll
-        for (int i = 0; i < CA_CH; ++i) acc[i] = fmaf(ds, ks[j][sub + CA_LANES * i], acc[i]);
-      }
+      for (int i = 0; i < CA_CH; ++i) acc[i] = fmaf(ds, ks[j][sub + CA_LANES * i], acc[i]);
     }
   }
-  if (!valid) return;
-  if constexpr (MODE == 0) {
-    ca_put<T>(P.o, b, row, h, P.D, sub, acc, l > 0.f ? 1.f / l : 0.f);
-    if (P.lse && sub == 0) P.lse[stat] = l > 0.f ? fmaf(m, CA_LN2, logf(l)) : -INFINITY;
-  } else {
-    ca_put<T>(P.dq, b, row, h, P.D, sub, acc, P.scale);
-  }
+  if (valid) ca_put<T>(P.dq, b, row, h, P.D, sub, acc, P.scale);
 }
 
 // dk and dv.  grid (row tiles of Sk, Hkv, B)
@@ -228,54 +146,70 @@ __global__ void __launch_bounds__(CA_ROWS* CA_LANES) cross_keys_kernel(const Cro
 
 template <typename T>
 static int cross_launch_t(const CrossParams& P, bool backward, cudaStream_t st) {
+  if (!backward) return fwd_launch<T>(P, st);
   const dim3 qgrid(static_cast<unsigned>((P.Sq + CA_ROWS - 1) / CA_ROWS), P.Hq, P.B);
   const dim3 kgrid(static_cast<unsigned>((P.Sk + CA_ROWS - 1) / CA_ROWS), P.Hkv, P.B);
   const int threads = CA_ROWS * CA_LANES;
-  if (!backward) {
-    cross_rows_kernel<T, 0><<<qgrid, threads, 0, st>>>(P);
-    return check_launch("cross_rows_kernel");
-  }
-  if (P.Sq > 0) cross_rows_kernel<T, 1><<<qgrid, threads, 0, st>>>(P);
+  if (P.Sq > 0) cross_rows_kernel<T><<<qgrid, threads, 0, st>>>(P);
   if (P.Sk > 0) cross_keys_kernel<T><<<kgrid, threads, 0, st>>>(P);
   return check_launch("cross_keys_kernel");
 }
 
-// Workspace: delta [B, Hq, Sq] (backward), the prepared mask [B, Skp] and its key counts [B]; parts 256-byte aligned.
+// Workspace, parts 256-byte aligned: the prepared mask [B, Skp] and its key counts [B]; delta [B, Hq, Sq] (backward);
+// partial outputs and log-sum-exps of the key splits (forward).
 struct CrossWs {
-  size_t delta, bias2, lens, total;
+  size_t bias2 = 0, lens = 0, delta = 0, part_o = 0, part_lse = 0, total = 0;
 };
-static CrossWs cross_ws(int64_t B, int64_t Sq, int64_t Sk, int Hq, int mask_kind, bool backward) {
-  auto up = [](size_t v) { return (v + 255) / 256 * 256; };
-  CrossWs w{};
-  size_t at = 0;
-  w.delta = at;
-  if (backward) at += up(static_cast<size_t>(B) * Hq * Sq * 4);
-  w.bias2 = at;
-  if (mask_kind != H3B_MASK_NONE) at += up(static_cast<size_t>(B) * ((Sk + 127) / 128 * 128) * 4);
-  w.lens = at;
-  if (mask_kind != H3B_MASK_NONE) at += up(static_cast<size_t>(B) * 4);
-  w.total = at;
+static CrossWs cross_plan(CrossParams& P, int mask_kind, bool backward) {
+  P.G = P.Hq / P.Hkv;
+  P.nq = CT / P.G;
+  P.Skp = (P.Sk + CT - 1) / CT * CT;
+  P.q_tiles = static_cast<int>((P.Sq + P.nq - 1) / P.nq);
+  P.units = (P.q_tiles + 1) / 2;
+  P.splits = backward ? 1 : fwd_splits(static_cast<int64_t>(P.units) * P.Hkv * P.B, P.Skp / CT);
+  CrossWs w;
+  auto take = [&](size_t bytes) {
+    const size_t at = w.total;
+    w.total += (bytes + 255) / 256 * 256;
+    return at;
+  };
+  const size_t rows = static_cast<size_t>(P.B) * P.Hq * P.Sq;
+  if (mask_kind != H3B_MASK_NONE) {
+    w.bias2 = take(static_cast<size_t>(P.B) * P.Skp * 4);
+    w.lens = take(static_cast<size_t>(P.B) * 4);
+  }
+  if (backward) w.delta = take(rows * 4);
+  if (P.splits > 1) {
+    w.part_o = take(rows * P.splits * P.D * 4);
+    w.part_lse = take(rows * P.splits * 4);
+  }
   return w;
+}
+static CrossParams cross_sizes(int64_t B, int64_t Sq, int64_t Sk, int Hq, int Hkv, int D) {
+  CrossParams P{};
+  P.B = static_cast<int>(B), P.Sq = Sq, P.Sk = Sk, P.Hq = Hq, P.Hkv = Hkv, P.D = D;
+  return P;
 }
 
 size_t cross_workspace(int64_t B, int64_t Sq, int64_t Sk, int Hq, int Hkv, int D, int mask_kind, bool backward) {
-  (void)Hkv, (void)D;
-  return cross_ws(B, Sq, Sk, Hq, mask_kind, backward).total;
+  CrossParams P = cross_sizes(B, Sq, Sk, Hq, Hkv, D);
+  return cross_plan(P, Sk > 0 ? mask_kind : H3B_MASK_NONE, backward).total;
 }
 
 int cross_launch(const h3b_attn_tensor* t, int dtype, int64_t B, int64_t Sq, int64_t Sk, int Hq, int Hkv, int D, float scale,
                  const int32_t* kv_lens, const void* mask, int mask_kind, int64_t ldm, float* lse, void* ws, bool backward,
                  cudaStream_t st) {
-  CrossParams P{};
+  CrossParams P = cross_sizes(B, Sq, Sk, Hq, Hkv, D);
+  const CrossWs w = cross_plan(P, mask_kind, backward);
   P.q = t[0], P.k = t[1], P.v = t[2], P.o = t[3];
   if (backward) P.go = t[4], P.dq = t[5], P.dk = t[6], P.dv = t[7];
   P.lse = lse;
-  const CrossWs w = cross_ws(B, Sq, Sk, Hq, mask_kind, backward);
   char* base = static_cast<char*>(ws);
   P.delta = reinterpret_cast<float*>(base + w.delta);
+  P.part_o = reinterpret_cast<float*>(base + w.part_o);
+  P.part_lse = reinterpret_cast<float*>(base + w.part_lse);
   P.kv_lens = kv_lens;
-  P.Sq = Sq, P.Sk = Sk, P.Skp = (Sk + 127) / 128 * 128;
-  P.B = static_cast<int>(B), P.Hq = Hq, P.Hkv = Hkv, P.G = Hq / Hkv, P.D = D, P.scale = scale, P.scale2 = scale * CA_LOG2E;
+  P.scale = scale, P.scale2 = scale * CA_LOG2E;
   if (mask_kind != H3B_MASK_NONE) {
     float* bias2 = reinterpret_cast<float*>(base + w.bias2);
     int32_t* lens = reinterpret_cast<int32_t*>(base + w.lens);

@@ -1,0 +1,262 @@
+// Shared parts of the cross-attention kernels (cross_fwd.cuh, cross_bwd.cuh): argument block, tensor maps, the bf16/fp16
+// tcgen05 wrappers, and the mask preparation.
+//
+//   s_ij = scale q_i . k_j + bias_j          bias_j: 0, the additive key bias (less its largest value), -inf if masked
+//   p_ij = exp(s_ij - lse_i),  lse_i = log sum_j exp(s_ij),  o_i = sum_j p_ij v_j;   no key left: o_i = 0, lse_i = -inf
+//   backward, with g = dL/do:  delta_i = g_i . o_i,  ds_ij = p_ij (g_i . v_j - delta_i)
+//     dv_j = sum_i p_ij g_i,  dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i
+//   Hq / Hkv query heads share a key head; their gradients add up in dk and dv.
+//
+// Query tiles: 128 rows are (128 / G) queries x the G = Hq / Hkv query heads of one key head, row = query * G + head, so
+// heads that share keys read them once; a 5-D tensor map (channel, head of the group, key head, query, batch) loads and
+// stores such a tile in one copy per 64 channels.  Channels are padded to 64 or 128 (DP) by the copy's zero fill.
+#pragma once
+
+#include <mutex>
+#include <type_traits>
+
+#include "h3b_common.cuh"
+#include "launch.h"
+
+namespace h3b {
+
+constexpr int CT = 128;  // rows of a query tile, keys of a key tile
+constexpr float CA_LOG2E = 1.4426950408889634f, CA_LN2 = 0.6931471805599453f;
+
+struct CrossParams {
+  h3b_attn_tensor q, k, v, o, go, dq, dk, dv;
+  float* lse;              // [B, Hq, Sq]
+  float* delta;            // [B, Hq, Sq]
+  const int32_t* kv_lens;  // [B] keys in use, or null: all
+  const float* bias2;      // [B, Skp] what is added to the scores, in units of log2; or null
+  float* part_o;           // [splits, B * Hq * Sq, D] partial outputs, each normalised by its own sum
+  float* part_lse;         // [splits, B * Hq * Sq] their log-sum-exps in units of log2
+  int64_t Sq, Sk, Skp;
+  int B, Hq, Hkv, G, D, nq;  // nq: queries of a tile
+  int q_tiles, units, splits;  // query tiles; work units (pairs of tiles) per key head; key splits of a unit
+  float scale, scale2;         // scale2 = scale log2(e)
+};
+
+__device__ __forceinline__ int64_t ca_len(const int32_t* lens, int b, int64_t Sk) {
+  if (!lens) return Sk;
+  const int64_t n = lens[b];
+  return n < 0 ? 0 : n > Sk ? Sk : n;
+}
+
+// ----------------------------------------------------------------------------------------------- PTX wrappers
+__device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2, int c3, int c4) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(
+          smem_u32(dst)),
+      "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(
+          smem_u32(dst)),
+      "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+__device__ __forceinline__ void tma_store_5d(const void* src, const CUtensorMap* map, int c0, int c1, int c2, int c3, int c4) {
+  asm volatile("cp.async.bulk.tensor.5d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5, %6}], [%1];" ::"l"(map),
+               "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
+               : "memory");
+}
+__device__ __forceinline__ void tma_store_4d(const void* src, const CUtensorMap* map, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(map),
+               "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void bulk_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+// D[tmem] (+)= A B, bf16/fp16 operands, fp32 accumulator; A from shared memory or from tensor memory
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// 32 lanes x 32 consecutive 32-bit columns: thread i of the warp writes its lane's 32 columns.
+__device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Instruction descriptor of tcgen05.mma kind::f16: A and B of one type, fp32 accumulator, M x N tile, A K-major,
+// B K-major or (b_mn) with its N index contiguous.
+template <typename T>
+__host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool b_mn) {
+  const uint32_t fmt = std::is_same_v<T, __nv_bfloat16> ? 1u : 0u;
+  return (1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(b_mn) << 16) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (static_cast<uint32_t>(m >> 4) << 24);
+}
+// A tile of shared memory: 128 rows, DP channels, in parts of 64 channels (128 rows x 128 bytes, 128-byte swizzle).
+constexpr uint32_t SUB_BYTES = CT * 128;
+// descriptor of 16 channels (step kk) of a tile whose rows are the operand's M or N index (K-major)
+__device__ __forceinline__ uint64_t desc_rows(uint32_t tile, int kk) {
+  return smem_desc_sw128(tile + (kk >> 2) * SUB_BYTES + (kk & 3) * 32);
+}
+// descriptor of 16 rows (step kk) of a tile whose channels are the operand's N index and whose rows are K (MN-major):
+// 64-channel parts SUB_BYTES apart (leading offset), groups of 8 rows 1024 bytes apart (stride offset)
+__device__ __forceinline__ uint64_t desc_chan(uint32_t tile, int kk) {
+  uint64_t d = smem_desc_sw128(tile + kk * 2048);
+  d &= ~(uint64_t(0x3FFF) << 16);
+  d |= static_cast<uint64_t>(SUB_BYTES >> 4) << 16;
+  return d;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (std::is_same_v<T, __half>) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <int R>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R));
+}
+template <int R>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R));
+}
+__device__ __forceinline__ void group_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+// every lane of the warp waits; one outcome for all (what follows are whole-warp instructions)
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort));
+}
+// write 8 packed values (16 bytes, chunk c of 8) of row r into a 64-channel part with the 128-byte swizzle
+__device__ __forceinline__ void put_swizzled(unsigned char* part, int r, int c, uint4 v) {
+  *reinterpret_cast<uint4*>(part + r * 128 + ((c ^ (r & 7)) << 4)) = v;
+}
+
+// ----------------------------------------------------------------------------------------------- mask preparation
+// One CTA per batch entry turns a key mask into what the kernels add to the scores: bias2[j] = log2(e) (bias_j - top),
+// top the largest bias in use (softmax does not change, and an entry whose keys all carry a large negative value keeps
+// its scores' digits and its log-sum-exp), -inf for keys that are out; and the number of keys up to the last one in use.
+constexpr int CA_PREP = 1024;
+__device__ __forceinline__ float ca_mask_value(const void* mask, int kind, int64_t i) {
+  return kind == H3B_MASK_BOOL ? (static_cast<const uint8_t*>(mask)[i] ? 0.f : -INFINITY) : static_cast<const float*>(mask)[i];
+}
+__global__ void __launch_bounds__(CA_PREP) cross_mask_kernel(const void* mask, int kind, int64_t ldm, const int32_t* kv_lens,
+                                                             int64_t Sk, int64_t Skp, float* bias2, int32_t* lens) {
+  __shared__ float top_s[CA_PREP / 32];
+  __shared__ int last_s[CA_PREP / 32];
+  const int b = blockIdx.x, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t len = ca_len(kv_lens, b, Sk);
+  float top = -INFINITY;
+  int last = 0;
+  for (int64_t j = threadIdx.x; j < len; j += CA_PREP) {
+    const float v = ca_mask_value(mask, kind, b * ldm + j);
+    if (v != -INFINITY) last = static_cast<int>(j) + 1;
+    top = fmaxf(top, v);
+  }
+  for (int o = 16; o; o >>= 1) {
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
+  }
+  if (lane == 0) top_s[w] = top, last_s[w] = last;
+  __syncthreads();
+  top = top_s[lane], last = last_s[lane];
+  for (int o = 16; o; o >>= 1) {
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
+  }
+  if (threadIdx.x == 0) lens[b] = last;
+  for (int64_t j = threadIdx.x; j < Skp; j += CA_PREP) {
+    const float v = j < len ? ca_mask_value(mask, kind, b * ldm + j) : -INFINITY;
+    bias2[b * Skp + j] = v == -INFINITY ? v : (v - top) * CA_LOG2E;
+  }
+}
+
+// ----------------------------------------------------------------------------------------------- tensor maps
+typedef CUresult (*CrossEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static CrossEncodeFn cross_encode_fn() {
+  static CrossEncodeFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<CrossEncodeFn>(p);
+  });
+  return fn;
+}
+// dims / strides (elements; strides of dims 1..) of a 2-byte tensor; box: 64 channels x the given extents
+static int cross_map(CUtensorMap* map, const void* base, bool half, int rank, const int64_t* ext, const int64_t* str,
+                     const int* box_ext) {
+  CrossEncodeFn fn = cross_encode_fn();
+  if (!fn) return fail(H3B_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable (driver too old?)");
+  cuuint64_t dims[5], strides[4];
+  cuuint32_t box[5], one[5];
+  for (int i = 0; i < rank; ++i) {
+    dims[i] = static_cast<cuuint64_t>(ext[i] > 0 ? ext[i] : 1);  // an empty side is never loaded
+    box[i] = static_cast<cuuint32_t>(box_ext[i]);
+    one[i] = 1;
+    // the stride of an extent of one is never used; any valid value will do
+    if (i) strides[i - 1] = ext[i] > 1 && str[i] > 0 ? static_cast<cuuint64_t>(str[i]) * 2 : 16;
+  }
+  const CUresult r = fn(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank,
+                        const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(H3B_ERR_CUDA, "cuTensorMapEncodeTiled failed (code " + std::to_string(int(r)) + ")");
+  return H3B_OK;
+}
+// (channel, head of the group, key head, query, batch), a box of 64 channels x G heads x nq queries
+static int cross_map_q(CUtensorMap* map, const CrossParams& P, const h3b_attn_tensor& t, bool half) {
+  const int64_t ext[5] = {P.D, P.G, P.Hkv, P.Sq, P.B};
+  const int64_t str[5] = {1, t.stride_h, t.stride_h * P.G, t.stride_s, t.stride_b};
+  const int box[5] = {64, P.G, 1, P.nq, 1};
+  return cross_map(map, t.ptr, half, 5, ext, str, box);
+}
+// (channel, key head, key, batch), a box of 64 channels x 128 keys
+static int cross_map_k(CUtensorMap* map, const CrossParams& P, const h3b_attn_tensor& t, bool half) {
+  const int64_t ext[4] = {P.D, P.Hkv, P.Sk, P.B};
+  const int64_t str[4] = {1, t.stride_h, t.stride_s, t.stride_b};
+  const int box[4] = {64, 1, CT, 1};
+  return cross_map(map, t.ptr, half, 4, ext, str, box);
+}
+
+static int cross_sms() {
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms;
+}
+
+}  // namespace h3b

@@ -1,0 +1,555 @@
+// Cross attention forward on the tcgen05 tensor cores.
+//
+// A work unit is a pair of query tiles (slots 0 and 1, 128 rows each) of one key head, over a range of key tiles.  One
+// persistent CTA per SM walks the units; its warps:
+//   0-3, 4-7   softmax of slot 0 and 1: one thread per row.  S (128 fp32 columns of tensor memory) -> registers, running
+//              maximum and sum in fp32, P = exp2(S scale2 - m) rounded to the operand type, back to tensor memory (over S).
+//              m only moves when a tile's maximum exceeds it by 8 (a factor 2^8: far from overflow in fp32 sums and fp16 P);
+//              then the same threads rescale O in tensor memory.  P rounded to 8 (bf16) or 11 (fp16) bits, relative to
+//              each probability: the product's operand type; the sum uses the unrounded values.
+//   8-11       epilogue: O / l to the operand type, through swizzled staging and a bulk tensor store; log-sum-exp
+//   12         MMA issue: S = Q K^T (both from shared memory), O += P V (P from tensor memory, V channel-major)
+//   13         copies: Q tiles, and a ring of K and V tiles, in the order of use
+//   14         zeroes the rows of V tiles whose keys are left out, before their product (0 x NaN would reach the sums)
+// Tensor memory: S0 S1 O0 O1, 128 columns each.  While one slot's softmax runs, the tensor cores work for the other.
+// Units with few query tiles split the keys over CTAs; cross_combine_kernel joins the partial results by their
+// log-sum-exps in a fixed order.
+#include "cross_common.cuh"
+
+namespace h3b {
+
+template <int DP>
+struct FwdCfg {
+  static constexpr int NSUB = DP / 64;
+  static constexpr int TILE = NSUB * static_cast<int>(SUB_BYTES);  // bytes of a 128-row tile
+  static constexpr int STAGES = DP == 128 ? 4 : 8;                 // ring of K and V tiles
+  static constexpr int STAGE_PARTS = 2;                            // staging buffers of 64 channels for the output
+  static constexpr int SMEM = 2 * TILE + STAGES * TILE + STAGE_PARTS * static_cast<int>(SUB_BYTES) + 2 * 2 * CT * 4 + 512;
+  static constexpr uint32_t TMEM_COLS = 512;
+};
+
+struct FwdUnit {
+  int b, hk, split, tile0, t0, t1;  // batch, key head, key split, first query tile, key tiles [t0, t1)
+  bool two;                         // the second query tile exists
+};
+
+__device__ __forceinline__ FwdUnit fwd_unit(const CrossParams& P, int64_t it) {
+  FwdUnit u;
+  const int pair = static_cast<int>(it % P.units);
+  int64_t r = it / P.units;
+  u.split = static_cast<int>(r % P.splits);
+  r /= P.splits;
+  u.hk = static_cast<int>(r % P.Hkv);
+  u.b = static_cast<int>(r / P.Hkv);
+  u.tile0 = pair * 2;
+  u.two = u.tile0 + 1 < P.q_tiles;
+  const int nt = static_cast<int>((ca_len(P.kv_lens, u.b, P.Sk) + CT - 1) / CT);
+  const int per = (nt + P.splits - 1) / P.splits;
+  u.t0 = min(u.split * per, nt);
+  u.t1 = min(u.t0 + per, nt);
+  return u;
+}
+// the next unit with key tiles
+__device__ __forceinline__ bool fwd_next(const CrossParams& P, int64_t& it, int64_t n, FwdUnit& u) {
+  for (; it < n; it += gridDim.x) {
+    u = fwd_unit(P, it);
+    if (u.t1 > u.t0) {
+      it += gridDim.x;
+      return true;
+    }
+  }
+  return false;
+}
+// V rows of tile t must be zeroed before use: a mask, or a length that ends inside the tile and before the tensor's end
+__device__ __forceinline__ bool needs_zeroing(const CrossParams& P, int64_t len, int t) {
+  return P.bias2 != nullptr || (len < P.Sk && static_cast<int64_t>(t + 1) * CT > len);
+}
+
+template <typename T, int DP, bool BIAS>
+__global__ void __launch_bounds__(512, 1)
+    cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, const CrossParams P) {
+  using C = FwdCfg<DP>;
+  extern __shared__ __align__(1024) unsigned char ca_smem[];
+  unsigned char* sQ = ca_smem;
+  unsigned char* sKV = sQ + 2 * C::TILE;
+  unsigned char* sO = sKV + C::STAGES * C::TILE;
+  float* stat = reinterpret_cast<float*>(sO + C::STAGE_PARTS * SUB_BYTES);  // [slot][l, m][row]
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(stat + 4 * CT);
+  uint64_t* q_empty = q_full + 2;
+  uint64_t* kv_full = q_empty + 2;
+  uint64_t* kv_empty = kv_full + C::STAGES;
+  uint64_t* v_clean = kv_empty + C::STAGES;
+  uint64_t* s_full = v_clean + C::STAGES;
+  uint64_t* p_full = s_full + 2;
+  uint64_t* o_full = p_full + 2;
+  uint64_t* o_empty = o_full + 2;
+  uint64_t* l_full = o_empty + 2;
+  uint64_t* done = l_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t n_items = static_cast<int64_t>(P.units) * P.splits * P.Hkv * P.B;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&q_full[s], 1);
+      mbar_init(&q_empty[s], 1);
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_full[s], 4);
+      mbar_init(&o_full[s], 1);
+      mbar_init(&o_empty[s], 4);
+      mbar_init(&l_full[s], 4);
+    }
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&kv_full[s], 1);
+      mbar_init(&kv_empty[s], 1);
+      mbar_init(&v_clean[s], 1);
+    }
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+    tma_prefetch_desc(&tmO);
+  }
+  if (warp == 12) {
+    tmem_alloc(tmem_slot, C::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp < 8) {
+    // ------------------------------------------------------------------------------------------ softmax
+    regs_inc<176>();
+    const int slot = warp >> 2, row = threadIdx.x & (CT - 1);
+    const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // lane offset (32 per warp) in bits 16..
+    const uint32_t tS = tmem + slot * CT + lanes, tO = tmem + 2 * CT + slot * CT + lanes;
+    uint32_t sph = 0, oph = 1;
+    FwdUnit u;
+    bool ok = true;
+    for (int64_t it = blockIdx.x; ok && fwd_next(P, it, n_items, u);) {
+      if (slot == 1 && !u.two) continue;
+      const int64_t len = ca_len(P.kv_lens, u.b, P.Sk);
+      const float* bias = BIAS ? P.bias2 + u.b * P.Skp : nullptr;
+      float m = -INFINITY, l = 0.f;
+      for (int t = u.t0; t < u.t1; ++t) {
+        if (!(ok = warp_wait(&s_full[slot], sph, abort_flag))) break;
+        sph ^= 1;
+        tc_fence_after();
+        uint32_t r[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(tS + 32 * c, r[c]);
+        tmem_ld_wait();
+        float mt[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if constexpr (BIAS) {
+          const float4* b4 = reinterpret_cast<const float4*>(bias + static_cast<int64_t>(t) * CT);
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float4 bb = __ldg(b4 + 8 * c + i);
+              const float bv[4] = {bb.x, bb.y, bb.z, bb.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {  // a masked key's score is replaced, whatever it was
+                const float x = fmaf(__uint_as_float(r[c][4 * i + e]), P.scale2, bv[e]);
+                r[c][4 * i + e] = __float_as_uint(bv[e] == -INFINITY ? -INFINITY : x);
+              }
+            }
+        } else {
+          const int64_t lim = len - static_cast<int64_t>(t) * CT;
+          if (lim < CT) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (32 * c + i >= lim) r[c][i] = 0xFF800000u;  // -inf
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) mt[c] = fmaxf(mt[c], __uint_as_float(r[c][i]));
+        float top = fmaxf(fmaxf(mt[0], mt[1]), fmaxf(mt[2], mt[3]));
+        if constexpr (!BIAS) top *= P.scale2;
+        if (t == u.t0) {
+          m = top;
+        } else if (__any_sync(0xffffffffu, top > m + 8.f)) {
+          // the product of the tile before is complete: its commit came before that of these scores
+          const float mn = fmaxf(m, top), f = mn == -INFINITY ? 1.f : ex2(m - mn);
+          m = mn;
+          l *= f;
+#pragma unroll 1
+          for (int c = 0; c < DP / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld_32x32b_x32(tO + 32 * c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_st_32x32b_x32(tO + 32 * c, o);
+          }
+        }
+        const float mm = m == -INFINITY ? 0.f : m;  // no key so far: every probability is exp2(-inf) = 0
+        float ls[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float x = __uint_as_float(r[c][i]);
+            const float p = ex2(BIAS ? x - mm : fmaf(x, P.scale2, -mm));
+            ls[i & 3] += p;
+            r[c][i] = __float_as_uint(p);
+          }
+        }
+        l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const int k = 64 * c + 2 * i;
+            pk[i] = pack2<T>(__uint_as_float(r[k >> 5][k & 31]), __uint_as_float(r[k >> 5][(k & 31) + 1]));
+          }
+          tmem_st_32x32b_x32(tS + 32 * c, pk);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[slot]);
+      }
+      if (!ok || !(ok = warp_wait(&o_empty[slot], oph, abort_flag))) break;
+      oph ^= 1;
+      stat[(slot * 2 + 0) * CT + row] = l;
+      stat[(slot * 2 + 1) * CT + row] = m;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&l_full[slot]);
+    }
+  } else if (warp < 12) {
+    // ------------------------------------------------------------------------------------------ epilogue
+    regs_dec<96>();
+    const int row = threadIdx.x & (CT - 1), qr = row / P.G, hg = row - qr * P.G;
+    const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
+    uint32_t ph[2] = {0, 0};
+    bool dead = false;
+    for (int64_t it = blockIdx.x; it < n_items; it += gridDim.x) {
+      const FwdUnit u = fwd_unit(P, it);
+      for (int slot = 0; slot < (u.two ? 2 : 1); ++slot) {
+        const int64_t s0 = static_cast<int64_t>(u.tile0 + slot) * P.nq, s = s0 + qr;
+        const bool valid = qr < P.nq && s < P.Sq, any = u.t1 > u.t0;
+        float l = 0.f, m = -INFINITY;
+        if (any) {
+          if (!warp_wait(&l_full[slot], ph[slot], abort_flag)) dead = true;
+          if (!warp_wait(&o_full[slot], ph[slot], abort_flag)) dead = true;
+          ph[slot] ^= 1;
+          l = stat[(slot * 2 + 0) * CT + row];
+          m = stat[(slot * 2 + 1) * CT + row];
+          tc_fence_after();
+        }
+        const bool none = l == 0.f;
+        const float inv = none ? 0.f : 1.f / l;
+        const uint32_t tO = tmem + 2 * CT + slot * CT + lanes;
+        const int64_t rid = (static_cast<int64_t>(u.b) * P.Hq + u.hk * P.G + hg) * P.Sq + s;
+        const float lse2 = none ? -INFINITY : m + log2f(l);
+        if (P.splits > 1) {
+          if (valid) P.part_lse[static_cast<int64_t>(u.split) * P.B * P.Hq * P.Sq + rid] = lse2;
+          float* dst = P.part_o + (static_cast<int64_t>(u.split) * P.B * P.Hq * P.Sq + rid) * P.D;
+          if (any) {
+#pragma unroll 1
+            for (int c = 0; c < DP / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld_32x32b_x32(tO + 32 * c, o);
+              tmem_ld_wait();
+              if (valid && !dead) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                  if (32 * c + 4 * i < P.D)
+                    *reinterpret_cast<float4*>(dst + 32 * c + 4 * i) =
+                        make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv,
+                                    __uint_as_float(o[4 * i + 2]) * inv, __uint_as_float(o[4 * i + 3]) * inv);
+              }
+            }
+          }
+        } else {
+          if (P.lse && valid) P.lse[rid] = lse2 * CA_LN2;
+#pragma unroll 1
+          for (int part = 0; part < C::NSUB; ++part) {
+            unsigned char* buf = sO + part * SUB_BYTES;
+            if (warp == 8 && lane == 0) bulk_wait_read<C::NSUB - 1>();  // this part's store before has left the buffer
+            group_sync(1, 128);
+#pragma unroll 1
+            for (int c = 0; c < 2; ++c) {
+              uint32_t o[32];
+              if (any) {
+                tmem_ld_32x32b_x32(tO + 64 * part + 32 * c, o);
+                tmem_ld_wait();
+              }
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                uint4 v;
+                uint32_t* vv = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  vv[e] = none ? 0u
+                               : pack2<T>(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
+                put_swizzled(buf, row, 4 * c + i, v);
+              }
+            }
+            fence_proxy_async_smem();
+            group_sync(1, 128);
+            if (warp == 8 && lane == 0 && !dead) {
+              tma_store_5d(buf, &tmO, 64 * part, 0, u.hk, static_cast<int>(s0), u.b);
+              bulk_commit();
+            }
+          }
+        }
+        if (any) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&o_empty[slot]);
+        }
+      }
+    }
+    if (warp == 8 && lane == 0) bulk_wait_all();
+  } else {
+    regs_dec<64>();
+    if (warp == 12) {
+      if (lane == 0) {
+        // -------------------------------------------------------------------------------------- MMA issue
+        constexpr uint32_t idQK = idesc_f16<T>(CT, CT, false), idPV = idesc_f16<T>(CT, DP, true);
+        const uint32_t aQ = smem_u32(sQ), aKV = smem_u32(sKV);
+        int st = 0;
+        uint32_t kph = 0, qph[2] = {0, 0}, pph[2] = {0, 0}, oph[2] = {1, 1}, cph = 0;  // cph: a phase bit per stage
+        auto step = [&] {
+          if (++st == C::STAGES) st = 0, kph ^= 1;
+        };
+        auto qk = [&](int slot, int kst) {
+          for (int kk = 0; kk < DP / 16; ++kk)
+            mma_f16_ss(tmem + slot * CT, desc_rows(aQ + slot * C::TILE, kk), desc_rows(aKV + kst * C::TILE, kk), idQK, kk > 0);
+          mma_commit(&s_full[slot]);
+        };
+        FwdUnit cur, nxt;
+        int64_t it = blockIdx.x;
+        bool have = fwd_next(P, it, n_items, cur), ok = true;
+        if (have) {
+          ok = mbar_wait(&kv_full[st], kph, abort_flag);
+          for (int s = 0; ok && s < (cur.two ? 2 : 1); ++s) {
+            ok = mbar_wait(&q_full[s], qph[s], abort_flag);
+            qph[s] ^= 1;
+            if (!ok) break;
+            tc_fence_after();
+            qk(s, st);
+            if (cur.t1 - cur.t0 == 1) mma_commit(&q_empty[s]);
+          }
+          mma_commit(&kv_empty[st]);
+          step();
+        }
+        while (have && ok) {
+          bool more = false;
+          const int64_t len = ca_len(P.kv_lens, cur.b, P.Sk);
+          for (int t = cur.t0; ok && t < cur.t1; ++t) {
+            const bool last = t == cur.t1 - 1;
+            if (last) more = fwd_next(P, it, n_items, nxt);
+            const int vst = st;
+            if (!(ok = mbar_wait(&kv_full[vst], kph, abort_flag))) break;
+            if (needs_zeroing(P, len, t)) {
+              if (!(ok = mbar_wait(&v_clean[vst], (cph >> vst) & 1, abort_flag))) break;
+              cph ^= 1u << vst;
+            }
+            step();
+            const bool then_qk = !last || more;
+            const int kst = st;
+            const uint32_t kparity = kph;
+            if (then_qk) step();
+            for (int s = 0; ok && s < 2; ++s) {
+              if (s == 0 || cur.two) {
+                if (!(ok = mbar_wait(&p_full[s], pph[s], abort_flag))) break;
+                pph[s] ^= 1;
+                if (t == cur.t0) {
+                  if (!(ok = mbar_wait(&o_empty[s], oph[s], abort_flag))) break;
+                  oph[s] ^= 1;
+                }
+                tc_fence_after();
+                for (int kk = 0; kk < CT / 16; ++kk)
+                  mma_f16_ts(tmem + 2 * CT + s * CT, tmem + s * CT + kk * 8, desc_chan(aKV + vst * C::TILE, kk), idPV,
+                             t > cur.t0 || kk > 0);
+                if (last) mma_commit(&o_full[s]);
+              }
+              if (then_qk && (s == 0 || (last ? nxt.two : cur.two))) {
+                if (!(ok = mbar_wait(&kv_full[kst], kparity, abort_flag))) break;
+                if (last) {
+                  if (!(ok = mbar_wait(&q_full[s], qph[s], abort_flag))) break;
+                  qph[s] ^= 1;
+                }
+                tc_fence_after();
+                qk(s, kst);
+                if (last ? nxt.t1 - nxt.t0 == 1 : t + 2 == cur.t1) mma_commit(&q_empty[s]);
+              }
+            }
+            if (!ok) break;
+            mma_commit(&kv_empty[vst]);
+            if (then_qk) mma_commit(&kv_empty[kst]);
+          }
+          cur = nxt;
+          have = more;
+        }
+      }
+      __syncwarp();
+    } else if (warp == 13) {
+      if (lane == 0) {
+        // -------------------------------------------------------------------------------------- copies
+        int st = 0, fills = 0, qfills[2] = {0, 0};
+        uint32_t kph = 1, qph[2] = {1, 1};
+        FwdUnit u;
+        bool ok = true;
+        const uint32_t q_bytes = static_cast<uint32_t>(C::NSUB * 128 * P.G * P.nq);
+        auto load = [&](const CUtensorMap* map, int t) {
+          if (!(ok = mbar_wait(&kv_empty[st], kph, abort_flag))) return;
+          mbar_arrive_expect_tx(&kv_full[st], C::TILE);
+          for (int p = 0; p < C::NSUB; ++p)
+            tma_load_4d(sKV + st * C::TILE + p * SUB_BYTES, map, &kv_full[st], 64 * p, u.hk, t * CT, u.b);
+          ++fills;
+          if (++st == C::STAGES) st = 0, kph ^= 1;
+        };
+        for (int64_t it = blockIdx.x; ok && fwd_next(P, it, n_items, u);) {
+          for (int s = 0; ok && s < (u.two ? 2 : 1); ++s) {
+            if (!(ok = mbar_wait(&q_empty[s], qph[s], abort_flag))) break;
+            qph[s] ^= 1;
+            mbar_arrive_expect_tx(&q_full[s], q_bytes);
+            for (int p = 0; p < C::NSUB; ++p)
+              tma_load_5d(sQ + s * C::TILE + p * SUB_BYTES, &tmQ, &q_full[s], 64 * p, 0, u.hk, (u.tile0 + s) * P.nq, u.b);
+            ++qfills[s];
+          }
+          for (int t = u.t0; ok && t < u.t1; ++t) {
+            load(&tmK, t);
+            if (ok) load(&tmV, t);
+          }
+        }
+        // copies in flight land in this CTA's shared memory: wait for the last ones before it goes away
+        for (int j = fills > C::STAGES ? fills - C::STAGES : 0; j < fills; ++j)
+          if (!mbar_wait_drain(&kv_full[j % C::STAGES], static_cast<uint32_t>((j / C::STAGES) & 1))) break;
+        for (int s = 0; s < 2; ++s)
+          if (qfills[s]) mbar_wait_drain(&q_full[s], static_cast<uint32_t>((qfills[s] - 1) & 1));
+      }
+      __syncwarp();
+    } else if (warp == 14) {
+      // ---------------------------------------------------------------------------------------- rows of masked keys
+      int st = 0;
+      uint32_t kph = 0;
+      FwdUnit u;
+      bool ok = true;
+      for (int64_t it = blockIdx.x; ok && fwd_next(P, it, n_items, u);) {
+        const int64_t len = ca_len(P.kv_lens, u.b, P.Sk);
+        for (int t = u.t0; ok && t < u.t1; ++t) {
+          if (++st == C::STAGES) st = 0, kph ^= 1;  // the K tile
+          if (needs_zeroing(P, len, t)) {
+            if (!(ok = warp_wait(&kv_full[st], kph, abort_flag))) break;
+            for (int j = lane; j < CT; j += 32) {
+              const int64_t key = static_cast<int64_t>(t) * CT + j;
+              if (key >= len || (BIAS && P.bias2[u.b * P.Skp + key] == -INFINITY))
+                for (int p = 0; p < C::NSUB; ++p)
+                  for (int c = 0; c < 8; ++c)
+                    *reinterpret_cast<uint4*>(sKV + st * C::TILE + p * SUB_BYTES + j * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&v_clean[st]);
+          }
+          if (++st == C::STAGES) st = 0, kph ^= 1;
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    if (lane == 0) {  // every product issued (after a wait that gave up some may still run) and its arrivals are over
+      mma_commit(done);
+      mbar_wait_drain(done, 0);
+    }
+    __syncwarp();
+    tmem_dealloc(tmem, C::TMEM_COLS);
+  }
+}
+
+// Joins the key splits of every row: weights exp2(lse_s - lse), in the order of the splits.  One warp per row.
+template <typename T>
+__global__ void __launch_bounds__(256) cross_combine_kernel(const CrossParams P) {
+  const int64_t rows = static_cast<int64_t>(P.B) * P.Hq * P.Sq;
+  const int lane = threadIdx.x & 31;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  float top = -INFINITY;
+  for (int s = lane; s < P.splits; s += 32) top = fmaxf(top, P.part_lse[s * rows + row]);
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float base = top == -INFINITY ? 0.f : top;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+  for (int s = 0; s < P.splits; ++s) {
+    const float e = P.part_lse[s * rows + row];
+    if (e == -INFINITY) continue;  // a split without keys wrote nothing else
+    const float w = ex2(e - base);
+    sum += w;
+    if (4 * lane < P.D) {
+      const float4 o = *reinterpret_cast<const float4*>(P.part_o + (s * rows + row) * P.D + 4 * lane);
+      acc.x = fmaf(w, o.x, acc.x), acc.y = fmaf(w, o.y, acc.y), acc.z = fmaf(w, o.z, acc.z), acc.w = fmaf(w, o.w, acc.w);
+    }
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int64_t s = row % P.Sq, bh = row / P.Sq, h = bh % P.Hq, b = bh / P.Hq;
+  if (4 * lane < P.D) {
+    uint2 v = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+    *reinterpret_cast<uint2*>(static_cast<T*>(P.o.ptr) + b * P.o.stride_b + s * P.o.stride_s + h * P.o.stride_h + 4 * lane) = v;
+  }
+  if (P.lse && lane == 0) P.lse[row] = sum == 0.f ? -INFINITY : (base + log2f(sum)) * CA_LN2;
+}
+
+// Key splits of the forward: enough that every SM has work, at the least time of the busiest SM, counted in key tiles
+// (a unit costs about two tiles to fill and drain, splitting at all about three for the second kernel).
+static int fwd_splits(int64_t units, int64_t key_tiles) {
+  const int sms = cross_sms();
+  if (units >= sms || key_tiles <= 1) return 1;
+  int best = 1;
+  int64_t best_cost = key_tiles + 2;
+  for (int s = 2; s <= 64 && s <= key_tiles; ++s) {
+    const int64_t waves = (units * s + sms - 1) / sms, cost = waves * ((key_tiles + s - 1) / s + 2) + 3;
+    if (cost < best_cost) best = s, best_cost = cost;
+  }
+  return best;
+}
+
+template <typename T, int DP, bool BIAS>
+static int fwd_launch_cfg(const CrossParams& P, cudaStream_t st) {
+  using C = FwdCfg<DP>;
+  CUtensorMap q, k, v, o;
+  const bool half = std::is_same_v<T, __half>;
+  int rc = cross_map_q(&q, P, P.q, half);
+  if (!rc) rc = cross_map_k(&k, P, P.Sk > 0 ? P.k : P.q, half);
+  if (!rc) rc = cross_map_k(&v, P, P.Sk > 0 ? P.v : P.q, half);
+  if (!rc) rc = cross_map_q(&o, P, P.o, half);
+  if (rc) return rc;
+  auto kern = cross_fwd_kernel<T, DP, BIAS>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  if (e != cudaSuccess) return cuda_fail(e, "cross_fwd_kernel shared memory");
+  const int64_t items = static_cast<int64_t>(P.units) * P.splits * P.Hkv * P.B;
+  const int grid = static_cast<int>(items < cross_sms() ? items : cross_sms());
+  kern<<<grid, 512, C::SMEM, st>>>(q, k, v, o, P);
+  rc = check_launch("cross_fwd_kernel");
+  if (rc || P.splits == 1) return rc;
+  const int64_t rows = static_cast<int64_t>(P.B) * P.Hq * P.Sq;
+  cross_combine_kernel<T><<<static_cast<unsigned>((rows + 7) / 8), 256, 0, st>>>(P);
+  return check_launch("cross_combine_kernel");
+}
+
+template <typename T>
+static int fwd_launch(const CrossParams& P, cudaStream_t st) {
+  if (P.D <= 64) return P.bias2 ? fwd_launch_cfg<T, 64, true>(P, st) : fwd_launch_cfg<T, 64, false>(P, st);
+  return P.bias2 ? fwd_launch_cfg<T, 128, true>(P, st) : fwd_launch_cfg<T, 128, false>(P, st);
+}
+
+}  // namespace h3b

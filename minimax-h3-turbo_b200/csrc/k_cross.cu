@@ -1,6 +1,4 @@
 // Translation unit: cross attention and its gradients (cross_attn.cuh).
-#include <type_traits>
-
 #include "cross_attn.cuh"
 
 namespace h3b {
