@@ -22,7 +22,7 @@ template <int DP>
 struct FwdCfg {
   static constexpr int NSUB = DP / 64;
   static constexpr int TILE = NSUB * static_cast<int>(SUB_BYTES);  // bytes of a 128-row tile
-  static constexpr int STAGES = DP == 128 ? 4 : 8;                 // ring of K and V tiles
+  static constexpr int STAGES = DP == 128 ? 4 : 8;                 // ring of K and V tiles (even: K in even stages)
   static constexpr int STAGE_PARTS = 2;                            // staging buffers of 64 channels for the output
   static constexpr int SMEM = 2 * TILE + STAGES * TILE + STAGE_PARTS * static_cast<int>(SUB_BYTES) + 2 * 2 * CT * 4 + 512;
   static constexpr uint32_t TMEM_COLS = 512;
@@ -91,6 +91,8 @@ __global__ void __launch_bounds__(512, 1)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t n_items = static_cast<int64_t>(P.units) * P.splits * P.Hkv * P.B;
+  // with any mask every V tile passes warp 14 (in step with the ring: a phase it skipped could be taken for another)
+  const bool masked = BIAS || P.kv_lens != nullptr;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) {
@@ -323,7 +325,7 @@ __global__ void __launch_bounds__(512, 1)
         constexpr uint32_t idQK = idesc_f16<T>(CT, CT, false), idPV = idesc_f16<T>(CT, DP, true);
         const uint32_t aQ = smem_u32(sQ), aKV = smem_u32(sKV);
         int st = 0;
-        uint32_t kph = 0, qph[2] = {0, 0}, pph[2] = {0, 0}, oph[2] = {1, 1}, cph = 0;  // cph: a phase bit per stage
+        uint32_t kph = 0, qph[2] = {0, 0}, pph[2] = {0, 0}, oph[2] = {1, 1};
         auto step = [&] {
           if (++st == C::STAGES) st = 0, kph ^= 1;
         };
@@ -350,16 +352,12 @@ __global__ void __launch_bounds__(512, 1)
         }
         while (have && ok) {
           bool more = false;
-          const int64_t len = ca_len(P.kv_lens, cur.b, P.Sk);
           for (int t = cur.t0; ok && t < cur.t1; ++t) {
             const bool last = t == cur.t1 - 1;
             if (last) more = fwd_next(P, it, n_items, nxt);
             const int vst = st;
             if (!(ok = mbar_wait(&kv_full[vst], kph, abort_flag))) break;
-            if (needs_zeroing(P, len, t)) {
-              if (!(ok = mbar_wait(&v_clean[vst], (cph >> vst) & 1, abort_flag))) break;
-              cph ^= 1u << vst;
-            }
+            if (masked && !(ok = mbar_wait(&v_clean[vst], kph, abort_flag))) break;
             step();
             const bool then_qk = !last || more;
             const int kst = st;
@@ -436,7 +434,7 @@ __global__ void __launch_bounds__(512, 1)
           if (qfills[s]) mbar_wait_drain(&q_full[s], static_cast<uint32_t>((qfills[s] - 1) & 1));
       }
       __syncwarp();
-    } else if (warp == 14) {
+    } else if (warp == 14 && masked) {
       // ---------------------------------------------------------------------------------------- rows of masked keys
       int st = 0;
       uint32_t kph = 0;
@@ -446,8 +444,8 @@ __global__ void __launch_bounds__(512, 1)
         const int64_t len = ca_len(P.kv_lens, u.b, P.Sk);
         for (int t = u.t0; ok && t < u.t1; ++t) {
           if (++st == C::STAGES) st = 0, kph ^= 1;  // the K tile
+          if (!(ok = warp_wait(&kv_full[st], kph, abort_flag))) break;
           if (needs_zeroing(P, len, t)) {
-            if (!(ok = warp_wait(&kv_full[st], kph, abort_flag))) break;
             for (int j = lane; j < CT; j += 32) {
               const int64_t key = static_cast<int64_t>(t) * CT + j;
               if (key >= len || (BIAS && P.bias2[u.b * P.Skp + key] == -INFINITY))
@@ -457,8 +455,8 @@ __global__ void __launch_bounds__(512, 1)
             }
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&v_clean[st]);
           }
+          if (lane == 0) mbar_arrive(&v_clean[st]);
           if (++st == C::STAGES) st = 0, kph ^= 1;
         }
       }

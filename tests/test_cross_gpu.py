@@ -85,6 +85,16 @@ def test_many_queries_over_few_keys_and_a_long_stream():
     check_all(q, k, v, do, kv_lens=torch.tensor([12345], device=DEV))
 
 
+@pytest.mark.parametrize("d,dt", [(128, BF), (64, FP)])
+@pytest.mark.parametrize("kind", ["none", "lens", "bias"])
+def test_more_work_than_ctas(d, dt, kind):
+    """Every CTA walks several pairs of query tiles, the last pair of a head is half empty, entries differ in length."""
+    q, k, v, do = make(3, 1400, 300, 20, 20, d, dt, seed=13)
+    check_all(q, k, v, do, **mask_of(kind, 3, 300))
+    q, k, v, do = make(4, 1290, 129, 12, 6, d, dt, seed=14)
+    check_all(q, k, v, do, **mask_of(kind, 4, 129))
+
+
 def test_large_scores_and_own_scale():
     for std, scale in ((6.0, None), (1.0, 0.7), (0.02, None)):  # nearly one-hot rows, an explicit scale, nearly flat rows
         q, k, v, do = make(2, 260, 390, 3, 3, 128, BF, seed=9, std=std)
