@@ -1,0 +1,925 @@
+// Cross attention gradients on the tcgen05 tensor cores, two kernels, no atomics.
+//
+// cross_dq_kernel: a unit is one query tile (128 rows) over a range of key tiles:
+//     S = Q K^T, dP = G V^T, dS = P (dP - delta), dQ += dS K           (rows of tensor memory are queries)
+//   and, once per row, delta = g . o.  When all keys fit one tile delta = sum_j p_j dP_j instead: the same number without
+//   the rounding of o, which is all there is to dS when one key takes the whole weight.  It writes -lse and delta of every
+//   tile row in tile order for the second kernel.
+// cross_dkv_kernel: a unit is one key tile over a range of query tiles of all heads that share it:
+//     S^T = K Q^T, dP^T = V G^T, dV += P^T G, dK += dS^T Q             (rows of tensor memory are keys)
+// Each computes S and dP: 7 products of the scores' size instead of 5.  The price of sharing them (dQ summed over key tiles
+// by atomics, in a changing order, through fp32 buffers in memory) is not paid: results have the same bits every time.
+// P and dS are rounded to the operand type for the second products (8 or 11 bits, relative to each element); sums are fp32.
+//
+// Warps of both: 0-7 elementwise work, thread = row, warps 0-3 the first 64 columns, 4-7 the other 64; 8-11 epilogue
+// (accumulators -> global memory); 12 MMA issue; 13 copies; 14 (dq) zeroes K rows of masked keys before their product.
+// P and dS go back to tensor memory over the columns that their own warps read S or dP from.
+#include "cross_common.cuh"
+
+namespace h3b {
+
+struct BwdTile {
+  int64_t it;
+  int b, hk, split, tile, t0, t1, t;  // `tile`: the unit's own tile; t: the tile of the other side
+  __device__ __forceinline__ bool first() const { return t == t0; }
+  __device__ __forceinline__ bool last() const { return t == t1 - 1; }
+};
+
+// range [t0, t1) of n tiles that split `s` of `splits` gets
+__device__ __forceinline__ void split_range(int n, int splits, int s, int& t0, int& t1) {
+  const int per = (n + splits - 1) / splits;
+  t0 = min(s * per, n);
+  t1 = min(t0 + per, n);
+}
+
+// Walks the units of this CTA.  DQ: own tiles are query tiles, the other side key tiles; else the other way round.
+template <bool DQ>
+struct BwdWalk {
+  const CrossParams& P;
+  int64_t n;
+  int own, splits;
+  BwdTile c;
+  bool valid;
+  __device__ __forceinline__ BwdWalk(const CrossParams& p) : P(p) {
+    own = DQ ? p.q_tiles : static_cast<int>(p.Skp / CT);
+    splits = DQ ? p.splits : p.kv_splits;
+    n = static_cast<int64_t>(own) * splits * p.Hkv * p.B;
+    c.it = blockIdx.x;
+    seek();
+  }
+  __device__ __forceinline__ void unit(int64_t it, BwdTile& u) const {
+    u.tile = static_cast<int>(it % own);
+    int64_t r = it / own;
+    u.split = static_cast<int>(r % splits);
+    r /= splits;
+    u.hk = static_cast<int>(r % P.Hkv);
+    u.b = static_cast<int>(r / P.Hkv);
+    const int64_t len = ca_len(P.kv_lens, u.b, P.Sk);
+    const int other = DQ ? static_cast<int>((len + CT - 1) / CT) : static_cast<int64_t>(u.tile) * CT < len ? P.q_tiles : 0;
+    split_range(other, splits, u.split, u.t0, u.t1);
+    u.t = u.t0;
+  }
+  __device__ __forceinline__ void seek() {  // the first unit from c.it on with work
+    for (valid = false; c.it < n; c.it += gridDim.x) {
+      unit(c.it, c);
+      if (c.t1 > c.t0) {
+        valid = true;
+        return;
+      }
+    }
+  }
+  __device__ __forceinline__ void next() {
+    if (++c.t < c.t1) return;
+    c.it += gridDim.x;
+    seek();
+  }
+};
+
+template <int DP>
+struct BwdCfg {
+  static constexpr int NSUB = DP / 64;
+  static constexpr int TILE = NSUB * static_cast<int>(SUB_BYTES);
+  static constexpr int SMEM = 7 * TILE + 2048 + 512;  // 7 tiles, small vectors, barriers
+  static constexpr uint32_t TMEM_COLS = 512;
+};
+
+// 32 columns of a row of 16-bit results: 16-byte stores (n: valid columns from here on, a multiple of 8)
+template <typename T>
+__device__ __forceinline__ void store_cols(T* dst, const uint32_t (&o)[32], float w, int n) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (8 * i < n) {
+      uint4 v;
+      uint32_t* vv = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        vv[e] = pack2<T>(__uint_as_float(o[8 * i + 2 * e]) * w, __uint_as_float(o[8 * i + 2 * e + 1]) * w);
+      *reinterpret_cast<uint4*>(dst + 8 * i) = v;
+    }
+}
+__device__ __forceinline__ void store_cols_f32(float* dst, const uint32_t (&o)[32], float w, int n) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (4 * i < n)
+      *reinterpret_cast<float4*>(dst + 4 * i) =
+          make_float4(__uint_as_float(o[4 * i]) * w, __uint_as_float(o[4 * i + 1]) * w, __uint_as_float(o[4 * i + 2]) * w,
+                      __uint_as_float(o[4 * i + 3]) * w);
+}
+
+// ------------------------------------------------------------------------------------------------ dQ
+template <typename T, int DP, bool BIAS>
+__global__ void __launch_bounds__(512, 1)
+    cross_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG,
+                    const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const CrossParams P) {
+  using C = BwdCfg<DP>;
+  constexpr int KS = 3, VS = 2;  // ring stages
+  extern __shared__ __align__(1024) unsigned char ca_smem[];
+  unsigned char* sQ = ca_smem;
+  unsigned char* sG = sQ + C::TILE;
+  unsigned char* sK = sG + C::TILE;
+  unsigned char* sV = sK + KS * C::TILE;
+  float* part = reinterpret_cast<float*>(sV + VS * C::TILE);  // [unit parity][2][128] halves of a row's delta
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(part + 512);
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* g_full = q_empty + 1;
+  uint64_t* g_empty = g_full + 1;
+  uint64_t* k_full = g_empty + 1;
+  uint64_t* k_empty = k_full + KS;
+  uint64_t* k_clean = k_empty + KS;
+  uint64_t* v_full = k_clean + KS;
+  uint64_t* v_empty = v_full + VS;
+  uint64_t* s_full = v_empty + VS;
+  uint64_t* dp_full = s_full + 2;
+  uint64_t* ds_full = dp_full + 1;
+  uint64_t* part_full = ds_full + 1;
+  uint64_t* dq_full = part_full + 1;
+  uint64_t* dq_empty = dq_full + 1;
+  uint64_t* done = dq_empty + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool masked = BIAS || P.kv_lens != nullptr;
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    mbar_init(g_full, 1);
+    mbar_init(g_empty, 9);  // the last dP product, and the eight warps that take delta from it
+    for (int s = 0; s < KS; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&k_clean[s], 1);
+    }
+    for (int s = 0; s < VS; ++s) {
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_empty[s], 1);
+    }
+    mbar_init(&s_full[0], 1);
+    mbar_init(&s_full[1], 1);
+    mbar_init(dp_full, 1);
+    mbar_init(ds_full, 8);
+    mbar_init(part_full, 8);
+    mbar_init(dq_full, 1);
+    mbar_init(dq_empty, 4);
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmG);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  if (warp == 12) {
+    tmem_alloc(tmem_slot, C::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t tDP = tmem + 2 * CT, tDQ = tmem + 3 * CT;  // S0 S1 dP dQ
+
+  if (warp < 8) {
+    // ------------------------------------------------------------------------------------------ P, dS
+    regs_inc<176>();
+    const int half = warp >> 2, row = threadIdx.x & (CT - 1), qr = row / P.G, hg = row - qr * P.G;
+    const uint32_t at = (static_cast<uint32_t>(warp & 3) << 21) + half * 64;  // this warp's lanes and columns
+    uint32_t sph = 0, dph = 0, gph = 0, xph = 0, sbuf = 0;
+    float nlse2 = -INFINITY, delta = 0.f;
+    bool ok = true, valid = false;
+    int64_t len = 0;
+    for (BwdWalk<true> w(P); ok && w.valid; w.next()) {
+      const BwdTile& u = w.c;
+      const int64_t s = static_cast<int64_t>(u.tile) * P.nq + qr;
+      const int64_t rid = (static_cast<int64_t>(u.b) * P.Hq + u.hk * P.G + hg) * P.Sq + s;
+      const bool one_tile = P.splits == 1 && u.t1 - u.t0 == 1;
+      if (u.first()) {
+        len = ca_len(P.kv_lens, u.b, P.Sk);
+        valid = qr < P.nq && s < P.Sq;
+        const float e = valid ? P.lse[rid] : -INFINITY;
+        nlse2 = e == -INFINITY ? -INFINITY : -e * CA_LOG2E;  // rows outside, and rows without keys: every p is 0
+      }
+      if (!(ok = warp_wait(&s_full[sbuf], sph, abort_flag))) break;
+      tc_fence_after();
+      const uint32_t tS = tmem + sbuf * CT + at;
+      float p[64];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t r[32];
+        tmem_ld_32x32b_x32(tS + 32 * c, r);
+        tmem_ld_wait();
+        if constexpr (BIAS) {
+          const float4* b4 = reinterpret_cast<const float4*>(P.bias2 + u.b * P.Skp + static_cast<int64_t>(u.t) * CT + half * 64 + 32 * c);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float4 bb = __ldg(b4 + i);
+            const float bv[4] = {bb.x, bb.y, bb.z, bb.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float x = ex2(fmaf(__uint_as_float(r[4 * i + e]), P.scale2, bv[e] + nlse2));
+              p[32 * c + 4 * i + e] = bv[e] == -INFINITY ? 0.f : x;
+            }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) p[32 * c + i] = ex2(fmaf(__uint_as_float(r[i]), P.scale2, nlse2));
+        }
+      }
+      const int64_t lim = len - (static_cast<int64_t>(u.t) * CT + half * 64);  // columns in use, from this warp's first
+      if (!BIAS && lim < 64) {
+#pragma unroll
+        for (int i = 0; i < 64; ++i)
+          if (i >= lim) p[i] = 0.f;
+      }
+      if (nlse2 == -INFINITY) {  // also when the row's own scores are not numbers
+#pragma unroll
+        for (int i = 0; i < 64; ++i) p[i] = 0.f;
+      }
+      if (u.first()) {
+        if (!(ok = warp_wait(g_full, gph, abort_flag))) break;
+        gph ^= 1;
+        if (!one_tile) {  // half of g . o of this row: channels [half DP / 2, ..)
+          float d = 0.f;
+          const T* orow = static_cast<const T*>(P.o.ptr) + u.b * P.o.stride_b + s * P.o.stride_s + (u.hk * P.G + hg) * P.o.stride_h;
+#pragma unroll
+          for (int c = 0; c < DP / 16; ++c) {
+            const int ch = half * (DP / 2) + 8 * c;
+            if (valid && ch < P.D) {
+              const uint4 ov = __ldg(reinterpret_cast<const uint4*>(orow + ch));
+              const uint4 gv = *reinterpret_cast<const uint4*>(sG + (ch >> 6) * SUB_BYTES + row * 128 +
+                                                               ((((ch & 63) >> 3) ^ (row & 7)) << 4));
+              const T* oe = reinterpret_cast<const T*>(&ov);
+              const T* ge = reinterpret_cast<const T*>(&gv);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) d = fmaf(static_cast<float>(oe[e]), static_cast<float>(ge[e]), d);
+            }
+          }
+          part[(2 * xph + half) * CT + row] = d;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(g_empty);
+      }
+      if (!(ok = warp_wait(dp_full, dph, abort_flag))) break;
+      dph ^= 1;
+      tc_fence_after();
+      float dp[64];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t r[32];
+        tmem_ld_32x32b_x32(tDP + at + 32 * c, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) dp[32 * c + i] = __uint_as_float(r[i]);
+      }
+      if (masked) {  // a masked key's dP may be anything
+#pragma unroll
+        for (int i = 0; i < 64; ++i) dp[i] = p[i] == 0.f ? 0.f : dp[i];
+      }
+      if (u.first()) {
+        if (one_tile) {
+          float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int i = 0; i < 64; ++i) d[i & 3] = fmaf(p[i], dp[i], d[i & 3]);
+          part[(2 * xph + half) * CT + row] = (d[0] + d[1]) + (d[2] + d[3]);
+        }
+        // a unit's halves are overwritten two units later: past the next unit's wait, which every warp's reads come before
+        __syncwarp();
+        if (lane == 0) mbar_arrive(part_full);
+        if (!(ok = warp_wait(part_full, xph, abort_flag))) break;
+        delta = part[2 * xph * CT + row] + part[(2 * xph + 1) * CT + row];
+        xph ^= 1;
+        if (u.split == 0 && half == 0) {
+          float* st = P.stats + ((static_cast<int64_t>(u.b) * P.Hkv + u.hk) * P.q_tiles + u.tile) * (2 * CT);
+          st[row] = nlse2;
+          st[CT + row] = valid ? delta : 0.f;
+        }
+      }
+      uint32_t pk[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) pk[i] = pack2<T>(p[2 * i] * (dp[2 * i] - delta), p[2 * i + 1] * (dp[2 * i + 1] - delta));
+      tmem_st_32x32b_x32(tS, pk);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ds_full);
+      sbuf ^= 1;
+      if (sbuf == 0) sph ^= 1;
+    }
+  } else if (warp < 12) {
+    // ------------------------------------------------------------------------------------------ epilogue
+    regs_dec<96>();
+    const int row = threadIdx.x & (CT - 1), qr = row / P.G, hg = row - qr * P.G;
+    const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
+    uint32_t ph = 0;
+    BwdWalk<true> w(P);
+    BwdTile u;
+    bool ok = true;
+    for (int64_t it = blockIdx.x; ok && it < w.n; it += gridDim.x) {
+      w.unit(it, u);
+      const int64_t s = static_cast<int64_t>(u.tile) * P.nq + qr;
+      const bool valid = qr < P.nq && s < P.Sq, any = u.t1 > u.t0;
+      if (any) {
+        if (!(ok = warp_wait(dq_full, ph, abort_flag))) break;
+        ph ^= 1;
+        tc_fence_after();
+      }
+      const int64_t rid = (static_cast<int64_t>(u.b) * P.Hq + u.hk * P.G + hg) * P.Sq + s;
+      T* dst = static_cast<T*>(P.dq.ptr) + u.b * P.dq.stride_b + s * P.dq.stride_s + (u.hk * P.G + hg) * P.dq.stride_h;
+      float* dst32 = P.part_dq + (static_cast<int64_t>(u.split) * P.B * P.Hq * P.Sq + rid) * P.D;
+#pragma unroll 1
+      for (int c = 0; c < DP / 32; ++c) {
+        uint32_t o[32];
+        if (any) {
+          tmem_ld_32x32b_x32(tDQ + lanes + 32 * c, o);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0;
+        }
+        if (!valid) continue;
+        if (P.splits > 1) store_cols_f32(dst32 + 32 * c, o, P.scale, P.D - 32 * c);
+        else store_cols<T>(dst + 32 * c, o, P.scale, P.D - 32 * c);
+      }
+      if (any) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(dq_empty);
+      }
+    }
+  } else {
+    regs_dec<64>();
+    if (warp == 12) {
+      if (lane == 0) {
+        // -------------------------------------------------------------------------------------- MMA issue
+        constexpr uint32_t idS = idesc_f16<T>(CT, CT, false), idD = idesc_f16<T>(CT, DP, true);
+        const uint32_t aQ = smem_u32(sQ), aG = smem_u32(sG), aK = smem_u32(sK), aV = smem_u32(sV);
+        BwdWalk<true> ws(P), wp(P), wd(P);  // the next S, dP and dQ product
+        int sk = 0, pv = 0, dk = 0;
+        uint32_t skph = 0, pvph = 0, qph = 0, gph = 0, dsph = 0, dqph = 1, sbuf = 0, dbuf = 0;
+        bool ok = true;
+        auto do_s = [&] {
+          if (!ok || !ws.valid) return;
+          if (!(ok = mbar_wait(&k_full[sk], skph, abort_flag))) return;
+          if (masked && !(ok = mbar_wait(&k_clean[sk], skph, abort_flag))) return;
+          if (ws.c.first()) {
+            if (!(ok = mbar_wait(q_full, qph, abort_flag))) return;
+            qph ^= 1;
+          }
+          tc_fence_after();
+          for (int kk = 0; kk < DP / 16; ++kk)
+            mma_f16_ss(tmem + sbuf * CT, desc_rows(aQ, kk), desc_rows(aK + sk * C::TILE, kk), idS, kk > 0);
+          mma_commit(&s_full[sbuf]);
+          if (ws.c.last()) mma_commit(q_empty);
+          sbuf ^= 1;
+          if (++sk == KS) sk = 0, skph ^= 1;
+          ws.next();
+        };
+        auto do_dp = [&] {
+          if (!ok || !wp.valid) return;
+          if (!(ok = mbar_wait(&v_full[pv], pvph, abort_flag))) return;
+          if (wp.c.first()) {
+            if (!(ok = mbar_wait(g_full, gph, abort_flag))) return;
+            gph ^= 1;
+          }
+          tc_fence_after();
+          for (int kk = 0; kk < DP / 16; ++kk) mma_f16_ss(tDP, desc_rows(aG, kk), desc_rows(aV + pv * C::TILE, kk), idS, kk > 0);
+          mma_commit(dp_full);
+          mma_commit(&v_empty[pv]);
+          if (wp.c.last()) mma_commit(g_empty);
+          if (++pv == VS) pv = 0, pvph ^= 1;
+          wp.next();
+        };
+        do_s();
+        do_dp();
+        do_s();
+        while (ok && wd.valid) {
+          if (!(ok = mbar_wait(ds_full, dsph, abort_flag))) break;  // dS is written, dP has been read
+          dsph ^= 1;
+          const bool same = wp.valid && wp.c.it == wd.c.it;
+          if (same) do_dp();  // a new unit's dP waits for its G tile: not before this unit's last product
+          if (!ok) break;
+          if (wd.c.first()) {
+            if (!(ok = mbar_wait(dq_empty, dqph, abort_flag))) break;
+            dqph ^= 1;
+          }
+          tc_fence_after();
+          for (int kk = 0; kk < CT / 16; ++kk)
+            mma_f16_ts(tDQ, tmem + dbuf * CT + (kk >> 2) * 64 + (kk & 3) * 8, desc_chan(aK + dk * C::TILE, kk), idD,
+                       !wd.c.first() || kk > 0);
+          mma_commit(&k_empty[dk]);
+          if (wd.c.last()) mma_commit(dq_full);
+          dbuf ^= 1;
+          if (++dk == KS) dk = 0;
+          wd.next();
+          if (!same) do_dp();
+          do_s();
+        }
+      }
+      __syncwarp();
+    } else if (warp == 13) {
+      if (lane == 0) {
+        // -------------------------------------------------------------------------------------- copies
+        int k = 0, v = 0, kfills = 0, vfills = 0, ufills = 0;
+        uint32_t kph = 1, vph = 1, uph = 1;
+        bool ok = true;
+        const uint32_t q_bytes = static_cast<uint32_t>(C::NSUB * 128 * P.G * P.nq);
+        for (BwdWalk<true> w(P); ok && w.valid; w.next()) {
+          const BwdTile& u = w.c;
+          if (u.first()) {
+            if (!(ok = mbar_wait(q_empty, uph, abort_flag))) break;
+            mbar_arrive_expect_tx(q_full, q_bytes);
+            for (int p = 0; p < C::NSUB; ++p) tma_load_5d(sQ + p * SUB_BYTES, &tmQ, q_full, 64 * p, 0, u.hk, u.tile * P.nq, u.b);
+          }
+          if (!(ok = mbar_wait(&k_empty[k], kph, abort_flag))) {
+            if (u.first()) mbar_wait_drain(q_full, (ufills) & 1);
+            break;
+          }
+          mbar_arrive_expect_tx(&k_full[k], C::TILE);
+          for (int p = 0; p < C::NSUB; ++p) tma_load_4d(sK + k * C::TILE + p * SUB_BYTES, &tmK, &k_full[k], 64 * p, u.hk, u.t * CT, u.b);
+          ++kfills;
+          if (++k == KS) k = 0, kph ^= 1;
+          if (u.first()) {
+            if (!(ok = mbar_wait(g_empty, uph, abort_flag))) {
+              mbar_wait_drain(q_full, (ufills) & 1);
+              break;
+            }
+            uph ^= 1;
+            mbar_arrive_expect_tx(g_full, q_bytes);
+            for (int p = 0; p < C::NSUB; ++p) tma_load_5d(sG + p * SUB_BYTES, &tmG, g_full, 64 * p, 0, u.hk, u.tile * P.nq, u.b);
+            ++ufills;
+          }
+          if (!(ok = mbar_wait(&v_empty[v], vph, abort_flag))) break;
+          mbar_arrive_expect_tx(&v_full[v], C::TILE);
+          for (int p = 0; p < C::NSUB; ++p) tma_load_4d(sV + v * C::TILE + p * SUB_BYTES, &tmV, &v_full[v], 64 * p, u.hk, u.t * CT, u.b);
+          ++vfills;
+          if (++v == VS) v = 0, vph ^= 1;
+        }
+        for (int j = kfills > KS ? kfills - KS : 0; j < kfills; ++j)  // copies in flight land before the memory goes away
+          if (!mbar_wait_drain(&k_full[j % KS], static_cast<uint32_t>((j / KS) & 1))) break;
+        for (int j = vfills > VS ? vfills - VS : 0; j < vfills; ++j)
+          if (!mbar_wait_drain(&v_full[j % VS], static_cast<uint32_t>((j / VS) & 1))) break;
+        if (ufills) {
+          mbar_wait_drain(q_full, static_cast<uint32_t>((ufills - 1) & 1));
+          mbar_wait_drain(g_full, static_cast<uint32_t>((ufills - 1) & 1));
+        }
+      }
+      __syncwarp();
+    } else if (warp == 14 && masked) {
+      // ---------------------------------------------------------------------------------------- rows of masked keys
+      int k = 0;
+      uint32_t kph = 0;
+      for (BwdWalk<true> w(P); w.valid; w.next()) {
+        const BwdTile& u = w.c;
+        if (!warp_wait(&k_full[k], kph, abort_flag)) break;
+        const int64_t len = ca_len(P.kv_lens, u.b, P.Sk);
+        if (BIAS || (len < P.Sk && static_cast<int64_t>(u.t + 1) * CT > len)) {
+          for (int j = lane; j < CT; j += 32) {
+            const int64_t key = static_cast<int64_t>(u.t) * CT + j;
+            if (key >= len || (BIAS && P.bias2[u.b * P.Skp + key] == -INFINITY))
+              for (int p = 0; p < C::NSUB; ++p)
+                for (int c = 0; c < 8; ++c)
+                  *reinterpret_cast<uint4*>(sK + k * C::TILE + p * SUB_BYTES + j * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        if (lane == 0) mbar_arrive(&k_clean[k]);
+        if (++k == KS) k = 0, kph ^= 1;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    if (lane == 0) {
+      mma_commit(done);
+      mbar_wait_drain(done, 0);
+    }
+    __syncwarp();
+    tmem_dealloc(tmem, C::TMEM_COLS);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ dK, dV
+template <typename T, int DP, bool BIAS>
+__global__ void __launch_bounds__(512, 1)
+    cross_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG,
+                     const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const CrossParams P) {
+  using C = BwdCfg<DP>;
+  constexpr int QS = 3, GS = 2, TS = 2;  // ring stages: Q and G tiles, row vectors
+  extern __shared__ __align__(1024) unsigned char ca_smem[];
+  unsigned char* sK = ca_smem;
+  unsigned char* sV = sK + C::TILE;
+  unsigned char* sQ = sV + C::TILE;
+  unsigned char* sG = sQ + QS * C::TILE;
+  float* sT = reinterpret_cast<float*>(sG + GS * C::TILE);  // [TS][-lse, delta][128]
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(sT + TS * 2 * CT);
+  uint64_t* k_empty = k_full + 1;
+  uint64_t* v_full = k_empty + 1;
+  uint64_t* v_empty = v_full + 1;
+  uint64_t* q_full = v_empty + 1;
+  uint64_t* q_empty = q_full + QS;
+  uint64_t* g_full = q_empty + QS;
+  uint64_t* g_empty = g_full + GS;
+  uint64_t* t_full = g_empty + GS;
+  uint64_t* t_empty = t_full + TS;
+  uint64_t* s_full = t_empty + TS;
+  uint64_t* p_full = s_full + 1;
+  uint64_t* dp_full = p_full + 1;
+  uint64_t* ds_full = dp_full + 1;
+  uint64_t* acc_full = ds_full + 1;
+  uint64_t* acc_empty = acc_full + 1;
+  uint64_t* done = acc_empty + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(k_full, 1);
+    mbar_init(k_empty, 1);
+    mbar_init(v_full, 1);
+    mbar_init(v_empty, 1);
+    for (int s = 0; s < QS; ++s) {
+      mbar_init(&q_full[s], 1);
+      mbar_init(&q_empty[s], 1);
+    }
+    for (int s = 0; s < GS; ++s) {
+      mbar_init(&g_full[s], 1);
+      mbar_init(&g_empty[s], 1);
+    }
+    for (int s = 0; s < TS; ++s) {
+      mbar_init(&t_full[s], 1);
+      mbar_init(&t_empty[s], 8);
+    }
+    mbar_init(s_full, 1);
+    mbar_init(p_full, 8);
+    mbar_init(dp_full, 1);
+    mbar_init(ds_full, 8);
+    mbar_init(acc_full, 1);
+    mbar_init(acc_empty, 4);
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmG);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  // rows of the query tiles that no copy writes (128 is not a multiple of G): their products have weight 0, but 0 x NaN
+  for (int i = threadIdx.x; i < (QS + GS) * C::NSUB * (CT - P.G * P.nq) * 8; i += blockDim.x) {
+    const int rows = CT - P.G * P.nq, c = i & 7, r = (i >> 3) % rows, p = (i >> 3) / rows;
+    *reinterpret_cast<uint4*>(sQ + p * SUB_BYTES + (P.G * P.nq + r) * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+  }
+  fence_proxy_async_smem();
+  if (warp == 12) {
+    tmem_alloc(tmem_slot, C::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t tDP = tmem + CT, tDV = tmem + 2 * CT, tDK = tmem + 3 * CT;  // S dP dV dK
+
+  if (warp < 8) {
+    // ------------------------------------------------------------------------------------------ P^T, dS^T
+    regs_inc<176>();
+    const int half = warp >> 2, row = threadIdx.x & (CT - 1);
+    const uint32_t at = (static_cast<uint32_t>(warp & 3) << 21) + half * 64;
+    uint32_t ph = 0, tph = 0;
+    int ts = 0;
+    bool ok = true, live = false;
+    float rb = 0.f;
+    for (BwdWalk<false> w(P); ok && w.valid; w.next()) {
+      const BwdTile& u = w.c;
+      if (u.first()) {
+        const int64_t key = static_cast<int64_t>(u.tile) * CT + row;
+        live = key < ca_len(P.kv_lens, u.b, P.Sk);
+        if constexpr (BIAS) {
+          rb = P.bias2[u.b * P.Skp + key];
+          live = live && rb != -INFINITY;
+        }
+      }
+      if (!(ok = warp_wait(&t_full[ts], tph, abort_flag))) break;
+      if (!(ok = warp_wait(s_full, ph, abort_flag))) break;
+      tc_fence_after();
+      const float4* nl = reinterpret_cast<const float4*>(sT + ts * 2 * CT + half * 64);
+      const float4* dl = reinterpret_cast<const float4*>(sT + ts * 2 * CT + CT + half * 64);
+      float p[64];
+      uint32_t pk[32];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t r[32];
+        tmem_ld_32x32b_x32(tmem + at + 32 * c, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float4 n4 = nl[8 * c + i];
+          const float nv[4] = {n4.x, n4.y, n4.z, n4.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = ex2(fmaf(__uint_as_float(r[4 * i + e]), P.scale2, BIAS ? nv[e] + rb : nv[e]));
+            p[32 * c + 4 * i + e] = live ? x : 0.f;
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 32; ++i) pk[i] = pack2<T>(p[2 * i], p[2 * i + 1]);
+      tmem_st_32x32b_x32(tmem + at, pk);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full);
+      if (!(ok = warp_wait(dp_full, ph, abort_flag))) break;
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t r[32];
+        tmem_ld_32x32b_x32(tDP + at + 32 * c, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float4 d4 = dl[8 * c + i];
+          const float dv[4] = {d4.x, d4.y, d4.z, d4.w};
+          float ds[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = p[32 * c + 4 * i + e] * (__uint_as_float(r[4 * i + e]) - dv[e]);
+            ds[e] = live ? x : 0.f;
+          }
+          pk[16 * c + 2 * i] = pack2<T>(ds[0], ds[1]);
+          pk[16 * c + 2 * i + 1] = pack2<T>(ds[2], ds[3]);
+        }
+      }
+      tmem_st_32x32b_x32(tDP + at, pk);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(ds_full);
+        mbar_arrive(&t_empty[ts]);
+      }
+      ph ^= 1;
+      if (++ts == TS) ts = 0, tph ^= 1;
+    }
+  } else if (warp < 12) {
+    // ------------------------------------------------------------------------------------------ epilogue
+    regs_dec<96>();
+    const int row = threadIdx.x & (CT - 1);
+    const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
+    uint32_t ph = 0;
+    BwdWalk<false> w(P);
+    BwdTile u;
+    bool ok = true;
+    const int64_t part = static_cast<int64_t>(P.B) * P.Hkv * P.Sk * P.D;  // elements of one split's dK or dV
+    for (int64_t it = blockIdx.x; ok && it < w.n; it += gridDim.x) {
+      w.unit(it, u);
+      const int64_t key = static_cast<int64_t>(u.tile) * CT + row;
+      const bool valid = key < P.Sk, any = u.t1 > u.t0;
+      if (any) {
+        if (!(ok = warp_wait(acc_full, ph, abort_flag))) break;
+        ph ^= 1;
+        tc_fence_after();
+      }
+      T* dk = static_cast<T*>(P.dk.ptr) + u.b * P.dk.stride_b + key * P.dk.stride_s + u.hk * P.dk.stride_h;
+      T* dv = static_cast<T*>(P.dv.ptr) + u.b * P.dv.stride_b + key * P.dv.stride_s + u.hk * P.dv.stride_h;
+      float* dk32 = P.part_dk + u.split * 2 * part + ((static_cast<int64_t>(u.b) * P.Hkv + u.hk) * P.Sk + key) * P.D;
+#pragma unroll 1
+      for (int c = 0; c < 2 * (DP / 32); ++c) {
+        const bool is_k = c >= DP / 32;
+        const int col = 32 * (is_k ? c - DP / 32 : c);
+        uint32_t o[32];
+        if (any) {
+          tmem_ld_32x32b_x32((is_k ? tDK : tDV) + lanes + col, o);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0;
+        }
+        if (!valid) continue;
+        const float f = is_k ? P.scale : 1.f;
+        if (P.kv_splits > 1) store_cols_f32(dk32 + (is_k ? 0 : part) + col, o, f, P.D - col);
+        else store_cols<T>((is_k ? dk : dv) + col, o, f, P.D - col);
+      }
+      if (any) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(acc_empty);
+      }
+    }
+  } else {
+    regs_dec<64>();
+    if (warp == 12) {
+      if (lane == 0) {
+        // -------------------------------------------------------------------------------------- MMA issue
+        constexpr uint32_t idS = idesc_f16<T>(CT, CT, false), idD = idesc_f16<T>(CT, DP, true);
+        const uint32_t aQ = smem_u32(sQ), aG = smem_u32(sG), aK = smem_u32(sK), aV = smem_u32(sV);
+        BwdWalk<false> ws(P), wp(P), wd(P);  // the next S^T, dP^T, and the tile in hand
+        int sq = 0, pg = 0, dq = 0, dg = 0;
+        uint32_t sqph = 0, pgph = 0, kph = 0, vph = 0, ph = 0, aph = 1;
+        bool ok = true;
+        auto do_s = [&] {
+          if (!ok || !ws.valid) return;
+          if (ws.c.first()) {
+            if (!(ok = mbar_wait(k_full, kph, abort_flag))) return;
+            kph ^= 1;
+          }
+          if (!(ok = mbar_wait(&q_full[sq], sqph, abort_flag))) return;
+          tc_fence_after();
+          for (int kk = 0; kk < DP / 16; ++kk) mma_f16_ss(tmem, desc_rows(aK, kk), desc_rows(aQ + sq * C::TILE, kk), idS, kk > 0);
+          mma_commit(s_full);
+          if (ws.c.last()) mma_commit(k_empty);
+          if (++sq == QS) sq = 0, sqph ^= 1;
+          ws.next();
+        };
+        auto do_dp = [&] {
+          if (!ok || !wp.valid) return;
+          if (wp.c.first()) {
+            if (!(ok = mbar_wait(v_full, vph, abort_flag))) return;
+            vph ^= 1;
+          }
+          if (!(ok = mbar_wait(&g_full[pg], pgph, abort_flag))) return;
+          tc_fence_after();
+          for (int kk = 0; kk < DP / 16; ++kk) mma_f16_ss(tDP, desc_rows(aV, kk), desc_rows(aG + pg * C::TILE, kk), idS, kk > 0);
+          mma_commit(dp_full);
+          if (wp.c.last()) mma_commit(v_empty);
+          if (++pg == GS) pg = 0, pgph ^= 1;
+          wp.next();
+        };
+        do_s();
+        do_dp();
+        while (ok && wd.valid) {
+          const uint32_t acc = !wd.c.first();
+          const bool last = wd.c.last();
+          if (!(ok = mbar_wait(p_full, ph, abort_flag))) break;
+          if (!acc) {
+            if (!(ok = mbar_wait(acc_empty, aph, abort_flag))) break;
+            aph ^= 1;
+          }
+          tc_fence_after();
+          for (int kk = 0; kk < CT / 16; ++kk)
+            mma_f16_ts(tDV, tmem + (kk >> 2) * 64 + (kk & 3) * 8, desc_chan(aG + dg * C::TILE, kk), idD, acc || kk > 0);
+          mma_commit(&g_empty[dg]);
+          if (++dg == GS) dg = 0;
+          do_s();
+          if (!ok || !(ok = mbar_wait(ds_full, ph, abort_flag))) break;
+          tc_fence_after();
+          for (int kk = 0; kk < CT / 16; ++kk)
+            mma_f16_ts(tDK, tDP + (kk >> 2) * 64 + (kk & 3) * 8, desc_chan(aQ + dq * C::TILE, kk), idD, acc || kk > 0);
+          mma_commit(&q_empty[dq]);
+          if (last) mma_commit(acc_full);
+          if (++dq == QS) dq = 0;
+          do_dp();
+          ph ^= 1;
+          wd.next();
+        }
+      }
+      __syncwarp();
+    } else if (warp == 13) {
+      if (lane == 0) {
+        // -------------------------------------------------------------------------------------- copies
+        int q = 0, g = 0, ts = 0, qfills = 0, gfills = 0, tfills = 0, kfills = 0, vfills = 0;
+        uint32_t qph = 1, gph = 1, tph = 1, uph = 1;
+        bool ok = true;
+        const uint32_t q_bytes = static_cast<uint32_t>(C::NSUB * 128 * P.G * P.nq);
+        for (BwdWalk<false> w(P); ok && w.valid; w.next()) {
+          const BwdTile& u = w.c;
+          if (u.first()) {
+            if (!(ok = mbar_wait(k_empty, uph, abort_flag))) break;
+            mbar_arrive_expect_tx(k_full, C::TILE);
+            for (int p = 0; p < C::NSUB; ++p) tma_load_4d(sK + p * SUB_BYTES, &tmK, k_full, 64 * p, u.hk, u.tile * CT, u.b);
+            ++kfills;
+          }
+          if (!(ok = mbar_wait(&q_empty[q], qph, abort_flag))) break;
+          mbar_arrive_expect_tx(&q_full[q], q_bytes);
+          for (int p = 0; p < C::NSUB; ++p) tma_load_5d(sQ + q * C::TILE + p * SUB_BYTES, &tmQ, &q_full[q], 64 * p, 0, u.hk, u.t * P.nq, u.b);
+          ++qfills;
+          if (++q == QS) q = 0, qph ^= 1;
+          if (!(ok = mbar_wait(&t_empty[ts], tph, abort_flag))) break;
+          mbar_arrive_expect_tx(&t_full[ts], 2 * CT * 4);
+          bulk_load(sT + ts * 2 * CT, P.stats + ((static_cast<int64_t>(u.b) * P.Hkv + u.hk) * P.q_tiles + u.t) * (2 * CT), 2 * CT * 4,
+                    &t_full[ts]);
+          ++tfills;
+          if (++ts == TS) ts = 0, tph ^= 1;
+          if (u.first()) {
+            if (!(ok = mbar_wait(v_empty, uph, abort_flag))) break;
+            uph ^= 1;
+            mbar_arrive_expect_tx(v_full, C::TILE);
+            for (int p = 0; p < C::NSUB; ++p) tma_load_4d(sV + p * SUB_BYTES, &tmV, v_full, 64 * p, u.hk, u.tile * CT, u.b);
+            ++vfills;
+          }
+          if (!(ok = mbar_wait(&g_empty[g], gph, abort_flag))) break;
+          mbar_arrive_expect_tx(&g_full[g], q_bytes);
+          for (int p = 0; p < C::NSUB; ++p) tma_load_5d(sG + g * C::TILE + p * SUB_BYTES, &tmG, &g_full[g], 64 * p, 0, u.hk, u.t * P.nq, u.b);
+          ++gfills;
+          if (++g == GS) g = 0, gph ^= 1;
+        }
+        auto drain = [](uint64_t* bars, int stages, int fills) {  // copies in flight land before the memory goes away
+          for (int j = fills > stages ? fills - stages : 0; j < fills; ++j)
+            if (!mbar_wait_drain(&bars[j % stages], static_cast<uint32_t>((j / stages) & 1))) break;
+        };
+        drain(q_full, QS, qfills);
+        drain(g_full, GS, gfills);
+        drain(t_full, TS, tfills);
+        drain(k_full, 1, kfills);
+        drain(v_full, 1, vfills);
+      }
+      __syncwarp();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    if (lane == 0) {
+      mma_commit(done);
+      mbar_wait_drain(done, 0);
+    }
+    __syncwarp();
+    tmem_dealloc(tmem, C::TMEM_COLS);
+  }
+}
+
+// Adds up the splits' partial gradients in order and rounds once.  Four channels per thread; `rows` rows of D channels,
+// row -> (b, s, h) with `inner` heads inside (dQ: [B, Hq, Sq], dK and dV: [B, Hkv, Sk]).
+template <typename T>
+__global__ void __launch_bounds__(256) cross_join_kernel(const float* part, int64_t stride, int splits, int64_t rows, int D,
+                                                         int64_t S, int H, h3b_attn_tensor out) {
+  const int per = D / 4;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (i >= rows * per) return;
+  const int64_t row = i / per;
+  const int c = static_cast<int>(i - row * per) * 4;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = 0; s < splits; ++s) {
+    const float4 v = *reinterpret_cast<const float4*>(part + s * stride + row * D + c);
+    a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
+  }
+  const int64_t s = row % S, bh = row / S, h = bh % H, b = bh / H;
+  *reinterpret_cast<uint2*>(static_cast<T*>(out.ptr) + b * out.stride_b + s * out.stride_s + h * out.stride_h + c) =
+      make_uint2(pack2<T>(a.x, a.y), pack2<T>(a.z, a.w));
+}
+template <typename T>
+static int join_launch(const float* part, int64_t stride, int splits, int64_t rows, int D, int64_t S, int H,
+                       const h3b_attn_tensor& out, cudaStream_t st) {
+  cross_join_kernel<T><<<static_cast<unsigned>((rows * (D / 4) + 255) / 256), 256, 0, st>>>(part, stride, splits, rows, D, S, H, out);
+  return check_launch("cross_join_kernel");
+}
+
+// Splits of the other side's tiles for `units` units of `tiles` tiles each: least time of the busiest SM, in tiles (a unit
+// costs about two more to fill and drain; splitting at all about three for the second kernel).
+static int bwd_splits(int64_t units, int64_t tiles) {
+  const int sms = cross_sms();
+  if (units >= 2 * sms || tiles <= 1) return 1;
+  int best = 1;
+  int64_t best_cost = (units + sms - 1) / sms * (tiles + 2);
+  for (int s = 2; s <= 64 && s <= tiles; ++s) {
+    const int64_t cost = (units * s + sms - 1) / sms * ((tiles + s - 1) / s + 2) + 3;
+    if (cost < best_cost) best = s, best_cost = cost;
+  }
+  return best;
+}
+
+template <typename T, int DP, bool BIAS>
+static int bwd_launch_cfg(const CrossParams& P, cudaStream_t st) {
+  using C = BwdCfg<DP>;
+  CUtensorMap q, g, k, v;
+  const bool half = std::is_same_v<T, __half>;
+  int rc = cross_map_q(&q, P, P.Sq > 0 ? P.q : P.k, half);
+  if (!rc) rc = cross_map_q(&g, P, P.Sq > 0 ? P.go : P.k, half);
+  if (!rc) rc = cross_map_k(&k, P, P.Sk > 0 ? P.k : P.q, half);
+  if (!rc) rc = cross_map_k(&v, P, P.Sk > 0 ? P.v : P.q, half);
+  if (rc) return rc;
+  const int sms = cross_sms();
+  auto kq = cross_dq_kernel<T, DP, BIAS>;
+  auto kkv = cross_dkv_kernel<T, DP, BIAS>;
+  cudaError_t e = cudaFuncSetAttribute(kq, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kkv, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  if (e != cudaSuccess) return cuda_fail(e, "cross_attention_backward shared memory");
+  if (P.Sq > 0) {
+    const int64_t n = static_cast<int64_t>(P.q_tiles) * P.splits * P.Hkv * P.B, rows = static_cast<int64_t>(P.B) * P.Hq * P.Sq;
+    kq<<<static_cast<int>(n < sms ? n : sms), 512, C::SMEM, st>>>(q, g, k, v, P);
+    rc = check_launch("cross_dq_kernel");
+    if (!rc && P.splits > 1) rc = join_launch<T>(P.part_dq, rows * P.D, P.splits, rows, P.D, P.Sq, P.Hq, P.dq, st);
+    if (rc) return rc;
+  }
+  if (P.Sk > 0) {
+    const int64_t n = P.Skp / CT * P.kv_splits * P.Hkv * P.B, rows = static_cast<int64_t>(P.B) * P.Hkv * P.Sk;
+    kkv<<<static_cast<int>(n < sms ? n : sms), 512, C::SMEM, st>>>(q, g, k, v, P);
+    rc = check_launch("cross_dkv_kernel");
+    if (!rc && P.kv_splits > 1) {
+      rc = join_launch<T>(P.part_dk, 2 * rows * P.D, P.kv_splits, rows, P.D, P.Sk, P.Hkv, P.dk, st);
+      if (!rc) rc = join_launch<T>(P.part_dk + rows * P.D, 2 * rows * P.D, P.kv_splits, rows, P.D, P.Sk, P.Hkv, P.dv, st);
+    }
+  }
+  return rc;
+}
+
+template <typename T>
+static int bwd_launch(const CrossParams& P, cudaStream_t st) {
+  if (P.D <= 64) return P.bias2 ? bwd_launch_cfg<T, 64, true>(P, st) : bwd_launch_cfg<T, 64, false>(P, st);
+  return P.bias2 ? bwd_launch_cfg<T, 128, true>(P, st) : bwd_launch_cfg<T, 128, false>(P, st);
+}
+
+}  // namespace h3b

@@ -26,14 +26,18 @@ constexpr float CA_LOG2E = 1.4426950408889634f, CA_LN2 = 0.6931471805599453f;
 struct CrossParams {
   h3b_attn_tensor q, k, v, o, go, dq, dk, dv;
   float* lse;              // [B, Hq, Sq]
-  float* delta;            // [B, Hq, Sq]
   const int32_t* kv_lens;  // [B] keys in use, or null: all
   const float* bias2;      // [B, Skp] what is added to the scores, in units of log2; or null
   float* part_o;           // [splits, B * Hq * Sq, D] partial outputs, each normalised by its own sum
   float* part_lse;         // [splits, B * Hq * Sq] their log-sum-exps in units of log2
+  float* stats;            // backward: [B, Hkv, q_tiles][-lse log2(e), delta][128 tile rows]
+  float* part_dq;          // [splits, B * Hq * Sq, D] partial dQ
+  float* part_dk;          // [kv_splits][dK, dV][B * Hkv * Sk, D] partial dK and dV
   int64_t Sq, Sk, Skp;
   int B, Hq, Hkv, G, D, nq;  // nq: queries of a tile
-  int q_tiles, units, splits;  // query tiles; work units (pairs of tiles) per key head; key splits of a unit
+  int q_tiles, units;  // query tiles; pairs of them
+  int splits;          // key splits of a unit (forward, dQ)
+  int kv_splits;       // query splits of a unit (dK, dV)
   float scale, scale2;         // scale2 = scale log2(e)
 };
 
@@ -63,9 +67,9 @@ __device__ __forceinline__ void tma_store_5d(const void* src, const CUtensorMap*
                "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
                : "memory");
 }
-__device__ __forceinline__ void tma_store_4d(const void* src, const CUtensorMap* map, int c0, int c1, int c2, int c3) {
-  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(map),
-               "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
                : "memory");
 }
 __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
