@@ -352,7 +352,10 @@ __global__ void __launch_bounds__(512, 1)
       if (lane == 0) {
         // -------------------------------------------------------------------------------------- MMA issue
         constexpr uint32_t idS = idesc_f16<T>(CT, CT, false), idD = idesc_f16<T>(CT, DP, true);
-        const uint32_t aQ = smem_u32(sQ), aG = smem_u32(sG), aK = smem_u32(sK), aV = smem_u32(sV);
+        constexpr uint64_t TILE16 = C::TILE >> 4;
+        const uint64_t rQ = desc_rows(smem_u32(sQ)), rG = desc_rows(smem_u32(sG)), rK = desc_rows(smem_u32(sK)),
+                       rV = desc_rows(smem_u32(sV));
+        const uint64_t cK = desc_chan(smem_u32(sK));
         BwdWalk<true> ws(P), wp(P), wd(P);  // the next S, dP and dQ product
         int sk = 0, pv = 0, dk = 0;
         uint32_t skph = 0, pvph = 0, qph = 0, gph = 0, dsph = 0, dqph = 1, sbuf = 0, dbuf = 0;
@@ -366,8 +369,7 @@ __global__ void __launch_bounds__(512, 1)
             qph ^= 1;
           }
           tc_fence_after();
-          for (int kk = 0; kk < DP / 16; ++kk)
-            mma_f16_ss(tmem + sbuf * CT, desc_rows(aQ, kk), desc_rows(aK + sk * C::TILE, kk), idS, kk > 0);
+          mma_rows<DP / 16>(tmem + sbuf * CT, rQ, rK + sk * TILE16, idS);
           mma_commit(&s_full[sbuf]);
           if (ws.c.last()) mma_commit(q_empty);
           sbuf ^= 1;
@@ -382,7 +384,7 @@ __global__ void __launch_bounds__(512, 1)
             gph ^= 1;
           }
           tc_fence_after();
-          for (int kk = 0; kk < DP / 16; ++kk) mma_f16_ss(tDP, desc_rows(aG, kk), desc_rows(aV + pv * C::TILE, kk), idS, kk > 0);
+          mma_rows<DP / 16>(tDP, rG, rV + pv * TILE16, idS);
           mma_commit(dp_full);
           mma_commit(&v_empty[pv]);
           if (wp.c.last()) mma_commit(g_empty);
@@ -403,9 +405,7 @@ __global__ void __launch_bounds__(512, 1)
             dqph ^= 1;
           }
           tc_fence_after();
-          for (int kk = 0; kk < CT / 16; ++kk)
-            mma_f16_ts(tDQ, tmem + dbuf * CT + (kk >> 2) * 64 + (kk & 3) * 8, desc_chan(aK + dk * C::TILE, kk), idD,
-                       !wd.c.first() || kk > 0);
+          mma_chan<true>(tDQ, tmem + dbuf * CT, cK + dk * TILE16, idD, !wd.c.first());
           mma_commit(&k_empty[dk]);
           if (wd.c.last()) mma_commit(dq_full);
           dbuf ^= 1;
@@ -714,7 +714,10 @@ __global__ void __launch_bounds__(512, 1)
       if (lane == 0) {
         // -------------------------------------------------------------------------------------- MMA issue
         constexpr uint32_t idS = idesc_f16<T>(CT, CT, false), idD = idesc_f16<T>(CT, DP, true);
-        const uint32_t aQ = smem_u32(sQ), aG = smem_u32(sG), aK = smem_u32(sK), aV = smem_u32(sV);
+        constexpr uint64_t TILE16 = C::TILE >> 4;
+        const uint64_t rQ = desc_rows(smem_u32(sQ)), rG = desc_rows(smem_u32(sG)), rK = desc_rows(smem_u32(sK)),
+                       rV = desc_rows(smem_u32(sV));
+        const uint64_t cQ = desc_chan(smem_u32(sQ)), cG = desc_chan(smem_u32(sG));
         BwdWalk<false> ws(P), wp(P), wd(P);  // the next S^T, dP^T, and the tile in hand
         int sq = 0, pg = 0, dq = 0, dg = 0;
         uint32_t sqph = 0, pgph = 0, kph = 0, vph = 0, ph = 0, aph = 1;
@@ -727,7 +730,7 @@ __global__ void __launch_bounds__(512, 1)
           }
           if (!(ok = mbar_wait(&q_full[sq], sqph, abort_flag))) return;
           tc_fence_after();
-          for (int kk = 0; kk < DP / 16; ++kk) mma_f16_ss(tmem, desc_rows(aK, kk), desc_rows(aQ + sq * C::TILE, kk), idS, kk > 0);
+          mma_rows<DP / 16>(tmem, rK, rQ + sq * TILE16, idS);
           mma_commit(s_full);
           if (ws.c.last()) mma_commit(k_empty);
           if (++sq == QS) sq = 0, sqph ^= 1;
@@ -741,7 +744,7 @@ __global__ void __launch_bounds__(512, 1)
           }
           if (!(ok = mbar_wait(&g_full[pg], pgph, abort_flag))) return;
           tc_fence_after();
-          for (int kk = 0; kk < DP / 16; ++kk) mma_f16_ss(tDP, desc_rows(aV, kk), desc_rows(aG + pg * C::TILE, kk), idS, kk > 0);
+          mma_rows<DP / 16>(tDP, rV, rG + pg * TILE16, idS);
           mma_commit(dp_full);
           if (wp.c.last()) mma_commit(v_empty);
           if (++pg == GS) pg = 0, pgph ^= 1;
@@ -758,15 +761,13 @@ __global__ void __launch_bounds__(512, 1)
             aph ^= 1;
           }
           tc_fence_after();
-          for (int kk = 0; kk < CT / 16; ++kk)
-            mma_f16_ts(tDV, tmem + (kk >> 2) * 64 + (kk & 3) * 8, desc_chan(aG + dg * C::TILE, kk), idD, acc || kk > 0);
+          mma_chan<true>(tDV, tmem, cG + dg * TILE16, idD, acc);
           mma_commit(&g_empty[dg]);
           if (++dg == GS) dg = 0;
           do_s();
           if (!ok || !(ok = mbar_wait(ds_full, ph, abort_flag))) break;
           tc_fence_after();
-          for (int kk = 0; kk < CT / 16; ++kk)
-            mma_f16_ts(tDK, tDP + (kk >> 2) * 64 + (kk & 3) * 8, desc_chan(aQ + dq * C::TILE, kk), idD, acc || kk > 0);
+          mma_chan<true>(tDK, tDP, cQ + dq * TILE16, idD, acc);
           mma_commit(&q_empty[dq]);
           if (last) mma_commit(acc_full);
           if (++dq == QS) dq = 0;

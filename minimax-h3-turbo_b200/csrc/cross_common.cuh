@@ -118,17 +118,29 @@ __host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool b_mn) {
 }
 // A tile of shared memory: 128 rows, DP channels, in parts of 64 channels (128 rows x 128 bytes, 128-byte swizzle).
 constexpr uint32_t SUB_BYTES = CT * 128;
-// descriptor of 16 channels (step kk) of a tile whose rows are the operand's M or N index (K-major)
-__device__ __forceinline__ uint64_t desc_rows(uint32_t tile, int kk) {
-  return smem_desc_sw128(tile + (kk >> 2) * SUB_BYTES + (kk & 3) * 32);
+// Descriptor of a tile whose rows are the operand's M or N index (K-major); step kk (16 channels) adds rows_step(kk).
+// Offsets are in units of 16 bytes and stay inside the 14-bit address field (shared memory is under 256 KB).
+__device__ __forceinline__ uint64_t desc_rows(uint32_t tile) { return smem_desc_sw128(tile); }
+__host__ __device__ constexpr uint64_t rows_step(int kk) { return ((kk >> 2) * SUB_BYTES + (kk & 3) * 32) >> 4; }
+// Descriptor of a tile whose channels are the operand's N index and whose rows are K (MN-major): 64-channel parts
+// SUB_BYTES apart (leading offset), groups of 8 rows 1024 bytes apart (stride offset); step kk (16 rows) adds chan_step(kk).
+__device__ __forceinline__ uint64_t desc_chan(uint32_t tile) {
+  return (smem_desc_sw128(tile) & ~(uint64_t(0x3FFF) << 16)) | (static_cast<uint64_t>(SUB_BYTES >> 4) << 16);
 }
-// descriptor of 16 rows (step kk) of a tile whose channels are the operand's N index and whose rows are K (MN-major):
-// 64-channel parts SUB_BYTES apart (leading offset), groups of 8 rows 1024 bytes apart (stride offset)
-__device__ __forceinline__ uint64_t desc_chan(uint32_t tile, int kk) {
-  uint64_t d = smem_desc_sw128(tile + kk * 2048);
-  d &= ~(uint64_t(0x3FFF) << 16);
-  d |= static_cast<uint64_t>(SUB_BYTES >> 4) << 16;
-  return d;
+__host__ __device__ constexpr uint64_t chan_step(int kk) { return (kk * 2048) >> 4; }
+// the products of one tile, in steps of 16: D (+)= A B^T with A and B K-major in shared memory
+template <int STEPS>
+__device__ __forceinline__ void mma_rows(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+#pragma unroll
+  for (int kk = 0; kk < STEPS; ++kk) mma_f16_ss(d, a + rows_step(kk), b + rows_step(kk), idesc, kk > 0);
+}
+// D (+)= A B with A [128 rows x 128] in tensor memory and B's 128 rows in shared memory.  HALVES: the columns of each half
+// of A start 64 columns apart (its halves were written over the scores that two groups of warps read)
+template <bool HALVES>
+__device__ __forceinline__ void mma_chan(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+#pragma unroll
+  for (int kk = 0; kk < CT / 16; ++kk)
+    mma_f16_ts(d, a + (HALVES ? (kk >> 2) * 64 + (kk & 3) * 8 : kk * 8), b + chan_step(kk), idesc, acc | (kk > 0));
 }
 
 template <typename T>

@@ -323,15 +323,15 @@ __global__ void __launch_bounds__(512, 1)
       if (lane == 0) {
         // -------------------------------------------------------------------------------------- MMA issue
         constexpr uint32_t idQK = idesc_f16<T>(CT, CT, false), idPV = idesc_f16<T>(CT, DP, true);
-        const uint32_t aQ = smem_u32(sQ), aKV = smem_u32(sKV);
+        constexpr uint64_t TILE16 = C::TILE >> 4;
+        const uint64_t dQ = desc_rows(smem_u32(sQ)), dK = desc_rows(smem_u32(sKV)), dV = desc_chan(smem_u32(sKV));
         int st = 0;
         uint32_t kph = 0, qph[2] = {0, 0}, pph[2] = {0, 0}, oph[2] = {1, 1};
         auto step = [&] {
           if (++st == C::STAGES) st = 0, kph ^= 1;
         };
         auto qk = [&](int slot, int kst) {
-          for (int kk = 0; kk < DP / 16; ++kk)
-            mma_f16_ss(tmem + slot * CT, desc_rows(aQ + slot * C::TILE, kk), desc_rows(aKV + kst * C::TILE, kk), idQK, kk > 0);
+          mma_rows<DP / 16>(tmem + slot * CT, dQ + slot * TILE16, dK + kst * TILE16, idQK);
           mma_commit(&s_full[slot]);
         };
         FwdUnit cur, nxt;
@@ -372,9 +372,7 @@ __global__ void __launch_bounds__(512, 1)
                   oph[s] ^= 1;
                 }
                 tc_fence_after();
-                for (int kk = 0; kk < CT / 16; ++kk)
-                  mma_f16_ts(tmem + 2 * CT + s * CT, tmem + s * CT + kk * 8, desc_chan(aKV + vst * C::TILE, kk), idPV,
-                             t > cur.t0 || kk > 0);
+                mma_chan<false>(tmem + 2 * CT + s * CT, tmem + s * CT, dV + vst * TILE16, idPV, t > cur.t0);
                 if (last) mma_commit(&o_full[s]);
               }
               if (then_qk && (s == 0 || (last ? nxt.two : cur.two))) {
