@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(512, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const bool masked = BIAS || P.kv_lens != nullptr;
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
@@ -349,73 +349,70 @@ __global__ void __launch_bounds__(512, 1)
   } else {
     regs_dec<64>();
     if (warp == 12) {
-      if (lane == 0) {
-        // -------------------------------------------------------------------------------------- MMA issue
-        constexpr uint32_t idS = idesc_f16<T>(CT, CT, false), idD = idesc_f16<T>(CT, DP, true);
-        constexpr uint64_t TILE16 = C::TILE >> 4;
-        const uint64_t rQ = desc_rows(smem_u32(sQ)), rG = desc_rows(smem_u32(sG)), rK = desc_rows(smem_u32(sK)),
-                       rV = desc_rows(smem_u32(sV));
-        const uint64_t cK = desc_chan(smem_u32(sK));
-        BwdWalk<true> ws(P), wp(P), wd(P);  // the next S, dP and dQ product
-        int sk = 0, pv = 0, dk = 0;
-        uint32_t skph = 0, pvph = 0, qph = 0, gph = 0, dsph = 0, dqph = 1, sbuf = 0, dbuf = 0;
-        bool ok = true;
-        auto do_s = [&] {
-          if (!ok || !ws.valid) return;
-          if (!(ok = mbar_wait(&k_full[sk], skph, abort_flag))) return;
-          if (masked && !(ok = mbar_wait(&k_clean[sk], skph, abort_flag))) return;
-          if (ws.c.first()) {
-            if (!(ok = mbar_wait(q_full, qph, abort_flag))) return;
-            qph ^= 1;
-          }
-          tc_fence_after();
-          mma_rows<DP / 16>(tmem + sbuf * CT, rQ, rK + sk * TILE16, idS);
-          mma_commit(&s_full[sbuf]);
-          if (ws.c.last()) mma_commit(q_empty);
-          sbuf ^= 1;
-          if (++sk == KS) sk = 0, skph ^= 1;
-          ws.next();
-        };
-        auto do_dp = [&] {
-          if (!ok || !wp.valid) return;
-          if (!(ok = mbar_wait(&v_full[pv], pvph, abort_flag))) return;
-          if (wp.c.first()) {
-            if (!(ok = mbar_wait(g_full, gph, abort_flag))) return;
-            gph ^= 1;
-          }
-          tc_fence_after();
-          mma_rows<DP / 16>(tDP, rG, rV + pv * TILE16, idS);
-          mma_commit(dp_full);
-          mma_commit(&v_empty[pv]);
-          if (wp.c.last()) mma_commit(g_empty);
-          if (++pv == VS) pv = 0, pvph ^= 1;
-          wp.next();
-        };
-        do_s();
-        do_dp();
-        do_s();
-        while (ok && wd.valid) {
-          if (!(ok = mbar_wait(ds_full, dsph, abort_flag))) break;  // dS is written, dP has been read
-          dsph ^= 1;
-          const bool same = wp.valid && wp.c.it == wd.c.it;
-          if (same) do_dp();  // a new unit's dP waits for its G tile: not before this unit's last product
-          if (!ok) break;
-          if (wd.c.first()) {
-            if (!(ok = mbar_wait(dq_empty, dqph, abort_flag))) break;
-            dqph ^= 1;
-          }
-          tc_fence_after();
-          mma_chan<true>(tDQ, tmem + dbuf * CT, cK + dk * TILE16, idD, !wd.c.first());
-          mma_commit(&k_empty[dk]);
-          if (wd.c.last()) mma_commit(dq_full);
-          dbuf ^= 1;
-          if (++dk == KS) dk = 0;
-          wd.next();
-          if (!same) do_dp();
-          do_s();
+      // -------------------------------------------------------------------------------------- MMA issue
+      constexpr uint32_t idS = idesc_f16<T>(CT, CT, false), idD = idesc_f16<T>(CT, DP, true);
+      constexpr uint64_t TILE16 = C::TILE >> 4;
+      const uint64_t rQ = desc_rows(smem_u32(sQ)), rG = desc_rows(smem_u32(sG)), rK = desc_rows(smem_u32(sK)),
+                     rV = desc_rows(smem_u32(sV));
+      const uint64_t cK = desc_chan(smem_u32(sK));
+      BwdWalk<true> ws(P), wp(P), wd(P);  // the next S, dP and dQ product
+      int sk = 0, pv = 0, dk = 0;
+      uint32_t skph = 0, pvph = 0, qph = 0, gph = 0, dsph = 0, dqph = 1, sbuf = 0, dbuf = 0;
+      bool ok = true;
+      auto do_s = [&] {
+        if (!ok || !ws.valid) return;
+        if (!(ok = warp_wait(&k_full[sk], skph, abort_flag))) return;
+        if (masked && !(ok = warp_wait(&k_clean[sk], skph, abort_flag))) return;
+        if (ws.c.first()) {
+          if (!(ok = warp_wait(q_full, qph, abort_flag))) return;
+          qph ^= 1;
         }
+        tc_fence_after();
+        mma_rows<DP / 16>(tmem + sbuf * CT, rQ, rK + sk * TILE16, idS);
+        commit_one(&s_full[sbuf]);
+        if (ws.c.last()) commit_one(q_empty);
+        sbuf ^= 1;
+        if (++sk == KS) sk = 0, skph ^= 1;
+        ws.next();
+      };
+      auto do_dp = [&] {
+        if (!ok || !wp.valid) return;
+        if (!(ok = warp_wait(&v_full[pv], pvph, abort_flag))) return;
+        if (wp.c.first()) {
+          if (!(ok = warp_wait(g_full, gph, abort_flag))) return;
+          gph ^= 1;
+        }
+        tc_fence_after();
+        mma_rows<DP / 16>(tDP, rG, rV + pv * TILE16, idS);
+        commit_one(dp_full);
+        commit_one(&v_empty[pv]);
+        if (wp.c.last()) commit_one(g_empty);
+        if (++pv == VS) pv = 0, pvph ^= 1;
+        wp.next();
+      };
+      do_s();
+      do_dp();
+      do_s();
+      while (ok && wd.valid) {
+        if (!(ok = warp_wait(ds_full, dsph, abort_flag))) break;  // dS is written, dP has been read
+        dsph ^= 1;
+        const bool same = wp.valid && wp.c.it == wd.c.it;
+        if (same) do_dp();  // a new unit's dP waits for its G tile: not before this unit's last product
+        if (!ok) break;
+        if (wd.c.first()) {
+          if (!(ok = warp_wait(dq_empty, dqph, abort_flag))) break;
+          dqph ^= 1;
+        }
+        tc_fence_after();
+        mma_chan<true>(tDQ, tmem + dbuf * CT, cK + dk * TILE16, idD, !wd.c.first());
+        commit_one(&k_empty[dk]);
+        if (wd.c.last()) commit_one(dq_full);
+        dbuf ^= 1;
+        if (++dk == KS) dk = 0;
+        wd.next();
+        if (!same) do_dp();
+        do_s();
       }
-      __syncwarp();
     } else if (warp == 13) {
       if (lane == 0) {
         // -------------------------------------------------------------------------------------- copies
@@ -492,10 +489,8 @@ __global__ void __launch_bounds__(512, 1)
   __syncthreads();
   if (warp == 12) {
     tc_fence_after();
-    if (lane == 0) {
-      mma_commit(done);
-      mbar_wait_drain(done, 0);
-    }
+    commit_one(done);
+    mbar_wait_drain(done, 0);
     __syncwarp();
     tmem_dealloc(tmem, C::TMEM_COLS);
   }
@@ -534,7 +529,7 @@ __global__ void __launch_bounds__(512, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     mbar_init(k_full, 1);
     mbar_init(k_empty, 1);
@@ -711,72 +706,69 @@ __global__ void __launch_bounds__(512, 1)
   } else {
     regs_dec<64>();
     if (warp == 12) {
-      if (lane == 0) {
-        // -------------------------------------------------------------------------------------- MMA issue
-        constexpr uint32_t idS = idesc_f16<T>(CT, CT, false), idD = idesc_f16<T>(CT, DP, true);
-        constexpr uint64_t TILE16 = C::TILE >> 4;
-        const uint64_t rQ = desc_rows(smem_u32(sQ)), rG = desc_rows(smem_u32(sG)), rK = desc_rows(smem_u32(sK)),
-                       rV = desc_rows(smem_u32(sV));
-        const uint64_t cQ = desc_chan(smem_u32(sQ)), cG = desc_chan(smem_u32(sG));
-        BwdWalk<false> ws(P), wp(P), wd(P);  // the next S^T, dP^T, and the tile in hand
-        int sq = 0, pg = 0, dq = 0, dg = 0;
-        uint32_t sqph = 0, pgph = 0, kph = 0, vph = 0, ph = 0, aph = 1;
-        bool ok = true;
-        auto do_s = [&] {
-          if (!ok || !ws.valid) return;
-          if (ws.c.first()) {
-            if (!(ok = mbar_wait(k_full, kph, abort_flag))) return;
-            kph ^= 1;
-          }
-          if (!(ok = mbar_wait(&q_full[sq], sqph, abort_flag))) return;
-          tc_fence_after();
-          mma_rows<DP / 16>(tmem, rK, rQ + sq * TILE16, idS);
-          mma_commit(s_full);
-          if (ws.c.last()) mma_commit(k_empty);
-          if (++sq == QS) sq = 0, sqph ^= 1;
-          ws.next();
-        };
-        auto do_dp = [&] {
-          if (!ok || !wp.valid) return;
-          if (wp.c.first()) {
-            if (!(ok = mbar_wait(v_full, vph, abort_flag))) return;
-            vph ^= 1;
-          }
-          if (!(ok = mbar_wait(&g_full[pg], pgph, abort_flag))) return;
-          tc_fence_after();
-          mma_rows<DP / 16>(tDP, rV, rG + pg * TILE16, idS);
-          mma_commit(dp_full);
-          if (wp.c.last()) mma_commit(v_empty);
-          if (++pg == GS) pg = 0, pgph ^= 1;
-          wp.next();
-        };
-        do_s();
-        do_dp();
-        while (ok && wd.valid) {
-          const uint32_t acc = !wd.c.first();
-          const bool last = wd.c.last();
-          if (!(ok = mbar_wait(p_full, ph, abort_flag))) break;
-          if (!acc) {
-            if (!(ok = mbar_wait(acc_empty, aph, abort_flag))) break;
-            aph ^= 1;
-          }
-          tc_fence_after();
-          mma_chan<true>(tDV, tmem, cG + dg * TILE16, idD, acc);
-          mma_commit(&g_empty[dg]);
-          if (++dg == GS) dg = 0;
-          do_s();
-          if (!ok || !(ok = mbar_wait(ds_full, ph, abort_flag))) break;
-          tc_fence_after();
-          mma_chan<true>(tDK, tDP, cQ + dq * TILE16, idD, acc);
-          mma_commit(&q_empty[dq]);
-          if (last) mma_commit(acc_full);
-          if (++dq == QS) dq = 0;
-          do_dp();
-          ph ^= 1;
-          wd.next();
+      // -------------------------------------------------------------------------------------- MMA issue
+      constexpr uint32_t idS = idesc_f16<T>(CT, CT, false), idD = idesc_f16<T>(CT, DP, true);
+      constexpr uint64_t TILE16 = C::TILE >> 4;
+      const uint64_t rQ = desc_rows(smem_u32(sQ)), rG = desc_rows(smem_u32(sG)), rK = desc_rows(smem_u32(sK)),
+                     rV = desc_rows(smem_u32(sV));
+      const uint64_t cQ = desc_chan(smem_u32(sQ)), cG = desc_chan(smem_u32(sG));
+      BwdWalk<false> ws(P), wp(P), wd(P);  // the next S^T, dP^T, and the tile in hand
+      int sq = 0, pg = 0, dq = 0, dg = 0;
+      uint32_t sqph = 0, pgph = 0, kph = 0, vph = 0, ph = 0, aph = 1;
+      bool ok = true;
+      auto do_s = [&] {
+        if (!ok || !ws.valid) return;
+        if (ws.c.first()) {
+          if (!(ok = warp_wait(k_full, kph, abort_flag))) return;
+          kph ^= 1;
         }
+        if (!(ok = warp_wait(&q_full[sq], sqph, abort_flag))) return;
+        tc_fence_after();
+        mma_rows<DP / 16>(tmem, rK, rQ + sq * TILE16, idS);
+        commit_one(s_full);
+        if (ws.c.last()) commit_one(k_empty);
+        if (++sq == QS) sq = 0, sqph ^= 1;
+        ws.next();
+      };
+      auto do_dp = [&] {
+        if (!ok || !wp.valid) return;
+        if (wp.c.first()) {
+          if (!(ok = warp_wait(v_full, vph, abort_flag))) return;
+          vph ^= 1;
+        }
+        if (!(ok = warp_wait(&g_full[pg], pgph, abort_flag))) return;
+        tc_fence_after();
+        mma_rows<DP / 16>(tDP, rV, rG + pg * TILE16, idS);
+        commit_one(dp_full);
+        if (wp.c.last()) commit_one(v_empty);
+        if (++pg == GS) pg = 0, pgph ^= 1;
+        wp.next();
+      };
+      do_s();
+      do_dp();
+      while (ok && wd.valid) {
+        const uint32_t acc = !wd.c.first();
+        const bool last = wd.c.last();
+        if (!(ok = warp_wait(p_full, ph, abort_flag))) break;
+        if (!acc) {
+          if (!(ok = warp_wait(acc_empty, aph, abort_flag))) break;
+          aph ^= 1;
+        }
+        tc_fence_after();
+        mma_chan<true>(tDV, tmem, cG + dg * TILE16, idD, acc);
+        commit_one(&g_empty[dg]);
+        if (++dg == GS) dg = 0;
+        do_s();
+        if (!ok || !(ok = warp_wait(ds_full, ph, abort_flag))) break;
+        tc_fence_after();
+        mma_chan<true>(tDK, tDP, cQ + dq * TILE16, idD, acc);
+        commit_one(&q_empty[dq]);
+        if (last) commit_one(acc_full);
+        if (++dq == QS) dq = 0;
+        do_dp();
+        ph ^= 1;
+        wd.next();
       }
-      __syncwarp();
     } else if (warp == 13) {
       if (lane == 0) {
         // -------------------------------------------------------------------------------------- copies
@@ -833,10 +825,8 @@ __global__ void __launch_bounds__(512, 1)
   __syncthreads();
   if (warp == 12) {
     tc_fence_after();
-    if (lane == 0) {
-      mma_commit(done);
-      mbar_wait_drain(done, 0);
-    }
+    commit_one(done);
+    mbar_wait_drain(done, 0);
     __syncwarp();
     tmem_dealloc(tmem, C::TMEM_COLS);
   }

@@ -108,6 +108,18 @@ __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// One lane of a converged warp, the same one every time.  The MMA warp runs its loop as a whole and elects a lane only around
+// the tcgen05 instructions: what they take from registers stays warp-uniform.  (With the loop inside `if (lane == 0)` every
+// operand of every product was moved to a uniform register by itself: 67 cycles a product, and 4550 instead of ~3200 cycles
+// for two query tiles x one key tile of the forward kernel.)
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+__device__ __forceinline__ void commit_one(uint64_t* bar) {
+  if (elect_one()) mma_commit(bar);
+}
 // Instruction descriptor of tcgen05.mma kind::f16: A and B of one type, fp32 accumulator, M x N tile, A K-major,
 // B K-major or (b_mn) with its N index contiguous.
 template <typename T>
@@ -131,16 +143,18 @@ __host__ __device__ constexpr uint64_t chan_step(int kk) { return (kk * 2048) >>
 // the products of one tile, in steps of 16: D (+)= A B^T with A and B K-major in shared memory
 template <int STEPS>
 __device__ __forceinline__ void mma_rows(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+  if (elect_one())
 #pragma unroll
-  for (int kk = 0; kk < STEPS; ++kk) mma_f16_ss(d, a + rows_step(kk), b + rows_step(kk), idesc, kk > 0);
+    for (int kk = 0; kk < STEPS; ++kk) mma_f16_ss(d, a + rows_step(kk), b + rows_step(kk), idesc, kk > 0);
 }
 // D (+)= A B with A [128 rows x 128] in tensor memory and B's 128 rows in shared memory.  HALVES: the columns of each half
 // of A start 64 columns apart (its halves were written over the scores that two groups of warps read)
 template <bool HALVES>
 __device__ __forceinline__ void mma_chan(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  if (elect_one())
 #pragma unroll
-  for (int kk = 0; kk < CT / 16; ++kk)
-    mma_f16_ts(d, a + (HALVES ? (kk >> 2) * 64 + (kk & 3) * 8 : kk * 8), b + chan_step(kk), idesc, acc | (kk > 0));
+    for (int kk = 0; kk < CT / 16; ++kk)
+      mma_f16_ts(d, a + (HALVES ? (kk >> 2) * 64 + (kk & 3) * 8 : kk * 8), b + chan_step(kk), idesc, acc | (kk > 0));
 }
 
 template <typename T>

@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(512, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int64_t n_items = static_cast<int64_t>(P.units) * P.splits * P.Hkv * P.B;
   // with any mask every V tile passes warp 14 (in step with the ring: a phase it skipped could be taken for another)
   const bool masked = BIAS || P.kv_lens != nullptr;
@@ -320,81 +320,78 @@ __global__ void __launch_bounds__(512, 1)
   } else {
     regs_dec<64>();
     if (warp == 12) {
-      if (lane == 0) {
-        // -------------------------------------------------------------------------------------- MMA issue
-        constexpr uint32_t idQK = idesc_f16<T>(CT, CT, false), idPV = idesc_f16<T>(CT, DP, true);
-        constexpr uint64_t TILE16 = C::TILE >> 4;
-        const uint64_t dQ = desc_rows(smem_u32(sQ)), dK = desc_rows(smem_u32(sKV)), dV = desc_chan(smem_u32(sKV));
-        int st = 0;
-        uint32_t kph = 0, qph[2] = {0, 0}, pph[2] = {0, 0}, oph[2] = {1, 1};
-        auto step = [&] {
-          if (++st == C::STAGES) st = 0, kph ^= 1;
-        };
-        auto qk = [&](int slot, int kst) {
-          mma_rows<DP / 16>(tmem + slot * CT, dQ + slot * TILE16, dK + kst * TILE16, idQK);
-          mma_commit(&s_full[slot]);
-        };
-        FwdUnit cur, nxt;
-        int64_t it = blockIdx.x;
-        bool have = fwd_next(P, it, n_items, cur), ok = true;
-        if (have) {
-          ok = mbar_wait(&kv_full[st], kph, abort_flag);
-          for (int s = 0; ok && s < (cur.two ? 2 : 1); ++s) {
-            ok = mbar_wait(&q_full[s], qph[s], abort_flag);
-            qph[s] ^= 1;
-            if (!ok) break;
-            tc_fence_after();
-            qk(s, st);
-            if (cur.t1 - cur.t0 == 1) mma_commit(&q_empty[s]);
-          }
-          mma_commit(&kv_empty[st]);
-          step();
+      // -------------------------------------------------------------------------------------- MMA issue
+      constexpr uint32_t idQK = idesc_f16<T>(CT, CT, false), idPV = idesc_f16<T>(CT, DP, true);
+      constexpr uint64_t TILE16 = C::TILE >> 4;
+      const uint64_t dQ = desc_rows(smem_u32(sQ)), dK = desc_rows(smem_u32(sKV)), dV = desc_chan(smem_u32(sKV));
+      int st = 0;
+      uint32_t kph = 0, qph[2] = {0, 0}, pph[2] = {0, 0}, oph[2] = {1, 1};
+      auto step = [&] {
+        if (++st == C::STAGES) st = 0, kph ^= 1;
+      };
+      auto qk = [&](int slot, int kst) {
+        mma_rows<DP / 16>(tmem + slot * CT, dQ + slot * TILE16, dK + kst * TILE16, idQK);
+        commit_one(&s_full[slot]);
+      };
+      FwdUnit cur, nxt;
+      int64_t it = blockIdx.x;
+      bool have = fwd_next(P, it, n_items, cur), ok = true;
+      if (have) {
+        ok = warp_wait(&kv_full[st], kph, abort_flag);
+        for (int s = 0; ok && s < (cur.two ? 2 : 1); ++s) {
+          ok = warp_wait(&q_full[s], qph[s], abort_flag);
+          qph[s] ^= 1;
+          if (!ok) break;
+          tc_fence_after();
+          qk(s, st);
+          if (cur.t1 - cur.t0 == 1) commit_one(&q_empty[s]);
         }
-        while (have && ok) {
-          bool more = false;
-          for (int t = cur.t0; ok && t < cur.t1; ++t) {
-            const bool last = t == cur.t1 - 1;
-            if (last) more = fwd_next(P, it, n_items, nxt);
-            const int vst = st;
-            if (!(ok = mbar_wait(&kv_full[vst], kph, abort_flag))) break;
-            if (masked && !(ok = mbar_wait(&v_clean[vst], kph, abort_flag))) break;
-            step();
-            const bool then_qk = !last || more;
-            const int kst = st;
-            const uint32_t kparity = kph;
-            if (then_qk) step();
-            for (int s = 0; ok && s < 2; ++s) {
-              if (s == 0 || cur.two) {
-                if (!(ok = mbar_wait(&p_full[s], pph[s], abort_flag))) break;
-                pph[s] ^= 1;
-                if (t == cur.t0) {
-                  if (!(ok = mbar_wait(&o_empty[s], oph[s], abort_flag))) break;
-                  oph[s] ^= 1;
-                }
-                tc_fence_after();
-                mma_chan<false>(tmem + 2 * CT + s * CT, tmem + s * CT, dV + vst * TILE16, idPV, t > cur.t0);
-                if (last) mma_commit(&o_full[s]);
-              }
-              if (then_qk && (s == 0 || (last ? nxt.two : cur.two))) {
-                if (!(ok = mbar_wait(&kv_full[kst], kparity, abort_flag))) break;
-                if (last) {
-                  if (!(ok = mbar_wait(&q_full[s], qph[s], abort_flag))) break;
-                  qph[s] ^= 1;
-                }
-                tc_fence_after();
-                qk(s, kst);
-                if (last ? nxt.t1 - nxt.t0 == 1 : t + 2 == cur.t1) mma_commit(&q_empty[s]);
-              }
-            }
-            if (!ok) break;
-            mma_commit(&kv_empty[vst]);
-            if (then_qk) mma_commit(&kv_empty[kst]);
-          }
-          cur = nxt;
-          have = more;
-        }
+        commit_one(&kv_empty[st]);
+        step();
       }
-      __syncwarp();
+      while (have && ok) {
+        bool more = false;
+        for (int t = cur.t0; ok && t < cur.t1; ++t) {
+          const bool last = t == cur.t1 - 1;
+          if (last) more = fwd_next(P, it, n_items, nxt);
+          const int vst = st;
+          if (!(ok = warp_wait(&kv_full[vst], kph, abort_flag))) break;
+          if (masked && !(ok = warp_wait(&v_clean[vst], kph, abort_flag))) break;
+          step();
+          const bool then_qk = !last || more;
+          const int kst = st;
+          const uint32_t kparity = kph;
+          if (then_qk) step();
+          for (int s = 0; ok && s < 2; ++s) {
+            if (s == 0 || cur.two) {
+              if (!(ok = warp_wait(&p_full[s], pph[s], abort_flag))) break;
+              pph[s] ^= 1;
+              if (t == cur.t0) {
+                if (!(ok = warp_wait(&o_empty[s], oph[s], abort_flag))) break;
+                oph[s] ^= 1;
+              }
+              tc_fence_after();
+              mma_chan<false>(tmem + 2 * CT + s * CT, tmem + s * CT, dV + vst * TILE16, idPV, t > cur.t0);
+              if (last) commit_one(&o_full[s]);
+            }
+            if (then_qk && (s == 0 || (last ? nxt.two : cur.two))) {
+              if (!(ok = warp_wait(&kv_full[kst], kparity, abort_flag))) break;
+              if (last) {
+                if (!(ok = warp_wait(&q_full[s], qph[s], abort_flag))) break;
+                qph[s] ^= 1;
+              }
+              tc_fence_after();
+              qk(s, kst);
+              if (last ? nxt.t1 - nxt.t0 == 1 : t + 2 == cur.t1) commit_one(&q_empty[s]);
+            }
+          }
+          if (!ok) break;
+          commit_one(&kv_empty[vst]);
+          if (then_qk) commit_one(&kv_empty[kst]);
+        }
+        cur = nxt;
+        have = more;
+      }
     } else if (warp == 13) {
       if (lane == 0) {
         // -------------------------------------------------------------------------------------- copies
@@ -464,10 +461,8 @@ __global__ void __launch_bounds__(512, 1)
   __syncthreads();
   if (warp == 12) {
     tc_fence_after();
-    if (lane == 0) {  // every product issued (after a wait that gave up some may still run) and its arrivals are over
-      mma_commit(done);
-      mbar_wait_drain(done, 0);
-    }
+    commit_one(done);  // every product issued (after a wait that gave up some may still run) and its arrivals are over
+    mbar_wait_drain(done, 0);
     __syncwarp();
     tmem_dealloc(tmem, C::TMEM_COLS);
   }
