@@ -83,29 +83,6 @@ struct BwdCfg {
   static constexpr uint32_t TMEM_COLS = 512;
 };
 
-// 32 columns of a row of 16-bit results: 16-byte stores (n: valid columns from here on, a multiple of 8)
-template <typename T>
-__device__ __forceinline__ void store_cols(T* dst, const uint32_t (&o)[32], float w, int n) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (8 * i < n) {
-      uint4 v;
-      uint32_t* vv = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        vv[e] = pack2<T>(__uint_as_float(o[8 * i + 2 * e]) * w, __uint_as_float(o[8 * i + 2 * e + 1]) * w);
-      *reinterpret_cast<uint4*>(dst + 8 * i) = v;
-    }
-}
-__device__ __forceinline__ void store_cols_f32(float* dst, const uint32_t (&o)[32], float w, int n) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (4 * i < n)
-      *reinterpret_cast<float4*>(dst + 4 * i) =
-          make_float4(__uint_as_float(o[4 * i]) * w, __uint_as_float(o[4 * i + 1]) * w, __uint_as_float(o[4 * i + 2]) * w,
-                      __uint_as_float(o[4 * i + 3]) * w);
-}
-
 // ------------------------------------------------------------------------------------------------ dQ
 template <typename T, int DP, bool BIAS>
 __global__ void __launch_bounds__(512, 1)

@@ -67,18 +67,17 @@ __device__ __forceinline__ void tma_store_5d(const void* src, const CUtensorMap*
                "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
                : "memory");
 }
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
-               "l"(src), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
-}
 __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void bulk_wait_read() {
   asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
-
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
 // D[tmem] (+)= A B, bf16/fp16 operands, fp32 accumulator; A from shared memory or from tensor memory
 __device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
@@ -92,6 +91,24 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, u
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
       "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// 32 lanes x 16 consecutive 32-bit columns: thread i of the warp gets its lane's 16 columns.
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 // 32 lanes x 32 consecutive 32-bit columns: thread i of the warp writes its lane's 32 columns.
@@ -180,16 +197,92 @@ template <int R>
 __device__ __forceinline__ void regs_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R));
 }
-__device__ __forceinline__ void group_sync(int id, int threads) {
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
 // every lane of the warp waits; one outcome for all (what follows are whole-warp instructions)
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort));
 }
+// Barriers of some warps of a CTA.  They have no bound: every warp of the group reaches each of them whatever its waits on
+// mbarriers came to (after a wait that gave up, a role goes through its loops without waiting).
+__device__ __forceinline__ void group_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ bool group_any(int id, int threads, bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %3, 0;\n\tbar.red.or.pred q, %1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"(threads), "r"(static_cast<uint32_t>(v))
+      : "memory");
+  return r != 0;
+}
 // write 8 packed values (16 bytes, chunk c of 8) of row r into a 64-channel part with the 128-byte swizzle
 __device__ __forceinline__ void put_swizzled(unsigned char* part, int r, int c, uint4 v) {
   *reinterpret_cast<uint4*>(part + r * 128 + ((c ^ (r & 7)) << 4)) = v;
+}
+
+// pairs of fp32 in one 64-bit register: one instruction per two sums or products
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 f2(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void f2_split(f32x2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f32x2 f2_fma(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 f2_add(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// exp2 of two numbers <= 16 on the FMA pipe (the special function unit's 4 results per cycle and scheduler are the bound of
+// softmax loops): x = n + f, |f| <= 1/2 by adding and taking off 1.5 * 2^23; 2^f by a degree-4 polynomial fitted to the least
+// largest relative error (2.6e-6); n into the exponent.  Below 2^-126: 2^-126.
+__device__ __forceinline__ f32x2 f2_exp2(float xa, float xb) {
+  const f32x2 x = f2(fmaxf(xa, -126.f), fmaxf(xb, -126.f));
+  const f32x2 t = f2_add(x, f2(12582912.f, 12582912.f));
+  const f32x2 f = f2_fma(f2_add(t, f2(-12582912.f, -12582912.f)), f2(-1.f, -1.f), x);
+  f32x2 p = f2_fma(f2(0.009570101946812917f, 0.009570101946812917f), f, f2(0.05591786158553334f, 0.05591786158553334f));
+  p = f2_fma(p, f, f2(0.24024744837984488f, 0.24024744837984488f));
+  p = f2_fma(p, f, f2(0.6931218145829676f, 0.6931218145829676f));
+  p = f2_fma(p, f, f2(0.9999992614392343f, 0.9999992614392343f));
+  float ta, tb, pa, pb;
+  f2_split(t, ta, tb);
+  f2_split(p, pa, pb);
+  return f2(__int_as_float(__float_as_int(pa) + (__float_as_int(ta) << 23)),
+            __int_as_float(__float_as_int(pb) + (__float_as_int(tb) << 23)));
+}
+// maximum that keeps a NaN
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 32 columns of a row of 16-bit results: 16-byte stores (n: valid columns from here on, a multiple of 8)
+template <typename T>
+__device__ __forceinline__ void store_cols(T* dst, const uint32_t (&o)[32], float w, int n) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (8 * i < n) {
+      uint4 v;
+      uint32_t* vv = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        vv[e] = pack2<T>(__uint_as_float(o[8 * i + 2 * e]) * w, __uint_as_float(o[8 * i + 2 * e + 1]) * w);
+      *reinterpret_cast<uint4*>(dst + 8 * i) = v;
+    }
+}
+__device__ __forceinline__ void store_cols_f32(float* dst, const uint32_t (&o)[32], float w, int n) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (4 * i < n)
+      *reinterpret_cast<float4*>(dst + 4 * i) =
+          make_float4(__uint_as_float(o[4 * i]) * w, __uint_as_float(o[4 * i + 1]) * w, __uint_as_float(o[4 * i + 2]) * w,
+                      __uint_as_float(o[4 * i + 3]) * w);
 }
 
 // ----------------------------------------------------------------------------------------------- mask preparation

@@ -2,15 +2,18 @@
 //
 // A work unit is a pair of query tiles (slots 0 and 1, 128 rows each) of one key head, over a range of key tiles.  One
 // persistent CTA per SM walks the units; its warps:
-//   0-3, 4-7   softmax of slot 0 and 1: one thread per row.  S (128 fp32 columns of tensor memory) -> registers, running
-//              maximum and sum in fp32, P = exp2(S scale2 - m) rounded to the operand type, back to tensor memory (over S).
-//              m only moves when a tile's maximum exceeds it by 8 (a factor 2^8: far from overflow in fp32 sums and fp16 P);
-//              then the same threads rescale O in tensor memory.  P rounded to 8 (bf16) or 11 (fp16) bits, relative to
-//              each probability: the product's operand type; the sum uses the unrounded values.
-//   8-11       epilogue: O / l to the operand type, through swizzled staging and a bulk tensor store; log-sum-exp
-//   12         MMA issue: S = Q K^T (both from shared memory), O += P V (P from tensor memory, V channel-major)
-//   13         copies: Q tiles, and a ring of K and V tiles, in the order of use
-//   14         zeroes the rows of V tiles whose keys are left out, before their product (0 x NaN would reach the sums)
+//   0-7, 8-15  softmax of slot 0 and 1: two threads per row, 64 scores each.  S (128 fp32 columns of tensor memory) ->
+//              registers, running maximum and sum in fp32, P = exp2(S scale2 - m) rounded to the operand type, back to
+//              tensor memory (over S).  P rounded to 8 (bf16) or 11 (fp16) bits, relative to each probability: the product's
+//              operand type; the sum uses the unrounded values.  m is an exact maximum of the tiles so far, but taken anew
+//              only when a tile exceeds it by more than 8 (a factor 2^8: far from overflow in fp32 sums and fp16 P): P of a
+//              tile is computed with the m at hand, without a pass for the maximum before it, and only such a tile is gone
+//              over again, after its threads have rescaled O in tensor memory.
+//   16-19      epilogue: O / l to the operand type, through swizzled staging and a bulk tensor store; log-sum-exp
+//   20         MMA issue: S = Q K^T (both from shared memory), O += P V (P from tensor memory, V channel-major)
+//   21         copies: Q tiles, and a ring of pairs (V of a key tile, K of the next): what one step of both slots reads,
+//              one barrier each way
+//   22         zeroes the rows of V tiles whose keys are left out, before their product (0 x NaN would reach the sums)
 // Tensor memory: S0 S1 O0 O1, 128 columns each.  While one slot's softmax runs, the tensor cores work for the other.
 // Units with few query tiles split the keys over CTAs; cross_combine_kernel joins the partial results by their
 // log-sum-exps in a fixed order.
@@ -22,9 +25,9 @@ template <int DP>
 struct FwdCfg {
   static constexpr int NSUB = DP / 64;
   static constexpr int TILE = NSUB * static_cast<int>(SUB_BYTES);  // bytes of a 128-row tile
-  static constexpr int STAGES = DP == 128 ? 4 : 8;                 // ring of K and V tiles (even: K in even stages)
-  static constexpr int STAGE_PARTS = 2;                            // staging buffers of 64 channels for the output
-  static constexpr int SMEM = 2 * TILE + STAGES * TILE + STAGE_PARTS * static_cast<int>(SUB_BYTES) + 2 * 2 * CT * 4 + 512;
+  static constexpr int STAGES = DP == 128 ? 2 : 4;                 // ring of (V, next K) pairs
+  static constexpr int SMEM = 2 * TILE + STAGES * 2 * TILE + static_cast<int>(SUB_BYTES) + 10 * CT * 4 + 512;
+  static constexpr int THREADS = 768;
   static constexpr uint32_t TMEM_COLS = 512;
 };
 
@@ -65,17 +68,73 @@ __device__ __forceinline__ bool needs_zeroing(const CrossParams& P, int64_t len,
   return P.bias2 != nullptr || (len < P.Sk && static_cast<int64_t>(t + 1) * CT > len);
 }
 
+// 16 scores of a row -> probabilities: x = s scale2 + nm (nm = -m), p = exp2(x).  MASK 0: all keys in use; 1: keys from
+// `lim` on are out; 2: b4 is what each key adds, -inf: out, whatever its score.  Of unmasked keys every POLY-th pair goes
+// through the FMA pipe's exp2.  Adds to the row's sums, raises `top` (NaN stays).
+template <typename T, int MASK>
+__device__ __forceinline__ void soft_chunk(const uint32_t (&r)[16], float scale2, float nm, int lim, const float4* b4,
+                                           uint32_t* pk, f32x2 (&sum)[2], float (&top)[2]) {
+  const f32x2 sc = f2(scale2, scale2), n2 = f2(nm, nm);
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    float4 bb;
+    if constexpr (MASK == 2) bb = __ldg(b4 + i / 2);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int k = 2 * (i + h);
+      float xa, xb;
+      const f32x2 sv = f2(__uint_as_float(r[k]), __uint_as_float(r[k + 1]));
+      if constexpr (MASK == 2) {
+        const float ba = h ? bb.z : bb.x, bc = h ? bb.w : bb.y;
+        f2_split(f2_fma(sv, sc, f2_add(f2(ba, bc), n2)), xa, xb);
+        if (ba == -INFINITY) xa = -INFINITY;
+        if (bc == -INFINITY) xb = -INFINITY;
+      } else {
+        f2_split(f2_fma(sv, sc, n2), xa, xb);
+        if constexpr (MASK == 1) {
+          if (k >= lim) xa = -INFINITY;
+          if (k + 1 >= lim) xb = -INFINITY;
+        }
+      }
+      top[h] = max_nan(top[h], xa, xb);
+      const f32x2 p = MASK == 0 && h && (i & 2) ? f2_exp2(xa, xb) : f2(ex2(xa), ex2(xb));
+      sum[h] = f2_add(sum[h], p);
+      float pa, pb;
+      f2_split(p, pa, pb);
+      pk[i + h] = pack2<T>(pa, pb);
+    }
+  }
+}
+// the largest s scale2 (+ bias) of 16 scores
+template <int MASK>
+__device__ __forceinline__ float max_chunk(const uint32_t (&r)[16], float scale2, int lim, const float4* b4, float top) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float4 bb = make_float4(0.f, 0.f, 0.f, 0.f);
+    if constexpr (MASK == 2) bb = __ldg(b4 + i);
+    const float bv[4] = {bb.x, bb.y, bb.z, bb.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float x = fmaf(__uint_as_float(r[4 * i + e]), scale2, bv[e]);
+      if (MASK == 0 || (MASK == 1 ? 4 * i + e < lim : bv[e] != -INFINITY)) top = fmaxf(top, x);
+    }
+  }
+  return top;
+}
+
 template <typename T, int DP, bool BIAS>
-__global__ void __launch_bounds__(512, 1)
+__global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
     cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                      const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, const CrossParams P) {
   using C = FwdCfg<DP>;
   extern __shared__ __align__(1024) unsigned char ca_smem[];
   unsigned char* sQ = ca_smem;
-  unsigned char* sKV = sQ + 2 * C::TILE;
-  unsigned char* sO = sKV + C::STAGES * C::TILE;
-  float* stat = reinterpret_cast<float*>(sO + C::STAGE_PARTS * SUB_BYTES);  // [slot][l, m][row]
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(stat + 4 * CT);
+  unsigned char* sV = sQ + 2 * C::TILE;  // stage: V tile, K tile
+  unsigned char* sO = sV + C::STAGES * 2 * C::TILE;
+  float* stat_l = reinterpret_cast<float*>(sO + SUB_BYTES);  // [slot][half][row] sums
+  float* stat_m = stat_l + 4 * CT;                            // [slot][row] maxima
+  float* tops = stat_m + 2 * CT;                              // [slot][half][row] maxima of the halves, while one is taken
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(tops + 4 * CT);
   uint64_t* q_empty = q_full + 2;
   uint64_t* kv_full = q_empty + 2;
   uint64_t* kv_empty = kv_full + C::STAGES;
@@ -99,10 +158,10 @@ __global__ void __launch_bounds__(512, 1)
       mbar_init(&q_full[s], 1);
       mbar_init(&q_empty[s], 1);
       mbar_init(&s_full[s], 1);
-      mbar_init(&p_full[s], 4);
+      mbar_init(&p_full[s], 8);
       mbar_init(&o_full[s], 1);
       mbar_init(&o_empty[s], 4);
-      mbar_init(&l_full[s], 4);
+      mbar_init(&l_full[s], 8);
     }
     for (int s = 0; s < C::STAGES; ++s) {
       mbar_init(&kv_full[s], 1);
@@ -117,7 +176,7 @@ __global__ void __launch_bounds__(512, 1)
     tma_prefetch_desc(&tmV);
     tma_prefetch_desc(&tmO);
   }
-  if (warp == 12) {
+  if (warp == 20) {
     tmem_alloc(tmem_slot, C::TMEM_COLS);
     tmem_relinquish();
   }
@@ -126,130 +185,118 @@ __global__ void __launch_bounds__(512, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp < 8) {
+  if (warp < 16) {
     // ------------------------------------------------------------------------------------------ softmax
-    regs_inc<176>();
-    const int slot = warp >> 2, row = threadIdx.x & (CT - 1);
+    regs_inc<96>();
+    const int slot = warp >> 3, half = (warp >> 2) & 1, row = threadIdx.x & (CT - 1);
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // lane offset (32 per warp) in bits 16..
     const uint32_t tS = tmem + slot * CT + lanes, tO = tmem + 2 * CT + slot * CT + lanes;
+    const int bar = 1 + slot * 4 + (warp & 3);  // the two warps of the same 32 rows
     uint32_t sph = 0, oph = 1;
     FwdUnit u;
-    bool ok = true;
-    for (int64_t it = blockIdx.x; ok && fwd_next(P, it, n_items, u);) {
+    bool dead = false;
+    for (int64_t it = blockIdx.x; fwd_next(P, it, n_items, u);) {
       if (slot == 1 && !u.two) continue;
       const int64_t len = ca_len(P.kv_lens, u.b, P.Sk);
-      const float* bias = BIAS ? P.bias2 + u.b * P.Skp : nullptr;
-      float m = -INFINITY, l = 0.f;
+      float m = -INFINITY;
+      f32x2 l = f2(0.f, 0.f);
       for (int t = u.t0; t < u.t1; ++t) {
-        if (!(ok = warp_wait(&s_full[slot], sph, abort_flag))) break;
+        dead = dead || !warp_wait(&s_full[slot], sph, abort_flag);
         sph ^= 1;
         tc_fence_after();
-        uint32_t r[4][32];
+        const int64_t left = len - static_cast<int64_t>(t) * CT - half * 64;
+        const int lim = left < 64 ? static_cast<int>(left) : 64;  // keys in use, of this thread's
+        const float4* b4 = BIAS ? reinterpret_cast<const float4*>(P.bias2 + u.b * P.Skp + static_cast<int64_t>(t) * CT + half * 64) : nullptr;
+        uint32_t pk[32];
+        f32x2 sum[2];
+        for (bool exact = t == u.t0;; exact = true) {
+          if (exact) {
+            float top = m;
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              uint32_t r[16];
+              tmem_ld_32x32b_x16(tS + half * 64 + 16 * c, r);
+              tmem_ld_wait();
+              if constexpr (BIAS) top = max_chunk<2>(r, P.scale2, 0, b4 + 4 * c, top);
+              else if (lim < 64) top = max_chunk<1>(r, P.scale2, lim - 16 * c, nullptr, top);
+              else top = max_chunk<0>(r, P.scale2, 0, nullptr, top);
+            }
+            tops[(slot * 2 + half) * CT + row] = top;
+            group_sync(bar, 64);  // (both have read by the barrier after the probabilities)
+            top = fmaxf(top, tops[(slot * 2 + 1 - half) * CT + row]);
+            if (t > u.t0) {  // the product of the tile before is complete: its commit came before that of these scores
+              const float f = top == -INFINITY ? 1.f : ex2(m - top);
+              float la, lb;
+              f2_split(l, la, lb);
+              l = f2(la * f, lb * f);
+#pragma unroll 1
+              for (int c = half * (DP / 32); c < (half + 1) * (DP / 32); ++c) {
+                uint32_t o[16];
+                tmem_ld_32x32b_x16(tO + 16 * c, o);
+                tmem_ld_wait();
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(tS + 32 * c, r[c]);
-        tmem_ld_wait();
-        float mt[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        if constexpr (BIAS) {
-          const float4* b4 = reinterpret_cast<const float4*>(bias + static_cast<int64_t>(t) * CT);
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float4 bb = __ldg(b4 + 8 * c + i);
-              const float bv[4] = {bb.x, bb.y, bb.z, bb.w};
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {  // a masked key's score is replaced, whatever it was
-                const float x = fmaf(__uint_as_float(r[c][4 * i + e]), P.scale2, bv[e]);
-                r[c][4 * i + e] = __float_as_uint(bv[e] == -INFINITY ? -INFINITY : x);
+                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                tmem_st_32x32b_x16(tO + 16 * c, o);
               }
             }
-        } else {
-          const int64_t lim = len - static_cast<int64_t>(t) * CT;
-          if (lim < CT) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (32 * c + i >= lim) r[c][i] = 0xFF800000u;  // -inf
+            m = top;
           }
-        }
+          const float nm = m == -INFINITY ? 0.f : -m;  // no key so far: every probability is exp2(-inf) = 0
+          float over[2] = {-INFINITY, -INFINITY};
+          sum[0] = sum[1] = f2(0.f, 0.f);
+          uint32_t r[2][16];
+          tmem_ld_32x32b_x16(tS + half * 64, r[0]);
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; ++i) mt[c] = fmaxf(mt[c], __uint_as_float(r[c][i]));
-        float top = fmaxf(fmaxf(mt[0], mt[1]), fmaxf(mt[2], mt[3]));
-        if constexpr (!BIAS) top *= P.scale2;
-        if (t == u.t0) {
-          m = top;
-        } else if (__any_sync(0xffffffffu, top > m + 8.f)) {
-          // the product of the tile before is complete: its commit came before that of these scores
-          const float mn = fmaxf(m, top), f = mn == -INFINITY ? 1.f : ex2(m - mn);
-          m = mn;
-          l *= f;
-#pragma unroll 1
-          for (int c = 0; c < DP / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld_32x32b_x32(tO + 32 * c, o);
+          for (int c = 0; c < 4; ++c) {
             tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-            tmem_st_32x32b_x32(tO + 32 * c, o);
+            if (c < 3) tmem_ld_32x32b_x16(tS + half * 64 + 16 * (c + 1), r[(c + 1) & 1]);
+            if constexpr (BIAS) soft_chunk<T, 2>(r[c & 1], P.scale2, nm, 0, b4 + 4 * c, pk + 8 * c, sum, over);
+            else if (lim < 64) soft_chunk<T, 1>(r[c & 1], P.scale2, nm, lim - 16 * c, nullptr, pk + 8 * c, sum, over);
+            else soft_chunk<T, 0>(r[c & 1], P.scale2, nm, 0, nullptr, pk + 8 * c, sum, over);
           }
+          over[0] = max_nan(over[0], over[1], over[1]);
+          if (over[0] != over[0]) sum[0] = f2(over[0], over[0]);  // a score that is not a number: so is the row
+          // past this barrier both warps have read S
+          if (!group_any(bar, 64, over[0] > (m == -INFINITY ? -INFINITY : 8.f)) || exact) break;
         }
-        const float mm = m == -INFINITY ? 0.f : m;  // no key so far: every probability is exp2(-inf) = 0
-        float ls[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float x = __uint_as_float(r[c][i]);
-            const float p = ex2(BIAS ? x - mm : fmaf(x, P.scale2, -mm));
-            ls[i & 3] += p;
-            r[c][i] = __float_as_uint(p);
-          }
-        }
-        l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t pk[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const int k = 64 * c + 2 * i;
-            pk[i] = pack2<T>(__uint_as_float(r[k >> 5][k & 31]), __uint_as_float(r[k >> 5][(k & 31) + 1]));
-          }
-          tmem_st_32x32b_x32(tS + 32 * c, pk);
-        }
+        l = f2_add(l, f2_add(sum[0], sum[1]));
+        tmem_st_32x32b_x32(tS + half * 32, pk);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[slot]);
       }
-      if (!ok || !(ok = warp_wait(&o_empty[slot], oph, abort_flag))) break;
+      dead = dead || !warp_wait(&o_empty[slot], oph, abort_flag);  // the epilogue has read the unit before
       oph ^= 1;
-      stat[(slot * 2 + 0) * CT + row] = l;
-      stat[(slot * 2 + 1) * CT + row] = m;
+      float la, lb;
+      f2_split(l, la, lb);
+      stat_l[(slot * 2 + half) * CT + row] = la + lb;
+      if (half == 0) stat_m[slot * CT + row] = m;
       __syncwarp();
       if (lane == 0) mbar_arrive(&l_full[slot]);
     }
-  } else if (warp < 12) {
+  } else if (warp < 20) {
     // ------------------------------------------------------------------------------------------ epilogue
-    regs_dec<96>();
+    regs_dec<48>();
     const int row = threadIdx.x & (CT - 1), qr = row / P.G, hg = row - qr * P.G;
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
+    const int64_t rows = static_cast<int64_t>(P.B) * P.Hq * P.Sq;
     uint32_t ph[2] = {0, 0};
     bool dead = false;
     for (int64_t it = blockIdx.x; it < n_items; it += gridDim.x) {
       const FwdUnit u = fwd_unit(P, it);
-      for (int slot = 0; slot < (u.two ? 2 : 1); ++slot) {
+      const bool any = u.t1 > u.t0;
+#pragma unroll
+      for (int slot = 0; slot < 2; ++slot) {
+        if (slot == 1 && !u.two) break;
         const int64_t s0 = static_cast<int64_t>(u.tile0 + slot) * P.nq, s = s0 + qr;
-        const bool valid = qr < P.nq && s < P.Sq, any = u.t1 > u.t0;
+        const bool valid = qr < P.nq && s < P.Sq;
         float l = 0.f, m = -INFINITY;
         if (any) {
-          if (!warp_wait(&l_full[slot], ph[slot], abort_flag)) dead = true;
-          if (!warp_wait(&o_full[slot], ph[slot], abort_flag)) dead = true;
+          dead = dead || !warp_wait(&l_full[slot], ph[slot], abort_flag) || !warp_wait(&o_full[slot], ph[slot], abort_flag);
           ph[slot] ^= 1;
-          l = stat[(slot * 2 + 0) * CT + row];
-          m = stat[(slot * 2 + 1) * CT + row];
+          l = stat_l[slot * 2 * CT + row] + stat_l[(slot * 2 + 1) * CT + row];
+          m = stat_m[slot * CT + row];
           tc_fence_after();
         }
         const bool none = l == 0.f;
@@ -257,54 +304,53 @@ __global__ void __launch_bounds__(512, 1)
         const uint32_t tO = tmem + 2 * CT + slot * CT + lanes;
         const int64_t rid = (static_cast<int64_t>(u.b) * P.Hq + u.hk * P.G + hg) * P.Sq + s;
         const float lse2 = none ? -INFINITY : m + log2f(l);
+        if (valid) {
+          if (P.splits > 1) P.part_lse[u.split * rows + rid] = lse2;
+          else if (P.lse) P.lse[rid] = lse2 * CA_LN2;
+        }
         if (P.splits > 1) {
-          if (valid) P.part_lse[static_cast<int64_t>(u.split) * P.B * P.Hq * P.Sq + rid] = lse2;
-          float* dst = P.part_o + (static_cast<int64_t>(u.split) * P.B * P.Hq * P.Sq + rid) * P.D;
-          if (any) {
+          float* dst = P.part_o + (u.split * rows + rid) * P.D;
 #pragma unroll 1
-            for (int c = 0; c < DP / 32; ++c) {
-              uint32_t o[32];
-              tmem_ld_32x32b_x32(tO + 32 * c, o);
-              tmem_ld_wait();
-              if (valid && !dead) {
+          for (int c = 0; any && c < DP / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld_32x32b_x16(tO + 16 * c, o);
+            tmem_ld_wait();
+            if (!valid) continue;
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                  if (32 * c + 4 * i < P.D)
-                    *reinterpret_cast<float4*>(dst + 32 * c + 4 * i) =
-                        make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv,
-                                    __uint_as_float(o[4 * i + 2]) * inv, __uint_as_float(o[4 * i + 3]) * inv);
-              }
-            }
+            for (int i = 0; i < 4; ++i)
+              if (16 * c + 4 * i < P.D)
+                *reinterpret_cast<float4*>(dst + 16 * c + 4 * i) =
+                    none ? make_float4(0.f, 0.f, 0.f, 0.f)
+                         : make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv,
+                                       __uint_as_float(o[4 * i + 2]) * inv, __uint_as_float(o[4 * i + 3]) * inv);
           }
         } else {
-          if (P.lse && valid) P.lse[rid] = lse2 * CA_LN2;
 #pragma unroll 1
           for (int part = 0; part < C::NSUB; ++part) {
-            unsigned char* buf = sO + part * SUB_BYTES;
-            if (warp == 8 && lane == 0) bulk_wait_read<C::NSUB - 1>();  // this part's store before has left the buffer
-            group_sync(1, 128);
+            if (warp == 16 && lane == 0) bulk_wait_read<0>();  // the store before has left the buffer
+            group_sync(9, 128);
 #pragma unroll 1
-            for (int c = 0; c < 2; ++c) {
-              uint32_t o[32];
+            for (int c = 0; c < 4; ++c) {
+              uint32_t o[16];
               if (any) {
-                tmem_ld_32x32b_x32(tO + 64 * part + 32 * c, o);
+                tmem_ld_32x32b_x16(tO + 64 * part + 16 * c, o);
                 tmem_ld_wait();
               }
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
+              for (int i = 0; i < 2; ++i) {
                 uint4 v;
                 uint32_t* vv = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
+                for (int e = 0; e < 4; ++e)  // no key took part: zero, whatever the products hold
                   vv[e] = none ? 0u
                                : pack2<T>(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
-                put_swizzled(buf, row, 4 * c + i, v);
+                put_swizzled(sO, row, 2 * c + i, v);
               }
             }
             fence_proxy_async_smem();
-            group_sync(1, 128);
-            if (warp == 8 && lane == 0 && !dead) {
-              tma_store_5d(buf, &tmO, 64 * part, 0, u.hk, static_cast<int>(s0), u.b);
+            group_sync(9, 128);
+            if (warp == 16 && lane == 0 && !dead) {
+              tma_store_5d(sO, &tmO, 64 * part, 0, u.hk, static_cast<int>(s0), u.b);
               bulk_commit();
             }
           }
@@ -316,53 +362,49 @@ __global__ void __launch_bounds__(512, 1)
         }
       }
     }
-    if (warp == 8 && lane == 0) bulk_wait_all();
+    if (warp == 16 && lane == 0) bulk_wait_all();
   } else {
-    regs_dec<64>();
-    if (warp == 12) {
+    regs_dec<48>();
+    if (warp == 20) {
       // -------------------------------------------------------------------------------------- MMA issue
       constexpr uint32_t idQK = idesc_f16<T>(CT, CT, false), idPV = idesc_f16<T>(CT, DP, true);
       constexpr uint64_t TILE16 = C::TILE >> 4;
-      const uint64_t dQ = desc_rows(smem_u32(sQ)), dK = desc_rows(smem_u32(sKV)), dV = desc_chan(smem_u32(sKV));
+      const uint64_t dQ = desc_rows(smem_u32(sQ)), dK = desc_rows(smem_u32(sV) + C::TILE), dV = desc_chan(smem_u32(sV));
       int st = 0;
       uint32_t kph = 0, qph[2] = {0, 0}, pph[2] = {0, 0}, oph[2] = {1, 1};
-      auto step = [&] {
-        if (++st == C::STAGES) st = 0, kph ^= 1;
-      };
-      auto qk = [&](int slot, int kst) {
-        mma_rows<DP / 16>(tmem + slot * CT, dQ + slot * TILE16, dK + kst * TILE16, idQK);
-        commit_one(&s_full[slot]);
-      };
       FwdUnit cur, nxt;
       int64_t it = blockIdx.x;
       bool have = fwd_next(P, it, n_items, cur), ok = true;
+      auto qk = [&](int slot, int kst, bool first, bool last) {  // S of a slot; its Q tile arrives with the unit's first
+        if (first) {
+          if (!(ok = warp_wait(&q_full[slot], qph[slot], abort_flag))) return;
+          qph[slot] ^= 1;
+          tc_fence_after();
+        }
+        mma_rows<DP / 16>(tmem + slot * CT, dQ + slot * TILE16, dK + kst * 2 * TILE16, idQK);
+        commit_one(&s_full[slot]);
+        if (last) commit_one(&q_empty[slot]);
+      };
+      auto advance = [&] {
+        commit_one(&kv_empty[st]);
+        if (++st == C::STAGES) st = 0, kph ^= 1;
+      };
       if (have) {
         ok = warp_wait(&kv_full[st], kph, abort_flag);
-        for (int s = 0; ok && s < (cur.two ? 2 : 1); ++s) {
-          ok = warp_wait(&q_full[s], qph[s], abort_flag);
-          qph[s] ^= 1;
-          if (!ok) break;
-          tc_fence_after();
-          qk(s, st);
-          if (cur.t1 - cur.t0 == 1) commit_one(&q_empty[s]);
-        }
-        commit_one(&kv_empty[st]);
-        step();
+        tc_fence_after();
+        if (ok) qk(0, st, true, cur.t1 - cur.t0 == 1);
+        if (ok && cur.two) qk(1, st, true, cur.t1 - cur.t0 == 1);
+        advance();
       }
       while (have && ok) {
-        bool more = false;
+        const bool more = fwd_next(P, it, n_items, nxt);
         for (int t = cur.t0; ok && t < cur.t1; ++t) {
-          const bool last = t == cur.t1 - 1;
-          if (last) more = fwd_next(P, it, n_items, nxt);
-          const int vst = st;
-          if (!(ok = warp_wait(&kv_full[vst], kph, abort_flag))) break;
-          if (masked && !(ok = warp_wait(&v_clean[vst], kph, abort_flag))) break;
-          step();
-          const bool then_qk = !last || more;
-          const int kst = st;
-          const uint32_t kparity = kph;
-          if (then_qk) step();
-          for (int s = 0; ok && s < 2; ++s) {
+          const bool last = t == cur.t1 - 1, then_qk = !last || more;
+          const bool qk_last = last ? nxt.t1 - nxt.t0 == 1 : t + 2 == cur.t1;
+          if (!(ok = warp_wait(&kv_full[st], kph, abort_flag))) break;
+          if (masked && !(ok = warp_wait(&v_clean[st], kph, abort_flag))) break;
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
             if (s == 0 || cur.two) {
               if (!(ok = warp_wait(&p_full[s], pph[s], abort_flag))) break;
               pph[s] ^= 1;
@@ -371,56 +413,64 @@ __global__ void __launch_bounds__(512, 1)
                 oph[s] ^= 1;
               }
               tc_fence_after();
-              mma_chan<false>(tmem + 2 * CT + s * CT, tmem + s * CT, dV + vst * TILE16, idPV, t > cur.t0);
+              mma_chan<false>(tmem + 2 * CT + s * CT, tmem + s * CT, dV + st * 2 * TILE16, idPV, t > cur.t0);
               if (last) commit_one(&o_full[s]);
             }
-            if (then_qk && (s == 0 || (last ? nxt.two : cur.two))) {
-              if (!(ok = warp_wait(&kv_full[kst], kparity, abort_flag))) break;
-              if (last) {
-                if (!(ok = warp_wait(&q_full[s], qph[s], abort_flag))) break;
-                qph[s] ^= 1;
-              }
-              tc_fence_after();
-              qk(s, kst);
-              if (last ? nxt.t1 - nxt.t0 == 1 : t + 2 == cur.t1) commit_one(&q_empty[s]);
-            }
+            if (then_qk && (s == 0 || (last ? nxt.two : cur.two))) qk(s, st, last, qk_last);
+            if (!ok) break;
           }
-          if (!ok) break;
-          commit_one(&kv_empty[vst]);
-          if (then_qk) commit_one(&kv_empty[kst]);
+          if (ok) advance();
         }
         cur = nxt;
         have = more;
       }
-    } else if (warp == 13) {
+    } else if (warp == 21) {
       if (lane == 0) {
         // -------------------------------------------------------------------------------------- copies
         int st = 0, fills = 0, qfills[2] = {0, 0};
         uint32_t kph = 1, qph[2] = {1, 1};
-        FwdUnit u;
+        FwdUnit u, nxt;
         bool ok = true;
         const uint32_t q_bytes = static_cast<uint32_t>(C::NSUB * 128 * P.G * P.nq);
-        auto load = [&](const CUtensorMap* map, int t) {
-          if (!(ok = mbar_wait(&kv_empty[st], kph, abort_flag))) return;
-          mbar_arrive_expect_tx(&kv_full[st], C::TILE);
+        auto load_q = [&](const FwdUnit& w, int s) {
+          if (!ok || !(ok = mbar_wait(&q_empty[s], qph[s], abort_flag))) return;
+          qph[s] ^= 1;
+          mbar_arrive_expect_tx(&q_full[s], q_bytes);
           for (int p = 0; p < C::NSUB; ++p)
-            tma_load_4d(sKV + st * C::TILE + p * SUB_BYTES, map, &kv_full[st], 64 * p, u.hk, t * CT, u.b);
+            tma_load_5d(sQ + s * C::TILE + p * SUB_BYTES, &tmQ, &q_full[s], 64 * p, 0, w.hk, (w.tile0 + s) * P.nq, w.b);
+          ++qfills[s];
+        };
+        // one stage: V of tile tv (if >= 0) of unit uv, K of tile tk (if >= 0) of unit uk
+        auto load_kv = [&](const FwdUnit& uv, int tv, const FwdUnit& uk, int tk) {
+          if (!ok || !(ok = mbar_wait(&kv_empty[st], kph, abort_flag))) return;
+          mbar_arrive_expect_tx(&kv_full[st], ((tv >= 0) + (tk >= 0)) * C::TILE);
+          unsigned char* dst = sV + st * 2 * C::TILE;
+          for (int p = 0; tv >= 0 && p < C::NSUB; ++p)
+            tma_load_4d(dst + p * SUB_BYTES, &tmV, &kv_full[st], 64 * p, uv.hk, tv * CT, uv.b);
+          for (int p = 0; tk >= 0 && p < C::NSUB; ++p)
+            tma_load_4d(dst + C::TILE + p * SUB_BYTES, &tmK, &kv_full[st], 64 * p, uk.hk, tk * CT, uk.b);
           ++fills;
           if (++st == C::STAGES) st = 0, kph ^= 1;
         };
-        for (int64_t it = blockIdx.x; ok && fwd_next(P, it, n_items, u);) {
-          for (int s = 0; ok && s < (u.two ? 2 : 1); ++s) {
-            if (!(ok = mbar_wait(&q_empty[s], qph[s], abort_flag))) break;
-            qph[s] ^= 1;
-            mbar_arrive_expect_tx(&q_full[s], q_bytes);
-            for (int p = 0; p < C::NSUB; ++p)
-              tma_load_5d(sQ + s * C::TILE + p * SUB_BYTES, &tmQ, &q_full[s], 64 * p, 0, u.hk, (u.tile0 + s) * P.nq, u.b);
-            ++qfills[s];
-          }
+        int64_t it = blockIdx.x;
+        bool have = fwd_next(P, it, n_items, u);
+        if (have) {
+          load_kv(u, -1, u, u.t0);
+          load_q(u, 0);
+          if (u.two) load_q(u, 1);
+        }
+        while (have && ok) {
+          const bool more = fwd_next(P, it, n_items, nxt);
           for (int t = u.t0; ok && t < u.t1; ++t) {
-            load(&tmK, t);
-            if (ok) load(&tmV, t);
+            const bool last = t == u.t1 - 1;
+            if (!last) load_kv(u, t, u, t + 1);
+            else load_kv(u, t, nxt, more ? nxt.t0 : -1);
           }
+          // the next unit's Q tiles come in while this one's last key tile is in hand
+          if (more) load_q(nxt, 0);
+          if (more && nxt.two) load_q(nxt, 1);
+          u = nxt;
+          have = more;
         }
         // copies in flight land in this CTA's shared memory: wait for the last ones before it goes away
         for (int j = fills > C::STAGES ? fills - C::STAGES : 0; j < fills; ++j)
@@ -429,16 +479,16 @@ __global__ void __launch_bounds__(512, 1)
           if (qfills[s]) mbar_wait_drain(&q_full[s], static_cast<uint32_t>((qfills[s] - 1) & 1));
       }
       __syncwarp();
-    } else if (warp == 14 && masked) {
+    } else if (warp == 22 && masked) {
       // ---------------------------------------------------------------------------------------- rows of masked keys
-      int st = 0;
+      if (lane == 0) mbar_arrive(&v_clean[0]);  // the first stage holds a K tile only
+      int st = 1;
       uint32_t kph = 0;
       FwdUnit u;
       bool ok = true;
       for (int64_t it = blockIdx.x; ok && fwd_next(P, it, n_items, u);) {
         const int64_t len = ca_len(P.kv_lens, u.b, P.Sk);
         for (int t = u.t0; ok && t < u.t1; ++t) {
-          if (++st == C::STAGES) st = 0, kph ^= 1;  // the K tile
           if (!(ok = warp_wait(&kv_full[st], kph, abort_flag))) break;
           if (needs_zeroing(P, len, t)) {
             for (int j = lane; j < CT; j += 32) {
@@ -446,7 +496,7 @@ __global__ void __launch_bounds__(512, 1)
               if (key >= len || (BIAS && P.bias2[u.b * P.Skp + key] == -INFINITY))
                 for (int p = 0; p < C::NSUB; ++p)
                   for (int c = 0; c < 8; ++c)
-                    *reinterpret_cast<uint4*>(sKV + st * C::TILE + p * SUB_BYTES + j * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4*>(sV + st * 2 * C::TILE + p * SUB_BYTES + j * 128 + c * 16) = make_uint4(0, 0, 0, 0);
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -459,7 +509,7 @@ __global__ void __launch_bounds__(512, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 20) {
     tc_fence_after();
     commit_one(done);  // every product issued (after a wait that gave up some may still run) and its arrivals are over
     mbar_wait_drain(done, 0);
@@ -529,7 +579,7 @@ static int fwd_launch_cfg(const CrossParams& P, cudaStream_t st) {
   if (e != cudaSuccess) return cuda_fail(e, "cross_fwd_kernel shared memory");
   const int64_t items = static_cast<int64_t>(P.units) * P.splits * P.Hkv * P.B;
   const int grid = static_cast<int>(items < cross_sms() ? items : cross_sms());
-  kern<<<grid, 512, C::SMEM, st>>>(q, k, v, o, P);
+  kern<<<grid, C::THREADS, C::SMEM, st>>>(q, k, v, o, P);
   rc = check_launch("cross_fwd_kernel");
   if (rc || P.splits == 1) return rc;
   const int64_t rows = static_cast<int64_t>(P.B) * P.Hq * P.Sq;
