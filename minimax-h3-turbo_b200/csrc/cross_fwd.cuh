@@ -9,11 +9,13 @@
 //              only when a tile exceeds it by more than 8 (a factor 2^8: far from overflow in fp32 sums and fp16 P): P of a
 //              tile is computed with the m at hand, without a pass for the maximum before it, and only such a tile is gone
 //              over again, after its threads have rescaled O in tensor memory.
-//   16-19      epilogue: O / l to the operand type, through swizzled staging and a bulk tensor store; log-sum-exp
-//   20         MMA issue: S = Q K^T (both from shared memory), O += P V (P from tensor memory, V channel-major)
-//   21         copies: Q tiles, and a ring of pairs (V of a key tile, K of the next): what one step of both slots reads,
+//              After a unit's last tile the same threads take O / l through swizzled staging to a bulk tensor store, while
+//              the next unit's first scores are on their way; and the log-sum-exp.
+//   16         MMA issue: S = Q K^T (both from shared memory), O += P V (P from tensor memory, V channel-major)
+//   17         copies: Q tiles, and a ring of pairs (V of a key tile, K of the next): what one step of both slots reads,
 //              one barrier each way
-//   22         zeroes the rows of V tiles whose keys are left out, before their product (0 x NaN would reach the sums)
+//   18         zeroes the rows of V tiles whose keys are left out, before their product (0 x NaN would reach the sums)
+//   19         stores
 // Tensor memory: S0 S1 O0 O1, 128 columns each.  While one slot's softmax runs, the tensor cores work for the other.
 // Units with few query tiles split the keys over CTAs; cross_combine_kernel joins the partial results by their
 // log-sum-exps in a fixed order.
@@ -26,8 +28,8 @@ struct FwdCfg {
   static constexpr int NSUB = DP / 64;
   static constexpr int TILE = NSUB * static_cast<int>(SUB_BYTES);  // bytes of a 128-row tile
   static constexpr int STAGES = DP == 128 ? 2 : 4;                 // ring of (V, next K) pairs
-  static constexpr int SMEM = 2 * TILE + STAGES * 2 * TILE + static_cast<int>(SUB_BYTES) + 10 * CT * 4 + 512;
-  static constexpr int THREADS = 768;
+  static constexpr int SMEM = 2 * TILE + STAGES * 2 * TILE + TILE + 4 * CT * 4 + 512;
+  static constexpr int THREADS = 640;
   static constexpr uint32_t TMEM_COLS = 512;
 };
 
@@ -36,24 +38,25 @@ struct FwdUnit {
   bool two;                         // the second query tile exists
 };
 
-__device__ __forceinline__ FwdUnit fwd_unit(const CrossParams& P, int64_t it) {
+__device__ __forceinline__ FwdUnit fwd_unit(const CrossParams& P, int it) {  // (32-bit divisions: 64-bit ones cost ~2000 cycles)
   FwdUnit u;
-  const int pair = static_cast<int>(it % P.units);
-  int64_t r = it / P.units;
+  unsigned r = static_cast<unsigned>(it);
+  const int pair = static_cast<int>(r % P.units);
+  r /= P.units;
   u.split = static_cast<int>(r % P.splits);
   r /= P.splits;
   u.hk = static_cast<int>(r % P.Hkv);
   u.b = static_cast<int>(r / P.Hkv);
   u.tile0 = pair * 2;
   u.two = u.tile0 + 1 < P.q_tiles;
-  const int nt = static_cast<int>((ca_len(P.kv_lens, u.b, P.Sk) + CT - 1) / CT);
-  const int per = (nt + P.splits - 1) / P.splits;
-  u.t0 = min(u.split * per, nt);
-  u.t1 = min(u.t0 + per, nt);
+  const unsigned nt = static_cast<unsigned>(ca_len(P.kv_lens, u.b, P.Sk) + CT - 1) / CT;
+  const unsigned per = (nt + P.splits - 1) / P.splits;
+  u.t0 = static_cast<int>(min(u.split * per, nt));
+  u.t1 = static_cast<int>(min(u.t0 + per, nt));
   return u;
 }
 // the next unit with key tiles
-__device__ __forceinline__ bool fwd_next(const CrossParams& P, int64_t& it, int64_t n, FwdUnit& u) {
+__device__ __forceinline__ bool fwd_next(const CrossParams& P, int& it, int n, FwdUnit& u) {
   for (; it < n; it += gridDim.x) {
     u = fwd_unit(P, it);
     if (u.t1 > u.t0) {
@@ -131,10 +134,8 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
   unsigned char* sQ = ca_smem;
   unsigned char* sV = sQ + 2 * C::TILE;  // stage: V tile, K tile
   unsigned char* sO = sV + C::STAGES * 2 * C::TILE;
-  float* stat_l = reinterpret_cast<float*>(sO + SUB_BYTES);  // [slot][half][row] sums
-  float* stat_m = stat_l + 4 * CT;                            // [slot][row] maxima
-  float* tops = stat_m + 2 * CT;                              // [slot][half][row] maxima of the halves, while one is taken
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(tops + 4 * CT);
+  float* halves = reinterpret_cast<float*>(sO + C::TILE);  // [slot][half][row] maxima or sums of a row's halves
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(halves + 4 * CT);
   uint64_t* q_empty = q_full + 2;
   uint64_t* kv_full = q_empty + 2;
   uint64_t* kv_empty = kv_full + C::STAGES;
@@ -142,14 +143,14 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
   uint64_t* s_full = v_clean + C::STAGES;
   uint64_t* p_full = s_full + 2;
   uint64_t* o_full = p_full + 2;
-  uint64_t* o_empty = o_full + 2;
-  uint64_t* l_full = o_empty + 2;
-  uint64_t* done = l_full + 2;
+  uint64_t* out_full = o_full + 2;  // the staging holds a slot's output
+  uint64_t* out_free = out_full + 1;  // [use & 1] and has been read
+  uint64_t* done = out_free + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int64_t n_items = static_cast<int64_t>(P.units) * P.splits * P.Hkv * P.B;
+  const int n_items = P.units * P.splits * P.Hkv * P.B;
   // with any mask every V tile passes warp 14 (in step with the ring: a phase it skipped could be taken for another)
   const bool masked = BIAS || P.kv_lens != nullptr;
 
@@ -160,14 +161,15 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
       mbar_init(&s_full[s], 1);
       mbar_init(&p_full[s], 8);
       mbar_init(&o_full[s], 1);
-      mbar_init(&o_empty[s], 4);
-      mbar_init(&l_full[s], 8);
     }
     for (int s = 0; s < C::STAGES; ++s) {
       mbar_init(&kv_full[s], 1);
       mbar_init(&kv_empty[s], 1);
       mbar_init(&v_clean[s], 1);
     }
+    mbar_init(out_full, 8);
+    mbar_init(&out_free[0], 1);
+    mbar_init(&out_free[1], 1);
     mbar_init(done, 1);
     *abort_flag = 0;
     mbar_fence_init();
@@ -176,7 +178,7 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
     tma_prefetch_desc(&tmV);
     tma_prefetch_desc(&tmO);
   }
-  if (warp == 20) {
+  if (warp == 16) {
     tmem_alloc(tmem_slot, C::TMEM_COLS);
     tmem_relinquish();
   }
@@ -187,16 +189,23 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
 
   if (warp < 16) {
     // ------------------------------------------------------------------------------------------ softmax
-    regs_inc<96>();
+    regs_inc<104>();
     const int slot = warp >> 3, half = (warp >> 2) & 1, row = threadIdx.x & (CT - 1);
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // lane offset (32 per warp) in bits 16..
     const uint32_t tS = tmem + slot * CT + lanes, tO = tmem + 2 * CT + slot * CT + lanes;
     const int bar = 1 + slot * 4 + (warp & 3);  // the two warps of the same 32 rows
-    uint32_t sph = 0, oph = 1;
-    FwdUnit u;
+    float* mine = halves + (slot * 2 + half) * CT + row;
+    const float* other = halves + (slot * 2 + 1 - half) * CT + row;
+    const int qr = row / P.G, hg = row - qr * P.G;
+    const int64_t rows = static_cast<int64_t>(P.B) * P.Hq * P.Sq;
+    uint32_t sph = 0, oph = 0, uses = slot;  // uses: of the staging by both slots before this one
     bool dead = false;
-    for (int64_t it = blockIdx.x; fwd_next(P, it, n_items, u);) {
-      if (slot == 1 && !u.two) continue;
+    FwdUnit u;
+    for (int it = blockIdx.x; fwd_next(P, it, n_items, u);) {
+      if (slot == 1 && !u.two) {
+        ++uses;
+        continue;
+      }
       const int64_t len = ca_len(P.kv_lens, u.b, P.Sk);
       float m = -INFINITY;
       f32x2 l = f2(0.f, 0.f);
@@ -221,9 +230,9 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
               else if (lim < 64) top = max_chunk<1>(r, P.scale2, lim - 16 * c, nullptr, top);
               else top = max_chunk<0>(r, P.scale2, 0, nullptr, top);
             }
-            tops[(slot * 2 + half) * CT + row] = top;
+            *mine = top;
             group_sync(bar, 64);  // (both have read by the barrier after the probabilities)
-            top = fmaxf(top, tops[(slot * 2 + 1 - half) * CT + row]);
+            top = fmaxf(top, *other);
             if (t > u.t0) {  // the product of the tile before is complete: its commit came before that of these scores
               const float f = top == -INFINITY ? 1.f : ex2(m - top);
               float la, lb;
@@ -266,114 +275,84 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[slot]);
       }
-      dead = dead || !warp_wait(&o_empty[slot], oph, abort_flag);  // the epilogue has read the unit before
-      oph ^= 1;
+      // ---- the unit's output
       float la, lb;
       f2_split(l, la, lb);
-      stat_l[(slot * 2 + half) * CT + row] = la + lb;
-      if (half == 0) stat_m[slot * CT + row] = m;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&l_full[slot]);
-    }
-  } else if (warp < 20) {
-    // ------------------------------------------------------------------------------------------ epilogue
-    regs_dec<48>();
-    const int row = threadIdx.x & (CT - 1), qr = row / P.G, hg = row - qr * P.G;
-    const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
-    const int64_t rows = static_cast<int64_t>(P.B) * P.Hq * P.Sq;
-    uint32_t ph[2] = {0, 0};
-    bool dead = false;
-    for (int64_t it = blockIdx.x; it < n_items; it += gridDim.x) {
-      const FwdUnit u = fwd_unit(P, it);
-      const bool any = u.t1 > u.t0;
-#pragma unroll
-      for (int slot = 0; slot < 2; ++slot) {
-        if (slot == 1 && !u.two) break;
-        const int64_t s0 = static_cast<int64_t>(u.tile0 + slot) * P.nq, s = s0 + qr;
-        const bool valid = qr < P.nq && s < P.Sq;
-        float l = 0.f, m = -INFINITY;
-        if (any) {
-          dead = dead || !warp_wait(&l_full[slot], ph[slot], abort_flag) || !warp_wait(&o_full[slot], ph[slot], abort_flag);
-          ph[slot] ^= 1;
-          l = stat_l[slot * 2 * CT + row] + stat_l[(slot * 2 + 1) * CT + row];
-          m = stat_m[slot * CT + row];
-          tc_fence_after();
-        }
-        const bool none = l == 0.f;
-        const float inv = none ? 0.f : 1.f / l;
-        const uint32_t tO = tmem + 2 * CT + slot * CT + lanes;
-        const int64_t rid = (static_cast<int64_t>(u.b) * P.Hq + u.hk * P.G + hg) * P.Sq + s;
-        const float lse2 = none ? -INFINITY : m + log2f(l);
-        if (valid) {
-          if (P.splits > 1) P.part_lse[u.split * rows + rid] = lse2;
-          else if (P.lse) P.lse[rid] = lse2 * CA_LN2;
-        }
-        if (P.splits > 1) {
-          float* dst = P.part_o + (u.split * rows + rid) * P.D;
-#pragma unroll 1
-          for (int c = 0; any && c < DP / 16; ++c) {
-            uint32_t o[16];
-            tmem_ld_32x32b_x16(tO + 16 * c, o);
-            tmem_ld_wait();
-            if (!valid) continue;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (16 * c + 4 * i < P.D)
-                *reinterpret_cast<float4*>(dst + 16 * c + 4 * i) =
-                    none ? make_float4(0.f, 0.f, 0.f, 0.f)
-                         : make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv,
-                                       __uint_as_float(o[4 * i + 2]) * inv, __uint_as_float(o[4 * i + 3]) * inv);
-          }
-        } else {
-#pragma unroll 1
-          for (int part = 0; part < C::NSUB; ++part) {
-            if (warp == 16 && lane == 0) bulk_wait_read<0>();  // the store before has left the buffer
-            group_sync(9, 128);
-#pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              uint32_t o[16];
-              if (any) {
-                tmem_ld_32x32b_x16(tO + 64 * part + 16 * c, o);
-                tmem_ld_wait();
-              }
-#pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                uint4 v;
-                uint32_t* vv = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-                for (int e = 0; e < 4; ++e)  // no key took part: zero, whatever the products hold
-                  vv[e] = none ? 0u
-                               : pack2<T>(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
-                put_swizzled(sO, row, 2 * c + i, v);
-              }
-            }
-            fence_proxy_async_smem();
-            group_sync(9, 128);
-            if (warp == 16 && lane == 0 && !dead) {
-              tma_store_5d(sO, &tmO, 64 * part, 0, u.hk, static_cast<int>(s0), u.b);
-              bulk_commit();
-            }
-          }
-        }
-        if (any) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&o_empty[slot]);
-        }
+      *mine = la + lb;
+      group_sync(bar, 64);
+      const float total = halves[slot * 2 * CT + row] + halves[(slot * 2 + 1) * CT + row];
+      group_sync(bar, 64);  // both have read before the next unit's maxima
+      const bool none = total == 0.f;  // no key took part: zero, whatever the products hold
+      const float inv = none ? 0.f : 1.f / total;
+      const int64_t s = static_cast<int64_t>(u.tile0 + slot) * P.nq + qr;
+      const bool valid = qr < P.nq && s < P.Sq;
+      const int64_t rid = (static_cast<int64_t>(u.b) * P.Hq + u.hk * P.G + hg) * P.Sq + s;
+      if (half == 0 && valid) {
+        const float lse2 = none ? -INFINITY : m + log2f(total);
+        if (P.splits > 1) P.part_lse[u.split * rows + rid] = lse2;
+        else if (P.lse) P.lse[rid] = lse2 * CA_LN2;
       }
+      dead = dead || !warp_wait(&o_full[slot], oph, abort_flag);
+      oph ^= 1;
+      tc_fence_after();
+      // this thread's columns: half of DP
+      if (P.splits > 1) {
+        float* dst = P.part_o + (u.split * rows + rid) * P.D;
+#pragma unroll 1
+        for (int c = half * (DP / 32); c < (half + 1) * (DP / 32); ++c) {
+          uint32_t o[16];
+          tmem_ld_32x32b_x16(tO + 16 * c, o);
+          tmem_ld_wait();
+          if (!valid) continue;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (16 * c + 4 * i < P.D)
+              *reinterpret_cast<float4*>(dst + 16 * c + 4 * i) =
+                  none ? make_float4(0.f, 0.f, 0.f, 0.f)
+                       : make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv,
+                                     __uint_as_float(o[4 * i + 2]) * inv, __uint_as_float(o[4 * i + 3]) * inv);
+        }
+      } else {
+        uint32_t o[2][16];
+        tmem_ld_32x32b_x16(tO + half * (DP / 2), o[0]);
+        // the use before this one (uses - 1) has left the staging.  Two barriers in turn: a slot gets here only after the use
+        // three before was read (its own last wait, or the other slot's, which the products in between came after), so a
+        // phase cannot be taken for the one before it
+        if (uses) dead = dead || !warp_wait(&out_free[(uses - 1) & 1], ((uses - 1) >> 1) & 1, abort_flag);
+#pragma unroll
+        for (int c = 0; c < DP / 32; ++c) {
+          tmem_ld_wait();
+          if (c + 1 < DP / 32) tmem_ld_32x32b_x16(tO + half * (DP / 2) + 16 * (c + 1), o[(c + 1) & 1]);
+          const int col = half * (DP / 2) + 16 * c;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            uint4 v;
+            uint32_t* vv = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              vv[e] = none ? 0u
+                           : pack2<T>(__uint_as_float(o[c & 1][8 * i + 2 * e]) * inv, __uint_as_float(o[c & 1][8 * i + 2 * e + 1]) * inv);
+            put_swizzled(sO + (col >> 6) * SUB_BYTES, row, ((col & 63) >> 3) + i, v);
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(out_full);
+      }
+      tc_fence_before();
+      uses += u.two ? 2 : 1;
     }
-    if (warp == 16 && lane == 0) bulk_wait_all();
   } else {
-    regs_dec<48>();
-    if (warp == 20) {
+    regs_dec<64>();
+    if (warp == 16) {
       // -------------------------------------------------------------------------------------- MMA issue
       constexpr uint32_t idQK = idesc_f16<T>(CT, CT, false), idPV = idesc_f16<T>(CT, DP, true);
       constexpr uint64_t TILE16 = C::TILE >> 4;
       const uint64_t dQ = desc_rows(smem_u32(sQ)), dK = desc_rows(smem_u32(sV) + C::TILE), dV = desc_chan(smem_u32(sV));
       int st = 0;
-      uint32_t kph = 0, qph[2] = {0, 0}, pph[2] = {0, 0}, oph[2] = {1, 1};
+      uint32_t kph = 0, qph[2] = {0, 0}, pph[2] = {0, 0};
       FwdUnit cur, nxt;
-      int64_t it = blockIdx.x;
+      int it = blockIdx.x;
       bool have = fwd_next(P, it, n_items, cur), ok = true;
       auto qk = [&](int slot, int kst, bool first, bool last) {  // S of a slot; its Q tile arrives with the unit's first
         if (first) {
@@ -408,11 +387,7 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
             if (s == 0 || cur.two) {
               if (!(ok = warp_wait(&p_full[s], pph[s], abort_flag))) break;
               pph[s] ^= 1;
-              if (t == cur.t0) {
-                if (!(ok = warp_wait(&o_empty[s], oph[s], abort_flag))) break;
-                oph[s] ^= 1;
-              }
-              tc_fence_after();
+              tc_fence_after();  // (a unit's first P comes after its threads have read the O before)
               mma_chan<false>(tmem + 2 * CT + s * CT, tmem + s * CT, dV + st * 2 * TILE16, idPV, t > cur.t0);
               if (last) commit_one(&o_full[s]);
             }
@@ -424,7 +399,7 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
         cur = nxt;
         have = more;
       }
-    } else if (warp == 21) {
+    } else if (warp == 17) {
       if (lane == 0) {
         // -------------------------------------------------------------------------------------- copies
         int st = 0, fills = 0, qfills[2] = {0, 0};
@@ -452,7 +427,7 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
           ++fills;
           if (++st == C::STAGES) st = 0, kph ^= 1;
         };
-        int64_t it = blockIdx.x;
+        int it = blockIdx.x;
         bool have = fwd_next(P, it, n_items, u);
         if (have) {
           load_kv(u, -1, u, u.t0);
@@ -461,6 +436,8 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
         }
         while (have && ok) {
           const bool more = fwd_next(P, it, n_items, nxt);
+          for (int s = 0; more && s < (nxt.two ? 2 : 1); ++s)
+            for (int p = 0; p < C::NSUB; ++p) tma_prefetch_5d(&tmQ, 64 * p, 0, nxt.hk, (nxt.tile0 + s) * P.nq, nxt.b);
           for (int t = u.t0; ok && t < u.t1; ++t) {
             const bool last = t == u.t1 - 1;
             if (!last) load_kv(u, t, u, t + 1);
@@ -479,14 +456,14 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
           if (qfills[s]) mbar_wait_drain(&q_full[s], static_cast<uint32_t>((qfills[s] - 1) & 1));
       }
       __syncwarp();
-    } else if (warp == 22 && masked) {
+    } else if (warp == 18 && masked) {
       // ---------------------------------------------------------------------------------------- rows of masked keys
       if (lane == 0) mbar_arrive(&v_clean[0]);  // the first stage holds a K tile only
       int st = 1;
       uint32_t kph = 0;
       FwdUnit u;
       bool ok = true;
-      for (int64_t it = blockIdx.x; ok && fwd_next(P, it, n_items, u);) {
+      for (int it = blockIdx.x; ok && fwd_next(P, it, n_items, u);) {
         const int64_t len = ca_len(P.kv_lens, u.b, P.Sk);
         for (int t = u.t0; ok && t < u.t1; ++t) {
           if (!(ok = warp_wait(&kv_full[st], kph, abort_flag))) break;
@@ -505,11 +482,48 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
           if (++st == C::STAGES) st = 0, kph ^= 1;
         }
       }
+    } else if (warp == 19) {
+      // ---------------------------------------------------------------------------------------- stores
+      uint32_t ph = 0, uses = 0;
+      bool ok = true;
+      for (int it = blockIdx.x; ok && it < n_items; it += gridDim.x) {
+        const FwdUnit u = fwd_unit(P, it);
+        for (int s = 0; ok && s < (u.two ? 2 : 1); ++s) {
+          const int64_t s0 = static_cast<int64_t>(u.tile0 + s) * P.nq;
+          if (u.t1 > u.t0) {
+            if (P.splits > 1) continue;
+            if (lane == 0 && (ok = mbar_wait(out_full, ph, abort_flag))) {
+              for (int p = 0; p < C::NSUB; ++p) tma_store_5d(sO + p * SUB_BYTES, &tmO, 64 * p, 0, u.hk, static_cast<int>(s0), u.b);
+              bulk_commit();
+              bulk_wait_read<0>();
+              mbar_arrive(&out_free[uses & 1]);
+            }
+            ok = __shfl_sync(0xffffffffu, ok, 0);
+            ph ^= 1;
+            ++uses;
+            continue;
+          }
+          for (int r = lane; r < P.nq * P.G; r += 32) {  // a unit without keys: zero rows
+            const int64_t q = s0 + r / P.G, h = u.hk * P.G + r % P.G;
+            if (q >= P.Sq) break;
+            const int64_t rid = (u.b * static_cast<int64_t>(P.Hq) + h) * P.Sq + q;
+            if (P.splits > 1) {
+              P.part_lse[u.split * static_cast<int64_t>(P.B) * P.Hq * P.Sq + rid] = -INFINITY;
+              continue;
+            }
+            if (P.lse) P.lse[rid] = -INFINITY;
+            T* dst = static_cast<T*>(P.o.ptr) + u.b * P.o.stride_b + q * P.o.stride_s + h * P.o.stride_h;
+            for (int c = 0; c < P.D; c += 8) *reinterpret_cast<uint4*>(dst + c) = make_uint4(0, 0, 0, 0);
+          }
+        }
+      }
+      if (lane == 0) bulk_wait_all();
+      __syncwarp();
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 20) {
+  if (warp == 16) {
     tc_fence_after();
     commit_one(done);  // every product issued (after a wait that gave up some may still run) and its arrivals are over
     mbar_wait_drain(done, 0);
@@ -578,6 +592,7 @@ static int fwd_launch_cfg(const CrossParams& P, cudaStream_t st) {
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   if (e != cudaSuccess) return cuda_fail(e, "cross_fwd_kernel shared memory");
   const int64_t items = static_cast<int64_t>(P.units) * P.splits * P.Hkv * P.B;
+  if (items >= (1 << 30)) return fail(H3B_ERR_UNSUPPORTED, "cross_attention: too many query tiles");
   const int grid = static_cast<int>(items < cross_sms() ? items : cross_sms());
   kern<<<grid, C::THREADS, C::SMEM, st>>>(q, k, v, o, P);
   rc = check_launch("cross_fwd_kernel");
