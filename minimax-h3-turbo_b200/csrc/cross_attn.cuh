@@ -18,6 +18,8 @@ static CrossWs cross_plan(CrossParams& P, int mask_kind, bool backward) {
   const int64_t heads = static_cast<int64_t>(P.Hkv) * P.B, key_tiles = P.Skp / CT;
   P.splits = backward ? bwd_splits(P.q_tiles * heads, key_tiles) : fwd_splits(P.units * heads, key_tiles);
   P.kv_splits = backward ? bwd_splits(key_tiles * heads, P.q_tiles) : 1;
+  P.by_g.set(P.G), P.by_hkv.set(P.Hkv), P.by_units.set(max(1, P.units)), P.by_splits.set(P.splits);
+  P.by_q_tiles.set(max(1, P.q_tiles)), P.by_k_tiles.set(max(1, static_cast<int>(key_tiles))), P.by_kv_splits.set(P.kv_splits);
   CrossWs w;
   auto take = [&](size_t bytes) {
     const size_t at = w.total;

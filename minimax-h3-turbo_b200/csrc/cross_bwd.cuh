@@ -19,44 +19,33 @@
 namespace h3b {
 
 struct BwdTile {
-  int64_t it;
-  int b, hk, split, tile, t0, t1, t;  // `tile`: the unit's own tile; t: the tile of the other side
+  int it, b, hk, split, tile, t0, t1, t;  // `tile`: the unit's own tile; t: the tile of the other side
   __device__ __forceinline__ bool first() const { return t == t0; }
   __device__ __forceinline__ bool last() const { return t == t1 - 1; }
 };
-
-// range [t0, t1) of n tiles that split `s` of `splits` gets
-__device__ __forceinline__ void split_range(int n, int splits, int s, int& t0, int& t1) {
-  const int per = (n + splits - 1) / splits;
-  t0 = min(s * per, n);
-  t1 = min(t0 + per, n);
-}
 
 // Walks the units of this CTA.  DQ: own tiles are query tiles, the other side key tiles; else the other way round.
 template <bool DQ>
 struct BwdWalk {
   const CrossParams& P;
-  int64_t n;
-  int own, splits;
+  int n, splits;
   BwdTile c;
   bool valid;
   __device__ __forceinline__ BwdWalk(const CrossParams& p) : P(p) {
-    own = DQ ? p.q_tiles : static_cast<int>(p.Skp / CT);
     splits = DQ ? p.splits : p.kv_splits;
-    n = static_cast<int64_t>(own) * splits * p.Hkv * p.B;
+    n = (DQ ? p.q_tiles : static_cast<int>(p.Skp / CT)) * splits * p.Hkv * p.B;
     c.it = blockIdx.x;
     seek();
   }
-  __device__ __forceinline__ void unit(int64_t it, BwdTile& u) const {
-    u.tile = static_cast<int>(it % own);
-    int64_t r = it / own;
-    u.split = static_cast<int>(r % splits);
-    r /= splits;
-    u.hk = static_cast<int>(r % P.Hkv);
-    u.b = static_cast<int>(r / P.Hkv);
+  __device__ __forceinline__ void unit(int it, BwdTile& u) const {
+    const FastDiv &by_own = DQ ? P.by_q_tiles : P.by_k_tiles, &by_split = DQ ? P.by_splits : P.by_kv_splits;
+    const int r = by_split.divmod(by_own.divmod(it, u.tile), u.split);
+    u.b = P.by_hkv.divmod(r, u.hk);
     const int64_t len = ca_len(P.kv_lens, u.b, P.Sk);
     const int other = DQ ? static_cast<int>((len + CT - 1) / CT) : static_cast<int64_t>(u.tile) * CT < len ? P.q_tiles : 0;
-    split_range(other, splits, u.split, u.t0, u.t1);
+    const int per = by_split.div(other + splits - 1);
+    u.t0 = min(u.split * per, other);
+    u.t1 = min(u.t0 + per, other);
     u.t = u.t0;
   }
   __device__ __forceinline__ void seek() {  // the first unit from c.it on with work
@@ -159,7 +148,7 @@ __global__ void __launch_bounds__(512, 1)
   if (warp < 8) {
     // ------------------------------------------------------------------------------------------ P, dS
     regs_inc<176>();
-    const int half = warp >> 2, row = threadIdx.x & (CT - 1), qr = row / P.G, hg = row - qr * P.G;
+    const int half = warp >> 2, row = threadIdx.x & (CT - 1), qr = P.by_g.div(row), hg = row - qr * P.G;
     const uint32_t at = (static_cast<uint32_t>(warp & 3) << 21) + half * 64;  // this warp's lanes and columns
     uint32_t sph = 0, dph = 0, gph = 0, xph = 0, sbuf = 0;
     float nlse2 = -INFINITY, delta = 0.f;
@@ -285,13 +274,13 @@ __global__ void __launch_bounds__(512, 1)
   } else if (warp < 12) {
     // ------------------------------------------------------------------------------------------ epilogue
     regs_dec<96>();
-    const int row = threadIdx.x & (CT - 1), qr = row / P.G, hg = row - qr * P.G;
+    const int row = threadIdx.x & (CT - 1), qr = P.by_g.div(row), hg = row - qr * P.G;
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
     uint32_t ph = 0;
     BwdWalk<true> w(P);
     BwdTile u;
     bool ok = true;
-    for (int64_t it = blockIdx.x; ok && it < w.n; it += gridDim.x) {
+    for (int it = blockIdx.x; ok && it < w.n; it += gridDim.x) {
       w.unit(it, u);
       const int64_t s = static_cast<int64_t>(u.tile) * P.nq + qr;
       const bool valid = qr < P.nq && s < P.Sq, any = u.t1 > u.t0;
@@ -645,7 +634,7 @@ __global__ void __launch_bounds__(512, 1)
     BwdTile u;
     bool ok = true;
     const int64_t part = static_cast<int64_t>(P.B) * P.Hkv * P.Sk * P.D;  // elements of one split's dK or dV
-    for (int64_t it = blockIdx.x; ok && it < w.n; it += gridDim.x) {
+    for (int it = blockIdx.x; ok && it < w.n; it += gridDim.x) {
       w.unit(it, u);
       const int64_t key = static_cast<int64_t>(u.tile) * CT + row;
       const bool valid = key < P.Sk, any = u.t1 > u.t0;
@@ -867,6 +856,7 @@ static int bwd_launch_cfg(const CrossParams& P, cudaStream_t st) {
   if (e != cudaSuccess) return cuda_fail(e, "cross_attention_backward shared memory");
   if (P.Sq > 0) {
     const int64_t n = static_cast<int64_t>(P.q_tiles) * P.splits * P.Hkv * P.B, rows = static_cast<int64_t>(P.B) * P.Hq * P.Sq;
+    if (n >= (1 << 30)) return fail(H3B_ERR_UNSUPPORTED, "cross_attention_backward: too many query tiles");
     kq<<<static_cast<int>(n < sms ? n : sms), 512, C::SMEM, st>>>(q, g, k, v, P);
     rc = check_launch("cross_dq_kernel");
     if (!rc && P.splits > 1) rc = join_launch<T>(P.part_dq, rows * P.D, P.splits, rows, P.D, P.Sq, P.Hq, P.dq, st);
@@ -874,6 +864,7 @@ static int bwd_launch_cfg(const CrossParams& P, cudaStream_t st) {
   }
   if (P.Sk > 0) {
     const int64_t n = P.Skp / CT * P.kv_splits * P.Hkv * P.B, rows = static_cast<int64_t>(P.B) * P.Hkv * P.Sk;
+    if (n >= (1 << 30)) return fail(H3B_ERR_UNSUPPORTED, "cross_attention_backward: too many key tiles");
     kkv<<<static_cast<int>(n < sms ? n : sms), 512, C::SMEM, st>>>(q, g, k, v, P);
     rc = check_launch("cross_dkv_kernel");
     if (!rc && P.kv_splits > 1) {

@@ -23,6 +23,27 @@ namespace h3b {
 constexpr int CT = 128;  // rows of a query tile, keys of a key tile
 constexpr float CA_LOG2E = 1.4426950408889634f, CA_LN2 = 0.6931471805599453f;
 
+// n / d and n % d for 0 <= n < 2^31 by one multiplication (a division by a number the compiler does not know takes some
+// dozens of instructions, on the path of every warp at every unit): q = (hi(n m) + n) >> l with l = ceil(log2 d),
+// m = floor(2^32 (2^l - d) / d) + 1.
+struct FastDiv {
+  uint32_t d, m, l;
+  __host__ void set(uint32_t v) {
+    d = v;
+    for (l = 0; l < 31 && (1u << l) < v; ++l) {
+    }
+    m = static_cast<uint32_t>((static_cast<uint64_t>(1) << 32) * ((static_cast<uint64_t>(1) << l) - v) / v + 1);
+  }
+  __device__ __forceinline__ int div(int n) const {
+    return static_cast<int>((__umulhi(static_cast<uint32_t>(n), m) + static_cast<uint32_t>(n)) >> l);
+  }
+  __device__ __forceinline__ int divmod(int n, int& rem) const {
+    const int q = div(n);
+    rem = n - q * static_cast<int>(d);
+    return q;
+  }
+};
+
 struct CrossParams {
   h3b_attn_tensor q, k, v, o, go, dq, dk, dv;
   float* lse;              // [B, Hq, Sq]
@@ -39,6 +60,7 @@ struct CrossParams {
   int splits;          // key splits of a unit (forward, dQ)
   int kv_splits;       // query splits of a unit (dK, dV)
   float scale, scale2;         // scale2 = scale log2(e)
+  FastDiv by_g, by_hkv, by_units, by_splits, by_q_tiles, by_k_tiles, by_kv_splits;
 };
 
 __device__ __forceinline__ int64_t ca_len(const int32_t* lens, int b, int64_t Sk) {
@@ -67,18 +89,15 @@ __device__ __forceinline__ void tma_store_5d(const void* src, const CUtensorMap*
                "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
                : "memory");
 }
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 // bring a tile into L2
 __device__ __forceinline__ void tma_prefetch_5d(const CUtensorMap* map, int c0, int c1, int c2, int c3, int c4) {
   asm volatile("cp.async.bulk.prefetch.tensor.5d.L2.global [%0, {%1, %2, %3, %4, %5}];" ::"l"(map), "r"(c0), "r"(c1), "r"(c2),
                "r"(c3), "r"(c4)
                : "memory");
 }
-__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void bulk_wait_read() {
-  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
                "l"(src), "r"(bytes), "r"(smem_u32(bar))

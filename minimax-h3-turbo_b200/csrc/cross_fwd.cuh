@@ -38,21 +38,17 @@ struct FwdUnit {
   bool two;                         // the second query tile exists
 };
 
-__device__ __forceinline__ FwdUnit fwd_unit(const CrossParams& P, int it) {  // (32-bit divisions: 64-bit ones cost ~2000 cycles)
+__device__ __forceinline__ FwdUnit fwd_unit(const CrossParams& P, int it) {
   FwdUnit u;
-  unsigned r = static_cast<unsigned>(it);
-  const int pair = static_cast<int>(r % P.units);
-  r /= P.units;
-  u.split = static_cast<int>(r % P.splits);
-  r /= P.splits;
-  u.hk = static_cast<int>(r % P.Hkv);
-  u.b = static_cast<int>(r / P.Hkv);
+  int pair;
+  const int r = P.by_splits.divmod(P.by_units.divmod(it, pair), u.split);
+  u.b = P.by_hkv.divmod(r, u.hk);
   u.tile0 = pair * 2;
   u.two = u.tile0 + 1 < P.q_tiles;
-  const unsigned nt = static_cast<unsigned>(ca_len(P.kv_lens, u.b, P.Sk) + CT - 1) / CT;
-  const unsigned per = (nt + P.splits - 1) / P.splits;
-  u.t0 = static_cast<int>(min(u.split * per, nt));
-  u.t1 = static_cast<int>(min(u.t0 + per, nt));
+  const int nt = static_cast<int>((ca_len(P.kv_lens, u.b, P.Sk) + CT - 1) / CT);
+  const int per = P.by_splits.div(nt + P.splits - 1);
+  u.t0 = min(u.split * per, nt);
+  u.t1 = min(u.t0 + per, nt);
   return u;
 }
 // the next unit with key tiles
@@ -108,21 +104,33 @@ __device__ __forceinline__ void soft_chunk(const uint32_t (&r)[16], float scale2
     }
   }
 }
-// the largest s scale2 (+ bias) of 16 scores
+// the largest of 32 scores (MASK 2: of s scale2 + bias).  Runs once a unit: from a cold instruction cache, at some nine cycles
+// per instruction, so it is kept short (two scores per maximum, the scale once at the end).
 template <int MASK>
-__device__ __forceinline__ float max_chunk(const uint32_t (&r)[16], float scale2, int lim, const float4* b4, float top) {
+__device__ __forceinline__ float max_chunk(const uint32_t (&r)[32], float scale2, int lim, const float4* b4, float top) {
+  float tp[2] = {top, -INFINITY};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float4 bb = make_float4(0.f, 0.f, 0.f, 0.f);
-    if constexpr (MASK == 2) bb = __ldg(b4 + i);
-    const float bv[4] = {bb.x, bb.y, bb.z, bb.w};
+  for (int i = 0; i < 8; ++i) {
+    float x[4];
+    if constexpr (MASK == 2) {
+      const float4 bb = __ldg(b4 + i);
+      const float bv[4] = {bb.x, bb.y, bb.z, bb.w};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float x = fmaf(__uint_as_float(r[4 * i + e]), scale2, bv[e]);
-      if (MASK == 0 || (MASK == 1 ? 4 * i + e < lim : bv[e] != -INFINITY)) top = fmaxf(top, x);
+      for (int e = 0; e < 4; ++e) {
+        x[e] = fmaf(__uint_as_float(r[4 * i + e]), scale2, bv[e]);
+        if (bv[e] == -INFINITY) x[e] = -INFINITY;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[e] = __uint_as_float(r[4 * i + e]);
+        if (MASK == 1 && 4 * i + e >= lim) x[e] = -INFINITY;
+      }
     }
+    tp[0] = fmaxf(tp[0], fmaxf(x[0], x[1]));
+    tp[1] = fmaxf(tp[1], fmaxf(x[2], x[3]));
   }
-  return top;
+  return fmaxf(tp[0], tp[1]);
 }
 
 template <typename T, int DP, bool BIAS>
@@ -196,14 +204,17 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
     const int bar = 1 + slot * 4 + (warp & 3);  // the two warps of the same 32 rows
     float* mine = halves + (slot * 2 + half) * CT + row;
     const float* other = halves + (slot * 2 + 1 - half) * CT + row;
-    const int qr = row / P.G, hg = row - qr * P.G;
+    int hg;
+    const int qr = P.by_g.divmod(row, hg);
     const int64_t rows = static_cast<int64_t>(P.B) * P.Hq * P.Sq;
     uint32_t sph = 0, oph = 0, uses = slot;  // uses: of the staging by both slots before this one
     bool dead = false;
-    FwdUnit u;
-    for (int it = blockIdx.x; fwd_next(P, it, n_items, u);) {
+    FwdUnit u, nxt;
+    int it = blockIdx.x;
+    for (bool have = fwd_next(P, it, n_items, u), more; have; u = nxt, have = more) {
       if (slot == 1 && !u.two) {
         ++uses;
+        more = fwd_next(P, it, n_items, nxt);
         continue;
       }
       const int64_t len = ca_len(P.kv_lens, u.b, P.Sk);
@@ -220,19 +231,23 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
         f32x2 sum[2];
         for (bool exact = t == u.t0;; exact = true) {
           if (exact) {
-            float top = m;
-#pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              uint32_t r[16];
-              tmem_ld_32x32b_x16(tS + half * 64 + 16 * c, r);
+            float top = -INFINITY;
+            {
+              uint32_t r[2][32];
+              tmem_ld_32x32b_x32(tS + half * 64, r[0]);
+              tmem_ld_32x32b_x32(tS + half * 64 + 32, r[1]);
               tmem_ld_wait();
-              if constexpr (BIAS) top = max_chunk<2>(r, P.scale2, 0, b4 + 4 * c, top);
-              else if (lim < 64) top = max_chunk<1>(r, P.scale2, lim - 16 * c, nullptr, top);
-              else top = max_chunk<0>(r, P.scale2, 0, nullptr, top);
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                if constexpr (BIAS) top = max_chunk<2>(r[c], P.scale2, 0, b4 + 8 * c, top);
+                else if (lim < 64) top = max_chunk<1>(r[c], P.scale2, lim - 32 * c, nullptr, top);
+                else top = max_chunk<0>(r[c], P.scale2, 0, nullptr, top);
+              }
             }
             *mine = top;
             group_sync(bar, 64);  // (both have read by the barrier after the probabilities)
             top = fmaxf(top, *other);
+            top = fmaxf(m, BIAS ? top : top * P.scale2);
             if (t > u.t0) {  // the product of the tile before is complete: its commit came before that of these scores
               const float f = top == -INFINITY ? 1.f : ex2(m - top);
               float la, lb;
@@ -274,6 +289,7 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[slot]);
+        if (t == u.t0) more = fwd_next(P, it, n_items, nxt);  // while the next scores are on their way
       }
       // ---- the unit's output
       float la, lb;
@@ -281,7 +297,6 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
       *mine = la + lb;
       group_sync(bar, 64);
       const float total = halves[slot * 2 * CT + row] + halves[(slot * 2 + 1) * CT + row];
-      group_sync(bar, 64);  // both have read before the next unit's maxima
       const bool none = total == 0.f;  // no key took part: zero, whatever the products hold
       const float inv = none ? 0.f : 1.f / total;
       const int64_t s = static_cast<int64_t>(u.tile0 + slot) * P.nq + qr;
@@ -313,26 +328,30 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
                                      __uint_as_float(o[4 * i + 2]) * inv, __uint_as_float(o[4 * i + 3]) * inv);
         }
       } else {
-        uint32_t o[2][16];
-        tmem_ld_32x32b_x16(tO + half * (DP / 2), o[0]);
         // the use before this one (uses - 1) has left the staging.  Two barriers in turn: a slot gets here only after the use
         // three before was read (its own last wait, or the other slot's, which the products in between came after), so a
         // phase cannot be taken for the one before it
         if (uses) dead = dead || !warp_wait(&out_free[(uses - 1) & 1], ((uses - 1) >> 1) & 1, abort_flag);
-#pragma unroll
-        for (int c = 0; c < DP / 32; ++c) {
+        const f32x2 inv2 = f2(inv, inv);
+#pragma unroll 1
+        for (int c = 0; c < DP / 64; ++c) {  // (a loop: see max_chunk)
+          const int col = half * (DP / 2) + 32 * c;
+          uint32_t o[32];
+          tmem_ld_32x32b_x32(tO + col, o);
           tmem_ld_wait();
-          if (c + 1 < DP / 32) tmem_ld_32x32b_x16(tO + half * (DP / 2) + 16 * (c + 1), o[(c + 1) & 1]);
-          const int col = half * (DP / 2) + 16 * c;
+          unsigned char* part = sO + (col >> 6) * SUB_BYTES;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
+          for (int i = 0; i < 4; ++i) {
             uint4 v;
             uint32_t* vv = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              vv[e] = none ? 0u
-                           : pack2<T>(__uint_as_float(o[c & 1][8 * i + 2 * e]) * inv, __uint_as_float(o[c & 1][8 * i + 2 * e + 1]) * inv);
-            put_swizzled(sO + (col >> 6) * SUB_BYTES, row, ((col & 63) >> 3) + i, v);
+            for (int e = 0; e < 4; ++e) {
+              float oa, ob;
+              f2_split(f2_fma(f2(__uint_as_float(o[8 * i + 2 * e]), __uint_as_float(o[8 * i + 2 * e + 1])), inv2, f2(0.f, 0.f)), oa, ob);
+              vv[e] = pack2<T>(oa, ob);
+            }
+            if (none) v = make_uint4(0, 0, 0, 0);
+            put_swizzled(part, row, ((col & 63) >> 3) + i, v);
           }
         }
         fence_proxy_async_smem();
@@ -340,6 +359,7 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
         if (lane == 0) mbar_arrive(out_full);
       }
       tc_fence_before();
+      group_sync(bar, 64);  // both have read the sums before the next unit's maxima
       uses += u.two ? 2 : 1;
     }
   } else {
@@ -495,7 +515,7 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
             if (lane == 0 && (ok = mbar_wait(out_full, ph, abort_flag))) {
               for (int p = 0; p < C::NSUB; ++p) tma_store_5d(sO + p * SUB_BYTES, &tmO, 64 * p, 0, u.hk, static_cast<int>(s0), u.b);
               bulk_commit();
-              bulk_wait_read<0>();
+              bulk_wait_read();
               mbar_arrive(&out_free[uses & 1]);
             }
             ok = __shfl_sync(0xffffffffu, ok, 0);
