@@ -147,7 +147,7 @@ typedef struct h3b_rope_operand {
   void* y;
   const void* pos;
   int64_t S, x_stride_b, x_stride_s, x_stride_h, y_stride_b, y_stride_s, y_stride_h, pos_stride_b, pos_stride_s;
-  int32_t heads;
+  int64_t heads;
 } h3b_rope_operand;
 int h3b_rope_axes(const h3b_rope_operand* q, const h3b_rope_operand* k, int x_dtype, int64_t B, int head_dim,
                   const float* inv_freq, const int32_t* sections, int n_axes, int pos_dtype, int pairing, int inverse,

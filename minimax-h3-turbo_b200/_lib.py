@@ -36,22 +36,8 @@ _load_error: Optional[str] = None
 
 _c_void_p, _i64, _int, _sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t
 
-
-class RopeOperand(ctypes.Structure):
-    """struct h3b_rope_operand"""
-
-    _fields_ = [("x", _c_void_p), ("y", _c_void_p), ("pos", _c_void_p),
-                *[(n, _i64) for n in ("S", "x_stride_b", "x_stride_s", "x_stride_h", "y_stride_b", "y_stride_s",
-                                      "y_stride_h", "pos_stride_b", "pos_stride_s")], ("heads", ctypes.c_int32)]
-
-
-class AttnTensor(ctypes.Structure):
-    """struct h3b_attn_tensor"""
-
-    _fields_ = [("ptr", _c_void_p), ("stride_b", _i64), ("stride_s", _i64), ("stride_h", _i64)]
-
-
-_rope_p, _attn_p = ctypes.POINTER(RopeOperand), ctypes.POINTER(AttnTensor)
+_rope_p = _c_void_p  # struct h3b_rope_operand: thirteen int64, the last one `heads`
+_attn_p = _c_void_p  # struct h3b_attn_tensor: four int64
 _SIGNATURES = {
     "h3b_version": ([], _int),
     "h3b_last_error": ([], ctypes.c_char_p),
@@ -166,6 +152,14 @@ def scale_code(dt: torch.dtype) -> int:
 
 def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # the handle alone, without a Stream object
+
+
+def raw_stream(index: int) -> int:
+    """The current stream's handle on device `index`."""
+    return _raw_stream(index) if _raw_stream else torch.cuda.current_stream(index).cuda_stream
 
 
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:

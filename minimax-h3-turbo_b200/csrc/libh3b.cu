@@ -266,7 +266,7 @@ int h3b_attn_merge(float* acc, float* acc_lse, const void* o, int64_t o_head_str
 
 static int check_rope_operand(const h3b_rope_operand* o, const char* name) {
   if (!o) return H3B_OK;
-  if (o->S < 0 || o->heads < 1) return fail(H3B_ERR_ARG, std::string("rope_axes: ") + name + " needs S >= 0 and heads >= 1");
+  if (o->S < 0 || o->heads < 1 || o->heads > (1 << 20)) return fail(H3B_ERR_ARG, std::string("rope_axes: ") + name + " needs S >= 0 and heads >= 1");
   if (o->S > 0 && (!o->x || !o->y || !o->pos)) return fail(H3B_ERR_ARG, std::string("rope_axes: ") + name + ": null tensor");
   return H3B_OK;
 }

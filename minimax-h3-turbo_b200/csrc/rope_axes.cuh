@@ -225,7 +225,7 @@ int rope_axes_launch(const h3b_rope_operand* q, const h3b_rope_operand* k, int x
     if (!o) continue;
     sd = RopeSide{static_cast<const char*>(o->x), static_cast<char*>(o->y), static_cast<const char*>(o->pos),
                   o->x_stride_b, o->x_stride_s, o->x_stride_h, o->y_stride_b, o->y_stride_s, o->y_stride_h,
-                  o->pos_stride_b, o->pos_stride_s, o->S, 0, o->heads};
+                  o->pos_stride_b, o->pos_stride_s, o->S, 0, static_cast<int>(o->heads)};
     for (int64_t v : {sd.xb, sd.xs, sd.xh, sd.yb, sd.ys, sd.yh}) vec = vec && v % vw == 0;
     vec = vec && reinterpret_cast<uintptr_t>(sd.x) % 16 == 0 && reinterpret_cast<uintptr_t>(sd.y) % 16 == 0;
   }

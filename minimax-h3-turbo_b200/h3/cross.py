@@ -11,114 +11,136 @@ from __future__ import annotations
 
 import ctypes
 import math
-from contextlib import nullcontext
 from typing import Optional, Tuple
 
 import torch
 
 from .. import _lib
 
-_DTYPES = (torch.bfloat16, torch.float16)
+_CODES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16}
+_Args8 = ctypes.c_int64 * 32  # up to eight struct h3b_attn_tensor {ptr, stride_b, stride_s, stride_h}
 
 
 def _guard(dev: torch.device):
     """The kernels launch on the current device: make it the tensors'."""
-    return nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+    return torch.cuda.device(dev)
 
 
 def _batched(t: torch.Tensor, name: str) -> torch.Tensor:
-    if t.dim() not in (3, 4):
+    if t.dim() == 4:
+        return t
+    if t.dim() != 3:
         raise ValueError(f"{name} must be [B, S, heads, D] or [S, heads, D], got {tuple(t.shape)}")
-    return t if t.dim() == 4 else t.unsqueeze(0)
+    return t.unsqueeze(0)
 
 
 def _readable(t: torch.Tensor) -> torch.Tensor:
     """t itself when the kernels can read it in place: channels contiguous, 16-byte aligned base and strides."""
-    st = t.stride()
-    ok = t.data_ptr() % 16 == 0 and (st[3] == 1 or t.shape[3] == 1)
-    for n, s in zip(t.shape[:3], st[:3]):
-        ok = ok and (n <= 1 or (s > 0 and s % 8 == 0))
-    if ok:
+    if t.is_contiguous():
+        ok = t.shape[3] % 8 == 0
+    else:
+        st = t.stride()
+        ok = st[3] == 1 or t.shape[3] == 1
+        for n, s in zip(t.shape[:3], st[:3]):
+            ok = ok and (n <= 1 or (s > 0 and s % 8 == 0))
+    if ok and t.data_ptr() % 16 == 0:
         return t
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _arg(t: torch.Tensor) -> _lib.AttnTensor:
+def _arg(t: torch.Tensor):
+    """(pointer, strides of batch, token and head) of a [B, S, heads, D] tensor; 0 for an extent of one."""
     (b, s, h, _), (sb, ss, sh, _) = t.shape, t.stride()
-    return _lib.AttnTensor(t.data_ptr(), sb if b > 1 else 0, ss if s > 1 else 0, sh if h > 1 else 0)
+    return t.data_ptr(), sb if b > 1 else 0, ss if s > 1 else 0, sh if h > 1 else 0
 
 
 class _Problem:
     """Checked sizes and arguments of one call, forward or backward."""
 
+    __slots__ = ("b", "sq", "sk", "hq", "hkv", "d", "scale", "q", "k", "v", "dev", "lens", "mask", "kind", "ldm", "code")
+
     def __init__(self, q, k, v, kv_lens, key_mask, scale):
         q, k, v = _batched(q, "q"), _batched(k, "k"), _batched(v, "v")
-        dev = q.device
         if not (q.is_cuda and k.is_cuda and v.is_cuda):
             raise RuntimeError("cross_attention: CUDA tensors only (there is no CPU path)")
-        if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+        dt = q.dtype
+        code = _CODES.get(dt)
+        if code is None or k.dtype != dt or v.dtype != dt:
             raise RuntimeError(f"cross_attention: q, k and v must be bf16 or fp16, all of one type, got {q.dtype}, {k.dtype}, "
                                f"{v.dtype} (there is no fp32 path)")
+        dev = q.device
         if k.device != dev or v.device != dev:
             raise ValueError("cross_attention: q, k and v must be on one device")
-        self.b, self.sq, self.hq, self.d = q.shape
-        self.sk, self.hkv = k.shape[1], k.shape[2]
-        if k.shape != v.shape or k.shape[0] != self.b or k.shape[3] != self.d:
-            raise ValueError(f"cross_attention: k and v must be [{self.b}, Sk, heads, {self.d}] alike, got {tuple(k.shape)} "
-                             f"and {tuple(v.shape)}")
-        if self.hkv == 0 or self.hq == 0 or self.hq % self.hkv:
-            raise ValueError(f"cross_attention: {self.hq} query heads are not a multiple of {self.hkv} key heads")
-        self.scale = 1.0 / math.sqrt(self.d) if scale is None else float(scale)
-        self.q, self.k, self.v, self.dev = _readable(q), _readable(k), _readable(v), dev
+        b, self.sq, hq, d = q.shape
+        kb, sk, hkv, kd = k.shape
+        if k.shape != v.shape or kb != b or kd != d:
+            raise ValueError(f"cross_attention: k and v must be [{b}, Sk, heads, {d}] alike, got {tuple(k.shape)} and "
+                             f"{tuple(v.shape)}")
+        if hkv == 0 or hq == 0 or hq % hkv:
+            raise ValueError(f"cross_attention: {hq} query heads are not a multiple of {hkv} key heads")
+        self.b, self.sk, self.hq, self.hkv, self.d, self.code, self.dev = b, sk, hq, hkv, d, code, dev
+        self.scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+        self.q, self.k, self.v = _readable(q), _readable(k), _readable(v)
         self.lens = self.mask = None
         self.kind, self.ldm = _lib.MASK_NONE, 0
         if kv_lens is not None:
-            if tuple(kv_lens.shape) != (self.b,) or kv_lens.dtype not in (torch.int32, torch.int64) or kv_lens.device != dev:
-                raise ValueError(f"cross_attention: kv_lens must be int32 or int64 [{self.b}] on {dev}")
+            if tuple(kv_lens.shape) != (b,) or kv_lens.dtype not in (torch.int32, torch.int64) or kv_lens.device != dev:
+                raise ValueError(f"cross_attention: kv_lens must be int32 or int64 [{b}] on {dev}")
             self.lens = kv_lens.to(torch.int32).contiguous()
         if key_mask is not None:
-            if key_mask.dim() != 2 or key_mask.shape[1] != self.sk or key_mask.shape[0] not in (1, self.b) or key_mask.device != dev:
-                raise ValueError(f"cross_attention: key_mask must be [{self.b}, {self.sk}] (or [1, {self.sk}]) on {dev}, got "
-                                 f"{tuple(key_mask.shape)} on {key_mask.device}")
-            if key_mask.requires_grad and torch.is_grad_enabled():
-                raise ValueError("cross_attention: key_mask has no gradient; detach it")
-            if key_mask.dtype == torch.bool:
-                self.kind = _lib.MASK_BOOL
-            elif key_mask.is_floating_point():
-                self.kind, key_mask = _lib.MASK_BIAS, key_mask.detach().float()
-            else:
-                raise ValueError(f"cross_attention: key_mask must be bool or floating point, got {key_mask.dtype}")
-            self.mask = key_mask if key_mask.stride(1) == 1 or self.sk == 1 else key_mask.contiguous()
-            self.ldm = self.mask.stride(0) if self.mask.shape[0] > 1 else 0
+            self._set_mask(key_mask)
 
-    def rows(self, t: torch.Tensor, name: str, like: torch.Tensor) -> torch.Tensor:
+    def _set_mask(self, m):
+        if m.dim() != 2 or m.shape[1] != self.sk or m.shape[0] not in (1, self.b) or m.device != self.dev:
+            raise ValueError(f"cross_attention: key_mask must be [{self.b}, {self.sk}] (or [1, {self.sk}]) on {self.dev}, got "
+                             f"{tuple(m.shape)} on {m.device}")
+        if m.requires_grad and torch.is_grad_enabled():
+            raise ValueError("cross_attention: key_mask has no gradient; detach it")
+        if m.dtype == torch.bool:
+            self.kind = _lib.MASK_BOOL
+        elif m.is_floating_point():
+            self.kind = _lib.MASK_BIAS
+            if m.dtype != torch.float32:
+                m = m.detach().float()
+        else:
+            raise ValueError(f"cross_attention: key_mask must be bool or floating point, got {m.dtype}")
+        self.mask = m if m.stride(1) == 1 or self.sk == 1 else m.contiguous()
+        self.ldm = self.mask.stride(0) if self.mask.shape[0] > 1 else 0
+
+    def rows(self, t: torch.Tensor, name: str) -> torch.Tensor:
         t = _batched(t, name)
-        if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
-            raise ValueError(f"cross_attention: {name} must be {tuple(like.shape)} {like.dtype} on {like.device}, got "
+        if t.shape != self.q.shape or t.dtype != self.q.dtype or t.device != self.dev:
+            raise ValueError(f"cross_attention: {name} must be {tuple(self.q.shape)} {self.q.dtype} on {self.dev}, got "
                              f"{tuple(t.shape)} {t.dtype} on {t.device}")
         return t
 
-    def sizes(self):
-        return self.b, self.sq, self.sk, self.hq, self.hkv, self.d
-
-    def workspace(self, backward: bool) -> Tuple[Optional[torch.Tensor], int]:
-        n = _lib.lib().h3b_cross_attention_workspace_bytes(*self.sizes(), self.kind, int(backward))
-        return (torch.empty(n, dtype=torch.uint8, device=self.dev) if n else None), n
-
-    def tail(self):
-        return (_lib.act_code(self.q.dtype), *self.sizes(), self.scale, _lib.ptr(self.lens), _lib.ptr(self.mask), self.kind,
-                self.ldm)
+    def call(self, entry: str, tensors, lse: Optional[torch.Tensor], backward: bool) -> None:
+        """Workspace, arguments and the call of one entry point; `tensors` in its order (lse after the fifth, backward)."""
+        lib = _lib.lib()
+        sizes = (self.b, self.sq, self.sk, self.hq, self.hkv, self.d)
+        n = lib.h3b_cross_attention_workspace_bytes(*sizes, self.kind, backward)
+        ws = torch.empty(n, dtype=torch.uint8, device=self.dev) if n else None
+        arr = _Args8(*[x for t in tensors for x in _arg(t)])
+        at = ctypes.addressof(arr)
+        ts = [at + 32 * i for i in range(len(tensors))]
+        mid = (self.code, *sizes, self.scale, _lib.ptr(self.lens), _lib.ptr(self.mask), self.kind, self.ldm)
+        tail = (_lib.ptr(ws), n, _lib.raw_stream(self.dev.index))
+        if backward:
+            rc = lib.h3b_cross_attention_backward(*ts[:5], lse.data_ptr(), *ts[5:], *mid, *tail)
+        else:
+            rc = lib.h3b_cross_attention(*ts, *mid, _lib.ptr(lse), *tail)
+        _lib.check(rc, entry)
 
 
 def _forward(p: _Problem, want_lse: bool, out: Optional[torch.Tensor]):
-    with _guard(p.dev):
-        o = torch.empty(p.b, p.sq, p.hq, p.d, dtype=p.q.dtype, device=p.dev) if out is None else out
-        lse = torch.empty(p.b, p.hq, p.sq, dtype=torch.float32, device=p.dev) if want_lse else None
-        ws, n = p.workspace(False)
-        ref = ctypes.byref
-        _lib.check(_lib.lib().h3b_cross_attention(ref(_arg(p.q)), ref(_arg(p.k)), ref(_arg(p.v)), ref(_arg(o)), *p.tail(),
-                                                  _lib.ptr(lse), _lib.ptr(ws), n, _lib.stream_ptr(p.dev)), "cross_attention")
+    o = torch.empty(p.b, p.sq, p.hq, p.d, dtype=p.q.dtype, device=p.dev) if out is None else out
+    lse = torch.empty(p.b, p.hq, p.sq, dtype=torch.float32, device=p.dev) if want_lse else None
+    if p.dev.index == torch.cuda.current_device():
+        p.call("cross_attention", (p.q, p.k, p.v, o), lse, False)
+    else:
+        with _guard(p.dev):
+            p.call("cross_attention", (p.q, p.k, p.v, o), lse, False)
     return o, lse
 
 
@@ -159,11 +181,14 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_len
         o, lse = _CrossAttention.apply(q, k, v, kv_lens, key_mask, scale)
         return (o, lse) if return_lse else o
     p = _Problem(q, k, v, kv_lens, key_mask, scale)
-    if out is not None and _readable(p.rows(out, "out", p.q)).data_ptr() != _batched(out, "out").data_ptr():
+    if out is not None and _readable(p.rows(out, "out")).data_ptr() != _batched(out, "out").data_ptr():
         raise ValueError("cross_attention: out needs contiguous channels, a 16-byte aligned base and strides that are "
                          "multiples of 8 elements")
     o, lse = _forward(p, return_lse, None if out is None else _batched(out, "out"))
-    o = out if out is not None else o.view(q.shape)
+    if out is not None:
+        o = out
+    elif q.dim() == 3:
+        o = o.view(q.shape)
     return (o, lse) if return_lse else o
 
 
@@ -176,16 +201,17 @@ def cross_attention_backward(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
     cross_attention(..., return_lse=True) gave them for the same arguments.  The heads that share a key head add up in dk
     and dv; keys that are left out get zeros.  The same call gives the same bits."""
     p = _Problem(q, k, v, kv_lens, None if key_mask is None else key_mask.detach(), scale)
-    do_, o_ = _readable(p.rows(do, "do", p.q)), _readable(p.rows(o, "o", p.q))
+    do_, o_ = _readable(p.rows(do, "do")), _readable(p.rows(o, "o"))
     if tuple(lse.shape) != (p.b, p.hq, p.sq) or lse.dtype != torch.float32 or lse.device != p.dev:
         raise ValueError(f"cross_attention: lse must be fp32 {(p.b, p.hq, p.sq)} on {p.dev}")
-    with _guard(p.dev):
-        lse = lse.contiguous()
-        dq = torch.empty(p.b, p.sq, p.hq, p.d, dtype=p.q.dtype, device=p.dev)
-        dk, dv = (torch.empty(p.b, p.sk, p.hkv, p.d, dtype=p.q.dtype, device=p.dev) for _ in range(2))
-        ws, n = p.workspace(True)
-        ref = ctypes.byref
-        _lib.check(_lib.lib().h3b_cross_attention_backward(
-            ref(_arg(do_)), ref(_arg(p.q)), ref(_arg(p.k)), ref(_arg(p.v)), ref(_arg(o_)), lse.data_ptr(), ref(_arg(dq)),
-            ref(_arg(dk)), ref(_arg(dv)), *p.tail(), _lib.ptr(ws), n, _lib.stream_ptr(p.dev)), "cross_attention_backward")
+    lse = lse.contiguous()
+    dq = torch.empty(p.b, p.sq, p.hq, p.d, dtype=p.q.dtype, device=p.dev)
+    dk = torch.empty(p.b, p.sk, p.hkv, p.d, dtype=p.q.dtype, device=p.dev)
+    dv = torch.empty_like(dk)
+    tensors = (do_, p.q, p.k, p.v, o_, dq, dk, dv)
+    if p.dev.index == torch.cuda.current_device():
+        p.call("cross_attention_backward", tensors, lse, True)
+    else:
+        with _guard(p.dev):
+            p.call("cross_attention_backward", tensors, lse, True)
     return dq.view(q.shape), dk.view(k.shape), dv.view(v.shape)

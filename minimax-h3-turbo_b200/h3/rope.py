@@ -73,11 +73,17 @@ def norm_rope_(q: torch.Tensor, k: torch.Tensor, wq: torch.Tensor, wk: torch.Ten
 _POS_CODES = {torch.float32: _lib.FP32, torch.int32: _lib.INT32, torch.int64: _lib.INT64}
 
 
-def _rope_operand(x: torch.Tensor, pos: torch.Tensor, axes: int, name: str):
+_RopeArg = ctypes.c_int64 * 13  # struct h3b_rope_operand
+
+
+def _rope_operand(x: torch.Tensor, pos: Optional[torch.Tensor], axes: int, name: str):
     """(struct, output, tensors to keep) of one side, x [B, S, heads, D] or [S, heads, D]."""
-    if x.dim() not in (3, 4):
+    if x.dim() == 4:
+        x4 = x
+    elif x.dim() == 3:
+        x4 = x.unsqueeze(0)
+    else:
         raise ValueError(f"{name} must be [B, S, heads, D] or [S, heads, D], got {tuple(x.shape)}")
-    x4 = x if x.dim() == 4 else x.unsqueeze(0)
     b, s, h, d = x4.shape
     if pos is None or pos.device != x.device or pos.dtype not in _POS_CODES:
         raise ValueError(f"{name}: positions must be fp32, int32 or int64 on {x.device}")
@@ -85,48 +91,55 @@ def _rope_operand(x: torch.Tensor, pos: torch.Tensor, axes: int, name: str):
         pos = pos.unsqueeze(0)
     if pos.dim() != 3 or pos.shape[0] not in (1, b) or pos.shape[1] != s or pos.shape[2] != axes:
         raise ValueError(f"{name}: positions must be [{s}, {axes}] or [{b}, {s}, {axes}], got {tuple(pos.shape)}")
-    if x4.stride(3) != 1 and d > 1:
+    sb, ss, sh, sd = x4.stride()
+    if sd != 1 and d > 1:
         x4 = x4.contiguous()
-    if pos.stride(2) != 1 and axes > 1:
+        sb, ss, sh, _ = x4.stride()
+    pb, ps, pa = pos.stride()
+    if pa != 1 and axes > 1:
         pos = pos.contiguous()
-    y = torch.empty(b, s, h, d, dtype=x.dtype, device=x.device)
-    st = tuple(v if n > 1 else 0 for n, v in zip(x4.shape, x4.stride()))
-    op = _lib.RopeOperand(x4.data_ptr(), y.data_ptr(), pos.data_ptr(), s, st[0], st[1], st[2], s * h * d, h * d, d,
-                          pos.stride(0) if pos.shape[0] > 1 else 0, pos.stride(1), h)
-    return op, y.view(x.shape), (x4, pos)
+        pb, ps, _ = pos.stride()
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    arg = _RopeArg(x4.data_ptr(), y.data_ptr(), pos.data_ptr(), s, sb if b > 1 else 0, ss if s > 1 else 0, sh if h > 1 else 0,
+                   s * h * d, h * d, d, pb if pos.shape[0] > 1 else 0, ps, h)
+    return arg, y, (x4, pos)
 
 
 def _rope_axes(q, k, q_pos, k_pos, inv_freq, sections, pairing, inverse):
     ref = q if q is not None else k
+    dev = ref.device
     if not ref.is_cuda or (k is not None and not k.is_cuda):
         raise RuntimeError("rope_axes: CUDA tensors only (there is no CPU path)")
     code = _lib.act_code(ref.dtype)
-    if inv_freq.dim() != 1 or inv_freq.device != ref.device:
-        raise ValueError(f"rope_axes: inv_freq must be 1-D on {ref.device}")
-    n = inv_freq.shape[0]
-    axes = q_pos if q is not None else k_pos
-    axes = axes.shape[-1] if axes is not None and axes.dim() in (2, 3) else 0
+    if inv_freq.dim() != 1 or inv_freq.device != dev:
+        raise ValueError(f"rope_axes: inv_freq must be 1-D on {dev}")
+    first = q_pos if q is not None else k_pos
+    axes = first.shape[-1] if first is not None and first.dim() in (2, 3) else 0
     if sections is None:  # every axis turns by all the frequencies, axis after axis
-        sections, inv_freq = (n,) * axes, inv_freq.repeat(axes)
+        sections, inv_freq = (inv_freq.shape[0],) * axes, inv_freq.repeat(axes)
     if len(sections) != axes or sum(sections) != inv_freq.shape[0]:
         raise ValueError(f"rope_axes: {axes} axes with {inv_freq.shape[0]} frequencies do not match sections {tuple(sections)}")
-    inv_freq = inv_freq.to(torch.float32).contiguous()
-    if q is not None and k is not None and (k.dtype != q.dtype or k.device != q.device or k.dim() != q.dim() or
-                                            k.shape[-1] != q.shape[-1] or (q.dim() == 4 and k.shape[0] != q.shape[0])):
-        raise ValueError(f"rope_axes: q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} do not match")
-    if q is not None and k is not None and k_pos is not None and k_pos.dtype != q_pos.dtype:
-        raise ValueError("rope_axes: positions of q and k must have one dtype")
+    if inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous():
+        inv_freq = inv_freq.to(torch.float32).contiguous()
+    if q is not None and k is not None:
+        if k.dtype != q.dtype or k.device != dev or k.dim() != q.dim() or k.shape[-1] != q.shape[-1] or \
+                (q.dim() == 4 and k.shape[0] != q.shape[0]):
+            raise ValueError(f"rope_axes: q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} do not match")
+        if k_pos is not None and first is not None and k_pos.dtype != first.dtype:
+            raise ValueError("rope_axes: positions of q and k must have one dtype")
     oq = _rope_operand(q, q_pos, axes, "q") if q is not None else None
     ok = _rope_operand(k, k_pos, axes, "k") if k is not None else None
-    pos = (oq or ok)[2][1]
-    b = ref.shape[0] if ref.dim() == 4 else 1
-    by = ctypes.byref
-    dev = ref.device
-    with torch.cuda.device(dev):
-        _lib.check(_lib.lib().h3b_rope_axes(by(oq[0]) if oq else None, by(ok[0]) if ok else None, code, b, ref.shape[-1],
-                                            inv_freq.data_ptr(), (ctypes.c_int32 * max(1, axes))(*sections), axes,
-                                            _POS_CODES[pos.dtype], _lib.PAIRING[pairing], int(inverse),
-                                            _lib.stream_ptr(dev)), "rope_axes")
+    args = (ctypes.addressof(oq[0]) if oq else None, ctypes.addressof(ok[0]) if ok else None, code,
+            ref.shape[0] if ref.dim() == 4 else 1, ref.shape[-1], inv_freq.data_ptr(),
+            (ctypes.c_int32 * max(1, axes))(*sections), axes, _POS_CODES[(oq or ok)[2][1].dtype], _lib.PAIRING[pairing],
+            int(inverse))
+    lib = _lib.lib()
+    if dev.index == torch.cuda.current_device():
+        rc = lib.h3b_rope_axes(*args, _lib.raw_stream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            rc = lib.h3b_rope_axes(*args, _lib.raw_stream(dev.index))
+    _lib.check(rc, "rope_axes")
     return (oq[1] if oq else None), (ok[1] if ok else None)
 
 
