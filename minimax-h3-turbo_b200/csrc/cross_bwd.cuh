@@ -799,18 +799,21 @@ __global__ void __launch_bounds__(512, 1)
 }
 
 // Adds up the splits' partial gradients in order and rounds once.  Four channels per thread; `rows` rows of D channels,
-// row -> (b, s, h) with `inner` heads inside (dQ: [B, Hq, Sq], dK and dV: [B, Hkv, Sk]).
+// row -> (b, h, s) with H heads and S rows (dQ: Hq, Sq; dK and dV: Hkv, Sk); the second tensor (blockIdx.y = 1) follows the
+// first in every split.
 template <typename T>
 __global__ void __launch_bounds__(256) cross_join_kernel(const float* part, int64_t stride, int splits, int64_t rows, int D,
-                                                         int64_t S, int H, h3b_attn_tensor out) {
+                                                         int64_t S, int H, h3b_attn_tensor out0, h3b_attn_tensor out1) {
   const int per = D / 4;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
   if (i >= rows * per) return;
+  const h3b_attn_tensor& out = blockIdx.y ? out1 : out0;
   const int64_t row = i / per;
   const int c = static_cast<int>(i - row * per) * 4;
+  const float* src = part + (blockIdx.y * rows + row) * D + c;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int s = 0; s < splits; ++s) {
-    const float4 v = *reinterpret_cast<const float4*>(part + s * stride + row * D + c);
+    const float4 v = *reinterpret_cast<const float4*>(src + s * stride);
     a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
   }
   const int64_t s = row % S, bh = row / S, h = bh % H, b = bh / H;
@@ -818,9 +821,11 @@ __global__ void __launch_bounds__(256) cross_join_kernel(const float* part, int6
       make_uint2(pack2<T>(a.x, a.y), pack2<T>(a.z, a.w));
 }
 template <typename T>
-static int join_launch(const float* part, int64_t stride, int splits, int64_t rows, int D, int64_t S, int H,
-                       const h3b_attn_tensor& out, cudaStream_t st) {
-  cross_join_kernel<T><<<static_cast<unsigned>((rows * (D / 4) + 255) / 256), 256, 0, st>>>(part, stride, splits, rows, D, S, H, out);
+static int join_launch(const float* part, int splits, int64_t rows, int D, int64_t S, int H, const h3b_attn_tensor& out0,
+                       const h3b_attn_tensor* out1, cudaStream_t st) {
+  const int n = out1 ? 2 : 1;
+  const dim3 grid(static_cast<unsigned>((rows * (D / 4) + 255) / 256), n);
+  cross_join_kernel<T><<<grid, 256, 0, st>>>(part, n * rows * D, splits, rows, D, S, H, out0, out1 ? *out1 : out0);
   return check_launch("cross_join_kernel");
 }
 
@@ -851,15 +856,16 @@ static int bwd_launch_cfg(const CrossParams& P, cudaStream_t st) {
   const int sms = cross_sms();
   auto kq = cross_dq_kernel<T, DP, BIAS>;
   auto kkv = cross_dkv_kernel<T, DP, BIAS>;
-  cudaError_t e = cudaFuncSetAttribute(kq, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(kkv, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-  if (e != cudaSuccess) return cuda_fail(e, "cross_attention_backward shared memory");
+  static std::atomic<bool> ready_q[CA_DEVICES], ready_kv[CA_DEVICES];
+  rc = cross_smem(reinterpret_cast<const void*>(kq), C::SMEM, ready_q, "cross_dq_kernel shared memory");
+  if (!rc) rc = cross_smem(reinterpret_cast<const void*>(kkv), C::SMEM, ready_kv, "cross_dkv_kernel shared memory");
+  if (rc) return rc;
   if (P.Sq > 0) {
     const int64_t n = static_cast<int64_t>(P.q_tiles) * P.splits * P.Hkv * P.B, rows = static_cast<int64_t>(P.B) * P.Hq * P.Sq;
     if (n >= (1 << 30)) return fail(H3B_ERR_UNSUPPORTED, "cross_attention_backward: too many query tiles");
     kq<<<static_cast<int>(n < sms ? n : sms), 512, C::SMEM, st>>>(q, g, k, v, P);
     rc = check_launch("cross_dq_kernel");
-    if (!rc && P.splits > 1) rc = join_launch<T>(P.part_dq, rows * P.D, P.splits, rows, P.D, P.Sq, P.Hq, P.dq, st);
+    if (!rc && P.splits > 1) rc = join_launch<T>(P.part_dq, P.splits, rows, P.D, P.Sq, P.Hq, P.dq, nullptr, st);
     if (rc) return rc;
   }
   if (P.Sk > 0) {
@@ -867,10 +873,7 @@ static int bwd_launch_cfg(const CrossParams& P, cudaStream_t st) {
     if (n >= (1 << 30)) return fail(H3B_ERR_UNSUPPORTED, "cross_attention_backward: too many key tiles");
     kkv<<<static_cast<int>(n < sms ? n : sms), 512, C::SMEM, st>>>(q, g, k, v, P);
     rc = check_launch("cross_dkv_kernel");
-    if (!rc && P.kv_splits > 1) {
-      rc = join_launch<T>(P.part_dk, 2 * rows * P.D, P.kv_splits, rows, P.D, P.Sk, P.Hkv, P.dk, st);
-      if (!rc) rc = join_launch<T>(P.part_dk + rows * P.D, 2 * rows * P.D, P.kv_splits, rows, P.D, P.Sk, P.Hkv, P.dv, st);
-    }
+    if (!rc && P.kv_splits > 1) rc = join_launch<T>(P.part_dk, P.kv_splits, rows, P.D, P.Sk, P.Hkv, P.dk, &P.dv, st);
   }
   return rc;
 }

@@ -12,6 +12,7 @@
 // stores such a tile in one copy per 64 channels.  Channels are padded to 64 or 128 (DP) by the copy's zero fill.
 #pragma once
 
+#include <atomic>
 #include <mutex>
 #include <type_traits>
 
@@ -400,11 +401,33 @@ static int cross_map_k(CUtensorMap* map, const CrossParams& P, const h3b_attn_te
   return cross_map(map, t.ptr, half, 4, ext, str, box);
 }
 
-static int cross_sms() {
-  int dev = 0, sms = 148;
+// SM count and what a kernel needs set before its first launch: asked for and set once per device (a property of the
+// device and of the kernel; a call spends over a microsecond on them otherwise).
+constexpr int CA_DEVICES = 64;
+static int cross_device() {
+  int dev = 0;
   cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return dev;
+}
+static int cross_sms() {
+  static std::atomic<int> known[CA_DEVICES];
+  const int dev = cross_device();
+  int sms = dev < CA_DEVICES ? known[dev].load(std::memory_order_relaxed) : 0;
+  if (sms == 0) {
+    sms = 148;
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (dev < CA_DEVICES) known[dev].store(sms, std::memory_order_relaxed);
+  }
   return sms;
+}
+// `done`: one flag per device of this kernel
+static int cross_smem(const void* kernel, int bytes, std::atomic<bool> (&done)[CA_DEVICES], const char* what) {
+  const int dev = cross_device();
+  if (dev < CA_DEVICES && done[dev].load(std::memory_order_acquire)) return H3B_OK;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return cuda_fail(e, what);
+  if (dev < CA_DEVICES) done[dev].store(true, std::memory_order_release);
+  return H3B_OK;
 }
 
 }  // namespace h3b

@@ -609,8 +609,9 @@ static int fwd_launch_cfg(const CrossParams& P, cudaStream_t st) {
   if (!rc) rc = cross_map_q(&o, P, P.o, half);
   if (rc) return rc;
   auto kern = cross_fwd_kernel<T, DP, BIAS>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-  if (e != cudaSuccess) return cuda_fail(e, "cross_fwd_kernel shared memory");
+  static std::atomic<bool> ready[CA_DEVICES];
+  rc = cross_smem(reinterpret_cast<const void*>(kern), C::SMEM, ready, "cross_fwd_kernel shared memory");
+  if (rc) return rc;
   const int64_t items = static_cast<int64_t>(P.units) * P.splits * P.Hkv * P.B;
   if (items >= (1 << 30)) return fail(H3B_ERR_UNSUPPORTED, "cross_attention: too many query tiles");
   const int grid = static_cast<int>(items < cross_sms() ? items : cross_sms());

@@ -9,8 +9,8 @@ block's other operators; there is no CPU path.
 """
 from __future__ import annotations
 
-import ctypes
 import math
+from array import array
 from typing import Optional, Tuple
 
 import torch
@@ -18,7 +18,6 @@ import torch
 from .. import _lib
 
 _CODES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16}
-_Args8 = ctypes.c_int64 * 32  # up to eight struct h3b_attn_tensor {ptr, stride_b, stride_s, stride_h}
 
 
 def _guard(dev: torch.device):
@@ -121,9 +120,11 @@ class _Problem:
         sizes = (self.b, self.sq, self.sk, self.hq, self.hkv, self.d)
         n = lib.h3b_cross_attention_workspace_bytes(*sizes, self.kind, backward)
         ws = torch.empty(n, dtype=torch.uint8, device=self.dev) if n else None
-        arr = _Args8(*[x for t in tensors for x in _arg(t)])
-        at = ctypes.addressof(arr)
-        ts = [at + 32 * i for i in range(len(tensors))]
+        arr = array("q")  # struct h3b_attn_tensor, one after the other
+        for t in tensors:
+            arr.extend(_arg(t))
+        at = arr.buffer_info()[0]
+        ts = range(at, at + 32 * len(tensors), 32)
         mid = (self.code, *sizes, self.scale, _lib.ptr(self.lens), _lib.ptr(self.mask), self.kind, self.ldm)
         tail = (_lib.ptr(ws), n, _lib.raw_stream(self.dev.index))
         if backward:
@@ -192,7 +193,6 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_len
     return (o, lse) if return_lse else o
 
 
-@torch.no_grad()
 def cross_attention_backward(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor,
                              lse: torch.Tensor, *, kv_lens: Optional[torch.Tensor] = None,
                              key_mask: Optional[torch.Tensor] = None, scale: Optional[float] = None
