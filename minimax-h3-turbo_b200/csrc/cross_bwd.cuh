@@ -11,9 +11,9 @@
 // by atomics, in a changing order, through fp32 buffers in memory) is not paid: results have the same bits every time.
 // P and dS are rounded to the operand type for the second products (8 or 11 bits, relative to each element); sums are fp32.
 //
-// Warps of both: 0-7 elementwise work, thread = row, warps 0-3 the first 64 columns, 4-7 the other 64; 8-11 epilogue
-// (accumulators -> global memory); 12 MMA issue; 13 copies; 14 (dq) zeroes K rows of masked keys before their product.
-// P and dS go back to tensor memory over the columns that their own warps read S or dP from.
+// Warps of both: 0-15 elementwise work, thread = row, four warps to the same 32 rows with 32 columns each; 16-19 epilogue
+// (accumulators -> global memory); 20 MMA issue; 21 copies; 22 (dQ) zeroes K rows of masked
+// keys before their product.  P and dS go back to tensor memory over the columns that their own warps read S or dP from.
 #include "cross_common.cuh"
 
 namespace h3b {
@@ -64,19 +64,53 @@ struct BwdWalk {
   }
 };
 
+// The same walk for the MMA warp, which needs only how many tiles a unit has.
+template <bool DQ>
+struct BwdCount {
+  const CrossParams& P;
+  int it, left;
+  bool first;
+  __device__ __forceinline__ BwdCount(const CrossParams& p) : P(p), it(blockIdx.x) { seek(); }
+  __device__ __forceinline__ bool valid() const { return left > 0; }
+  __device__ __forceinline__ bool last() const { return left == 1; }
+  __device__ __forceinline__ void seek() {
+    const int splits = DQ ? P.splits : P.kv_splits;
+    const int n = (DQ ? P.q_tiles : static_cast<int>(P.Skp / CT)) * splits * P.Hkv * P.B;
+    first = true;
+    for (left = 0; it < n; it += gridDim.x) {
+      const FastDiv &by_own = DQ ? P.by_q_tiles : P.by_k_tiles, &by_split = DQ ? P.by_splits : P.by_kv_splits;
+      int tile, split;
+      const int b = P.by_hkv.div(by_split.divmod(by_own.divmod(it, tile), split));
+      const int64_t len = ca_len(P.kv_lens, b, P.Sk);
+      const int other = DQ ? static_cast<int>((len + CT - 1) / CT) : static_cast<int64_t>(tile) * CT < len ? P.q_tiles : 0;
+      const int per = by_split.div(other + splits - 1);
+      left = min(per, other - min(split * per, other));
+      if (left > 0) return;
+    }
+  }
+  __device__ __forceinline__ void next() {
+    first = false;
+    if (--left > 0) return;
+    it += gridDim.x;
+    seek();
+  }
+};
+
 template <int DP>
 struct BwdCfg {
   static constexpr int NSUB = DP / 64;
   static constexpr int TILE = NSUB * static_cast<int>(SUB_BYTES);
-  static constexpr int SMEM = 7 * TILE + 2048 + 512;  // 7 tiles, small vectors, barriers
+  static constexpr int SMEM = 7 * TILE + 5 * CT * 4 + 512;  // 7 tiles, small vectors, barriers
+  static constexpr int THREADS = 768;
   static constexpr uint32_t TMEM_COLS = 512;
 };
 
 // ------------------------------------------------------------------------------------------------ dQ
 template <typename T, int DP, bool BIAS>
-__global__ void __launch_bounds__(512, 1)
+__global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
     cross_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG,
-                    const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const CrossParams P) {
+                    const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                    const __grid_constant__ CUtensorMap tmO, const CrossParams P) {
   using C = BwdCfg<DP>;
   constexpr int KS = 3, VS = 2;  // ring stages
   extern __shared__ __align__(1024) unsigned char ca_smem[];
@@ -84,8 +118,9 @@ __global__ void __launch_bounds__(512, 1)
   unsigned char* sG = sQ + C::TILE;
   unsigned char* sK = sG + C::TILE;
   unsigned char* sV = sK + KS * C::TILE;
-  float* part = reinterpret_cast<float*>(sV + VS * C::TILE);  // [unit parity][2][128] halves of a row's delta
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(part + 512);
+  float* part = reinterpret_cast<float*>(sV + VS * C::TILE);  // [4][128] quarters of a row's delta
+  float* deltas = part + 4 * CT;                               // [128] delta
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(deltas + CT);
   uint64_t* q_empty = q_full + 1;
   uint64_t* g_full = q_empty + 1;
   uint64_t* g_empty = g_full + 1;
@@ -110,7 +145,7 @@ __global__ void __launch_bounds__(512, 1)
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
     mbar_init(g_full, 1);
-    mbar_init(g_empty, 9);  // the last dP product, and the eight warps that take delta from it
+    mbar_init(g_empty, 1);
     for (int s = 0; s < KS; ++s) {
       mbar_init(&k_full[s], 1);
       mbar_init(&k_empty[s], 1);
@@ -123,8 +158,8 @@ __global__ void __launch_bounds__(512, 1)
     mbar_init(&s_full[0], 1);
     mbar_init(&s_full[1], 1);
     mbar_init(dp_full, 1);
-    mbar_init(ds_full, 8);
-    mbar_init(part_full, 8);
+    mbar_init(ds_full, 16);
+    mbar_init(part_full, 16);
     mbar_init(dq_full, 1);
     mbar_init(dq_empty, 4);
     mbar_init(done, 1);
@@ -135,7 +170,7 @@ __global__ void __launch_bounds__(512, 1)
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
   }
-  if (warp == 12) {
+  if (warp == 20) {
     tmem_alloc(tmem_slot, C::TMEM_COLS);
     tmem_relinquish();
   }
@@ -145,125 +180,136 @@ __global__ void __launch_bounds__(512, 1)
   const uint32_t tmem = *tmem_slot;
   const uint32_t tDP = tmem + 2 * CT, tDQ = tmem + 3 * CT;  // S0 S1 dP dQ
 
-  if (warp < 8) {
+  if (warp < 16) {
     // ------------------------------------------------------------------------------------------ P, dS
-    regs_inc<176>();
-    const int half = warp >> 2, row = threadIdx.x & (CT - 1), qr = P.by_g.div(row), hg = row - qr * P.G;
-    const uint32_t at = (static_cast<uint32_t>(warp & 3) << 21) + half * 64;  // this warp's lanes and columns
-    uint32_t sph = 0, dph = 0, gph = 0, xph = 0, sbuf = 0;
+    regs_inc<96>();
+    const int quarter = warp >> 2, row = threadIdx.x & (CT - 1);
+    int hg;
+    const int qr = P.by_g.divmod(row, hg);
+    const uint32_t at = (static_cast<uint32_t>(warp & 3) << 21) + quarter * 32;  // this warp's lanes and columns
+    uint32_t sph = 0, dph = 0, xph = 0, sbuf = 0;
     float nlse2 = -INFINITY, delta = 0.f;
     bool ok = true, valid = false;
     int64_t len = 0;
     for (BwdWalk<true> w(P); ok && w.valid; w.next()) {
       const BwdTile& u = w.c;
-      const int64_t s = static_cast<int64_t>(u.tile) * P.nq + qr;
-      const int64_t rid = (static_cast<int64_t>(u.b) * P.Hq + u.hk * P.G + hg) * P.Sq + s;
       const bool one_tile = P.splits == 1 && u.t1 - u.t0 == 1;
       if (u.first()) {
+        const int64_t s = static_cast<int64_t>(u.tile) * P.nq + qr;
         len = ca_len(P.kv_lens, u.b, P.Sk);
         valid = qr < P.nq && s < P.Sq;
-        const float e = valid ? P.lse[rid] : -INFINITY;
+        const float e = valid ? P.lse[(static_cast<int64_t>(u.b) * P.Hq + u.hk * P.G + hg) * P.Sq + s] : -INFINITY;
         nlse2 = e == -INFINITY ? -INFINITY : -e * CA_LOG2E;  // rows outside, and rows without keys: every p is 0
       }
       if (!(ok = warp_wait(&s_full[sbuf], sph, abort_flag))) break;
       tc_fence_after();
       const uint32_t tS = tmem + sbuf * CT + at;
-      float p[64];
+      float p[32];
+      uint32_t r[32];
+      tmem_ld_32x32b_x32(tS, r);
+      tmem_ld_wait();
+      if constexpr (BIAS) {
+        const float4* b4 = reinterpret_cast<const float4*>(P.bias2 + u.b * P.Skp + static_cast<int64_t>(u.t) * CT + quarter * 32);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t r[32];
-        tmem_ld_32x32b_x32(tS + 32 * c, r);
-        tmem_ld_wait();
-        if constexpr (BIAS) {
-          const float4* b4 = reinterpret_cast<const float4*>(P.bias2 + u.b * P.Skp + static_cast<int64_t>(u.t) * CT + half * 64 + 32 * c);
+        for (int i = 0; i < 8; ++i) {
+          const float4 bb = __ldg(b4 + i);
+          const float bv[4] = {bb.x, bb.y, bb.z, bb.w};
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float4 bb = __ldg(b4 + i);
-            const float bv[4] = {bb.x, bb.y, bb.z, bb.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float x = ex2(fmaf(__uint_as_float(r[4 * i + e]), P.scale2, bv[e] + nlse2));
-              p[32 * c + 4 * i + e] = bv[e] == -INFINITY ? 0.f : x;
-            }
+          for (int e = 0; e < 4; ++e) {
+            const float x = ex2(fmaf(__uint_as_float(r[4 * i + e]), P.scale2, bv[e] + nlse2));
+            p[4 * i + e] = bv[e] == -INFINITY ? 0.f : x;
           }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) p[32 * c + i] = ex2(fmaf(__uint_as_float(r[i]), P.scale2, nlse2));
         }
-      }
-      const int64_t lim = len - (static_cast<int64_t>(u.t) * CT + half * 64);  // columns in use, from this warp's first
-      if (!BIAS && lim < 64) {
+      } else {
 #pragma unroll
-        for (int i = 0; i < 64; ++i)
-          if (i >= lim) p[i] = 0.f;
+        for (int i = 0; i < 32; ++i) p[i] = ex2(fmaf(__uint_as_float(r[i]), P.scale2, nlse2));
+        const int64_t lim = len - (static_cast<int64_t>(u.t) * CT + quarter * 32);  // columns in use, from this warp's first
+        if (lim < 32) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (i >= lim) p[i] = 0.f;
+        }
       }
       if (nlse2 == -INFINITY) {  // also when the row's own scores are not numbers
 #pragma unroll
-        for (int i = 0; i < 64; ++i) p[i] = 0.f;
+        for (int i = 0; i < 32; ++i) p[i] = 0.f;
       }
-      if (u.first()) {
-        if (!(ok = warp_wait(g_full, gph, abort_flag))) break;
-        gph ^= 1;
-        if (!one_tile) {  // half of g . o of this row: channels [half DP / 2, ..)
-          float d = 0.f;
-          const T* orow = static_cast<const T*>(P.o.ptr) + u.b * P.o.stride_b + s * P.o.stride_s + (u.hk * P.G + hg) * P.o.stride_h;
+      if (u.first() && !one_tile) {
+        // delta = g . o, whole rows at a time: this warp takes 8 of the tile's, while the unit's first dP is on its way
+        constexpr int PER_ROW = DP / 8, PER_PASS = 32 / PER_ROW, PASSES = 8 / PER_PASS;
+        const int ch = lane % PER_ROW * 8, r0 = warp * 8 + lane / PER_ROW;
+        const T* ob = static_cast<const T*>(P.o.ptr) + u.b * P.o.stride_b + u.hk * P.G * P.o.stride_h + ch;
+        const T* gb = static_cast<const T*>(P.go.ptr) + u.b * P.go.stride_b + u.hk * P.G * P.go.stride_h + ch;
+        uint4 ov[PASSES], gv[PASSES];
 #pragma unroll
-          for (int c = 0; c < DP / 16; ++c) {
-            const int ch = half * (DP / 2) + 8 * c;
-            if (valid && ch < P.D) {
-              const uint4 ov = __ldg(reinterpret_cast<const uint4*>(orow + ch));
-              const uint4 gv = *reinterpret_cast<const uint4*>(sG + (ch >> 6) * SUB_BYTES + row * 128 +
-                                                               ((((ch & 63) >> 3) ^ (row & 7)) << 4));
-              const T* oe = reinterpret_cast<const T*>(&ov);
-              const T* ge = reinterpret_cast<const T*>(&gv);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) d = fmaf(static_cast<float>(oe[e]), static_cast<float>(ge[e]), d);
-            }
+        for (int a = 0; a < PASSES; ++a) {
+          int h;
+          const int q = P.by_g.divmod(r0 + a * PER_PASS, h);
+          const int64_t s = static_cast<int64_t>(u.tile) * P.nq + q;
+          ov[a] = gv[a] = make_uint4(0, 0, 0, 0);
+          if (q < P.nq && s < P.Sq && ch < P.D) {
+            ov[a] = __ldg(reinterpret_cast<const uint4*>(ob + s * P.o.stride_s + h * P.o.stride_h));
+            gv[a] = __ldg(reinterpret_cast<const uint4*>(gb + s * P.go.stride_s + h * P.go.stride_h));
           }
-          part[(2 * xph + half) * CT + row] = d;
         }
+#pragma unroll
+        for (int a = 0; a < PASSES; ++a) {
+          const T* oe = reinterpret_cast<const T*>(&ov[a]);
+          const T* ge = reinterpret_cast<const T*>(&gv[a]);
+          float d = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) d = fmaf(static_cast<float>(oe[e]), static_cast<float>(ge[e]), d);
+#pragma unroll
+          for (int o = PER_ROW / 2; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+          if (lane % PER_ROW == 0) deltas[r0 + a * PER_PASS] = d;
+        }
+        // every warp has read the unit before's: this unit's scores were issued after all had handed in that one's first dS
         __syncwarp();
-        if (lane == 0) mbar_arrive(g_empty);
+        if (lane == 0) mbar_arrive(part_full);
+        if (!(ok = warp_wait(part_full, xph, abort_flag))) break;
+        xph ^= 1;
+        delta = deltas[row];
+        if (u.t1 - u.t0 == 1) {  // (not so when a unit is one tile of several: once more, after reading)
+          __syncwarp();
+          if (lane == 0) mbar_arrive(part_full);
+          if (!(ok = warp_wait(part_full, xph, abort_flag))) break;
+          xph ^= 1;
+        }
       }
       if (!(ok = warp_wait(dp_full, dph, abort_flag))) break;
       dph ^= 1;
       tc_fence_after();
-      float dp[64];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t r[32];
-        tmem_ld_32x32b_x32(tDP + at + 32 * c, r);
-        tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < 32; ++i) dp[32 * c + i] = __uint_as_float(r[i]);
-      }
+      tmem_ld_32x32b_x32(tDP + at, r);
+      tmem_ld_wait();
       if (masked) {  // a masked key's dP may be anything
 #pragma unroll
-        for (int i = 0; i < 64; ++i) dp[i] = p[i] == 0.f ? 0.f : dp[i];
+        for (int i = 0; i < 32; ++i)
+          if (p[i] == 0.f) r[i] = 0;
       }
       if (u.first()) {
         if (one_tile) {
           float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int i = 0; i < 64; ++i) d[i & 3] = fmaf(p[i], dp[i], d[i & 3]);
-          part[(2 * xph + half) * CT + row] = (d[0] + d[1]) + (d[2] + d[3]);
+          for (int i = 0; i < 32; ++i) d[i & 3] = fmaf(p[i], __uint_as_float(r[i]), d[i & 3]);
+          // (the next unit's dP, which its quarters come from, is issued after every warp has handed in this unit's dS)
+          part[quarter * CT + row] = (d[0] + d[1]) + (d[2] + d[3]);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(part_full);
+          if (!(ok = warp_wait(part_full, xph, abort_flag))) break;
+          xph ^= 1;
+          delta = (part[row] + part[CT + row]) + (part[2 * CT + row] + part[3 * CT + row]);
         }
-        // a unit's halves are overwritten two units later: past the next unit's wait, which every warp's reads come before
-        __syncwarp();
-        if (lane == 0) mbar_arrive(part_full);
-        if (!(ok = warp_wait(part_full, xph, abort_flag))) break;
-        delta = part[2 * xph * CT + row] + part[(2 * xph + 1) * CT + row];
-        xph ^= 1;
-        if (u.split == 0 && half == 0) {
+        if (u.split == 0 && quarter == 0) {
           float* st = P.stats + ((static_cast<int64_t>(u.b) * P.Hkv + u.hk) * P.q_tiles + u.tile) * (2 * CT);
           st[row] = nlse2;
           st[CT + row] = valid ? delta : 0.f;
         }
       }
-      uint32_t pk[32];
+      uint32_t pk[16];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) pk[i] = pack2<T>(p[2 * i] * (dp[2 * i] - delta), p[2 * i + 1] * (dp[2 * i + 1] - delta));
-      tmem_st_32x32b_x32(tS, pk);
+      for (int i = 0; i < 16; ++i)
+        pk[i] = pack2<T>(p[2 * i] * (__uint_as_float(r[2 * i]) - delta), p[2 * i + 1] * (__uint_as_float(r[2 * i + 1]) - delta));
+      tmem_st_32x32b_x16(tS, pk);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -271,15 +317,17 @@ __global__ void __launch_bounds__(512, 1)
       sbuf ^= 1;
       if (sbuf == 0) sph ^= 1;
     }
-  } else if (warp < 12) {
+  } else if (warp < 20) {
     // ------------------------------------------------------------------------------------------ epilogue
-    regs_dec<96>();
-    const int row = threadIdx.x & (CT - 1), qr = P.by_g.div(row), hg = row - qr * P.G;
+    regs_dec<48>();
+    const int row = threadIdx.x & (CT - 1);
+    int hg;
+    const int qr = P.by_g.divmod(row, hg);
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
     uint32_t ph = 0;
+    bool ok = true;
     BwdWalk<true> w(P);
     BwdTile u;
-    bool ok = true;
     for (int it = blockIdx.x; ok && it < w.n; it += gridDim.x) {
       w.unit(it, u);
       const int64_t s = static_cast<int64_t>(u.tile) * P.nq + qr;
@@ -293,18 +341,18 @@ __global__ void __launch_bounds__(512, 1)
       T* dst = static_cast<T*>(P.dq.ptr) + u.b * P.dq.stride_b + s * P.dq.stride_s + (u.hk * P.G + hg) * P.dq.stride_h;
       float* dst32 = P.part_dq + (static_cast<int64_t>(u.split) * P.B * P.Hq * P.Sq + rid) * P.D;
 #pragma unroll 1
-      for (int c = 0; c < DP / 32; ++c) {
-        uint32_t o[32];
+      for (int c = 0; c < DP / 16; ++c) {
+        uint32_t o[16];
         if (any) {
-          tmem_ld_32x32b_x32(tDQ + lanes + 32 * c, o);
+          tmem_ld_32x32b_x16(tDQ + lanes + 16 * c, o);
           tmem_ld_wait();
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0;
+          for (int i = 0; i < 16; ++i) o[i] = 0;
         }
         if (!valid) continue;
-        if (P.splits > 1) store_cols_f32(dst32 + 32 * c, o, P.scale, P.D - 32 * c);
-        else store_cols<T>(dst + 32 * c, o, P.scale, P.D - 32 * c);
+        if (P.splits > 1) store_cols_f32(dst32 + 16 * c, o, P.scale, P.D - 16 * c);
+        else store_cols<T>(dst + 16 * c, o, P.scale, P.D - 16 * c);
       }
       if (any) {
         tc_fence_before();
@@ -313,38 +361,38 @@ __global__ void __launch_bounds__(512, 1)
       }
     }
   } else {
-    regs_dec<64>();
-    if (warp == 12) {
+    regs_dec<48>();
+    if (warp == 20) {
       // -------------------------------------------------------------------------------------- MMA issue
       constexpr uint32_t idS = idesc_f16<T>(CT, CT, false), idD = idesc_f16<T>(CT, DP, true);
       constexpr uint64_t TILE16 = C::TILE >> 4;
       const uint64_t rQ = desc_rows(smem_u32(sQ)), rG = desc_rows(smem_u32(sG)), rK = desc_rows(smem_u32(sK)),
                      rV = desc_rows(smem_u32(sV));
       const uint64_t cK = desc_chan(smem_u32(sK));
-      BwdWalk<true> ws(P), wp(P), wd(P);  // the next S, dP and dQ product
+      BwdCount<true> ws(P), wp(P), wd(P);  // the next S, dP and dQ product
       int sk = 0, pv = 0, dk = 0;
       uint32_t skph = 0, pvph = 0, qph = 0, gph = 0, dsph = 0, dqph = 1, sbuf = 0, dbuf = 0;
       bool ok = true;
       auto do_s = [&] {
-        if (!ok || !ws.valid) return;
+        if (!ok || !ws.valid()) return;
         if (!(ok = warp_wait(&k_full[sk], skph, abort_flag))) return;
         if (masked && !(ok = warp_wait(&k_clean[sk], skph, abort_flag))) return;
-        if (ws.c.first()) {
+        if (ws.first) {
           if (!(ok = warp_wait(q_full, qph, abort_flag))) return;
           qph ^= 1;
         }
         tc_fence_after();
         mma_rows<DP / 16>(tmem + sbuf * CT, rQ, rK + sk * TILE16, idS);
         commit_one(&s_full[sbuf]);
-        if (ws.c.last()) commit_one(q_empty);
+        if (ws.last()) commit_one(q_empty);
         sbuf ^= 1;
         if (++sk == KS) sk = 0, skph ^= 1;
         ws.next();
       };
       auto do_dp = [&] {
-        if (!ok || !wp.valid) return;
+        if (!ok || !wp.valid()) return;
         if (!(ok = warp_wait(&v_full[pv], pvph, abort_flag))) return;
-        if (wp.c.first()) {
+        if (wp.first) {
           if (!(ok = warp_wait(g_full, gph, abort_flag))) return;
           gph ^= 1;
         }
@@ -352,64 +400,74 @@ __global__ void __launch_bounds__(512, 1)
         mma_rows<DP / 16>(tDP, rG, rV + pv * TILE16, idS);
         commit_one(dp_full);
         commit_one(&v_empty[pv]);
-        if (wp.c.last()) commit_one(g_empty);
+        if (wp.last()) commit_one(g_empty);
         if (++pv == VS) pv = 0, pvph ^= 1;
         wp.next();
       };
       do_s();
       do_dp();
       do_s();
-      while (ok && wd.valid) {
+      while (ok && wd.valid()) {
         if (!(ok = warp_wait(ds_full, dsph, abort_flag))) break;  // dS is written, dP has been read
         dsph ^= 1;
-        const bool same = wp.valid && wp.c.it == wd.c.it;
+        tc_fence_after();
+        const bool same = wp.valid() && wp.it == wd.it;
         if (same) do_dp();  // a new unit's dP waits for its G tile: not before this unit's last product
         if (!ok) break;
-        if (wd.c.first()) {
+        if (wd.first) {
           if (!(ok = warp_wait(dq_empty, dqph, abort_flag))) break;
           dqph ^= 1;
+          tc_fence_after();
         }
-        tc_fence_after();
-        mma_chan<true>(tDQ, tmem + dbuf * CT, cK + dk * TILE16, idD, !wd.c.first());
+        mma_chan<4>(tDQ, tmem + dbuf * CT, cK + dk * TILE16, idD, !wd.first);
         commit_one(&k_empty[dk]);
-        if (wd.c.last()) commit_one(dq_full);
+        if (wd.last()) commit_one(dq_full);
         dbuf ^= 1;
         if (++dk == KS) dk = 0;
         wd.next();
         if (!same) do_dp();
         do_s();
       }
-    } else if (warp == 13) {
+    } else if (warp == 21) {
       if (lane == 0) {
         // -------------------------------------------------------------------------------------- copies
-        int k = 0, v = 0, kfills = 0, vfills = 0, ufills = 0;
-        uint32_t kph = 1, vph = 1, uph = 1;
+        int k = 0, v = 0, kfills = 0, vfills = 0, qfills = 0, gfills = 0;
+        uint32_t kph = 1, vph = 1, qph = 1, gph = 1;
         bool ok = true;
         const uint32_t q_bytes = static_cast<uint32_t>(C::NSUB * 128 * P.G * P.nq);
-        for (BwdWalk<true> w(P); ok && w.valid; w.next()) {
+        BwdWalk<true> w(P);
+        auto prefetch = [&](int it) {  // Q, G and O tiles of a unit to come into L2: two units ahead of their use
+          if (it >= w.n) return;
+          BwdTile nx;
+          w.unit(it, nx);
+          for (int p = 0; p < C::NSUB; ++p) {
+            tma_prefetch_5d(&tmO, 64 * p, 0, nx.hk, nx.tile * P.nq, nx.b);
+            tma_prefetch_5d(&tmG, 64 * p, 0, nx.hk, nx.tile * P.nq, nx.b);
+            tma_prefetch_5d(&tmQ, 64 * p, 0, nx.hk, nx.tile * P.nq, nx.b);
+          }
+        };
+        prefetch(static_cast<int>(blockIdx.x + gridDim.x));
+        for (; ok && w.valid; w.next()) {
           const BwdTile& u = w.c;
           if (u.first()) {
-            if (!(ok = mbar_wait(q_empty, uph, abort_flag))) break;
+            if (!(ok = mbar_wait(q_empty, qph, abort_flag))) break;
+            qph ^= 1;
             mbar_arrive_expect_tx(q_full, q_bytes);
             for (int p = 0; p < C::NSUB; ++p) tma_load_5d(sQ + p * SUB_BYTES, &tmQ, q_full, 64 * p, 0, u.hk, u.tile * P.nq, u.b);
+            ++qfills;
           }
-          if (!(ok = mbar_wait(&k_empty[k], kph, abort_flag))) {
-            if (u.first()) mbar_wait_drain(q_full, (ufills) & 1);
-            break;
-          }
+          if (!(ok = mbar_wait(&k_empty[k], kph, abort_flag))) break;
           mbar_arrive_expect_tx(&k_full[k], C::TILE);
           for (int p = 0; p < C::NSUB; ++p) tma_load_4d(sK + k * C::TILE + p * SUB_BYTES, &tmK, &k_full[k], 64 * p, u.hk, u.t * CT, u.b);
           ++kfills;
           if (++k == KS) k = 0, kph ^= 1;
           if (u.first()) {
-            if (!(ok = mbar_wait(g_empty, uph, abort_flag))) {
-              mbar_wait_drain(q_full, (ufills) & 1);
-              break;
-            }
-            uph ^= 1;
+            if (!(ok = mbar_wait(g_empty, gph, abort_flag))) break;
+            gph ^= 1;
             mbar_arrive_expect_tx(g_full, q_bytes);
             for (int p = 0; p < C::NSUB; ++p) tma_load_5d(sG + p * SUB_BYTES, &tmG, g_full, 64 * p, 0, u.hk, u.tile * P.nq, u.b);
-            ++ufills;
+            ++gfills;
+            prefetch(u.it + 2 * static_cast<int>(gridDim.x));
           }
           if (!(ok = mbar_wait(&v_empty[v], vph, abort_flag))) break;
           mbar_arrive_expect_tx(&v_full[v], C::TILE);
@@ -417,17 +475,17 @@ __global__ void __launch_bounds__(512, 1)
           ++vfills;
           if (++v == VS) v = 0, vph ^= 1;
         }
-        for (int j = kfills > KS ? kfills - KS : 0; j < kfills; ++j)  // copies in flight land before the memory goes away
-          if (!mbar_wait_drain(&k_full[j % KS], static_cast<uint32_t>((j / KS) & 1))) break;
-        for (int j = vfills > VS ? vfills - VS : 0; j < vfills; ++j)
-          if (!mbar_wait_drain(&v_full[j % VS], static_cast<uint32_t>((j / VS) & 1))) break;
-        if (ufills) {
-          mbar_wait_drain(q_full, static_cast<uint32_t>((ufills - 1) & 1));
-          mbar_wait_drain(g_full, static_cast<uint32_t>((ufills - 1) & 1));
-        }
+        auto drain = [](uint64_t* bars, int stages, int fills) {  // copies in flight land before the memory goes away
+          for (int j = fills > stages ? fills - stages : 0; j < fills; ++j)
+            if (!mbar_wait_drain(&bars[j % stages], static_cast<uint32_t>((j / stages) & 1))) break;
+        };
+        drain(k_full, KS, kfills);
+        drain(v_full, VS, vfills);
+        drain(q_full, 1, qfills);
+        drain(g_full, 1, gfills);
       }
       __syncwarp();
-    } else if (warp == 14 && masked) {
+    } else if (warp == 22 && masked) {
       // ---------------------------------------------------------------------------------------- rows of masked keys
       int k = 0;
       uint32_t kph = 0;
@@ -453,7 +511,7 @@ __global__ void __launch_bounds__(512, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 20) {
     tc_fence_after();
     commit_one(done);
     mbar_wait_drain(done, 0);
@@ -464,7 +522,7 @@ __global__ void __launch_bounds__(512, 1)
 
 // ------------------------------------------------------------------------------------------------ dK, dV
 template <typename T, int DP, bool BIAS>
-__global__ void __launch_bounds__(512, 1)
+__global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
     cross_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG,
                      const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const CrossParams P) {
   using C = BwdCfg<DP>;
@@ -511,12 +569,12 @@ __global__ void __launch_bounds__(512, 1)
     }
     for (int s = 0; s < TS; ++s) {
       mbar_init(&t_full[s], 1);
-      mbar_init(&t_empty[s], 8);
+      mbar_init(&t_empty[s], 16);
     }
     mbar_init(s_full, 1);
-    mbar_init(p_full, 8);
+    mbar_init(p_full, 16);
     mbar_init(dp_full, 1);
-    mbar_init(ds_full, 8);
+    mbar_init(ds_full, 16);
     mbar_init(acc_full, 1);
     mbar_init(acc_empty, 4);
     mbar_init(done, 1);
@@ -533,7 +591,7 @@ __global__ void __launch_bounds__(512, 1)
     *reinterpret_cast<uint4*>(sQ + p * SUB_BYTES + (P.G * P.nq + r) * 128 + c * 16) = make_uint4(0, 0, 0, 0);
   }
   fence_proxy_async_smem();
-  if (warp == 12) {
+  if (warp == 20) {
     tmem_alloc(tmem_slot, C::TMEM_COLS);
     tmem_relinquish();
   }
@@ -543,11 +601,11 @@ __global__ void __launch_bounds__(512, 1)
   const uint32_t tmem = *tmem_slot;
   const uint32_t tDP = tmem + CT, tDV = tmem + 2 * CT, tDK = tmem + 3 * CT;  // S dP dV dK
 
-  if (warp < 8) {
+  if (warp < 16) {
     // ------------------------------------------------------------------------------------------ P^T, dS^T
-    regs_inc<176>();
-    const int half = warp >> 2, row = threadIdx.x & (CT - 1);
-    const uint32_t at = (static_cast<uint32_t>(warp & 3) << 21) + half * 64;
+    regs_inc<96>();
+    const int quarter = warp >> 2, row = threadIdx.x & (CT - 1);
+    const uint32_t at = (static_cast<uint32_t>(warp & 3) << 21) + quarter * 32;
     uint32_t ph = 0, tph = 0;
     int ts = 0;
     bool ok = true, live = false;
@@ -565,55 +623,53 @@ __global__ void __launch_bounds__(512, 1)
       if (!(ok = warp_wait(&t_full[ts], tph, abort_flag))) break;
       if (!(ok = warp_wait(s_full, ph, abort_flag))) break;
       tc_fence_after();
-      const float4* nl = reinterpret_cast<const float4*>(sT + ts * 2 * CT + half * 64);
-      const float4* dl = reinterpret_cast<const float4*>(sT + ts * 2 * CT + CT + half * 64);
-      float p[64];
-      uint32_t pk[32];
+      const float4* nl = reinterpret_cast<const float4*>(sT + ts * 2 * CT + quarter * 32);
+      const float4* dl = reinterpret_cast<const float4*>(sT + ts * 2 * CT + CT + quarter * 32);
+      float p[32];
+      uint32_t r[32], pk[16];
+      const f32x2 sc = f2(P.scale2, P.scale2);
+      tmem_ld_32x32b_x32(tmem + at, r);
+      tmem_ld_wait();
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t r[32];
-        tmem_ld_32x32b_x32(tmem + at + 32 * c, r);
-        tmem_ld_wait();
+      for (int i = 0; i < 8; ++i) {  // every other pair through the FMA pipe's exp2: this phase is what the products wait for
+        const float4 n4 = nl[i];
+        f32x2 na = f2(n4.x, n4.y), nb = f2(n4.z, n4.w);
+        if constexpr (BIAS) na = f2_add(na, f2(rb, rb)), nb = f2_add(nb, f2(rb, rb));
+        float xa, xb, xc, xd;
+        f2_split(f2_fma(f2(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1])), sc, na), xa, xb);
+        f2_split(f2_fma(f2(__uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3])), sc, nb), xc, xd);
+        p[4 * i] = ex2(xa), p[4 * i + 1] = ex2(xb);
+        f2_split(f2_exp2<true>(xc, xd), p[4 * i + 2], p[4 * i + 3]);
+      }
+      if (!live) {  // this row's key is out: whatever its scores were
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float4 n4 = nl[8 * c + i];
-          const float nv[4] = {n4.x, n4.y, n4.z, n4.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float x = ex2(fmaf(__uint_as_float(r[4 * i + e]), P.scale2, BIAS ? nv[e] + rb : nv[e]));
-            p[32 * c + 4 * i + e] = live ? x : 0.f;
-          }
-        }
+        for (int i = 0; i < 32; ++i) p[i] = 0.f;
       }
 #pragma unroll
-      for (int i = 0; i < 32; ++i) pk[i] = pack2<T>(p[2 * i], p[2 * i + 1]);
-      tmem_st_32x32b_x32(tmem + at, pk);
+      for (int i = 0; i < 16; ++i) pk[i] = pack2<T>(p[2 * i], p[2 * i + 1]);
+      tmem_st_32x32b_x16(tmem + at, pk);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(p_full);
       if (!(ok = warp_wait(dp_full, ph, abort_flag))) break;
       tc_fence_after();
+      tmem_ld_32x32b_x32(tDP + at, r);
+      tmem_ld_wait();
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t r[32];
-        tmem_ld_32x32b_x32(tDP + at + 32 * c, r);
-        tmem_ld_wait();
+      for (int i = 0; i < 8; ++i) {
+        const float4 d4 = dl[i];
+        const float dv[4] = {d4.x, d4.y, d4.z, d4.w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float4 d4 = dl[8 * c + i];
-          const float dv[4] = {d4.x, d4.y, d4.z, d4.w};
-          float ds[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float x = p[32 * c + 4 * i + e] * (__uint_as_float(r[4 * i + e]) - dv[e]);
-            ds[e] = live ? x : 0.f;
-          }
-          pk[16 * c + 2 * i] = pack2<T>(ds[0], ds[1]);
-          pk[16 * c + 2 * i + 1] = pack2<T>(ds[2], ds[3]);
-        }
+        for (int e = 0; e < 4; ++e) p[4 * i + e] *= __uint_as_float(r[4 * i + e]) - dv[e];
       }
-      tmem_st_32x32b_x32(tDP + at, pk);
+      if (!live) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) p[i] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) pk[i] = pack2<T>(p[2 * i], p[2 * i + 1]);
+      tmem_st_32x32b_x16(tDP + at, pk);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -624,9 +680,9 @@ __global__ void __launch_bounds__(512, 1)
       ph ^= 1;
       if (++ts == TS) ts = 0, tph ^= 1;
     }
-  } else if (warp < 12) {
+  } else if (warp < 20) {
     // ------------------------------------------------------------------------------------------ epilogue
-    regs_dec<96>();
+    regs_dec<48>();
     const int row = threadIdx.x & (CT - 1);
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
     uint32_t ph = 0;
@@ -647,16 +703,16 @@ __global__ void __launch_bounds__(512, 1)
       T* dv = static_cast<T*>(P.dv.ptr) + u.b * P.dv.stride_b + key * P.dv.stride_s + u.hk * P.dv.stride_h;
       float* dk32 = P.part_dk + u.split * 2 * part + ((static_cast<int64_t>(u.b) * P.Hkv + u.hk) * P.Sk + key) * P.D;
 #pragma unroll 1
-      for (int c = 0; c < 2 * (DP / 32); ++c) {
-        const bool is_k = c >= DP / 32;
-        const int col = 32 * (is_k ? c - DP / 32 : c);
-        uint32_t o[32];
+      for (int c = 0; c < 2 * (DP / 16); ++c) {
+        const bool is_k = c >= DP / 16;
+        const int col = 16 * (is_k ? c - DP / 16 : c);
+        uint32_t o[16];
         if (any) {
-          tmem_ld_32x32b_x32((is_k ? tDK : tDV) + lanes + col, o);
+          tmem_ld_32x32b_x16((is_k ? tDK : tDV) + lanes + col, o);
           tmem_ld_wait();
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0;
+          for (int i = 0; i < 16; ++i) o[i] = 0;
         }
         if (!valid) continue;
         const float f = is_k ? P.scale : 1.f;
@@ -670,21 +726,21 @@ __global__ void __launch_bounds__(512, 1)
       }
     }
   } else {
-    regs_dec<64>();
-    if (warp == 12) {
+    regs_dec<48>();
+    if (warp == 20) {
       // -------------------------------------------------------------------------------------- MMA issue
       constexpr uint32_t idS = idesc_f16<T>(CT, CT, false), idD = idesc_f16<T>(CT, DP, true);
       constexpr uint64_t TILE16 = C::TILE >> 4;
       const uint64_t rQ = desc_rows(smem_u32(sQ)), rG = desc_rows(smem_u32(sG)), rK = desc_rows(smem_u32(sK)),
                      rV = desc_rows(smem_u32(sV));
       const uint64_t cQ = desc_chan(smem_u32(sQ)), cG = desc_chan(smem_u32(sG));
-      BwdWalk<false> ws(P), wp(P), wd(P);  // the next S^T, dP^T, and the tile in hand
+      BwdCount<false> ws(P), wp(P), wd(P);  // the next S^T, dP^T, and the tile in hand
       int sq = 0, pg = 0, dq = 0, dg = 0;
       uint32_t sqph = 0, pgph = 0, kph = 0, vph = 0, ph = 0, aph = 1;
       bool ok = true;
       auto do_s = [&] {
-        if (!ok || !ws.valid) return;
-        if (ws.c.first()) {
+        if (!ok || !ws.valid()) return;
+        if (ws.first) {
           if (!(ok = warp_wait(k_full, kph, abort_flag))) return;
           kph ^= 1;
         }
@@ -692,13 +748,13 @@ __global__ void __launch_bounds__(512, 1)
         tc_fence_after();
         mma_rows<DP / 16>(tmem, rK, rQ + sq * TILE16, idS);
         commit_one(s_full);
-        if (ws.c.last()) commit_one(k_empty);
+        if (ws.last()) commit_one(k_empty);
         if (++sq == QS) sq = 0, sqph ^= 1;
         ws.next();
       };
       auto do_dp = [&] {
-        if (!ok || !wp.valid) return;
-        if (wp.c.first()) {
+        if (!ok || !wp.valid()) return;
+        if (wp.first) {
           if (!(ok = warp_wait(v_full, vph, abort_flag))) return;
           vph ^= 1;
         }
@@ -706,28 +762,28 @@ __global__ void __launch_bounds__(512, 1)
         tc_fence_after();
         mma_rows<DP / 16>(tDP, rV, rG + pg * TILE16, idS);
         commit_one(dp_full);
-        if (wp.c.last()) commit_one(v_empty);
+        if (wp.last()) commit_one(v_empty);
         if (++pg == GS) pg = 0, pgph ^= 1;
         wp.next();
       };
       do_s();
       do_dp();
-      while (ok && wd.valid) {
-        const uint32_t acc = !wd.c.first();
-        const bool last = wd.c.last();
+      while (ok && wd.valid()) {
+        const uint32_t acc = !wd.first;
+        const bool last = wd.last();
         if (!(ok = warp_wait(p_full, ph, abort_flag))) break;
         if (!acc) {
           if (!(ok = warp_wait(acc_empty, aph, abort_flag))) break;
           aph ^= 1;
         }
         tc_fence_after();
-        mma_chan<true>(tDV, tmem, cG + dg * TILE16, idD, acc);
+        mma_chan<4>(tDV, tmem, cG + dg * TILE16, idD, acc);
         commit_one(&g_empty[dg]);
         if (++dg == GS) dg = 0;
         do_s();
         if (!ok || !(ok = warp_wait(ds_full, ph, abort_flag))) break;
         tc_fence_after();
-        mma_chan<true>(tDK, tDP, cQ + dq * TILE16, idD, acc);
+        mma_chan<4>(tDK, tDP, cQ + dq * TILE16, idD, acc);
         commit_one(&q_empty[dq]);
         if (last) commit_one(acc_full);
         if (++dq == QS) dq = 0;
@@ -735,7 +791,7 @@ __global__ void __launch_bounds__(512, 1)
         ph ^= 1;
         wd.next();
       }
-    } else if (warp == 13) {
+    } else if (warp == 21) {
       if (lane == 0) {
         // -------------------------------------------------------------------------------------- copies
         int q = 0, g = 0, ts = 0, qfills = 0, gfills = 0, tfills = 0, kfills = 0, vfills = 0;
@@ -789,7 +845,7 @@ __global__ void __launch_bounds__(512, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 20) {
     tc_fence_after();
     commit_one(done);
     mbar_wait_drain(done, 0);
@@ -846,9 +902,10 @@ static int bwd_splits(int64_t units, int64_t tiles) {
 template <typename T, int DP, bool BIAS>
 static int bwd_launch_cfg(const CrossParams& P, cudaStream_t st) {
   using C = BwdCfg<DP>;
-  CUtensorMap q, g, k, v;
+  CUtensorMap q, g, k, v, o;
   const bool half = std::is_same_v<T, __half>;
   int rc = cross_map_q(&q, P, P.Sq > 0 ? P.q : P.k, half);
+  if (!rc) rc = cross_map_q(&o, P, P.Sq > 0 ? P.o : P.k, half);
   if (!rc) rc = cross_map_q(&g, P, P.Sq > 0 ? P.go : P.k, half);
   if (!rc) rc = cross_map_k(&k, P, P.Sk > 0 ? P.k : P.q, half);
   if (!rc) rc = cross_map_k(&v, P, P.Sk > 0 ? P.v : P.q, half);
@@ -863,7 +920,7 @@ static int bwd_launch_cfg(const CrossParams& P, cudaStream_t st) {
   if (P.Sq > 0) {
     const int64_t n = static_cast<int64_t>(P.q_tiles) * P.splits * P.Hkv * P.B, rows = static_cast<int64_t>(P.B) * P.Hq * P.Sq;
     if (n >= (1 << 30)) return fail(H3B_ERR_UNSUPPORTED, "cross_attention_backward: too many query tiles");
-    kq<<<static_cast<int>(n < sms ? n : sms), 512, C::SMEM, st>>>(q, g, k, v, P);
+    kq<<<static_cast<int>(n < sms ? n : sms), C::THREADS, C::SMEM, st>>>(q, g, k, v, o, P);
     rc = check_launch("cross_dq_kernel");
     if (!rc && P.splits > 1) rc = join_launch<T>(P.part_dq, P.splits, rows, P.D, P.Sq, P.Hq, P.dq, nullptr, st);
     if (rc) return rc;
@@ -871,7 +928,7 @@ static int bwd_launch_cfg(const CrossParams& P, cudaStream_t st) {
   if (P.Sk > 0) {
     const int64_t n = P.Skp / CT * P.kv_splits * P.Hkv * P.B, rows = static_cast<int64_t>(P.B) * P.Hkv * P.Sk;
     if (n >= (1 << 30)) return fail(H3B_ERR_UNSUPPORTED, "cross_attention_backward: too many key tiles");
-    kkv<<<static_cast<int>(n < sms ? n : sms), 512, C::SMEM, st>>>(q, g, k, v, P);
+    kkv<<<static_cast<int>(n < sms ? n : sms), C::THREADS, C::SMEM, st>>>(q, g, k, v, P);
     rc = check_launch("cross_dkv_kernel");
     if (!rc && P.kv_splits > 1) rc = join_launch<T>(P.part_dk, P.kv_splits, rows, P.D, P.Sk, P.Hkv, P.dk, &P.dv, st);
   }

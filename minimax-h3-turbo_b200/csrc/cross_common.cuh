@@ -190,14 +190,15 @@ __device__ __forceinline__ void mma_rows(uint32_t d, uint64_t a, uint64_t b, uin
 #pragma unroll
     for (int kk = 0; kk < STEPS; ++kk) mma_f16_ss(d, a + rows_step(kk), b + rows_step(kk), idesc, kk > 0);
 }
-// D (+)= A B with A [128 rows x 128] in tensor memory and B's 128 rows in shared memory.  HALVES: the columns of each half
-// of A start 64 columns apart (its halves were written over the scores that two groups of warps read)
-template <bool HALVES>
+// D (+)= A B with A [128 rows x 128] in tensor memory and B's 128 rows in shared memory.  A's 16-bit columns lie side by
+// side (PARTS 1), or in PARTS parts at the first columns of the fp32 values that one group of warps each read.
+template <int PARTS>
 __device__ __forceinline__ void mma_chan(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  constexpr int PER = CT / 16 / PARTS;
   if (elect_one())
 #pragma unroll
     for (int kk = 0; kk < CT / 16; ++kk)
-      mma_f16_ts(d, a + (HALVES ? (kk >> 2) * 64 + (kk & 3) * 8 : kk * 8), b + chan_step(kk), idesc, acc | (kk > 0));
+      mma_f16_ts(d, a + kk / PER * (CT / PARTS) * (PARTS > 1) + (PARTS > 1 ? kk % PER : kk) * 8, b + chan_step(kk), idesc, acc | (kk > 0));
 }
 
 template <typename T>
@@ -264,11 +265,29 @@ __device__ __forceinline__ f32x2 f2_add(f32x2 a, f32x2 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+__device__ __forceinline__ f32x2 f2_mul(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {  // a NaN stays
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 // exp2 of two numbers <= 16 on the FMA pipe (the special function unit's 4 results per cycle and scheduler are the bound of
 // softmax loops): x = n + f, |f| <= 1/2 by adding and taking off 1.5 * 2^23; 2^f by a degree-4 polynomial fitted to the least
-// largest relative error (2.6e-6); n into the exponent.  Below 2^-126: 2^-126.
+// largest relative error (2.6e-6).  TAIL false: n is added to the exponent; below 2^-126 that is 2^-126, and NaN may come out
+// as any number.  TAIL true, one instruction more: times 2^n, with 0 below 2^-126 (the bits of 2^n end at n = -127, and x is
+// held there); NaN stays.
+template <bool TAIL>
 __device__ __forceinline__ f32x2 f2_exp2(float xa, float xb) {
-  const f32x2 x = f2(fmaxf(xa, -126.f), fmaxf(xb, -126.f));
+  const f32x2 x = TAIL ? f2(max_nan(xa, -127.f), max_nan(xb, -127.f)) : f2(fmaxf(xa, -126.f), fmaxf(xb, -126.f));
   const f32x2 t = f2_add(x, f2(12582912.f, 12582912.f));
   const f32x2 f = f2_fma(f2_add(t, f2(-12582912.f, -12582912.f)), f2(-1.f, -1.f), x);
   f32x2 p = f2_fma(f2(0.009570101946812917f, 0.009570101946812917f), f, f2(0.05591786158553334f, 0.05591786158553334f));
@@ -276,23 +295,18 @@ __device__ __forceinline__ f32x2 f2_exp2(float xa, float xb) {
   p = f2_fma(p, f, f2(0.6931218145829676f, 0.6931218145829676f));
   p = f2_fma(p, f, f2(0.9999992614392343f, 0.9999992614392343f));
   float ta, tb, pa, pb;
-  f2_split(t, ta, tb);
+  f2_split(t, ta, tb);  // the low bits of t are n
+  const int na = __float_as_int(ta) << 23, nb = __float_as_int(tb) << 23;
+  if constexpr (TAIL) return f2_mul(p, f2(__int_as_float(na + (127 << 23)), __int_as_float(nb + (127 << 23))));
   f2_split(p, pa, pb);
-  return f2(__int_as_float(__float_as_int(pa) + (__float_as_int(ta) << 23)),
-            __int_as_float(__float_as_int(pb) + (__float_as_int(tb) << 23)));
-}
-// maximum that keeps a NaN
-__device__ __forceinline__ float max_nan(float a, float b, float c) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
+  return f2(__int_as_float(__float_as_int(pa) + na), __int_as_float(__float_as_int(pb) + nb));
 }
 
-// 32 columns of a row of 16-bit results: 16-byte stores (n: valid columns from here on, a multiple of 8)
+// 16 columns of a row of results: 16-byte stores (n: valid columns from here on, a multiple of 8)
 template <typename T>
-__device__ __forceinline__ void store_cols(T* dst, const uint32_t (&o)[32], float w, int n) {
+__device__ __forceinline__ void store_cols(T* dst, const uint32_t (&o)[16], float w, int n) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < 2; ++i)
     if (8 * i < n) {
       uint4 v;
       uint32_t* vv = reinterpret_cast<uint32_t*>(&v);
@@ -302,9 +316,9 @@ __device__ __forceinline__ void store_cols(T* dst, const uint32_t (&o)[32], floa
       *reinterpret_cast<uint4*>(dst + 8 * i) = v;
     }
 }
-__device__ __forceinline__ void store_cols_f32(float* dst, const uint32_t (&o)[32], float w, int n) {
+__device__ __forceinline__ void store_cols_f32(float* dst, const uint32_t (&o)[16], float w, int n) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < 4; ++i)
     if (4 * i < n)
       *reinterpret_cast<float4*>(dst + 4 * i) =
           make_float4(__uint_as_float(o[4 * i]) * w, __uint_as_float(o[4 * i + 1]) * w, __uint_as_float(o[4 * i + 2]) * w,

@@ -96,7 +96,7 @@ __device__ __forceinline__ void soft_chunk(const uint32_t (&r)[16], float scale2
         }
       }
       top[h] = max_nan(top[h], xa, xb);
-      const f32x2 p = MASK == 0 && h && (i & 2) ? f2_exp2(xa, xb) : f2(ex2(xa), ex2(xb));
+      const f32x2 p = MASK == 0 && h && (i & 2) ? f2_exp2<false>(xa, xb) : f2(ex2(xa), ex2(xb));
       sum[h] = f2_add(sum[h], p);
       float pa, pb;
       f2_split(p, pa, pb);
@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
             else if (lim < 64) soft_chunk<T, 1>(r[c & 1], P.scale2, nm, lim - 16 * c, nullptr, pk + 8 * c, sum, over);
             else soft_chunk<T, 0>(r[c & 1], P.scale2, nm, 0, nullptr, pk + 8 * c, sum, over);
           }
-          over[0] = max_nan(over[0], over[1], over[1]);
+          over[0] = max_nan(over[0], over[1]);
           if (over[0] != over[0]) sum[0] = f2(over[0], over[0]);  // a score that is not a number: so is the row
           // past this barrier both warps have read S
           if (!group_any(bar, 64, over[0] > (m == -INFINITY ? -INFINITY : 8.f)) || exact) break;
@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
               if (!(ok = warp_wait(&p_full[s], pph[s], abort_flag))) break;
               pph[s] ^= 1;
               tc_fence_after();  // (a unit's first P comes after its threads have read the O before)
-              mma_chan<false>(tmem + 2 * CT + s * CT, tmem + s * CT, dV + st * 2 * TILE16, idPV, t > cur.t0);
+              mma_chan<1>(tmem + 2 * CT + s * CT, tmem + s * CT, dV + st * 2 * TILE16, idPV, t > cur.t0);
               if (last) commit_one(&o_full[s]);
             }
             if (then_qk && (s == 0 || (last ? nxt.two : cur.two))) qk(s, st, last, qk_last);
