@@ -1,10 +1,10 @@
-// Cross attention gradients on the tcgen05 tensor cores, two kernels, no atomics.
+// Cross attention gradients on the tcgen05 tensor cores, two kernels after one for the row vectors, no atomics.
 //
 // cross_dq_kernel: a unit is one query tile (128 rows) over a range of key tiles:
 //     S = Q K^T, dP = G V^T, dS = P (dP - delta), dQ += dS K           (rows of tensor memory are queries)
-//   and, once per row, delta = g . o.  When all keys fit one tile delta = sum_j p_j dP_j instead: the same number without
-//   the rounding of o, which is all there is to dS when one key takes the whole weight.  It writes -lse and delta of every
-//   tile row in tile order for the second kernel.
+//   delta = g . o comes from cross_stats_kernel, which writes it and -lse of every tile row in tile order (inside this
+//   kernel it cost over 3 us a unit).  When all keys fit one tile delta = sum_j p_j dP_j instead: the same number without
+//   the rounding of o, which is all there is to dS when one key takes the whole weight.
 // cross_dkv_kernel: a unit is one key tile over a range of query tiles of all heads that share it:
 //     S^T = K Q^T, dP^T = V G^T, dV += P^T G, dK += dS^T Q             (rows of tensor memory are keys)
 // Each computes S and dP: 7 products of the scores' size instead of 5.  The price of sharing them (dQ summed over key tiles
@@ -100,17 +100,66 @@ template <int DP>
 struct BwdCfg {
   static constexpr int NSUB = DP / 64;
   static constexpr int TILE = NSUB * static_cast<int>(SUB_BYTES);
-  static constexpr int SMEM = 7 * TILE + 5 * CT * 4 + 512;  // 7 tiles, small vectors, barriers
+  static constexpr int SMEM = 7 * TILE + 4 * CT * 4 + 512;  // 7 tiles, small vectors, barriers
   static constexpr int THREADS = 768;
   static constexpr uint32_t TMEM_COLS = 512;
 };
+
+// ------------------------------------------------------------------------------------------------ row vectors
+// -lse in units of log2 (-inf for tile rows outside the tensor and rows without keys) and delta = g . o, in tile order.  One
+// warp per DP / 8 lanes x 16 bytes of a row; reads o and g once: HBM-bound.  delta is left out (0) where the dQ kernel takes
+// it from P and dP.
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) cross_stats_kernel(const CrossParams P) {
+  constexpr int PER_ROW = DP / 8, ROWS = 256 / PER_ROW, PASSES = CT / ROWS;
+  int tile;
+  const int bh = P.by_q_tiles.divmod(blockIdx.x, tile);
+  int hk;
+  const int b = P.by_hkv.divmod(bh, hk);
+  const int64_t len = ca_len(P.kv_lens, b, P.Sk);
+  const bool need = P.splits > 1 || len > CT;
+  const int ch = threadIdx.x % PER_ROW * 8;
+  float* st = P.stats + static_cast<int64_t>(blockIdx.x) * (2 * CT);
+  const T* ob = static_cast<const T*>(P.o.ptr) + b * P.o.stride_b + ch;
+  const T* gb = static_cast<const T*>(P.go.ptr) + b * P.go.stride_b + ch;
+  uint4 ov[PASSES], gv[PASSES];
+#pragma unroll
+  for (int a = 0; a < PASSES; ++a) {
+    int h;
+    const int q = P.by_g.divmod(a * ROWS + threadIdx.x / PER_ROW, h);
+    h += hk * P.G;
+    const int64_t s = static_cast<int64_t>(tile) * P.nq + q;
+    ov[a] = gv[a] = make_uint4(0, 0, 0, 0);
+    if (need && q < P.nq && s < P.Sq && ch < P.D) {
+      ov[a] = __ldg(reinterpret_cast<const uint4*>(ob + s * P.o.stride_s + h * P.o.stride_h));
+      gv[a] = __ldg(reinterpret_cast<const uint4*>(gb + s * P.go.stride_s + h * P.go.stride_h));
+    }
+  }
+  if (threadIdx.x < CT) {
+    int h;
+    const int q = P.by_g.divmod(threadIdx.x, h);
+    const int64_t s = static_cast<int64_t>(tile) * P.nq + q;
+    const float e = q < P.nq && s < P.Sq ? P.lse[(static_cast<int64_t>(b) * P.Hq + hk * P.G + h) * P.Sq + s] : -INFINITY;
+    st[threadIdx.x] = e == -INFINITY ? -INFINITY : -e * CA_LOG2E;
+  }
+#pragma unroll
+  for (int a = 0; a < PASSES; ++a) {
+    const T* oe = reinterpret_cast<const T*>(&ov[a]);
+    const T* ge = reinterpret_cast<const T*>(&gv[a]);
+    float d = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) d = fmaf(static_cast<float>(oe[e]), static_cast<float>(ge[e]), d);
+#pragma unroll
+    for (int o = PER_ROW / 2; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+    if (threadIdx.x % PER_ROW == 0) st[CT + a * ROWS + threadIdx.x / PER_ROW] = d;
+  }
+}
 
 // ------------------------------------------------------------------------------------------------ dQ
 template <typename T, int DP, bool BIAS>
 __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
     cross_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG,
-                    const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                    const __grid_constant__ CUtensorMap tmO, const CrossParams P) {
+                    const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const CrossParams P) {
   using C = BwdCfg<DP>;
   constexpr int KS = 3, VS = 2;  // ring stages
   extern __shared__ __align__(1024) unsigned char ca_smem[];
@@ -119,8 +168,7 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
   unsigned char* sK = sG + C::TILE;
   unsigned char* sV = sK + KS * C::TILE;
   float* part = reinterpret_cast<float*>(sV + VS * C::TILE);  // [4][128] quarters of a row's delta
-  float* deltas = part + 4 * CT;                               // [128] delta
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(deltas + CT);
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(part + 4 * CT);
   uint64_t* q_empty = q_full + 1;
   uint64_t* g_full = q_empty + 1;
   uint64_t* g_empty = g_full + 1;
@@ -184,22 +232,20 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
     // ------------------------------------------------------------------------------------------ P, dS
     regs_inc<96>();
     const int quarter = warp >> 2, row = threadIdx.x & (CT - 1);
-    int hg;
-    const int qr = P.by_g.divmod(row, hg);
     const uint32_t at = (static_cast<uint32_t>(warp & 3) << 21) + quarter * 32;  // this warp's lanes and columns
     uint32_t sph = 0, dph = 0, xph = 0, sbuf = 0;
     float nlse2 = -INFINITY, delta = 0.f;
-    bool ok = true, valid = false;
+    bool ok = true;
     int64_t len = 0;
+    float* stat = nullptr;
     for (BwdWalk<true> w(P); ok && w.valid; w.next()) {
       const BwdTile& u = w.c;
       const bool one_tile = P.splits == 1 && u.t1 - u.t0 == 1;
       if (u.first()) {
-        const int64_t s = static_cast<int64_t>(u.tile) * P.nq + qr;
         len = ca_len(P.kv_lens, u.b, P.Sk);
-        valid = qr < P.nq && s < P.Sq;
-        const float e = valid ? P.lse[(static_cast<int64_t>(u.b) * P.Hq + u.hk * P.G + hg) * P.Sq + s] : -INFINITY;
-        nlse2 = e == -INFINITY ? -INFINITY : -e * CA_LOG2E;  // rows outside, and rows without keys: every p is 0
+        stat = P.stats + ((static_cast<int64_t>(u.b) * P.Hkv + u.hk) * P.q_tiles + u.tile) * (2 * CT);
+        nlse2 = stat[row];  // -inf for rows outside and rows without keys: every p is 0
+        delta = stat[CT + row];
       }
       if (!(ok = warp_wait(&s_full[sbuf], sph, abort_flag))) break;
       tc_fence_after();
@@ -222,7 +268,14 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) p[i] = ex2(fmaf(__uint_as_float(r[i]), P.scale2, nlse2));
+        for (int i = 0; i < 32; i += 4) {  // every other pair through the FMA pipe's exp2
+          const f32x2 sc = f2(P.scale2, P.scale2), n2 = f2(nlse2, nlse2);
+          float xa, xb, xc, xd;
+          f2_split(f2_fma(f2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), sc, n2), xa, xb);
+          f2_split(f2_fma(f2(__uint_as_float(r[i + 2]), __uint_as_float(r[i + 3])), sc, n2), xc, xd);
+          p[i] = ex2(xa), p[i + 1] = ex2(xb);
+          f2_split(f2_exp2<true>(xc, xd), p[i + 2], p[i + 3]);
+        }
         const int64_t lim = len - (static_cast<int64_t>(u.t) * CT + quarter * 32);  // columns in use, from this warp's first
         if (lim < 32) {
 #pragma unroll
@@ -233,48 +286,6 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
       if (nlse2 == -INFINITY) {  // also when the row's own scores are not numbers
 #pragma unroll
         for (int i = 0; i < 32; ++i) p[i] = 0.f;
-      }
-      if (u.first() && !one_tile) {
-        // delta = g . o, whole rows at a time: this warp takes 8 of the tile's, while the unit's first dP is on its way
-        constexpr int PER_ROW = DP / 8, PER_PASS = 32 / PER_ROW, PASSES = 8 / PER_PASS;
-        const int ch = lane % PER_ROW * 8, r0 = warp * 8 + lane / PER_ROW;
-        const T* ob = static_cast<const T*>(P.o.ptr) + u.b * P.o.stride_b + u.hk * P.G * P.o.stride_h + ch;
-        const T* gb = static_cast<const T*>(P.go.ptr) + u.b * P.go.stride_b + u.hk * P.G * P.go.stride_h + ch;
-        uint4 ov[PASSES], gv[PASSES];
-#pragma unroll
-        for (int a = 0; a < PASSES; ++a) {
-          int h;
-          const int q = P.by_g.divmod(r0 + a * PER_PASS, h);
-          const int64_t s = static_cast<int64_t>(u.tile) * P.nq + q;
-          ov[a] = gv[a] = make_uint4(0, 0, 0, 0);
-          if (q < P.nq && s < P.Sq && ch < P.D) {
-            ov[a] = __ldg(reinterpret_cast<const uint4*>(ob + s * P.o.stride_s + h * P.o.stride_h));
-            gv[a] = __ldg(reinterpret_cast<const uint4*>(gb + s * P.go.stride_s + h * P.go.stride_h));
-          }
-        }
-#pragma unroll
-        for (int a = 0; a < PASSES; ++a) {
-          const T* oe = reinterpret_cast<const T*>(&ov[a]);
-          const T* ge = reinterpret_cast<const T*>(&gv[a]);
-          float d = 0.f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) d = fmaf(static_cast<float>(oe[e]), static_cast<float>(ge[e]), d);
-#pragma unroll
-          for (int o = PER_ROW / 2; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-          if (lane % PER_ROW == 0) deltas[r0 + a * PER_PASS] = d;
-        }
-        // every warp has read the unit before's: this unit's scores were issued after all had handed in that one's first dS
-        __syncwarp();
-        if (lane == 0) mbar_arrive(part_full);
-        if (!(ok = warp_wait(part_full, xph, abort_flag))) break;
-        xph ^= 1;
-        delta = deltas[row];
-        if (u.t1 - u.t0 == 1) {  // (not so when a unit is one tile of several: once more, after reading)
-          __syncwarp();
-          if (lane == 0) mbar_arrive(part_full);
-          if (!(ok = warp_wait(part_full, xph, abort_flag))) break;
-          xph ^= 1;
-        }
       }
       if (!(ok = warp_wait(dp_full, dph, abort_flag))) break;
       dph ^= 1;
@@ -298,11 +309,7 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
           if (!(ok = warp_wait(part_full, xph, abort_flag))) break;
           xph ^= 1;
           delta = (part[row] + part[CT + row]) + (part[2 * CT + row] + part[3 * CT + row]);
-        }
-        if (u.split == 0 && quarter == 0) {
-          float* st = P.stats + ((static_cast<int64_t>(u.b) * P.Hkv + u.hk) * P.q_tiles + u.tile) * (2 * CT);
-          st[row] = nlse2;
-          st[CT + row] = valid ? delta : 0.f;
+          if (quarter == 0) stat[CT + row] = delta;
         }
       }
       uint32_t pk[16];
@@ -436,17 +443,15 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
         bool ok = true;
         const uint32_t q_bytes = static_cast<uint32_t>(C::NSUB * 128 * P.G * P.nq);
         BwdWalk<true> w(P);
-        auto prefetch = [&](int it) {  // Q, G and O tiles of a unit to come into L2: two units ahead of their use
+        auto prefetch = [&](int it) {  // Q and G tiles of a unit to come into L2
           if (it >= w.n) return;
           BwdTile nx;
           w.unit(it, nx);
           for (int p = 0; p < C::NSUB; ++p) {
-            tma_prefetch_5d(&tmO, 64 * p, 0, nx.hk, nx.tile * P.nq, nx.b);
             tma_prefetch_5d(&tmG, 64 * p, 0, nx.hk, nx.tile * P.nq, nx.b);
             tma_prefetch_5d(&tmQ, 64 * p, 0, nx.hk, nx.tile * P.nq, nx.b);
           }
         };
-        prefetch(static_cast<int>(blockIdx.x + gridDim.x));
         for (; ok && w.valid; w.next()) {
           const BwdTile& u = w.c;
           if (u.first()) {
@@ -467,7 +472,7 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
             mbar_arrive_expect_tx(g_full, q_bytes);
             for (int p = 0; p < C::NSUB; ++p) tma_load_5d(sG + p * SUB_BYTES, &tmG, g_full, 64 * p, 0, u.hk, u.tile * P.nq, u.b);
             ++gfills;
-            prefetch(u.it + 2 * static_cast<int>(gridDim.x));
+            prefetch(u.it + static_cast<int>(gridDim.x));
           }
           if (!(ok = mbar_wait(&v_empty[v], vph, abort_flag))) break;
           mbar_arrive_expect_tx(&v_full[v], C::TILE);
@@ -902,10 +907,9 @@ static int bwd_splits(int64_t units, int64_t tiles) {
 template <typename T, int DP, bool BIAS>
 static int bwd_launch_cfg(const CrossParams& P, cudaStream_t st) {
   using C = BwdCfg<DP>;
-  CUtensorMap q, g, k, v, o;
+  CUtensorMap q, g, k, v;
   const bool half = std::is_same_v<T, __half>;
   int rc = cross_map_q(&q, P, P.Sq > 0 ? P.q : P.k, half);
-  if (!rc) rc = cross_map_q(&o, P, P.Sq > 0 ? P.o : P.k, half);
   if (!rc) rc = cross_map_q(&g, P, P.Sq > 0 ? P.go : P.k, half);
   if (!rc) rc = cross_map_k(&k, P, P.Sk > 0 ? P.k : P.q, half);
   if (!rc) rc = cross_map_k(&v, P, P.Sk > 0 ? P.v : P.q, half);
@@ -920,7 +924,11 @@ static int bwd_launch_cfg(const CrossParams& P, cudaStream_t st) {
   if (P.Sq > 0) {
     const int64_t n = static_cast<int64_t>(P.q_tiles) * P.splits * P.Hkv * P.B, rows = static_cast<int64_t>(P.B) * P.Hq * P.Sq;
     if (n >= (1 << 30)) return fail(H3B_ERR_UNSUPPORTED, "cross_attention_backward: too many query tiles");
-    kq<<<static_cast<int>(n < sms ? n : sms), C::THREADS, C::SMEM, st>>>(q, g, k, v, o, P);
+    const int64_t tiles = static_cast<int64_t>(P.q_tiles) * P.Hkv * P.B;
+    cross_stats_kernel<T, DP><<<static_cast<unsigned>(tiles), 256, 0, st>>>(P);
+    rc = check_launch("cross_stats_kernel");
+    if (rc) return rc;
+    kq<<<static_cast<int>(n < sms ? n : sms), C::THREADS, C::SMEM, st>>>(q, g, k, v, P);
     rc = check_launch("cross_dq_kernel");
     if (!rc && P.splits > 1) rc = join_launch<T>(P.part_dq, P.splits, rows, P.D, P.Sq, P.Hq, P.dq, nullptr, st);
     if (rc) return rc;
