@@ -10,16 +10,21 @@
 // One rounding per output element, from fp32 products.
 //
 // HBM-bound: every element is read once and written once.  A CTA owns a few tokens of q or k: its threads fill a table
-// of the tokens' (cos, sin) in shared memory -- one evaluation per token and pair, not per head -- then walk the heads
-// with 16-byte accesses.
+// of the tokens' (cos, sin) in shared memory -- one evaluation per token and pair, not per head -- then go through the
+// tokens' rows in 16-byte units.  What hides the latency is full occupancy: eight CTAs of 256 threads per SM at 32 registers;
+// with the registers left to the compiler (41, six CTAs) it is 1.15 to 1.2 times slower, with four units loaded ahead per
+// thread 1.9 times.  59440 tokens x 2 x 40 heads of 128 channels, bf16 (2.43 GB): 390 to 404 us, 6.0 to 6.2 TB/s.  Partners
+// off the 16-byte grid ("half" with F not a multiple of the unit) are bound by instructions: 2.1 to 2.5 TB/s in 16 bits, 4.4
+// to 4.9 in 32 (two aligned units and a shift instead of element loads measured slower: both paths run in most warps).
+// Few tokens: one token per CTA, so that the heads of a handful of tokens spread over the SMs.
+#include "fastdiv.cuh"
 #include "h3b_common.cuh"
 #include "launch.h"
 
 namespace h3b {
 
 constexpr int RA_THREADS = 256;
-constexpr int RA_MAX_TOKENS = 8;   // tokens per CTA
-constexpr int RA_MAX_PAIRS = 512;  // F: pairs of one head
+constexpr int RA_MAX_TOKENS = 8;  // tokens per CTA
 
 struct RopeSide {
   const char* x;
@@ -28,14 +33,16 @@ struct RopeSide {
   int64_t xb, xs, xh, yb, ys, yh, pb, ps;  // strides in elements (channels contiguous)
   int64_t S, tiles;                        // tokens per batch entry; CTAs of this side
   int heads;
+  FastDiv by_row;  // units of a token
 };
 
 struct RopeParams {
   RopeSide side[2];
   const float* inv_freq;
   int64_t B;
-  int D, F, axes, pos_dtype, inverse, tokens;  // tokens: per CTA
+  int D, F, ld, axes, pos_dtype, inverse, tokens;  // ld: F rounded up to even; tokens: per CTA
   int section_end[H3B_MAX_AXES];
+  FastDiv by_units, by_pairs;  // units of a head; F
 };
 
 enum { RA_HALF = 0, RA_HALF_ANY = 1, RA_ADJACENT = 2 };
@@ -88,29 +95,30 @@ __device__ __forceinline__ void ra_store(T* p, const RaVec<T>& v, int n) {
 //   RA_HALF_ANY  output chunk u; partners are read one by one (the second read of a line comes from L1)
 //   RA_ADJACENT  output chunk u, its pairs are inside
 template <typename T, bool VEC, int MODE>
-__device__ __forceinline__ void ra_unit(const T* xr, T* yr, int u, int D, int F, const float2* cs) {
+__device__ __forceinline__ void ra_unit(const T* x, T* y, int u, int D, int F, const float2* cs) {
   constexpr int V = 16 / sizeof(T);
   if constexpr (MODE == RA_HALF) {
     if (u < F / V) {
-      const RaVec<T> a = ra_load<T, VEC>(xr + u * V, V), b = ra_load<T, VEC>(xr + u * V + F, V);
-      RaVec<T> oa, ob;
+      RaVec<T> a = ra_load<T, VEC>(x + u * V, V), b = ra_load<T, VEC>(x + u * V + F, V);
+      const float4* t4 = reinterpret_cast<const float4*>(cs + u * V);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float2 t = cs[u * V + i];
-        const float fa = ra_f(a.e[i]), fb = ra_f(b.e[i]);
-        oa.e[i] = ra_t<T>(fa * t.x - fb * t.y);
-        ob.e[i] = ra_t<T>(fa * t.y + fb * t.x);
+      for (int i = 0; i < V; i += 2) {
+        const float4 t = t4[i / 2];
+        const float a0 = ra_f(a.e[i]), b0 = ra_f(b.e[i]), a1 = ra_f(a.e[i + 1]), b1 = ra_f(b.e[i + 1]);
+        a.e[i] = ra_t<T>(a0 * t.x - b0 * t.y);
+        b.e[i] = ra_t<T>(a0 * t.y + b0 * t.x);
+        a.e[i + 1] = ra_t<T>(a1 * t.z - b1 * t.w);
+        b.e[i + 1] = ra_t<T>(a1 * t.w + b1 * t.z);
       }
-      ra_store<T, VEC>(yr + u * V, oa, V);
-      ra_store<T, VEC>(yr + u * V + F, ob, V);
+      ra_store<T, VEC>(y + u * V, a, V);
+      ra_store<T, VEC>(y + u * V + F, b, V);
     } else {
-      const int c = 2 * F + (u - F / V) * V;
-      ra_store<T, VEC>(yr + c, ra_load<T, VEC>(xr + c, min(V, D - c)), min(V, D - c));
+      const int c = F + u * V, n = min(V, D - c);
+      ra_store<T, VEC>(y + c, ra_load<T, VEC>(x + c, n), n);
     }
   } else {
     const int c = u * V, n = min(V, D - c);
-    const RaVec<T> a = ra_load<T, VEC>(xr + c, n);
-    RaVec<T> o = a;
+    RaVec<T> a = ra_load<T, VEC>(x + c, n);
     if constexpr (MODE == RA_HALF_ANY) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
@@ -118,8 +126,8 @@ __device__ __forceinline__ void ra_unit(const T* xr, T* yr, int u, int D, int F,
         if (i < n && ch < 2 * F) {
           const bool lo = ch < F;
           const float2 t = cs[lo ? ch : ch - F];
-          const float mine = ra_f(a.e[i]), other = ra_f(xr[lo ? ch + F : ch - F]);
-          o.e[i] = ra_t<T>(lo ? mine * t.x - other * t.y : other * t.y + mine * t.x);
+          const float mine = ra_f(a.e[i]), other = ra_f(x[lo ? ch + F : ch - F]);
+          a.e[i] = ra_t<T>(lo ? mine * t.x - other * t.y : other * t.y + mine * t.x);
         }
       }
     } else {
@@ -128,12 +136,12 @@ __device__ __forceinline__ void ra_unit(const T* xr, T* yr, int u, int D, int F,
         if (c + i < 2 * F) {
           const float2 t = cs[(c + i) / 2];
           const float fa = ra_f(a.e[i]), fb = ra_f(a.e[i + 1]);
-          o.e[i] = ra_t<T>(fa * t.x - fb * t.y);
-          o.e[i + 1] = ra_t<T>(fa * t.y + fb * t.x);
+          a.e[i] = ra_t<T>(fa * t.x - fb * t.y);
+          a.e[i + 1] = ra_t<T>(fa * t.y + fb * t.x);
         }
       }
     }
-    ra_store<T, VEC>(yr + c, o, n);
+    ra_store<T, VEC>(y + c, a, n);
   }
 }
 
@@ -144,17 +152,22 @@ __device__ __forceinline__ double ra_pos(const char* p, int64_t i, int dt) {
 }
 
 template <typename T, bool VEC, int MODE>
-__global__ void __launch_bounds__(RA_THREADS) rope_axes_kernel(const RopeParams P) {
-  constexpr int V = 16 / sizeof(T);
-  extern __shared__ float2 cs_table[];  // [tokens][F]
+__global__ void __launch_bounds__(RA_THREADS, 2048 / RA_THREADS) rope_axes_kernel(const RopeParams P) {
+  extern __shared__ __align__(16) float2 cs_table[];  // [tokens][ld]
+  __shared__ int64_t x_at[RA_MAX_TOKENS], y_at[RA_MAX_TOKENS];
   const bool second = static_cast<int64_t>(blockIdx.x) >= P.side[0].tiles;
   const RopeSide& sd = P.side[second];
   const int64_t tile = static_cast<int64_t>(blockIdx.x) - (second ? P.side[0].tiles : 0);
   const int64_t total = P.B * sd.S, tok0 = tile * P.tokens;
   const int ntok = static_cast<int>(total - tok0 < P.tokens ? total - tok0 : P.tokens);
+  if (threadIdx.x < ntok) {
+    const int64_t tok = tok0 + threadIdx.x, b = tok / sd.S, s = tok - b * sd.S;
+    x_at[threadIdx.x] = b * sd.xb + s * sd.xs;
+    y_at[threadIdx.x] = b * sd.yb + s * sd.ys;
+  }
   for (int i = threadIdx.x; i < ntok * P.F; i += RA_THREADS) {
-    const int t = i / P.F, j = i - t * P.F;
-    int axis = 0;
+    int j, axis = 0;
+    const int t = P.by_pairs.divmod(i, j);
     while (j >= P.section_end[axis]) ++axis;
     const int64_t tok = tok0 + t, b = tok / sd.S, s = tok - b * sd.S;
     double turns = ra_pos(sd.pos, b * sd.pb + s * sd.ps + axis, P.pos_dtype) * static_cast<double>(__ldg(P.inv_freq + j)) *
@@ -162,35 +175,39 @@ __global__ void __launch_bounds__(RA_THREADS) rope_axes_kernel(const RopeParams 
     turns -= rint(turns);
     float sn, c;
     sincospif(2.f * static_cast<float>(turns), &sn, &c);
-    cs_table[i] = make_float2(c, P.inverse ? -sn : sn);
+    cs_table[t * P.ld + j] = make_float2(c, P.inverse ? -sn : sn);
   }
   __syncthreads();
-  const int units = MODE == RA_HALF ? P.F / V + (P.D - 2 * P.F + V - 1) / V : (P.D + V - 1) / V;
-  const int per_tok = units * sd.heads;
-  for (int t = 0; t < ntok; ++t) {
-    const int64_t tok = tok0 + t, b = tok / sd.S, s = tok - b * sd.S;
-    const T* xt = reinterpret_cast<const T*>(sd.x) + b * sd.xb + s * sd.xs;
-    T* yt = reinterpret_cast<T*>(sd.y) + b * sd.yb + s * sd.ys;
-    for (int i = threadIdx.x; i < per_tok; i += RA_THREADS) {
-      const int h = i / units, u = i - h * units;
-      ra_unit<T, VEC, MODE>(xt + h * sd.xh, yt + h * sd.yh, u, P.D, P.F, cs_table + t * P.F);
-    }
+  const T* x = reinterpret_cast<const T*>(sd.x);
+  T* y = reinterpret_cast<T*>(sd.y);
+  const int n = ntok * static_cast<int>(sd.by_row.d);
+  for (int i = threadIdx.x; i < n; i += RA_THREADS) {
+    int w, u;
+    const int t = sd.by_row.divmod(i, w), h = P.by_units.divmod(w, u);
+    ra_unit<T, VEC, MODE>(x + x_at[t] + h * sd.xh, y + y_at[t] + h * sd.yh, u, P.D, P.F, cs_table + t * P.ld);
   }
 }
 
 template <typename T>
-static int rope_axes_launch_t(RopeParams& P, int pairing, bool vec, cudaStream_t st) {
+static int rope_axes_launch_t(RopeParams& P, int pairing, bool vec, int sms, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
-  P.tokens = RA_MAX_TOKENS;
-  int64_t blocks = 0;
+  const int mode = pairing == H3B_PAIR_ADJACENT ? RA_ADJACENT : P.F % V == 0 ? RA_HALF : RA_HALF_ANY;
+  const int units = mode == RA_HALF ? P.F / V + (P.D - 2 * P.F + V - 1) / V : (P.D + V - 1) / V;
+  P.by_units.set(units);
+  P.by_pairs.set(P.F);
+  P.ld = (P.F + 1) & ~1;
+  int64_t tokens = 0, blocks = 0;
+  for (const auto& sd : P.side) tokens += sd.x ? P.B * sd.S : 0;
+  const int64_t per = tokens / (8 * static_cast<int64_t>(sms));  // eight CTAs per SM before a CTA takes several tokens
+  P.tokens = static_cast<int>(per < 1 ? 1 : per > RA_MAX_TOKENS ? RA_MAX_TOKENS : per);
   for (auto& sd : P.side) {
     sd.tiles = sd.x ? (P.B * sd.S + P.tokens - 1) / P.tokens : 0;
+    sd.by_row.set(units * (sd.x ? sd.heads : 1));
     blocks += sd.tiles;
   }
   if (blocks == 0) return H3B_OK;
   if (blocks > 0x7FFFFFFF) return fail(H3B_ERR_UNSUPPORTED, "rope_axes: too many tokens for one launch");
-  const size_t smem = static_cast<size_t>(P.tokens) * P.F * sizeof(float2);
-  const int mode = pairing == H3B_PAIR_ADJACENT ? RA_ADJACENT : P.F % V == 0 ? RA_HALF : RA_HALF_ANY;
+  const size_t smem = static_cast<size_t>(P.tokens) * P.ld * sizeof(float2);
 #define H3B_RA(VEC, MODE) rope_axes_kernel<T, VEC, MODE><<<static_cast<int>(blocks), RA_THREADS, smem, st>>>(P)
   if (vec) {
     if (mode == RA_HALF) H3B_RA(true, RA_HALF);
@@ -223,15 +240,20 @@ int rope_axes_launch(const h3b_rope_operand* q, const h3b_rope_operand* k, int x
     const h3b_rope_operand* o = ops[i];
     RopeSide& sd = P.side[i];
     if (!o) continue;
-    sd = RopeSide{static_cast<const char*>(o->x), static_cast<char*>(o->y), static_cast<const char*>(o->pos),
-                  o->x_stride_b, o->x_stride_s, o->x_stride_h, o->y_stride_b, o->y_stride_s, o->y_stride_h,
-                  o->pos_stride_b, o->pos_stride_s, o->S, 0, static_cast<int>(o->heads)};
+    sd.x = static_cast<const char*>(o->x), sd.y = static_cast<char*>(o->y), sd.pos = static_cast<const char*>(o->pos);
+    sd.xb = o->x_stride_b, sd.xs = o->x_stride_s, sd.xh = o->x_stride_h;
+    sd.yb = o->y_stride_b, sd.ys = o->y_stride_s, sd.yh = o->y_stride_h;
+    sd.pb = o->pos_stride_b, sd.ps = o->pos_stride_s;
+    sd.S = o->S, sd.heads = static_cast<int>(o->heads);
     for (int64_t v : {sd.xb, sd.xs, sd.xh, sd.yb, sd.ys, sd.yh}) vec = vec && v % vw == 0;
     vec = vec && reinterpret_cast<uintptr_t>(sd.x) % 16 == 0 && reinterpret_cast<uintptr_t>(sd.y) % 16 == 0;
   }
-  if (x_dtype == H3B_BF16) return rope_axes_launch_t<__nv_bfloat16>(P, pairing, vec, st);
-  if (x_dtype == H3B_FP16) return rope_axes_launch_t<__half>(P, pairing, vec, st);
-  return rope_axes_launch_t<float>(P, pairing, vec, st);
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (x_dtype == H3B_BF16) return rope_axes_launch_t<__nv_bfloat16>(P, pairing, vec, sms, st);
+  if (x_dtype == H3B_FP16) return rope_axes_launch_t<__half>(P, pairing, vec, sms, st);
+  return rope_axes_launch_t<float>(P, pairing, vec, sms, st);
 }
 
 }  // namespace h3b
