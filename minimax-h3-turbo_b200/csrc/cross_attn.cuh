@@ -72,8 +72,8 @@ int cross_launch(const h3b_attn_tensor* t, int dtype, int64_t B, int64_t Sq, int
   if (mask_kind != H3B_MASK_NONE) {
     float* bias2 = reinterpret_cast<float*>(base + w.bias2);
     int32_t* lens = reinterpret_cast<int32_t*>(base + w.lens);
-    cross_mask_kernel<<<P.B, CA_PREP, 0, st>>>(mask, mask_kind, ldm, kv_lens, Sk, P.Skp, bias2, lens);
-    const int rc = check_launch("cross_mask_kernel");
+    const int rc = cross_launch_after("cross_mask_kernel", cross_mask_kernel, dim3(P.B), CA_PREP, 0, st, mask, mask_kind, ldm, kv_lens,
+                                      Sk, P.Skp, bias2, lens);
     if (rc) return rc;
     P.bias2 = bias2;
     P.kv_lens = lens;

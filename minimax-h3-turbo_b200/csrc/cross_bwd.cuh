@@ -112,6 +112,7 @@ struct BwdCfg {
 template <typename T, int DP>
 __global__ void __launch_bounds__(256) cross_stats_kernel(const CrossParams P) {
   constexpr int PER_ROW = DP / 8, ROWS = 256 / PER_ROW, PASSES = CT / ROWS;
+  after_previous();
   int tile;
   const int bh = P.by_q_tiles.divmod(blockIdx.x, tile);
   int hk;
@@ -226,6 +227,7 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  after_previous();
   const uint32_t tDP = tmem + 2 * CT, tDQ = tmem + 3 * CT;  // S0 S1 dP dQ
 
   if (warp < 16) {
@@ -604,6 +606,7 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  after_previous();
   const uint32_t tDP = tmem + CT, tDV = tmem + 2 * CT, tDK = tmem + 3 * CT;  // S dP dV dK
 
   if (warp < 16) {
@@ -865,6 +868,7 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
 template <typename T>
 __global__ void __launch_bounds__(256) cross_join_kernel(const float* part, int64_t stride, int splits, int64_t rows, int D,
                                                          int64_t S, int H, h3b_attn_tensor out0, h3b_attn_tensor out1) {
+  after_previous();
   const int per = D / 4;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
   if (i >= rows * per) return;
@@ -886,8 +890,8 @@ static int join_launch(const float* part, int splits, int64_t rows, int D, int64
                        const h3b_attn_tensor* out1, cudaStream_t st) {
   const int n = out1 ? 2 : 1;
   const dim3 grid(static_cast<unsigned>((rows * (D / 4) + 255) / 256), n);
-  cross_join_kernel<T><<<grid, 256, 0, st>>>(part, n * rows * D, splits, rows, D, S, H, out0, out1 ? *out1 : out0);
-  return check_launch("cross_join_kernel");
+  return cross_launch_after("cross_join_kernel", cross_join_kernel<T>, grid, 256, 0, st, part, n * rows * D, splits, rows, D, S,
+                            H, out0, out1 ? *out1 : out0);
 }
 
 // Splits of the other side's tiles for `units` units of `tiles` tiles each: least time of the busiest SM, in tiles (a unit
@@ -925,19 +929,16 @@ static int bwd_launch_cfg(const CrossParams& P, cudaStream_t st) {
     const int64_t n = static_cast<int64_t>(P.q_tiles) * P.splits * P.Hkv * P.B, rows = static_cast<int64_t>(P.B) * P.Hq * P.Sq;
     if (n >= (1 << 30)) return fail(H3B_ERR_UNSUPPORTED, "cross_attention_backward: too many query tiles");
     const int64_t tiles = static_cast<int64_t>(P.q_tiles) * P.Hkv * P.B;
-    cross_stats_kernel<T, DP><<<static_cast<unsigned>(tiles), 256, 0, st>>>(P);
-    rc = check_launch("cross_stats_kernel");
+    rc = cross_launch_after("cross_stats_kernel", cross_stats_kernel<T, DP>, dim3(static_cast<unsigned>(tiles)), 256, 0, st, P);
     if (rc) return rc;
-    kq<<<static_cast<int>(n < sms ? n : sms), C::THREADS, C::SMEM, st>>>(q, g, k, v, P);
-    rc = check_launch("cross_dq_kernel");
+    rc = cross_launch_after("cross_dq_kernel", kq, dim3(static_cast<unsigned>(n < sms ? n : sms)), C::THREADS, C::SMEM, st, q, g, k, v, P);
     if (!rc && P.splits > 1) rc = join_launch<T>(P.part_dq, P.splits, rows, P.D, P.Sq, P.Hq, P.dq, nullptr, st);
     if (rc) return rc;
   }
   if (P.Sk > 0) {
     const int64_t n = P.Skp / CT * P.kv_splits * P.Hkv * P.B, rows = static_cast<int64_t>(P.B) * P.Hkv * P.Sk;
     if (n >= (1 << 30)) return fail(H3B_ERR_UNSUPPORTED, "cross_attention_backward: too many key tiles");
-    kkv<<<static_cast<int>(n < sms ? n : sms), C::THREADS, C::SMEM, st>>>(q, g, k, v, P);
-    rc = check_launch("cross_dkv_kernel");
+    rc = cross_launch_after("cross_dkv_kernel", kkv, dim3(static_cast<unsigned>(n < sms ? n : sms)), C::THREADS, C::SMEM, st, q, g, k, v, P);
     if (!rc && P.kv_splits > 1) rc = join_launch<T>(P.part_dk, P.kv_splits, rows, P.D, P.Sk, P.Hkv, P.dk, &P.dv, st);
   }
   return rc;

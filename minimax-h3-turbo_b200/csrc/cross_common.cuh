@@ -191,6 +191,8 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&h);
   }
 }
+// wait for the kernel before this one in the stream (and its writes)
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -313,8 +315,9 @@ constexpr int CA_PREP = 1024;
 __device__ __forceinline__ float ca_mask_value(const void* mask, int kind, int64_t i) {
   return kind == H3B_MASK_BOOL ? (static_cast<const uint8_t*>(mask)[i] ? 0.f : -INFINITY) : static_cast<const float*>(mask)[i];
 }
-__global__ void __launch_bounds__(CA_PREP) cross_mask_kernel(const void* mask, int kind, int64_t ldm, const int32_t* kv_lens,
+static __global__ void __launch_bounds__(CA_PREP) cross_mask_kernel(const void* mask, int kind, int64_t ldm, const int32_t* kv_lens,
                                                              int64_t Sk, int64_t Skp, float* bias2, int32_t* lens) {
+  after_previous();
   __shared__ float top_s[CA_PREP / 32];
   __shared__ int last_s[CA_PREP / 32];
   const int b = blockIdx.x, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
@@ -393,6 +396,25 @@ static int cross_map_k(CUtensorMap* map, const CrossParams& P, const h3b_attn_te
   const int64_t str[4] = {1, t.stride_h, t.stride_s, t.stride_b};
   const int box[4] = {64, 1, CT, 1};
   return cross_map(map, t.ptr, half, 4, ext, str, box);
+}
+
+// Launch that may begin while the kernel before it in the stream finishes: set-up (barriers, tensor memory, descriptors)
+// overlaps its tail.  (The kernel before gives no early signal:
+// CTAs of the next one that wait on an SM cost the running one a tenth of its time.)  Every kernel launched so calls after_previous() before it touches global memory.
+template <typename... KA, typename... A>
+static int cross_launch_after(const char* what, void (*kernel)(KA...), dim3 grid, int threads, int smem, cudaStream_t st, A&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<KA>(args)...);
+  return e == cudaSuccess ? check_launch(what) : cuda_fail(e, what);
 }
 
 // SM count and what a kernel needs set before its first launch: asked for and set once per device (a property of the

@@ -194,6 +194,7 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  after_previous();
 
   if (warp < 16) {
     // ------------------------------------------------------------------------------------------ softmax
@@ -218,9 +219,19 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
         continue;
       }
       const int64_t len = ca_len(P.kv_lens, u.b, P.Sk);
+      const int64_t s = static_cast<int64_t>(u.tile0 + slot) * P.nq + qr;
+      const bool valid = qr < P.nq && s < P.Sq;
+      const bool idle = !__any_sync(0xffffffffu, valid);  // none of these 32 rows exists: with few queries most warps
       float m = -INFINITY;
       f32x2 l = f2(0.f, 0.f);
-      for (int t = u.t0; t < u.t1; ++t) {
+      if (idle) {  // their P is whatever the columns hold: nobody reads what comes of it
+        for (int t = u.t0; t < u.t1; ++t, sph ^= 1) {
+          dead = dead || !warp_wait(&s_full[slot], sph, abort_flag);
+          if (lane == 0) mbar_arrive(&p_full[slot]);
+        }
+        more = fwd_next(P, it, n_items, nxt);
+      }
+      for (int t = idle ? u.t1 : u.t0; t < u.t1; ++t) {
         dead = dead || !warp_wait(&s_full[slot], sph, abort_flag);
         sph ^= 1;
         tc_fence_after();
@@ -299,8 +310,6 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
       const float total = halves[slot * 2 * CT + row] + halves[(slot * 2 + 1) * CT + row];
       const bool none = total == 0.f;  // no key took part: zero, whatever the products hold
       const float inv = none ? 0.f : 1.f / total;
-      const int64_t s = static_cast<int64_t>(u.tile0 + slot) * P.nq + qr;
-      const bool valid = qr < P.nq && s < P.Sq;
       const int64_t rid = (static_cast<int64_t>(u.b) * P.Hq + u.hk * P.G + hg) * P.Sq + s;
       if (half == 0 && valid) {
         const float lse2 = none ? -INFINITY : m + log2f(total);
@@ -314,7 +323,7 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
       if (P.splits > 1) {
         float* dst = P.part_o + (u.split * rows + rid) * P.D;
 #pragma unroll 1
-        for (int c = half * (DP / 32); c < (half + 1) * (DP / 32); ++c) {
+        for (int c = half * (DP / 32); !idle && c < (half + 1) * (DP / 32); ++c) {
           uint32_t o[16];
           tmem_ld_32x32b_x16(tO + 16 * c, o);
           tmem_ld_wait();
@@ -334,7 +343,7 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
         if (uses) dead = dead || !warp_wait(&out_free[(uses - 1) & 1], ((uses - 1) >> 1) & 1, abort_flag);
         const f32x2 inv2 = f2(inv, inv);
 #pragma unroll 1
-        for (int c = 0; c < DP / 64; ++c) {  // (a loop: see max_chunk)
+        for (int c = idle ? DP / 64 : 0; c < DP / 64; ++c) {  // (a loop: see max_chunk)
           const int col = half * (DP / 2) + 32 * c;
           uint32_t o[32];
           tmem_ld_32x32b_x32(tO + col, o);
@@ -552,28 +561,35 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
   }
 }
 
-// Joins the key splits of every row: weights exp2(lse_s - lse), in the order of the splits.  One warp per row.
+// Joins the key splits of every row: weights exp2(lse_s - lse), always in the same order.  One warp per row, eight splits on
+// their way at a time.  No shared memory: with four warps per row that add up there, the attention kernels around this one took
+// 7 us longer each (33 us launches, measured).
 template <typename T>
-__global__ void __launch_bounds__(256) cross_combine_kernel(const CrossParams P) {
-  const int64_t rows = static_cast<int64_t>(P.B) * P.Hq * P.Sq;
-  const int lane = threadIdx.x & 31;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (row >= rows) return;
-  float top = -INFINITY;
-  for (int s = lane; s < P.splits; s += 32) top = fmaxf(top, P.part_lse[s * rows + row]);
+__global__ void __launch_bounds__(32) cross_combine_kernel(const CrossParams P) {
+  after_previous();
+  const int64_t rows = static_cast<int64_t>(P.B) * P.Hq * P.Sq, row = blockIdx.x;
+  const int lane = threadIdx.x;
+  float e[2], top = -INFINITY, sum = 0.f;  // at most 64 splits
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    e[i] = lane + 32 * i < P.splits ? P.part_lse[(lane + 32 * i) * rows + row] : -INFINITY;
+    top = fmaxf(top, e[i]);
+  }
   for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    e[i] = ex2(e[i] - base);
+    sum += e[i];
+  }
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float sum = 0.f;
+#pragma unroll 8
   for (int s = 0; s < P.splits; ++s) {
-    const float e = P.part_lse[s * rows + row];
-    if (e == -INFINITY) continue;  // a split without keys wrote nothing else
-    const float w = ex2(e - base);
-    sum += w;
-    if (4 * lane < P.D) {
-      const float4 o = *reinterpret_cast<const float4*>(P.part_o + (s * rows + row) * P.D + 4 * lane);
-      acc.x = fmaf(w, o.x, acc.x), acc.y = fmaf(w, o.y, acc.y), acc.z = fmaf(w, o.z, acc.z), acc.w = fmaf(w, o.w, acc.w);
-    }
+    const float w = __shfl_sync(0xffffffffu, s < 32 ? e[0] : e[1], s & 31);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);  // a split without keys wrote nothing
+    if (w != 0.f && 4 * lane < P.D) o = *reinterpret_cast<const float4*>(P.part_o + (s * rows + row) * P.D + 4 * lane);
+    acc.x = fmaf(w, o.x, acc.x), acc.y = fmaf(w, o.y, acc.y), acc.z = fmaf(w, o.z, acc.z), acc.w = fmaf(w, o.w, acc.w);
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int64_t s = row % P.Sq, bh = row / P.Sq, h = bh % P.Hq, b = bh / P.Hq;
@@ -615,12 +631,10 @@ static int fwd_launch_cfg(const CrossParams& P, cudaStream_t st) {
   const int64_t items = static_cast<int64_t>(P.units) * P.splits * P.Hkv * P.B;
   if (items >= (1 << 30)) return fail(H3B_ERR_UNSUPPORTED, "cross_attention: too many query tiles");
   const int grid = static_cast<int>(items < cross_sms() ? items : cross_sms());
-  kern<<<grid, C::THREADS, C::SMEM, st>>>(q, k, v, o, P);
-  rc = check_launch("cross_fwd_kernel");
+  rc = cross_launch_after("cross_fwd_kernel", kern, dim3(grid), C::THREADS, C::SMEM, st, q, k, v, o, P);
   if (rc || P.splits == 1) return rc;
   const int64_t rows = static_cast<int64_t>(P.B) * P.Hq * P.Sq;
-  cross_combine_kernel<T><<<static_cast<unsigned>((rows + 7) / 8), 256, 0, st>>>(P);
-  return check_launch("cross_combine_kernel");
+  return cross_launch_after("cross_combine_kernel", cross_combine_kernel<T>, dim3(static_cast<unsigned>(rows)), 32, 0, st, P);
 }
 
 template <typename T>
