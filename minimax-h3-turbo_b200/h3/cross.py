@@ -5,17 +5,23 @@ gradients.  No reference counterpart: the reference's attention is one stream's 
     s_ij = scale * q_i . k_j + bias_j        o_i = sum_j softmax_j(s_ij) v_j        lse_i = log sum_j exp(s_ij)
 
 Kernels: h3b_cross_attention and h3b_cross_attention_backward (include/h3b.h).  bf16/fp16 CUDA tensors only, as the
-block's other operators; there is no CPU path.
+block's other operators; there is no CPU path.  `CrossLayer` runs them as a residual layer between W4A8 linears, with the
+rotary embedding of both streams' positions (rope.rope_axes).
 """
 from __future__ import annotations
 
 import math
 from array import array
-from typing import Optional, Tuple
+from dataclasses import dataclass
+from typing import Optional, Sequence, Tuple
 
 import torch
 
 from .. import _lib
+from . import block as blk
+from . import qlinear as ql
+from .rope import rope_axes
+from .types import Weight
 
 _CODES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16}
 
@@ -215,3 +221,53 @@ def cross_attention_backward(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
         with _guard(p.dev):
             p.call("cross_attention_backward", tensors, lse, True)
     return dq.view(q.shape), dk.view(k.shape), dv.view(v.shape)
+
+
+@dataclass
+class CrossWeights:
+    """Weights of one cross-attention layer: W4A8 or dense [N, K] linears and the norm of the residual stream."""
+
+    q: Weight     # [heads * head_dim, hidden]
+    kv: Weight    # [2 * kv_heads * head_dim, width of the other stream]: keys, then values
+    out: Weight   # [hidden, heads * head_dim]
+    norm: torch.Tensor  # [hidden]
+
+
+class CrossLayer:
+    """x += gate * out(attention(rope(q(h)), rope(k), v)),  h = rms(x, norm) * (1 + scale) + shift: the residual stream x
+    [S, hidden] attends to another stream's states [Sk, width], with the block's modulation rows and segments.
+
+    The keys and values depend on the other stream only: `keys_values` computes them once for all denoising steps (with
+    their rotary embedding); a call takes the pair.  sections / pairing: how rope_axes deals the frequencies out; without
+    inv_freq nothing is turned."""
+
+    def __init__(self, heads: int, head_dim: int, kv_heads: Optional[int] = None, norm_eps: float = 1e-5,
+                 precision: str = "a8", sections: Optional[Sequence[int]] = None, pairing: str = "half"):
+        self.heads, self.head_dim = heads, head_dim
+        self.kv_heads = heads if kv_heads is None else kv_heads
+        if self.kv_heads < 1 or heads % self.kv_heads:
+            raise ValueError(f"{heads} query heads are not a multiple of {self.kv_heads} key heads")
+        self.norm_eps, self.precision, self.sections, self.pairing = norm_eps, precision, sections, pairing
+
+    def keys_values(self, states: torch.Tensor, w: CrossWeights, positions: Optional[torch.Tensor] = None,
+                    inv_freq: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """(k, v) [Sk, kv_heads, head_dim] of the other stream's states [Sk, width], k turned by its positions."""
+        inner = self.kv_heads * self.head_dim
+        k, v = (t.unflatten(-1, (self.kv_heads, self.head_dim)) for t in
+                ql.linear(states, w.kv, precision=self.precision).split(inner, dim=-1))
+        if inv_freq is not None:
+            _, k = rope_axes(None, k, None, inv_freq, self.sections, k_positions=positions, pairing=self.pairing)
+        return k, v
+
+    def __call__(self, x: torch.Tensor, w: CrossWeights, kv: Tuple[torch.Tensor, torch.Tensor], shift: torch.Tensor,
+                 scale: torch.Tensor, gate: torch.Tensor, segments: Sequence[blk.Segment],
+                 positions: Optional[torch.Tensor] = None, inv_freq: Optional[torch.Tensor] = None, *,
+                 kv_lens: Optional[torch.Tensor] = None, key_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """x (updated in place and returned); kv from keys_values; kv_lens [1] / key_mask [1, Sk] as in cross_attention."""
+        s = x.shape[0]
+        pre = blk.Prenorm(x, w.norm, self.norm_eps, shift, scale, segments)
+        q = blk.prenorm_linear(pre, w.q, self.precision).view(s, self.heads, self.head_dim)
+        if inv_freq is not None:
+            q, _ = rope_axes(q, None, positions, inv_freq, self.sections, pairing=self.pairing)
+        o = cross_attention(q, *kv, kv_lens=kv_lens, key_mask=key_mask)
+        return blk.gate_(x, gate, ql.linear(o.view(s, -1), w.out, precision=self.precision), segments)
