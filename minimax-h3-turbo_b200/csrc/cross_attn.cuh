@@ -69,17 +69,19 @@ int cross_launch(const h3b_attn_tensor* t, int dtype, int64_t B, int64_t Sq, int
   P.part_lse = reinterpret_cast<float*>(base + w.part_lse);
   P.kv_lens = kv_lens;
   P.scale = scale, P.scale2 = scale * CA_LOG2E;
+  MaskArgs m{};
+  m.kv_lens = kv_lens;
   if (mask_kind != H3B_MASK_NONE) {
-    float* bias2 = reinterpret_cast<float*>(base + w.bias2);
-    int32_t* lens = reinterpret_cast<int32_t*>(base + w.lens);
-    const int rc = cross_launch_after("cross_mask_kernel", cross_mask_kernel, dim3(P.B), CA_PREP, 0, st, mask, mask_kind, ldm, kv_lens,
-                                      Sk, P.Skp, bias2, lens);
-    if (rc) return rc;
-    P.bias2 = bias2;
-    P.kv_lens = lens;
+    m = MaskArgs{mask, kv_lens, reinterpret_cast<float*>(base + w.bias2), reinterpret_cast<int32_t*>(base + w.lens), ldm, Sk, P.Skp, mask_kind};
+    P.bias2 = m.bias2;
+    P.kv_lens = m.lens;
+    if (!backward || Sq == 0) {  // the backward pass prepares it with its row vectors
+      const int rc = cross_launch_after("cross_mask_kernel", cross_mask_kernel, dim3(P.B), CA_PREP, 0, st, m);
+      if (rc) return rc;
+    }
   }
-  if (dtype == H3B_BF16) return backward ? bwd_launch<__nv_bfloat16>(P, st) : fwd_launch<__nv_bfloat16>(P, st);
-  return backward ? bwd_launch<__half>(P, st) : fwd_launch<__half>(P, st);
+  if (dtype == H3B_BF16) return backward ? bwd_launch<__nv_bfloat16>(P, m, st) : fwd_launch<__nv_bfloat16>(P, st);
+  return backward ? bwd_launch<__half>(P, m, st) : fwd_launch<__half>(P, st);
 }
 
 }  // namespace h3b

@@ -107,20 +107,27 @@ struct BwdCfg {
 
 // ------------------------------------------------------------------------------------------------ row vectors
 // -lse in units of log2 (-inf for tile rows outside the tensor and rows without keys) and delta = g . o, in tile order.  One
-// warp per DP / 8 lanes x 16 bytes of a row; reads o and g once: HBM-bound.  delta is left out (0) where the dQ kernel takes
-// it from P and dP.
+// row is DP / 8 lanes x 16 bytes; reads o and g once: HBM-bound.  delta is left out (0) where the dQ kernel surely takes it from
+// P and dP.  With a key mask the first B CTAs prepare it instead (a launch less).
 template <typename T, int DP>
-__global__ void __launch_bounds__(256) cross_stats_kernel(const CrossParams P) {
+__global__ void __launch_bounds__(256) cross_stats_kernel(const CrossParams P, const MaskArgs mask) {
   constexpr int PER_ROW = DP / 8, ROWS = 256 / PER_ROW, PASSES = CT / ROWS;
   after_previous();
+  int unit = blockIdx.x;
+  if (mask.mask) {
+    if (unit < P.B) {
+      prepare_mask<256>(mask, unit);
+      return;
+    }
+    unit -= P.B;
+  }
   int tile;
-  const int bh = P.by_q_tiles.divmod(blockIdx.x, tile);
+  const int bh = P.by_q_tiles.divmod(unit, tile);
   int hk;
   const int b = P.by_hkv.divmod(bh, hk);
-  const int64_t len = ca_len(P.kv_lens, b, P.Sk);
-  const bool need = P.splits > 1 || len > CT;
+  const bool need = P.splits > 1 || ca_len(mask.kv_lens, b, P.Sk) > CT;  // the lengths before the mask
   const int ch = threadIdx.x % PER_ROW * 8;
-  float* st = P.stats + static_cast<int64_t>(blockIdx.x) * (2 * CT);
+  float* st = P.stats + static_cast<int64_t>(unit) * (2 * CT);
   const T* ob = static_cast<const T*>(P.o.ptr) + b * P.o.stride_b + ch;
   const T* gb = static_cast<const T*>(P.go.ptr) + b * P.go.stride_b + ch;
   uint4 ov[PASSES], gv[PASSES];
@@ -909,7 +916,7 @@ static int bwd_splits(int64_t units, int64_t tiles) {
 }
 
 template <typename T, int DP, bool BIAS>
-static int bwd_launch_cfg(const CrossParams& P, cudaStream_t st) {
+static int bwd_launch_cfg(const CrossParams& P, const MaskArgs& mask, cudaStream_t st) {
   using C = BwdCfg<DP>;
   CUtensorMap q, g, k, v;
   const bool half = std::is_same_v<T, __half>;
@@ -929,7 +936,8 @@ static int bwd_launch_cfg(const CrossParams& P, cudaStream_t st) {
     const int64_t n = static_cast<int64_t>(P.q_tiles) * P.splits * P.Hkv * P.B, rows = static_cast<int64_t>(P.B) * P.Hq * P.Sq;
     if (n >= (1 << 30)) return fail(H3B_ERR_UNSUPPORTED, "cross_attention_backward: too many query tiles");
     const int64_t tiles = static_cast<int64_t>(P.q_tiles) * P.Hkv * P.B;
-    rc = cross_launch_after("cross_stats_kernel", cross_stats_kernel<T, DP>, dim3(static_cast<unsigned>(tiles)), 256, 0, st, P);
+    rc = cross_launch_after("cross_stats_kernel", cross_stats_kernel<T, DP>, dim3(static_cast<unsigned>(tiles + (mask.mask ? P.B : 0))), 256, 0,
+                            st, P, mask);
     if (rc) return rc;
     rc = cross_launch_after("cross_dq_kernel", kq, dim3(static_cast<unsigned>(n < sms ? n : sms)), C::THREADS, C::SMEM, st, q, g, k, v, P);
     if (!rc && P.splits > 1) rc = join_launch<T>(P.part_dq, P.splits, rows, P.D, P.Sq, P.Hq, P.dq, nullptr, st);
@@ -945,9 +953,9 @@ static int bwd_launch_cfg(const CrossParams& P, cudaStream_t st) {
 }
 
 template <typename T>
-static int bwd_launch(const CrossParams& P, cudaStream_t st) {
-  if (P.D <= 64) return P.bias2 ? bwd_launch_cfg<T, 64, true>(P, st) : bwd_launch_cfg<T, 64, false>(P, st);
-  return P.bias2 ? bwd_launch_cfg<T, 128, true>(P, st) : bwd_launch_cfg<T, 128, false>(P, st);
+static int bwd_launch(const CrossParams& P, const MaskArgs& mask, cudaStream_t st) {
+  if (P.D <= 64) return P.bias2 ? bwd_launch_cfg<T, 64, true>(P, mask, st) : bwd_launch_cfg<T, 64, false>(P, mask, st);
+  return P.bias2 ? bwd_launch_cfg<T, 128, true>(P, mask, st) : bwd_launch_cfg<T, 128, false>(P, mask, st);
 }
 
 }  // namespace h3b

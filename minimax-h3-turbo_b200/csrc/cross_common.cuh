@@ -311,21 +311,28 @@ __device__ __forceinline__ void store_cols_f32(float* dst, const uint32_t (&o)[1
 // One CTA per batch entry turns a key mask into what the kernels add to the scores: bias2[j] = log2(e) (bias_j - top),
 // top the largest bias in use (softmax does not change, and an entry whose keys all carry a large negative value keeps
 // its scores' digits and its log-sum-exp), -inf for keys that are out; and the number of keys up to the last one in use.
-constexpr int CA_PREP = 1024;
-__device__ __forceinline__ float ca_mask_value(const void* mask, int kind, int64_t i) {
-  return kind == H3B_MASK_BOOL ? (static_cast<const uint8_t*>(mask)[i] ? 0.f : -INFINITY) : static_cast<const float*>(mask)[i];
+struct MaskArgs {
+  const void* mask;  // null: none
+  const int32_t* kv_lens;
+  float* bias2;
+  int32_t* lens;
+  int64_t ldm, Sk, Skp;
+  int kind;
+};
+__device__ __forceinline__ float ca_mask_value(const MaskArgs& a, int64_t i) {
+  return a.kind == H3B_MASK_BOOL ? (static_cast<const uint8_t*>(a.mask)[i] ? 0.f : -INFINITY) : static_cast<const float*>(a.mask)[i];
 }
-static __global__ void __launch_bounds__(CA_PREP) cross_mask_kernel(const void* mask, int kind, int64_t ldm, const int32_t* kv_lens,
-                                                             int64_t Sk, int64_t Skp, float* bias2, int32_t* lens) {
-  after_previous();
-  __shared__ float top_s[CA_PREP / 32];
-  __shared__ int last_s[CA_PREP / 32];
-  const int b = blockIdx.x, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int64_t len = ca_len(kv_lens, b, Sk);
+template <int THREADS>
+__device__ __forceinline__ void prepare_mask(const MaskArgs& a, int b) {
+  constexpr int W = THREADS / 32;
+  __shared__ float top_s[W];
+  __shared__ int last_s[W];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t len = ca_len(a.kv_lens, b, a.Sk);
   float top = -INFINITY;
   int last = 0;
-  for (int64_t j = threadIdx.x; j < len; j += CA_PREP) {
-    const float v = ca_mask_value(mask, kind, b * ldm + j);
+  for (int64_t j = threadIdx.x; j < len; j += THREADS) {
+    const float v = ca_mask_value(a, b * a.ldm + j);
     if (v != -INFINITY) last = static_cast<int>(j) + 1;
     top = fmaxf(top, v);
   }
@@ -335,16 +342,21 @@ static __global__ void __launch_bounds__(CA_PREP) cross_mask_kernel(const void* 
   }
   if (lane == 0) top_s[w] = top, last_s[w] = last;
   __syncthreads();
-  top = top_s[lane], last = last_s[lane];
-  for (int o = 16; o; o >>= 1) {
+  top = top_s[lane % W], last = last_s[lane % W];
+  for (int o = W / 2; o; o >>= 1) {
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
   }
-  if (threadIdx.x == 0) lens[b] = last;
-  for (int64_t j = threadIdx.x; j < Skp; j += CA_PREP) {
-    const float v = j < len ? ca_mask_value(mask, kind, b * ldm + j) : -INFINITY;
-    bias2[b * Skp + j] = v == -INFINITY ? v : (v - top) * CA_LOG2E;
+  if (threadIdx.x == 0) a.lens[b] = last;
+  for (int64_t j = threadIdx.x; j < a.Skp; j += THREADS) {
+    const float v = j < len ? ca_mask_value(a, b * a.ldm + j) : -INFINITY;
+    a.bias2[b * a.Skp + j] = v == -INFINITY ? v : (v - top) * CA_LOG2E;
   }
+}
+constexpr int CA_PREP = 1024;
+static __global__ void __launch_bounds__(CA_PREP) cross_mask_kernel(const MaskArgs a) {
+  after_previous();
+  prepare_mask<CA_PREP>(a, blockIdx.x);
 }
 
 // ----------------------------------------------------------------------------------------------- tensor maps

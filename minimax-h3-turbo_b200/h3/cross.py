@@ -90,7 +90,7 @@ class _Problem:
         self.lens = self.mask = None
         self.kind, self.ldm = _lib.MASK_NONE, 0
         if kv_lens is not None:
-            if tuple(kv_lens.shape) != (b,) or kv_lens.dtype not in (torch.int32, torch.int64) or kv_lens.device != dev:
+            if kv_lens.shape != (b,) or kv_lens.dtype not in (torch.int32, torch.int64) or kv_lens.device != dev:
                 raise ValueError(f"cross_attention: kv_lens must be int32 or int64 [{b}] on {dev}")
             self.lens = kv_lens.to(torch.int32).contiguous()
         if key_mask is not None:
@@ -137,11 +137,12 @@ class _Problem:
             rc = lib.h3b_cross_attention_backward(*ts[:5], lse.data_ptr(), *ts[5:], *mid, *tail)
         else:
             rc = lib.h3b_cross_attention(*ts, *mid, _lib.ptr(lse), *tail)
-        _lib.check(rc, entry)
+        if rc:
+            _lib.check(rc, entry)
 
 
 def _forward(p: _Problem, want_lse: bool, out: Optional[torch.Tensor]):
-    o = torch.empty(p.b, p.sq, p.hq, p.d, dtype=p.q.dtype, device=p.dev) if out is None else out
+    o = torch.empty_like(p.q, memory_format=torch.contiguous_format) if out is None else out
     lse = torch.empty(p.b, p.hq, p.sq, dtype=torch.float32, device=p.dev) if want_lse else None
     if p.dev.index == torch.cuda.current_device():
         p.call("cross_attention", (p.q, p.k, p.v, o), lse, False)
@@ -211,16 +212,14 @@ def cross_attention_backward(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
     if tuple(lse.shape) != (p.b, p.hq, p.sq) or lse.dtype != torch.float32 or lse.device != p.dev:
         raise ValueError(f"cross_attention: lse must be fp32 {(p.b, p.hq, p.sq)} on {p.dev}")
     lse = lse.contiguous()
-    dq = torch.empty(p.b, p.sq, p.hq, p.d, dtype=p.q.dtype, device=p.dev)
-    dk = torch.empty(p.b, p.sk, p.hkv, p.d, dtype=p.q.dtype, device=p.dev)
-    dv = torch.empty_like(dk)
+    dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (p.q, p.k, p.v))
     tensors = (do_, p.q, p.k, p.v, o_, dq, dk, dv)
     if p.dev.index == torch.cuda.current_device():
         p.call("cross_attention_backward", tensors, lse, True)
     else:
         with _guard(p.dev):
             p.call("cross_attention_backward", tensors, lse, True)
-    return dq.view(q.shape), dk.view(k.shape), dv.view(v.shape)
+    return tuple(g if t.dim() == 4 else g.view(t.shape) for g, t in ((dq, q), (dk, k), (dv, v)))
 
 
 @dataclass

@@ -11,6 +11,7 @@ and k of different lengths and head counts, bf16/fp16/fp32, in both directions (
 from __future__ import annotations
 
 import ctypes
+from array import array
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -73,74 +74,99 @@ def norm_rope_(q: torch.Tensor, k: torch.Tensor, wq: torch.Tensor, wk: torch.Ten
 _POS_CODES = {torch.float32: _lib.FP32, torch.int32: _lib.INT32, torch.int64: _lib.INT64}
 
 
-_RopeArg = ctypes.c_int64 * 13  # struct h3b_rope_operand
+_section_tables = {}  # tuple of sections -> the C table of it
 
 
-def _rope_operand(x: torch.Tensor, pos: Optional[torch.Tensor], axes: int, name: str):
-    """(struct, output, tensors to keep) of one side, x [B, S, heads, D] or [S, heads, D]."""
+def _section_table(sections: Tuple[int, ...]):
+    t = _section_tables.get(sections)
+    if t is None:
+        if len(_section_tables) > 256:
+            _section_tables.clear()
+        t = _section_tables[sections] = (ctypes.c_int32 * max(1, len(sections)))(*sections)
+    return t
+
+
+def _rope_operand(arg: array, x: torch.Tensor, pos: Optional[torch.Tensor], axes: int, name: str, keep: list) -> torch.Tensor:
+    """Appends struct h3b_rope_operand of one side, x [B, S, heads, D] or [S, heads, D], to `arg` and copies it had to make
+    to `keep`; the output."""
     if x.dim() == 4:
-        x4 = x
+        b, s, h, d = x.shape
+        sb, ss, sh, sd = x.stride()
     elif x.dim() == 3:
-        x4 = x.unsqueeze(0)
+        b, sb = 1, 0
+        s, h, d = x.shape
+        ss, sh, sd = x.stride()
     else:
         raise ValueError(f"{name} must be [B, S, heads, D] or [S, heads, D], got {tuple(x.shape)}")
-    b, s, h, d = x4.shape
     if pos is None or pos.device != x.device or pos.dtype not in _POS_CODES:
         raise ValueError(f"{name}: positions must be fp32, int32 or int64 on {x.device}")
-    if pos.dim() == 2:
-        pos = pos.unsqueeze(0)
-    if pos.dim() != 3 or pos.shape[0] not in (1, b) or pos.shape[1] != s or pos.shape[2] != axes:
+    if pos.dim() == 3:
+        pn, n, pa = pos.shape
+        pb, ps, stride = pos.stride()
+    elif pos.dim() == 2:
+        pn, pb = 1, 0
+        n, pa = pos.shape
+        ps, stride = pos.stride()
+    else:
+        pn = n = pa = stride = -1
+    if pn not in (1, b) or n != s or pa != axes:
         raise ValueError(f"{name}: positions must be [{s}, {axes}] or [{b}, {s}, {axes}], got {tuple(pos.shape)}")
-    sb, ss, sh, sd = x4.stride()
-    if sd != 1 and d > 1:
-        x4 = x4.contiguous()
-        sb, ss, sh, _ = x4.stride()
-    pb, ps, pa = pos.stride()
-    if pa != 1 and axes > 1:
+    if stride != 1 and axes > 1:
         pos = pos.contiguous()
-        pb, ps, _ = pos.stride()
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    arg = _RopeArg(x4.data_ptr(), y.data_ptr(), pos.data_ptr(), s, sb if b > 1 else 0, ss if s > 1 else 0, sh if h > 1 else 0,
-                   s * h * d, h * d, d, pb if pos.shape[0] > 1 else 0, ps, h)
-    return arg, y, (x4, pos)
+        keep.append(pos)
+        pb, ps = s * axes, axes
+    if sd != 1 and d > 1:
+        x = x.contiguous()
+        keep.append(x)
+        sb, ss, sh = s * h * d, h * d, d
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    arg.extend((x.data_ptr(), y.data_ptr(), pos.data_ptr(), s, sb if b > 1 else 0, ss, sh, s * h * d, h * d, d,
+                pb if pn > 1 else 0, ps, h))
+    return y
 
 
 def _rope_axes(q, k, q_pos, k_pos, inv_freq, sections, pairing, inverse):
     ref = q if q is not None else k
-    dev = ref.device
     if not ref.is_cuda or (k is not None and not k.is_cuda):
         raise RuntimeError("rope_axes: CUDA tensors only (there is no CPU path)")
-    code = _lib.act_code(ref.dtype)
+    dev, dt = ref.device, ref.dtype
+    code = _lib.act_code(dt)
     if inv_freq.dim() != 1 or inv_freq.device != dev:
         raise ValueError(f"rope_axes: inv_freq must be 1-D on {dev}")
     first = q_pos if q is not None else k_pos
     axes = first.shape[-1] if first is not None and first.dim() in (2, 3) else 0
     if sections is None:  # every axis turns by all the frequencies, axis after axis
         sections, inv_freq = (inv_freq.shape[0],) * axes, inv_freq.repeat(axes)
+    sections = tuple(sections)
     if len(sections) != axes or sum(sections) != inv_freq.shape[0]:
-        raise ValueError(f"rope_axes: {axes} axes with {inv_freq.shape[0]} frequencies do not match sections {tuple(sections)}")
+        raise ValueError(f"rope_axes: {axes} axes with {inv_freq.shape[0]} frequencies do not match sections {sections}")
     if inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous():
         inv_freq = inv_freq.to(torch.float32).contiguous()
-    if q is not None and k is not None:
-        if k.dtype != q.dtype or k.device != dev or k.dim() != q.dim() or k.shape[-1] != q.shape[-1] or \
-                (q.dim() == 4 and k.shape[0] != q.shape[0]):
-            raise ValueError(f"rope_axes: q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} do not match")
-        if k_pos is not None and first is not None and k_pos.dtype != first.dtype:
-            raise ValueError("rope_axes: positions of q and k must have one dtype")
-    oq = _rope_operand(q, q_pos, axes, "q") if q is not None else None
-    ok = _rope_operand(k, k_pos, axes, "k") if k is not None else None
-    args = (ctypes.addressof(oq[0]) if oq else None, ctypes.addressof(ok[0]) if ok else None, code,
-            ref.shape[0] if ref.dim() == 4 else 1, ref.shape[-1], inv_freq.data_ptr(),
-            (ctypes.c_int32 * max(1, axes))(*sections), axes, _POS_CODES[(oq or ok)[2][1].dtype], _lib.PAIRING[pairing],
-            int(inverse))
+    arg, keep = array("q"), []
+    yq = yk = None
+    if q is not None:
+        if k is not None:
+            if k.dtype != dt or k.device != dev or k.dim() != q.dim() or k.shape[-1] != q.shape[-1] or \
+                    (q.dim() == 4 and k.shape[0] != q.shape[0]):
+                raise ValueError(f"rope_axes: q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} do not match")
+            if k_pos is not None and first is not None and k_pos.dtype != first.dtype:
+                raise ValueError("rope_axes: positions of q and k must have one dtype")
+        yq = _rope_operand(arg, q, q_pos, axes, "q", keep)
+    if k is not None:
+        yk = _rope_operand(arg, k, k_pos, axes, "k", keep)
+    at = arg.buffer_info()[0]
+    args = (at if q is not None else None, None if k is None else at + 104 if q is not None else at, code,
+            ref.shape[0] if ref.dim() == 4 else 1, ref.shape[-1], inv_freq.data_ptr(), _section_table(sections), axes,
+            _POS_CODES[first.dtype], _lib.PAIRING[pairing], int(inverse))
     lib = _lib.lib()
     if dev.index == torch.cuda.current_device():
         rc = lib.h3b_rope_axes(*args, _lib.raw_stream(dev.index))
     else:
         with torch.cuda.device(dev):
             rc = lib.h3b_rope_axes(*args, _lib.raw_stream(dev.index))
-    _lib.check(rc, "rope_axes")
-    return (oq[1] if oq else None), (ok[1] if ok else None)
+    if rc:
+        _lib.check(rc, "rope_axes")
+    return yq, yk
 
 
 class _RopeAxes(torch.autograd.Function):
@@ -176,6 +202,6 @@ def rope_axes(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions: O
     if pairing not in _lib.PAIRING:
         raise ValueError(f"pairing must be 'half' or 'adjacent', got {pairing!r}")
     k_positions = positions if k_positions is None else k_positions
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k)):
+    if torch.is_grad_enabled() and ((q is not None and q.requires_grad) or (k is not None and k.requires_grad)):
         return _RopeAxes.apply(q, k, positions, k_positions, inv_freq, sections, pairing, inverse)
     return _rope_axes(q, k, positions, k_positions, inv_freq, sections, pairing, inverse)
