@@ -59,7 +59,12 @@ int cross_launch(const h3b_attn_tensor* t, int dtype, int64_t B, int64_t Sq, int
   CrossParams P = cross_sizes(B, Sq, Sk, Hq, Hkv, D);
   const CrossWs w = cross_plan(P, mask_kind, backward);
   P.q = t[0], P.k = t[1], P.v = t[2], P.o = t[3];
-  if (backward) P.go = t[4], P.dq = t[5], P.dk = t[6], P.dv = t[7];
+  if (backward) {
+    P.go = t[4], P.dq = t[5], P.dk = t[6], P.dv = t[7];
+    P.wide = D % 16 == 0;
+    for (const h3b_attn_tensor* g : {&P.dq, &P.dk, &P.dv})
+      P.wide = P.wide && reinterpret_cast<uintptr_t>(g->ptr) % 32 == 0 && (g->stride_b | g->stride_s | g->stride_h) % 16 == 0;
+  }
   P.lse = lse;
   char* base = static_cast<char*>(ws);
   P.stats = reinterpret_cast<float*>(base + w.stats);

@@ -164,6 +164,9 @@ __global__ void __launch_bounds__(256) cross_stats_kernel(const CrossParams P, c
 }
 
 // ------------------------------------------------------------------------------------------------ dQ
+// What bounds the products here is the shared memory's bandwidth (two K-major operands there take all of it at N = 128), so a
+// unit's Q and G tiles, the A operands of S and dP, are moved to tensor memory once: S dP dQ Q G = 512 columns.  dS goes over
+// dP; the next S is issued as soon as S has been read, so it and the next dP run under the elementwise work.
 template <typename T, int DP, bool BIAS>
 __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
     cross_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG,
@@ -186,7 +189,9 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
   uint64_t* v_full = k_clean + KS;
   uint64_t* v_empty = v_full + VS;
   uint64_t* s_full = v_empty + VS;
-  uint64_t* dp_full = s_full + 2;
+  uint64_t* s_read = s_full + 1;
+  uint64_t* qg_tmem = s_read + 1;
+  uint64_t* dp_full = qg_tmem + 1;
   uint64_t* ds_full = dp_full + 1;
   uint64_t* part_full = ds_full + 1;
   uint64_t* dq_full = part_full + 1;
@@ -199,9 +204,9 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
   const bool masked = BIAS || P.kv_lens != nullptr;
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
+    mbar_init(q_empty, 16);
     mbar_init(g_full, 1);
-    mbar_init(g_empty, 1);
+    mbar_init(g_empty, 16);
     for (int s = 0; s < KS; ++s) {
       mbar_init(&k_full[s], 1);
       mbar_init(&k_empty[s], 1);
@@ -211,8 +216,9 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
       mbar_init(&v_full[s], 1);
       mbar_init(&v_empty[s], 1);
     }
-    mbar_init(&s_full[0], 1);
-    mbar_init(&s_full[1], 1);
+    mbar_init(s_full, 1);
+    mbar_init(s_read, 16);
+    mbar_init(qg_tmem, 16);
     mbar_init(dp_full, 1);
     mbar_init(ds_full, 16);
     mbar_init(part_full, 16);
@@ -235,14 +241,14 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   after_previous();
-  const uint32_t tDP = tmem + 2 * CT, tDQ = tmem + 3 * CT;  // S0 S1 dP dQ
+  const uint32_t tDP = tmem + CT, tDQ = tmem + 2 * CT, tQ = tmem + 3 * CT, tG = tQ + 64;  // S dP dQ Q G
 
   if (warp < 16) {
     // ------------------------------------------------------------------------------------------ P, dS
     regs_inc<96>();
     const int quarter = warp >> 2, row = threadIdx.x & (CT - 1);
     const uint32_t at = (static_cast<uint32_t>(warp & 3) << 21) + quarter * 32;  // this warp's lanes and columns
-    uint32_t sph = 0, dph = 0, xph = 0, sbuf = 0;
+    uint32_t ph = 0, xph = 0, uph = 0;
     float nlse2 = -INFINITY, delta = 0.f;
     bool ok = true;
     int64_t len = 0;
@@ -255,14 +261,41 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
         stat = P.stats + ((static_cast<int64_t>(u.b) * P.Hkv + u.hk) * P.q_tiles + u.tile) * (2 * CT);
         nlse2 = stat[row];  // -inf for rows outside and rows without keys: every p is 0
         delta = stat[CT + row];
+        // Q and G to tensor memory, this warp's 32 rows and quarter of the channels; the products of the unit before that
+        // read them there are complete (its last S and dP have been waited for)
+#pragma unroll 1
+        for (int m = 0; m < 2; ++m) {
+          if (!(ok = warp_wait(m ? g_full : q_full, uph, abort_flag))) break;
+          const unsigned char* tile = m ? sG : sQ;
+          uint32_t v[DP / 8];
+#pragma unroll
+          for (int i = 0; i < DP / 32; ++i) {
+            const int ch = quarter * (DP / 4) + 8 * i;
+            const uint4 x = *reinterpret_cast<const uint4*>(tile + (ch >> 6) * SUB_BYTES + row * 128 + ((((ch & 63) >> 3) ^ (row & 7)) << 4));
+            v[4 * i] = x.x, v[4 * i + 1] = x.y, v[4 * i + 2] = x.z, v[4 * i + 3] = x.w;
+          }
+          const uint32_t dst = (m ? tG : tQ) + (static_cast<uint32_t>(warp & 3) << 21) + quarter * (DP / 8);
+          if constexpr (DP == 128) tmem_st_32x32b_x16(dst, v);
+          else tmem_st_32x32b_x8(dst, v);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(m ? g_empty : q_empty);
+        }
+        if (!ok) break;
+        uph ^= 1;
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(qg_tmem);
       }
-      if (!(ok = warp_wait(&s_full[sbuf], sph, abort_flag))) break;
+      if (!(ok = warp_wait(s_full, ph, abort_flag))) break;
       tc_fence_after();
-      const uint32_t tS = tmem + sbuf * CT + at;
       float p[32];
       uint32_t r[32];
-      tmem_ld_32x32b_x32(tS, r);
+      tmem_ld_32x32b_x32(tmem + at, r);
       tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s_read);
       if constexpr (BIAS) {
         const float4* b4 = reinterpret_cast<const float4*>(P.bias2 + u.b * P.Skp + static_cast<int64_t>(u.t) * CT + quarter * 32);
 #pragma unroll
@@ -296,8 +329,8 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
 #pragma unroll
         for (int i = 0; i < 32; ++i) p[i] = 0.f;
       }
-      if (!(ok = warp_wait(dp_full, dph, abort_flag))) break;
-      dph ^= 1;
+      if (!(ok = warp_wait(dp_full, ph, abort_flag))) break;
+      ph ^= 1;
       tc_fence_after();
       tmem_ld_32x32b_x32(tDP + at, r);
       tmem_ld_wait();
@@ -325,13 +358,11 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         pk[i] = pack2<T>(p[2 * i] * (__uint_as_float(r[2 * i]) - delta), p[2 * i + 1] * (__uint_as_float(r[2 * i + 1]) - delta));
-      tmem_st_32x32b_x16(tS, pk);
+      tmem_st_32x32b_x16(tDP + at, pk);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(ds_full);
-      sbuf ^= 1;
-      if (sbuf == 0) sph ^= 1;
     }
   } else if (warp < 20) {
     // ------------------------------------------------------------------------------------------ epilogue
@@ -368,7 +399,7 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
         }
         if (!valid) continue;
         if (P.splits > 1) store_cols_f32(dst32 + 16 * c, o, P.scale, P.D - 16 * c);
-        else store_cols<T>(dst + 16 * c, o, P.scale, P.D - 16 * c);
+        else store_cols<T>(dst + 16 * c, o, P.scale, P.D - 16 * c, P.wide);
       }
       if (any) {
         tc_fence_before();
@@ -382,67 +413,59 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
       // -------------------------------------------------------------------------------------- MMA issue
       constexpr uint32_t idS = idesc_f16<T>(CT, CT, false), idD = idesc_f16<T>(CT, DP, true);
       constexpr uint64_t TILE16 = C::TILE >> 4;
-      const uint64_t rQ = desc_rows(smem_u32(sQ)), rG = desc_rows(smem_u32(sG)), rK = desc_rows(smem_u32(sK)),
-                     rV = desc_rows(smem_u32(sV));
-      const uint64_t cK = desc_chan(smem_u32(sK));
+      const uint64_t rK = desc_rows(smem_u32(sK)), rV = desc_rows(smem_u32(sV)), cK = desc_chan(smem_u32(sK));
       BwdCount<true> ws(P), wp(P), wd(P);  // the next S, dP and dQ product
       int sk = 0, pv = 0, dk = 0;
-      uint32_t skph = 0, pvph = 0, qph = 0, gph = 0, dsph = 0, dqph = 1, sbuf = 0, dbuf = 0;
+      uint32_t skph = 0, pvph = 0, srph = 1, uph = 0, dsph = 0, dqph = 1;
       bool ok = true;
       auto do_s = [&] {
-        if (!ok || !ws.valid()) return;
+        if (!ok) return;
         if (!(ok = warp_wait(&k_full[sk], skph, abort_flag))) return;
         if (masked && !(ok = warp_wait(&k_clean[sk], skph, abort_flag))) return;
+        if (!(ok = warp_wait(s_read, srph, abort_flag))) return;  // the S before has been read
+        srph ^= 1;
         if (ws.first) {
-          if (!(ok = warp_wait(q_full, qph, abort_flag))) return;
-          qph ^= 1;
+          if (!(ok = warp_wait(qg_tmem, uph, abort_flag))) return;
+          uph ^= 1;
         }
         tc_fence_after();
-        mma_rows<DP / 16>(tmem + sbuf * CT, rQ, rK + sk * TILE16, idS);
-        commit_one(&s_full[sbuf]);
-        if (ws.last()) commit_one(q_empty);
-        sbuf ^= 1;
+        mma_rows_ta<DP / 16>(tmem, tQ, rK + sk * TILE16, idS);
+        commit_one(s_full);
         if (++sk == KS) sk = 0, skph ^= 1;
         ws.next();
       };
       auto do_dp = [&] {
-        if (!ok || !wp.valid()) return;
+        if (!ok) return;
         if (!(ok = warp_wait(&v_full[pv], pvph, abort_flag))) return;
-        if (wp.first) {
-          if (!(ok = warp_wait(g_full, gph, abort_flag))) return;
-          gph ^= 1;
-        }
         tc_fence_after();
-        mma_rows<DP / 16>(tDP, rG, rV + pv * TILE16, idS);
+        mma_rows_ta<DP / 16>(tDP, tG, rV + pv * TILE16, idS);
         commit_one(dp_full);
         commit_one(&v_empty[pv]);
-        if (wp.last()) commit_one(g_empty);
         if (++pv == VS) pv = 0, pvph ^= 1;
         wp.next();
       };
-      do_s();
-      do_dp();
-      do_s();
       while (ok && wd.valid()) {
-        if (!(ok = warp_wait(ds_full, dsph, abort_flag))) break;  // dS is written, dP has been read
+        if (wd.first) {  // a unit begins: its Q and G are in tensor memory once the one before is through
+          do_s();
+          do_dp();
+          if (ws.valid() && ws.it == wd.it) do_s();
+        }
+        if (!ok || !(ok = warp_wait(ds_full, dsph, abort_flag))) break;  // dS is written, dP has been read
         dsph ^= 1;
-        tc_fence_after();
-        const bool same = wp.valid() && wp.it == wd.it;
-        if (same) do_dp();  // a new unit's dP waits for its G tile: not before this unit's last product
-        if (!ok) break;
         if (wd.first) {
           if (!(ok = warp_wait(dq_empty, dqph, abort_flag))) break;
           dqph ^= 1;
-          tc_fence_after();
         }
-        mma_chan<4>(tDQ, tmem + dbuf * CT, cK + dk * TILE16, idD, !wd.first);
+        tc_fence_after();
+        mma_chan<4>(tDQ, tDP, cK + dk * TILE16, idD, !wd.first);
         commit_one(&k_empty[dk]);
         if (wd.last()) commit_one(dq_full);
-        dbuf ^= 1;
         if (++dk == KS) dk = 0;
         wd.next();
-        if (!same) do_dp();
-        do_s();
+        if (wd.valid() && !wd.first) {
+          do_dp();
+          if (ws.valid() && ws.it == wd.it) do_s();
+        }
       }
     } else if (warp == 21) {
       if (lane == 0) {
@@ -732,7 +755,7 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
         if (!valid) continue;
         const float f = is_k ? P.scale : 1.f;
         if (P.kv_splits > 1) store_cols_f32(dk32 + (is_k ? 0 : part) + col, o, f, P.D - col);
-        else store_cols<T>((is_k ? dk : dv) + col, o, f, P.D - col);
+        else store_cols<T>((is_k ? dk : dv) + col, o, f, P.D - col, P.wide);
       }
       if (any) {
         tc_fence_before();

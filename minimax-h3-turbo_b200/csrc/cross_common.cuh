@@ -41,6 +41,7 @@ struct CrossParams {
   int splits;          // key splits of a unit (forward, dQ)
   int kv_splits;       // query splits of a unit (dK, dV)
   float scale, scale2;         // scale2 = scale log2(e)
+  bool wide;                   // backward: rows of dq, dk and dv start on 32-byte boundaries and are multiples of 32 bytes
   FastDiv by_g, by_hkv, by_units, by_splits, by_q_tiles, by_k_tiles, by_kv_splits;
 };
 
@@ -129,6 +130,11 @@ __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st_32x32b_x8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // One lane of a converged warp, the same one every time.  The MMA warp runs its loop as a whole and elects a lane only around
@@ -169,6 +175,13 @@ __device__ __forceinline__ void mma_rows(uint32_t d, uint64_t a, uint64_t b, uin
   if (elect_one())
 #pragma unroll
     for (int kk = 0; kk < STEPS; ++kk) mma_f16_ss(d, a + rows_step(kk), b + rows_step(kk), idesc, kk > 0);
+}
+// D = A B^T with A [128 rows, STEPS x 16 channels] in tensor memory (16-bit columns side by side), B K-major in shared memory
+template <int STEPS>
+__device__ __forceinline__ void mma_rows_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
+  if (elect_one())
+#pragma unroll
+    for (int kk = 0; kk < STEPS; ++kk) mma_f16_ts(d, a + kk * 8, b + rows_step(kk), idesc, kk > 0);
 }
 // D (+)= A B with A [128 rows x 128] in tensor memory and B's 128 rows in shared memory.  A's 16-bit columns lie side by
 // side (PARTS 1), or in PARTS parts at the first columns of the fp32 values that one group of warps each read.
@@ -284,19 +297,23 @@ __device__ __forceinline__ f32x2 f2_exp2(float xa, float xb) {
   return f2(__int_as_float(__float_as_int(pa) + na), __int_as_float(__float_as_int(pb) + nb));
 }
 
-// 16 columns of a row of results: 16-byte stores (n: valid columns from here on, a multiple of 8)
+// 16 columns of a row of results (n: valid columns from here on, a multiple of 8): one 32-byte store where every row allows it
+// (`wide`), else 16-byte ones.  A lane per row: an instruction touches 32 lines either way, so half the instructions count.
 template <typename T>
-__device__ __forceinline__ void store_cols(T* dst, const uint32_t (&o)[16], float w, int n) {
+__device__ __forceinline__ void store_cols(T* dst, const uint32_t (&o)[16], float w, int n, bool wide) {
+  uint32_t v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = pack2<T>(__uint_as_float(o[2 * i]) * w, __uint_as_float(o[2 * i + 1]) * w);
+  if (wide) {
+    if (n > 0)
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+                   "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                   : "memory");
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < 2; ++i)
-    if (8 * i < n) {
-      uint4 v;
-      uint32_t* vv = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        vv[e] = pack2<T>(__uint_as_float(o[8 * i + 2 * e]) * w, __uint_as_float(o[8 * i + 2 * e + 1]) * w);
-      *reinterpret_cast<uint4*>(dst + 8 * i) = v;
-    }
+    if (8 * i < n) *reinterpret_cast<uint4*>(dst + 8 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
 }
 __device__ __forceinline__ void store_cols_f32(float* dst, const uint32_t (&o)[16], float w, int n) {
 #pragma unroll
