@@ -125,13 +125,11 @@ __global__ void __launch_bounds__(256) cross_stats_kernel(const CrossParams P, c
     }
     unit -= P.B;
   }
-  int tile;
-  const int bh = P.by_q_tiles.divmod(unit, tile);
-  int hk;
-  const int b = P.by_hkv.divmod(bh, hk);
+  int tile, hk;  // key heads next to one another: CTAs that run together read the same stretch of memory
+  const int b = P.by_q_tiles.divmod(P.by_hkv.divmod(unit, hk), tile);
   const bool need = P.splits > 1 || ca_len(mask.kv_lens, b, P.Sk) > CT;  // the lengths before the mask
   const int ch = threadIdx.x % PER_ROW * 8;
-  float* st = P.stats + static_cast<int64_t>(unit) * (2 * CT);
+  float* st = P.stats + (static_cast<int64_t>(b * P.Hkv + hk) * P.q_tiles + tile) * (2 * CT);
   const T* ob = static_cast<const T*>(P.o.ptr) + b * P.o.stride_b + ch;
   const T* gb = static_cast<const T*>(P.go.ptr) + b * P.go.stride_b + ch;
   uint4 ov[PASSES], gv[PASSES];
