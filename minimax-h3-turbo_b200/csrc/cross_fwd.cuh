@@ -8,7 +8,9 @@
 //              operand type; the sum uses the unrounded values.  m is an exact maximum of the tiles so far, but taken anew
 //              only when a tile exceeds it by more than 8 (a factor 2^8: far from overflow in fp32 sums and fp16 P): P of a
 //              tile is computed with the m at hand, without a pass for the maximum before it, and only such a tile is gone
-//              over again, after its threads have rescaled O in tensor memory.
+//              over again, after its threads have rescaled O in tensor memory.  A unit's first tile, if all its keys are in use,
+//              is tried with m = 0, which does for normalised q and k: kept if the largest of every 64 scores is between 0
+//              and 8, as it may be for any later tile.
 //              After a unit's last tile the same threads take O / l through swizzled staging to a bulk tensor store, while
 //              the next unit's first scores are on their way; and the log-sum-exp.
 //   16         MMA issue: S = Q K^T (both from shared memory), O += P V (P from tensor memory, V channel-major)
@@ -246,7 +248,8 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
         const float4* b4 = BIAS ? reinterpret_cast<const float4*>(P.bias2 + u.b * P.Skp + static_cast<int64_t>(t) * CT + half * 64) : nullptr;
         uint32_t pk[32];
         f32x2 sum[2];
-        for (bool exact = t == u.t0;; exact = true) {
+        const bool guess = !BIAS && t == u.t0 && len - static_cast<int64_t>(t) * CT >= CT;
+        for (bool exact = t == u.t0 && !guess;; exact = true) {
           if (exact) {
             float top = -INFINITY;
             {
@@ -282,7 +285,7 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
             }
             m = top;
           }
-          const float nm = m == -INFINITY ? 0.f : -m;  // no key so far: every probability is exp2(-inf) = 0
+          const float nm = m == -INFINITY ? 0.f : -m;  // no key so far: the guess, or every probability is exp2(-inf) = 0
           float over[2] = {-INFINITY, -INFINITY};
           sum[0] = sum[1] = f2(0.f, 0.f);
           uint32_t r[2][16];
@@ -298,7 +301,12 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
           over[0] = max_nan(over[0], over[1]);
           if (over[0] != over[0]) sum[0] = f2(over[0], over[0]);  // a score that is not a number: so is the row
           // past this barrier both warps have read S
-          if (!group_any(bar, 64, over[0] > (m == -INFINITY ? -INFINITY : 8.f)) || exact) break;
+          const bool again = group_any(bar, 64, guess ? !(over[0] >= 0.f && over[0] <= 8.f) : over[0] > (m == -INFINITY ? -INFINITY : 8.f));
+          if (exact) break;
+          if (!again) {
+            if (guess) m = 0.f;
+            break;
+          }
         }
         l = f2_add(l, f2_add(sum[0], sum[1]));
         tmem_st_32x32b_x32(tS + half * 32, pk);

@@ -105,6 +105,17 @@ def test_large_scores_and_own_scale():
     check_all(q, k, v, do)
 
 
+@pytest.mark.parametrize("dt", [BF, FP])
+@pytest.mark.parametrize("shift", [-40.0, -2.0, 2.0, 40.0])
+def test_scores_far_from_zero(shift, dt):
+    """Every score of a row moved by the same amount, up or down; then only those of the first or of the later keys."""
+    for keys in (slice(None), slice(0, 128), slice(128, None), slice(64, 128)):
+        q, k, v, do = make(1, 300, 400, 3, 3, 64, dt, seed=21)
+        q[..., 0], k[..., 0] = 1, 0
+        k[:, keys, :, 0] = shift * 8  # scale 1/8
+        check_all(q, k, v, do)
+
+
 @pytest.mark.parametrize("sq", [3, 300])
 def test_masked_keys_may_hold_anything(sq):
     q, k, v, do = make(2, sq, 300, 4, 2, 64, BF, seed=5)
