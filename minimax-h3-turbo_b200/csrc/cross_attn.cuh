@@ -8,6 +8,7 @@ namespace h3b {
 // partial outputs and log-sum-exps; the backward's row vectors in tile order and partial gradients.
 struct CrossWs {
   size_t bias2 = 0, lens = 0, part_o = 0, part_lse = 0, stats = 0, part_dq = 0, part_dk = 0, total = 0;
+  int room = 1;  // splits that the forward's partial outputs have room for
 };
 static CrossWs cross_plan(CrossParams& P, int mask_kind, bool backward) {
   P.G = P.Hq / P.Hkv;
@@ -19,6 +20,7 @@ static CrossWs cross_plan(CrossParams& P, int mask_kind, bool backward) {
   P.splits = backward ? bwd_splits(P.q_tiles * heads, key_tiles) : fwd_splits(P.units * heads, key_tiles);
   P.kv_splits = backward ? bwd_splits(key_tiles * heads, P.q_tiles) : 1;
   P.by_g.set(P.G), P.by_hkv.set(P.Hkv), P.by_units.set(max(1, P.units)), P.by_splits.set(P.splits);
+  P.by_batch.set(max(1, P.B));
   P.by_q_tiles.set(max(1, P.q_tiles)), P.by_k_tiles.set(max(1, static_cast<int>(key_tiles))), P.by_kv_splits.set(P.kv_splits);
   CrossWs w;
   auto take = [&](size_t bytes) {
@@ -32,8 +34,9 @@ static CrossWs cross_plan(CrossParams& P, int mask_kind, bool backward) {
     w.lens = take(static_cast<size_t>(P.B) * 4);
   }
   if (!backward && P.splits > 1) {
-    w.part_o = take(rows * P.splits * P.D * 4);
-    w.part_lse = take(rows * P.splits * 4);
+    w.room = static_cast<int>(min(static_cast<int64_t>(min(64, 2 * P.splits)), key_tiles));
+    w.part_o = take(rows * w.room * P.D * 4);
+    w.part_lse = take(rows * w.room * 4);
   }
   if (backward) {
     w.stats = take(static_cast<size_t>(heads) * P.q_tiles * 2 * CT * 4);
@@ -84,6 +87,12 @@ int cross_launch(const h3b_attn_tensor* t, int dtype, int64_t B, int64_t Sq, int
       const int rc = cross_launch_after("cross_mask_kernel", cross_mask_kernel, dim3(P.B), CA_PREP, 0, st, m);
       if (rc) return rc;
     }
+  }
+  if (!backward && P.splits > 1 && P.kv_lens) {  // entries of different length: see ragged_unit
+    const int heads = P.units * P.Hkv;
+    P.ragged = max(cross_sms() / heads, P.splits * P.B);
+    P.splits = w.room;
+    P.by_splits.set(P.splits);
   }
   if (dtype == H3B_BF16) return backward ? bwd_launch<__nv_bfloat16>(P, m, st) : fwd_launch<__nv_bfloat16>(P, st);
   return backward ? bwd_launch<__half>(P, m, st) : fwd_launch<__half>(P, st);

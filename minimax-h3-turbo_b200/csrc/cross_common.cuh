@@ -39,10 +39,11 @@ struct CrossParams {
   int B, Hq, Hkv, G, D, nq;  // nq: queries of a tile
   int q_tiles, units;  // query tiles; pairs of them
   int splits;          // key splits of a unit (forward, dQ)
+  int ragged;          // forward: 0, or how many splits of all entries there are at most, of a size chosen from the lengths
   int kv_splits;       // query splits of a unit (dK, dV)
   float scale, scale2;         // scale2 = scale log2(e)
   bool wide;                   // backward: rows of dq, dk and dv start on 32-byte boundaries and are multiples of 32 bytes
-  FastDiv by_g, by_hkv, by_units, by_splits, by_q_tiles, by_k_tiles, by_kv_splits;
+  FastDiv by_g, by_hkv, by_units, by_splits, by_q_tiles, by_k_tiles, by_kv_splits, by_batch;
 };
 
 __device__ __forceinline__ int64_t ca_len(const int32_t* lens, int b, int64_t Sk) {

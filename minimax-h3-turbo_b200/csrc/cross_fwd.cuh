@@ -46,25 +46,66 @@ struct FwdUnit {
   bool two;                         // the second query tile exists
 };
 
-__device__ __forceinline__ FwdUnit fwd_unit(const CrossParams& P, int it) {
+__device__ __forceinline__ int key_tiles(const CrossParams& P, int b) {
+  return static_cast<int>((ca_len(P.kv_lens, b, P.Sk) + CT - 1) / CT);
+}
+// Where entries differ in length (P.ragged), splits have the same number of key tiles in all entries, the smallest that makes
+// no more splits than P.ragged, so that a short entry takes few SMs instead of many for a short while; an entry without keys
+// has one.  Sets `per`, and `first` to this CTA's only unit (n_items: none).  Called by whole warps.  5 queries over 12090, 8059
+// and 4028 keys, 56 over 8 heads x 128: 29.5 us, 34.9 with as many splits for every entry; equal lengths pay 2 to 3 us.
+__device__ __forceinline__ int ragged_splits(const CrossParams& P, int b, int per) { return max(1, (key_tiles(P, b) + per - 1) / per); }
+__device__ __forceinline__ void ragged_unit(const CrossParams& P, int n_items, int& per, int& first) {
+  const int lane = threadIdx.x & 31, equal = P.ragged / P.B;  // (as many splits for each entry are surely not too many)
+  int most = 1;
+  for (int b = lane; b < P.B; b += 32) most = max(most, key_tiles(P, b));
+  most = __reduce_max_sync(0xffffffffu, most);
+  per = (most + P.splits - 1) / P.splits;
+  for (int hi = max(per, (most + equal - 1) / equal); per < hi;) {
+    const int mid = (per + hi) / 2;
+    int n = 0;
+    for (int b = lane; b < P.B; b += 32) n += ragged_splits(P, b, mid);
+    if (__reduce_add_sync(0xffffffffu, n) <= P.ragged) hi = mid;
+    else per = mid + 1;
+  }
+  int pair, hk, r = P.by_hkv.divmod(P.by_units.divmod(blockIdx.x, pair), hk);  // the r-th split of all entries
+  first = n_items;
+  for (int b0 = 0; b0 < P.B; b0 += 32) {
+    const int n = b0 + lane < P.B ? ragged_splits(P, b0 + lane, per) : 0;
+    int upto = n;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    const unsigned after = __ballot_sync(0xffffffffu, upto > r);
+    if (after) {
+      const int at = __ffs(after) - 1, split = r - __shfl_sync(0xffffffffu, upto - n, at);
+      first = ((split * P.B + b0 + at) * P.Hkv + hk) * P.units + pair;
+      return;
+    }
+    r -= __shfl_sync(0xffffffffu, upto, 31);
+  }
+}
+
+// `per`: 0, or the key tiles of a split (ragged_unit).
+__device__ __forceinline__ FwdUnit fwd_unit(const CrossParams& P, int it, int per) {
   FwdUnit u;
   int pair;
-  const int r = P.by_splits.divmod(P.by_units.divmod(it, pair), u.split);
-  u.b = P.by_hkv.divmod(r, u.hk);
+  u.split = P.by_batch.divmod(P.by_hkv.divmod(P.by_units.divmod(it, pair), u.hk), u.b);
   u.tile0 = pair * 2;
   u.two = u.tile0 + 1 < P.q_tiles;
-  const int nt = static_cast<int>((ca_len(P.kv_lens, u.b, P.Sk) + CT - 1) / CT);
-  const int per = P.by_splits.div(nt + P.splits - 1);
+  const int nt = key_tiles(P, u.b);
+  if (!per) per = P.by_splits.div(nt + P.splits - 1);
   u.t0 = min(u.split * per, nt);
   u.t1 = min(u.t0 + per, nt);
   return u;
 }
 // the next unit with key tiles
-__device__ __forceinline__ bool fwd_next(const CrossParams& P, int& it, int n, FwdUnit& u) {
-  for (; it < n; it += gridDim.x) {
-    u = fwd_unit(P, it);
+template <bool RAGGED>
+__device__ __forceinline__ bool fwd_next(const CrossParams& P, int per, int& it, int n, FwdUnit& u) {
+  for (; it < n; it += RAGGED ? n : gridDim.x) {
+    u = fwd_unit(P, it, per);
     if (u.t1 > u.t0) {
-      it += gridDim.x;
+      it += RAGGED ? n : gridDim.x;
       return true;
     }
   }
@@ -141,7 +182,8 @@ __device__ __forceinline__ float max_chunk(const uint32_t (&r)[32], float scale2
   return fmaxf(tp[0], tp[1]);
 }
 
-template <typename T, int DP, bool BIAS>
+// RAGGED: one unit per CTA, chosen from the lengths (a variant of its own: inside the other one it cost 2 %)
+template <typename T, int DP, bool BIAS, bool RAGGED>
 __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
     cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                      const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, const CrossParams P) {
@@ -203,6 +245,8 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   after_previous();
+  int per = 0, first = blockIdx.x;  // this CTA's first unit
+  if constexpr (RAGGED) ragged_unit(P, n_items, per, first);
 
   if (warp < 16) {
     // ------------------------------------------------------------------------------------------ softmax
@@ -219,11 +263,11 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
     uint32_t sph = 0, oph = 0, uses = slot;  // uses: of the staging by both slots before this one
     bool dead = false;
     FwdUnit u, nxt;
-    int it = blockIdx.x;
-    for (bool have = fwd_next(P, it, n_items, u), more; have; u = nxt, have = more) {
+    int it = first;
+    for (bool have = fwd_next<RAGGED>(P, per, it, n_items, u), more; have; u = nxt, have = more) {
       if (slot == 1 && !u.two) {
         ++uses;
-        more = fwd_next(P, it, n_items, nxt);
+        more = fwd_next<RAGGED>(P, per, it, n_items, nxt);
         continue;
       }
       const int64_t len = ca_len(P.kv_lens, u.b, P.Sk);
@@ -237,7 +281,7 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
           dead = dead || !warp_wait(&s_full[slot], sph, abort_flag);
           if (lane == 0) mbar_arrive(&p_full[slot]);
         }
-        more = fwd_next(P, it, n_items, nxt);
+        more = fwd_next<RAGGED>(P, per, it, n_items, nxt);
       }
       for (int t = idle ? u.t1 : u.t0; t < u.t1; ++t) {
         dead = dead || !warp_wait(&s_full[slot], sph, abort_flag);
@@ -314,7 +358,7 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[slot]);
-        if (t == u.t0) more = fwd_next(P, it, n_items, nxt);  // while the next scores are on their way
+        if (t == u.t0) more = fwd_next<RAGGED>(P, per, it, n_items, nxt);  // while the next scores are on their way
       }
       // ---- the unit's output
       float la, lb;
@@ -395,8 +439,8 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
       int st = 0;
       uint32_t kph = 0, qph[2] = {0, 0}, pph[2] = {0, 0};
       FwdUnit cur, nxt;
-      int it = blockIdx.x;
-      bool have = fwd_next(P, it, n_items, cur), ok = true;
+      int it = first;
+      bool have = fwd_next<RAGGED>(P, per, it, n_items, cur), ok = true;
       auto qk = [&](int slot, int kst, bool first, bool last) {  // S of a slot; its Q tile arrives with the unit's first
         if (first) {
           if (!(ok = warp_wait(&q_full[slot], qph[slot], abort_flag))) return;
@@ -419,7 +463,7 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
         advance();
       }
       while (have && ok) {
-        const bool more = fwd_next(P, it, n_items, nxt);
+        const bool more = fwd_next<RAGGED>(P, per, it, n_items, nxt);
         for (int t = cur.t0; ok && t < cur.t1; ++t) {
           const bool last = t == cur.t1 - 1, then_qk = !last || more;
           const bool qk_last = last ? nxt.t1 - nxt.t0 == 1 : t + 2 == cur.t1;
@@ -470,15 +514,15 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
           ++fills;
           if (++st == C::STAGES) st = 0, kph ^= 1;
         };
-        int it = blockIdx.x;
-        bool have = fwd_next(P, it, n_items, u);
+        int it = first;
+        bool have = fwd_next<RAGGED>(P, per, it, n_items, u);
         if (have) {
           load_kv(u, -1, u, u.t0);
           load_q(u, 0);
           if (u.two) load_q(u, 1);
         }
         while (have && ok) {
-          const bool more = fwd_next(P, it, n_items, nxt);
+          const bool more = fwd_next<RAGGED>(P, per, it, n_items, nxt);
           for (int s = 0; more && s < (nxt.two ? 2 : 1); ++s)
             for (int p = 0; p < C::NSUB; ++p) tma_prefetch_5d(&tmQ, 64 * p, 0, nxt.hk, (nxt.tile0 + s) * P.nq, nxt.b);
           for (int t = u.t0; ok && t < u.t1; ++t) {
@@ -506,7 +550,7 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
       uint32_t kph = 0;
       FwdUnit u;
       bool ok = true;
-      for (int it = blockIdx.x; ok && fwd_next(P, it, n_items, u);) {
+      for (int it = first; ok && fwd_next<RAGGED>(P, per, it, n_items, u);) {
         const int64_t len = ca_len(P.kv_lens, u.b, P.Sk);
         for (int t = u.t0; ok && t < u.t1; ++t) {
           if (!(ok = warp_wait(&kv_full[st], kph, abort_flag))) break;
@@ -529,8 +573,15 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
       // ---------------------------------------------------------------------------------------- stores
       uint32_t ph = 0, uses = 0;
       bool ok = true;
-      for (int it = blockIdx.x; ok && it < n_items; it += gridDim.x) {
-        const FwdUnit u = fwd_unit(P, it);
+      for (int it = first; ok && it < n_items; it += RAGGED ? n_items : gridDim.x) {
+        const FwdUnit u = fwd_unit(P, it, per);
+        // the splits that this entry has not got
+        for (int r = lane; RAGGED && u.split == 0 && r < (u.two ? 2 : 1) * P.nq * P.G; r += 32) {
+          int h;
+          const int64_t q = static_cast<int64_t>(u.tile0) * P.nq + P.by_g.divmod(r, h), rows = static_cast<int64_t>(P.B) * P.Hq * P.Sq;
+          for (int x = ragged_splits(P, u.b, per); x < P.splits && q < P.Sq; ++x)
+            P.part_lse[x * rows + (static_cast<int64_t>(u.b) * P.Hq + u.hk * P.G + h) * P.Sq + q] = -INFINITY;
+        }
         for (int s = 0; ok && s < (u.two ? 2 : 1); ++s) {
           const int64_t s0 = static_cast<int64_t>(u.tile0 + s) * P.nq;
           if (u.t1 > u.t0) {
@@ -628,7 +679,7 @@ static int fwd_splits(int64_t units, int64_t key_tiles) {
   return best;
 }
 
-template <typename T, int DP, bool BIAS>
+template <typename T, int DP, bool BIAS, bool RAGGED>
 static int fwd_launch_cfg(const CrossParams& P, cudaStream_t st) {
   using C = FwdCfg<DP>;
   CUtensorMap q, k, v, o;
@@ -638,23 +689,27 @@ static int fwd_launch_cfg(const CrossParams& P, cudaStream_t st) {
   if (!rc) rc = cross_map_k(&v, P, P.Sk > 0 ? P.v : P.q, half);
   if (!rc) rc = cross_map_q(&o, P, P.o, half);
   if (rc) return rc;
-  auto kern = cross_fwd_kernel<T, DP, BIAS>;
+  auto kern = cross_fwd_kernel<T, DP, BIAS, RAGGED>;
   static std::atomic<bool> ready[CA_DEVICES];
   rc = cross_smem(reinterpret_cast<const void*>(kern), C::SMEM, ready, "cross_fwd_kernel shared memory");
   if (rc) return rc;
   const int64_t items = static_cast<int64_t>(P.units) * P.splits * P.Hkv * P.B;
   if (items >= (1 << 30)) return fail(H3B_ERR_UNSUPPORTED, "cross_attention: too many query tiles");
-  const int grid = static_cast<int>(items < cross_sms() ? items : cross_sms());
+  const int grid = RAGGED ? P.ragged * P.units * P.Hkv : static_cast<int>(items < cross_sms() ? items : cross_sms());
   rc = cross_launch_after("cross_fwd_kernel", kern, dim3(grid), C::THREADS, C::SMEM, st, q, k, v, o, P);
   if (rc || P.splits == 1) return rc;
   const int64_t rows = static_cast<int64_t>(P.B) * P.Hq * P.Sq;
   return cross_launch_after("cross_combine_kernel", cross_combine_kernel<T>, dim3(static_cast<unsigned>(rows)), 32, 0, st, P);
 }
 
+template <typename T, int DP>
+static int fwd_launch_dp(const CrossParams& P, cudaStream_t st) {
+  if (P.bias2) return P.ragged ? fwd_launch_cfg<T, DP, true, true>(P, st) : fwd_launch_cfg<T, DP, true, false>(P, st);
+  return P.ragged ? fwd_launch_cfg<T, DP, false, true>(P, st) : fwd_launch_cfg<T, DP, false, false>(P, st);
+}
 template <typename T>
 static int fwd_launch(const CrossParams& P, cudaStream_t st) {
-  if (P.D <= 64) return P.bias2 ? fwd_launch_cfg<T, 64, true>(P, st) : fwd_launch_cfg<T, 64, false>(P, st);
-  return P.bias2 ? fwd_launch_cfg<T, 128, true>(P, st) : fwd_launch_cfg<T, 128, false>(P, st);
+  return P.D <= 64 ? fwd_launch_dp<T, 64>(P, st) : fwd_launch_dp<T, 128>(P, st);
 }
 
 }  // namespace h3b

@@ -85,6 +85,16 @@ def test_many_queries_over_few_keys_and_a_long_stream():
     check_all(q, k, v, do, kv_lens=torch.tensor([12345], device=DEV))
 
 
+@pytest.mark.parametrize("lens", [[9000, 5000, 300, 0, 1], [0, 0, 129], [128], [700], [9000], [0], [50] * 39 + [4000]])
+@pytest.mark.parametrize("sq,hq,hkv,d,dt", [(1, 4, 4, 128, BF), (5, 14, 2, 64, FP), (70, 5, 1, 72, BF)])
+def test_few_queries_over_ragged_lengths(lens, sq, hq, hkv, d, dt):
+    b = len(lens)
+    q, k, v, do = make(b, sq, 9000 if b < 40 else 4000, hq, hkv, d, dt, seed=b + sq)
+    kv = torch.tensor(lens, device=DEV)
+    check_all(q, k, v, do, kv_lens=kv)
+    check_all(q, k, v, do, key_mask=torch.arange(k.shape[1], device=DEV) < kv.view(b, 1))
+
+
 @pytest.mark.parametrize("d,dt", [(128, BF), (64, FP)])
 @pytest.mark.parametrize("kind", ["none", "lens", "bias"])
 def test_more_work_than_ctas(d, dt, kind):
