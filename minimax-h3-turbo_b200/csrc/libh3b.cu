@@ -299,6 +299,14 @@ int h3b_rope_axes(const h3b_rope_operand* q, const h3b_rope_operand* k, int x_dt
                           static_cast<cudaStream_t>(stream));
 }
 
+// the strides of extents of one are not looked at
+static h3b_attn_tensor used_strides(h3b_attn_tensor t, int64_t B, int64_t S, int H) {
+  if (B <= 1) t.stride_b = 0;
+  if (S <= 1) t.stride_s = 0;
+  if (H <= 1) t.stride_h = 0;
+  return t;
+}
+
 static int check_cross(const h3b_attn_tensor* const* t, const bool* key_side, int n, int dtype, int64_t B, int64_t Sq,
                        int64_t Sk, int Hq, int Hkv, int D, float scale, const void* mask, int mask_kind, int64_t ldm,
                        const void* ws, size_t ws_bytes, bool backward) {
@@ -315,8 +323,9 @@ static int check_cross(const h3b_attn_tensor* const* t, const bool* key_side, in
   for (int i = 0; i < n; ++i) {
     if (!t[i]) return fail(H3B_ERR_ARG, "cross_attention: a tensor is missing");
     if (B == 0 || (key_side[i] ? Sk : Sq) == 0) continue;
-    if (!t[i]->ptr || !aligned(t[i]->ptr, 16) || t[i]->stride_b % 8 || t[i]->stride_s % 8 || t[i]->stride_h % 8 ||
-        t[i]->stride_b < 0 || t[i]->stride_s < 0 || t[i]->stride_h < 0)
+    const h3b_attn_tensor a = used_strides(*t[i], B, key_side[i] ? Sk : Sq, key_side[i] ? Hkv : Hq);
+    if (!a.ptr || !aligned(a.ptr, 16) || a.stride_b % 8 || a.stride_s % 8 || a.stride_h % 8 || a.stride_b < 0 ||
+        a.stride_s < 0 || a.stride_h < 0)
       return fail(H3B_ERR_ARG, "cross_attention: tensors must be 16-byte aligned with strides that are multiples of 8 elements");
   }
   const size_t need = cross_workspace(B, Sq, Sk, Hq, Hkv, D, mask_kind, backward);
@@ -341,7 +350,8 @@ int h3b_cross_attention(const h3b_attn_tensor* q, const h3b_attn_tensor* k, cons
                              ws_bytes, false);
   if (rc) return rc;
   if (B == 0 || Sq == 0) return H3B_OK;
-  const h3b_attn_tensor all[4] = {*q, *k, *v, *o};
+  h3b_attn_tensor all[4];
+  for (int i = 0; i < 4; ++i) all[i] = used_strides(*t[i], B, key_side[i] ? Sk : Sq, key_side[i] ? Hkv : Hq);
   return cross_launch(all, dtype, B, Sq, Sk, Hq, Hkv, head_dim, scale, kv_lens, mask, Sk > 0 ? mask_kind : H3B_MASK_NONE, ldm,
                       lse, workspace, false, static_cast<cudaStream_t>(stream));
 }
@@ -359,7 +369,8 @@ int h3b_cross_attention_backward(const h3b_attn_tensor* grad_o, const h3b_attn_t
   if (rc) return rc;
   if (B == 0 || (Sq == 0 && Sk == 0)) return H3B_OK;
   if (Sq > 0 && !lse) return fail(H3B_ERR_ARG, "cross_attention_backward: lse is missing");
-  const h3b_attn_tensor all[8] = {*q, *k, *v, *o, *grad_o, *dq, *dk, *dv};
+  h3b_attn_tensor all[8];
+  for (int i = 0; i < 8; ++i) all[i] = used_strides(*t[i], B, key_side[i] ? Sk : Sq, key_side[i] ? Hkv : Hq);
   return cross_launch(all, dtype, B, Sq, Sk, Hq, Hkv, head_dim, scale, kv_lens, mask, Sk > 0 ? mask_kind : H3B_MASK_NONE, ldm,
                       const_cast<float*>(lse), workspace, true, static_cast<cudaStream_t>(stream));
 }

@@ -13,6 +13,7 @@ from __future__ import annotations
 import math
 from array import array
 from dataclasses import dataclass
+from functools import lru_cache
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -54,10 +55,14 @@ def _readable(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _arg(t: torch.Tensor):
-    """(pointer, strides of batch, token and head) of a [B, S, heads, D] tensor; 0 for an extent of one."""
-    (b, s, h, _), (sb, ss, sh, _) = t.shape, t.stride()
-    return t.data_ptr(), sb if b > 1 else 0, ss if s > 1 else 0, sh if h > 1 else 0
+def _empty(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+@lru_cache(maxsize=4096)
+def _workspace_bytes(device: int, sizes: Tuple[int, ...], kind: int, backward: bool) -> int:
+    """A number per problem size and device: kept, since it takes a microsecond of a short call."""
+    return _lib.lib().h3b_cross_attention_workspace_bytes(*sizes, kind, backward)
 
 
 class _Problem:
@@ -67,15 +72,15 @@ class _Problem:
 
     def __init__(self, q, k, v, kv_lens, key_mask, scale):
         q, k, v = _batched(q, "q"), _batched(k, "k"), _batched(v, "v")
-        if not (q.is_cuda and k.is_cuda and v.is_cuda):
+        dev, dt = q.device, q.dtype
+        one_device = k.device == dev and v.device == dev
+        if not (q.is_cuda and (one_device or (k.is_cuda and v.is_cuda))):
             raise RuntimeError("cross_attention: CUDA tensors only (there is no CPU path)")
-        dt = q.dtype
         code = _CODES.get(dt)
         if code is None or k.dtype != dt or v.dtype != dt:
             raise RuntimeError(f"cross_attention: q, k and v must be bf16 or fp16, all of one type, got {q.dtype}, {k.dtype}, "
                                f"{v.dtype} (there is no fp32 path)")
-        dev = q.device
-        if k.device != dev or v.device != dev:
+        if not one_device:
             raise ValueError("cross_attention: q, k and v must be on one device")
         b, self.sq, hq, d = q.shape
         kb, sk, hkv, kd = k.shape
@@ -124,11 +129,12 @@ class _Problem:
         """Workspace, arguments and the call of one entry point; `tensors` in its order (lse after the fifth, backward)."""
         lib = _lib.lib()
         sizes = (self.b, self.sq, self.sk, self.hq, self.hkv, self.d)
-        n = lib.h3b_cross_attention_workspace_bytes(*sizes, self.kind, backward)
+        n = _workspace_bytes(self.dev.index, sizes, self.kind, backward)
         ws = torch.empty(n, dtype=torch.uint8, device=self.dev) if n else None
-        arr = array("q")  # struct h3b_attn_tensor, one after the other
+        arr = array("q")  # struct h3b_attn_tensor, one after the other: pointer, strides of batch, token and head
         for t in tensors:
-            arr.extend(_arg(t))
+            arr.append(t.data_ptr())
+            arr.extend(t.stride()[:3])
         at = arr.buffer_info()[0]
         ts = range(at, at + 32 * len(tensors), 32)
         mid = (self.code, *sizes, self.scale, _lib.ptr(self.lens), _lib.ptr(self.mask), self.kind, self.ldm)
@@ -142,7 +148,7 @@ class _Problem:
 
 
 def _forward(p: _Problem, want_lse: bool, out: Optional[torch.Tensor]):
-    o = torch.empty_like(p.q, memory_format=torch.contiguous_format) if out is None else out
+    o = _empty(p.q) if out is None else out
     lse = torch.empty(p.b, p.hq, p.sq, dtype=torch.float32, device=p.dev) if want_lse else None
     if p.dev.index == torch.cuda.current_device():
         p.call("cross_attention", (p.q, p.k, p.v, o), lse, False)
@@ -212,7 +218,7 @@ def cross_attention_backward(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
     if tuple(lse.shape) != (p.b, p.hq, p.sq) or lse.dtype != torch.float32 or lse.device != p.dev:
         raise ValueError(f"cross_attention: lse must be fp32 {(p.b, p.hq, p.sq)} on {p.dev}")
     lse = lse.contiguous()
-    dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (p.q, p.k, p.v))
+    dq, dk, dv = _empty(p.q), _empty(p.k), _empty(p.v)
     tensors = (do_, p.q, p.k, p.v, o_, dq, dk, dv)
     if p.dev.index == torch.cuda.current_device():
         p.call("cross_attention_backward", tensors, lse, True)

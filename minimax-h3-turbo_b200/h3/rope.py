@@ -119,7 +119,7 @@ def _rope_operand(arg: array, x: torch.Tensor, pos: Optional[torch.Tensor], axes
         x = x.contiguous()
         keep.append(x)
         sb, ss, sh = s * h * d, h * d, d
-    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    y = torch.empty_like(x) if x.is_contiguous() else torch.empty_like(x, memory_format=torch.contiguous_format)
     arg.extend((x.data_ptr(), y.data_ptr(), pos.data_ptr(), s, sb if b > 1 else 0, ss, sh, s * h * d, h * d, d,
                 pb if pn > 1 else 0, ps, h))
     return y

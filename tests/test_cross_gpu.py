@@ -201,6 +201,17 @@ def test_views_orders_and_alignment():
     assert torch.equal(cross.cross_attention(q, k[:1].expand(b, -1, -1, -1), v[:1].expand(b, -1, -1, -1))[0], want[0])
 
 
+def test_strides_of_extents_of_one():
+    """Views with one query, one key, one head or one entry: whatever the stride of that extent is, it is not used."""
+    base = torch.randn(3, 5, 7, 72, device=DEV, dtype=BF)[..., :64]
+    one_q, one_h = base.as_strided((3, 1, 7, 64), (2520, 3, 72, 1)), base.as_strided((3, 5, 1, 64), (2520, 504, 5, 1))
+    one_b = base.as_strided((1, 5, 7, 64), (9, 504, 72, 1))
+    check_all(one_q, base, base, torch.randn_like(one_q))
+    check_all(base, one_q, one_q, torch.randn_like(base))
+    check_all(base, one_h, one_h, torch.randn_like(base))
+    check_all(one_b, one_b, one_b, torch.randn_like(one_b))
+
+
 def test_offsets_past_32_bits():
     sk, d = 520, 128
     base = torch.empty(sk, 4_200_000, dtype=BF, device=DEV)  # rows 8.4 MB apart: the last starts past 2^31 elements
