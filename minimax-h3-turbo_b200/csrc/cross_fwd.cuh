@@ -25,8 +25,8 @@
 // Bound by the chain scores -> softmax -> second product: 3150 cycles for two query tiles x one key tile, of which the
 // products alone take 2048 (tensor pipe 62 % active; exponentials 47 %).  Two threads per row and two slots, because one
 // thread per row takes longer for a softmax than the other slot's products last.  bf16, 40 heads x 128 channels: 57840
-// queries x 1600 keys 1580 to 1650 us (1150 to 1200 TFLOP/s by the card's clock), 12090 x 512 135 us (938), one query x
-// 57840 keys 207 us (HBM, 5.7 TB/s).
+// queries x 1600 keys 1600 to 1680 us (1130 to 1180 TFLOP/s by the card's clock), 12090 x 512 128 us (990), one query x
+// 57840 keys 204 us (HBM, 5.8 TB/s).
 #include "cross_common.cuh"
 
 namespace h3b {
