@@ -16,8 +16,8 @@
 // keys before their product.  P and dS go back to tensor memory over the columns that their own warps read S or dP from.
 //
 // bf16, 40 heads x 128 channels, both with the row vectors: 2 x 4096 queries x 512 keys 323 to 333 us (902 to 929 TFLOP/s of
-// 7 products), 12090 x 1600 1152 to 1195 us (1160 to 1204).  Tensor pipe 68 % (dQ) and 72 % (dK, dV) active; neither HBM (8 %) nor the FMA pipe (40 %)
-// is near its limit: the chain scores -> elementwise work -> second product is.
+// 7 products), 12090 x 1600 1152 to 1195 us (1160 to 1204).  Tensor pipe 68 % (dQ) and 72 % (dK, dV) active; neither HBM
+// (8 %) nor the FMA pipe (40 %) is near its limit: the chain scores -> elementwise work -> second product is.
 #include "cross_common.cuh"
 
 namespace h3b {
