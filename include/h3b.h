@@ -173,6 +173,7 @@ typedef struct h3b_attn_tensor {
   void* ptr;
   int64_t stride_b, stride_s, stride_h;
 } h3b_attn_tensor;
+/* 0 where none is needed, and for sizes that the calls refuse (h3b_last_error says why). */
 size_t h3b_cross_attention_workspace_bytes(int64_t B, int64_t Sq, int64_t Sk, int Hq, int Hkv, int head_dim, int mask_kind,
                                            int backward);
 int h3b_cross_attention(const h3b_attn_tensor* q, const h3b_attn_tensor* k, const h3b_attn_tensor* v,

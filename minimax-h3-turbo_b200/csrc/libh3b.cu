@@ -307,16 +307,23 @@ static h3b_attn_tensor used_strides(h3b_attn_tensor t, int64_t B, int64_t S, int
   return t;
 }
 
+// what the plan of the launches (and so of the workspace) divides and multiplies by
+static int check_cross_sizes(int64_t B, int64_t Sq, int64_t Sk, int Hq, int Hkv, int D) {
+  if (B < 0 || Sq < 0 || Sk < 0 || Hq < 1 || Hkv < 1) return fail(H3B_ERR_ARG, "cross_attention: negative size or no heads");
+  if (Hq % Hkv || Hq / Hkv > 128) return fail(H3B_ERR_ARG, "cross_attention: query heads must be 1 to 128 times the key heads");
+  if (D < 8 || D > 128 || D % 8) return fail(H3B_ERR_ARG, "cross_attention: head_dim must be a multiple of 8, at most 128");
+  if (Sq > 0x7FFFFF00 || Sk > 0x7FFFFF00 || B > 65535 || Hq > 65535)
+    return fail(H3B_ERR_UNSUPPORTED, "cross_attention: at most 2^31 rows, 65535 batch entries and heads");
+  return H3B_OK;
+}
+
 static int check_cross(const h3b_attn_tensor* const* t, const bool* key_side, int n, int dtype, int64_t B, int64_t Sq,
                        int64_t Sk, int Hq, int Hkv, int D, float scale, const void* mask, int mask_kind, int64_t ldm,
                        const void* ws, size_t ws_bytes, bool backward) {
   if (dtype != H3B_BF16 && dtype != H3B_FP16) return fail(H3B_ERR_ARG, "cross_attention: q, k and v must be bf16 or fp16");
-  if (B < 0 || Sq < 0 || Sk < 0 || Hq < 1 || Hkv < 1) return fail(H3B_ERR_ARG, "cross_attention: negative size or no heads");
-  if (Hq % Hkv || Hq / Hkv > 128) return fail(H3B_ERR_ARG, "cross_attention: query heads must be 1 to 128 times the key heads");
-  if (D < 8 || D > 128 || D % 8) return fail(H3B_ERR_ARG, "cross_attention: head_dim must be a multiple of 8, at most 128");
+  const int rc = check_cross_sizes(B, Sq, Sk, Hq, Hkv, D);
+  if (rc) return rc;
   if (!(scale > 0.f) || !(scale < INFINITY)) return fail(H3B_ERR_ARG, "cross_attention: scale must be positive and finite");
-  if (Sq > 0x7FFFFF00 || Sk > 0x7FFFFF00 || B > 65535 || Hq > 65535)
-    return fail(H3B_ERR_UNSUPPORTED, "cross_attention: at most 2^31 rows, 65535 batch entries and heads");
   if (mask_kind != H3B_MASK_NONE && mask_kind != H3B_MASK_BOOL && mask_kind != H3B_MASK_BIAS)
     return fail(H3B_ERR_ARG, "cross_attention: unknown mask kind");
   if (mask_kind != H3B_MASK_NONE && B > 0 && Sk > 0 && (!mask || ldm < 0)) return fail(H3B_ERR_ARG, "cross_attention: the mask is missing");
@@ -336,7 +343,7 @@ static int check_cross(const h3b_attn_tensor* const* t, const bool* key_side, in
 
 size_t h3b_cross_attention_workspace_bytes(int64_t B, int64_t Sq, int64_t Sk, int Hq, int Hkv, int head_dim, int mask_kind,
                                            int backward) {
-  if (B <= 0 || Sq < 0 || Sk < 0 || Hq < 1 || Hkv < 1 || head_dim < 1) return 0;
+  if (B == 0 || check_cross_sizes(B, Sq, Sk, Hq, Hkv, head_dim)) return 0;
   return cross_workspace(B, Sq, Sk, Hq, Hkv, head_dim, mask_kind, backward != 0);
 }
 

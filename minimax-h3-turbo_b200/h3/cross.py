@@ -89,6 +89,8 @@ class _Problem:
                              f"{tuple(v.shape)}")
         if hkv == 0 or hq == 0 or hq % hkv:
             raise ValueError(f"cross_attention: {hq} query heads are not a multiple of {hkv} key heads")
+        if hq > 128 * hkv:
+            raise ValueError(f"cross_attention: at most 128 query heads to a key head, got {hq} to {hkv}")
         self.b, self.sk, self.hq, self.hkv, self.d, self.code, self.dev = b, sk, hq, hkv, d, code, dev
         self.scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
         self.q, self.k, self.v = _readable(q), _readable(k), _readable(v)
