@@ -948,10 +948,10 @@ static int bwd_launch_cfg(const CrossParams& P, const MaskArgs& mask, cudaStream
   using C = BwdCfg<DP>;
   CUtensorMap q, g, k, v;
   const bool half = std::is_same_v<T, __half>;
-  int rc = cross_map_q(&q, P, P.Sq > 0 ? P.q : P.k, half);
-  if (!rc) rc = cross_map_q(&g, P, P.Sq > 0 ? P.go : P.k, half);
-  if (!rc) rc = cross_map_k(&k, P, P.Sk > 0 ? P.k : P.q, half);
-  if (!rc) rc = cross_map_k(&v, P, P.Sk > 0 ? P.v : P.q, half);
+  int rc = cross_map_q(&q, P, P.Sq > 0 ? P.q : cross_stand_in(P.k), half);
+  if (!rc) rc = cross_map_q(&g, P, P.Sq > 0 ? P.go : cross_stand_in(P.k), half);
+  if (!rc) rc = cross_map_k(&k, P, P.Sk > 0 ? P.k : cross_stand_in(P.q), half);
+  if (!rc) rc = cross_map_k(&v, P, P.Sk > 0 ? P.v : cross_stand_in(P.q), half);
   if (rc) return rc;
   const int sms = cross_sms();
   auto kq = cross_dq_kernel<T, DP, BIAS>;

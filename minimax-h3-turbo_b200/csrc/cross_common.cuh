@@ -405,7 +405,7 @@ static int cross_map(CUtensorMap* map, const void* base, bool half, int rank, co
     box[i] = static_cast<cuuint32_t>(box_ext[i]);
     one[i] = 1;
     // the stride of an extent of one is never used; any valid value will do
-    if (i) strides[i - 1] = ext[i] > 1 && str[i] > 0 ? static_cast<cuuint64_t>(str[i]) * 2 : 16;
+    if (i) strides[i - 1] = ext[i] > 1 ? static_cast<cuuint64_t>(str[i]) * 2 : 16;
   }
   const CUresult r = fn(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank,
                         const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -413,6 +413,8 @@ static int cross_map(CUtensorMap* map, const void* base, bool half, int rank, co
   if (r != CUDA_SUCCESS) return fail(H3B_ERR_CUDA, "cuTensorMapEncodeTiled failed (code " + std::to_string(int(r)) + ")");
   return H3B_OK;
 }
+// What the map of an empty side is made of (nothing loads from it): a pointer and strides that a map may have.
+static h3b_attn_tensor cross_stand_in(const h3b_attn_tensor& t) { return h3b_attn_tensor{t.ptr, 8, 8, 8}; }
 // (channel, head of the group, key head, query, batch), a box of 64 channels x G heads x nq queries
 static int cross_map_q(CUtensorMap* map, const CrossParams& P, const h3b_attn_tensor& t, bool half) {
   const int64_t ext[5] = {P.D, P.G, P.Hkv, P.Sq, P.B};

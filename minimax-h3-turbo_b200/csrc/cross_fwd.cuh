@@ -685,8 +685,8 @@ static int fwd_launch_cfg(const CrossParams& P, cudaStream_t st) {
   CUtensorMap q, k, v, o;
   const bool half = std::is_same_v<T, __half>;
   int rc = cross_map_q(&q, P, P.q, half);
-  if (!rc) rc = cross_map_k(&k, P, P.Sk > 0 ? P.k : P.q, half);
-  if (!rc) rc = cross_map_k(&v, P, P.Sk > 0 ? P.v : P.q, half);
+  if (!rc) rc = cross_map_k(&k, P, P.Sk > 0 ? P.k : cross_stand_in(P.q), half);
+  if (!rc) rc = cross_map_k(&v, P, P.Sk > 0 ? P.v : cross_stand_in(P.q), half);
   if (!rc) rc = cross_map_q(&o, P, P.o, half);
   if (rc) return rc;
   auto kern = cross_fwd_kernel<T, DP, BIAS, RAGGED>;

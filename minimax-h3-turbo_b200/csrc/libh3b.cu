@@ -317,7 +317,9 @@ static int check_cross_sizes(int64_t B, int64_t Sq, int64_t Sk, int Hq, int Hkv,
   return H3B_OK;
 }
 
-static int check_cross(const h3b_attn_tensor* const* t, const bool* key_side, int n, int dtype, int64_t B, int64_t Sq,
+// t: the first n_in tensors are read, the others written.  Strides are checked where the extent is above one: tensor maps take
+// no 0 there, and what is written must not fold onto itself
+static int check_cross(const h3b_attn_tensor* const* t, const bool* key_side, int n, int n_in, int dtype, int64_t B, int64_t Sq,
                        int64_t Sk, int Hq, int Hkv, int D, float scale, const void* mask, int mask_kind, int64_t ldm,
                        const void* ws, size_t ws_bytes, bool backward) {
   if (dtype != H3B_BF16 && dtype != H3B_FP16) return fail(H3B_ERR_ARG, "cross_attention: q, k and v must be bf16 or fp16");
@@ -330,10 +332,12 @@ static int check_cross(const h3b_attn_tensor* const* t, const bool* key_side, in
   for (int i = 0; i < n; ++i) {
     if (!t[i]) return fail(H3B_ERR_ARG, "cross_attention: a tensor is missing");
     if (B == 0 || (key_side[i] ? Sk : Sq) == 0) continue;
-    const h3b_attn_tensor a = used_strides(*t[i], B, key_side[i] ? Sk : Sq, key_side[i] ? Hkv : Hq);
-    if (!a.ptr || !aligned(a.ptr, 16) || a.stride_b % 8 || a.stride_s % 8 || a.stride_h % 8 || a.stride_b < 0 ||
-        a.stride_s < 0 || a.stride_h < 0)
-      return fail(H3B_ERR_ARG, "cross_attention: tensors must be 16-byte aligned with strides that are multiples of 8 elements");
+    if (!t[i]->ptr || !aligned(t[i]->ptr, 16)) return fail(H3B_ERR_ARG, "cross_attention: tensors must be 16-byte aligned, none null");
+    const int64_t ext[3] = {B, key_side[i] ? Sk : Sq, key_side[i] ? Hkv : Hq};
+    const int64_t str[3] = {t[i]->stride_b, t[i]->stride_s, t[i]->stride_h};
+    for (int a = 0; a < 3; ++a)
+      if (ext[a] > 1 && (str[a] % 8 || str[a] < (i < n_in ? 8 : D)))
+        return fail(H3B_ERR_ARG, "cross_attention: strides must be multiples of 8 elements, at least 8, of outputs at least head_dim");
   }
   const size_t need = cross_workspace(B, Sq, Sk, Hq, Hkv, D, mask_kind, backward);
   if (need > 0 && (!ws || ws_bytes < need || !aligned(ws, 256)))
@@ -353,7 +357,7 @@ int h3b_cross_attention(const h3b_attn_tensor* q, const h3b_attn_tensor* k, cons
                         float* lse, void* workspace, size_t ws_bytes, void* stream) {
   const h3b_attn_tensor* t[4] = {q, k, v, o};
   const bool key_side[4] = {false, true, true, false};
-  const int rc = check_cross(t, key_side, 4, dtype, B, Sq, Sk, Hq, Hkv, head_dim, scale, mask, mask_kind, ldm, workspace,
+  const int rc = check_cross(t, key_side, 4, 3, dtype, B, Sq, Sk, Hq, Hkv, head_dim, scale, mask, mask_kind, ldm, workspace,
                              ws_bytes, false);
   if (rc) return rc;
   if (B == 0 || Sq == 0) return H3B_OK;
@@ -371,7 +375,7 @@ int h3b_cross_attention_backward(const h3b_attn_tensor* grad_o, const h3b_attn_t
                                  size_t ws_bytes, void* stream) {
   const h3b_attn_tensor* t[8] = {q, k, v, o, grad_o, dq, dk, dv};
   const bool key_side[8] = {false, true, true, false, false, false, true, true};
-  const int rc = check_cross(t, key_side, 8, dtype, B, Sq, Sk, Hq, Hkv, head_dim, scale, mask, mask_kind, ldm, workspace,
+  const int rc = check_cross(t, key_side, 8, 5, dtype, B, Sq, Sk, Hq, Hkv, head_dim, scale, mask, mask_kind, ldm, workspace,
                              ws_bytes, true);
   if (rc) return rc;
   if (B == 0 || (Sq == 0 && Sk == 0)) return H3B_OK;

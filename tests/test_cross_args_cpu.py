@@ -30,3 +30,40 @@ def test_workspace_of_refused_sizes_is_none():
                   (0, 4, 8, 1, 1, 64)):
         assert workspace_bytes(*sizes, _lib.MASK_BIAS, 1) == 0, sizes
     assert workspace_bytes(1, 4, 8, 128, 1, 64, 0, 1) > 0
+
+
+def tensor(p, b, s, h):
+    return (ctypes.c_int64 * 4)(p, b, s, h)
+
+
+def call(tensors, sizes, p, lens=None, mask=None, lse=None):
+    """The forward call for four tensors, the backward call for eight (in the entry's order), with an additive mask and without
+    the workspace that it needs: nothing is ever launched."""
+    a = [ctypes.addressof(t) for t in tensors]
+    rest = (_lib.BF16, *sizes, 0.125, lens, p if mask is None else mask, _lib.MASK_BIAS, 0)
+    lse = p if lse is None else lse
+    if len(a) == 4:
+        rc = _lib.lib().h3b_cross_attention(*a, *rest, lse, None, 0, None)
+    else:
+        rc = _lib.lib().h3b_cross_attention_backward(*a[:5], lse, *a[5:], *rest, None, 0, None)
+    assert rc == _lib.ERR_ARG
+    return _lib.lib().h3b_last_error().decode()
+
+
+@pytest.mark.parametrize("n", [4, 8])
+def test_strides_of_zero_and_outputs_that_fold_are_refused(n):
+    buf = ctypes.create_string_buffer(1 << 16)
+    p = ctypes.addressof(buf) + (-ctypes.addressof(buf)) % 256
+    sizes = (2, 200, 200, 2, 2, 64)  # every extent above one
+    fits = (200 * 128, 128, 64)
+    assert "workspace" in call([tensor(p, *fits)] * n, sizes, p)
+    assert "workspace" in call([tensor(p, 0, 0, 0)] * n, (1, 1, 1, 1, 1, 64), p)  # extents of one
+    written = (3,) if n == 4 else (5, 6, 7)
+    for i in range(n):
+        for axis in range(3):
+            for bad in (0, -64, 4) + ((56,) if i in written else ()):
+                st = list(fits)
+                st[axis] = bad
+                ts = [tensor(p, *fits) for _ in range(n)]
+                ts[i] = tensor(p, *st)
+                assert "strides" in call(ts, sizes, p), (i, axis, bad)
