@@ -137,7 +137,7 @@ int h3b_attn_merge(float* acc, float* acc_lse, const void* o, int64_t o_head_str
  *   pair j: channels (j, j + F) H3B_PAIR_HALF, (2 j, 2 j + 1) H3B_PAIR_ADJACENT; channels >= 2 F are copied
  *   (a, b) -> (a cos - b sin, a sin + b cos) in fp32, one rounding;  inverse != 0: by -theta (the gradient's direction)
  *   q, k       one of them may be null; S tokens (0 is valid) of `heads` heads, strides in elements, channels contiguous;
- *              any stride and alignment (16-byte aligned rows are faster); y must not overlap x
+ *              any stride (16-byte aligned rows are faster); pointers aligned to their elements; y must not overlap x or itself
  *   pos        [B, S, n_axes] of pos_dtype (fp32, int32, int64), axes contiguous, strides in elements (0: shared)
  *   inv_freq   DEVICE fp32 [F];  sections: HOST int32 [n_axes], n_axes <= H3B_MAX_AXES, 2 F <= head_dim <= 1024 */
 #define H3B_MAX_AXES 8
@@ -165,6 +165,7 @@ int h3b_rope_axes(const h3b_rope_operand* q, const h3b_rope_operand* k, int x_dt
  *              in use of a batch entry is taken off all of them first: the softmax does not change, and `lse` is that of
  *              the scores so shifted
  *   lse        optional fp32 [B, Hq, Sq]: natural log of sum_j exp(s_ij)
+ *   kv_lens, an additive mask and lse are 4-byte aligned
  * A query without keys (Sk = 0, kv_lens 0, all masked) gets o = 0 and lse = -inf.  What keys that are left out hold (NaN
  * and infinities too) never reaches a result.  Products take operands of dtype and add up in fp32; softmax and sums are
  * fp32; the probabilities are rounded to dtype for the second product.

@@ -295,6 +295,11 @@ int h3b_rope_axes(const h3b_rope_operand* q, const h3b_rope_operand* k, int x_dt
   const h3b_rope_operand* qq = q && q->S > 0 ? q : nullptr;
   const h3b_rope_operand* kk = k && k->S > 0 ? k : nullptr;
   if (!qq && !kk) return H3B_OK;
+  const size_t es = act_size(x_dtype), ps = pos_dtype == H3B_INT64 ? 8 : 4;
+  for (const h3b_rope_operand* o : {qq, kk})
+    if (o && (!aligned(o->x, es) || !aligned(o->y, es) || !aligned(o->pos, ps)))
+      return fail(H3B_ERR_ARG, "rope_axes: x, y and the positions must be aligned to their elements");
+  if (!aligned(inv_freq, 4)) return fail(H3B_ERR_ARG, "rope_axes: inv_freq must be 4-byte aligned");
   return rope_axes_launch(qq, kk, x_dtype, B, head_dim, inv_freq, sections, n_axes, pos_dtype, pairing, inverse,
                           static_cast<cudaStream_t>(stream));
 }
@@ -320,8 +325,8 @@ static int check_cross_sizes(int64_t B, int64_t Sq, int64_t Sk, int Hq, int Hkv,
 // t: the first n_in tensors are read, the others written.  Strides are checked where the extent is above one: tensor maps take
 // no 0 there, and what is written must not fold onto itself
 static int check_cross(const h3b_attn_tensor* const* t, const bool* key_side, int n, int n_in, int dtype, int64_t B, int64_t Sq,
-                       int64_t Sk, int Hq, int Hkv, int D, float scale, const void* mask, int mask_kind, int64_t ldm,
-                       const void* ws, size_t ws_bytes, bool backward) {
+                       int64_t Sk, int Hq, int Hkv, int D, float scale, const int32_t* kv_lens, const void* mask,
+                       int mask_kind, int64_t ldm, const float* lse, const void* ws, size_t ws_bytes, bool backward) {
   if (dtype != H3B_BF16 && dtype != H3B_FP16) return fail(H3B_ERR_ARG, "cross_attention: q, k and v must be bf16 or fp16");
   const int rc = check_cross_sizes(B, Sq, Sk, Hq, Hkv, D);
   if (rc) return rc;
@@ -329,6 +334,8 @@ static int check_cross(const h3b_attn_tensor* const* t, const bool* key_side, in
   if (mask_kind != H3B_MASK_NONE && mask_kind != H3B_MASK_BOOL && mask_kind != H3B_MASK_BIAS)
     return fail(H3B_ERR_ARG, "cross_attention: unknown mask kind");
   if (mask_kind != H3B_MASK_NONE && B > 0 && Sk > 0 && (!mask || ldm < 0)) return fail(H3B_ERR_ARG, "cross_attention: the mask is missing");
+  if (!aligned(kv_lens, 4) || !aligned(lse, 4) || (mask_kind == H3B_MASK_BIAS && !aligned(mask, 4)))
+    return fail(H3B_ERR_ARG, "cross_attention: kv_lens, an additive mask and lse must be 4-byte aligned");
   for (int i = 0; i < n; ++i) {
     if (!t[i]) return fail(H3B_ERR_ARG, "cross_attention: a tensor is missing");
     if (B == 0 || (key_side[i] ? Sk : Sq) == 0) continue;
@@ -357,8 +364,8 @@ int h3b_cross_attention(const h3b_attn_tensor* q, const h3b_attn_tensor* k, cons
                         float* lse, void* workspace, size_t ws_bytes, void* stream) {
   const h3b_attn_tensor* t[4] = {q, k, v, o};
   const bool key_side[4] = {false, true, true, false};
-  const int rc = check_cross(t, key_side, 4, 3, dtype, B, Sq, Sk, Hq, Hkv, head_dim, scale, mask, mask_kind, ldm, workspace,
-                             ws_bytes, false);
+  const int rc = check_cross(t, key_side, 4, 3, dtype, B, Sq, Sk, Hq, Hkv, head_dim, scale, kv_lens, mask, mask_kind, ldm, lse,
+                             workspace, ws_bytes, false);
   if (rc) return rc;
   if (B == 0 || Sq == 0) return H3B_OK;
   h3b_attn_tensor all[4];
@@ -375,8 +382,8 @@ int h3b_cross_attention_backward(const h3b_attn_tensor* grad_o, const h3b_attn_t
                                  size_t ws_bytes, void* stream) {
   const h3b_attn_tensor* t[8] = {q, k, v, o, grad_o, dq, dk, dv};
   const bool key_side[8] = {false, true, true, false, false, false, true, true};
-  const int rc = check_cross(t, key_side, 8, 5, dtype, B, Sq, Sk, Hq, Hkv, head_dim, scale, mask, mask_kind, ldm, workspace,
-                             ws_bytes, true);
+  const int rc = check_cross(t, key_side, 8, 5, dtype, B, Sq, Sk, Hq, Hkv, head_dim, scale, kv_lens, mask, mask_kind, ldm, lse,
+                             workspace, ws_bytes, true);
   if (rc) return rc;
   if (B == 0 || (Sq == 0 && Sk == 0)) return H3B_OK;
   if (Sq > 0 && !lse) return fail(H3B_ERR_ARG, "cross_attention_backward: lse is missing");

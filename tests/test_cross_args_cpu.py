@@ -67,3 +67,34 @@ def test_strides_of_zero_and_outputs_that_fold_are_refused(n):
                 ts = [tensor(p, *fits) for _ in range(n)]
                 ts[i] = tensor(p, *st)
                 assert "strides" in call(ts, sizes, p), (i, axis, bad)
+
+
+@pytest.mark.parametrize("n", [4, 8])
+def test_misaligned_vectors_are_refused(n):
+    buf = ctypes.create_string_buffer(1 << 12)
+    p = ctypes.addressof(buf) + (-ctypes.addressof(buf)) % 256
+    ts, sizes = [tensor(p, 0, 64, 0)] * n, (1, 4, 8, 1, 1, 64)
+    assert "workspace" in call(ts, sizes, p, lens=p + 4, mask=p + 4, lse=p + 4)
+    for kw in (dict(lens=p + 2), dict(mask=p + 1), dict(lse=p + 2)):
+        assert "4-byte aligned" in call(ts, sizes, p, **kw), kw
+
+
+def test_misaligned_rope_pointers_are_refused():
+    buf = ctypes.create_string_buffer(1 << 12)
+    p = ctypes.addressof(buf) + (-ctypes.addressof(buf)) % 256
+    sec = (ctypes.c_int32 * 1)(8)
+
+    def call_rope(x, y, pos, inv, dtype, pos_dtype, second):
+        op = (ctypes.c_int64 * 13)(x, y, pos, 4, 0, 128, 64, 0, 128, 64, 0, 1, 2)
+        at = ctypes.addressof(op)
+        rc = _lib.lib().h3b_rope_axes(None if second else at, at if second else None, dtype, 1, 64, inv, sec, 1, pos_dtype, 0,
+                                      0, None)
+        return rc, _lib.lib().h3b_last_error().decode()
+
+    for second in (False, True):
+        for dtype, size in ((_lib.BF16, 2), (_lib.FP16, 2), (_lib.FP32, 4)):
+            for bad in ((p + size // 2, p, p, p), (p, p + size // 2, p, p), (p, p, p + 2, p), (p, p, p, p + 2)):
+                rc, msg = call_rope(*bad, dtype, _lib.FP32, second)
+                assert rc == _lib.ERR_ARG and "aligned" in msg, (dtype, bad, rc, msg)
+            rc, msg = call_rope(p, p, p + 4, p, dtype, _lib.INT64, second)
+            assert rc == _lib.ERR_ARG and "aligned" in msg
