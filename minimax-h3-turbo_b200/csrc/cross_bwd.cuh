@@ -141,8 +141,8 @@ __global__ void __launch_bounds__(256) cross_stats_kernel(const CrossParams P, c
     const int64_t s = static_cast<int64_t>(tile) * P.nq + q;
     ov[a] = gv[a] = make_uint4(0, 0, 0, 0);
     if (need && q < P.nq && s < P.Sq && ch < P.D) {
-      ov[a] = __ldg(reinterpret_cast<const uint4*>(ob + s * P.o.stride_s + h * P.o.stride_h));
-      gv[a] = __ldg(reinterpret_cast<const uint4*>(gb + s * P.go.stride_s + h * P.go.stride_h));
+      ov[a] = *reinterpret_cast<const uint4*>(ob + s * P.o.stride_s + h * P.o.stride_h);
+      gv[a] = *reinterpret_cast<const uint4*>(gb + s * P.go.stride_s + h * P.go.stride_h);
     }
   }
   if (threadIdx.x < CT) {
@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
         const float4* b4 = reinterpret_cast<const float4*>(P.bias2 + u.b * P.Skp + static_cast<int64_t>(u.t) * CT + quarter * 32);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float4 bb = __ldg(b4 + i);
+          const float4 bb = b4[i];
           const float bv[4] = {bb.x, bb.y, bb.z, bb.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {

@@ -432,7 +432,8 @@ static int cross_map_k(CUtensorMap* map, const CrossParams& P, const h3b_attn_te
 
 // Launch that may begin while the kernel before it in the stream finishes: set-up (barriers, tensor memory, descriptors)
 // overlaps its tail.  (The kernel before gives no early signal: CTAs of the next one that wait on an SM cost the running one
-// a tenth of its time.)  Every kernel launched so calls after_previous() before it touches global memory.
+// a tenth of its time.)  Every kernel launched so calls after_previous() before it touches global memory, and reads it with
+// plain loads: the read-only path (__ldg) is for data that nobody writes while the kernel runs, its waiting part included.
 template <typename... KA, typename... A>
 static int cross_launch_after(const char* what, void (*kernel)(KA...), dim3 grid, int threads, int smem, cudaStream_t st, A&&... args) {
   cudaLaunchConfig_t cfg{};

@@ -117,23 +117,21 @@ __device__ __forceinline__ bool needs_zeroing(const CrossParams& P, int64_t len,
 }
 
 // 16 scores of a row -> probabilities: x = s scale2 + nm (nm = -m), p = exp2(x).  MASK 0: all keys in use; 1: keys from
-// `lim` on are out; 2: b4 is what each key adds, -inf: out, whatever its score.  Of unmasked keys every POLY-th pair goes
+// `lim` on are out; 2: `bias` is what each key adds, -inf: out, whatever its score.  Of unmasked keys every POLY-th pair goes
 // through the FMA pipe's exp2.  Adds to the row's sums, raises `top` (NaN stays).
 template <typename T, int MASK>
-__device__ __forceinline__ void soft_chunk(const uint32_t (&r)[16], float scale2, float nm, int lim, const float4* b4,
+__device__ __forceinline__ void soft_chunk(const uint32_t (&r)[16], float scale2, float nm, int lim, const float4 (&bias)[4],
                                            uint32_t* pk, f32x2 (&sum)[2], float (&top)[2]) {
   const f32x2 sc = f2(scale2, scale2), n2 = f2(nm, nm);
 #pragma unroll
   for (int i = 0; i < 8; i += 2) {
-    float4 bb;
-    if constexpr (MASK == 2) bb = __ldg(b4 + i / 2);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int k = 2 * (i + h);
       float xa, xb;
       const f32x2 sv = f2(__uint_as_float(r[k]), __uint_as_float(r[k + 1]));
       if constexpr (MASK == 2) {
-        const float ba = h ? bb.z : bb.x, bc = h ? bb.w : bb.y;
+        const float ba = h ? bias[i / 2].z : bias[i / 2].x, bc = h ? bias[i / 2].w : bias[i / 2].y;
         f2_split(f2_fma(sv, sc, f2_add(f2(ba, bc), n2)), xa, xb);
         if (ba == -INFINITY) xa = -INFINITY;
         if (bc == -INFINITY) xb = -INFINITY;
@@ -156,14 +154,13 @@ __device__ __forceinline__ void soft_chunk(const uint32_t (&r)[16], float scale2
 // the largest of 32 scores (MASK 2: of s scale2 + bias).  Runs once a unit: from a cold instruction cache, at some nine cycles
 // per instruction, so it is kept short (two scores per maximum, the scale once at the end).
 template <int MASK>
-__device__ __forceinline__ float max_chunk(const uint32_t (&r)[32], float scale2, int lim, const float4* b4, float top) {
+__device__ __forceinline__ float max_chunk(const uint32_t (&r)[32], float scale2, int lim, const float4 (&bias)[8], float top) {
   float tp[2] = {top, -INFINITY};
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     float x[4];
     if constexpr (MASK == 2) {
-      const float4 bb = __ldg(b4 + i);
-      const float bv[4] = {bb.x, bb.y, bb.z, bb.w};
+      const float bv[4] = {bias[i].x, bias[i].y, bias[i].z, bias[i].w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         x[e] = fmaf(__uint_as_float(r[4 * i + e]), scale2, bv[e]);
@@ -298,14 +295,20 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
             float top = -INFINITY;
             {
               uint32_t r[2][32];
+              float4 bias[8];
               tmem_ld_32x32b_x32(tS + half * 64, r[0]);
-              tmem_ld_32x32b_x32(tS + half * 64 + 32, r[1]);
-              tmem_ld_wait();
+              if constexpr (!BIAS) tmem_ld_32x32b_x32(tS + half * 64 + 32, r[1]);
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
-                if constexpr (BIAS) top = max_chunk<2>(r[c], P.scale2, 0, b4 + 8 * c, top);
-                else if (lim < 64) top = max_chunk<1>(r[c], P.scale2, lim - 32 * c, nullptr, top);
-                else top = max_chunk<0>(r[c], P.scale2, 0, nullptr, top);
+                if constexpr (BIAS) {  // on its way while the scores are; 32 of either at a time
+                  if (c) tmem_ld_32x32b_x32(tS + half * 64 + 32, r[1]);
+#pragma unroll
+                  for (int i = 0; i < 8; ++i) bias[i] = b4[8 * c + i];
+                }
+                if (BIAS || c == 0) tmem_ld_wait();
+                if constexpr (BIAS) top = max_chunk<2>(r[c], P.scale2, 0, bias, top);
+                else if (lim < 64) top = max_chunk<1>(r[c], P.scale2, lim - 32 * c, bias, top);
+                else top = max_chunk<0>(r[c], P.scale2, 0, bias, top);
               }
             }
             *mine = top;
@@ -336,11 +339,16 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
           tmem_ld_32x32b_x16(tS + half * 64, r[0]);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
+            float4 bias[4];  // on its way while the scores are
+            if constexpr (BIAS) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) bias[i] = b4[4 * c + i];
+            }
             tmem_ld_wait();
             if (c < 3) tmem_ld_32x32b_x16(tS + half * 64 + 16 * (c + 1), r[(c + 1) & 1]);
-            if constexpr (BIAS) soft_chunk<T, 2>(r[c & 1], P.scale2, nm, 0, b4 + 4 * c, pk + 8 * c, sum, over);
-            else if (lim < 64) soft_chunk<T, 1>(r[c & 1], P.scale2, nm, lim - 16 * c, nullptr, pk + 8 * c, sum, over);
-            else soft_chunk<T, 0>(r[c & 1], P.scale2, nm, 0, nullptr, pk + 8 * c, sum, over);
+            if constexpr (BIAS) soft_chunk<T, 2>(r[c & 1], P.scale2, nm, 0, bias, pk + 8 * c, sum, over);
+            else if (lim < 64) soft_chunk<T, 1>(r[c & 1], P.scale2, nm, lim - 16 * c, bias, pk + 8 * c, sum, over);
+            else soft_chunk<T, 0>(r[c & 1], P.scale2, nm, 0, bias, pk + 8 * c, sum, over);
           }
           over[0] = max_nan(over[0], over[1]);
           if (over[0] != over[0]) sum[0] = f2(over[0], over[0]);  // a score that is not a number: so is the row
