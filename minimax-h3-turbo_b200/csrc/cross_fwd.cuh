@@ -353,7 +353,10 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
           over[0] = max_nan(over[0], over[1]);
           if (over[0] != over[0]) sum[0] = f2(over[0], over[0]);  // a score that is not a number: so is the row
           // past this barrier both warps have read S
-          const bool again = group_any(bar, 64, guess ? !(over[0] >= 0.f && over[0] <= 8.f) : over[0] > (m == -INFINITY ? -INFINITY : 8.f));
+          // (rows that no query fills have no say: what they hold is left from another tile or kernel, and a maximum taken
+          // anew changes how every row's P is rounded)
+          const bool far = guess ? !(over[0] >= 0.f && over[0] <= 8.f) : over[0] > (m == -INFINITY ? -INFINITY : 8.f);
+          const bool again = group_any(bar, 64, valid & far);
           if (exact) break;
           if (!again) {
             if (guess) m = 0.f;
