@@ -414,8 +414,8 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
     if (warp == 20) {
       // -------------------------------------------------------------------------------------- MMA issue
       constexpr uint32_t idS = idesc_f16<T>(CT, CT, false), idD = idesc_f16<T>(CT, DP, true);
-      constexpr uint64_t TILE16 = C::TILE >> 4;
-      const uint64_t rK = desc_rows(smem_u32(sK)), rV = desc_rows(smem_u32(sV)), cK = desc_chan(smem_u32(sK));
+      constexpr uint32_t TILE16 = C::TILE >> 4;
+      const uint32_t rK = desc_rows(smem_u32(sK)), rV = desc_rows(smem_u32(sV)), cK = desc_chan(smem_u32(sK));
       BwdCount<true> ws(P), wp(P), wd(P);  // the next S, dP and dQ product
       int sk = 0, pv = 0, dk = 0;
       uint32_t skph = 0, pvph = 0, srph = 1, uph = 0, dsph = 0, dqph = 1;
@@ -773,10 +773,10 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
     if (warp == 20) {
       // -------------------------------------------------------------------------------------- MMA issue
       constexpr uint32_t idS = idesc_f16<T>(CT, CT, false), idD = idesc_f16<T>(CT, DP, true);
-      constexpr uint64_t TILE16 = C::TILE >> 4;
-      const uint64_t rQ = desc_rows(smem_u32(sQ)), rG = desc_rows(smem_u32(sG)), rK = desc_rows(smem_u32(sK)),
+      constexpr uint32_t TILE16 = C::TILE >> 4;
+      const uint32_t rQ = desc_rows(smem_u32(sQ)), rG = desc_rows(smem_u32(sG)), rK = desc_rows(smem_u32(sK)),
                      rV = desc_rows(smem_u32(sV));
-      const uint64_t cQ = desc_chan(smem_u32(sQ)), cG = desc_chan(smem_u32(sG));
+      const uint32_t cQ = desc_chan(smem_u32(sQ)), cG = desc_chan(smem_u32(sG));
       BwdCount<false> ws(P), wp(P), wd(P);  // the next S^T, dP^T, and the tile in hand
       int sq = 0, pg = 0, dq = 0, dg = 0;
       uint32_t sqph = 0, pgph = 0, kph = 0, vph = 0, ph = 0, aph = 1;

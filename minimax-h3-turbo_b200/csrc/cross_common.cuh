@@ -86,19 +86,26 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                "l"(src), "r"(bytes), "r"(smem_u32(bar))
                : "memory");
 }
-// D[tmem] (+)= A B, bf16/fp16 operands, fp32 accumulator; A from shared memory or from tensor memory
-__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// D[tmem] (+)= A B, bf16/fp16 operands, fp32 accumulator; A from shared memory or from tensor memory.  Operands in shared memory
+// are given by the low words of their descriptors (desc_rows, desc_chan): the high word is the same constant for all of them
+// (groups of 8 rows 1024 bytes apart, descriptor version 1, 128-byte swizzle) and is joined here, next to its use.  As 64-bit
+// values kept through the loops, the compiler (12.9) lost their swizzle bits in one variant of the gradient kernels after an edit
+// elsewhere in the kernel: the product then read the tile as if it were not swizzled.
+constexpr uint32_t DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n\t.reg .pred p;\n\t.reg .b32 h;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b32 h, %5;\n\t"
+      "mov.b64 a, {%1, h};\n\tmov.b64 b, {%2, h};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "n"(DESC_HI)
       : "memory");
 }
-__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n\t.reg .pred p;\n\t.reg .b32 h;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b32 h, %5;\n\t"
+      "mov.b64 b, {%2, h};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "n"(DESC_HI)
       : "memory");
 }
 // 32 lanes x 16 consecutive 32-bit columns: thread i of the warp gets its lane's 16 columns.
@@ -160,26 +167,25 @@ __host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool b_mn) {
 }
 // A tile of shared memory: 128 rows, DP channels, in parts of 64 channels (128 rows x 128 bytes, 128-byte swizzle).
 constexpr uint32_t SUB_BYTES = CT * 128;
-// Descriptor of a tile whose rows are the operand's M or N index (K-major); step kk (16 channels) adds rows_step(kk).
-// Offsets are in units of 16 bytes and stay inside the 14-bit address field (shared memory is under 256 KB).
-__device__ __forceinline__ uint64_t desc_rows(uint32_t tile) { return smem_desc_sw128(tile); }
-__host__ __device__ constexpr uint64_t rows_step(int kk) { return ((kk >> 2) * SUB_BYTES + (kk & 3) * 32) >> 4; }
+// Descriptor (its low word: start address, leading offset) of a tile whose rows are the operand's M or N index (K-major); step kk
+// (16 channels) adds rows_step(kk).  Offsets are in units of 16 bytes and stay inside the 14-bit address field (shared memory is
+// under 256 KB).
+__device__ __forceinline__ uint32_t desc_rows(uint32_t tile) { return (tile & 0x3FFFFu) >> 4 | 1u << 16; }
+__host__ __device__ constexpr uint32_t rows_step(int kk) { return ((kk >> 2) * SUB_BYTES + (kk & 3) * 32) >> 4; }
 // Descriptor of a tile whose channels are the operand's N index and whose rows are K (MN-major): 64-channel parts
 // SUB_BYTES apart (leading offset), groups of 8 rows 1024 bytes apart (stride offset); step kk (16 rows) adds chan_step(kk).
-__device__ __forceinline__ uint64_t desc_chan(uint32_t tile) {
-  return (smem_desc_sw128(tile) & ~(uint64_t(0x3FFF) << 16)) | (static_cast<uint64_t>(SUB_BYTES >> 4) << 16);
-}
-__host__ __device__ constexpr uint64_t chan_step(int kk) { return (kk * 2048) >> 4; }
+__device__ __forceinline__ uint32_t desc_chan(uint32_t tile) { return (tile & 0x3FFFFu) >> 4 | (SUB_BYTES >> 4) << 16; }
+__host__ __device__ constexpr uint32_t chan_step(int kk) { return (kk * 2048) >> 4; }
 // the products of one tile, in steps of 16: D (+)= A B^T with A and B K-major in shared memory
 template <int STEPS>
-__device__ __forceinline__ void mma_rows(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
   if (elect_one())
 #pragma unroll
     for (int kk = 0; kk < STEPS; ++kk) mma_f16_ss(d, a + rows_step(kk), b + rows_step(kk), idesc, kk > 0);
 }
 // D = A B^T with A [128 rows, STEPS x 16 channels] in tensor memory (16-bit columns side by side), B K-major in shared memory
 template <int STEPS>
-__device__ __forceinline__ void mma_rows_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
+__device__ __forceinline__ void mma_rows_ta(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
   if (elect_one())
 #pragma unroll
     for (int kk = 0; kk < STEPS; ++kk) mma_f16_ts(d, a + kk * 8, b + rows_step(kk), idesc, kk > 0);
@@ -187,7 +193,7 @@ __device__ __forceinline__ void mma_rows_ta(uint32_t d, uint32_t a, uint64_t b, 
 // D (+)= A B with A [128 rows x 128] in tensor memory and B's 128 rows in shared memory.  A's 16-bit columns lie side by
 // side (PARTS 1), or in PARTS parts at the first columns of the fp32 values that one group of warps each read.
 template <int PARTS>
-__device__ __forceinline__ void mma_chan(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_chan(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   constexpr int PER = CT / 16 / PARTS;
   if (elect_one())
 #pragma unroll

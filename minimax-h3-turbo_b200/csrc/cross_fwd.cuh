@@ -445,8 +445,8 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, 1)
     if (warp == 16) {
       // -------------------------------------------------------------------------------------- MMA issue
       constexpr uint32_t idQK = idesc_f16<T>(CT, CT, false), idPV = idesc_f16<T>(CT, DP, true);
-      constexpr uint64_t TILE16 = C::TILE >> 4;
-      const uint64_t dQ = desc_rows(smem_u32(sQ)), dK = desc_rows(smem_u32(sV) + C::TILE), dV = desc_chan(smem_u32(sV));
+      constexpr uint32_t TILE16 = C::TILE >> 4;
+      const uint32_t dQ = desc_rows(smem_u32(sQ)), dK = desc_rows(smem_u32(sV) + C::TILE), dV = desc_chan(smem_u32(sV));
       int st = 0;
       uint32_t kph = 0, qph[2] = {0, 0}, pph[2] = {0, 0};
       FwdUnit cur, nxt;
