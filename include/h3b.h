@@ -186,6 +186,8 @@ int h3b_cross_attention(const h3b_attn_tensor* q, const h3b_attn_tensor* k, cons
 /* Gradients of h3b_cross_attention's o with respect to q, k and v; o and lse are the forward's, the other arguments the
  * same.  grad_o, dq: as q; dk, dv: as k.  Shared heads add up; keys that are left out get zero gradients.  Every sum has a
  * fixed order (no atomics): the same call gives the same bits.  The mask has no gradient.
+ * P and its gradient are rounded to dtype for the second products, in fp16 after scaling by powers of two into its range, so
+ * that gradients of any size keep 11 bits.
  * workspace >= h3b_cross_attention_workspace_bytes(..., backward = 1). */
 int h3b_cross_attention_backward(const h3b_attn_tensor* grad_o, const h3b_attn_tensor* q, const h3b_attn_tensor* k,
                                  const h3b_attn_tensor* v, const h3b_attn_tensor* o, const float* lse,

@@ -5,9 +5,9 @@
 namespace h3b {
 
 // Workspace, parts 256-byte aligned: the prepared mask [B, Skp] and its key counts [B]; the forward's
-// partial outputs and log-sum-exps; the backward's row vectors in tile order and partial gradients.
+// partial outputs and log-sum-exps; the backward's row vectors in tile order, norms (used in fp16) and partial gradients.
 struct CrossWs {
-  size_t bias2 = 0, lens = 0, part_o = 0, part_lse = 0, stats = 0, part_dq = 0, part_dk = 0, total = 0;
+  size_t bias2 = 0, lens = 0, part_o = 0, part_lse = 0, stats = 0, g_norm2 = 0, g_top2 = 0, v_top2 = 0, v_all2 = 0, part_dq = 0, part_dk = 0, total = 0;
   int room = 1;  // splits that the forward's partial outputs have room for
 };
 static CrossWs cross_plan(CrossParams& P, int mask_kind, bool backward) {
@@ -40,6 +40,10 @@ static CrossWs cross_plan(CrossParams& P, int mask_kind, bool backward) {
   }
   if (backward) {
     w.stats = take(static_cast<size_t>(heads) * P.q_tiles * 2 * CT * 4);
+    w.g_norm2 = take(static_cast<size_t>(heads) * P.q_tiles * CT * 4);
+    w.g_top2 = take(static_cast<size_t>(heads) * P.q_tiles * 4);
+    w.v_top2 = take(static_cast<size_t>(heads) * key_tiles * 4);
+    w.v_all2 = take(static_cast<size_t>(heads) * 4);
     if (P.splits > 1) w.part_dq = take(rows * P.splits * P.D * 4);
     if (P.kv_splits > 1) w.part_dk = take(static_cast<size_t>(heads) * P.Sk * P.kv_splits * 2 * P.D * 4);
   }
@@ -71,6 +75,10 @@ int cross_launch(const h3b_attn_tensor* t, int dtype, int64_t B, int64_t Sq, int
   P.lse = lse;
   char* base = static_cast<char*>(ws);
   P.stats = reinterpret_cast<float*>(base + w.stats);
+  P.g_norm2 = reinterpret_cast<float*>(base + w.g_norm2);
+  P.g_top2 = reinterpret_cast<float*>(base + w.g_top2);
+  P.v_top2 = reinterpret_cast<float*>(base + w.v_top2);
+  P.v_all2 = reinterpret_cast<float*>(base + w.v_all2);
   P.part_dq = reinterpret_cast<float*>(base + w.part_dq);
   P.part_dk = reinterpret_cast<float*>(base + w.part_dk);
   P.part_o = reinterpret_cast<float*>(base + w.part_o);

@@ -10,6 +10,12 @@
 // Each computes S and dP: 7 products of the scores' size instead of 5.  The price of sharing them (dQ summed over key tiles
 // by atomics, in a changing order, through fp32 buffers in memory) is not paid: results have the same bits every time.
 // P and dS are rounded to the operand type for the second products (8 or 11 bits, relative to each element); sums are fp32.
+// fp16 has few exponents: P of 12090 keys lies where its steps are absolute, and so does dS of a gradient of ordinary size, or
+// past its range (do of 1e-3 over 12090 keys: dq off by 1.6e-2 if rounded as they are).  So both are held times a power of two
+// that the fp32 results are divided by: P times 2^14, dS times what keeps its bound 2 |g| max |v| below 2^14, |g| of the row for
+// dQ, the largest of the unit's rows for dK (there rows are what is summed over).  cross_stats_kernel takes the norms, for which it
+// reads the values once more: 2 x 12090 queries x 512 keys x 40 heads x 64 697 -> 737 us, 3 x 5 queries x 12090 keys, 56 over 8
+// heads x 128 108 -> 139 us, against the same kernels without the factors.
 //
 // Warps of both: 0-15 elementwise work, thread = row, four warps to the same 32 rows with 32 columns each; 16-19 epilogue
 // (accumulators -> global memory); 20 MMA issue; 21 copies; 22 (dQ) zeroes K rows of masked
@@ -104,15 +110,84 @@ template <int DP>
 struct BwdCfg {
   static constexpr int NSUB = DP / 64;
   static constexpr int TILE = NSUB * static_cast<int>(SUB_BYTES);
-  static constexpr int SMEM = 7 * TILE + 4 * CT * 4 + 512;  // 7 tiles, small vectors, barriers
+  static constexpr int SMEM = 7 * TILE + 4 * CT * 4 + 512;  // 7 tiles, small vectors, barriers and exponents (472 bytes)
   static constexpr int THREADS = 768;
   static constexpr uint32_t TMEM_COLS = 512;
 };
 
+// ------------------------------------------------------------------------------------------------ fp16's range
+constexpr int P_EXP = 14;  // fp16: P is held times 2^P_EXP
+template <typename T>
+constexpr bool scaled = std::is_same_v<T, __half>;
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + e) << 23); }
+// e of the factor 2^e for dS: |dS| = p |dP - delta| <= 2 |g| |v| (delta is a mean of dP), and 2^e times that is below 2^14.
+// Norms that are not finite, or 0, give the ends of the range: the results are not numbers, or 0, whatever the factor.
+__device__ __forceinline__ int ds_exp(float g2, float v2) {
+  const int k = ((__float_as_int(4.f * g2 * v2) >> 23) & 255) - 127;  // the bound's square is below 2^(k + 1)
+  return min(60, 14 - ((k + 2) >> 1));
+}
+// the largest of n numbers >= 0; called by whole warps
+__device__ __forceinline__ float warp_top(const float* p, int n) {
+  float top = 0.f;
+#pragma unroll 4
+  for (int i = threadIdx.x & 31; i < n; i += 32) top = fmaxf(top, p[i]);
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  return top;
+}
+// of all key tiles of a head; the dQ kernel leaves it for the dK/dV kernel, whose units may be shorter than that list
+__device__ __forceinline__ float values_top(const CrossParams& P, int b, int hk) {
+  const int n = static_cast<int>(P.Skp / CT), at = b * P.Hkv + hk;
+  const float top = warp_top(P.v_top2 + static_cast<int64_t>(at) * n, n);
+  if (threadIdx.x == 0) P.v_all2[at] = top;  // (every unit of the head writes the same number)
+  return top;
+}
+__device__ __forceinline__ float rows_top(const CrossParams& P, int b, int hk) {
+  return warp_top(P.g_top2 + (static_cast<int64_t>(b) * P.Hkv + hk) * P.q_tiles, P.q_tiles);
+}
+
 // ------------------------------------------------------------------------------------------------ row vectors
-// -lse in units of log2 (-inf for tile rows outside the tensor and rows without keys) and delta = g . o, in tile order.  One
-// row is DP / 8 lanes x 16 bytes; reads o and g once: HBM-bound.  delta is left out (0) where the dQ kernel surely takes it from
-// P and dP.  With a key mask the first B CTAs prepare it instead (a launch less).
+// -lse in units of log2 (-inf for tile rows outside the tensor and rows without keys; fp16: P_EXP more, so that what the kernels
+// take from it is P 2^P_EXP) and delta = g . o, in tile order.  One row is DP / 8 lanes x 16 bytes; reads o and g once: HBM-bound.
+// delta is left out (0) where the dQ kernel surely takes it from P and dP.  With a key mask the first B CTAs prepare it instead
+// (a launch less).  fp16: also the squared norms of g, and in CTAs before these those of the values in use, which it reads once.
+template <int N>
+__device__ __forceinline__ float lanes_sum(float d) {
+#pragma unroll
+  for (int o = N / 2; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+  return d;
+}
+// largest squared norm of a tile's values that are in use and finite (one that is not makes its results so by itself)
+template <typename T, int DP>
+__device__ __forceinline__ void tile_values_top(const CrossParams& P, const MaskArgs& mask, int unit) {
+  constexpr int PER_ROW = DP / 8, ROWS = 256 / PER_ROW, PASSES = CT / ROWS;
+  __shared__ float tops[8];
+  int tile, hk;
+  const int b = P.by_k_tiles.divmod(P.by_hkv.divmod(unit, hk), tile);
+  const int64_t len = ca_len(mask.kv_lens, b, P.Sk);
+  const int ch = threadIdx.x % PER_ROW * 8;
+  const T* vb = static_cast<const T*>(P.v.ptr) + b * P.v.stride_b + hk * P.v.stride_h + ch;
+  float top = 0.f;
+#pragma unroll
+  for (int a = 0; a < PASSES; ++a) {
+    const int64_t key = static_cast<int64_t>(tile) * CT + a * ROWS + threadIdx.x / PER_ROW;
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (key < len && ch < P.D && !(mask.mask && ca_mask_value(mask, b * mask.ldm + key) == -INFINITY))
+      x = *reinterpret_cast<const uint4*>(vb + key * P.v.stride_s);
+    const T* xe = reinterpret_cast<const T*>(&x);
+    float d = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) d = fmaf(static_cast<float>(xe[e]), static_cast<float>(xe[e]), d);
+    d = lanes_sum<PER_ROW>(d);
+    if (d < INFINITY) top = fmaxf(top, d);
+  }
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (float t : tops) top = fmaxf(top, t);
+    P.v_top2[(static_cast<int64_t>(b) * P.Hkv + hk) * (P.Skp / CT) + tile] = top;
+  }
+}
 template <typename T, int DP>
 __global__ void __launch_bounds__(256) cross_stats_kernel(const CrossParams P, const MaskArgs mask) {
   constexpr int PER_ROW = DP / 8, ROWS = 256 / PER_ROW, PASSES = CT / ROWS;
@@ -125,11 +200,20 @@ __global__ void __launch_bounds__(256) cross_stats_kernel(const CrossParams P, c
     }
     unit -= P.B;
   }
+  if constexpr (scaled<T>) {
+    const int n = static_cast<int>(P.Skp / CT) * P.Hkv * P.B;
+    if (unit < n) {
+      tile_values_top<T, DP>(P, mask, unit);
+      return;
+    }
+    unit -= n;
+  }
   int tile, hk;  // key heads next to one another: CTAs that run together read the same stretch of memory
   const int b = P.by_q_tiles.divmod(P.by_hkv.divmod(unit, hk), tile);
   const bool need = P.splits > 1 || ca_len(mask.kv_lens, b, P.Sk) > CT;  // the lengths before the mask
   const int ch = threadIdx.x % PER_ROW * 8;
-  float* st = P.stats + (static_cast<int64_t>(b * P.Hkv + hk) * P.q_tiles + tile) * (2 * CT);
+  const int64_t at = (static_cast<int64_t>(b) * P.Hkv + hk) * P.q_tiles + tile;
+  float* st = P.stats + at * (2 * CT);
   const T* ob = static_cast<const T*>(P.o.ptr) + b * P.o.stride_b + ch;
   const T* gb = static_cast<const T*>(P.go.ptr) + b * P.go.stride_b + ch;
   uint4 ov[PASSES], gv[PASSES];
@@ -140,28 +224,49 @@ __global__ void __launch_bounds__(256) cross_stats_kernel(const CrossParams P, c
     h += hk * P.G;
     const int64_t s = static_cast<int64_t>(tile) * P.nq + q;
     ov[a] = gv[a] = make_uint4(0, 0, 0, 0);
-    if (need && q < P.nq && s < P.Sq && ch < P.D) {
-      ov[a] = *reinterpret_cast<const uint4*>(ob + s * P.o.stride_s + h * P.o.stride_h);
+    if ((need || scaled<T>) && q < P.nq && s < P.Sq && ch < P.D) {
+      if (need) ov[a] = *reinterpret_cast<const uint4*>(ob + s * P.o.stride_s + h * P.o.stride_h);
       gv[a] = *reinterpret_cast<const uint4*>(gb + s * P.go.stride_s + h * P.go.stride_h);
     }
   }
+  float e = -INFINITY;  // of this thread's row, below
   if (threadIdx.x < CT) {
     int h;
     const int q = P.by_g.divmod(threadIdx.x, h);
     const int64_t s = static_cast<int64_t>(tile) * P.nq + q;
-    const float e = q < P.nq && s < P.Sq ? P.lse[(static_cast<int64_t>(b) * P.Hq + hk * P.G + h) * P.Sq + s] : -INFINITY;
-    st[threadIdx.x] = e == -INFINITY ? -INFINITY : -e * CA_LOG2E;
+    if (q < P.nq && s < P.Sq) e = P.lse[(static_cast<int64_t>(b) * P.Hq + hk * P.G + h) * P.Sq + s];
+    st[threadIdx.x] = e == -INFINITY ? -INFINITY : fmaf(-e, CA_LOG2E, scaled<T> ? P_EXP : 0.f);
   }
+  __shared__ float norms[CT], tops[CT / 32];
 #pragma unroll
   for (int a = 0; a < PASSES; ++a) {
     const T* oe = reinterpret_cast<const T*>(&ov[a]);
     const T* ge = reinterpret_cast<const T*>(&gv[a]);
+    const int row = a * ROWS + threadIdx.x / PER_ROW;
     float d = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) d = fmaf(static_cast<float>(oe[e]), static_cast<float>(ge[e]), d);
+    for (int i = 0; i < 8; ++i) d = fmaf(static_cast<float>(oe[i]), static_cast<float>(ge[i]), d);
+    d = lanes_sum<PER_ROW>(d);
+    if (threadIdx.x % PER_ROW == 0) st[CT + row] = d;
+    if constexpr (scaled<T>) {
+      float n = 0.f;
 #pragma unroll
-    for (int o = PER_ROW / 2; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-    if (threadIdx.x % PER_ROW == 0) st[CT + a * ROWS + threadIdx.x / PER_ROW] = d;
+      for (int i = 0; i < 8; ++i) n = fmaf(static_cast<float>(ge[i]), static_cast<float>(ge[i]), n);
+      n = lanes_sum<PER_ROW>(n);
+      if (threadIdx.x % PER_ROW == 0) norms[row] = n;
+    }
+  }
+  if constexpr (scaled<T>) {
+    __syncthreads();
+    if (threadIdx.x < CT) {
+      const float n = norms[threadIdx.x];
+      P.g_norm2[at * CT + threadIdx.x] = n;
+      float top = e != -INFINITY && n < INFINITY ? n : 0.f;  // of rows that have keys
+      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) P.g_top2[at] = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
   }
 }
 
@@ -201,6 +306,7 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
   uint64_t* done = dq_empty + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  signed char* row_exp = reinterpret_cast<signed char*>(tmem_slot + 2);  // fp16: [unit & 1][128] ds_exp of the rows
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const bool masked = BIAS || P.kv_lens != nullptr;
@@ -252,6 +358,8 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
     const uint32_t at = (static_cast<uint32_t>(warp & 3) << 21) + quarter * 32;  // this warp's lanes and columns
     uint32_t ph = 0, xph = 0, uph = 0;
     float nlse2 = -INFINITY, delta = 0.f;
+    float c = 1.f;  // fp16: what P 2^P_EXP (dP - delta) is multiplied by
+    int exp = 0, slot = 0;
     bool ok = true;
     int64_t len = 0;
     float* stat = nullptr;
@@ -263,6 +371,11 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
         stat = P.stats + ((static_cast<int64_t>(u.b) * P.Hkv + u.hk) * P.q_tiles + u.tile) * (2 * CT);
         nlse2 = stat[row];  // -inf for rows outside and rows without keys: every p is 0
         delta = stat[CT + row];
+        if constexpr (scaled<T>) {
+          const float g2 = P.g_norm2[((static_cast<int64_t>(u.b) * P.Hkv + u.hk) * P.q_tiles + u.tile) * CT + row];
+          exp = ds_exp(g2, values_top(P, u.b, u.hk));
+          c = pow2(exp - P_EXP);
+        }
         // Q and G to tensor memory, this warp's 32 rows and quarter of the channels; the products of the unit before that
         // read them there are complete (its last S and dP have been waited for)
 #pragma unroll 1
@@ -291,6 +404,10 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
       }
       if (!(ok = warp_wait(s_full, ph, abort_flag))) break;
       tc_fence_after();
+      if (scaled<T> && u.first()) {  // (this S was issued after the epilogue had taken the unit before the last, and with it its slot)
+        if (quarter == 0) row_exp[slot * CT + row] = static_cast<signed char>(exp);
+        slot ^= 1;
+      }
       float p[32];
       uint32_t r[32];
       tmem_ld_32x32b_x32(tmem + at, r);
@@ -353,13 +470,23 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
           if (!(ok = warp_wait(part_full, xph, abort_flag))) break;
           xph ^= 1;
           delta = (part[row] + part[CT + row]) + (part[2 * CT + row] + part[3 * CT + row]);
+          if constexpr (scaled<T>) delta *= pow2(-P_EXP);
           if (quarter == 0) stat[CT + row] = delta;
         }
       }
       uint32_t pk[16];
+      const float cd = -delta * c;
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        pk[i] = pack2<T>(p[2 * i] * (__uint_as_float(r[2 * i]) - delta), p[2 * i + 1] * (__uint_as_float(r[2 * i + 1]) - delta));
+      for (int i = 0; i < 16; ++i) {
+        if constexpr (scaled<T>) {  // c is a power of two: the same rounding as of dP - delta
+          float da, db;
+          const f32x2 d = f2_fma(f2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), f2(c, c), f2(cd, cd));
+          f2_split(f2_mul(f2(p[2 * i], p[2 * i + 1]), d), da, db);
+          pk[i] = pack2<T>(da, db);
+        } else {
+          pk[i] = pack2<T>(p[2 * i] * (__uint_as_float(r[2 * i]) - delta), p[2 * i + 1] * (__uint_as_float(r[2 * i + 1]) - delta));
+        }
+      }
       tmem_st_32x32b_x16(tDP + at, pk);
       tmem_st_wait();
       tc_fence_before();
@@ -374,6 +501,7 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
     const int qr = P.by_g.divmod(row, hg);
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
     uint32_t ph = 0;
+    int slot = 0;
     bool ok = true;
     BwdWalk<true> w(P);
     BwdTile u;
@@ -389,6 +517,11 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
       const int64_t rid = (static_cast<int64_t>(u.b) * P.Hq + u.hk * P.G + hg) * P.Sq + s;
       T* dst = static_cast<T*>(P.dq.ptr) + u.b * P.dq.stride_b + s * P.dq.stride_s + (u.hk * P.G + hg) * P.dq.stride_h;
       float* dst32 = P.part_dq + (static_cast<int64_t>(u.split) * P.B * P.Hq * P.Sq + rid) * P.D;
+      float f = P.scale;
+      if (scaled<T> && any) {
+        f *= pow2(-row_exp[slot * CT + row]);
+        slot ^= 1;
+      }
 #pragma unroll 1
       for (int c = 0; c < DP / 16; ++c) {
         uint32_t o[16];
@@ -400,8 +533,8 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
           for (int i = 0; i < 16; ++i) o[i] = 0;
         }
         if (!valid) continue;
-        if (P.splits > 1) store_cols_f32(dst32 + 16 * c, o, P.scale, P.D - 16 * c);
-        else store_cols<T>(dst + 16 * c, o, P.scale, P.D - 16 * c, P.wide);
+        if (P.splits > 1) store_cols_f32(dst32 + 16 * c, o, f, P.D - 16 * c);
+        else store_cols<T>(dst + 16 * c, o, f, P.D - 16 * c, P.wide);
       }
       if (any) {
         tc_fence_before();
@@ -594,6 +727,7 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
   uint64_t* done = acc_empty + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* unit_exp = reinterpret_cast<int*>(tmem_slot + 2);  // fp16: [unit & 1] ds_exp of a unit
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -652,7 +786,8 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
     uint32_t ph = 0, tph = 0;
     int ts = 0;
     bool ok = true, live = false;
-    float rb = 0.f;
+    float rb = 0.f, c = 1.f;  // c: as for dQ, one for all rows
+    int exp = 0, slot = 0;
     for (BwdWalk<false> w(P); ok && w.valid; w.next()) {
       const BwdTile& u = w.c;
       if (u.first()) {
@@ -662,10 +797,18 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
           rb = P.bias2[u.b * P.Skp + key];
           live = live && rb != -INFINITY;
         }
+        if constexpr (scaled<T>) {
+          exp = ds_exp(rows_top(P, u.b, u.hk), P.v_all2[u.b * P.Hkv + u.hk]);
+          c = pow2(exp - P_EXP);
+        }
       }
       if (!(ok = warp_wait(&t_full[ts], tph, abort_flag))) break;
       if (!(ok = warp_wait(s_full, ph, abort_flag))) break;
       tc_fence_after();
+      if (scaled<T> && u.first()) {  // (as for dQ)
+        if (threadIdx.x == 0) unit_exp[slot] = exp;
+        slot ^= 1;
+      }
       const float4* nl = reinterpret_cast<const float4*>(sT + ts * 2 * CT + quarter * 32);
       const float4* dl = reinterpret_cast<const float4*>(sT + ts * 2 * CT + CT + quarter * 32);
       float p[32];
@@ -703,8 +846,17 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
       for (int i = 0; i < 8; ++i) {
         const float4 d4 = dl[i];
         const float dv[4] = {d4.x, d4.y, d4.z, d4.w};
+        if constexpr (scaled<T>) {  // c is a power of two: the same rounding as of dP - delta
 #pragma unroll
-        for (int e = 0; e < 4; ++e) p[4 * i + e] *= __uint_as_float(r[4 * i + e]) - dv[e];
+          for (int e = 0; e < 4; e += 2) {
+            const int k = 4 * i + e;
+            const f32x2 d = f2_fma(f2(__uint_as_float(r[k]), __uint_as_float(r[k + 1])), f2(c, c), f2_mul(f2(dv[e], dv[e + 1]), f2(-c, -c)));
+            f2_split(f2_mul(f2(p[k], p[k + 1]), d), p[k], p[k + 1]);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) p[4 * i + e] *= __uint_as_float(r[4 * i + e]) - dv[e];
+        }
       }
       if (!live) {
 #pragma unroll
@@ -729,6 +881,7 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
     const int row = threadIdx.x & (CT - 1);
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
     uint32_t ph = 0;
+    int slot = 0;
     BwdWalk<false> w(P);
     BwdTile u;
     bool ok = true;
@@ -744,6 +897,12 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
       }
       T* dk = static_cast<T*>(P.dk.ptr) + u.b * P.dk.stride_b + key * P.dk.stride_s + u.hk * P.dk.stride_h;
       T* dv = static_cast<T*>(P.dv.ptr) + u.b * P.dv.stride_b + key * P.dv.stride_s + u.hk * P.dv.stride_h;
+      float f_k = P.scale, f_v = 1.f;
+      if (scaled<T> && any) {
+        f_k *= pow2(-unit_exp[slot]);
+        slot ^= 1;
+        f_v = pow2(-P_EXP);
+      }
       float* dk32 = P.part_dk + u.split * 2 * part + ((static_cast<int64_t>(u.b) * P.Hkv + u.hk) * P.Sk + key) * P.D;
 #pragma unroll 1
       for (int c = 0; c < 2 * (DP / 16); ++c) {
@@ -758,7 +917,7 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
           for (int i = 0; i < 16; ++i) o[i] = 0;
         }
         if (!valid) continue;
-        const float f = is_k ? P.scale : 1.f;
+        const float f = is_k ? f_k : f_v;
         if (P.kv_splits > 1) store_cols_f32(dk32 + (is_k ? 0 : part) + col, o, f, P.D - col);
         else store_cols<T>((is_k ? dk : dv) + col, o, f, P.D - col, P.wide);
       }
@@ -962,8 +1121,8 @@ static int bwd_launch_cfg(const CrossParams& P, const MaskArgs& mask, cudaStream
   if (rc) return rc;
   if (P.Sq > 0) {
     const int64_t n = static_cast<int64_t>(P.q_tiles) * P.splits * P.Hkv * P.B, rows = static_cast<int64_t>(P.B) * P.Hq * P.Sq;
-    if (n >= (1 << 30)) return fail(H3B_ERR_UNSUPPORTED, "cross_attention_backward: too many query tiles");
-    const int64_t tiles = static_cast<int64_t>(P.q_tiles) * P.Hkv * P.B;
+    const int64_t tiles = (P.q_tiles + (scaled<T> ? P.Skp / CT : 0)) * P.Hkv * P.B;
+    if (n >= (1 << 30) || tiles >= (1 << 30)) return fail(H3B_ERR_UNSUPPORTED, "cross_attention_backward: too many tiles");
     rc = cross_launch_after("cross_stats_kernel", cross_stats_kernel<T, DP>, dim3(static_cast<unsigned>(tiles + (mask.mask ? P.B : 0))), 256, 0,
                             st, P, mask);
     if (rc) return rc;

@@ -33,6 +33,10 @@ struct CrossParams {
   float* part_o;           // [splits, B * Hq * Sq, D] partial outputs, each normalised by its own sum
   float* part_lse;         // [splits, B * Hq * Sq] their log-sum-exps in units of log2
   float* stats;            // backward: [B, Hkv, q_tiles][-lse log2(e), delta][128 tile rows]
+  float* g_norm2;          // backward, fp16: [B, Hkv, q_tiles][128 tile rows] squared norms of g
+  float* g_top2;           // [B, Hkv, q_tiles] the largest of a tile's
+  float* v_top2;           // [B, Hkv, Skp / 128] the largest squared norm of the values in use of a key tile
+  float* v_all2;           // [B, Hkv] the largest of all tiles
   float* part_dq;          // [splits, B * Hq * Sq, D] partial dQ
   float* part_dk;          // [kv_splits][dK, dV][B * Hkv * Sk, D] partial dK and dV
   int64_t Sq, Sk, Skp;

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from cross_ref import cross_ref
 from minimax_h3_turbo_b200.h3 import cross
 
 pytestmark = pytest.mark.gpu
@@ -29,3 +30,71 @@ def test_same_bits_whatever_ran_before(g, d, dt):
         results.append((o, lse, *cross.cross_attention_backward(do, q, k, v, o, lse)))
     for other in results[1:]:
         assert all(torch.equal(a, b) for a, b in zip(results[0], other))
+
+
+def norm_error(got, want):
+    """Relative error over the whole tensor, and that of the exact result rounded to the same type."""
+    top = want.norm()
+    return float((got.double() - want).norm() / top), float((want.to(got.dtype).double() - want).norm() / top)
+
+
+# fp16 gradients hold their digits whatever the size of the output's gradient.  P, dS and the o that delta is taken from are
+# rounded to 11 bits: each at most 2^-11 of a term, 2^-11 / sqrt(3) = 2.8e-4 root mean square, three of them 5e-4 of the
+# result; twice that is asked, beside the rounding of the result itself (which has few digits where it is small).
+FP16_LIMIT = 1e-3
+
+
+@pytest.mark.parametrize("mask", [False, True])
+@pytest.mark.parametrize("std", [1.0, 1e-2, 1e-3])
+@pytest.mark.parametrize("sq,sk,hq,hkv,d", [(64, 12090, 2, 1, 64), (300, 12090, 1, 1, 128), (17, 57840, 3, 1, 64),
+                                            (500, 100, 2, 2, 64)])
+def test_small_fp16_gradients_keep_their_digits(sq, sk, hq, hkv, d, std, mask):
+    q, k, v, do = make(1, sq, sk, hq, hkv, d, FP, seed=sk)
+    do = (do.float() * std).half()
+    kw = {"key_mask": torch.zeros(1, sk, device=DEV)} if mask else {}
+    r = cross_ref(q, k, v, do=do, **kw)
+    o, lse = cross.cross_attention(q, k, v, return_lse=True, **kw)
+    for name, got in zip(("dq", "dk", "dv"), cross.cross_attention_backward(do, q, k, v, o, lse, **kw)):
+        err, own = norm_error(got, r[name])
+        assert err <= own + FP16_LIMIT, (name, err, own)
+
+
+def test_fp16_rows_of_different_size():
+    """Every query's dq has its own digits, next to rows whose gradients are a thousand times larger."""
+    q, k, v, do = make(1, 256, 12090, 1, 1, 64, FP, seed=1)
+    do[:, ::2] = (do[:, ::2].float() * 1e-3).half()
+    r = cross_ref(q, k, v, do=do)
+    o, lse = cross.cross_attention(q, k, v, return_lse=True)
+    dq = cross.cross_attention_backward(do, q, k, v, o, lse)[0]
+    for rows in (slice(0, None, 2), slice(1, None, 2)):
+        err, own = norm_error(dq[:, rows], r["dq"][:, rows])
+        assert err <= own + FP16_LIMIT, (rows, err, own)
+
+
+@pytest.mark.parametrize("sk", [3, 200])
+def test_large_fp16_gradients_do_not_overflow_inside(sk):
+    """dS is past fp16's range, every result is not."""
+    q, k, v, do = make(1, 16, sk, 2, 2, 64, FP, seed=2)
+    q, k, v, do = q * 0.05, k * 0.05, v * 4, (do.float() * 8000).half()
+    m = torch.full((1, sk), -40.0, device=DEV)
+    m[:, :3] = 0
+    r = cross_ref(q, k, v, do=do, key_mask=m)
+    assert all(float(r[n].abs().max()) < 60000 for n in ("dq", "dk", "dv"))
+    o, lse = cross.cross_attention(q, k, v, return_lse=True, key_mask=m)
+    for name, got in zip(("dq", "dk", "dv"), cross.cross_attention_backward(do, q, k, v, o, lse, key_mask=m)):
+        err, own = norm_error(got, r[name])
+        assert err <= own + FP16_LIMIT, (name, err, own)
+
+
+def test_fp16_gradients_do_not_see_what_masked_values_hold():
+    """Large finite values in keys that are left out: the same bits as with zeros there."""
+    q, k, v, do = make(2, 40, 300, 4, 2, 64, FP, seed=3)
+    mask = torch.rand(2, 300, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV) < 0.7
+    lens = torch.tensor([250, 120], device=DEV)
+    out = (~mask | (torch.arange(300, device=DEV) >= lens.view(2, 1))).view(2, 300, 1, 1)
+    res = []
+    for junk in (0.0, 6e4):
+        kj, vj = k.masked_fill(out, junk), v.masked_fill(out, junk)
+        o, lse = cross.cross_attention(q, kj, vj, key_mask=mask, kv_lens=lens, return_lse=True)
+        res.append((o, lse, *cross.cross_attention_backward(do, q, kj, vj, o, lse, key_mask=mask, kv_lens=lens)))
+    assert all(torch.equal(a, b) for a, b in zip(*res))
