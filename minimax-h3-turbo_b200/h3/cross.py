@@ -99,7 +99,9 @@ class _Problem:
         if kv_lens is not None:
             if kv_lens.shape != (b,) or kv_lens.dtype not in (torch.int32, torch.int64) or kv_lens.device != dev:
                 raise ValueError(f"cross_attention: kv_lens must be int32 or int64 [{b}] on {dev}")
-            self.lens = kv_lens.to(torch.int32).contiguous()
+            if kv_lens.dtype == torch.int64:  # before they lose their upper half
+                kv_lens = kv_lens.clamp(0, sk).to(torch.int32)
+            self.lens = kv_lens.contiguous()
         if key_mask is not None:
             self._set_mask(key_mask)
 

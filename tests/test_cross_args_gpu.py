@@ -17,3 +17,14 @@ def test_too_many_query_heads_to_a_key_head():
         cross.cross_attention_backward(q, q, k, k, q, torch.zeros(1, 129, 4, device=DEV))
     with pytest.raises(ValueError, match="128"):
         cross.cross_attention(q.requires_grad_(), k, k)
+
+
+def test_lengths_past_32_bits():
+    q, k, v = (torch.randn(4, s, 2, 64, device=DEV, dtype=BF) for s in (5, 30, 30))
+    far = torch.tensor([2 ** 32 + 5, -(2 ** 33) + 7, 2 ** 31, 2 ** 63 - 1], device=DEV)
+    near = torch.tensor([30, 0, 30, 30], dtype=torch.int32, device=DEV)
+    assert torch.equal(cross.cross_attention(q, k, v, kv_lens=far), cross.cross_attention(q, k, v, kv_lens=near))
+    strided = torch.tensor([7, 99, 5, 99, 30, 99, -1, 99], device=DEV)[::2]  # both types, any stride
+    want = cross.cross_attention(q, k, v, kv_lens=strided.clamp(min=0).to(torch.int32))
+    assert torch.equal(cross.cross_attention(q, k, v, kv_lens=strided), want)
+    assert torch.equal(cross.cross_attention(q, k, v, kv_lens=strided.to(torch.int32).repeat_interleave(2)[::2]), want)
