@@ -109,8 +109,6 @@ class _Problem:
         if m.dim() != 2 or m.shape[1] != self.sk or m.shape[0] not in (1, self.b) or m.device != self.dev:
             raise ValueError(f"cross_attention: key_mask must be [{self.b}, {self.sk}] (or [1, {self.sk}]) on {self.dev}, got "
                              f"{tuple(m.shape)} on {m.device}")
-        if m.requires_grad and torch.is_grad_enabled():
-            raise ValueError("cross_attention: key_mask has no gradient; detach it")
         if m.dtype == torch.bool:
             self.kind = _lib.MASK_BOOL
         elif m.is_floating_point():
@@ -191,8 +189,11 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_len
     others are copied.  kv_lens: int [B], keys in use of each entry of a padded batch.  key_mask: [B, Sk] (or [1, Sk]) bool,
     False leaves a key out; or floating point, added to the scaled scores (a key's log weight), -inf leaves it out; the
     entry's largest value is taken off first, which changes lse but not o.  A query without keys gets 0 (lse -inf); what
-    keys that are left out hold never reaches a result.  Differentiable in q, k and v.  out: a [B, Sq, Hq, D] tensor to
+    keys that are left out hold never reaches a result.  Differentiable in q, k and v (not in
+    key_mask, nor through lse).  out: a [B, Sq, Hq, D] tensor to
     write (16-byte aligned rows; not with gradients)."""
+    if key_mask is not None and key_mask.requires_grad and torch.is_grad_enabled():
+        raise ValueError("cross_attention: key_mask has no gradient; detach it")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         if out is not None:
             raise ValueError("cross_attention: out cannot be given where gradients are recorded")
@@ -217,7 +218,7 @@ def cross_attention_backward(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
     """Gradients (dq, dk, dv) of cross_attention's o with respect to q, k and v, from the gradient do of o; o and lse as
     cross_attention(..., return_lse=True) gave them for the same arguments.  The heads that share a key head add up in dk
     and dv; keys that are left out get zeros.  The same call gives the same bits."""
-    p = _Problem(q, k, v, kv_lens, None if key_mask is None else key_mask.detach(), scale)
+    p = _Problem(q, k, v, kv_lens, key_mask, scale)
     do_, o_ = _readable(p.rows(do, "do")), _readable(p.rows(o, "o"))
     if tuple(lse.shape) != (p.b, p.hq, p.sq) or lse.dtype != torch.float32 or lse.device != p.dev:
         raise ValueError(f"cross_attention: lse must be fp32 {(p.b, p.hq, p.sq)} on {p.dev}")

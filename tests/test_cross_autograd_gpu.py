@@ -1,0 +1,28 @@
+"""What autograd may ask of the rotary embedding and of cross attention: what they have is right, what they have not is
+refused, never left out without a word."""
+import pytest
+import torch
+
+from minimax_h3_turbo_b200.h3 import cross
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda")
+BF, FP = torch.bfloat16, torch.float16
+
+
+def make(b, sq, sk, hq, hkv, d, dt, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return [torch.randn(b, s, h, d, generator=g, device=DEV).to(dt) for s, h in ((sq, hq), (sk, hkv), (sk, hkv), (sq, hq))]
+
+
+@pytest.mark.parametrize("leaf", [(), (0,), (1, 2)])
+def test_a_mask_that_wants_a_gradient_is_refused(leaf):
+    ts = make(1, 5, 9, 2, 2, 64, BF)[:3]
+    for i in leaf:
+        ts[i].requires_grad_()
+    mask = torch.zeros(1, 9, device=DEV, requires_grad=True)
+    with pytest.raises(ValueError, match="key_mask"):
+        cross.cross_attention(*ts, key_mask=mask)
+    cross.cross_attention(*ts, key_mask=mask.detach())
+    with torch.no_grad():
+        cross.cross_attention(*ts, key_mask=mask)
