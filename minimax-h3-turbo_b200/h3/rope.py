@@ -196,12 +196,14 @@ def rope_axes(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions: O
     positions[axis(j)] * inv_freq[j]: sections (n_0, ..., n_{A-1}) deals the sum(sections) frequencies out to the axes in
     order; None lets every axis turn by all of inv_freq, as rope_angles does.  pairing "half": channels (j, j + F), F the
     number of pairs, as norm_rope_ rotates; "adjacent": (2j, 2j + 1).  Channels >= 2 F are copied.  inverse=True turns back:
-    the gradient's direction.  bf16, fp16 or fp32 (rounded once); differentiable in q and k."""
+    the gradient's direction.  bf16, fp16 or fp32 (rounded once); differentiable in q and k (not in positions or inv_freq)."""
     if q is None and k is None:
         raise ValueError("rope_axes: q and k are both None")
     if pairing not in _lib.PAIRING:
         raise ValueError(f"pairing must be 'half' or 'adjacent', got {pairing!r}")
     k_positions = positions if k_positions is None else k_positions
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (positions, k_positions, inv_freq)):
+        raise ValueError("rope_axes: positions and inv_freq have no gradient; detach them")
     if torch.is_grad_enabled() and ((q is not None and q.requires_grad) or (k is not None and k.requires_grad)):
         return _RopeAxes.apply(q, k, positions, k_positions, inv_freq, sections, pairing, inverse)
     return _rope_axes(q, k, positions, k_positions, inv_freq, sections, pairing, inverse)

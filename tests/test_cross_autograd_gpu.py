@@ -3,7 +3,7 @@ refused, never left out without a word."""
 import pytest
 import torch
 
-from minimax_h3_turbo_b200.h3 import cross
+from minimax_h3_turbo_b200.h3 import cross, rope
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda")
@@ -26,3 +26,15 @@ def test_a_mask_that_wants_a_gradient_is_refused(leaf):
     cross.cross_attention(*ts, key_mask=mask.detach())
     with torch.no_grad():
         cross.cross_attention(*ts, key_mask=mask)
+
+
+@pytest.mark.parametrize("leaf", [False, True])
+def test_rope_refuses_gradients_of_positions_and_frequencies(leaf):
+    q = torch.randn(6, 2, 64, device=DEV, requires_grad=leaf)
+    pos, inv = torch.rand(6, 1, device=DEV), torch.rand(32, device=DEV)
+    for args in ((pos.clone().requires_grad_(), inv, {}), (pos, inv.clone().requires_grad_(), {}),
+                 (pos, inv, {"k_positions": pos.clone().requires_grad_()})):
+        with pytest.raises(ValueError, match="gradient"):
+            rope.rope_axes(q, q.detach(), args[0], args[1], **args[2])
+        with torch.no_grad():
+            rope.rope_axes(q, q.detach(), args[0], args[1], **args[2])
