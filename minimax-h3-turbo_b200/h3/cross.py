@@ -160,6 +160,34 @@ def _forward(p: _Problem, want_lse: bool, out: Optional[torch.Tensor]):
     return o, lse
 
 
+def _backward(do, q, k, v, o, lse, kv_lens, key_mask, scale):
+    p = _Problem(q, k, v, kv_lens, key_mask, scale)
+    do_, o_ = _readable(p.rows(do, "do")), _readable(p.rows(o, "o"))
+    if tuple(lse.shape) != (p.b, p.hq, p.sq) or lse.dtype != torch.float32 or lse.device != p.dev:
+        raise ValueError(f"cross_attention: lse must be fp32 {(p.b, p.hq, p.sq)} on {p.dev}")
+    lse = lse.contiguous()
+    dq, dk, dv = _empty(p.q), _empty(p.k), _empty(p.v)
+    tensors = (do_, p.q, p.k, p.v, o_, dq, dk, dv)
+    if p.dev.index == torch.cuda.current_device():
+        p.call("cross_attention_backward", tensors, lse, True)
+    else:
+        with _guard(p.dev):
+            p.call("cross_attention_backward", tensors, lse, True)
+    return tuple(g if t.dim() == 4 else g.view(t.shape) for g, t in ((dq, q), (dk, k), (dv, v)))
+
+
+class _CrossAttentionGrads(torch.autograd.Function):
+    """The gradients where autograd records: they have no derivatives of their own, and say so when one is asked for."""
+
+    @staticmethod
+    def forward(ctx, *args):
+        return _backward(*args)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("cross_attention has no second derivatives")
+
+
 class _CrossAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, kv_lens, key_mask, scale):
@@ -217,20 +245,12 @@ def cross_attention_backward(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
                              ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Gradients (dq, dk, dv) of cross_attention's o with respect to q, k and v, from the gradient do of o; o and lse as
     cross_attention(..., return_lse=True) gave them for the same arguments.  The heads that share a key head add up in dk
-    and dv; keys that are left out get zeros.  The same call gives the same bits."""
-    p = _Problem(q, k, v, kv_lens, key_mask, scale)
-    do_, o_ = _readable(p.rows(do, "do")), _readable(p.rows(o, "o"))
-    if tuple(lse.shape) != (p.b, p.hq, p.sq) or lse.dtype != torch.float32 or lse.device != p.dev:
-        raise ValueError(f"cross_attention: lse must be fp32 {(p.b, p.hq, p.sq)} on {p.dev}")
-    lse = lse.contiguous()
-    dq, dk, dv = _empty(p.q), _empty(p.k), _empty(p.v)
-    tensors = (do_, p.q, p.k, p.v, o_, dq, dk, dv)
-    if p.dev.index == torch.cuda.current_device():
-        p.call("cross_attention_backward", tensors, lse, True)
-    else:
-        with _guard(p.dev):
-            p.call("cross_attention_backward", tensors, lse, True)
-    return tuple(g if t.dim() == 4 else g.view(t.shape) for g, t in ((dq, q), (dk, k), (dv, v)))
+    and dv; keys that are left out get zeros.  The same call gives the same bits.  There are no second derivatives: asking
+    for them raises RuntimeError."""
+    args = (do, q, k, v, o, lse, kv_lens, key_mask, scale)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in args[:6]):
+        return _CrossAttentionGrads.apply(*args)
+    return _backward(*args)
 
 
 @dataclass

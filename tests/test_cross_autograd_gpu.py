@@ -38,3 +38,24 @@ def test_rope_refuses_gradients_of_positions_and_frequencies(leaf):
             rope.rope_axes(q, q.detach(), args[0], args[1], **args[2])
         with torch.no_grad():
             rope.rope_axes(q, q.detach(), args[0], args[1], **args[2])
+
+
+def test_second_derivatives_of_attention_are_refused():
+    q, k, v, do = make(1, 5, 9, 2, 2, 64, FP)
+    q.requires_grad_()
+    g, = torch.autograd.grad(cross.cross_attention(q, k, v), q, do, create_graph=True)  # the first ones are there
+    with torch.no_grad():
+        o, lse = cross.cross_attention(q, k, v, return_lse=True)
+        assert torch.equal(g, cross.cross_attention_backward(do, q, k, v, o, lse)[0])
+    with pytest.raises(RuntimeError, match="second"):
+        (g.float().square().sum() + q.float().sum()).backward()
+    # gradients of the gradient's own argument too
+    w = do.clone().requires_grad_()
+    g, = torch.autograd.grad(cross.cross_attention(q, k, v), q, w, create_graph=True)
+    with pytest.raises(RuntimeError, match="second"):
+        torch.autograd.grad(g.float().sum() + w.float().sum(), w)
+    # and those that a direct call of the backward function would lose
+    o, lse = cross.cross_attention(q, k, v, return_lse=True)
+    dq = cross.cross_attention_backward(do, q, k, v, o, lse)[0]
+    with pytest.raises(RuntimeError, match="second"):
+        (dq.float().sum() + q.float().sum()).backward()
