@@ -181,7 +181,9 @@ class _RopeAxes(torch.autograd.Function):
         (q_pos, k_pos, inv_freq), (sections, pairing, inverse) = ctx.saved_tensors, ctx.rest
         if gq is None and gk is None:
             return (None,) * 8
-        dq, dk = _rope_axes(gq, gk, q_pos, k_pos, inv_freq, sections, pairing, not inverse)
+        # where autograd records (second derivatives), the rotation back is one of its own
+        turn = _RopeAxes.apply if torch.is_grad_enabled() else _rope_axes
+        dq, dk = turn(gq, gk, q_pos, k_pos, inv_freq, sections, pairing, not inverse)
         return dq, dk, None, None, None, None, None, None
 
 

@@ -59,3 +59,20 @@ def test_second_derivatives_of_attention_are_refused():
     dq = cross.cross_attention_backward(do, q, k, v, o, lse)[0]
     with pytest.raises(RuntimeError, match="second"):
         (dq.float().sum() + q.float().sum()).backward()
+
+
+@pytest.mark.parametrize("pairing", ["half", "adjacent"])
+def test_second_derivatives_of_the_rotation(pairing):
+    g = torch.Generator(device=DEV).manual_seed(0)
+    q, k = (torch.randn(2, s, 2, 64, generator=g, device=DEV).requires_grad_() for s in (7, 5))
+    pos = [torch.randint(0, 50, (s, 2), generator=g, device=DEV) for s in (7, 5)]
+    inv = torch.rand(24, generator=g, device=DEV)
+    call = lambda a, b, **kw: rope.rope_axes(a, b, pos[0], inv, (12, 12), k_positions=pos[1], pairing=pairing, **kw)  # noqa: E731
+    yq, yk = call(q, k)
+    gq, gk = torch.autograd.grad(yq.pow(3).sum() + yk.pow(3).sum(), (q, k), create_graph=True)
+    hq, hk = torch.autograd.grad(gq.pow(2).sum() + gk.pow(2).sum(), (q, k))
+    # with y = R x: g = R^T 3 y^2, and the gradient of |g|^2 is R^T (6 y * R 2 g)
+    with torch.no_grad():
+        ref = call(*(6 * y * 2 * t for y, t in zip((yq, yk), call(gq, gk))), inverse=True)
+    for have, want in zip((hq, hk), ref):
+        assert torch.allclose(have, want, rtol=1e-5, atol=1e-4 * float(want.abs().max()))
