@@ -21,7 +21,7 @@ import torch
 from .. import _lib
 from . import block as blk
 from . import qlinear as ql
-from .rope import rope_axes
+from .rope import no_tangents, rope_axes
 from .types import Weight
 
 _CODES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16}
@@ -220,6 +220,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_len
     keys that are left out hold never reaches a result.  Differentiable in q, k and v (not in
     key_mask, nor through lse).  out: a [B, Sq, Hq, D] tensor to
     write (16-byte aligned rows; not with gradients)."""
+    no_tangents("cross_attention", q, k, v, key_mask)
     if key_mask is not None and key_mask.requires_grad and torch.is_grad_enabled():
         raise ValueError("cross_attention: key_mask has no gradient; detach it")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
@@ -248,6 +249,7 @@ def cross_attention_backward(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
     and dv; keys that are left out get zeros.  The same call gives the same bits.  There are no second derivatives: asking
     for them raises RuntimeError."""
     args = (do, q, k, v, o, lse, kv_lens, key_mask, scale)
+    no_tangents("cross_attention", *args[:6], key_mask)
     if torch.is_grad_enabled() and any(t.requires_grad for t in args[:6]):
         return _CrossAttentionGrads.apply(*args)
     return _backward(*args)

@@ -15,6 +15,7 @@ from array import array
 from typing import Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 
@@ -72,6 +73,13 @@ def norm_rope_(q: torch.Tensor, k: torch.Tensor, wq: torch.Tensor, wk: torch.Ten
 
 # ------------------------------------------------------------------------------------------- rotary from positions
 _POS_CODES = {torch.float32: _lib.FP32, torch.int32: _lib.INT32, torch.int64: _lib.INT64}
+
+
+def no_tangents(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Raises where one of these carries a forward-mode tangent (requires_grad does not tell): the kernels would lose it."""
+    if getattr(forward_ad, "_current_level", 0) >= 0 and \
+            any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what} has no forward-mode derivatives")
 
 
 _section_tables = {}  # tuple of sections -> the C table of it
@@ -204,6 +212,7 @@ def rope_axes(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions: O
     if pairing not in _lib.PAIRING:
         raise ValueError(f"pairing must be 'half' or 'adjacent', got {pairing!r}")
     k_positions = positions if k_positions is None else k_positions
+    no_tangents("rope_axes", q, k, positions, k_positions, inv_freq)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (positions, k_positions, inv_freq)):
         raise ValueError("rope_axes: positions and inv_freq have no gradient; detach them")
     if torch.is_grad_enabled() and ((q is not None and q.requires_grad) or (k is not None and k.requires_grad)):

@@ -2,6 +2,7 @@
 refused, never left out without a word."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 from minimax_h3_turbo_b200.h3 import cross, rope
 
@@ -76,3 +77,18 @@ def test_second_derivatives_of_the_rotation(pairing):
         ref = call(*(6 * y * 2 * t for y, t in zip((yq, yk), call(gq, gk))), inverse=True)
     for have, want in zip((hq, hk), ref):
         assert torch.allclose(have, want, rtol=1e-5, atol=1e-4 * float(want.abs().max()))
+
+
+def test_forward_mode_is_refused():
+    q, k, v, t = make(1, 5, 9, 2, 2, 64, FP)
+    pos, inv = torch.rand(5, 1, device=DEV), torch.rand(32, device=DEV)
+    with fwd.dual_level():
+        dual = fwd.make_dual(q, t)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            cross.cross_attention(dual, k, v)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            rope.rope_axes(dual, None, pos, inv)
+        cross.cross_attention(q, k, v)  # others pass
+        rope.rope_axes(q, None, pos, inv)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            cross.cross_attention_backward(dual, q, k, v, q, torch.zeros(1, 2, 5, device=DEV))
