@@ -161,10 +161,10 @@ int h3b_rope_axes(const h3b_rope_operand* q, const h3b_rope_operand* k, int x_dt
  *              contiguous, every tensor 16-byte aligned; head_dim a multiple of 8, at most 128; scale > 0
  *   kv_lens    optional DEVICE int32 [B]: only keys j < kv_lens[b] take part
  *   mask       optional DEVICE key mask, rows ldm elements apart (0: shared): H3B_MASK_BOOL uint8 [B, Sk], 0 leaves the
- *              key out; H3B_MASK_BIAS fp32 [B, Sk] added to the scaled scores, -inf leaves the key out.  The largest bias
- *              in use of a batch entry is taken off all of them first: the softmax does not change, and `lse` is that of
- *              the scores so shifted
- *   lse        optional fp32 [B, Hq, Sq]: natural log of sum_j exp(s_ij)
+ *              key out; H3B_MASK_BIAS fp32 [B, Sk] added to the scaled scores, -inf leaves the key out
+ *   lse        optional fp32 [B, Hq, Sq]: natural log of sum_j exp(s_ij - t), t = 0, or with H3B_MASK_BIAS the largest bias in
+ *              use of the batch entry (a mask of large negative values keeps the scores' digits so, here and in the gradients,
+ *              which take this lse).  To merge results over disjoint key sets by their log-sum-exps, add t
  *   kv_lens, an additive mask and lse are 4-byte aligned
  * A query without keys (Sk = 0, kv_lens 0, all masked) gets o = 0 and lse = -inf.  What keys that are left out hold (NaN
  * and infinities too) never reaches a result.  Products take operands of dtype and add up in fp32; softmax and sums are

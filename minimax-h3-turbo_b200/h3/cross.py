@@ -2,7 +2,10 @@
 audio tokens or to a text encoder's states, audio tokens to the video, one new query to a long stream), with its
 gradients.  No reference counterpart: the reference's attention is one stream's own (h3turbo/h3/model.py:196-228).
 
-    s_ij = scale * q_i . k_j + bias_j        o_i = sum_j softmax_j(s_ij) v_j        lse_i = log sum_j exp(s_ij)
+    s_ij = scale * q_i . k_j + bias_j        o_i = sum_j softmax_j(s_ij) v_j        lse_i = log sum_j exp(s_ij - t)
+
+t is 0, or with an additive mask the largest bias in use of the batch entry: a mask of large negative values keeps the scores'
+digits that way, in lse and so in the gradients, which are computed from it.  `full_lse` adds t back.
 
 Kernels: h3b_cross_attention and h3b_cross_attention_backward (include/h3b.h).  bf16/fp16 CUDA tensors only, as the
 block's other operators; there is no CPU path.  `CrossLayer` runs them as a residual layer between W4A8 linears, with the
@@ -216,7 +219,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_len
     h // (Hq // Hkv)); views whose channels are contiguous and whose strides are multiples of 8 elements are read in place,
     others are copied.  kv_lens: int [B], keys in use of each entry of a padded batch.  key_mask: [B, Sk] (or [1, Sk]) bool,
     False leaves a key out; or floating point, added to the scaled scores (a key's log weight), -inf leaves it out; the
-    entry's largest value is taken off first, which changes lse but not o.  A query without keys gets 0 (lse -inf); what
+    entry's largest value is taken off first, which changes lse (full_lse puts it back) but not o.  A query without keys gets 0 (lse -inf); what
     keys that are left out hold never reaches a result.  Differentiable in q, k and v (not in
     key_mask, nor through lse).  out: a [B, Sq, Hq, D] tensor to
     write (16-byte aligned rows; not with gradients)."""
@@ -253,6 +256,25 @@ def cross_attention_backward(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
     if torch.is_grad_enabled() and any(t.requires_grad for t in args[:6]):
         return _CrossAttentionGrads.apply(*args)
     return _backward(*args)
+
+
+def full_lse(lse: torch.Tensor, *, kv_lens: Optional[torch.Tensor] = None, key_mask: Optional[torch.Tensor] = None
+             ) -> torch.Tensor:
+    """The log-sum-exp of the scores with their whole bias, [B, Hq, Sq] fp32, from lse as cross_attention(...,
+    return_lse=True) gave it for the same kv_lens and key_mask: adds the largest bias in use of each entry's additive mask.
+    This is what results over disjoint sets of keys are merged by (block.AttnMerger); cross_attention_backward takes lse as it
+    came."""
+    if lse.dim() != 3 or lse.dtype != torch.float32:
+        raise ValueError(f"full_lse: lse must be [B, Hq, Sq] fp32, got {tuple(lse.shape)} {lse.dtype}")
+    if key_mask is None or key_mask.dtype == torch.bool or key_mask.numel() == 0:
+        return lse
+    if key_mask.dim() != 2 or key_mask.shape[0] not in (1, lse.shape[0]) or not key_mask.is_floating_point():
+        raise ValueError(f"full_lse: key_mask must be [{lse.shape[0]}, Sk] (or [1, Sk]) bool or floating point")
+    bias = key_mask.float()
+    if kv_lens is not None:
+        bias = bias.masked_fill(torch.arange(bias.shape[1], device=bias.device) >= kv_lens.view(-1, 1), -math.inf)
+    top = bias.amax(1)
+    return lse + top.masked_fill(top == -math.inf, 0.0).view(-1, 1, 1)
 
 
 @dataclass
