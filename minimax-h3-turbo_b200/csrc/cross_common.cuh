@@ -288,7 +288,8 @@ __device__ __forceinline__ float max_nan(float a, float b, float c) {
 }
 // exp2 of two numbers <= 16 on the FMA pipe (the special function unit's 4 results per cycle and scheduler are the bound of
 // softmax loops): x = n + f, |f| <= 1/2 by adding and taking off 1.5 * 2^23; 2^f by a degree-4 polynomial fitted to the least
-// largest relative error (2.6e-6).  TAIL false: n is added to the exponent; below 2^-126 that is 2^-126, and NaN may come out
+// largest relative error (2.6e-6; 2.7e-6 as evaluated in fp32).  Range reduction and minimax polynomials are textbook (Muller,
+// Elementary Functions); taking part of a softmax's exponentials so is a published technique of attention kernels.  TAIL false: n is added to the exponent; below 2^-126 that is 2^-126, and NaN may come out
 // as any number.  TAIL true, one instruction more: times 2^n, with 0 below 2^-126 (the bits of 2^n end at n = -127, and x is
 // held there); NaN stays.
 template <bool TAIL>

@@ -5,7 +5,9 @@
 //   0-7, 8-15  softmax of slot 0 and 1: two threads per row, 64 scores each.  S (128 fp32 columns of tensor memory) ->
 //              registers, running maximum and sum in fp32, P = exp2(S scale2 - m) rounded to the operand type, back to
 //              tensor memory (over S).  P rounded to 8 (bf16) or 11 (fp16) bits, relative to each probability: the product's
-//              operand type; the sum uses the unrounded values.  m is an exact maximum of the tiles so far, but taken anew
+//              operand type; the sum uses the unrounded values.  (Running maximum and sum in one pass: Milakov and
+//              Gimelshein, Online normalizer calculation for softmax, 2018; rescaling only past a bound is a published
+//              refinement of it.)  m is an exact maximum of the tiles so far, but taken anew
 //              only when a tile exceeds it by more than 8 (a factor 2^8: far from overflow in fp32 sums and fp16 P): P of a
 //              tile is computed with the m at hand, without a pass for the maximum before it, and only such a tile is gone
 //              over again, after its threads have rescaled O in tensor memory.  A unit's first tile, if all its keys are in use,

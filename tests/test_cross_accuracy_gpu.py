@@ -1,4 +1,6 @@
 """Cross attention on GPU: digits and bits that depend on the operands' size, on what ran before, and on the exp2 in use."""
+import math
+
 import pytest
 import torch
 
@@ -98,3 +100,23 @@ def test_fp16_gradients_do_not_see_what_masked_values_hold():
         o, lse = cross.cross_attention(q, kj, vj, key_mask=mask, kv_lens=lens, return_lse=True)
         res.append((o, lse, *cross.cross_attention_backward(do, q, kj, vj, o, lse, key_mask=mask, kv_lens=lens)))
     assert all(torch.equal(a, b) for a, b in zip(*res))
+
+
+@pytest.mark.parametrize("residue", range(8))
+def test_exponentials(residue):
+    """The forward pass's exp2 by both units it is taken from (special functions, and a polynomial on the FMA pipe), by the key's place:
+    rows whose keys in one residue class mod 8 all score a, the others 60 below: lse = a + log(keys of the class).  lse is
+    from sums of unrounded probabilities.  The first tile is taken with maximum 0 where scores are between 0 and 8 (in log2).
+    Bounds: 2.7e-6 for the polynomial, 2^-22 for the special function unit, 2^-24 for each of the 16 additions of a thread's
+    sum, the score's product, and the log and its two products (4 roundings of a number below 8)."""
+    n, d = 2000, 64
+    a = (torch.arange(n, device=DEV) * (5.5 / n)).half()  # up to 7.9 in log2
+    q = torch.zeros(1, n, 1, d, device=DEV, dtype=FP)
+    q[0, :, 0, 0], q[0, :, 0, 1] = a, 1
+    for sk in (128, 512):
+        k = torch.zeros(1, sk, 1, d, device=DEV, dtype=FP)
+        k[0, :, 0, 0] = 1
+        k[0, torch.arange(sk, device=DEV) % 8 != residue, 0, 1] = -60
+        _, lse = cross.cross_attention(q, k, torch.ones_like(k), scale=1.0, return_lse=True)
+        err = (lse[0, 0].double() - a.double() - math.log(sk // 8)).abs().max()
+        assert float(err) <= 2.7e-6 + 2.0 ** -22 + 2.0 ** -24 * (16 + 8 + 4 * 16), float(err)
