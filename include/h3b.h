@@ -139,6 +139,7 @@ int h3b_attn_merge(float* acc, float* acc_lse, const void* o, int64_t o_head_str
  *   q, k       one of them may be null; S tokens (0 is valid) of `heads` heads, strides in elements, channels contiguous;
  *              any stride (16-byte aligned rows are faster); pointers aligned to their elements; y must not overlap x or itself
  *   pos        [B, S, n_axes] of pos_dtype (fp32, int32, int64), axes contiguous, strides in elements (0: shared)
+ *              (angles are exact to fp32 up to |theta| = 2^28 and to 4 * 2^-53 |theta| beyond)
  *   inv_freq   DEVICE fp32 [F];  sections: HOST int32 [n_axes], n_axes <= H3B_MAX_AXES, 2 F <= head_dim <= 1024 */
 #define H3B_MAX_AXES 8
 enum h3b_rope_pairing { H3B_PAIR_HALF = 0, H3B_PAIR_ADJACENT = 1 };

@@ -5,8 +5,10 @@
 //   (a, b) -> (a cos - b sin, a sin + b cos);  channels >= 2 F are copied
 // The rotation is orthogonal, so its gradient is the rotation back (inverse: sin -> -sin).
 //
-// Angles: the product of a 32-bit position and a 32-bit frequency is exact in fp64, turns (theta / 2 pi) are reduced to
-// [-1/2, 1/2] there, and sincospif takes the remainder: full fp32 accuracy at any position, no slow large-argument path.
+// Angles: theta in turns (theta / 2 pi) is computed and reduced to [-1/2, 1/2] in fp64, and sincospif takes the remainder: no slow
+// large-argument path.  Position times frequency is exact there for fp32 positions and for integers below 2^29; with the roundings
+// of larger ones, of 1 / (2 pi) and of the product with it the angle is off by at most 4 * 2^-53 |theta|, which is below the
+// error of cos and sin in fp32 up to |theta| = 2^28 and 5e-4 at 2^40.
 // One rounding per output element, from fp32 products.
 //
 // HBM-bound: every element is read once and written once.  A CTA owns a few tokens of q or k: its threads fill a table
