@@ -159,7 +159,8 @@ int h3b_rope_axes(const h3b_rope_operand* q, const h3b_rope_operand* k, int x_dt
  *   q, o       [B, Sq, Hq, head_dim];  k, v: [B, Sk, Hkv, head_dim] of dtype (bf16 or fp16); Hq a multiple of Hkv (query
  *              head h reads key head h / (Hq / Hkv)); strides in elements, multiples of 8 and at least 8 (0, a tensor shared
  *              along an axis, is refused), those of o at least head_dim; those of extents of one are not looked at; channels
- *              contiguous, every tensor 16-byte aligned; head_dim a multiple of 8, at most 128; scale > 0
+ *              contiguous, every tensor 16-byte aligned; o must not overlap k or v; head_dim a multiple of 8, at most 128;
+ *              scale > 0
  *   kv_lens    optional DEVICE int32 [B]: only keys j < kv_lens[b] take part
  *   mask       optional DEVICE key mask, rows ldm elements apart (0: shared): H3B_MASK_BOOL uint8 [B, Sk], 0 leaves the
  *              key out; H3B_MASK_BIAS fp32 [B, Sk] added to the scaled scores, -inf leaves the key out

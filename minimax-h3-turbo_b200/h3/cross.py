@@ -222,7 +222,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_len
     entry's largest value is taken off first, which changes lse (full_lse puts it back) but not o.  A query without keys gets 0 (lse -inf); what
     keys that are left out hold never reaches a result.  Differentiable in q, k and v (not in
     key_mask, nor through lse).  out: a [B, Sq, Hq, D] tensor to
-    write (16-byte aligned rows; not with gradients)."""
+    write (16-byte aligned rows; not with gradients; no part of k or v, which are read while it is written)."""
     no_tangents("cross_attention", q, k, v, key_mask)
     if key_mask is not None and key_mask.requires_grad and torch.is_grad_enabled():
         raise ValueError("cross_attention: key_mask has no gradient; detach it")
@@ -232,9 +232,12 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_len
         o, lse = _CrossAttention.apply(q, k, v, kv_lens, key_mask, scale)
         return (o, lse) if return_lse else o
     p = _Problem(q, k, v, kv_lens, key_mask, scale)
-    if out is not None and _readable(p.rows(out, "out")).data_ptr() != _batched(out, "out").data_ptr():
-        raise ValueError("cross_attention: out needs contiguous channels, a 16-byte aligned base and strides that are "
-                         "multiples of 8 elements")
+    if out is not None:
+        if _readable(p.rows(out, "out")).data_ptr() != _batched(out, "out").data_ptr():
+            raise ValueError("cross_attention: out needs contiguous channels, a 16-byte aligned base and strides that are "
+                             "multiples of 8 elements")
+        if out.numel() and out.data_ptr() in (p.k.data_ptr(), p.v.data_ptr()):
+            raise ValueError("cross_attention: out must not overlap k or v")
     o, lse = _forward(p, return_lse, None if out is None else _batched(out, "out"))
     if out is not None:
         o = out

@@ -28,3 +28,17 @@ def test_lengths_past_32_bits():
     want = cross.cross_attention(q, k, v, kv_lens=strided.clamp(min=0).to(torch.int32))
     assert torch.equal(cross.cross_attention(q, k, v, kv_lens=strided), want)
     assert torch.equal(cross.cross_attention(q, k, v, kv_lens=strided.to(torch.int32).repeat_interleave(2)[::2]), want)
+
+
+def test_out_is_no_part_of_what_is_read():
+    q, k, v = (torch.randn(2, 30, 2, 64, device=DEV, dtype=BF) for _ in range(3))
+    want = cross.cross_attention(q, k, v)
+    for out in (k, v):
+        with pytest.raises(ValueError, match="overlap"):
+            cross.cross_attention(q, k, v, out=out)
+    with pytest.raises(ValueError):  # rows that fold onto one another
+        cross.cross_attention(q, k, v, out=torch.empty(10000, dtype=BF, device=DEV).as_strided(q.shape, (3840, 128, 8, 1)))
+    both = torch.empty(2, 30, 2, 2, 64, dtype=BF, device=DEV)  # keys and results side by side in one buffer
+    both[:, :, 0] = k
+    assert torch.equal(cross.cross_attention(q, both[:, :, 0], v, out=both[:, :, 1]), want)
+    assert torch.equal(both[:, :, 0], k)
