@@ -224,13 +224,14 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_len
     key_mask, nor through lse).  out: a [B, Sq, Hq, D] tensor to
     write (16-byte aligned rows; not with gradients; no part of k or v, which are read while it is written)."""
     no_tangents("cross_attention", q, k, v, key_mask)
-    if key_mask is not None and key_mask.requires_grad and torch.is_grad_enabled():
-        raise ValueError("cross_attention: key_mask has no gradient; detach it")
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        if out is not None:
-            raise ValueError("cross_attention: out cannot be given where gradients are recorded")
-        o, lse = _CrossAttention.apply(q, k, v, kv_lens, key_mask, scale)
-        return (o, lse) if return_lse else o
+    if torch.is_grad_enabled():
+        if key_mask is not None and key_mask.requires_grad:
+            raise ValueError("cross_attention: key_mask has no gradient; detach it")
+        if q.requires_grad or k.requires_grad or v.requires_grad:
+            if out is not None:
+                raise ValueError("cross_attention: out cannot be given where gradients are recorded")
+            o, lse = _CrossAttention.apply(q, k, v, kv_lens, key_mask, scale)
+            return (o, lse) if return_lse else o
     p = _Problem(q, k, v, kv_lens, key_mask, scale)
     if out is not None:
         if _readable(p.rows(out, "out")).data_ptr() != _batched(out, "out").data_ptr():
@@ -256,7 +257,8 @@ def cross_attention_backward(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
     for them raises RuntimeError."""
     args = (do, q, k, v, o, lse, kv_lens, key_mask, scale)
     no_tangents("cross_attention", *args[:6], key_mask)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in args[:6]):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or do.requires_grad or o.requires_grad
+                                    or lse.requires_grad):
         return _CrossAttentionGrads.apply(*args)
     return _backward(*args)
 

@@ -213,8 +213,10 @@ def rope_axes(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions: O
         raise ValueError(f"pairing must be 'half' or 'adjacent', got {pairing!r}")
     k_positions = positions if k_positions is None else k_positions
     no_tangents("rope_axes", q, k, positions, k_positions, inv_freq)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (positions, k_positions, inv_freq)):
-        raise ValueError("rope_axes: positions and inv_freq have no gradient; detach them")
-    if torch.is_grad_enabled() and ((q is not None and q.requires_grad) or (k is not None and k.requires_grad)):
-        return _RopeAxes.apply(q, k, positions, k_positions, inv_freq, sections, pairing, inverse)
+    if torch.is_grad_enabled():
+        if inv_freq.requires_grad or (positions is not None and positions.requires_grad) or \
+                (k_positions is not None and k_positions.requires_grad):
+            raise ValueError("rope_axes: positions and inv_freq have no gradient; detach them")
+        if (q is not None and q.requires_grad) or (k is not None and k.requires_grad):
+            return _RopeAxes.apply(q, k, positions, k_positions, inv_freq, sections, pairing, inverse)
     return _rope_axes(q, k, positions, k_positions, inv_freq, sections, pairing, inverse)
