@@ -15,7 +15,7 @@
 // that the fp32 results are divided by: P times 2^14, dS times what keeps its bound 2 |g| max |v| below 2^14, |g| of the row for
 // dQ, the largest of the unit's rows for dK (there rows are what is summed over).  cross_stats_kernel takes the norms, for which it
 // reads the values once more: 2 x 12090 queries x 512 keys x 40 heads x 64 697 -> 737 us, 3 x 5 queries x 12090 keys, 56 over 8
-// heads x 128 108 -> 139 us, against the same kernels without the factors.
+// heads x 128 108 -> 129 us, against the same kernels without the factors.
 //
 // Warps of both: 0-15 elementwise work, thread = row, four warps to the same 32 rows with 32 columns each; 16-19 epilogue
 // (accumulators -> global memory); 20 MMA issue; 21 copies; 22 (dQ) zeroes K rows of masked
@@ -166,14 +166,18 @@ __device__ __forceinline__ void tile_values_top(const CrossParams& P, const Mask
   const int64_t len = ca_len(mask.kv_lens, b, P.Sk);
   const int ch = threadIdx.x % PER_ROW * 8;
   const T* vb = static_cast<const T*>(P.v.ptr) + b * P.v.stride_b + hk * P.v.stride_h + ch;
-  float top = 0.f;
+  uint4 x[PASSES];
 #pragma unroll
   for (int a = 0; a < PASSES; ++a) {
     const int64_t key = static_cast<int64_t>(tile) * CT + a * ROWS + threadIdx.x / PER_ROW;
-    uint4 x = make_uint4(0, 0, 0, 0);
+    x[a] = make_uint4(0, 0, 0, 0);
     if (key < len && ch < P.D && !(mask.mask && ca_mask_value(mask, b * mask.ldm + key) == -INFINITY))
-      x = *reinterpret_cast<const uint4*>(vb + key * P.v.stride_s);
-    const T* xe = reinterpret_cast<const T*>(&x);
+      x[a] = *reinterpret_cast<const uint4*>(vb + key * P.v.stride_s);
+  }
+  float top = 0.f;
+#pragma unroll
+  for (int a = 0; a < PASSES; ++a) {
+    const T* xe = reinterpret_cast<const T*>(&x[a]);
     float d = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) d = fmaf(static_cast<float>(xe[e]), static_cast<float>(xe[e]), d);
