@@ -21,9 +21,10 @@
 // (accumulators -> global memory); 20 MMA issue; 21 copies; 22 (dQ) zeroes K rows of masked
 // keys before their product.  P and dS go back to tensor memory over the columns that their own warps read S or dP from.
 //
-// bf16, 40 heads x 128 channels, both with the row vectors: 2 x 4096 queries x 512 keys 323 to 333 us (902 to 929 TFLOP/s of
-// 7 products), 12090 x 1600 1152 to 1195 us (1160 to 1204).  Tensor pipe 68 % (dQ) and 72 % (dK, dV) active; neither HBM
-// (8 %) nor the FMA pipe (40 %) is near its limit: the chain scores -> elementwise work -> second product is.
+// bf16, 40 heads x 128 channels, both with the row vectors, at 1965 MHz / in a row under the power limit: 2 x 4096 queries x 512 keys
+// 340 / 375 us (885 / 800 TFLOP/s of 7 products), 12090 x 1600 1200 / 1380 us (1160 / 1005).  Tensor pipe 65 % (dQ)
+// and 74 % (dK, dV) active; neither HBM (8 %) nor the FMA pipe (40 %) is near its limit: the chain scores -> elementwise work ->
+// second product is.
 #include "cross_common.cuh"
 
 namespace h3b {
@@ -698,8 +699,8 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
 
 // ------------------------------------------------------------------------------------------------ dK, dV
 // Q and G arrive in rings (K and V stay): Q 3 stages, because dK's product, the last of a query tile, reads it; G 2.  11840
-// queries x 40 heads x 128 channels: 243 us over 256 keys, 831 over 2048 (4 products: 1195 TFLOP/s); dQ there 196 and 611
-// (3 products: 1220).
+// queries x 40 heads x 128 channels: 122 us over 256 keys, 795 over 2048 (4 products: 1250 TFLOP/s); dQ there 112 and 605
+// (3 products: 1230).
 template <typename T, int DP, bool BIAS>
 __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
     cross_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG,

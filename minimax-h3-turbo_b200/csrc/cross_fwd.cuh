@@ -25,10 +25,12 @@
 // log-sum-exps in a fixed order.
 //
 // Bound by the chain scores -> softmax -> second product: 3150 cycles for two query tiles x one key tile, of which the
-// products alone take 2048 (tensor pipe 62 % active; exponentials 47 %).  Two threads per row and two slots, because one
-// thread per row takes longer for a softmax than the other slot's products last.  bf16, 40 heads x 128 channels: 57840
-// queries x 1600 keys 1600 to 1680 us (1130 to 1180 TFLOP/s by the card's clock), 12090 x 512 128 us (990), one query x
-// 57840 keys 204 us (HBM, 5.8 TB/s).
+// products alone take 2048 (tensor pipe 60 % active; exponentials 45 %).  Two threads per row and two slots, because one
+// thread per row takes longer for a softmax than the other slot's products last.
+// bf16, 40 heads x 128 channels, normalised q and k, at 1965 MHz / in a row under the power limit: 57840 queries x 1600 keys 1650 /
+// 1915 us (1150 / 990 TFLOP/s), 2 x 12090 x 512 260 / 302 us (975 / 840), one query x 57840 keys 205 / 235 us (HBM, 5.8 / 5.0 TB/s).
+// Scores of a larger spread are gone over twice more often: 2 x 12090 x 512 at standard deviations 1, 1.4, 2, 4, 8: 259, 368, 304,
+// 391, 407 us.
 #include "cross_common.cuh"
 
 namespace h3b {

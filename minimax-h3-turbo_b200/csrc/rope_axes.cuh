@@ -15,9 +15,9 @@
 // of the tokens' (cos, sin) in shared memory -- one evaluation per token and pair, not per head -- then go through the
 // tokens' rows in 16-byte units.  What hides the latency is full occupancy: eight CTAs of 256 threads per SM at 32 registers;
 // with the registers left to the compiler (41, six CTAs) it is 1.15 to 1.2 times slower, with four units loaded ahead per
-// thread 1.9 times.  59440 tokens x 2 x 40 heads of 128 channels, bf16 (2.43 GB): 390 to 404 us, 6.0 to 6.2 TB/s.  Partners
-// off the 16-byte grid ("half" with F not a multiple of the unit) are bound by instructions: 2.1 to 2.5 TB/s in 16 bits, 4.4
-// to 4.9 in 32 (two aligned units and a shift instead of element loads measured slower: both paths run in most warps).
+// thread 1.9 times.  59440 tokens x 2 x 40 heads of 128 channels, bf16 (2.43 GB): 400 us, 6.1 TB/s, at 1965 MHz; 442 us, 5.5 TB/s,
+// in a row under the power limit.  Partners off the 16-byte grid ("half" with F not a multiple of the unit) are bound by
+// instructions: 2.1 to 2.5 TB/s in 16 bits, 4.4 to 4.9 in 32 (two aligned units and a shift instead of element loads measured slower: both paths run in most warps).
 // Few tokens: one token per CTA, so that the heads of a handful of tokens spread over the SMs.
 #include "fastdiv.cuh"
 #include "h3b_common.cuh"

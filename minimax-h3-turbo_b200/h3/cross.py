@@ -219,10 +219,10 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_len
     h // (Hq // Hkv)); views whose channels are contiguous and whose strides are multiples of 8 elements are read in place,
     others are copied.  kv_lens: int [B], keys in use of each entry of a padded batch.  key_mask: [B, Sk] (or [1, Sk]) bool,
     False leaves a key out; or floating point, added to the scaled scores (a key's log weight), -inf leaves it out; the
-    entry's largest value is taken off first, which changes lse (full_lse puts it back) but not o.  A query without keys gets 0 (lse -inf); what
-    keys that are left out hold never reaches a result.  Differentiable in q, k and v (not in
-    key_mask, nor through lse).  out: a [B, Sq, Hq, D] tensor to
-    write (16-byte aligned rows; not with gradients; no part of k or v, which are read while it is written)."""
+    entry's largest value is taken off first, which changes lse (full_lse puts it back) but not o.  A query without keys gets
+    0 (lse -inf); what keys that are left out hold never reaches a result.  Differentiable in q, k and v (not in key_mask, nor
+    through lse).  out: a [B, Sq, Hq, D] tensor to write (16-byte aligned rows; not with gradients; no part of k or v, which are
+    read while it is written)."""
     no_tangents("cross_attention", q, k, v, key_mask)
     if torch.is_grad_enabled():
         if key_mask is not None and key_mask.requires_grad:
