@@ -476,6 +476,8 @@ __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, 1)
           xph ^= 1;
           delta = (part[row] + part[CT + row]) + (part[2 * CT + row] + part[3 * CT + row]);
           if constexpr (scaled<T>) delta *= pow2(-P_EXP);
+          // (rows that no query fills have 0 x whatever shared memory held; the dK/dV kernel multiplies by what is written here)
+          if (nlse2 == -INFINITY) delta = 0.f;
           if (quarter == 0) stat[CT + row] = delta;
         }
       }

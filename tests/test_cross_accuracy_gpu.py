@@ -120,3 +120,25 @@ def test_exponentials(residue):
         _, lse = cross.cross_attention(q, k, torch.ones_like(k), scale=1.0, return_lse=True)
         err = (lse[0, 0].double() - a.double() - math.log(sk // 8)).abs().max()
         assert float(err) <= 2.7e-6 + 2.0 ** -22 + 2.0 ** -24 * (16 + 8 + 4 * 16), float(err)
+
+
+@pytest.mark.parametrize("d,dt", [(64, BF), (128, FP), (128, BF), (64, FP)])
+@pytest.mark.parametrize("g,sk,masked", [(3, 100, False), (5, 128, False), (7, 1, False), (7, 90, True)])
+def test_few_keys_whatever_ran_before(g, sk, masked, d, dt):
+    """All keys in one tile (delta comes from P and dP there), head groups that do not divide 128, numbers that are none left in
+    every SM's shared memory: they must not reach any result."""
+    q, k, v, do = make(2, 3 * (128 // g) + 1, sk, 2 * g, 2, d, dt, seed=g + sk)
+    kw = {"key_mask": torch.arange(sk, device=DEV).view(1, -1) % 3 > 0} if masked else {}
+    before = make(1, 128 * 148 * 2, 128, 1, 1, d, dt, seed=51)
+    r = cross_ref(q, k, v, do=do, **kw)
+    results = []
+    for junk in (0.0, float("nan")):
+        stale = [t * junk for t in before[:1] + before[3:]]
+        cross.cross_attention(stale[0], *before[1:3])
+        o, lse = cross.cross_attention(q, k, v, return_lse=True, **kw)
+        ob, lb = cross.cross_attention(before[0], *before[1:3], return_lse=True)
+        cross.cross_attention_backward(stale[1], stale[0], *before[1:3], ob, lb)
+        results.append((o, *cross.cross_attention_backward(do, q, k, v, o, lse, **kw)))
+    for name, a, b in zip(("o", "dq", "dk", "dv"), *results):
+        assert ((b.double() - r[name]).abs() <= r["tol_" + name]).all(), name
+        assert torch.equal(a, b), name
