@@ -12,7 +12,7 @@
 // P and dS are rounded to the operand type for the second products (8 or 11 bits, relative to each element); sums are fp32.
 // fp16 has few exponents: P of 12090 keys lies where its steps are absolute, and so does dS of a gradient of ordinary size, or
 // past its range (do of 1e-3 over 12090 keys: dq off by 1.6e-2 if rounded as they are).  So both are held times a power of two
-// that the fp32 results are divided by: P times 2^14, dS times what keeps its bound 2 |g| max |v| below 2^14, |g| of the row for
+// that the fp32 results are divided by: P times 2^14, dS times what keeps its bound |g| max |v| / 2 below 2^15, |g| of the row for
 // dQ, the largest of the unit's rows for dK (there rows are what is summed over).  cross_stats_kernel takes the norms, for which it
 // reads the values once more: 2 x 12090 queries x 512 keys x 40 heads x 64 697 -> 737 us, 3 x 5 queries x 12090 keys, 56 over 8
 // heads x 128 108 -> 129 us, against the same kernels without the factors.
@@ -121,11 +121,12 @@ constexpr int P_EXP = 14;  // fp16: P is held times 2^P_EXP
 template <typename T>
 constexpr bool scaled = std::is_same_v<T, __half>;
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + e) << 23); }
-// e of the factor 2^e for dS: |dS| = p |dP - delta| <= 2 |g| |v| (delta is a mean of dP), and 2^e times that is below 2^14.
-// Norms that are not finite, or 0, give the ends of the range: the results are not numbers, or 0, whatever the factor.
+// e of the factor 2^e for dS.  dP_j - delta = (1 - p_j) (dP_j - mean of the others), so |dS| <= p (1 - p) 2 |g| |v| <= |g| |v| / 2;
+// 2^e times that is below 2^15, which leaves a factor of two for what roundings add.  Norms that are not finite, or 0, give the ends
+// of the range: the results are not numbers, or 0, whatever the factor.
 __device__ __forceinline__ int ds_exp(float g2, float v2) {
-  const int k = ((__float_as_int(4.f * g2 * v2) >> 23) & 255) - 127;  // the bound's square is below 2^(k + 1)
-  return min(60, 14 - ((k + 2) >> 1));
+  const int k = ((__float_as_int(0.25f * g2 * v2) >> 23) & 255) - 127;  // the bound's square is below 2^(k + 1)
+  return min(60, 15 - ((k + 2) >> 1));
 }
 // the largest of n numbers >= 0; called by whole warps
 __device__ __forceinline__ float warp_top(const float* p, int n) {
