@@ -198,6 +198,36 @@ int h3b_cross_attention_backward(const h3b_attn_tensor* grad_o, const h3b_attn_t
                                  const int32_t* kv_lens, const void* mask, int mask_kind, int64_t ldm, void* workspace,
                                  size_t ws_bytes, void* stream);
 
+/* ---- low-rank adapters of many requests beside a shared projection (no reference counterpart):
+ *     out_i = base_i + s_g (x_i A_g^T) B_g^T,   g the adapter of row i; a row without one keeps base_i.
+ * A plan says which rows an adapter has; it is made once for a batch and serves every projection of every layer.
+ *   rows [M] adapter of each row; numbers outside 0 .. adapters - 1: none.  Any order.
+ *   plan  h3b_adapter_plan_ints(M, adapters) numbers (device memory, 16-byte aligned), written by h3b_adapter_plan; only plans
+ *         that it wrote for the same M and adapters may be passed on. */
+#define H3B_MAX_RANK 128
+#define H3B_MAX_ADAPTERS 65535
+int64_t h3b_adapter_plan_ints(int64_t M, int64_t adapters);
+int h3b_adapter_plan(const int32_t* rows, int64_t M, int64_t adapters, int32_t* plan, int64_t plan_ints, void* stream);
+
+/* x [M, ldx], base and out [M, ld]: bf16 or fp16 rows of K and N channels (multiples of 8; 16-byte aligned rows); a [adapters,
+ * rank, K] and b [adapters, N, rank] of the same type, contiguous; scales [adapters] fp32 or NULL (1); base NULL: zeros; out may be
+ * base (rows without an adapter are then left as they are), and otherwise overlaps nothing.  Sums are held in fp32; x A^T is
+ * rounded to dtype for the second product, in fp16 after scaling each row into its range by a power of two.
+ *   hidden     h3b_low_rank_hidden_bytes(M, rank) (256-byte aligned) for the gradients, or NULL
+ *   workspace  h3b_low_rank_workspace_bytes(..., backward = 0), 256-byte aligned; the size queries give 0 for refused sizes. */
+size_t h3b_low_rank_hidden_bytes(int64_t M, int rank);
+size_t h3b_low_rank_workspace_bytes(int64_t M, int64_t K, int64_t N, int rank, int64_t adapters, int backward);
+int h3b_low_rank(const void* x, int64_t ldx, const void* a, const void* b, const void* base, int64_t ldbase, void* out,
+                 int64_t ldo, int dtype, int64_t M, int64_t K, int64_t N, int rank, int64_t adapters, const float* scales,
+                 const int32_t* plan, void* hidden, void* workspace, size_t ws_bytes, void* stream);
+/* Gradients with respect to x, a and b (each may be NULL: not asked for); that of base is grad_out itself.  hidden as
+ * h3b_low_rank left it for the same arguments.  Adapters without rows and rows without an adapter get zeros.  Every sum has a
+ * fixed order: the same call gives the same bits. */
+int h3b_low_rank_backward(const void* grad_out, int64_t ldgo, const void* x, int64_t ldx, const void* a, const void* b,
+                          const void* hidden, void* dx, int64_t lddx, void* da, void* db, int dtype, int64_t M, int64_t K,
+                          int64_t N, int rank, int64_t adapters, const float* scales, const int32_t* plan, void* workspace,
+                          size_t ws_bytes, void* stream);
+
 /* int4 codebook indices + group scales -> the exact int8 grid [N, K] (row stride ldg bytes).
  * Replaces decode_int8_grid / _decode_rows / _pair_lut (qlinear.py:157-204).
  *   q4     [N, ldq4 bytes] packed nibbles, low nibble first (types.py:14-16)

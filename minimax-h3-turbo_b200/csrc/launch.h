@@ -6,6 +6,7 @@
 //                 attention merge (attn_merge.cuh)
 //   k_rope_axes.cu  rotary embedding from positions on several axes (rope_axes.cuh)
 //   k_cross.cu    cross attention and its gradients (cross_attn.cuh)
+//   k_lowrank.cu  low-rank adapters beside a shared projection, and their gradients (lowrank.cuh)
 //   k_decode.cu   int4 -> int8 grid decode (decode.cuh)
 //   k_gemm.cu     int8 GEMM + epilogue, 1-CTA and CTA-pair kernels (gemm_sm100.cuh)
 //   k_w4.cu       dispatch of the decode-in-producer W4A8 GEMM for few M tiles (gemm_w4.cuh), instantiated per group
@@ -75,6 +76,25 @@ int cross_launch(const h3b_attn_tensor* t, int dtype, int64_t B, int64_t Sq, int
                  const int32_t* kv_lens, const void* mask, int mask_kind, int64_t ldm, float* lse, void* ws, bool backward,
                  cudaStream_t st);
 
+// ---- k_lowrank.cu
+struct LrArgs {  // of h3b_low_rank and h3b_low_rank_backward
+  const void *x, *a, *b, *base, *go;
+  int64_t ldx, ldbase, ldo, ldgo, lddx;
+  void *out, *dx, *da, *db;
+  int64_t M, K, N, R;
+  int rank, dtype;
+  const float* scales;
+  const int32_t* plan;
+  void* hidden;
+  void* ws;
+};
+int64_t lr_plan_size(int64_t M, int64_t R);  // int32 numbers of a plan
+int lr_plan_launch(const int32_t* rows, int64_t M, int64_t R, int32_t* plan, cudaStream_t st);
+size_t lr_hidden_bytes(int64_t M, int rank);
+size_t lr_workspace(int64_t M, int64_t K, int64_t N, int rank, int64_t R, bool backward);
+int lr_forward(const LrArgs& a, cudaStream_t st);
+int lr_backward(const LrArgs& a, cudaStream_t st);
+
 // ---- k_decode.cu
 int decode_launch(const void* q4, int64_t N, int64_t K, int64_t ldq4, const void* s_rel, int s_dtype, int64_t lds,
                   const float* codebook, int group, int8_t* grid, int64_t ldg, cudaStream_t st);
@@ -102,5 +122,6 @@ cudaError_t device_error_w4_fp16(unsigned* v, int clear);
 cudaError_t device_error_w4_bf16(unsigned* v, int clear);
 cudaError_t device_error_w4_fp32(unsigned* v, int clear);
 cudaError_t device_error_cross(unsigned* v, int clear);
+cudaError_t device_error_lowrank(unsigned* v, int clear);
 
 }  // namespace h3b

@@ -393,6 +393,78 @@ int h3b_cross_attention_backward(const h3b_attn_tensor* grad_o, const h3b_attn_t
                       const_cast<float*>(lse), workspace, true, static_cast<cudaStream_t>(stream));
 }
 
+// ranks, rows and widths that the plan, the workspace and the launches take
+static int check_low_rank_sizes(int64_t M, int64_t K, int64_t N, int rank, int64_t R) {
+  if (M < 0 || K < 8 || N < 8 || K % 8 || N % 8) return fail(H3B_ERR_ARG, "low_rank: M >= 0, and widths that are positive multiples of 8, are required");
+  if (rank < 1 || rank > H3B_MAX_RANK) return fail(H3B_ERR_ARG, "low_rank: the rank must be 1 to " + std::to_string(H3B_MAX_RANK));
+  if (R < 1 || R > H3B_MAX_ADAPTERS) return fail(H3B_ERR_ARG, "low_rank: 1 to " + std::to_string(H3B_MAX_ADAPTERS) + " adapters");
+  if (M > 0x3FFFFF00 || K > 0x3FFFFF00 || N > 0x3FFFFF00) return fail(H3B_ERR_UNSUPPORTED, "low_rank: at most 2^30 rows and channels");
+  return H3B_OK;
+}
+// a row-major operand of `width` columns: 16-byte aligned rows that do not overlap
+static int check_rows(const void* p, int64_t ld, int64_t width, const char* name) {
+  if (!p || !aligned(p, 16) || ld < width || ld % 8)
+    return fail(H3B_ERR_ARG, std::string("low_rank: ") + name + " must be 16-byte aligned rows, their stride a multiple of 8 and at least the width");
+  return H3B_OK;
+}
+static int check_low_rank(const LrArgs& a, size_t ws_bytes, bool backward) {
+  if (a.dtype != H3B_BF16 && a.dtype != H3B_FP16) return fail(H3B_ERR_ARG, "low_rank: bf16 or fp16 operands");
+  if (int rc = check_low_rank_sizes(a.M, a.K, a.N, a.rank, a.R)) return rc;
+  if (!a.a || !a.b || !aligned(a.a, 16) || !aligned(a.b, 16)) return fail(H3B_ERR_ARG, "low_rank: a and b must be 16-byte aligned, none null");
+  if (!aligned(a.scales, 4)) return fail(H3B_ERR_ARG, "low_rank: scales must be 4-byte aligned");
+  if (!aligned(a.da, 16) || !aligned(a.db, 16)) return fail(H3B_ERR_ARG, "low_rank: the gradients of a and b must be 16-byte aligned");
+  if (a.M > 0) {
+    int rc = check_rows(a.x, a.ldx, a.K, "x");
+    if (!rc && !backward) rc = check_rows(a.out, a.ldo, a.N, "out");
+    if (!rc && a.base) rc = check_rows(a.base, a.ldbase, a.N, "base");
+    if (!rc && backward) rc = check_rows(a.go, a.ldgo, a.N, "grad_out");
+    if (!rc && a.dx) rc = check_rows(a.dx, a.lddx, a.K, "dx");
+    if (rc) return rc;
+    if (!a.plan || !aligned(a.plan, 16)) return fail(H3B_ERR_ARG, "low_rank: the plan must be 16-byte aligned, not null");
+    if ((backward && !a.hidden) || !aligned(a.hidden, 256)) return fail(H3B_ERR_ARG, "low_rank: hidden must be 256-byte aligned, and given for the gradients");
+  }
+  const size_t need = lr_workspace(a.M, a.K, a.N, a.rank, a.R, backward);
+  if (need > 0 && (!a.ws || ws_bytes < need || !aligned(a.ws, 256)))
+    return fail(H3B_ERR_ARG, "low_rank: workspace must be 256-byte aligned and hold " + std::to_string(need) + " bytes");
+  return H3B_OK;
+}
+
+int64_t h3b_adapter_plan_ints(int64_t M, int64_t adapters) {
+  return check_low_rank_sizes(M, 8, 8, 1, adapters) ? 0 : lr_plan_size(M, adapters);
+}
+int h3b_adapter_plan(const int32_t* rows, int64_t M, int64_t adapters, int32_t* plan, int64_t plan_ints, void* stream) {
+  if (int rc = check_low_rank_sizes(M, 8, 8, 1, adapters)) return rc;
+  if (M == 0) return H3B_OK;
+  if (!rows || !aligned(rows, 4)) return fail(H3B_ERR_ARG, "adapter_plan: rows must be 4-byte aligned, not null");
+  if (!plan || !aligned(plan, 16) || plan_ints < lr_plan_size(M, adapters))
+    return fail(H3B_ERR_ARG, "adapter_plan: the plan must be 16-byte aligned and hold " + std::to_string(lr_plan_size(M, adapters)) + " numbers");
+  return lr_plan_launch(rows, M, adapters, plan, static_cast<cudaStream_t>(stream));
+}
+size_t h3b_low_rank_hidden_bytes(int64_t M, int rank) { return check_low_rank_sizes(M, 8, 8, rank, 1) ? 0 : lr_hidden_bytes(M, rank); }
+size_t h3b_low_rank_workspace_bytes(int64_t M, int64_t K, int64_t N, int rank, int64_t adapters, int backward) {
+  return check_low_rank_sizes(M, K, N, rank, adapters) ? 0 : lr_workspace(M, K, N, rank, adapters, backward != 0);
+}
+int h3b_low_rank(const void* x, int64_t ldx, const void* a, const void* b, const void* base, int64_t ldbase, void* out,
+                 int64_t ldo, int dtype, int64_t M, int64_t K, int64_t N, int rank, int64_t adapters, const float* scales,
+                 const int32_t* plan, void* hidden, void* workspace, size_t ws_bytes, void* stream) {
+  LrArgs g{};
+  g.x = x, g.ldx = ldx, g.a = a, g.b = b, g.base = base, g.ldbase = ldbase, g.out = out, g.ldo = ldo, g.dtype = dtype;
+  g.M = M, g.K = K, g.N = N, g.rank = rank, g.R = adapters, g.scales = scales, g.plan = plan, g.hidden = hidden, g.ws = workspace;
+  if (int rc = check_low_rank(g, ws_bytes, false)) return rc;
+  return M == 0 ? H3B_OK : lr_forward(g, static_cast<cudaStream_t>(stream));
+}
+int h3b_low_rank_backward(const void* grad_out, int64_t ldgo, const void* x, int64_t ldx, const void* a, const void* b,
+                          const void* hidden, void* dx, int64_t lddx, void* da, void* db, int dtype, int64_t M, int64_t K,
+                          int64_t N, int rank, int64_t adapters, const float* scales, const int32_t* plan, void* workspace,
+                          size_t ws_bytes, void* stream) {
+  LrArgs g{};
+  g.go = grad_out, g.ldgo = ldgo, g.x = x, g.ldx = ldx, g.a = a, g.b = b, g.hidden = const_cast<void*>(hidden), g.dx = dx;
+  g.lddx = lddx, g.da = da, g.db = db, g.dtype = dtype, g.M = M, g.K = K, g.N = N, g.rank = rank, g.R = adapters;
+  g.scales = scales, g.plan = plan, g.ws = workspace;
+  if (int rc = check_low_rank(g, ws_bytes, true)) return rc;
+  return lr_backward(g, static_cast<cudaStream_t>(stream));
+}
+
 int h3b_decode_grid(const void* q4, int64_t N, int64_t K, int64_t ldq4, const void* s_rel, int s_dtype, int64_t lds,
                     const float* codebook, int group, int8_t* grid, int64_t ldg, void* stream) {
   int rc = check_weight_args(q4, N, K, ldq4, s_rel, s_dtype, lds, codebook, group);
@@ -699,7 +771,7 @@ int h3b_device_error(int clear) {
   cudaError_t (*const units[])(unsigned*, int) = {device_error_abi, device_error_act, device_error_decode,
                                                   device_error_gemm, device_error_w4, device_error_w4_fp8,
                                                   device_error_w4_fp16, device_error_w4_bf16, device_error_w4_fp32,
-                                                  device_error_cross};
+                                                  device_error_cross, device_error_lowrank};
   for (auto unit : units) {
     unsigned u = 0;
     e = unit(&u, clear);
