@@ -198,6 +198,35 @@ int h3b_cross_attention_backward(const h3b_attn_tensor* grad_o, const h3b_attn_t
                                  const int32_t* kv_lens, const void* mask, int mask_kind, int64_t ldm, void* workspace,
                                  size_t ws_bytes, void* stream);
 
+/* ---- the residual's addition with its root-mean-square norm and 8-bit output (no reference counterpart as one operator: _gate_,
+ * _rms, _scale_shift_ and the activation half of the W4A8 linear, model.py:64-66, 106-115, 239-241, qlinear.py:267-303, whose
+ * intermediate roundings this one leaves out):
+ *   t = dt(x + gate y);  r = rsqrt(mean t^2 + eps);  h = t r w (1 + scale) + shift in fp32, rounded once where it is written
+ *   z = h rotated by blocks of 256 as the W4A8 linears take it;  scales = max|z| / 127;  codes = rint(z / scales)
+ *   x, y, t, h   [M, K] rows of dtype (bf16 or fp16), K a multiple of 8 (of 256 with codes), at most H3B_MAX_RESIDUAL; t may be x
+ *                or y, h may not be any of them
+ *   w            [K] of w_dtype;  gate, shift, scale: [n_rows, K] of m_dtype, rows ldm apart, each row of a token's segment.
+ *                gate NULL: 1 for every row; shift and scale NULL (together): none
+ *   segments / token_rows as h3b_rms_modulate (numbers outside 0 .. n_rows - 1: none): a row outside every segment keeps t = x
+ *                (where there is a gate) and h = t r w
+ *   h, codes (with scales [M]) and rstd [M] (the gradients take it) may each be NULL: not written
+ *   A row whose h has a NaN or an infinity gets codes 0 and a scale that is NaN or infinite; a row of zeros scale 0. */
+#define H3B_MAX_RESIDUAL 16384
+size_t h3b_residual_norm_workspace_bytes(int64_t M, int64_t K, int backward);
+int h3b_residual_norm(const void* x, int64_t ldx, const void* y, int64_t ldy, int dtype, int64_t M, int64_t K, const void* w,
+                      int w_dtype, float eps, const void* gate, const void* shift, const void* scale, int64_t ldm,
+                      int64_t n_rows, int m_dtype, const int32_t* segments, int n_segments, const int32_t* token_rows, void* t,
+                      int64_t ldt, void* h, int64_t ldh, int8_t* codes, int64_t ldc, float* scales, float* rstd,
+                      void* workspace, size_t ws_bytes, void* stream);
+/* Gradients with respect to x, y and w from those of t (grad_t, NULL: none) and h; t and rstd as h3b_residual_norm wrote them, the
+ * other arguments the same.  dx is written; dy only with a gate (without one it is dx), NULL: not asked for; dw [K] of w_dtype or
+ * NULL.  gate, shift and scale have no gradient here.  dx may be grad_t or grad_h.  Every sum has a fixed order. */
+int h3b_residual_norm_backward(const void* grad_t, int64_t lddt, const void* grad_h, int64_t lddh, const void* t, int64_t ldt,
+                               const float* rstd, int dtype, int64_t M, int64_t K, const void* w, int w_dtype, const void* gate,
+                               const void* scale, int64_t ldm, int64_t n_rows, int m_dtype, const int32_t* segments,
+                               int n_segments, const int32_t* token_rows, void* dx, int64_t lddx, void* dy, int64_t lddy,
+                               void* dw, void* workspace, size_t ws_bytes, void* stream);
+
 /* ---- low-rank adapters of many requests beside a shared projection (no reference counterpart):
  *     out_i = base_i + s_g (x_i A_g^T) B_g^T,   g the adapter of row i; a row without one keeps base_i.
  * A plan says which rows an adapter has; it is made once for a batch and serves every projection of every layer.

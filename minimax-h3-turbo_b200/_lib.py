@@ -23,6 +23,7 @@ BF16, FP16, FP32, FP8_E4M3, INT32, INT64 = 0, 1, 2, 3, 4, 5
 PAIRING = {"half": 0, "adjacent": 1}  # enum h3b_rope_pairing
 MASK_NONE, MASK_BOOL, MASK_BIAS = 0, 1, 2  # enum h3b_mask_kind
 MAX_AXES = 8  # H3B_MAX_AXES
+MAX_RESIDUAL = 16384  # H3B_MAX_RESIDUAL
 MAX_RANK, MAX_ADAPTERS = 128, 65535  # H3B_MAX_RANK, H3B_MAX_ADAPTERS
 QMODE = {"ck": 0, "eager": 1}
 COPY_DIRECT, COPY_STAGED, COPY_PAGEABLE = 0, 1, 2
@@ -61,6 +62,13 @@ _SIGNATURES = {
     "h3b_cross_attention_backward": ([_attn_p] * 5 + [_c_void_p] + [_attn_p] * 3 +
                                      [_int, _i64, _i64, _i64, _int, _int, _int, ctypes.c_float, _c_void_p, _c_void_p, _int,
                                       _i64, _c_void_p, _sz, _c_void_p], _int),
+    "h3b_residual_norm_workspace_bytes": ([_i64, _i64, _int], _sz),
+    "h3b_residual_norm": ([_c_void_p, _i64, _c_void_p, _i64, _int, _i64, _i64, _c_void_p, _int, ctypes.c_float, _c_void_p, _c_void_p,
+                           _c_void_p, _i64, _i64, _int, _c_void_p, _int, _c_void_p, _c_void_p, _i64, _c_void_p, _i64, _c_void_p,
+                           _i64, _c_void_p, _c_void_p, _c_void_p, _sz, _c_void_p], _int),
+    "h3b_residual_norm_backward": ([_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _c_void_p, _int, _i64, _i64, _c_void_p, _int,
+                                    _c_void_p, _c_void_p, _i64, _i64, _int, _c_void_p, _int, _c_void_p, _c_void_p, _i64, _c_void_p,
+                                    _i64, _c_void_p, _c_void_p, _sz, _c_void_p], _int),
     "h3b_adapter_plan_ints": ([_i64, _i64], _i64),
     "h3b_adapter_plan": ([_c_void_p, _i64, _i64, _c_void_p, _i64, _c_void_p], _int),
     "h3b_low_rank_hidden_bytes": ([_i64, _int], _sz),

@@ -7,6 +7,7 @@
 //   k_rope_axes.cu  rotary embedding from positions on several axes (rope_axes.cuh)
 //   k_cross.cu    cross attention and its gradients (cross_attn.cuh)
 //   k_lowrank.cu  low-rank adapters beside a shared projection, and their gradients (lowrank.cuh)
+//   k_resnorm.cu  the residual's addition with its norm and 8-bit output, and their gradients (resnorm.cuh)
 //   k_decode.cu   int4 -> int8 grid decode (decode.cuh)
 //   k_gemm.cu     int8 GEMM + epilogue, 1-CTA and CTA-pair kernels (gemm_sm100.cuh)
 //   k_w4.cu       dispatch of the decode-in-producer W4A8 GEMM for few M tiles (gemm_w4.cuh), instantiated per group
@@ -94,6 +95,23 @@ size_t lr_hidden_bytes(int64_t M, int rank);
 size_t lr_workspace(int64_t M, int64_t K, int64_t N, int rank, int64_t R, bool backward);
 int lr_forward(const LrArgs& a, cudaStream_t st);
 int lr_backward(const LrArgs& a, cudaStream_t st);
+
+// ---- k_resnorm.cu
+struct ResNormArgs {  // of h3b_residual_norm and h3b_residual_norm_backward
+  const void *x, *y, *w, *gate, *shift, *scale, *dt, *dh;
+  void *t, *h, *dx, *dy, *dw;
+  int8_t* codes;
+  float *scales, *rstd;
+  int64_t ldx, ldy, ldm, ldt, ldh, ldc, lddt, lddh, lddx, lddy, M;
+  int K, dtype, w_dtype, m_dtype;
+  float eps;
+  const int* token_rows;  // modulation row of each token (outside 0 .. n_rows - 1: none), or null: the segments decide
+  int n_rows;
+  SegTable segs;
+  void* ws;
+};
+size_t resnorm_workspace(int64_t M, int K, bool backward);
+int resnorm_launch(const ResNormArgs& a, bool backward, cudaStream_t st);
 
 // ---- k_decode.cu
 int decode_launch(const void* q4, int64_t N, int64_t K, int64_t ldq4, const void* s_rel, int s_dtype, int64_t lds,

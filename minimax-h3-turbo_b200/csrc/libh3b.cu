@@ -393,6 +393,91 @@ int h3b_cross_attention_backward(const h3b_attn_tensor* grad_o, const h3b_attn_t
                       const_cast<float*>(lse), workspace, true, static_cast<cudaStream_t>(stream));
 }
 
+static int check_residual_sizes(int64_t M, int64_t K) {
+  if (M < 0 || K < 8 || K % 8) return fail(H3B_ERR_ARG, "residual_norm: M >= 0, and a width that is a positive multiple of 8, are required");
+  if (K > H3B_MAX_RESIDUAL || M > 0x3FFFFF00) return fail(H3B_ERR_UNSUPPORTED, "residual_norm: at most " + std::to_string(H3B_MAX_RESIDUAL) + " channels and 2^30 rows");
+  return H3B_OK;
+}
+static int check_residual(const ResNormArgs& a, int64_t n_rows, const int32_t* segments, int n_segments, size_t ws_bytes, bool backward) {
+  auto rows = [&](const void* p, int64_t ld, const char* name) {
+    if (p && aligned(p, 16) && ld >= a.K && ld % 8 == 0) return true;
+    fail(H3B_ERR_ARG, std::string("residual_norm: ") + name + " must be 16-byte aligned rows, their stride a multiple of 8 and at least the width");
+    return false;
+  };
+  if (a.dtype != H3B_BF16 && a.dtype != H3B_FP16) return fail(H3B_ERR_ARG, "residual_norm: bf16 or fp16 rows");
+  if (int rc = check_residual_sizes(a.M, a.K)) return rc;
+  if (!a.w || !is_act(a.w_dtype) || !aligned(a.w, 16)) return fail(H3B_ERR_ARG, "residual_norm: the weight must be 16-byte aligned bf16, fp16 or fp32");
+  if (n_segments < 0 || n_segments > H3B_MAX_SEGMENTS || (n_segments > 0 && !segments))
+    return fail(H3B_ERR_ARG, "residual_norm: at most H3B_MAX_SEGMENTS segments, given as a host table");
+  if (!backward && !a.shift != !a.scale) return fail(H3B_ERR_ARG, "residual_norm: shift and scale go together");
+  if (n_rows < 0 || n_rows > 0x7FFFFFFF) return fail(H3B_ERR_ARG, "residual_norm: bad number of modulation rows");
+  for (const void* p : {a.gate, a.shift, a.scale})
+    if (p && (n_rows < 1 || !is_act(a.m_dtype) || !rows(p, a.ldm, "gate, shift and scale")))
+      return fail(H3B_ERR_ARG, "residual_norm: gate, shift and scale must be [n_rows, width] bf16, fp16 or fp32, in 16-byte aligned rows");
+  for (int i = 0; i < n_segments; ++i)
+    if (segments[3 * i] < 0 || segments[3 * i + 1] < segments[3 * i] || segments[3 * i + 2] < 0 || segments[3 * i + 2] >= n_rows)
+      return fail(H3B_ERR_ARG, "residual_norm: a segment has a negative bound, ends before it starts, or names a row >= n_rows");
+  if (!aligned(a.token_rows, 4) || !aligned(a.rstd, 4) || !aligned(a.scales, 4)) return fail(H3B_ERR_ARG, "residual_norm: token_rows, rstd and scales must be 4-byte aligned");
+  if (a.M > 0) {
+    if (!rows(a.t, a.ldt, "t")) return H3B_ERR_ARG;
+    if (!backward) {
+      if (!rows(a.x, a.ldx, "x") || !rows(a.y, a.ldy, "y") || (a.h && !rows(a.h, a.ldh, "h"))) return H3B_ERR_ARG;
+      if (a.codes && (a.K % 256 || a.ldc < a.K || a.ldc % 16 || !aligned(a.codes, 16) || !a.scales))
+        return fail(H3B_ERR_ARG, "residual_norm: codes need a width that is a multiple of 256, 16-byte aligned rows and scales");
+    } else {
+      if (!rows(a.dh, a.lddh, "grad_h") || !rows(a.dx, a.lddx, "dx") || (a.dt && !rows(a.dt, a.lddt, "grad_t")) ||
+          (a.dy && !rows(a.dy, a.lddy, "dy")))
+        return H3B_ERR_ARG;
+      if (a.dy && !a.gate) return fail(H3B_ERR_ARG, "residual_norm: without a gate dy is dx");
+      if (!a.rstd) return fail(H3B_ERR_ARG, "residual_norm: rstd is missing");
+    }
+  }
+  if (backward && a.dw && !aligned(a.dw, 16)) return fail(H3B_ERR_ARG, "residual_norm: dw must be 16-byte aligned");
+  const size_t need = resnorm_workspace(a.M, a.K, backward);
+  if (need > 0 && (!a.ws || ws_bytes < need || !aligned(a.ws, 256)))
+    return fail(H3B_ERR_ARG, "residual_norm: workspace must be 256-byte aligned and hold " + std::to_string(need) + " bytes");
+  return H3B_OK;
+}
+static void set_segments(ResNormArgs& a, const int32_t* segments, int n) {
+  a.segs.n = a.token_rows ? 0 : n;
+  for (int i = 0; i < a.segs.n; ++i) a.segs.first[i] = segments[3 * i], a.segs.end[i] = segments[3 * i + 1], a.segs.row[i] = segments[3 * i + 2];
+}
+
+size_t h3b_residual_norm_workspace_bytes(int64_t M, int64_t K, int backward) {
+  return check_residual_sizes(M, K) ? 0 : resnorm_workspace(M, static_cast<int>(K), backward != 0);
+}
+int h3b_residual_norm(const void* x, int64_t ldx, const void* y, int64_t ldy, int dtype, int64_t M, int64_t K, const void* w,
+                      int w_dtype, float eps, const void* gate, const void* shift, const void* scale, int64_t ldm,
+                      int64_t n_rows, int m_dtype, const int32_t* segments, int n_segments, const int32_t* token_rows, void* t,
+                      int64_t ldt, void* h, int64_t ldh, int8_t* codes, int64_t ldc, float* scales, float* rstd,
+                      void* workspace, size_t ws_bytes, void* stream) {
+  if (int rc = check_residual_sizes(M, K)) return rc;
+  ResNormArgs a{};
+  a.x = x, a.ldx = ldx, a.y = y, a.ldy = ldy, a.dtype = dtype, a.M = M, a.K = static_cast<int>(K), a.w = w, a.w_dtype = w_dtype;
+  a.eps = eps, a.gate = gate, a.shift = shift, a.scale = scale, a.ldm = ldm, a.m_dtype = m_dtype, a.token_rows = token_rows;
+  a.t = t, a.ldt = ldt, a.h = h, a.ldh = ldh, a.codes = codes, a.ldc = ldc, a.scales = scales, a.rstd = rstd, a.ws = workspace;
+  if (int rc = check_residual(a, n_rows, segments, n_segments, ws_bytes, false)) return rc;
+  a.n_rows = static_cast<int>(n_rows);
+  set_segments(a, segments, n_segments);
+  return M == 0 ? H3B_OK : resnorm_launch(a, false, static_cast<cudaStream_t>(stream));
+}
+int h3b_residual_norm_backward(const void* grad_t, int64_t lddt, const void* grad_h, int64_t lddh, const void* t, int64_t ldt,
+                               const float* rstd, int dtype, int64_t M, int64_t K, const void* w, int w_dtype, const void* gate,
+                               const void* scale, int64_t ldm, int64_t n_rows, int m_dtype, const int32_t* segments,
+                               int n_segments, const int32_t* token_rows, void* dx, int64_t lddx, void* dy, int64_t lddy,
+                               void* dw, void* workspace, size_t ws_bytes, void* stream) {
+  if (int rc = check_residual_sizes(M, K)) return rc;
+  ResNormArgs a{};
+  a.dt = grad_t, a.lddt = lddt, a.dh = grad_h, a.lddh = lddh, a.t = const_cast<void*>(t), a.ldt = ldt;
+  a.rstd = const_cast<float*>(rstd), a.dtype = dtype, a.M = M, a.K = static_cast<int>(K), a.w = w, a.w_dtype = w_dtype, a.gate = gate;
+  a.scale = scale, a.ldm = ldm, a.m_dtype = m_dtype, a.token_rows = token_rows, a.dx = dx, a.lddx = lddx, a.dy = dy;
+  a.lddy = lddy, a.dw = dw, a.ws = workspace;
+  if (int rc = check_residual(a, n_rows, segments, n_segments, ws_bytes, true)) return rc;
+  a.n_rows = static_cast<int>(n_rows);
+  set_segments(a, segments, n_segments);
+  return resnorm_launch(a, true, static_cast<cudaStream_t>(stream));
+}
+
 // ranks, rows and widths that the plan, the workspace and the launches take
 static int check_low_rank_sizes(int64_t M, int64_t K, int64_t N, int rank, int64_t R) {
   if (M < 0 || K < 8 || N < 8 || K % 8 || N % 8) return fail(H3B_ERR_ARG, "low_rank: M >= 0, and widths that are positive multiples of 8, are required");

@@ -21,6 +21,7 @@ from . import qlinear as ql
 from .rope import no_tangents
 from .types import Weight
 
+Scales = Union[None, float, torch.Tensor]
 Rows = Union[torch.Tensor, Sequence[Tuple[int, int, int]]]
 _CODES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16}
 
@@ -167,6 +168,27 @@ class _Problem:
             _lib.check(rc, what)
 
 
+@dataclass(frozen=True)
+class Adapters:
+    """The adapters beside one projection: a [adapters, rank, K], b [adapters, N, rank], scales a number or fp32 [adapters]."""
+
+    a: torch.Tensor
+    b: torch.Tensor
+    scales: Scales = None
+
+
+@dataclass(frozen=True)
+class BlockAdapters:
+    """The adapters of one DiT block (None: that projection has none) and the plan of the batch's rows.  fc2's read what fc2
+    reads: swiglu of fc1's output."""
+
+    plan: AdapterPlan
+    qkv: Optional[Adapters] = None
+    out: Optional[Adapters] = None
+    fc1: Optional[Adapters] = None
+    fc2: Optional[Adapters] = None
+
+
 def _whole(m: int, dev: torch.device) -> AdapterPlan:
     """All rows have the one adapter."""
     return plan(torch.zeros(m, dtype=torch.int32, device=dev), 1)
@@ -254,7 +276,7 @@ class _LowRank(torch.autograd.Function):
 
 
 def low_rank(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, plan: Optional[AdapterPlan] = None, *,
-             base: Optional[torch.Tensor] = None, scales: Union[None, float, torch.Tensor] = None,
+             base: Optional[torch.Tensor] = None, scales: Scales = None,
              out: Optional[torch.Tensor] = None, return_hidden: bool = False):
     """out_i = base_i + s_g (x_i A_g^T) B_g^T for x [..., K] -> [..., N], or (out, hidden) with return_hidden.
 
@@ -289,7 +311,7 @@ def low_rank(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, plan: Optional[A
 
 
 def low_rank_backward(do: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, plan: Optional[AdapterPlan],
-                      hidden: torch.Tensor, *, scales: Union[None, float, torch.Tensor] = None,
+                      hidden: torch.Tensor, *, scales: Scales = None,
                       need: Tuple[bool, bool, bool] = (True, True, True)
                       ) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor], Optional[torch.Tensor]]:
     """Gradients (dx, da, db) of low_rank's out with respect to x, a and b from the gradient do of out (base's gradient is do
@@ -303,7 +325,7 @@ def low_rank_backward(do: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: tor
 
 
 def linear(x: torch.Tensor, w: Weight, a: torch.Tensor, b: torch.Tensor, plan: Optional[AdapterPlan] = None,
-           bias: Optional[torch.Tensor] = None, *, scales: Union[None, float, torch.Tensor] = None, **kw) -> torch.Tensor:
+           bias: Optional[torch.Tensor] = None, *, scales: Scales = None, **kw) -> torch.Tensor:
     """The shared projection and its adapters: qlinear.linear(x, w, bias, **kw) + s_g (x A_g^T) B_g^T.  kw as qlinear.linear
     takes it, without input_act (the adapters read x as it is) and with outputs of x's type.  A W4A8 weight has no gradient
     for x: where x requires one, that raises (a dense weight gives it)."""

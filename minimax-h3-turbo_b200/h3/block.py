@@ -425,12 +425,14 @@ class DiTBlock:
     "ring" (shards passed round the ranks, one attention call and merge per shard).  `ops`: the operator set (KernelOps; tests of the
     sharding plumbing on CPU ranks pass the reference's torch formulas).  `probe(tag)`, when given, is called on the
     host at the phase boundaries of the attention ("qk_ready", "local_done", "kv_ready", "attn_done") so a caller can
-    record CUDA events there."""
+    record CUDA events there.  fuse_residual: between attention and MLP, the gated residual, the norm and fc1's quantiser are
+    one pass (residual.residual_norm); it rounds once where the separate operators round after every step, so results differ
+    from theirs in the last bits (off by default)."""
 
     def __init__(self, heads: int, head_dim: int, norm_eps: float = 1e-5, qk_norm_eps: float = 1e-5,
                  precision: str = "a8", attn_chunk: Optional[int] = None, linear=None, kv_exchange: str = "gather",
                  fuse_norm: Optional[bool] = None, kv_groups: int = 1, ops=None,
-                 probe: Optional[Callable[[str], None]] = None):
+                 probe: Optional[Callable[[str], None]] = None, fuse_residual: bool = False):
         if kv_exchange not in KV_EXCHANGES:
             raise ValueError(f"kv_exchange must be one of {KV_EXCHANGES}, got {kv_exchange!r}")
         if kv_groups < 1:
@@ -448,22 +450,38 @@ class DiTBlock:
         # RMSNorm + modulation fused into the quantiser of the qkv and fc1 linears: on for the default linear; a custom
         # linear opts in with fuse_norm=True and then receives a Prenorm for those two
         self._fuse_norm = linear is None if fuse_norm is None else fuse_norm
+        if fuse_residual and not (self._fuse_norm and linear is None and ops is None and precision == "a8"):
+            raise ValueError("fuse_residual runs with the block's own linear, operators and int8 activations")
+        self.fuse_residual = fuse_residual
 
     def _mark(self, tag: str) -> None:
         if self.probe:
             self.probe(tag)
 
-    def _in_linear(self, h, w) -> torch.Tensor:
-        """The linear that reads the normalised stream (qkv, fc1): h is a tensor or a Prenorm."""
+    def _in_linear(self, h, w, low=None, plan=None) -> torch.Tensor:
+        """The linear that reads the normalised stream (qkv, fc1): h is a tensor or a Prenorm; low: the adapters beside it."""
         if isinstance(h, Prenorm) and self._linear_is_default:
-            return prenorm_linear(h, w, self.precision)
-        return self._linear(h, w)
+            return self._adapted(prenorm_linear(h, w, self.precision), None if low is None else h.materialize(), low, plan)
+        return self._adapted(self._linear(h, w), h.materialize() if low is not None and isinstance(h, Prenorm) else h, low, plan)
+
+    @staticmethod
+    def _adapted(y: torch.Tensor, x: Optional[torch.Tensor], low, plan) -> torch.Tensor:
+        """y, what a linear of this block gave for x, with the products of the adapters beside it added in place."""
+        if low is None:
+            return y
+        from .adapters import low_rank
+
+        return low_rank(x, low.a, low.b, plan, base=y, scales=low.scales, out=y)
+
+    def _out_linear(self, o: torch.Tensor, w: BlockWeights, adapters) -> torch.Tensor:
+        y = self._linear(o, w.out)
+        return y if adapters is None else self._adapted(y, o, adapters.out, adapters.plan)
 
     def attention(self, h: torch.Tensor, w: BlockWeights, cos: torch.Tensor, sin: torch.Tensor,
-                  spec: Optional[ShardSpec] = None) -> torch.Tensor:
+                  spec: Optional[ShardSpec] = None, adapters=None) -> torch.Tensor:
         s, heads, hd = h.shape[0], self.heads, self.head_dim
         inner = heads * hd
-        qkv = self._in_linear(h, w.qkv)
+        qkv = self._in_linear(h, w.qkv, *((None, None) if adapters is None else (adapters.qkv, adapters.plan)))
         q, k, v = (t.view(s, heads, hd) for t in qkv.split(inner, dim=-1))
         self.ops.norm_rope_(q, k, w.q_norm, w.k_norm, self.qk_norm_eps, cos, sin)
         self._mark("qk_ready")
@@ -471,17 +489,17 @@ class DiTBlock:
         if sharded and self.kv_exchange == "overlap":
             o = overlap_attention(q, qkv[:, inner:], spec, self.ops, self.probe)
             self._mark("attn_done")
-            return self._linear(o, w.out)
+            return self._out_linear(o, w, adapters)
         if sharded and self.kv_exchange == "ring":
             o = ring_attention(q, k, v, spec, self.ops)
             self._mark("attn_done")
-            return self._linear(o, w.out)
+            return self._out_linear(o, w, adapters)
         if sharded:  # "gather": every query needs every key and value
             groups = self.kv_groups if heads % self.kv_groups == 0 and not (self.attn_chunk and self.attn_chunk < s) else 1
             if groups > 1:
                 o = self._grouped_gather_attention(q, k, v, spec, groups)
                 self._mark("attn_done")
-                return self._linear(o, w.out)
+                return self._out_linear(o, w, adapters)
             k = gather_rows(k.reshape(s, inner).contiguous(), spec).view(-1, heads, hd)
             v = gather_rows(v.reshape(s, inner).contiguous(), spec).view(-1, heads, hd)
             self._mark("kv_ready")
@@ -494,7 +512,7 @@ class DiTBlock:
             for a in range(0, s, step):
                 o[a:a + step] = self.ops.attention(qh[:, :, a:a + step], kh, vh)[0].transpose(0, 1).reshape(-1, inner)
         self._mark("attn_done")
-        return self._linear(o, w.out)
+        return self._out_linear(o, w, adapters)
 
     def _grouped_gather_attention(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, spec: ShardSpec,
                                   groups: int) -> torch.Tensor:
@@ -518,17 +536,41 @@ class DiTBlock:
                                                               _heads_first(vg))[0].transpose(0, 1).reshape(s, hg * hd)
         return o
 
-    def mlp(self, h: torch.Tensor, w: BlockWeights) -> torch.Tensor:
-        return self._linear(self._in_linear(h, w.fc1), w.fc2, input_act="swiglu")
+    def mlp(self, h: torch.Tensor, w: BlockWeights, adapters=None) -> torch.Tensor:
+        if adapters is None:
+            return self._fc2(self._in_linear(h, w.fc1), w)
+        return self._fc2(self._in_linear(h, w.fc1, adapters.fc1, adapters.plan), w, adapters)
+
+    def _fc2(self, f: torch.Tensor, w: BlockWeights, adapters=None) -> torch.Tensor:
+        y = self._linear(f, w.fc2, input_act="swiglu")
+        if adapters is None or adapters.fc2 is None:
+            return y
+        return self._adapted(y, ql._swiglu(f), adapters.fc2, adapters.plan)
+
+    def _fused_mlp(self, x: torch.Tensor, att: torch.Tensor, w: BlockWeights, mod: Modulation, segments: Sequence[Segment],
+                   adapters) -> torch.Tensor:
+        """x += gate_a att in place, then the MLP of the normalised x: one pass over the stream up to fc1's codes."""
+        from . import residual
+
+        low = None if adapters is None else adapters.fc1
+        w4 = isinstance(w.fc1, ql.W4A8Weight)
+        r = residual.residual_norm(x, att, w.norm2, self.norm_eps, gate=mod.gate_a, shift=mod.shift_m, scale=mod.scale_m,
+                                   segments=segments, codes=w4, hidden=not w4 or low is not None, out=x)
+        f = self._adapted(residual.linear(r, w.fc1), r.hidden, low, None if low is None else adapters.plan)
+        return self._fc2(f, w, adapters)
 
     def __call__(self, x: torch.Tensor, w: BlockWeights, mod: Modulation, segments: Sequence[Segment], cos: torch.Tensor,
-                 sin: torch.Tensor, spec: Optional[ShardSpec] = None) -> torch.Tensor:
-        """x: [S_local, hidden] residual stream (updated in place and returned); cos/sin: [S_local, half] for these rows."""
+                 sin: torch.Tensor, spec: Optional[ShardSpec] = None, adapters=None) -> torch.Tensor:
+        """x: [S_local, hidden] residual stream (updated in place and returned); cos/sin: [S_local, half] for these rows;
+        adapters (adapters.BlockAdapters): the low-rank adapters beside the block's linears, their plan of these rows."""
         norm = Prenorm if self._fuse_norm else self.ops.rms_modulate
         h = norm(x, w.norm1, self.norm_eps, mod.shift_a, mod.scale_a, segments)
-        self.ops.gate_(x, mod.gate_a, self.attention(h, w, cos, sin, spec), segments)
+        att = self.attention(h, w, cos, sin, spec, adapters)
+        if self.fuse_residual:
+            return self.ops.gate_(x, mod.gate_m, self._fused_mlp(x, att, w, mod, segments, adapters), segments)
+        self.ops.gate_(x, mod.gate_a, att, segments)
         h = norm(x, w.norm2, self.norm_eps, mod.shift_m, mod.scale_m, segments)
-        return self.ops.gate_(x, mod.gate_m, self.mlp(h, w), segments)
+        return self.ops.gate_(x, mod.gate_m, self.mlp(h, w, adapters), segments)
 
 
 def rope_tables(positions: torch.Tensor, inv_freq: torch.Tensor, dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor]:
