@@ -483,7 +483,7 @@ static int check_low_rank_sizes(int64_t M, int64_t K, int64_t N, int rank, int64
   if (M < 0 || K < 8 || N < 8 || K % 8 || N % 8) return fail(H3B_ERR_ARG, "low_rank: M >= 0, and widths that are positive multiples of 8, are required");
   if (rank < 1 || rank > H3B_MAX_RANK) return fail(H3B_ERR_ARG, "low_rank: the rank must be 1 to " + std::to_string(H3B_MAX_RANK));
   if (R < 1 || R > H3B_MAX_ADAPTERS) return fail(H3B_ERR_ARG, "low_rank: 1 to " + std::to_string(H3B_MAX_ADAPTERS) + " adapters");
-  if (M > 0x3FFFFF00 || K > 0x3FFFFF00 || N > 0x3FFFFF00) return fail(H3B_ERR_UNSUPPORTED, "low_rank: at most 2^30 rows and channels");
+  if (M > (1 << 27) || K > (1 << 20) || N > (1 << 20)) return fail(H3B_ERR_UNSUPPORTED, "low_rank: at most 2^27 rows and 2^20 channels");
   return H3B_OK;
 }
 // a row-major operand of `width` columns: 16-byte aligned rows that do not overlap
@@ -502,6 +502,7 @@ static int check_low_rank(const LrArgs& a, size_t ws_bytes, bool backward) {
     int rc = check_rows(a.x, a.ldx, a.K, "x");
     if (!rc && !backward) rc = check_rows(a.out, a.ldo, a.N, "out");
     if (!rc && a.base) rc = check_rows(a.base, a.ldbase, a.N, "base");
+    if (!rc && a.base && a.base == a.out && a.ldbase != a.ldo) rc = fail(H3B_ERR_ARG, "low_rank: rows of an out that is base have base's stride");
     if (!rc && backward) rc = check_rows(a.go, a.ldgo, a.N, "grad_out");
     if (!rc && a.dx) rc = check_rows(a.dx, a.lddx, a.K, "dx");
     if (rc) return rc;
