@@ -188,7 +188,7 @@ static LrHidden lr_hidden(void* p, int64_t M, int rank) {
 // ----------------------------------------------------------------------------------------------- common parts of the tile kernels
 // 16 bytes from global to shared memory without passing through registers; zeros where ok is false (nothing is read then)
 __device__ __forceinline__ void lr_copy16(uint32_t dst, const void* src, bool ok) {
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16u : 0u) : "memory");
+  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16u : 0u) : "memory");
 }
 __device__ __forceinline__ void lr_copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -212,6 +212,84 @@ __device__ __forceinline__ void lr_arrive_full(uint64_t* bar) {
   if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
+// ----------------------------------------------------------------------------------------------- rows through registers
+// The first two products have 2 rank flops to a byte of x, base or out and are HBM-bound, so what counts is how these bytes travel.
+// They go between global memory and the registers that feed mma.sync directly, 32 bytes to a lane and 128 to a row (four lanes)
+// an instruction.  Fragments of m16n8k16 would have a lane touch 4 bytes of a row; but which numbers a product calls its k (or
+// its n) is free as long as both operands agree, so lane t of a row takes 16 numbers in one piece and hands them out as the
+// fragments' k (n) 2 t, 2 t + 1 (and 2 t + 8, 2 t + 9) of several products; the small operand W is put in that order in shared memory.
+// (tcgen05 forms of both, X by cp.async or out by way of tensor memory, measured 2 to 3 times their floors: 37 us for X of 12090 x
+// 5120, 220 us for base and out of 12090 x 15360; they have too few bytes under way next to their buffers.)
+template <typename T>
+__device__ __forceinline__ void lr_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same_v<T, __half>)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// four 8 x 8 matrices of 16-bit numbers, each transposed on the way: lane l gives the address of row l % 8 of matrix l / 8
+__device__ __forceinline__ void lr_ldmatrix_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+// 16 numbers of a row from p on, `left` of them there (a multiple of 8, also negative); wide: rows start on 32-byte boundaries
+template <typename T>
+__device__ __forceinline__ void lr_load16(const T* p, int64_t left, bool wide, uint32_t (&v)[8]) {
+  if (wide && left >= 16) {
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                 : "l"(p)
+                 : "memory");
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    uint4 u = make_uint4(0, 0, 0, 0);
+    if (left > 8 * i) u = *reinterpret_cast<const uint4*>(p + 8 * i);
+    v[4 * i] = u.x, v[4 * i + 1] = u.y, v[4 * i + 2] = u.z, v[4 * i + 3] = u.w;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void lr_store16(T* p, int64_t left, bool wide, const uint32_t (&v)[8]) {
+  if (wide && left >= 16) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (left > 8 * i) *reinterpret_cast<uint4*>(p + 8 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+}
+template <typename T>
+__device__ __forceinline__ float2 lr_unpack2(uint32_t w) {
+  if constexpr (std::is_same_v<T, __half>) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+// 8 numbers of a row of `rank`, from j on, into shared memory; zeros behind the rank and where ok is false.  Rows of ranks that are no
+// multiples of 8 do not start on 16-byte boundaries and are read number by number.
+template <typename T>
+__device__ __forceinline__ void lr_stage8(uint32_t dst, const T* row, int j, int rank, bool ok) {
+  if (rank % 8 == 0) {
+    lr_copy16(dst, ok && j < rank ? row + j : row, ok && j < rank);
+  } else {
+    uint32_t v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t lo = ok && j + 2 * i < rank ? *reinterpret_cast<const uint16_t*>(row + j + 2 * i) : 0u;
+      const uint32_t hi = ok && j + 2 * i + 1 < rank ? *reinterpret_cast<const uint16_t*>(row + j + 2 * i + 1) : 0u;
+      v[i] = lo | hi << 16;
+    }
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+  }
+}
+
 // ----------------------------------------------------------------------------------------------- first product: hidden rows
 // H [128 rows, rp] of a tile = X [128, C] W, C the contraction: W is A_g [rank, C] (W_ROWS) or B_g [C, rank].  HBM-bound: X is read
 // once, 2 rank flops a byte.  The CTAs of a cluster share a tile's C (95 tiles of 12090 rows would leave a third of the SMs idle)
@@ -219,26 +297,27 @@ __device__ __forceinline__ void lr_arrive_full(uint64_t* bar) {
 // gathered.  Warps 0-3 copy, then read the accumulators; warp 4 issues the products.
 constexpr int LR_XPART = LR_TILE * 128;  // 64 channels of 128 rows
 constexpr int LR_SHRINK_THREADS = 160;
-template <int STAGES>  // 5 with W_ROWS only: B_g's parts are 64 channels wide
+template <int RPM>  // the largest rp of this variant: 64 or 128
 struct LrShrinkCfg {
-  static constexpr int RP = STAGES == 5 ? 32 : STAGES == 4 ? 64 : 128;  // the largest rp of this variant
-  static constexpr int WBYTES = RP * 128;
+  static constexpr int STAGES = 3, CTAS = RPM == 128 ? 2 : 3;  // stages, CTAs to an SM
+  static constexpr int WBYTES = RPM == 128 ? 16384 : 8192;
   static constexpr int STAGE = LR_XPART + WBYTES;
   static constexpr int SMEM = STAGES * STAGE + 1024;
 };
-// The power of two that brings a row whose largest magnitude is `top` into [1, 2); the smallest for rows of zeros (which
-// then has no say in the largest of several rows), 1 for infinities and NaN.
+// The power of two that brings a row whose largest magnitude is `top` into [1, 2), 2^-60 at least (rows below add nothing that
+// fp16 holds; and a row of zeros has no say in the largest power of several rows); 1 for infinities and NaN.
 __device__ __forceinline__ float lr_power(float top) {
   const int e = (__float_as_int(top) >> 23) & 0xFF;
-  return e >= 253 ? 1.f : __int_as_float(max(e, 1) << 23);
+  return e >= 253 ? 1.f : __int_as_float(max(e, 127 - 60) << 23);
 }
 
-template <typename T, bool W_ROWS, int STAGES>
+template <typename T, bool W_ROWS, int RPM>
 __global__ void __launch_bounds__(LR_SHRINK_THREADS) lr_shrink_kernel(const LrPlan p, const T* x, int64_t ldx, int64_t C,
-                                                                      const T* w, int rank, int ldw, int rp, int R, const float* scales, const LrHidden out,
+                                                                      const T* w, int rank, int rp, int R, const float* scales, const LrHidden out,
                                                                       int splits) {
-  using Cfg = LrShrinkCfg<STAGES>;
-  extern __shared__ unsigned char lr_smem[];
+  using Cfg = LrShrinkCfg<RPM>;
+  constexpr int STAGES = Cfg::STAGES;
+  extern __shared__ __align__(1024) unsigned char lr_smem[];
   __shared__ uint64_t full[STAGES], empty[STAGES], done;
   __shared__ uint32_t tmem_at;
   __shared__ int abort_flag;
@@ -290,7 +369,7 @@ __global__ void __launch_bounds__(LR_SHRINK_THREADS) lr_shrink_kernel(const LrPl
       const int r = r0 + 16 * i;
       xr[i] = r < t.z ? x + static_cast<int64_t>(p.order[t.y + r]) * ldx + ch * 8 : nullptr;
     }
-    const T* wg = w + static_cast<int64_t>(t.x) * (W_ROWS ? rank * C : C * ldw);
+    const T* wg = w + static_cast<int64_t>(t.x) * rank * C;
     const uint32_t at = static_cast<uint32_t>(r0 * 128 + ((ch ^ (r0 & 7)) << 4));
     for (int i = 0; i < n + STAGES - 1; ++i) {
       if (i < n) {
@@ -303,20 +382,19 @@ __global__ void __launch_bounds__(LR_SHRINK_THREADS) lr_shrink_kernel(const LrPl
         for (int j = 0; j < 8; ++j) lr_copy16(xs + j * 2048, xr[j] && in ? xr[j] + c : x, xr[j] && in);
         if constexpr (W_ROWS) {
 #pragma unroll
-          for (int j = 0; j < Cfg::RP / 16; ++j) {
+          for (int j = 0; j < RPM / 16; ++j) {
             const int r = r0 + 16 * j;
             if (16 * j < rp) lr_copy16(ws + j * 2048, r < rank && in ? wg + r * C + c + ch * 8 : w, r < rank && in);
           }
         } else {
 #pragma unroll
-          for (int part = 0; part < (Cfg::RP + 63) / 64; ++part) {
+          for (int part = 0; part < (RPM + 63) / 64; ++part) {
             const int k = part * 64 + ch * 8;
             if (k < rp) {
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
                 const int64_t r = c + r0 + 16 * j;
-                const bool ok = r < C && k < ldw;
-                lr_copy16(ws + part * 8192 + j * 2048, ok ? wg + r * ldw + k : w, ok);
+                lr_stage8(ws + part * 8192 + j * 2048, r < C ? wg + r * rank : w, k, rank, r < C);
               }
             }
           }
@@ -392,216 +470,136 @@ __global__ void __launch_bounds__(LR_SHRINK_THREADS) lr_shrink_kernel(const LrPl
 }
 
 // ----------------------------------------------------------------------------------------------- second product: out or dx
-// out [128 rows, N] of a tile = base + H W^T: W is B_g [N, rank] (W_ROWS) or A_g [rank, N].  HBM-bound: base and out are touched once,
-// 32 bytes of a row per thread and instruction (full sectors), the next 128 columns' base on the way while these are added.  Warps
-// 0-7 read the accumulators (a row per lane, 64 columns per warp), 8-11 copy, 12 issues the products.
-constexpr int LR_NT = 128;  // columns of a step
-constexpr int LR_EXPAND_THREADS = 416;
-template <int RPM>  // the largest rp of this variant: 64 or 128
+// out [128 rows, N] of a tile = base + H W^T: W is B_g [N, rank] (W_ROWS) or A_g [rank, N].  A CTA has 64 CB columns of a tile, a warp 16
+// rows of them: all of its base is asked for at once, then W goes to shared memory, then the products are added and stored.
+//   block of 64 columns: lane t has columns 16 t .. 16 t + 15; 2 j, 2 j + 1 of these are product j's n = 2 t, 2 t + 1
+constexpr int LR_THREADS = 256;
+template <int NQ, bool W_ROWS>  // 16 NQ: the largest rp of this variant
 struct LrExpandCfg {
-  static constexpr int PARTS = RPM / 64, STAGES = RPM == 64 ? 3 : 2;
-  static constexpr int TILE = PARTS * LR_XPART;
-  static constexpr int SMEM = TILE + STAGES * TILE + 1024;
+  static constexpr int CB = 2, COLS = 64 * CB;
+  // rows of W: [COLS][16 NQ], 32 bytes apart from a multiple of 64; or [16 NQ][COLS], 16 from a multiple of 128: no bank conflicts
+  static constexpr int LDW = W_ROWS ? (32 * NQ + 31) / 64 * 64 + 32 : 2 * COLS + 16;
+  static constexpr int SMEM = LDW * (W_ROWS ? COLS : 16 * NQ);
+  static constexpr int CTAS = NQ <= 4 ? 3 : 2;
 };
-// 16 columns of a row, `left` of them in the tensor (a multiple of 8)
-template <typename T>
-__device__ __forceinline__ void lr_load16(const T* p, int64_t left, bool wide, uint32_t (&v)[8]) {
-  if (left >= 16 && wide) {
-    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
-                 : "l"(p)
-                 : "memory");
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    uint4 u = make_uint4(0, 0, 0, 0);
-    if (left > 8 * i) u = *reinterpret_cast<const uint4*>(p + 8 * i);
-    v[4 * i] = u.x, v[4 * i + 1] = u.y, v[4 * i + 2] = u.z, v[4 * i + 3] = u.w;
-  }
-}
-template <typename T>
-__device__ __forceinline__ void lr_store16(T* p, int64_t left, bool wide, const uint32_t (&v)[8]) {
-  if (left >= 16 && wide) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
-                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-                 : "memory");
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    if (left > 8 * i) *reinterpret_cast<uint4*>(p + 8 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-}
-template <typename T>
-__device__ __forceinline__ float2 lr_unpack2(uint32_t w) {
-  if constexpr (std::is_same_v<T, __half>) return __half22float2(*reinterpret_cast<const __half2*>(&w));
-  else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
-}
-
-template <typename T, bool W_ROWS, int RPM>
-__global__ void __launch_bounds__(LR_EXPAND_THREADS, 2) lr_expand_kernel(const LrPlan p, const LrHidden hid, const T* w,
-                                                                         int rank, int ldw, int rp, int R, const T* base, int64_t ldb,
-                                                                         T* out, int64_t ldo, int64_t N, int per, int parts, bool wide) {
-  using Cfg = LrExpandCfg<RPM>;
-  constexpr int ST = Cfg::STAGES;
-  extern __shared__ unsigned char lr_smem[];
-  __shared__ uint64_t full[ST], empty[ST], h_full, acc_full[2], acc_empty[2];
-  __shared__ uint32_t tmem_at;
-  __shared__ int abort_flag;
+template <typename T, bool W_ROWS, int NQ>
+__global__ void __launch_bounds__(LR_THREADS, LrExpandCfg<NQ, W_ROWS>::CTAS)
+    lr_expand_kernel(const LrPlan p, const LrHidden hid, const T* w, int rank, int rp, int R, const T* base, int64_t ldb, T* out,
+                     int64_t ldo, int64_t N, int parts, bool wide) {
+  using Cfg = LrExpandCfg<NQ, W_ROWS>;
+  constexpr int CB = Cfg::CB, COLS = Cfg::COLS, LDW = Cfg::LDW;
+  extern __shared__ __align__(1024) unsigned char lr_smem[];
   after_previous();
-  const int tile = blockIdx.x / parts;  // `parts` CTAs to a tile, `per` steps of columns each
+  const int tile = blockIdx.x / parts;
+  const int64_t c0 = static_cast<int64_t>(blockIdx.x - tile * parts) * COLS;
   const int4 t = p.tiles[tile];
-  if (t.z == 0) return;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int steps = static_cast<int>((N + LR_NT - 1) / LR_NT), s0 = (blockIdx.x - tile * parts) * per, n = min(per, steps - s0);
+  if (t.z == 0 || (t.x >= R && base == out)) return;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q4 = lane & 3;
+  const int r0 = 16 * warp + g;
+  const int64_t c = c0 + 16 * q4;
+  int row[2];
+  uint32_t v[CB][2][8];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) row[h] = r0 + 8 * h < t.z ? p.order[t.y + r0 + 8 * h] : -1;
+#pragma unroll
+  for (int b = 0; b < CB; ++b)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) lr_load16(base + row[h] * ldb + c + 64 * b, base && row[h] >= 0 ? N - c - 64 * b : 0, wide, v[b][h]);
   if (t.x >= R) {  // rows without an adapter
-    if (base == out) return;
-    const int64_t from = static_cast<int64_t>(s0) * LR_NT, cols = min(static_cast<int64_t>(n) * LR_NT, N - from) / 8;
-    for (int r = warp; r < t.z; r += LR_EXPAND_THREADS / 32) {
-      const int64_t row = p.order[t.y + r];
-      for (int64_t c = lane; c < cols; c += 32)
-        *reinterpret_cast<uint4*>(out + row * ldo + from + 8 * c) =
-            base ? *reinterpret_cast<const uint4*>(base + row * ldb + from + 8 * c) : make_uint4(0, 0, 0, 0);
-    }
+#pragma unroll
+    for (int b = 0; b < CB; ++b)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) lr_store16(out + row[h] * ldo + c + 64 * b, row[h] >= 0 ? N - c - 64 * b : 0, wide, v[b][h]);
     return;
   }
-  unsigned char* const hs = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(lr_smem) + 1023) & ~static_cast<uintptr_t>(1023));
-  unsigned char* const wsm = hs + Cfg::TILE;
-  volatile int* abort = &abort_flag;
-  if (warp == 12) {
-    if (lane == 0) {
-      for (int i = 0; i < ST; ++i) mbar_init(&full[i], 4), mbar_init(&empty[i], 1);
-      for (int i = 0; i < 2; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], 8);
-      mbar_init(&h_full, 4);
-      mbar_fence_init();
-      abort_flag = 0;
-    }
-    tmem_alloc(&tmem_at, 2 * LR_NT);
-    tmem_relinquish();
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = tmem_at;
-  if (warp < 8) {
-    const int r = 32 * (warp & 3) + lane, half = warp >> 2;
-    const bool valid = r < t.z;
-    const int64_t row = valid ? p.order[t.y + r] : 0;
-    const float mult = std::is_same_v<T, __half> && valid ? hid.mult[t.y + r] : 1.f;
-    int64_t c = static_cast<int64_t>(s0) * LR_NT + half * 64;
-    const T* b = base + row * ldb + c;
-    T* o = out + row * ldo + c;
-    int64_t left = valid ? N - c : 0;
-    uint32_t v[4][8];
+  const uint32_t sm = smem_u32(lr_smem);
+  const T* wg = w + static_cast<int64_t>(t.x) * rank * N;
+  if constexpr (W_ROWS) {
+    // column 16 a + 2 j + i of a block of 64 lies at 8 j + 2 a + i: the eight columns of a product in a piece
 #pragma unroll
-    for (int k = 0; k < 4; ++k) lr_load16(b + 16 * k, base ? left - 16 * k : 0, wide, v[k]);
-    for (int i = 0; i < n; ++i) {
-      const int buf = i & 1;
-      warp_wait(&acc_full[buf], (i >> 1) & 1, abort);
-      tc_fence_after();
-      const bool more = i + 1 < n && base;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        uint32_t a[16];
-        tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + buf * LR_NT + half * 64 + 16 * k, a);
-        tmem_ld_wait();
-        if (k == 3) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&acc_empty[buf]);
-        }
-        uint32_t res[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float2 f = lr_unpack2<T>(v[k][j]);
-          res[j] = pack2<T>(fmaf(__uint_as_float(a[2 * j]), mult, f.x), fmaf(__uint_as_float(a[2 * j + 1]), mult, f.y));
-        }
-        if (more) lr_load16(b + LR_NT + 16 * k, left - LR_NT - 16 * k, wide, v[k]);
-        lr_store16(o + 16 * k, left - 16 * k, wide, res);
-      }
-      b += LR_NT, o += LR_NT, left -= LR_NT;
-    }
-  } else if (warp < 12) {
-    const int pt = tid - 256, r0 = pt >> 3, ch = pt & 7;
-    const uint32_t at = static_cast<uint32_t>(r0 * 128 + ((ch ^ (r0 & 7)) << 4));
-    const T* h = static_cast<const T*>(hid.h);
-#pragma unroll
-    for (int part = 0; part < Cfg::PARTS; ++part) {
-      const int k = part * 64 + ch * 8;
-      if (k < rp) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int r = r0 + 16 * j;
-          lr_copy16(smem_u32(hs + part * LR_XPART) + at + j * 2048, r < t.z ? h + static_cast<int64_t>(t.y + r) * rp + k : h, r < t.z);
-        }
-      }
+    for (int e = tid; e < COLS * 2 * NQ; e += LR_THREADS) {
+      const int n = e / (2 * NQ), j = e % (2 * NQ) * 8, b = n & 63;
+      const int at = (n & ~63) + (b >> 1 & 7) * 8 + (b >> 4) * 2 + (b & 1);
+      const bool ok = c0 + n < N;
+      if (j < rp) lr_stage8(sm + at * LDW + 2 * j, ok ? wg + (c0 + n) * rank : w, j, rank, ok);
     }
     lr_copy_commit();
-    const T* wg = w + static_cast<int64_t>(t.x) * (W_ROWS ? N * ldw : rank * N);
-    for (int i = 0; i < n + ST - 1; ++i) {
-      if (i < n) {
-        const int s = i % ST;
-        mbar_wait(&empty[s], ((i / ST) & 1) ^ 1, abort);
-        const uint32_t dst = smem_u32(wsm + s * Cfg::TILE) + at;
-        const int64_t c = static_cast<int64_t>(s0 + i) * LR_NT;
-        if constexpr (W_ROWS) {
-#pragma unroll
-          for (int part = 0; part < Cfg::PARTS; ++part) {
-            const int k = part * 64 + ch * 8;
-            if (k < rp) {
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const int64_t r = c + r0 + 16 * j;
-                const bool ok = r < N && k < ldw;
-                lr_copy16(dst + part * LR_XPART + j * 2048, ok ? wg + r * ldw + k : w, ok);
-              }
-            }
-          }
-        } else {
-#pragma unroll
-          for (int part = 0; part < 2; ++part) {
-            const int64_t k = c + part * 64 + ch * 8;
-#pragma unroll
-            for (int j = 0; j < RPM / 16; ++j) {
-              const int r = r0 + 16 * j;
-              const bool ok = r < rank && k < N;
-              if (16 * j < rp) lr_copy16(dst + part * rp * 128 + j * 2048, ok ? wg + r * N + k : w, ok);
-            }
-          }
-        }
-      }
-      lr_copy_commit();
-      if (i == 0) {
-        lr_copy_wait<1>();
-        lr_arrive_full(&h_full);
-      }
-      if (i >= ST - 1) {
-        lr_copy_wait<ST - 1>();
-        lr_arrive_full(&full[(i - (ST - 1)) % ST]);
-      }
-    }
   } else {
-    const uint32_t idesc = lr_idesc<T>(LR_TILE, LR_NT, false, !W_ROWS), ha = desc_rows(smem_u32(hs));
-    warp_wait(&h_full, 0, abort);
-    for (int i = 0; i < n; ++i) {
-      const int s = i % ST, buf = i & 1;
-      warp_wait(&full[s], (i / ST) & 1, abort);
-      warp_wait(&acc_empty[buf], ((i >> 1) & 1) ^ 1, abort);
-      tc_fence_after();
-      const uint32_t ws = smem_u32(wsm + s * Cfg::TILE);
-      if (elect_one())
-        for (int kk = 0; kk < rp / 16; ++kk)
-          mma_f16_ss(tmem + buf * LR_NT, ha + rows_step(kk), W_ROWS ? desc_rows(ws) + rows_step(kk) : lr_desc_mn(ws, rp * 128) + kk * 128,
-                     idesc, kk > 0);
-      __syncwarp();
-      commit_one(&empty[s]);
-      commit_one(&acc_full[buf]);
+    // the same order of columns; pairs of columns stay together
+#pragma unroll
+    for (int e = tid; e < 16 * NQ * (COLS / 8); e += LR_THREADS) {
+      const int r = e / (COLS / 8), n = e % (COLS / 8) * 8, b = n & 63;
+      if (r >= rp) break;
+      uint4 u = make_uint4(0, 0, 0, 0);
+      if (r < rank && c0 + n < N) u = *reinterpret_cast<const uint4*>(wg + r * N + c0 + n);
+      const uint32_t to = sm + r * LDW + 2 * ((n & ~63) + (b >> 1 & 7) * 8 + (b >> 4) * 2);
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(to), "r"(u.x) : "memory");
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + 16), "r"(u.y) : "memory");
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + 32), "r"(u.z) : "memory");
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + 48), "r"(u.w) : "memory");
     }
   }
+  // H: this lane's k are 4 t .. 4 t + 3 of every 16 (W_ROWS), or 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+  uint32_t a[NQ][4];
+  float mult[2], inv[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int64_t pos = t.y + (row[h] >= 0 ? r0 + 8 * h : 0);
+    const T* hr = static_cast<const T*>(hid.h) + pos * rp;
+    mult[h] = std::is_same_v<T, __half> ? hid.mult[pos] : 1.f;
+    inv[h] = 1.f / mult[h];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      uint2 u = make_uint2(0, 0);
+      if (16 * q < rp) {
+        if constexpr (W_ROWS) u = *reinterpret_cast<const uint2*>(hr + 16 * q + 4 * q4);
+        else u = make_uint2(*reinterpret_cast<const uint32_t*>(hr + 16 * q + 2 * q4), *reinterpret_cast<const uint32_t*>(hr + 16 * q + 2 * q4 + 8));
+      }
+      a[q][h] = u.x, a[q][2 + h] = u.y;
+    }
+  }
+  lr_copy_wait<0>();
   __syncthreads();
-  if (warp == 12) {
-    tc_fence_after();
-    tmem_dealloc(tmem, 2 * LR_NT);
+#pragma unroll
+  for (int b = 0; b < CB; ++b) {
+    float d[8][4];  // the sums begin with base (in fp16 over the row's power of two, which is exact)
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float2 f = lr_unpack2<T>(v[b][h][j]);
+        d[j][2 * h] = std::is_same_v<T, __half> ? f.x * inv[h] : f.x;
+        d[j][2 * h + 1] = std::is_same_v<T, __half> ? f.y * inv[h] : f.y;
+      }
+    if constexpr (W_ROWS) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+          if (16 * q >= rp) break;
+          const uint2 u = *reinterpret_cast<const uint2*>(lr_smem + (64 * b + 8 * j + g) * LDW + 32 * q + 8 * q4);
+          lr_mma<T>(d[j], a[q][0], a[q][1], a[q][2], a[q][3], u.x, u.y);
+        }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j += 2)
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+          if (16 * q >= rp) break;
+          uint32_t m[4];
+          lr_ldmatrix_t(m, sm + (16 * q + (lane & 15)) * LDW + 2 * (64 * b + 8 * j) + (lane >> 4) * 16);
+          lr_mma<T>(d[j], a[q][0], a[q][1], a[q][2], a[q][3], m[0], m[1]);
+          lr_mma<T>(d[j + 1], a[q][0], a[q][1], a[q][2], a[q][3], m[2], m[3]);
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t res[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        res[j] = std::is_same_v<T, __half> ? pack2<T>(d[j][2 * h] * mult[h], d[j][2 * h + 1] * mult[h]) : pack2<T>(d[j][2 * h], d[j][2 * h + 1]);
+      lr_store16(out + row[h] * ldo + c + 64 * b, row[h] >= 0 ? N - c - 64 * b : 0, wide, res);
+    }
   }
 }
 
@@ -613,7 +611,7 @@ __global__ void __launch_bounds__(LR_EXPAND_THREADS, 2) lr_expand_kernel(const L
 constexpr int LR_KROWS = 64;  // rows of a stage
 template <int RPM>
 struct LrWgradCfg {
-  static constexpr int PARTS = RPM / 64, STAGES = RPM == 64 ? 4 : 3;
+  static constexpr int PARTS = RPM / 64, STAGES = 3;
   static constexpr int XBYTES = 2 * LR_KROWS * 128, STAGE = XBYTES + PARTS * LR_KROWS * 128;
   static constexpr int SMEM = STAGES * STAGE + 1024;
 };
@@ -632,7 +630,7 @@ __global__ void __launch_bounds__(160) lr_wgrad_kernel(const LrPlan p, const LrW
                                                        int R) {
   using Cfg = LrWgradCfg<RPM>;
   constexpr int ST = Cfg::STAGES;
-  extern __shared__ unsigned char lr_smem[];
+  extern __shared__ __align__(1024) unsigned char lr_smem[];
   __shared__ uint64_t full[ST], empty[ST], done;
   __shared__ uint32_t tmem_at;
   __shared__ int abort_flag;
@@ -772,11 +770,12 @@ __global__ void __launch_bounds__(160) lr_wgrad_kernel(const LrPlan p, const LrW
     tmem_dealloc(tmem, lr_tmem_cols(rp));
   }
 }
-// The parts of an adapter's units, added up in their order; zeros for adapters without rows.  A CTA: 32 channels of one adapter.
+// The parts of an adapter's units, added up in their order; zeros for adapters without rows.  A CTA: 1024 numbers (1024 / rp channels)
+// of one adapter, four to a thread, so that the loads of 16 parts are on the way at once.
 template <typename T>
 __global__ void __launch_bounds__(256) lr_join_kernel(const LrPlan p, const LrWgradSide<T> sa, const LrWgradSide<T> sb, int blocks_a,
                                                       int rank, int rp) {
-  __shared__ float sums[32][H3B_MAX_RANK + 1];
+  __shared__ float sums[1024 + 128];  // a line of rp + 1 numbers to a channel
   after_previous();
   const int g = blockIdx.y;
   const int s0 = p.slot[g], s1 = p.slot[g + 1];
@@ -784,57 +783,59 @@ __global__ void __launch_bounds__(256) lr_join_kernel(const LrPlan p, const LrWg
   if (s0 == s1 && !none) return;
   const bool second = static_cast<int>(blockIdx.x) >= blocks_a;
   const LrWgradSide<T>& sd = second ? sb : sa;
-  const int64_t col = static_cast<int64_t>(second ? blockIdx.x - blocks_a : blockIdx.x) * 32;
-  const int cols = static_cast<int>(min(static_cast<int64_t>(32), sd.C - col));
-  for (int e = threadIdx.x; e < cols * rp; e += 256) {
-    const float* from = sd.part + col * rp + e;
-    float sum = 0.f;
-#pragma unroll 8
-    for (int s = s0; s < s1; ++s) sum += from[s * sd.C * rp];
-    sums[e / rp][e % rp] = sum;
+  const int chans = 1024 / rp;
+  const int64_t col = static_cast<int64_t>(second ? blockIdx.x - blocks_a : blockIdx.x) * chans;
+  const int cols = static_cast<int>(min(static_cast<int64_t>(chans), sd.C - col));
+  const int e = threadIdx.x * 4, c = e / rp, j = e - c * rp;
+  if (c < cols) {
+    const float4* from = reinterpret_cast<const float4*>(sd.part + col * rp + e);
+    const int64_t step = sd.C * rp / 4;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = s0; s < s1; s += 16) {
+      float4 v[16];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) v[k] = s + k < s1 ? from[(s + k) * step] : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < 16; ++k) sum.x += v[k].x, sum.y += v[k].y, sum.z += v[k].z, sum.w += v[k].w;
+    }
+    float* to = sums + c * (rp + 1) + j;
+    to[0] = sum.x, to[1] = sum.y, to[2] = sum.z, to[3] = sum.w;
   }
   __syncthreads();
   T* out = sd.grad + static_cast<int64_t>(g) * rank * sd.C;
-  for (int e = threadIdx.x; e < cols * rank; e += 256) {
-    const int c = sd.by_rank ? e % cols : e / rank, j = sd.by_rank ? e / cols : e % rank;
-    out[sd.by_rank ? j * sd.C + col + c : (col + c) * rank + j] = lr_t<T>(sums[c][j]);
-  }
-}
-
-// b [R, N, rank] with rows of ld = rank rounded up to 8 (zeros behind): rows of other ranks do not start on 16-byte boundaries
-template <typename T>
-__global__ void __launch_bounds__(256) lr_pad_kernel(const T* __restrict__ b, T* __restrict__ to, int64_t rows, int rank, int ld) {
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < rows * ld; i += gridDim.x * 256ll) {
-    const int64_t r = i / ld;
-    const int j = static_cast<int>(i - r * ld);
-    to[i] = j < rank ? b[r * rank + j] : lr_t<T>(0.f);
+  for (int i = threadIdx.x; i < cols * rank; i += 256) {
+    const int cc = sd.by_rank ? i % cols : i / rank, jj = sd.by_rank ? i / cols : i % rank;
+    out[sd.by_rank ? jj * sd.C + col + cc : (col + cc) * rank + jj] = lr_t<T>(sums[cc * (rp + 1) + jj]);
   }
 }
 
 // ----------------------------------------------------------------------------------------------- launches
-static int lr_ldw(int rank) { return (rank + 7) / 8 * 8; }
-// A workspace: hidden rows, padded b, parts of the weight gradients
+// A workspace: hidden rows, parts of the weight gradients
 struct LrSpace {
-  size_t hidden, pad, part_a, part_b, total;
+  size_t part_a, part_b, total;
 };
-static LrSpace lr_space(int64_t M, int64_t K, int64_t N, int rank, int64_t R, bool backward) {
+static LrSpace lr_space(int64_t M, int64_t K, int64_t N, int rank, bool backward) {
   LrSpace s{};
-  s.pad = lr_hidden_bytes(M, rank);
-  s.part_a = s.pad + (rank % 8 ? lr_up256(static_cast<size_t>(R) * N * lr_ldw(rank) * 2) : 0);
+  s.part_a = lr_hidden_bytes(M, rank);
   const size_t slot = backward ? static_cast<size_t>(lr_slots(M)) * lr_rp(rank) * 4 : 0;
   s.part_b = s.part_a + lr_up256(slot * K);
   s.total = s.part_b + lr_up256(slot * N);
   return s;
 }
 size_t lr_workspace(int64_t M, int64_t K, int64_t N, int rank, int64_t R, bool backward) {
-  return M == 0 ? 0 : lr_space(M, K, N, rank, R, backward).total;
+  return M == 0 ? 0 : lr_space(M, K, N, rank, backward).total;
 }
-// CTAs of a cluster that share a tile's contraction: as many as fill the SMs twice, at most a fourth of the steps
-static int lr_splits(int64_t tiles, int64_t C) {
-  const int64_t chunks = (C + 63) / 64;
-  int s = 1;
-  while (s < 8 && tiles * s < 2 * cross_sms() && chunks >= 8 * s) s *= 2;
-  return s;
+// How many CTAs share a tile's steps, 1, 2, 4 or 8: the fewest rounds of resident CTAs times the steps that each takes, with what a
+// CTA's start and end cost (`extra` steps).
+static int64_t lr_cost(int64_t tiles, int64_t steps, int64_t parts, int64_t slots, int64_t extra) {
+  return ((tiles * parts + slots - 1) / slots) * ((steps + parts - 1) / parts + extra);
+}
+static int lr_splits(int64_t tiles, int64_t chunks, int ctas) {
+  const int64_t slots = static_cast<int64_t>(ctas) * cross_sms();
+  int best = 1;
+  for (int n = 2; n <= 8; n *= 2)
+    if (lr_cost(tiles, chunks, n, slots, 6) < lr_cost(tiles, chunks, best, slots, 6)) best = n;
+  return best;
 }
 template <typename... KA, typename... A>
 static int lr_launch(const char* what, void (*kernel)(KA...), std::atomic<bool> (&ready)[CA_DEVICES], dim3 grid, int threads, int smem,
@@ -855,44 +856,40 @@ static int lr_launch(const char* what, void (*kernel)(KA...), std::atomic<bool> 
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<KA>(args)...);
   return e == cudaSuccess ? check_launch(what) : cuda_fail(e, what);
 }
-template <typename T, bool W_ROWS, int STAGES>
-static int lr_shrink_s(const LrPlan& p, const T* x, int64_t ldx, int64_t C, const T* w, int rank, int ldw, int rp, int R,
-                       const float* scales, const LrHidden& h, cudaStream_t st) {
+static bool lr_wide(const void* p, int64_t ld) { return !p || (ld % 16 == 0 && reinterpret_cast<uintptr_t>(p) % 32 == 0); }
+template <typename T, bool W_ROWS, int RPM>
+static int lr_shrink_s(const LrPlan& p, const T* x, int64_t ldx, int64_t C, const T* w, int rank, int rp, int R, const float* scales,
+                       const LrHidden& h, cudaStream_t st) {
+  using Cfg = LrShrinkCfg<RPM>;
   static std::atomic<bool> ready[CA_DEVICES];
-  const int splits = lr_splits(p.n_tiles, C);
-  return lr_launch("lr_shrink_kernel", lr_shrink_kernel<T, W_ROWS, STAGES>, ready, dim3(static_cast<unsigned>(p.n_tiles * splits)),
-                   LR_SHRINK_THREADS, LrShrinkCfg<STAGES>::SMEM, splits, st, p, x, ldx, C, w, rank, ldw, rp, R, scales, h, splits);
+  const int splits = lr_splits(p.n_tiles, (C + 63) / 64, Cfg::CTAS);
+  return lr_launch("lr_shrink_kernel", lr_shrink_kernel<T, W_ROWS, RPM>, ready, dim3(static_cast<unsigned>(p.n_tiles * splits)),
+                   LR_SHRINK_THREADS, Cfg::SMEM, splits, st, p, x, ldx, C, w, rank, rp, R, scales, h, splits);
 }
 template <typename T, bool W_ROWS>
-static int lr_shrink(const LrPlan& p, const T* x, int64_t ldx, int64_t C, const T* w, int rank, int ldw, int R, const float* scales,
+static int lr_shrink(const LrPlan& p, const T* x, int64_t ldx, int64_t C, const T* w, int rank, int R, const float* scales,
                      const LrHidden& h, cudaStream_t st) {
   const int rp = lr_rp(rank);
-  if constexpr (W_ROWS)
-    if (rp <= 32) return lr_shrink_s<T, W_ROWS, 5>(p, x, ldx, C, w, rank, ldw, rp, R, scales, h, st);
-  if (rp <= 64) return lr_shrink_s<T, W_ROWS, 4>(p, x, ldx, C, w, rank, ldw, rp, R, scales, h, st);
-  return lr_shrink_s<T, W_ROWS, 3>(p, x, ldx, C, w, rank, ldw, rp, R, scales, h, st);
+  if (rp <= 64) return lr_shrink_s<T, W_ROWS, 64>(p, x, ldx, C, w, rank, rp, R, scales, h, st);
+  return lr_shrink_s<T, W_ROWS, 128>(p, x, ldx, C, w, rank, rp, R, scales, h, st);
 }
-template <typename T, bool W_ROWS, int RPM>
-static int lr_expand_s(const LrPlan& p, const LrHidden& h, const T* w, int rank, int ldw, int rp, int R, const T* base, int64_t ldb, T* out,
+template <typename T, bool W_ROWS, int NQ>
+static int lr_expand_s(const LrPlan& p, const LrHidden& h, const T* w, int rank, int rp, int R, const T* base, int64_t ldb, T* out,
                        int64_t ldo, int64_t N, cudaStream_t st) {
+  using Cfg = LrExpandCfg<NQ, W_ROWS>;
   static std::atomic<bool> ready[CA_DEVICES];
-  const int64_t steps = (N + LR_NT - 1) / LR_NT;
-  // eight CTAs to an SM in all, of two steps at least (a CTA's start costs about as much as one)
-  int64_t per = p.n_tiles * steps / (8 * cross_sms());
-  per = per < 2 ? 2 : per > 16 ? 16 : per;
-  const int parts = static_cast<int>((steps + per - 1) / per);
-  const bool wide = ldo % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 32 == 0 &&
-                    (!base || (ldb % 16 == 0 && reinterpret_cast<uintptr_t>(base) % 32 == 0));
-  return lr_launch("lr_expand_kernel", lr_expand_kernel<T, W_ROWS, RPM>, ready,
-                   dim3(static_cast<unsigned>(p.n_tiles * parts)), LR_EXPAND_THREADS, LrExpandCfg<RPM>::SMEM, 1, st, p, h, w, rank, ldw,
-                   rp, R, base, ldb, out, ldo, N, static_cast<int>(per), parts, wide);
+  const int parts = static_cast<int>((N + Cfg::COLS - 1) / Cfg::COLS);
+  return lr_launch("lr_expand_kernel", lr_expand_kernel<T, W_ROWS, NQ>, ready, dim3(static_cast<unsigned>(p.n_tiles * parts)), LR_THREADS,
+                   Cfg::SMEM, 1, st, p, h, w, rank, rp, R, base, ldb, out, ldo, N, parts, lr_wide(base, ldb) && lr_wide(out, ldo));
 }
 template <typename T, bool W_ROWS>
-static int lr_expand(const LrPlan& p, const LrHidden& h, const T* w, int rank, int ldw, int R, const T* base, int64_t ldb, T* out, int64_t ldo,
+static int lr_expand(const LrPlan& p, const LrHidden& h, const T* w, int rank, int R, const T* base, int64_t ldb, T* out, int64_t ldo,
                      int64_t N, cudaStream_t st) {
   const int rp = lr_rp(rank);
-  if (rp <= 64) return lr_expand_s<T, W_ROWS, 64>(p, h, w, rank, ldw, rp, R, base, ldb, out, ldo, N, st);
-  return lr_expand_s<T, W_ROWS, 128>(p, h, w, rank, ldw, rp, R, base, ldb, out, ldo, N, st);
+  if (rp <= 16) return lr_expand_s<T, W_ROWS, 1>(p, h, w, rank, rp, R, base, ldb, out, ldo, N, st);
+  if (rp <= 32) return lr_expand_s<T, W_ROWS, 2>(p, h, w, rank, rp, R, base, ldb, out, ldo, N, st);
+  if (rp <= 64) return lr_expand_s<T, W_ROWS, 4>(p, h, w, rank, rp, R, base, ldb, out, ldo, N, st);
+  return lr_expand_s<T, W_ROWS, 8>(p, h, w, rank, rp, R, base, ldb, out, ldo, N, st);
 }
 template <typename T, int RPM>
 static int lr_wgrad(const LrPlan& p, const LrWgradSide<T>& a, const LrWgradSide<T>& b, int rank, int R, cudaStream_t st) {
@@ -902,45 +899,31 @@ static int lr_wgrad(const LrPlan& p, const LrWgradSide<T>& a, const LrWgradSide<
   if (int rc = lr_launch("lr_wgrad_kernel", lr_wgrad_kernel<T, RPM>, ready, dim3(static_cast<unsigned>(grid)), 160, LrWgradCfg<RPM>::SMEM,
                          1, st, p, a, b, rank, rp, R))
     return rc;
-  const int ja = static_cast<int>((a.blocks ? a.C + 31 : 0) / 32), jb = static_cast<int>((b.blocks ? b.C + 31 : 0) / 32);
+  const int chans = 1024 / rp;
+  const int ja = static_cast<int>((a.blocks ? a.C + chans - 1 : 0) / chans), jb = static_cast<int>((b.blocks ? b.C + chans - 1 : 0) / chans);
   return lr_launch("lr_join_kernel", lr_join_kernel<T>, joined, dim3(ja + jb, R), 256, 0, 1, st, p, a, b, ja, rank, rp);
 }
 template <typename T>
-static int lr_pad(const LrArgs& a, const LrSpace& s, const T*& b, cudaStream_t st) {
-  if (a.rank % 8 == 0) return H3B_OK;
-  T* to = reinterpret_cast<T*>(static_cast<char*>(a.ws) + s.pad);
-  const int64_t rows = a.R * a.N, blocks = (rows * lr_ldw(a.rank) + 1023) / 1024, cap = 8ll * cross_sms();
-  lr_pad_kernel<T><<<static_cast<unsigned>(blocks < cap ? blocks : cap), 256, 0, st>>>(b, to, rows, a.rank, lr_ldw(a.rank));
-  b = to;
-  return check_launch("lr_pad_kernel");
-}
-
-template <typename T>
 static int lr_forward_t(const LrArgs& a, cudaStream_t st) {
   const LrPlan p = lr_plan(a.plan, a.M, a.R);
-  const LrSpace s = lr_space(a.M, a.K, a.N, a.rank, a.R, false);
   const LrHidden h = lr_hidden(a.hidden ? a.hidden : a.ws, a.M, a.rank);
   const int R = static_cast<int>(a.R);
-  const T* b = static_cast<const T*>(a.b);
-  if (int rc = lr_pad<T>(a, s, b, st)) return rc;
-  if (int rc = lr_shrink<T, true>(p, static_cast<const T*>(a.x), a.ldx, a.K, static_cast<const T*>(a.a), a.rank, 0, R, a.scales, h, st))
+  if (int rc = lr_shrink<T, true>(p, static_cast<const T*>(a.x), a.ldx, a.K, static_cast<const T*>(a.a), a.rank, R, a.scales, h, st))
     return rc;
-  return lr_expand<T, true>(p, h, b, a.rank, lr_ldw(a.rank), R, static_cast<const T*>(a.base), a.ldbase, static_cast<T*>(a.out), a.ldo,
-                            a.N, st);
+  return lr_expand<T, true>(p, h, static_cast<const T*>(a.b), a.rank, R, static_cast<const T*>(a.base), a.ldbase, static_cast<T*>(a.out),
+                            a.ldo, a.N, st);
 }
 template <typename T>
 static int lr_backward_t(const LrArgs& a, cudaStream_t st) {
   const LrPlan p = lr_plan(a.plan, a.M, a.R);
-  const LrSpace s = lr_space(a.M, a.K, a.N, a.rank, a.R, true);
+  const LrSpace s = lr_space(a.M, a.K, a.N, a.rank, true);
   const LrHidden h = lr_hidden(a.hidden, a.M, a.rank), dh = lr_hidden(a.ws, a.M, a.rank);
   const int R = static_cast<int>(a.R);
-  const T *x = static_cast<const T*>(a.x), *go = static_cast<const T*>(a.go), *b = static_cast<const T*>(a.b);
-  if (a.dx || a.da) {
-    if (int rc = lr_pad<T>(a, s, b, st)) return rc;
-    if (int rc = lr_shrink<T, false>(p, go, a.ldgo, a.N, b, a.rank, lr_ldw(a.rank), R, a.scales, dh, st)) return rc;
-  }
+  const T *x = static_cast<const T*>(a.x), *go = static_cast<const T*>(a.go);
+  if (a.dx || a.da)
+    if (int rc = lr_shrink<T, false>(p, go, a.ldgo, a.N, static_cast<const T*>(a.b), a.rank, R, a.scales, dh, st)) return rc;
   if (a.dx)
-    if (int rc = lr_expand<T, false>(p, dh, static_cast<const T*>(a.a), a.rank, 0, R, nullptr, 0, static_cast<T*>(a.dx), a.lddx, a.K, st))
+    if (int rc = lr_expand<T, false>(p, dh, static_cast<const T*>(a.a), a.rank, R, nullptr, 0, static_cast<T*>(a.dx), a.lddx, a.K, st))
       return rc;
   if (!a.da && !a.db) return H3B_OK;
   char* ws = static_cast<char*>(a.ws);
