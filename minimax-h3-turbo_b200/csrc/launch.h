@@ -2,12 +2,11 @@
 // C ABI (libh3b.cu), the small argument structs they share, and the per-unit device failure flags.
 //
 // Translation units (compiled in parallel, linked into one library without relocatable device code):
-//   k_act.cu      rotate + quantise (rotq.cuh), RMSNorm + modulation (rmsmod.cuh), q/k norm + RoPE (rope.cuh),
-//                 attention merge (attn_merge.cuh)
+//   k_act.cu      rotate + quantise (rotq.cuh), RMSNorm + modulation (rmsmod.cuh), the residual's addition with its norm
+//                 and 8-bit output (resnorm.cuh), q/k norm + RoPE (rope.cuh), attention merge (attn_merge.cuh)
 //   k_rope_axes.cu  rotary embedding from positions on several axes (rope_axes.cuh)
 //   k_cross.cu    cross attention and its gradients (cross_attn.cuh)
 //   k_lowrank.cu  low-rank adapters beside a shared projection, and their gradients (lowrank.cuh)
-//   k_resnorm.cu  the residual's addition with its norm and 8-bit output, and their gradients (resnorm.cuh)
 //   k_decode.cu   int4 -> int8 grid decode (decode.cuh)
 //   k_gemm.cu     int8 GEMM + epilogue, 1-CTA and CTA-pair kernels (gemm_sm100.cuh)
 //   k_w4.cu       dispatch of the decode-in-producer W4A8 GEMM for few M tiles (gemm_w4.cuh), instantiated per group
@@ -65,6 +64,23 @@ int qk_norm_rope_launch(void* q, int64_t ldq, void* k, int64_t ldk, int x_dtype,
 int attn_merge_launch(float* acc, float* acc_lse, const void* o, int64_t o_sh, int64_t o_sq, const float* lse, int64_t H,
                       int64_t Q, int D, int first, void* out, int64_t ldo, cudaStream_t st);
 
+// of h3b_residual_norm and h3b_residual_norm_backward
+struct ResNormArgs {  // of h3b_residual_norm and h3b_residual_norm_backward
+  const void *x, *y, *w, *gate, *shift, *scale, *dt, *dh;
+  void *t, *h, *dx, *dy, *dw;
+  int8_t* codes;
+  float *scales, *rstd;
+  int64_t ldx, ldy, ldm, ldt, ldh, ldc, lddt, lddh, lddx, lddy, M;
+  int K, dtype, w_dtype, m_dtype;
+  float eps;
+  const int* token_rows;  // modulation row of each token (outside 0 .. n_rows - 1: none), or null: the segments decide
+  int n_rows;
+  SegTable segs;
+  void* ws;
+};
+size_t resnorm_workspace(int64_t M, int K, bool backward);
+int resnorm_launch(const ResNormArgs& a, bool backward, cudaStream_t st);
+
 // ---- k_rope_axes.cu
 int rope_axes_launch(const h3b_rope_operand* q, const h3b_rope_operand* k, int x_dtype, int64_t B, int D,
                      const float* inv_freq, const int32_t* sections, int axes, int pos_dtype, int pairing, int inverse,
@@ -95,23 +111,6 @@ size_t lr_hidden_bytes(int64_t M, int rank);
 size_t lr_workspace(int64_t M, int64_t K, int64_t N, int rank, int64_t R, bool backward);
 int lr_forward(const LrArgs& a, cudaStream_t st);
 int lr_backward(const LrArgs& a, cudaStream_t st);
-
-// ---- k_resnorm.cu
-struct ResNormArgs {  // of h3b_residual_norm and h3b_residual_norm_backward
-  const void *x, *y, *w, *gate, *shift, *scale, *dt, *dh;
-  void *t, *h, *dx, *dy, *dw;
-  int8_t* codes;
-  float *scales, *rstd;
-  int64_t ldx, ldy, ldm, ldt, ldh, ldc, lddt, lddh, lddx, lddy, M;
-  int K, dtype, w_dtype, m_dtype;
-  float eps;
-  const int* token_rows;  // modulation row of each token (outside 0 .. n_rows - 1: none), or null: the segments decide
-  int n_rows;
-  SegTable segs;
-  void* ws;
-};
-size_t resnorm_workspace(int64_t M, int K, bool backward);
-int resnorm_launch(const ResNormArgs& a, bool backward, cudaStream_t st);
 
 // ---- k_decode.cu
 int decode_launch(const void* q4, int64_t N, int64_t K, int64_t ldq4, const void* s_rel, int s_dtype, int64_t lds,

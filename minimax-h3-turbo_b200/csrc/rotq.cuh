@@ -31,6 +31,7 @@
 // quotient goes straight to integers (cvt.rni.s32.bf16, half-to-even) and a saturating byte pack (cvt.pack.sat.s8);
 // fp16 and fp32: the fp32 magic constant 1.5 * 2^23 rounds half-to-even after a clamp in the dt domain, and the code is
 // the low byte of the sum's bit pattern.
+#pragma once
 #include <mutex>
 #include <type_traits>
 
