@@ -9,65 +9,46 @@
 // gate t = x + y everywhere.
 //
 // HBM-bound: x and y are read and t and the codes written once, 7 bytes a channel (9 with h; the gradients 8 or 10).  A thread has 16
-// channels of a row, so that a row stays in registers from its first load to its codes: the rotation's four butterfly digits are two in
-// registers and two over the 16 threads of a block (through shared memory, as in rotq.cuh).  Two rows go through the butterflies at
-// once, as the halves of packed fp32 instructions.  CTAs are persistent, and the next rows are on their way while these are worked on.
-// w, gate, scale and shift come from L1 every time: 4 bytes a channel and pair of rows.
+// channels of two rows (or 16 and 16 of one row, SPLIT, where a row is long), the halves of packed fp32 instructions, from their
+// arrival to their codes: the rotation's four butterfly digits are two in registers and two over the 16 threads of a block (through
+// shared memory, as in rotq.cuh).  CTAs are persistent; while rows are worked on, the next ones come into shared memory as bulk copies
+// of whole rows (held in registers instead, they left room for 10 warps to an SM: 763 us for 59440 x 5120 into codes).  w, gate,
+// scale and shift come from L1 every time: 4 bytes a channel and pair of rows.
 #pragma once
 #include "rotq.cuh"
 
 namespace h3b {
 
-constexpr int RN_AHEAD = 512;  // up to so many threads to a row the next rows' numbers fit in registers
-
 template <int DT>
-__device__ __forceinline__ void rn_unpack(const uint32_t (&w)[8], float (&f)[16]) {
+__device__ __forceinline__ void rn_unpack(const uint4& u, float (&f)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 4; ++i) {
     const float2 v = unpack2<DT>(w[i]);
     f[2 * i] = v.x, f[2 * i + 1] = v.y;
   }
 }
-// 16 numbers of 16 bits from p on, `left` of them there (a multiple of 8, also negative); wide: p on a 32-byte boundary
-__device__ __forceinline__ void rn_load(const void* p, int left, bool wide, uint32_t (&v)[8]) {
-  if (wide && left >= 16) {
-    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
-                 : "l"(p)
-                 : "memory");
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    uint4 u = make_uint4(0, 0, 0, 0);
-    if (left > 8 * i) u = reinterpret_cast<const uint4*>(p)[i];
-    v[4 * i] = u.x, v[4 * i + 1] = u.y, v[4 * i + 2] = u.z, v[4 * i + 3] = u.w;
-  }
+template <int DT>
+__device__ __forceinline__ uint4 rn_pack(const float (&f)[8]) {
+  return make_uint4(pack2<DT>(make_float2(f[0], f[1])), pack2<DT>(make_float2(f[2], f[3])), pack2<DT>(make_float2(f[4], f[5])),
+                    pack2<DT>(make_float2(f[6], f[7])));
 }
-__device__ __forceinline__ void rn_store(void* p, int left, bool wide, const uint32_t (&v)[8]) {
-  if (wide && left >= 16) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
-                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-                 : "memory");
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    if (left > 8 * i) reinterpret_cast<uint4*>(p)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+__device__ __forceinline__ uint4 rn_load(const unsigned char* p, bool ok) {
+  return ok ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
 }
-// 16 numbers of the weight or of a modulation row, of the stream's type (FAST) or of any
+__device__ __forceinline__ void rn_bulk(void* dst, const void* src, int bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+// 8 numbers of the weight or of a modulation row, of the stream's type (FAST) or of any
 template <int DT, bool FAST>
-__device__ __forceinline__ void rn_param(const void* p, int64_t at, int dt, int left, float (&f)[16]) {
+__device__ __forceinline__ void rn_param(const void* p, int64_t at, int dt, bool ok, float (&f)[8]) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (left > 8 * i) {
-      if constexpr (FAST) load8(p, at + 8 * i, DT == DT_BF16 ? H3B_BF16 : H3B_FP16, v);
-      else load8(p, at + 8 * i, dt, v);
-    }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) f[8 * i + k] = v[k];
-  }
+  for (int i = 0; i < 8; ++i) f[i] = 0.f;
+  if (!ok) return;
+  if constexpr (FAST) load8(p, at, DT == DT_BF16 ? H3B_BF16 : H3B_FP16, f);
+  else load8(p, at, dt, f);
 }
 __device__ __forceinline__ int rn_mod_row(const ResNormArgs& a, int64_t r) {
   int m = -1;
@@ -95,102 +76,133 @@ __device__ __forceinline__ float2 rn_sum(float2 v, float2* part, int mine, int f
   return s;
 }
 
-// blockDim = G groups of T = K / 16 threads, rounded up to whole warps; a group has two rows at a time.
-template <int DT, bool CODES, bool FAST, bool AHEAD>
-__global__ void __launch_bounds__(AHEAD ? RN_AHEAD : 1024) resnorm_kernel(const ResNormArgs a, int T, int G, bool wide) {
-  extern __shared__ __align__(16) unsigned char rn_smem[];
-  const int tid = threadIdx.x, unit = tid / T, tr = tid - unit * T, col = 16 * tr, left = unit < G ? a.K - col : 0;
-  const int half = tid >> 4, halves = blockDim.x >> 4, t16 = tid & 15, first = unit < G ? unit * (T >> 4) : 0, parts = unit < G ? T >> 4 : 0;
-  float2* const part = reinterpret_cast<float2*>(rn_smem);
+// What a launch is made of: groups of T threads, G to a CTA (rounded up to whole warps); a group has two rows, or one (SPLIT: its lanes'
+// columns are `off` apart, half the row rounded up to whole blocks of 256, so that both are at the same place of theirs).
+struct RnShape {
+  int T, G, threads, blocks, off, smem, ahead;
+  bool split;
+};
+constexpr int RN_PAIR = 384;  // threads that a pair of rows has at most
+// Shared memory: barrier and abort flag (32 bytes), the groups' sums, their rows, the rotation's exchange
+__host__ __device__ inline int rn_rows_at(int threads) { return 32 + threads; }  // threads / 16 half-warps x (8 + 8) bytes
+__host__ __device__ inline int rn_group_bytes(int K, bool split) { return (split ? 2 : 4) * 2 * K; }
+
+template <int DT, bool CODES, bool FAST, bool SPLIT>
+__global__ void __launch_bounds__(SPLIT ? 512 : RN_PAIR, SPLIT ? 1 : 2) resnorm_kernel(const ResNormArgs a, const RnShape s) {
+  extern __shared__ __align__(128) unsigned char rn_smem[];
+  const int tid = threadIdx.x, T = s.T, G = s.G, unit = tid / T, tr = tid - unit * T, K = a.K;
+  const int half = tid >> 4, halves = blockDim.x >> 4, t16 = tid & 15, parts = unit < G ? T >> 4 : 0, first = unit * parts;
+  const int col[2] = {16 * tr, 16 * tr + (SPLIT ? s.off : 0)};
+  uint64_t* const bar = reinterpret_cast<uint64_t*>(rn_smem);
+  volatile int* const abort = reinterpret_cast<volatile int*>(rn_smem + 8);
+  float2* const part = reinterpret_cast<float2*>(rn_smem + 32);
   uint2* const tops = reinterpret_cast<uint2*>(part + halves);
-  float2* const gbuf = reinterpret_cast<float2*>(rn_smem + ((16 * halves + 15) & ~15)) + half * xgrp(16);
-  const int64_t pairs = (a.M + 1) / 2, step = static_cast<int64_t>(gridDim.x) * G;
-  int64_t r0 = 2 * (static_cast<int64_t>(blockIdx.x) * G + unit);
+  unsigned char* const mine = rn_smem + rn_rows_at(blockDim.x) + (unit < G ? unit : 0) * rn_group_bytes(K, SPLIT);
+  float2* const gbuf = reinterpret_cast<float2*>(rn_smem + rn_rows_at(blockDim.x) + G * rn_group_bytes(K, SPLIT)) + half * xgrp(16);
+  constexpr int ROWS = SPLIT ? 1 : 2;
+  const int64_t groups = (a.M + ROWS - 1) / ROWS, step = static_cast<int64_t>(gridDim.x) * G;
+  int64_t r0 = ROWS * (static_cast<int64_t>(blockIdx.x) * G + unit);
   if (unit >= G) r0 = a.M;  // threads behind the last group: no rows, but every barrier
-  const float over_k = 1.f / static_cast<float>(a.K);
-  uint32_t xs[2][8], ys[2][8];
-  auto load = [&](int64_t r) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int n = r + h < a.M ? left : 0;
-      rn_load(rn_at(a.x, r + h, a.ldx, col), n, wide, xs[h]);
-      rn_load(rn_at(a.y, r + h, a.ldy, col), n, wide, ys[h]);
-    }
+  if (tid == 0) {
+    mbar_init(bar, G);
+    mbar_fence_init();
+    *abort = 0;
+  }
+  __syncthreads();
+  auto bring = [&](int64_t r) {  // by a group's first thread
+    int n = 0;
+    for (int h = 0; h < ROWS; ++h) n += r + h < a.M ? 4 * K : 0;
+    mbar_arrive_expect_tx(bar, n);
+    for (int h = 0; h < ROWS; ++h)
+      if (r + h < a.M) {
+        rn_bulk(mine + h * 4 * K, rn_at(a.x, r + h, a.ldx, 0), 2 * K, bar);
+        rn_bulk(mine + h * 4 * K + 2 * K, rn_at(a.y, r + h, a.ldy, 0), 2 * K, bar);
+      }
   };
-  if (AHEAD) load(r0);
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * G; base < pairs; base += step, r0 += 2 * step) {
-    if (!AHEAD) load(r0);
-    const int n[2] = {r0 < a.M ? left : 0, r0 + 1 < a.M ? left : 0};
-    const int mrow[2] = {rn_mod_row(a, r0), rn_mod_row(a, r0 + 1)};
-    const bool same = mrow[0] == mrow[1];
+  const bool leads = tr == 0 && unit < G;
+  if (leads) bring(r0);
+  const float over_k = 1.f / static_cast<float>(K);
+  uint32_t turn = 0;
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * G; base < groups; base += step, r0 += ROWS * step, turn ^= 1) {
+    const int64_t row[2] = {r0, r0 + ROWS - 1};
+    const int n[2] = {row[0] < a.M ? K - col[0] : 0, row[1] < a.M ? K - col[1] : 0};
+    const int mrow[2] = {rn_mod_row(a, row[0]), SPLIT ? rn_mod_row(a, row[0]) : rn_mod_row(a, row[1])};
+    const bool same = !SPLIT && mrow[0] == mrow[1];  // one load of a modulation row serves both lanes
+    mbar_wait(bar, turn, abort);
     // ---- the stream
     float2 v[16], ss = make_float2(0.f, 0.f);
-    float p[16];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float f[16], y[16];
-      rn_unpack<DT>(xs[h], f);
-      rn_unpack<DT>(ys[h], y);
-      if (a.gate) {
-        if (mrow[h] >= 0) {
-          if (h == 0 || !same) rn_param<DT, FAST>(a.gate, mrow[h] * a.ldm + col, a.m_dtype, left, p);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) f[i] = __fadd_rn(f[i], __fmul_rn(y[i], p[i]));
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) f[i] = __fadd_rn(f[i], y[i]);
-      }
-      uint32_t t[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) t[i] = pack2<DT>(make_float2(f[2 * i], f[2 * i + 1]));
-      rn_store(rn_at(a.t, r0 + h, a.ldt, col), n[h], wide, t);
-      rn_unpack<DT>(t, f);
-      float s = 0.f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s = fmaf(f[i], f[i], s);
-        if (h == 0) v[i].x = f[i];
-        else v[i].y = f[i];
-      }
-      if (h == 0) ss.x = s;
-      else ss.y = s;
-    }
-    if (AHEAD && base + step < pairs) load(r0 + 2 * step);
-    ss = rn_sum(ss, part, half, first, parts);
-    const float2 rs = make_float2(rsqrtf(fmaf(ss.x, over_k, a.eps)), rsqrtf(fmaf(ss.y, over_k, a.eps)));
-    if (a.rstd && tr == 0) {
-      if (r0 < a.M) a.rstd[r0] = rs.x;
-      if (r0 + 1 < a.M) a.rstd[r0 + 1] = rs.y;
-    }
-    // ---- the norm and its modulation
-    rn_param<DT, FAST>(a.w, col, a.w_dtype, left, p);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = __fmul2_rn(__fmul2_rn(v[i], rs), make_float2(p[i], p[i]));
-    if (a.scale) {
-      float q[16];
+    for (int k = 0; k < 2; ++k) {  // 8 channels at a time
+      float p[8];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if (mrow[h] < 0) continue;
-        if (h == 0 || !same) {
-          rn_param<DT, FAST>(a.scale, mrow[h] * a.ldm + col, a.m_dtype, left, p);
-          rn_param<DT, FAST>(a.shift, mrow[h] * a.ldm + col, a.m_dtype, left, q);
-        }
+        float f[8], y[8];
+        const bool ok = n[h] > 8 * k;
+        const int c = col[h] + 8 * k;
+        const unsigned char* at = mine + (SPLIT ? 0 : h) * 4 * K + 2 * c;
+        rn_unpack<DT>(rn_load(at, ok), f);
+        rn_unpack<DT>(rn_load(at + 2 * K, ok), y);
+        if (a.gate) {
+          if (mrow[h] >= 0) {
+            if (h == 0 || !same) rn_param<DT, FAST>(a.gate, mrow[h] * a.ldm + c, a.m_dtype, ok, p);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          if (h == 0) v[i].x = fmaf(v[i].x, 1.f + p[i], q[i]);
-          else v[i].y = fmaf(v[i].y, 1.f + p[i], q[i]);
+            for (int i = 0; i < 8; ++i) f[i] = __fadd_rn(f[i], __fmul_rn(y[i], p[i]));
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] = __fadd_rn(f[i], y[i]);
+        }
+        const uint4 t = rn_pack<DT>(f);
+        if (ok) *reinterpret_cast<uint4*>(rn_at(a.t, row[h], a.ldt, c)) = t;
+        rn_unpack<DT>(t, f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (h == 0) ss.x = fmaf(f[i], f[i], ss.x), v[8 * k + i].x = f[i];
+          else ss.y = fmaf(f[i], f[i], ss.y), v[8 * k + i].y = f[i];
         }
       }
     }
-    if (a.h) {
-      uint32_t o[8];
+    if (SPLIT) ss.x = ss.y = ss.x + ss.y;
+    ss = rn_sum(ss, part, half, first, parts);
+    // everyone has read the rows: the next ones may come
+    if (leads && base + step < groups) bring(r0 + ROWS * step);
+    const float2 rs = make_float2(rsqrtf(fmaf(ss.x, over_k, a.eps)), rsqrtf(fmaf(ss.y, over_k, a.eps)));
+    if (a.rstd && leads) {
+      if (row[0] < a.M) a.rstd[row[0]] = rs.x;
+      if (!SPLIT && row[1] < a.M) a.rstd[row[1]] = rs.y;
+    }
+    // ---- the norm and its modulation
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] = pack2<DT>(make_float2(v[2 * i].x, v[2 * i + 1].x));
-      rn_store(rn_at(a.h, r0, a.ldh, col), n[0], wide, o);
+    for (int k = 0; k < 2; ++k) {
+      float p[8], q[8];
+      rn_param<DT, FAST>(a.w, col[0] + 8 * k, a.w_dtype, unit < G && K - col[0] > 8 * k, p);
+      if (SPLIT) rn_param<DT, FAST>(a.w, col[1] + 8 * k, a.w_dtype, unit < G && K - col[1] > 8 * k, q);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] = pack2<DT>(make_float2(v[2 * i].y, v[2 * i + 1].y));
-      rn_store(rn_at(a.h, r0 + 1, a.ldh, col), n[1], wide, o);
+      for (int i = 0; i < 8; ++i)
+        v[8 * k + i] = __fmul2_rn(__fmul2_rn(v[8 * k + i], rs), make_float2(p[i], SPLIT ? q[i] : p[i]));
+      if (a.scale) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (mrow[h] < 0) continue;
+          if (h == 0 || !same) {
+            rn_param<DT, FAST>(a.scale, mrow[h] * a.ldm + col[h] + 8 * k, a.m_dtype, n[h] > 8 * k, p);
+            rn_param<DT, FAST>(a.shift, mrow[h] * a.ldm + col[h] + 8 * k, a.m_dtype, n[h] > 8 * k, q);
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (h == 0) v[8 * k + i].x = fmaf(v[8 * k + i].x, 1.f + p[i], q[i]);
+            else v[8 * k + i].y = fmaf(v[8 * k + i].y, 1.f + p[i], q[i]);
+          }
+        }
+      }
+      if (a.h) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) p[i] = h == 0 ? v[8 * k + i].x : v[8 * k + i].y;
+          if (n[h] > 8 * k) *reinterpret_cast<uint4*>(rn_at(a.h, row[h], a.ldh, col[h] + 8 * k)) = rn_pack<DT>(p);
+        }
+      }
     }
     if constexpr (CODES) {
       // ---- the rotation: digits d0, d1 in registers, d2, d3 over the block's 16 threads
@@ -216,19 +228,21 @@ __global__ void __launch_bounds__(AHEAD ? RN_AHEAD : 1024) resnorm_kernel(const 
         top.x = max(top.x, __float_as_uint(v[i].x) & 0x7FFFFFFFu);
         top.y = max(top.y, __float_as_uint(v[i].y) & 0x7FFFFFFFu);
       }
+      if (SPLIT) top.x = top.y = max(top.x, top.y);
 #pragma unroll
       for (int o = 8; o; o >>= 1) {
         top.x = max(top.x, __shfl_xor_sync(0xffffffffu, top.x, o));
-        top.y = max(top.y, __shfl_xor_sync(0xffffffffu, top.y, o));
+        if (!SPLIT) top.y = max(top.y, __shfl_xor_sync(0xffffffffu, top.y, o));
       }
       if (t16 == 0) tops[half] = top;
       __syncthreads();
 #pragma unroll 4
       for (int i = 0; i < parts; ++i) top.x = max(top.x, tops[first + i].x), top.y = max(top.y, tops[first + i].y);
+      if (SPLIT) top.y = top.x;
       const float2 amax = make_float2(__uint_as_float(top.x), __uint_as_float(top.y));
-      if (tr == 0) {
-        if (r0 < a.M) a.scales[r0] = __fdiv_rn(amax.x, 127.f);
-        if (r0 + 1 < a.M) a.scales[r0 + 1] = __fdiv_rn(amax.y, 127.f);
+      if (leads) {
+        if (row[0] < a.M) a.scales[row[0]] = __fdiv_rn(amax.x, 127.f);
+        if (!SPLIT && row[1] < a.M) a.scales[row[1]] = __fdiv_rn(amax.y, 127.f);
       }
       // ---- codes: 0 for rows of zeros and rows without a finite largest magnitude
       const float2 inv = make_float2(amax.x > 0.f && amax.x < INFINITY ? fminf(__fdiv_rn(127.f, amax.x), 3e38f) : 0.f,
@@ -256,91 +270,134 @@ __global__ void __launch_bounds__(AHEAD ? RN_AHEAD : 1024) resnorm_kernel(const 
       __syncwarp();
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        if (n[h] > 0) *reinterpret_cast<uint4*>(a.codes + (r0 + h) * a.ldc + col) = make_uint4(o[h][0], o[h][1], o[h][2], o[h][3]);
+        if (n[h] > 0) *reinterpret_cast<uint4*>(a.codes + row[h] * a.ldc + col[h]) = make_uint4(o[h][0], o[h][1], o[h][2], o[h][3]);
     } else {
       __syncthreads();  // the next rows' sums
     }
   }
 }
 
-// Gradients: a group has one row at a time; its threads keep their channels' part of dw over all its rows.
-template <int DT, bool FAST, bool AHEAD>
-__global__ void __launch_bounds__(AHEAD ? RN_AHEAD : 1024) resnorm_grad_kernel(const ResNormArgs a, int T, int G, bool wide, float* dw) {
-  extern __shared__ __align__(16) unsigned char rn_smem[];
-  const int tid = threadIdx.x, unit = tid / T, tr = tid - unit * T, col = 16 * tr, left = unit < G ? a.K - col : 0;
-  const int half = tid >> 4, halves = blockDim.x >> 4, first = unit < G ? unit * (T >> 4) : 0, parts = unit < G ? T >> 4 : 0;
-  float* const part = reinterpret_cast<float*>(rn_smem);  // two rows' sums in turn: one barrier a row
+// Gradients: a group has one row at a time, a thread 16 channels (or 16 and 16, SPLIT) of it; its part of dw over all its rows stays in
+// registers.  Rows come as bulk copies two rows ahead, into three buffers in turn (one ahead and two buffers where three do not fit).
+constexpr int RN_AHEAD = 3;
+template <int DT, bool FAST, bool SPLIT>
+__global__ void __launch_bounds__(SPLIT ? 512 : RN_PAIR, SPLIT ? 1 : 2) resnorm_grad_kernel(const ResNormArgs a, const RnShape s,
+                                                                                           float* dw) {
+  constexpr int L = SPLIT ? 2 : 1;
+  extern __shared__ __align__(128) unsigned char rn_smem[];
+  const int tid = threadIdx.x, T = s.T, G = s.G, unit = tid / T, tr = tid - unit * T, K = a.K;
+  const int half = tid >> 4, halves = blockDim.x >> 4, parts = unit < G ? T >> 4 : 0, first = unit * parts;
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(rn_smem);  // three
+  volatile int* const abort = reinterpret_cast<volatile int*>(rn_smem + 24);
+  float* const part = reinterpret_cast<float*>(rn_smem + 32);  // two rows' sums in turn: one barrier a row
+  const int bytes = (a.dt ? 6 : 4) * K;  // dh, t, dt
+  unsigned char* const mine = rn_smem + rn_rows_at(blockDim.x) + (unit < G ? unit : 0) * s.ahead * bytes;
   const int64_t step = static_cast<int64_t>(gridDim.x) * G;
   int64_t r = static_cast<int64_t>(blockIdx.x) * G + unit;
   if (unit >= G) r = a.M;
-  const float over_k = 1.f / static_cast<float>(a.K);
-  uint32_t td[8], hd[8], ts[8];
-  auto load = [&](int64_t row) {
-    const int n = row < a.M ? left : 0;
-    rn_load(rn_at(a.dh, row, a.lddh, col), n, wide, hd);
-    rn_load(rn_at(a.t, row, a.ldt, col), n, wide, ts);
-    rn_load(rn_at(a.dt, row, a.lddt, col), a.dt ? n : 0, wide, td);
+  if (tid == 0) {
+    for (int i = 0; i < RN_AHEAD; ++i) mbar_init(bars + i, G);
+    mbar_fence_init();
+    *abort = 0;
+  }
+  __syncthreads();
+  auto bring = [&](int64_t row, int i) {  // by a group's first thread, into buffer i
+    const bool ok = row < a.M;
+    mbar_arrive_expect_tx(bars + i, ok ? bytes : 0);
+    if (!ok) return;
+    unsigned char* const to = mine + i * bytes;
+    rn_bulk(to, rn_at(a.dh, row, a.lddh, 0), 2 * K, bars + i);
+    rn_bulk(to + 2 * K, rn_at(a.t, row, a.ldt, 0), 2 * K, bars + i);
+    if (a.dt) rn_bulk(to + 4 * K, rn_at(a.dt, row, a.lddt, 0), 2 * K, bars + i);
   };
-  float sum[16];
+  const bool leads = tr == 0 && unit < G;
+  const int64_t left = (a.M - static_cast<int64_t>(blockIdx.x) * G + step - 1) / step;  // rounds of this CTA
+  if (leads)
+    for (int i = 0; i < s.ahead - 1 && i < left; ++i) bring(r + i * step, i);
+  const float over_k = 1.f / static_cast<float>(K);
+  float sum[L][16];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) sum[i] = 0.f;
-  if (AHEAD) load(r);
-  int turn = 0;
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * G; base < a.M; base += step, r += step, turn ^= 1) {
-    if (!AHEAD) load(r);
-    const int n = r < a.M ? left : 0;
+  for (int l = 0; l < L; ++l)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum[l][i] = 0.f;
+  int buf = 0;
+  uint32_t phase = 0;
+  for (int64_t k = 0; k < left; ++k, r += step) {
     const int mrow = rn_mod_row(a, r);
     const float rs = r < a.M ? a.rstd[r] : 0.f;
-    float g[16], x[16], d[16], p[16];
-    rn_unpack<DT>(hd, g);
-    rn_unpack<DT>(ts, x);
-    rn_unpack<DT>(td, d);
-    if (AHEAD && base + step < a.M) load(r + step);
-    if (a.scale && mrow >= 0) {
-      rn_param<DT, FAST>(a.scale, mrow * a.ldm + col, a.m_dtype, left, p);
+    mbar_wait(bars + buf, phase, abort);
+    const unsigned char* const at = mine + buf * bytes;
+    float g[L][16], x[L][16], dot = 0.f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) g[i] *= 1.f + p[i];
-    }
-    rn_param<DT, FAST>(a.w, col, a.w_dtype, left, p);
-    float dot = 0.f;
+    for (int l = 0; l < L; ++l) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      x[i] *= rs;
-      sum[i] = fmaf(g[i], x[i], sum[i]);
-      g[i] *= p[i];
-      dot = fmaf(g[i], x[i], dot);
+      for (int k = 0; k < 2; ++k) {
+        const int col = 16 * tr + l * s.off + 8 * k;
+        const bool ok = r < a.M && col < K;
+        float p[8], f[8];
+        rn_unpack<DT>(rn_load(at + 2 * col, ok), f);
+        if (a.scale && mrow >= 0) {
+          rn_param<DT, FAST>(a.scale, mrow * a.ldm + col, a.m_dtype, ok, p);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] *= 1.f + p[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[l][8 * k + i] = f[i];
+        rn_unpack<DT>(rn_load(at + 2 * K + 2 * col, ok), f);
+        rn_param<DT, FAST>(a.w, col, a.w_dtype, ok, p);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int e = 8 * k + i;
+          x[l][e] = f[i] * rs;
+          sum[l][e] = fmaf(g[l][e], x[l][e], sum[l][e]);
+          g[l][e] *= p[i];
+          dot = fmaf(g[l][e], x[l][e], dot);
+        }
+      }
     }
 #pragma unroll
     for (int o = 8; o; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    if ((tid & 15) == 0) part[turn * halves + half] = dot;
+    float* const here = part + (k & 1) * halves;
+    if ((tid & 15) == 0) here[half] = dot;
     __syncthreads();
+    // everyone is through with the row before: its buffer is free
+    const int free = buf == 0 ? s.ahead - 1 : buf - 1;
+    if (leads && k + s.ahead - 1 < left) bring(r + (s.ahead - 1) * step, free);
     dot = 0.f;
 #pragma unroll 4
-    for (int i = 0; i < parts; ++i) dot += part[turn * halves + first + i];
+    for (int i = 0; i < parts; ++i) dot += here[first + i];
     dot *= over_k;
-    uint32_t o[8];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) d[i] = fmaf(rs, g[i] - x[i] * dot, d[i]);
+    for (int l = 0; l < L; ++l) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = pack2<DT>(make_float2(d[2 * i], d[2 * i + 1]));
-    rn_store(rn_at(a.dx, r, a.lddx, col), n, wide, o);
-    if (a.dy) {
-      if (mrow >= 0) {
-        rn_param<DT, FAST>(a.gate, mrow * a.ldm + col, a.m_dtype, left, p);
+      for (int k = 0; k < 2; ++k) {
+        const int col = 16 * tr + l * s.off + 8 * k;
+        const bool ok = r < a.M && col < K;
+        float d[8];
+        rn_unpack<DT>(rn_load(at + 4 * K + 2 * col, ok && a.dt), d);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = pack2<DT>(make_float2(d[2 * i] * p[2 * i], d[2 * i + 1] * p[2 * i + 1]));
-      } else {
+        for (int i = 0; i < 8; ++i) d[i] = fmaf(rs, g[l][8 * k + i] - x[l][8 * k + i] * dot, d[i]);
+        if (ok) *reinterpret_cast<uint4*>(rn_at(a.dx, r, a.lddx, col)) = rn_pack<DT>(d);
+        if (a.dy) {
+          float p[8];
+          rn_param<DT, FAST>(a.gate, mrow * a.ldm + col, a.m_dtype, ok && mrow >= 0, p);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = 0u;
+          for (int i = 0; i < 8; ++i) d[i] = mrow >= 0 ? d[i] * p[i] : 0.f;
+          if (ok) *reinterpret_cast<uint4*>(rn_at(a.dy, r, a.lddy, col)) = rn_pack<DT>(d);
+        }
       }
-      rn_store(rn_at(a.dy, r, a.lddy, col), n, wide, o);
     }
+    if (++buf == s.ahead) buf = 0, phase ^= 1;
   }
   if (dw && unit < G) {
-    float* to = dw + (static_cast<int64_t>(blockIdx.x) * G + unit) * a.K + col;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (left > 4 * i) *reinterpret_cast<float4*>(to + 4 * i) = make_float4(sum[4 * i], sum[4 * i + 1], sum[4 * i + 2], sum[4 * i + 3]);
+    for (int l = 0; l < L; ++l) {
+      const int col = 16 * tr + l * s.off;
+      float* to = dw + (static_cast<int64_t>(blockIdx.x) * G + unit) * K + col;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (K - col > 4 * i) *reinterpret_cast<float4*>(to + 4 * i) = make_float4(sum[l][4 * i], sum[l][4 * i + 1], sum[l][4 * i + 2], sum[l][4 * i + 3]);
+    }
   }
 }
 // dw: the groups' parts, eight stretches of them by a warp each, then these in order.  A CTA has 32 channels.
@@ -362,52 +419,57 @@ __global__ void __launch_bounds__(256) resnorm_dw_kernel(const float* part, int6
   else static_cast<__nv_bfloat16*>(dw)[c] = __float2bfloat16_rn(s);
 }
 
-// Groups of a CTA and CTAs of the launch.  CTAs of about 256 threads, as many to an SM as give it 1024 (768 from 257 threads on).
-struct RnShape {
-  int T, G, threads, blocks;
-};
 static int rn_sms() {
   int dev = 0, sms = 148;
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   return sms;
 }
-static RnShape rn_shape(int64_t groups, int K) {
+// CTAs of about 320 threads, as many to an SM as 768 threads and its shared memory allow
+static RnShape rn_shape(int64_t M, int K, bool codes, bool backward) {
   RnShape s{};
   s.T = (K + 255) / 256 * 16;
-  s.G = s.T >= 256 ? 1 : 256 / s.T;
+  s.split = s.T > RN_PAIR;
+  if (s.split) s.off = (K + 511) / 512 * 256, s.T = s.off / 16;
+  s.G = s.T >= 192 ? 1 : 320 / s.T;
+  const int64_t groups = backward || s.split ? M : (M + 1) / 2;
+  if (groups < 2 * rn_sms() && s.G > 1) s.G = 1;  // few rows: spread over the SMs
   s.threads = (s.T * s.G + 31) / 32 * 32;
-  const int64_t want = (groups + s.G - 1) / s.G, cap = static_cast<int64_t>(rn_sms()) * (s.threads >= 1024 ? 1 : 1024 / s.threads);
+  s.ahead = RN_AHEAD * 6 * K > 220 * 1024 ? 2 : RN_AHEAD;
+  s.smem = rn_rows_at(s.threads) + s.G * (backward ? s.ahead * 6 * K : rn_group_bytes(K, s.split)) +
+           (codes ? s.threads / 16 * xgrp(16) * 8 : 0);
+  int per = 768 / s.threads;
+  if (per > 225 * 1024 / (s.smem + 1024)) per = 225 * 1024 / (s.smem + 1024);
+  if (per < 1) per = 1;
+  const int64_t want = (groups + s.G - 1) / s.G, cap = static_cast<int64_t>(rn_sms()) * per;
   s.blocks = static_cast<int>(want < cap ? want : cap);
   return s;
 }
 size_t resnorm_workspace(int64_t M, int K, bool backward) {
   if (!backward || M == 0) return 0;
-  const RnShape s = rn_shape(M, K);
+  const RnShape s = rn_shape(M, K, false, true);
   return static_cast<size_t>(s.blocks) * s.G * K * 4;
 }
-static bool rn_wide(const void* p, int64_t ld) { return !p || (ld % 16 == 0 && reinterpret_cast<uintptr_t>(p) % 32 == 0); }
+template <typename F>
+static int rn_ready(F* kernel, int smem) {
+  if (smem <= 48 * 1024) return H3B_OK;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  return e == cudaSuccess ? H3B_OK : cuda_fail(e, "cudaFuncSetAttribute(resnorm)");
+}
 
-template <int DT, bool CODES, bool FAST, bool AHEAD>
-static int resnorm_forward_t(const ResNormArgs& a, cudaStream_t st) {
-  const RnShape s = rn_shape((a.M + 1) / 2, a.K);
-  auto kernel = resnorm_kernel<DT, CODES, FAST, AHEAD>;
-  const int halves = s.threads / 16;
-  const int smem = (16 * halves + 15) / 16 * 16 + (CODES ? halves * xgrp(16) * 8 : 0);
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(resnorm)");
-  }
-  const bool wide = rn_wide(a.x, a.ldx) && rn_wide(a.y, a.ldy) && rn_wide(a.t, a.ldt) && rn_wide(a.h, a.ldh);
-  kernel<<<s.blocks, s.threads, smem, st>>>(a, s.T, s.G, wide);
+template <int DT, bool CODES, bool FAST, bool SPLIT>
+static int resnorm_forward_t(const ResNormArgs& a, const RnShape& s, cudaStream_t st) {
+  auto kernel = resnorm_kernel<DT, CODES, FAST, SPLIT>;
+  if (int rc = rn_ready(kernel, s.smem)) return rc;
+  kernel<<<s.blocks, s.threads, s.smem, st>>>(a, s);
   return check_launch("resnorm_kernel");
 }
-template <int DT, bool FAST, bool AHEAD>
-static int resnorm_backward_t(const ResNormArgs& a, cudaStream_t st) {
-  const RnShape s = rn_shape(a.M, a.K);
-  const bool wide = rn_wide(a.dt, a.lddt) && rn_wide(a.dh, a.lddh) && rn_wide(a.t, a.ldt) && rn_wide(a.dx, a.lddx) && rn_wide(a.dy, a.lddy);
+template <int DT, bool FAST, bool SPLIT>
+static int resnorm_backward_t(const ResNormArgs& a, const RnShape& s, cudaStream_t st) {
+  auto kernel = resnorm_grad_kernel<DT, FAST, SPLIT>;
+  if (int rc = rn_ready(kernel, s.smem)) return rc;
   float* part = a.dw ? static_cast<float*>(a.ws) : nullptr;
-  resnorm_grad_kernel<DT, FAST, AHEAD><<<s.blocks, s.threads, 2 * s.threads / 16 * 4, st>>>(a, s.T, s.G, wide, part);
+  kernel<<<s.blocks, s.threads, s.smem, st>>>(a, s, part);
   if (int rc = check_launch("resnorm_grad_kernel")) return rc;
   if (!a.dw) return H3B_OK;
   resnorm_dw_kernel<<<(a.K + 31) / 32, 256, 0, st>>>(part, static_cast<int64_t>(s.blocks) * s.G, a.K, a.dw, a.w_dtype);
@@ -416,17 +478,18 @@ static int resnorm_backward_t(const ResNormArgs& a, cudaStream_t st) {
 template <int DT>
 static int resnorm_t(const ResNormArgs& a, bool backward, cudaStream_t st) {
   constexpr int CODE = DT == DT_BF16 ? H3B_BF16 : H3B_FP16;
-  const bool fast = a.w_dtype == CODE && ((!a.gate && !a.scale) || a.m_dtype == CODE), ahead = (a.K + 255) / 256 * 16 <= RN_AHEAD;
+  const bool fast = a.w_dtype == CODE && ((!a.gate && !a.scale) || a.m_dtype == CODE);
+  const RnShape s = rn_shape(a.M, a.K, !backward && a.codes, backward);
   if (backward) {
-    if (fast) return ahead ? resnorm_backward_t<DT, true, true>(a, st) : resnorm_backward_t<DT, true, false>(a, st);
-    return ahead ? resnorm_backward_t<DT, false, true>(a, st) : resnorm_backward_t<DT, false, false>(a, st);
+    if (fast) return s.split ? resnorm_backward_t<DT, true, true>(a, s, st) : resnorm_backward_t<DT, true, false>(a, s, st);
+    return s.split ? resnorm_backward_t<DT, false, true>(a, s, st) : resnorm_backward_t<DT, false, false>(a, s, st);
   }
   if (a.codes) {
-    if (fast) return ahead ? resnorm_forward_t<DT, true, true, true>(a, st) : resnorm_forward_t<DT, true, true, false>(a, st);
-    return ahead ? resnorm_forward_t<DT, true, false, true>(a, st) : resnorm_forward_t<DT, true, false, false>(a, st);
+    if (fast) return s.split ? resnorm_forward_t<DT, true, true, true>(a, s, st) : resnorm_forward_t<DT, true, true, false>(a, s, st);
+    return s.split ? resnorm_forward_t<DT, true, false, true>(a, s, st) : resnorm_forward_t<DT, true, false, false>(a, s, st);
   }
-  if (fast) return ahead ? resnorm_forward_t<DT, false, true, true>(a, st) : resnorm_forward_t<DT, false, true, false>(a, st);
-  return ahead ? resnorm_forward_t<DT, false, false, true>(a, st) : resnorm_forward_t<DT, false, false, false>(a, st);
+  if (fast) return s.split ? resnorm_forward_t<DT, false, true, true>(a, s, st) : resnorm_forward_t<DT, false, true, false>(a, s, st);
+  return s.split ? resnorm_forward_t<DT, false, false, true>(a, s, st) : resnorm_forward_t<DT, false, false, false>(a, s, st);
 }
 int resnorm_launch(const ResNormArgs& a, bool backward, cudaStream_t st) {
   if (backward && a.M == 0) {  // nothing to add up
