@@ -41,22 +41,29 @@ __device__ __forceinline__ void rn_bulk(void* dst, const void* src, int bytes, u
                "l"(src), "r"(bytes), "r"(smem_u32(bar))
                : "memory");
 }
-// 8 numbers of the weight or of a modulation row, of the stream's type (FAST) or of any
+// Address of number `col` of the weight or of a modulation row, of the stream's type (FAST) or of any
+template <bool FAST>
+__device__ __forceinline__ const char* rn_param_at(const void* p, int64_t at, int dt) {
+  return static_cast<const char*>(p) + (FAST || dt != H3B_FP32 ? 2 : 4) * at;
+}
+// 8 numbers, the k-th 8 from there
 template <int DT, bool FAST>
-__device__ __forceinline__ void rn_param(const void* p, int64_t at, int dt, bool ok, float (&f)[8]) {
+__device__ __forceinline__ void rn_param(const char* p, int k, int dt, bool ok, float (&f)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) f[i] = 0.f;
   if (!ok) return;
-  if constexpr (FAST) load8(p, at, DT == DT_BF16 ? H3B_BF16 : H3B_FP16, f);
-  else load8(p, at, dt, f);
+  if constexpr (FAST) load8(p, 8 * k, DT == DT_BF16 ? H3B_BF16 : H3B_FP16, f);
+  else load8(p, 8 * k, dt, f);
 }
-__device__ __forceinline__ int rn_mod_row(const ResNormArgs& a, int64_t r) {
+__device__ __forceinline__ int rn_mod_row(const ResNormArgs& a, int64_t row) {
   int m = -1;
-  if (r >= a.M) return m;
+  if (row >= a.M) return m;
   if (a.token_rows) {
-    m = a.token_rows[r];
+    m = a.token_rows[row];
     return m < a.n_rows ? m : -1;
   }
+  const int r = static_cast<int>(row);  // below 2^30
+#pragma unroll 2
   for (int s = 0; s < a.segs.n; ++s)
     if (r >= a.segs.first[s] && r < a.segs.end[s]) m = a.segs.row[s];
   return m;
@@ -64,16 +71,20 @@ __device__ __forceinline__ int rn_mod_row(const ResNormArgs& a, int64_t r) {
 __device__ __forceinline__ char* rn_at(const void* p, int64_t row, int64_t ld, int col) {
   return static_cast<char*>(const_cast<void*>(p)) + 2 * (row * ld + col);
 }
-// A row's sum: every 16 threads leave theirs in `part`, everyone adds up the row's T / 16.  The barrier is the CTA's.
-__device__ __forceinline__ float2 rn_sum(float2 v, float2* part, int mine, int first, int n) {
+// A row's sum: every 16 threads leave theirs in `part`; behind the barrier (the CTA's) every 16 threads add up the row's n <= 32.
+__device__ __forceinline__ float rn_sum16(float v) {
 #pragma unroll
-  for (int o = 8; o; o >>= 1) v.x += __shfl_xor_sync(0xffffffffu, v.x, o), v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
-  if ((threadIdx.x & 15) == 0) part[mine] = v;
+  for (int o = 8; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ float2 rn_sum(float2 v, float2* part, int mine, int first, int n) {
+  const int t = threadIdx.x & 15;
+  v = make_float2(rn_sum16(v.x), rn_sum16(v.y));
+  if (t == 0) part[mine] = v;
   __syncthreads();
-  float2 s = make_float2(0.f, 0.f);
-#pragma unroll 4
-  for (int i = 0; i < n; ++i) s.x += part[first + i].x, s.y += part[first + i].y;
-  return s;
+  const float2 lo = t < n ? part[first + t] : make_float2(0.f, 0.f);
+  const float2 hi = t + 16 < n ? part[first + 16 + t] : make_float2(0.f, 0.f);
+  return make_float2(rn_sum16(lo.x + hi.x), rn_sum16(lo.y + hi.y));
 }
 
 // What a launch is made of: groups of T threads, G to a CTA (rounded up to whole warps); a group has two rows, or one (SPLIT: its lanes'
@@ -82,20 +93,24 @@ struct RnShape {
   int T, G, threads, blocks, off, smem, ahead;
   bool split;
 };
-constexpr int RN_PAIR = 384;  // threads that a pair of rows has at most
-// Shared memory: barrier and abort flag (32 bytes), the groups' sums, their rows, the rotation's exchange
-__host__ __device__ inline int rn_rows_at(int threads) { return 32 + threads; }  // threads / 16 half-warps x (8 + 8) bytes
+constexpr int RN_THREADS = 320;  // a CTA's, with 96 registers each and 20 warps to an SM; groups of more (WIDE) are CTAs of up to 512
+                                 // with 128 registers and 16 warps
+// Shared memory: barriers and abort flag (32 bytes), the groups' modulation rows (at most RN_GRAD_THREADS / 16 pairs of them), their
+// sums, their rows, the rotation's exchange
+constexpr int RN_HEAD = 256;
+__host__ __device__ inline int rn_rows_at(int threads) { return RN_HEAD + threads; }  // threads / 16 half-warps x (8 + 8) bytes
 __host__ __device__ inline int rn_group_bytes(int K, bool split) { return (split ? 2 : 4) * 2 * K; }
 
-template <int DT, bool CODES, bool FAST, bool SPLIT>
-__global__ void __launch_bounds__(SPLIT ? 512 : RN_PAIR, SPLIT ? 1 : 2) resnorm_kernel(const ResNormArgs a, const RnShape s) {
+template <int DT, bool CODES, bool FAST, bool SPLIT, bool WIDE>
+__global__ void __launch_bounds__(WIDE ? 512 : RN_THREADS, WIDE ? 1 : 2) resnorm_kernel(const ResNormArgs a, const RnShape s) {
   extern __shared__ __align__(128) unsigned char rn_smem[];
   const int tid = threadIdx.x, T = s.T, G = s.G, unit = tid / T, tr = tid - unit * T, K = a.K;
   const int half = tid >> 4, halves = blockDim.x >> 4, t16 = tid & 15, parts = unit < G ? T >> 4 : 0, first = unit * parts;
   const int col[2] = {16 * tr, 16 * tr + (SPLIT ? s.off : 0)};
   uint64_t* const bar = reinterpret_cast<uint64_t*>(rn_smem);
   volatile int* const abort = reinterpret_cast<volatile int*>(rn_smem + 8);
-  float2* const part = reinterpret_cast<float2*>(rn_smem + 32);
+  float2* const part = reinterpret_cast<float2*>(rn_smem + RN_HEAD);
+  int2* const rows_of = reinterpret_cast<int2*>(rn_smem + 32) + (unit < G ? unit : 0);
   uint2* const tops = reinterpret_cast<uint2*>(part + halves);
   unsigned char* const mine = rn_smem + rn_rows_at(blockDim.x) + (unit < G ? unit : 0) * rn_group_bytes(K, SPLIT);
   float2* const gbuf = reinterpret_cast<float2*>(rn_smem + rn_rows_at(blockDim.x) + G * rn_group_bytes(K, SPLIT)) + half * xgrp(16);
@@ -108,6 +123,15 @@ __global__ void __launch_bounds__(SPLIT ? 512 : RN_PAIR, SPLIT ? 1 : 2) resnorm_
     mbar_fence_init();
     *abort = 0;
   }
+  // a group's first thread finds the modulation rows of the next round too (a row that is not there has its neighbour's)
+  auto find = [&](int64_t r) {
+    int2 m;
+    m.x = m.y = rn_mod_row(a, r);
+    if (!SPLIT && r + 1 < a.M) m.y = rn_mod_row(a, r + 1);
+    *rows_of = m;
+  };
+  const bool leads = tr == 0 && unit < G;
+  if (leads) find(r0);
   __syncthreads();
   auto bring = [&](int64_t r) {  // by a group's first thread
     int n = 0;
@@ -119,88 +143,160 @@ __global__ void __launch_bounds__(SPLIT ? 512 : RN_PAIR, SPLIT ? 1 : 2) resnorm_
         rn_bulk(mine + h * 4 * K + 2 * K, rn_at(a.y, r + h, a.ldy, 0), 2 * K, bar);
       }
   };
-  const bool leads = tr == 0 && unit < G;
   if (leads) bring(r0);
+  const bool mods = FAST && a.gate && a.scale;
   const float over_k = 1.f / static_cast<float>(K);
   uint32_t turn = 0;
   for (int64_t base = static_cast<int64_t>(blockIdx.x) * G; base < groups; base += step, r0 += ROWS * step, turn ^= 1) {
     const int64_t row[2] = {r0, r0 + ROWS - 1};
     const int n[2] = {row[0] < a.M ? K - col[0] : 0, row[1] < a.M ? K - col[1] : 0};
-    const int mrow[2] = {rn_mod_row(a, row[0]), SPLIT ? rn_mod_row(a, row[0]) : rn_mod_row(a, row[1])};
+    const int2 both = *rows_of;
+    const int mrow[2] = {both.x, both.y};
     const bool same = !SPLIT && mrow[0] == mrow[1];  // one load of a modulation row serves both lanes
+    // the ordinary case by itself, without a branch inside: rows of one segment (of codes: 16 channels to every thread that has any)
+    const bool plain = CODES && mods && same && mrow[0] >= 0 && unit < G;
+    const int64_t mod0 = 2 * (mrow[0] * a.ldm + col[0]);  // bytes into gate, scale and shift
     mbar_wait(bar, turn, abort);
     // ---- the stream
     float2 v[16], ss = make_float2(0.f, 0.f);
+    if (plain) {
+      const unsigned char* at = mine + 2 * col[0];
+      char* const to = rn_at(a.t, row[0], a.ldt, col[0]);
+      const int64_t next = row[1] < a.M ? 2 * a.ldt : 0;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {  // 8 channels at a time
-      float p[8];
+      for (int k = 0; k < 2; ++k) {
+        float g[8], f[8], y[8];
+        load8(static_cast<const char*>(a.gate) + mod0, 8 * k, DT == DT_BF16 ? H3B_BF16 : H3B_FP16, g);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          rn_unpack<DT>(*reinterpret_cast<const uint4*>(at + h * 4 * K + 16 * k), f);
+          rn_unpack<DT>(*reinterpret_cast<const uint4*>(at + h * 4 * K + 2 * K + 16 * k), y);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] = fmaf(y[i], g[i], f[i]);  // the product of two numbers of 16 bits is exact
+          const uint4 t = rn_pack<DT>(f);
+          if (h == 0 || next) *reinterpret_cast<uint4*>(to + h * next + 16 * k) = t;
+          rn_unpack<DT>(t, f);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (h == 0) v[8 * k + i].x = f[i];
+            else v[8 * k + i].y = f[i];
+          }
+        }
+      }
+    } else {
+      const char* pg[2];
+      char* to[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float f[8], y[8];
-        const bool ok = n[h] > 8 * k;
-        const int c = col[h] + 8 * k;
-        const unsigned char* at = mine + (SPLIT ? 0 : h) * 4 * K + 2 * c;
-        rn_unpack<DT>(rn_load(at, ok), f);
-        rn_unpack<DT>(rn_load(at + 2 * K, ok), y);
-        if (a.gate) {
-          if (mrow[h] >= 0) {
-            if (h == 0 || !same) rn_param<DT, FAST>(a.gate, mrow[h] * a.ldm + c, a.m_dtype, ok, p);
+        pg[h] = rn_param_at<FAST>(a.gate, mrow[h] * a.ldm + col[h], a.m_dtype);
+        to[h] = rn_at(a.t, row[h], a.ldt, col[h]);
+      }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = __fadd_rn(f[i], __fmul_rn(y[i], p[i]));
+      for (int k = 0; k < 2; ++k) {  // 8 channels at a time
+        float p[8];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float f[8], y[8];
+          const bool ok = n[h] > 8 * k;
+          const unsigned char* at = mine + (SPLIT ? 0 : h) * 4 * K + 2 * col[h] + 16 * k;
+          rn_unpack<DT>(rn_load(at, ok), f);
+          rn_unpack<DT>(rn_load(at + 2 * K, ok), y);
+          if (a.gate) {
+            if (mrow[h] >= 0) {
+              if (h == 0 || !same) rn_param<DT, FAST>(pg[h], k, a.m_dtype, ok, p);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) f[i] = __fadd_rn(f[i], __fmul_rn(y[i], p[i]));
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = __fadd_rn(f[i], y[i]);
           }
-        } else {
+          const uint4 t = rn_pack<DT>(f);
+          if (ok) *reinterpret_cast<uint4*>(to[h] + 16 * k) = t;
+          rn_unpack<DT>(t, f);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = __fadd_rn(f[i], y[i]);
-        }
-        const uint4 t = rn_pack<DT>(f);
-        if (ok) *reinterpret_cast<uint4*>(rn_at(a.t, row[h], a.ldt, c)) = t;
-        rn_unpack<DT>(t, f);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (h == 0) ss.x = fmaf(f[i], f[i], ss.x), v[8 * k + i].x = f[i];
-          else ss.y = fmaf(f[i], f[i], ss.y), v[8 * k + i].y = f[i];
+          for (int i = 0; i < 8; ++i) {
+            if (h == 0) v[8 * k + i].x = f[i];
+            else v[8 * k + i].y = f[i];
+          }
         }
       }
     }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) ss = __ffma2_rn(v[i], v[i], ss);
     if (SPLIT) ss.x = ss.y = ss.x + ss.y;
     ss = rn_sum(ss, part, half, first, parts);
     // everyone has read the rows: the next ones may come
-    if (leads && base + step < groups) bring(r0 + ROWS * step);
+    if (leads && base + step < groups) bring(r0 + ROWS * step), find(r0 + ROWS * step);
     const float2 rs = make_float2(rsqrtf(fmaf(ss.x, over_k, a.eps)), rsqrtf(fmaf(ss.y, over_k, a.eps)));
     if (a.rstd && leads) {
       if (row[0] < a.M) a.rstd[row[0]] = rs.x;
       if (!SPLIT && row[1] < a.M) a.rstd[row[1]] = rs.y;
     }
     // ---- the norm and its modulation
+    if (plain && !a.h) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      float p[8], q[8];
-      rn_param<DT, FAST>(a.w, col[0] + 8 * k, a.w_dtype, unit < G && K - col[0] > 8 * k, p);
-      if (SPLIT) rn_param<DT, FAST>(a.w, col[1] + 8 * k, a.w_dtype, unit < G && K - col[1] > 8 * k, q);
+      for (int k = 0; k < 2; ++k) {
+        float p[8], u[8], q[8];
+        load8(a.w, col[0] + 8 * k, DT == DT_BF16 ? H3B_BF16 : H3B_FP16, p);
+        load8(static_cast<const char*>(a.scale) + mod0, 8 * k, DT == DT_BF16 ? H3B_BF16 : H3B_FP16, u);
+        load8(static_cast<const char*>(a.shift) + mod0, 8 * k, DT == DT_BF16 ? H3B_BF16 : H3B_FP16, q);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        v[8 * k + i] = __fmul2_rn(__fmul2_rn(v[8 * k + i], rs), make_float2(p[i], SPLIT ? q[i] : p[i]));
-      if (a.scale) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (mrow[h] < 0) continue;
-          if (h == 0 || !same) {
-            rn_param<DT, FAST>(a.scale, mrow[h] * a.ldm + col[h] + 8 * k, a.m_dtype, n[h] > 8 * k, p);
-            rn_param<DT, FAST>(a.shift, mrow[h] * a.ldm + col[h] + 8 * k, a.m_dtype, n[h] > 8 * k, q);
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if (h == 0) v[8 * k + i].x = fmaf(v[8 * k + i].x, 1.f + p[i], q[i]);
-            else v[8 * k + i].y = fmaf(v[8 * k + i].y, 1.f + p[i], q[i]);
-          }
+        for (int i = 0; i < 8; ++i) {
+          const float c = 1.f + u[i];
+          float2& z = v[8 * k + i];
+          z = __fmul2_rn(__fmul2_rn(z, rs), make_float2(p[i], p[i]));
+          z = __ffma2_rn(z, make_float2(c, c), make_float2(q[i], q[i]));
         }
       }
-      if (a.h) {
+    } else {
+      const char *pw[2], *ps[2], *pt[2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < 2; ++h) {
+        pw[h] = rn_param_at<FAST>(a.w, col[h], a.w_dtype);
+        ps[h] = rn_param_at<FAST>(a.scale, mrow[h] * a.ldm + col[h], a.m_dtype);
+        pt[h] = rn_param_at<FAST>(a.shift, mrow[h] * a.ldm + col[h], a.m_dtype);
+      }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) p[i] = h == 0 ? v[8 * k + i].x : v[8 * k + i].y;
-          if (n[h] > 8 * k) *reinterpret_cast<uint4*>(rn_at(a.h, row[h], a.ldh, col[h] + 8 * k)) = rn_pack<DT>(p);
+      for (int k = 0; k < 2; ++k) {
+        float p[8], q[8];
+        rn_param<DT, FAST>(pw[0], k, a.w_dtype, unit < G && K - col[0] > 8 * k, p);
+        if (SPLIT) rn_param<DT, FAST>(pw[1], k, a.w_dtype, unit < G && K - col[1] > 8 * k, q);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          v[8 * k + i] = __fmul2_rn(__fmul2_rn(v[8 * k + i], rs), make_float2(p[i], SPLIT ? q[i] : p[i]));
+        if (a.scale) {
+          if (same) {
+            if (mrow[0] >= 0) {
+              rn_param<DT, FAST>(ps[0], k, a.m_dtype, n[0] > 8 * k, p);
+              rn_param<DT, FAST>(pt[0], k, a.m_dtype, n[0] > 8 * k, q);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float u = 1.f + p[i];
+                v[8 * k + i] = __ffma2_rn(v[8 * k + i], make_float2(u, u), make_float2(q[i], q[i]));
+              }
+            }
+          } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (mrow[h] < 0) continue;
+              rn_param<DT, FAST>(ps[h], k, a.m_dtype, n[h] > 8 * k, p);
+              rn_param<DT, FAST>(pt[h], k, a.m_dtype, n[h] > 8 * k, q);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                if (h == 0) v[8 * k + i].x = fmaf(v[8 * k + i].x, 1.f + p[i], q[i]);
+                else v[8 * k + i].y = fmaf(v[8 * k + i].y, 1.f + p[i], q[i]);
+              }
+            }
+          }
+        }
+        if (a.h) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) p[i] = h == 0 ? v[8 * k + i].x : v[8 * k + i].y;
+            if (n[h] > 8 * k) *reinterpret_cast<uint4*>(rn_at(a.h, row[h], a.ldh, col[h] + 8 * k)) = rn_pack<DT>(p);
+          }
         }
       }
     }
@@ -221,23 +317,29 @@ __global__ void __launch_bounds__(SPLIT ? 512 : RN_PAIR, SPLIT ? 1 : 2) resnorm_
       for (int i = 0; i < 4; ++i) h4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], 1.0f);
 #pragma unroll
       for (int i = 0; i < 4; ++i) h4(v[i], v[i + 4], v[i + 8], v[i + 12], 0.0625f);
-      // ---- the largest magnitude, as bits: a NaN's are above infinity's and stay
-      uint2 top = make_uint2(0u, 0u);
+      // ---- the largest magnitude.  max leaves NaN out, but every number of a block is a sum over all of it: one that is not finite
+      // makes them all so, and then the first one's bits (infinity's and NaN's are above the others') say it
+      float2 m = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        top.x = max(top.x, __float_as_uint(v[i].x) & 0x7FFFFFFFu);
-        top.y = max(top.y, __float_as_uint(v[i].y) & 0x7FFFFFFFu);
-      }
-      if (SPLIT) top.x = top.y = max(top.x, top.y);
+      for (int i = 0; i < 16; i += 2) m.x = max3f(m.x, fabsf(v[i].x), fabsf(v[i + 1].x)), m.y = max3f(m.y, fabsf(v[i].y), fabsf(v[i + 1].y));
+      uint2 top = make_uint2(max(__float_as_uint(m.x), __float_as_uint(v[0].x) & 0x7FFFFFFFu),
+                             max(__float_as_uint(m.y), __float_as_uint(v[0].y) & 0x7FFFFFFFu));
+      if (SPLIT) top.x = max(top.x, top.y);
+      auto top16 = [&] {
 #pragma unroll
-      for (int o = 8; o; o >>= 1) {
-        top.x = max(top.x, __shfl_xor_sync(0xffffffffu, top.x, o));
-        if (!SPLIT) top.y = max(top.y, __shfl_xor_sync(0xffffffffu, top.y, o));
-      }
+        for (int o = 8; o; o >>= 1) {
+          top.x = max(top.x, __shfl_xor_sync(0xffffffffu, top.x, o));
+          if (!SPLIT) top.y = max(top.y, __shfl_xor_sync(0xffffffffu, top.y, o));
+        }
+      };
+      top16();
       if (t16 == 0) tops[half] = top;
       __syncthreads();
-#pragma unroll 4
-      for (int i = 0; i < parts; ++i) top.x = max(top.x, tops[first + i].x), top.y = max(top.y, tops[first + i].y);
+      {
+        const uint2 lo = t16 < parts ? tops[first + t16] : make_uint2(0u, 0u), hi = t16 + 16 < parts ? tops[first + 16 + t16] : make_uint2(0u, 0u);
+        top = make_uint2(max(lo.x, hi.x), max(lo.y, hi.y));
+      }
+      top16();
       if (SPLIT) top.y = top.x;
       const float2 amax = make_float2(__uint_as_float(top.x), __uint_as_float(top.y));
       if (leads) {
@@ -280,8 +382,9 @@ __global__ void __launch_bounds__(SPLIT ? 512 : RN_PAIR, SPLIT ? 1 : 2) resnorm_
 // Gradients: a group has one row at a time, a thread 16 channels (or 16 and 16, SPLIT) of it; its part of dw over all its rows stays in
 // registers.  Rows come as bulk copies two rows ahead, into three buffers in turn (one ahead and two buffers where three do not fit).
 constexpr int RN_AHEAD = 3;
+constexpr int RN_GRAD_THREADS = 384;  // of a row that is not split, with 80 registers each and 24 warps to an SM; split ones have up to 512 with 128
 template <int DT, bool FAST, bool SPLIT>
-__global__ void __launch_bounds__(SPLIT ? 512 : RN_PAIR, SPLIT ? 1 : 2) resnorm_grad_kernel(const ResNormArgs a, const RnShape s,
+__global__ void __launch_bounds__(SPLIT ? 512 : RN_GRAD_THREADS, SPLIT ? 1 : 2) resnorm_grad_kernel(const ResNormArgs a, const RnShape s,
                                                                                            float* dw) {
   constexpr int L = SPLIT ? 2 : 1;
   extern __shared__ __align__(128) unsigned char rn_smem[];
@@ -289,7 +392,7 @@ __global__ void __launch_bounds__(SPLIT ? 512 : RN_PAIR, SPLIT ? 1 : 2) resnorm_
   const int half = tid >> 4, halves = blockDim.x >> 4, parts = unit < G ? T >> 4 : 0, first = unit * parts;
   uint64_t* const bars = reinterpret_cast<uint64_t*>(rn_smem);  // three
   volatile int* const abort = reinterpret_cast<volatile int*>(rn_smem + 24);
-  float* const part = reinterpret_cast<float*>(rn_smem + 32);  // two rows' sums in turn: one barrier a row
+  float* const part = reinterpret_cast<float*>(rn_smem + RN_HEAD);  // two rows' sums in turn: one barrier a row
   const int bytes = (a.dt ? 6 : 4) * K;  // dh, t, dt
   unsigned char* const mine = rn_smem + rn_rows_at(blockDim.x) + (unit < G ? unit : 0) * s.ahead * bytes;
   const int64_t step = static_cast<int64_t>(gridDim.x) * G;
@@ -337,14 +440,14 @@ __global__ void __launch_bounds__(SPLIT ? 512 : RN_PAIR, SPLIT ? 1 : 2) resnorm_
         float p[8], f[8];
         rn_unpack<DT>(rn_load(at + 2 * col, ok), f);
         if (a.scale && mrow >= 0) {
-          rn_param<DT, FAST>(a.scale, mrow * a.ldm + col, a.m_dtype, ok, p);
+          rn_param<DT, FAST>(rn_param_at<FAST>(a.scale, mrow * a.ldm + col, a.m_dtype), 0, a.m_dtype, ok, p);
 #pragma unroll
           for (int i = 0; i < 8; ++i) f[i] *= 1.f + p[i];
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) g[l][8 * k + i] = f[i];
         rn_unpack<DT>(rn_load(at + 2 * K + 2 * col, ok), f);
-        rn_param<DT, FAST>(a.w, col, a.w_dtype, ok, p);
+        rn_param<DT, FAST>(rn_param_at<FAST>(a.w, col, a.w_dtype), 0, a.w_dtype, ok, p);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int e = 8 * k + i;
@@ -355,18 +458,15 @@ __global__ void __launch_bounds__(SPLIT ? 512 : RN_PAIR, SPLIT ? 1 : 2) resnorm_
         }
       }
     }
-#pragma unroll
-    for (int o = 8; o; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    dot = rn_sum16(dot);
     float* const here = part + (k & 1) * halves;
     if ((tid & 15) == 0) here[half] = dot;
     __syncthreads();
     // everyone is through with the row before: its buffer is free
     const int free = buf == 0 ? s.ahead - 1 : buf - 1;
     if (leads && k + s.ahead - 1 < left) bring(r + (s.ahead - 1) * step, free);
-    dot = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < parts; ++i) dot += here[first + i];
-    dot *= over_k;
+    const int t16 = tid & 15;
+    dot = rn_sum16((t16 < parts ? here[first + t16] : 0.f) + (t16 + 16 < parts ? here[first + 16 + t16] : 0.f)) * over_k;
 #pragma unroll
     for (int l = 0; l < L; ++l) {
 #pragma unroll
@@ -380,7 +480,7 @@ __global__ void __launch_bounds__(SPLIT ? 512 : RN_PAIR, SPLIT ? 1 : 2) resnorm_
         if (ok) *reinterpret_cast<uint4*>(rn_at(a.dx, r, a.lddx, col)) = rn_pack<DT>(d);
         if (a.dy) {
           float p[8];
-          rn_param<DT, FAST>(a.gate, mrow * a.ldm + col, a.m_dtype, ok && mrow >= 0, p);
+          rn_param<DT, FAST>(rn_param_at<FAST>(a.gate, mrow * a.ldm + col, a.m_dtype), 0, a.m_dtype, ok && mrow >= 0, p);
 #pragma unroll
           for (int i = 0; i < 8; ++i) d[i] = mrow >= 0 ? d[i] * p[i] : 0.f;
           if (ok) *reinterpret_cast<uint4*>(rn_at(a.dy, r, a.lddy, col)) = rn_pack<DT>(d);
@@ -425,20 +525,21 @@ static int rn_sms() {
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   return sms;
 }
-// CTAs of about 320 threads, as many to an SM as 768 threads and its shared memory allow
+// CTAs of up to 320 threads, as many to an SM as its registers and its shared memory allow
 static RnShape rn_shape(int64_t M, int K, bool codes, bool backward) {
   RnShape s{};
   s.T = (K + 255) / 256 * 16;
-  s.split = s.T > RN_PAIR;
+  const int most = backward ? RN_GRAD_THREADS : RN_THREADS;
+  s.split = s.T > most;
   if (s.split) s.off = (K + 511) / 512 * 256, s.T = s.off / 16;
-  s.G = s.T >= 192 ? 1 : 320 / s.T;
+  s.G = s.T > most ? 1 : most / s.T;
   const int64_t groups = backward || s.split ? M : (M + 1) / 2;
   if (groups < 2 * rn_sms() && s.G > 1) s.G = 1;  // few rows: spread over the SMs
   s.threads = (s.T * s.G + 31) / 32 * 32;
   s.ahead = RN_AHEAD * 6 * K > 220 * 1024 ? 2 : RN_AHEAD;
   s.smem = rn_rows_at(s.threads) + s.G * (backward ? s.ahead * 6 * K : rn_group_bytes(K, s.split)) +
            (codes ? s.threads / 16 * xgrp(16) * 8 : 0);
-  int per = 768 / s.threads;
+  int per = (backward ? (s.split ? 16 : 24) : s.threads > RN_THREADS ? 16 : 20) / (s.threads / 32);
   if (per > 225 * 1024 / (s.smem + 1024)) per = 225 * 1024 / (s.smem + 1024);
   if (per < 1) per = 1;
   const int64_t want = (groups + s.G - 1) / s.G, cap = static_cast<int64_t>(rn_sms()) * per;
@@ -457,22 +558,21 @@ static int rn_ready(F* kernel, int smem) {
   return e == cudaSuccess ? H3B_OK : cuda_fail(e, "cudaFuncSetAttribute(resnorm)");
 }
 
-template <int DT, bool CODES, bool FAST, bool SPLIT>
+template <int DT, bool FAST, bool SPLIT, bool WIDE>
 static int resnorm_forward_t(const ResNormArgs& a, const RnShape& s, cudaStream_t st) {
-  auto kernel = resnorm_kernel<DT, CODES, FAST, SPLIT>;
+  auto kernel = a.codes ? resnorm_kernel<DT, true, FAST, SPLIT, WIDE> : resnorm_kernel<DT, false, FAST, SPLIT, WIDE>;
   if (int rc = rn_ready(kernel, s.smem)) return rc;
   kernel<<<s.blocks, s.threads, s.smem, st>>>(a, s);
   return check_launch("resnorm_kernel");
 }
-template <int DT, bool FAST, bool SPLIT>
+template <int DT, bool FAST>
 static int resnorm_backward_t(const ResNormArgs& a, const RnShape& s, cudaStream_t st) {
-  auto kernel = resnorm_grad_kernel<DT, FAST, SPLIT>;
+  auto kernel = s.split ? resnorm_grad_kernel<DT, FAST, true> : resnorm_grad_kernel<DT, FAST, false>;
   if (int rc = rn_ready(kernel, s.smem)) return rc;
-  float* part = a.dw ? static_cast<float*>(a.ws) : nullptr;
-  kernel<<<s.blocks, s.threads, s.smem, st>>>(a, s, part);
+  kernel<<<s.blocks, s.threads, s.smem, st>>>(a, s, a.dw ? static_cast<float*>(a.ws) : nullptr);
   if (int rc = check_launch("resnorm_grad_kernel")) return rc;
   if (!a.dw) return H3B_OK;
-  resnorm_dw_kernel<<<(a.K + 31) / 32, 256, 0, st>>>(part, static_cast<int64_t>(s.blocks) * s.G, a.K, a.dw, a.w_dtype);
+  resnorm_dw_kernel<<<(a.K + 31) / 32, 256, 0, st>>>(static_cast<float*>(a.ws), static_cast<int64_t>(s.blocks) * s.G, a.K, a.dw, a.w_dtype);
   return check_launch("resnorm_dw_kernel");
 }
 template <int DT>
@@ -480,16 +580,13 @@ static int resnorm_t(const ResNormArgs& a, bool backward, cudaStream_t st) {
   constexpr int CODE = DT == DT_BF16 ? H3B_BF16 : H3B_FP16;
   const bool fast = a.w_dtype == CODE && ((!a.gate && !a.scale) || a.m_dtype == CODE);
   const RnShape s = rn_shape(a.M, a.K, !backward && a.codes, backward);
-  if (backward) {
-    if (fast) return s.split ? resnorm_backward_t<DT, true, true>(a, s, st) : resnorm_backward_t<DT, true, false>(a, s, st);
-    return s.split ? resnorm_backward_t<DT, false, true>(a, s, st) : resnorm_backward_t<DT, false, false>(a, s, st);
-  }
-  if (a.codes) {
-    if (fast) return s.split ? resnorm_forward_t<DT, true, true, true>(a, s, st) : resnorm_forward_t<DT, true, true, false>(a, s, st);
-    return s.split ? resnorm_forward_t<DT, true, false, true>(a, s, st) : resnorm_forward_t<DT, true, false, false>(a, s, st);
-  }
-  if (fast) return s.split ? resnorm_forward_t<DT, false, true, true>(a, s, st) : resnorm_forward_t<DT, false, true, false>(a, s, st);
-  return s.split ? resnorm_forward_t<DT, false, false, true>(a, s, st) : resnorm_forward_t<DT, false, false, false>(a, s, st);
+  if (backward) return fast ? resnorm_backward_t<DT, true>(a, s, st) : resnorm_backward_t<DT, false>(a, s, st);
+  const bool wide = s.threads > RN_THREADS;  // only of split rows
+  if (fast)
+    return wide ? resnorm_forward_t<DT, true, true, true>(a, s, st)
+                : s.split ? resnorm_forward_t<DT, true, true, false>(a, s, st) : resnorm_forward_t<DT, true, false, false>(a, s, st);
+  return wide ? resnorm_forward_t<DT, false, true, true>(a, s, st)
+              : s.split ? resnorm_forward_t<DT, false, true, false>(a, s, st) : resnorm_forward_t<DT, false, false, false>(a, s, st);
 }
 int resnorm_launch(const ResNormArgs& a, bool backward, cudaStream_t st) {
   if (backward && a.M == 0) {  // nothing to add up
