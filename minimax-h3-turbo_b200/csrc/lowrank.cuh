@@ -603,6 +603,178 @@ __global__ void __launch_bounds__(LR_THREADS, LrExpandCfg<NQ, W_ROWS>::CTAS)
   }
 }
 
+// ----------------------------------------------------------------------------------------------- few rows
+// Up to eight rows of one adapter, as single tokens of many requests have them: everything is the adapters' weights, read once, and
+// latency.  Weights go from memory straight to fragments; K is dealt out to `splits` CTAs of a tile, whose parts the second kernel adds
+// up in a fixed order.  The second kernel is let in when every CTA of the first has begun, and asks for its weights and base
+// before it waits for the parts: the two products' weights come in one stream.  (A cluster of eight CTAs for both products, its parts
+// in distributed shared memory: 16.2 us for one row of rank 64, 91 us for 64 rows of 64 adapters 5120 -> 15360.)
+//   32 columns (ranks) of a row: lane t has 8 t .. 8 t + 7, which are k = 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of two products
+constexpr int LR_FEW_THREADS = 128;
+__device__ __forceinline__ void lr_let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void lr_prefetch(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+template <typename T>
+__device__ __forceinline__ uint4 lr_row8(const T* row, int64_t j, int64_t n, bool aligned) {  // numbers j .. j + 7 of n, zeros behind
+  uint4 v = make_uint4(0, 0, 0, 0);
+  if (aligned) {
+    if (j < n) v = *reinterpret_cast<const uint4*>(row + j);
+  } else {
+    uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (j + i < n) w[i / 2] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(row + j + i)) << (16 * (i & 1));
+  }
+  return v;
+}
+// part[tile][split][row of 8][rp] = x A_g^T over the split's columns: 16 ranks x 8 rows a product
+template <typename T, int RB>  // 16 RB: the largest rp of this variant
+__global__ void __launch_bounds__(LR_FEW_THREADS) lr_few_down_kernel(const LrPlan p, const T* x, int64_t ldx, int64_t K, const T* a, int rank,
+                                                                     int rp, int R, int splits, float* part) {
+  constexpr int W = LR_FEW_THREADS / 32;
+  __shared__ float red[W][8][16 * RB + 4];
+  after_previous();
+  lr_let_next();
+  const int tile = blockIdx.x / splits, split = blockIdx.x - tile * splits;
+  const int4 t = p.few[tile];
+  if (t.z == 0 || t.x >= R) return;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q4 = lane & 3;
+  const int row = g < t.z ? p.order[t.y + g] : -1;  // this lane's row
+  const T* ag = a + static_cast<int64_t>(t.x) * rank * K;
+  float acc[RB][4];
+#pragma unroll
+  for (int i = 0; i < RB; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+  const int blocks = static_cast<int>((K + 31) / 32), b0 = split * blocks / splits, b1 = (split + 1) * blocks / splits;
+#pragma unroll 2
+  for (int i = b0 + warp; i < b1; i += W) {
+    const int64_t k = i * 32 + 8 * q4;
+    const uint4 xv = lr_row8(x + row * ldx, k, row >= 0 ? K : 0, true);
+    uint4 w[RB][2];
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int j = 16 * r + 8 * h + g;
+        w[r][h] = lr_row8(ag + j * K, k, j < rank ? K : 0, true);
+      }
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+      lr_mma<T>(acc[r], w[r][0].x, w[r][1].x, w[r][0].y, w[r][1].y, xv.x, xv.y);
+      lr_mma<T>(acc[r], w[r][0].z, w[r][1].z, w[r][0].w, w[r][1].w, xv.z, xv.w);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < RB; ++r)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) red[warp][2 * q4 + (e & 1)][16 * r + g + 8 * (e >> 1)] = acc[r][e];
+  __syncthreads();
+  float* to = part + static_cast<int64_t>(blockIdx.x) * 8 * rp;
+  for (int e = tid; e < t.z * rp; e += LR_FEW_THREADS) {
+    const int m = e / rp, j = e - m * rp;
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) sum += red[w][m][j];
+    to[e] = sum;
+  }
+}
+// out [rows, 64 columns of a warp]: lane t has columns 16 t .. 16 t + 15, of which 2 j, 2 j + 1 are product j's n = 2 t, 2 t + 1
+template <typename T, int RB>
+__global__ void __launch_bounds__(LR_FEW_THREADS) lr_few_up_kernel(const LrPlan p, const T* b, int rank, int rp, int R, const float* scales,
+                                                                   const T* base, int64_t ldb, T* out, int64_t ldo, int64_t N, int columns,
+                                                                   bool wide, const float* part, int splits, const LrHidden hid, bool keep) {
+  constexpr int KB = (RB + 1) / 2, AT_ONCE = KB > 2 ? 4 : 8;  // blocks of 32 ranks; products whose weights are held
+  __shared__ float h[8][16 * RB];
+  __shared__ __align__(16) T hs[8][32 * KB + 8];
+  __shared__ float mults[8];
+  const int tile = blockIdx.x / columns, at = blockIdx.x - tile * columns;
+  const int4 t = p.few[tile];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q4 = lane & 3;
+  if (t.z == 0 || (t.x >= R && base == out)) {
+    after_previous();
+    return;
+  }
+  const int row = g < t.z ? p.order[t.y + g] : -1;  // this lane's row
+  const int64_t c0 = (static_cast<int64_t>(at) * (LR_FEW_THREADS / 32) + warp) * 64, c = c0 + 16 * q4, n0 = c0 + 16 * (g >> 1) + (g & 1);
+  uint32_t v[8];
+  lr_load16(base + row * ldb + c, base && row >= 0 ? N - c : 0, wide, v);
+  if (t.x >= R) {  // rows without an adapter
+    after_previous();
+    lr_store16(out + row * ldo + c, row >= 0 ? N - c : 0, wide, v);
+    return;
+  }
+  const T* bg = b + static_cast<int64_t>(t.x) * rank * N;
+  const bool aligned = rank % 8 == 0;
+  uint4 w[AT_ONCE][KB];
+  auto weights = [&](int j0) {
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j)
+#pragma unroll
+      for (int k = 0; k < KB; ++k) {
+        const int64_t n = n0 + 2 * (j0 + j);
+        w[j][k] = lr_row8(bg + n * rank, 32 * k + 8 * q4, n < N ? rank : 0, aligned);
+      }
+  };
+  weights(0);
+  if (AT_ONCE < 8) {
+#pragma unroll
+    for (int j = AT_ONCE; j < 8; ++j)
+      if (n0 + 2 * j < N && q4 * 64 < rank) lr_prefetch(bg + (n0 + 2 * j) * rank + q4 * 64);
+  }
+  after_previous();
+  // ---- h: the splits' parts; a row's power of two (fp16); the operand of this product
+  const float scale = scales ? scales[t.x] : 1.f;
+  for (int e = tid; e < t.z * rp; e += LR_FEW_THREADS) {
+    const float* from = part + static_cast<int64_t>(tile) * splits * 8 * rp + e;
+    float sum = 0.f;
+#pragma unroll 8
+    for (int s = 0; s < splits; ++s) sum += from[static_cast<int64_t>(s) * 8 * rp];
+    h[e / rp][e % rp] = sum * scale;
+  }
+  __syncthreads();
+  const bool first = keep && at == 0;
+  for (int m = warp; m < 8; m += LR_FEW_THREADS / 32) {
+    float mult = 1.f;
+    if constexpr (std::is_same_v<T, __half>) {
+      float top = 0.f;
+      for (int j = lane; j < rp; j += 32) top = fmaxf(top, m < t.z ? fabsf(h[m][j]) : 0.f);
+      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      mult = lr_power(top);
+    }
+    const float inv = 1.f / mult;
+    for (int j = lane; j < 32 * KB; j += 32) {
+      const T u = lr_t<T>(m < t.z && j < rp ? h[m][j] * inv : 0.f);
+      hs[m][j] = u;
+      if (first && j < rp && m < t.z) static_cast<T*>(hid.h)[static_cast<int64_t>(t.y + m) * rp + j] = u;
+    }
+    if (lane == 0) {
+      mults[m] = mult;
+      if (first && m < t.z) hid.mult[t.y + m] = mult;
+    }
+  }
+  __syncthreads();
+  uint4 ha[KB];
+#pragma unroll
+  for (int k = 0; k < KB; ++k) ha[k] = *reinterpret_cast<const uint4*>(&hs[g][32 * k + 8 * q4]);
+  const float mult = mults[g];
+#pragma unroll
+  for (int j0 = 0; j0 < 8; j0 += AT_ONCE) {
+    if (j0 > 0) weights(j0);
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) {
+      float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < KB; ++k) {
+        lr_mma<T>(d, ha[k].x, 0u, ha[k].y, 0u, w[j][k].x, w[j][k].y);
+        lr_mma<T>(d, ha[k].z, 0u, ha[k].w, 0u, w[j][k].z, w[j][k].w);
+      }
+      const float2 f = lr_unpack2<T>(v[j0 + j]);
+      v[j0 + j] = pack2<T>(fmaf(d[0], mult, f.x), fmaf(d[1], mult, f.y));
+    }
+  }
+  lr_store16(out + row * ldo + c, row >= 0 ? N - c : 0, wide, v);
+}
+
 // ----------------------------------------------------------------------------------------------- weight gradients
 // D [128 channels, rp] = X^T H over the rows of a unit (a stretch of one adapter's rows): X's columns are M, H's are N, rows are K,
 // all read as they lie in memory.  HBM-bound: X is read once; H comes from L2.  Rows behind the last are zeros in both operands.  One
@@ -810,20 +982,35 @@ __global__ void __launch_bounds__(256) lr_join_kernel(const LrPlan p, const LrWg
 }
 
 // ----------------------------------------------------------------------------------------------- launches
-// A workspace: hidden rows, parts of the weight gradients
+// Whether a batch's rows go by eights or by 128: while the weights that every eight rows read again cost less than the other kernels'
+// fixed times (5120 -> 5120, us by eights and by 128: rank 16 512 rows 9.5, 13.5, 1024 rows 19.3, 14.5; rank 64 128 rows 13.8, 19.4,
+// 512 rows 19.9, 20.8; rank 128 64 rows 23, 27, 256 rows 34, 28), and where most adapters have no more than eight rows anyway.
+static bool lr_are_few(int64_t M, int64_t R, int rank) { return M <= 8 * R || (M <= 512 && M * lr_rp(rank) <= 12288); }
+// CTAs that share the first product of a tile of few rows: some four to an SM in all, of four blocks of 32 columns at least,
+// and 16 at most (their parts are added up by every CTA of the second product)
+static int lr_few_splits(int64_t tiles, int64_t K) {
+  const int64_t most = K / 128 < 16 ? K / 128 : 16, want = 4 * 148 / tiles;
+  return static_cast<int>(want > most ? (most < 1 ? 1 : most) : want < 1 ? 1 : want);
+}
+// A workspace: hidden rows, then parts of the weight gradients or of few rows' first product
 struct LrSpace {
   size_t part_a, part_b, total;
 };
-static LrSpace lr_space(int64_t M, int64_t K, int64_t N, int rank, bool backward) {
+static LrSpace lr_space(int64_t M, int64_t K, int64_t N, int rank, int64_t R, bool backward) {
   LrSpace s{};
   s.part_a = lr_hidden_bytes(M, rank);
-  const size_t slot = backward ? static_cast<size_t>(lr_slots(M)) * lr_rp(rank) * 4 : 0;
+  if (!backward) {
+    const int64_t tiles = lr_lines(M, R, LR_FEW);
+    s.part_b = s.total = s.part_a + (lr_are_few(M, R, rank) ? lr_up256(static_cast<size_t>(tiles) * lr_few_splits(tiles, K) * 8 * lr_rp(rank) * 4) : 0);
+    return s;
+  }
+  const size_t slot = static_cast<size_t>(lr_slots(M)) * lr_rp(rank) * 4;
   s.part_b = s.part_a + lr_up256(slot * K);
   s.total = s.part_b + lr_up256(slot * N);
   return s;
 }
 size_t lr_workspace(int64_t M, int64_t K, int64_t N, int rank, int64_t R, bool backward) {
-  return M == 0 ? 0 : lr_space(M, K, N, rank, backward).total;
+  return M == 0 ? 0 : lr_space(M, K, N, rank, R, backward).total;
 }
 // How many CTAs share a tile's steps, 1, 2, 4 or 8: the fewest rounds of resident CTAs times the steps that each takes, with what a
 // CTA's start and end cost (`extra` steps).
@@ -903,11 +1090,36 @@ static int lr_wgrad(const LrPlan& p, const LrWgradSide<T>& a, const LrWgradSide<
   const int ja = static_cast<int>((a.blocks ? a.C + chans - 1 : 0) / chans), jb = static_cast<int>((b.blocks ? b.C + chans - 1 : 0) / chans);
   return lr_launch("lr_join_kernel", lr_join_kernel<T>, joined, dim3(ja + jb, R), 256, 0, 1, st, p, a, b, ja, rank, rp);
 }
+template <typename T, int RB>
+static int lr_few_s(const LrPlan& p, const LrArgs& a, int rp, const LrHidden& h, float* part, cudaStream_t st) {
+  static std::atomic<bool> ready[2][CA_DEVICES];
+  const T* base = static_cast<const T*>(a.base);
+  T* out = static_cast<T*>(a.out);
+  const int splits = lr_few_splits(p.n_few, a.K), R = static_cast<int>(a.R);
+  const int columns = static_cast<int>((a.N + 2 * LR_FEW_THREADS - 1) / (2 * LR_FEW_THREADS));
+  if (int rc = lr_launch("lr_few_down_kernel", lr_few_down_kernel<T, RB>, ready[0], dim3(static_cast<unsigned>(p.n_few * splits)),
+                         LR_FEW_THREADS, 0, 1, st, p, static_cast<const T*>(a.x), a.ldx, a.K, static_cast<const T*>(a.a), a.rank, rp, R,
+                         splits, part))
+    return rc;
+  return lr_launch("lr_few_up_kernel", lr_few_up_kernel<T, RB>, ready[1], dim3(static_cast<unsigned>(p.n_few * columns)), LR_FEW_THREADS, 0, 1,
+                   st, p, static_cast<const T*>(a.b), a.rank, rp, R, a.scales, base, a.ldbase, out, a.ldo, a.N, columns,
+                   lr_wide(base, a.ldbase) && lr_wide(out, a.ldo), part, splits, h, a.hidden != nullptr);
+}
+template <typename T>
+static int lr_few(const LrPlan& p, const LrArgs& a, const LrHidden& h, float* part, cudaStream_t st) {
+  const int rp = lr_rp(a.rank);
+  if (rp <= 16) return lr_few_s<T, 1>(p, a, rp, h, part, st);
+  if (rp <= 32) return lr_few_s<T, 2>(p, a, rp, h, part, st);
+  if (rp <= 64) return lr_few_s<T, 4>(p, a, rp, h, part, st);
+  return lr_few_s<T, 8>(p, a, rp, h, part, st);
+}
 template <typename T>
 static int lr_forward_t(const LrArgs& a, cudaStream_t st) {
   const LrPlan p = lr_plan(a.plan, a.M, a.R);
   const LrHidden h = lr_hidden(a.hidden ? a.hidden : a.ws, a.M, a.rank);
   const int R = static_cast<int>(a.R);
+  if (lr_are_few(a.M, a.R, a.rank))
+    return lr_few<T>(p, a, h, reinterpret_cast<float*>(static_cast<char*>(a.ws) + lr_space(a.M, a.K, a.N, a.rank, a.R, false).part_a), st);
   if (int rc = lr_shrink<T, true>(p, static_cast<const T*>(a.x), a.ldx, a.K, static_cast<const T*>(a.a), a.rank, R, a.scales, h, st))
     return rc;
   return lr_expand<T, true>(p, h, static_cast<const T*>(a.b), a.rank, R, static_cast<const T*>(a.base), a.ldbase, static_cast<T*>(a.out),
@@ -916,7 +1128,7 @@ static int lr_forward_t(const LrArgs& a, cudaStream_t st) {
 template <typename T>
 static int lr_backward_t(const LrArgs& a, cudaStream_t st) {
   const LrPlan p = lr_plan(a.plan, a.M, a.R);
-  const LrSpace s = lr_space(a.M, a.K, a.N, a.rank, true);
+  const LrSpace s = lr_space(a.M, a.K, a.N, a.rank, a.R, true);
   const LrHidden h = lr_hidden(a.hidden, a.M, a.rank), dh = lr_hidden(a.ws, a.M, a.rank);
   const int R = static_cast<int>(a.R);
   const T *x = static_cast<const T*>(a.x), *go = static_cast<const T*>(a.go);
