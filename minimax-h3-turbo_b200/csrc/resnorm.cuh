@@ -15,6 +15,8 @@
 // of whole rows (held in registers instead, they left room for 10 warps to an SM: 763 us for 59440 x 5120 into codes).  w, gate,
 // scale and shift come from L1 every time: 4 bytes a channel and pair of rows.
 #pragma once
+#include <atomic>
+
 #include "rotq.cuh"
 
 namespace h3b {
@@ -519,10 +521,22 @@ __global__ void __launch_bounds__(256) resnorm_dw_kernel(const float* part, int6
   else static_cast<__nv_bfloat16*>(dw)[c] = __float2bfloat16_rn(s);
 }
 
-static int rn_sms() {
-  int dev = 0, sms = 148;
+// SM count, and whether a kernel's shared memory has been asked for: once per device (a call spends microseconds on them otherwise)
+constexpr int RN_DEVICES = 64;
+static int rn_device() {
+  int dev = 0;
   cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return dev;
+}
+static int rn_sms() {
+  static std::atomic<int> known[RN_DEVICES];
+  const int dev = rn_device();
+  int sms = dev < RN_DEVICES ? known[dev].load(std::memory_order_relaxed) : 0;
+  if (sms == 0) {
+    sms = 148;
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (dev < RN_DEVICES) known[dev].store(sms, std::memory_order_relaxed);
+  }
   return sms;
 }
 // CTAs of up to 320 threads, as many to an SM as its registers and its shared memory allow
@@ -552,23 +566,29 @@ size_t resnorm_workspace(int64_t M, int K, bool backward) {
   return static_cast<size_t>(s.blocks) * s.G * K * 4;
 }
 template <typename F>
-static int rn_ready(F* kernel, int smem) {
+static int rn_ready(F* kernel, int smem, std::atomic<bool> (&done)[RN_DEVICES]) {
   if (smem <= 48 * 1024) return H3B_OK;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  return e == cudaSuccess ? H3B_OK : cuda_fail(e, "cudaFuncSetAttribute(resnorm)");
+  const int dev = rn_device();
+  if (dev < RN_DEVICES && done[dev].load(std::memory_order_acquire)) return H3B_OK;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(resnorm)");
+  if (dev < RN_DEVICES) done[dev].store(true, std::memory_order_release);
+  return H3B_OK;
 }
 
 template <int DT, bool FAST, bool SPLIT, bool WIDE>
 static int resnorm_forward_t(const ResNormArgs& a, const RnShape& s, cudaStream_t st) {
   auto kernel = a.codes ? resnorm_kernel<DT, true, FAST, SPLIT, WIDE> : resnorm_kernel<DT, false, FAST, SPLIT, WIDE>;
-  if (int rc = rn_ready(kernel, s.smem)) return rc;
+  static std::atomic<bool> ready[2][RN_DEVICES];
+  if (int rc = rn_ready(kernel, s.smem, ready[a.codes != nullptr])) return rc;
   kernel<<<s.blocks, s.threads, s.smem, st>>>(a, s);
   return check_launch("resnorm_kernel");
 }
 template <int DT, bool FAST>
 static int resnorm_backward_t(const ResNormArgs& a, const RnShape& s, cudaStream_t st) {
   auto kernel = s.split ? resnorm_grad_kernel<DT, FAST, true> : resnorm_grad_kernel<DT, FAST, false>;
-  if (int rc = rn_ready(kernel, s.smem)) return rc;
+  static std::atomic<bool> ready[2][RN_DEVICES];
+  if (int rc = rn_ready(kernel, s.smem, ready[s.split])) return rc;
   kernel<<<s.blocks, s.threads, s.smem, st>>>(a, s, a.dw ? static_cast<float*>(a.ws) : nullptr);
   if (int rc = check_launch("resnorm_grad_kernel")) return rc;
   if (!a.dw) return H3B_OK;

@@ -83,6 +83,8 @@ def _sizes(m: int, k: int, n: int, rank: int, adapters: int, backward: bool) -> 
 
 def _readable(t: torch.Tensor) -> torch.Tensor:
     """[M, width] rows the kernels can read in place (contiguous channels, 16-byte aligned rows that do not overlap), or a copy."""
+    if t.is_contiguous():  # rows of multiples of 8
+        return t if t.data_ptr() % 16 == 0 else t.clone()
     m, width = t.shape
     st = t.stride()
     if (st[1] == 1 or width == 1) and (m <= 1 or (st[0] % 8 == 0 and st[0] >= width)) and t.data_ptr() % 16 == 0:
@@ -154,16 +156,18 @@ class _Problem:
                              f"{t.dtype} on {t.device}")
         return t if t.dim() == 2 else t.reshape(self.m, width)
 
-    def scratch(self, backward: bool):
-        n, _ = _sizes(self.m, self.k, self.n, self.rank, self.adapters, backward)
-        return (torch.empty(n, dtype=torch.uint8, device=self.dev) if n else None), n
-
-    def launch(self, fn, args, what: str) -> None:
-        if self.dev.index == torch.cuda.current_device():
-            rc = fn(*args, _lib.raw_stream(self.dev.index))
+    def launch(self, fn, head, tail, backward: bool, what: str) -> None:
+        """Workspace and the call: fn(*head, workspace, its bytes, stream) with the sizes that both entry points share in between."""
+        n = _sizes(self.m, self.k, self.n, self.rank, self.adapters, backward)[0]
+        ws = torch.empty(n, dtype=torch.uint8, device=self.dev) if n else None
+        args = (*head, self.code, self.m, self.k, self.n, self.rank, self.adapters, _lib.ptr(self.scales), _lib.ptr(self.plan.table),
+                *tail, _lib.ptr(ws), n)
+        index = self.dev.index
+        if index == torch.cuda.current_device():
+            rc = fn(*args, _lib.raw_stream(index))
         else:
             with torch.cuda.device(self.dev):
-                rc = fn(*args, _lib.raw_stream(self.dev.index))
+                rc = fn(*args, _lib.raw_stream(index))
         if rc:
             _lib.check(rc, what)
 
@@ -212,11 +216,9 @@ def _forward(p: _Problem, base, out, want_hidden: bool):
     if want_hidden:
         hidden = torch.empty(_sizes(p.m, p.k, p.n, p.rank, p.adapters, False)[1], dtype=torch.uint8, device=p.dev)
     if p.m:
-        ws, n = p.scratch(False)
         p.launch(_lib.lib().h3b_low_rank, (p.x.data_ptr(), _ld(p.x), p.a.data_ptr(), p.b.data_ptr(), _lib.ptr(base),
-                                           0 if base is None else _ld(base), y.data_ptr(), _ld(y), p.code, p.m, p.k, p.n, p.rank,
-                                           p.adapters, _lib.ptr(p.scales), p.plan.table.data_ptr(), _lib.ptr(hidden), _lib.ptr(ws),
-                                           n), "low_rank")
+                                           0 if base is None else _ld(base), y.data_ptr(), p.n if out is None else _ld(y)),
+                 (_lib.ptr(hidden),), False, "low_rank")
     return y, hidden
 
 
@@ -231,12 +233,9 @@ def _backward(do, x, a, b, pl, hidden, scales, need):
     da = torch.empty(p.a.shape, dtype=p.dt, device=p.dev) if need[1] else None
     db = torch.empty(p.b.shape, dtype=p.dt, device=p.dev) if need[2] else None
     if any(need):
-        ws, n = p.scratch(True)
-        table = p.plan.table
         p.launch(_lib.lib().h3b_low_rank_backward,
                  (do.data_ptr(), _ld(do), p.x.data_ptr(), _ld(p.x), p.a.data_ptr(), p.b.data_ptr(), hidden.data_ptr(), _lib.ptr(dx),
-                  p.k, _lib.ptr(da), _lib.ptr(db), p.code, p.m, p.k, p.n, p.rank, p.adapters, _lib.ptr(p.scales), _lib.ptr(table),
-                  _lib.ptr(ws), n), "low_rank_backward")
+                  p.k, _lib.ptr(da), _lib.ptr(db)), (), True, "low_rank_backward")
     return (None if dx is None else dx.view(x.shape), None if da is None else da.view(a.shape),
             None if db is None else db.view(b.shape))
 
@@ -297,17 +296,20 @@ def low_rank(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, plan: Optional[A
     p = _Problem(x, a, b, plan, scales)
     y = None
     base2 = None if base is None else p.rows(base, p.n, "base")
-    if out is not None:
-        y = p.rows(out, p.n, "out")
-        if y.data_ptr() != out.data_ptr() or _readable(y).data_ptr() != y.data_ptr():
-            raise ValueError("low_rank: out needs contiguous channels, a 16-byte aligned base and row strides that are multiples of 8")
-        if base is not None and (base is out or (base2.data_ptr() == y.data_ptr() and _ld(base2) == _ld(y))):
-            base2 = y
-        if any(_overlap(y, t) for t in (p.x, p.a, p.b, *([] if base2 is None or base2 is y else [base2]))):
-            raise ValueError("low_rank: out must not overlap x, a, b or a part of base")
-    y, hidden = _forward(p, base2, y, return_hidden)
-    y = out if out is not None else y.view(*p.lead, p.n)
-    return (y, hidden) if return_hidden else y
+    if out is None:
+        y, hidden = _forward(p, base2, None, return_hidden)
+        if x.dim() != 2:
+            y = y.view(*p.lead, p.n)
+        return (y, hidden) if return_hidden else y
+    y = p.rows(out, p.n, "out")
+    if y.data_ptr() != out.data_ptr() or _readable(y).data_ptr() != y.data_ptr():
+        raise ValueError("low_rank: out needs contiguous channels, a 16-byte aligned base and row strides that are multiples of 8")
+    if base is not None and (base is out or (base2.data_ptr() == y.data_ptr() and _ld(base2) == _ld(y))):
+        base2 = y
+    if any(_overlap(y, t) for t in (p.x, p.a, p.b, *([] if base2 is None or base2 is y else [base2]))):
+        raise ValueError("low_rank: out must not overlap x, a, b or a part of base")
+    _, hidden = _forward(p, base2, y, return_hidden)
+    return (out, hidden) if return_hidden else out
 
 
 def low_rank_backward(do: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, plan: Optional[AdapterPlan],

@@ -40,6 +40,8 @@ def _workspace_bytes(m: int, k: int, backward: bool) -> int:
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """t itself when the kernels can read its rows in place, or a copy."""
+    if t.is_contiguous():  # rows of multiples of 8
+        return t if t.data_ptr() % 16 == 0 else t.clone()
     if t.stride(1) == 1 and t.data_ptr() % 16 == 0 and (t.shape[0] <= 1 or (t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1])):
         return t
     t = t.contiguous()
@@ -52,6 +54,26 @@ def _ld(t: Optional[torch.Tensor]) -> int:
 
 def _code(t: Optional[torch.Tensor]) -> int:
     return _lib.BF16 if t is None else _lib.act_code(t.dtype)
+
+
+_tables = {}  # (segments, rows, modulation rows) -> the C table of them and its length
+
+
+def _segments(segments, m: int, n_rows: int, device):
+    """block._segment_args, its tables of plain numbers kept (a table is a few numbers by value; making one takes microseconds)."""
+    try:
+        key = (tuple(segments), m, n_rows)
+        found = _tables.get(key)
+    except TypeError:  # per-token rows
+        return blk._segment_args(segments, m, n_rows, device)
+    if found is None:
+        table, n, rows = blk._segment_args(segments, m, n_rows, device)
+        if rows is not None or any(type(v) is not int for seg in key[0] for v in seg):
+            return table, n, rows
+        if len(_tables) > 256:
+            _tables.clear()
+        found = _tables[key] = (table, n)
+    return (*found, None)
 
 
 class _Problem:
@@ -79,11 +101,13 @@ class _Problem:
         self.table, self.n_seg, self.token_rows, self.n_rows = None, 0, None, 0
         if mods:
             self.n_rows = mods[0].shape[0]
-            self.table, self.n_seg, self.token_rows = blk._segment_args(segments or (), self.m, self.n_rows, self.dev)
-            if any(t.dtype != mods[0].dtype for t in mods):
+            self.table, self.n_seg, self.token_rows = _segments(segments or (), self.m, self.n_rows, self.dev)
+            dt = mods[0].dtype
+            if any(t.dtype != dt for t in mods):
                 mods = [t.float() for t in mods]
             mods = [_rows(t) for t in mods]
-            if any(_ld(t) != _ld(mods[0]) for t in mods):
+            ld = _ld(mods[0])
+            if any(_ld(t) != ld for t in mods):
                 mods = [t.contiguous() for t in mods]
         it = iter(mods)
         self.gate, self.shift, self.scale = (None if t is None else next(it) for t in (gate, shift, scale))
