@@ -28,7 +28,7 @@ __device__ __forceinline__ T lr_t(float v) {
 // ----------------------------------------------------------------------------------------------- plan
 // A plan is one int32 array: order [M], the rows by adapter, those without one last; offset [R + 2], where each adapter's rows
 // begin in it (group R: rows without one); slot [R + 1], below; then tables of four numbers a line:
-//   tiles  (adapter, first place in order, rows, 0), up to LR_TILE rows each
+//   tiles  (adapter, first place in order, rows, first row if they follow one another, else -1), up to LR_TILE rows each
 //   few    the same, up to LR_FEW rows each
 //   units  (adapter, first tile, tiles, slot), up to lr_unit_tiles(M) tiles each: what a CTA of the weight gradients adds up.  The
 //          units of an adapter that has several have a slot each, slot[g] to slot[g + 1], for their partial sums; else -1
@@ -111,6 +111,13 @@ static __global__ void __launch_bounds__(LR_PLAN_THREADS) lr_order_kernel(const 
     at += __popc(m);
   }
 }
+// rows of an adapter are in ascending order: they follow one another where the last is as far from the first as their number says
+__device__ __forceinline__ int4 lr_line(const int32_t* order, int who, int from, int n) {
+  const int first = order[from], last = order[from + n - 1];
+  return make_int4(who, from, n, last - first == n - 1 ? first : -1);
+}
+// row i of a tile
+__device__ __forceinline__ int lr_row(const LrPlan& p, const int4& t, int i) { return t.w >= 0 ? t.w + i : p.order[t.y + i]; }
 // One CTA: the tables, from the offsets.  1024 adapters at a time: their numbers of lines are added up, then every warp writes
 // those of its 32 adapters, a lane per line.
 static __global__ void __launch_bounds__(LR_PLAN_THREADS) lr_tables_kernel(const LrPlan p, int R) {
@@ -150,15 +157,15 @@ static __global__ void __launch_bounds__(LR_PLAN_THREADS) lr_tables_kernel(const
       const int4 t = make_int4(__shfl_sync(0xffffffffu, at.x, l), __shfl_sync(0xffffffffu, at.y, l),
                                __shfl_sync(0xffffffffu, at.z, l), __shfl_sync(0xffffffffu, at.w, l));
       const int nt = (rows + LR_TILE - 1) / LR_TILE, nu = who < R ? (nt + per - 1) / per : 0;
-      for (int i = lane; i < nt; i += 32) tiles[t.x + i] = make_int4(who, from + i * LR_TILE, min(LR_TILE, rows - i * LR_TILE), 0);
+      for (int i = lane; i < nt; i += 32) tiles[t.x + i] = lr_line(p.order, who, from + i * LR_TILE, min(LR_TILE, rows - i * LR_TILE));
       for (int i = lane; i < (rows + LR_FEW - 1) / LR_FEW; i += 32)
-        few[t.y + i] = make_int4(who, from + i * LR_FEW, min(LR_FEW, rows - i * LR_FEW), 0);
+        few[t.y + i] = lr_line(p.order, who, from + i * LR_FEW, min(LR_FEW, rows - i * LR_FEW));
       for (int i = lane; i < nu; i += 32) units[t.z + i] = make_int4(who, t.x + i * per, min(per, nt - i * per), nu > 1 ? t.w + i : -1);
     }
     __syncthreads();
   }
-  for (int64_t i = base.x + threadIdx.x; i < p.n_tiles; i += LR_PLAN_THREADS) tiles[i] = make_int4(R, 0, 0, 0);
-  for (int64_t i = base.y + threadIdx.x; i < p.n_few; i += LR_PLAN_THREADS) few[i] = make_int4(R, 0, 0, 0);
+  for (int64_t i = base.x + threadIdx.x; i < p.n_tiles; i += LR_PLAN_THREADS) tiles[i] = make_int4(R, 0, 0, -1);
+  for (int64_t i = base.y + threadIdx.x; i < p.n_few; i += LR_PLAN_THREADS) few[i] = make_int4(R, 0, 0, -1);
   for (int64_t i = base.z + threadIdx.x; i < p.n_units; i += LR_PLAN_THREADS) units[i] = make_int4(R, 0, 0, -1);
 }
 int lr_plan_launch(const int32_t* rows, int64_t M, int64_t R, int32_t* plan, cudaStream_t st) {
@@ -223,11 +230,11 @@ __device__ __forceinline__ void lr_arrive_full(uint64_t* bar) {
 template <typename T>
 __device__ __forceinline__ void lr_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if constexpr (std::is_same_v<T, __half>)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -238,7 +245,7 @@ __device__ __forceinline__ void lr_ldmatrix_t(uint32_t (&r)[4], uint32_t addr) {
                : "r"(addr)
                : "memory");
 }
-// 16 numbers of a row from p on, `left` of them there (a multiple of 8, also negative); wide: rows start on 32-byte boundaries
+// 16 numbers of a row from p on, `left` of them there (a multiple of 8, also negative); wide: rows start on 32-byte boundaries and are multiples of 16 long
 template <typename T>
 __device__ __forceinline__ void lr_load16(const T* p, int64_t left, bool wide, uint32_t (&v)[8]) {
   if (wide && left >= 16) {
@@ -257,9 +264,10 @@ __device__ __forceinline__ void lr_load16(const T* p, int64_t left, bool wide, u
 }
 template <typename T>
 __device__ __forceinline__ void lr_store16(T* p, int64_t left, bool wide, const uint32_t (&v)[8]) {
-  if (wide && left >= 16) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
-                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+  if (wide) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %9, 0;\n\t@p st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n\t}" ::"l"(p),
+                 "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+                 "r"(static_cast<uint32_t>(left >= 16))
                  : "memory");
     return;
   }
@@ -367,7 +375,7 @@ __global__ void __launch_bounds__(LR_SHRINK_THREADS) lr_shrink_kernel(const LrPl
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int r = r0 + 16 * i;
-      xr[i] = r < t.z ? x + static_cast<int64_t>(p.order[t.y + r]) * ldx + ch * 8 : nullptr;
+      xr[i] = r < t.z ? x + static_cast<int64_t>(lr_row(p, t, r)) * ldx + ch * 8 : nullptr;
     }
     const T* wg = w + static_cast<int64_t>(t.x) * rank * C;
     const uint32_t at = static_cast<uint32_t>(r0 * 128 + ((ch ^ (r0 & 7)) << 4));
@@ -473,6 +481,7 @@ __global__ void __launch_bounds__(LR_SHRINK_THREADS) lr_shrink_kernel(const LrPl
 // out [128 rows, N] of a tile = base + H W^T: W is B_g [N, rank] (W_ROWS) or A_g [rank, N].  A CTA has 64 CB columns of a tile, a warp 16
 // rows of them: all of its base is asked for at once, then W goes to shared memory, then the products are added and stored.
 //   block of 64 columns: lane t has columns 16 t .. 16 t + 15; 2 j, 2 j + 1 of these are product j's n = 2 t, 2 t + 1
+// Ranks are filled up with zeros to 16 NQ: leaving products out by the rank cost 13 instructions to a product.
 constexpr int LR_THREADS = 256;
 template <int NQ, bool W_ROWS>  // 16 NQ: the largest rp of this variant
 struct LrExpandCfg {
@@ -497,15 +506,18 @@ __global__ void __launch_bounds__(LR_THREADS, LrExpandCfg<NQ, W_ROWS>::CTAS)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q4 = lane & 3;
   const int r0 = 16 * warp + g;
   const int64_t c = c0 + 16 * q4;
-  int row[2];
+  int row[2];  // on their way while the small operands are asked for
+#pragma unroll
+  for (int h = 0; h < 2; ++h) row[h] = r0 + 8 * h < t.z ? lr_row(p, t, r0 + 8 * h) : -1;
   uint32_t v[CB][2][8];
+  auto ask = [&] {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) row[h] = r0 + 8 * h < t.z ? p.order[t.y + r0 + 8 * h] : -1;
+    for (int b = 0; b < CB; ++b)
 #pragma unroll
-  for (int b = 0; b < CB; ++b)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) lr_load16(base + row[h] * ldb + c + 64 * b, base && row[h] >= 0 ? N - c - 64 * b : 0, wide, v[b][h]);
+      for (int h = 0; h < 2; ++h) lr_load16(base + row[h] * ldb + c + 64 * b, base && row[h] >= 0 ? N - c - 64 * b : 0, wide, v[b][h]);
+  };
   if (t.x >= R) {  // rows without an adapter
+    ask();
 #pragma unroll
     for (int b = 0; b < CB; ++b)
 #pragma unroll
@@ -521,7 +533,7 @@ __global__ void __launch_bounds__(LR_THREADS, LrExpandCfg<NQ, W_ROWS>::CTAS)
       const int n = e / (2 * NQ), j = e % (2 * NQ) * 8, b = n & 63;
       const int at = (n & ~63) + (b >> 1 & 7) * 8 + (b >> 4) * 2 + (b & 1);
       const bool ok = c0 + n < N;
-      if (j < rp) lr_stage8(sm + at * LDW + 2 * j, ok ? wg + (c0 + n) * rank : w, j, rank, ok);
+      lr_stage8(sm + at * LDW + 2 * j, ok ? wg + (c0 + n) * rank : w, j, rank, ok);
     }
     lr_copy_commit();
   } else {
@@ -529,7 +541,6 @@ __global__ void __launch_bounds__(LR_THREADS, LrExpandCfg<NQ, W_ROWS>::CTAS)
 #pragma unroll
     for (int e = tid; e < 16 * NQ * (COLS / 8); e += LR_THREADS) {
       const int r = e / (COLS / 8), n = e % (COLS / 8) * 8, b = n & 63;
-      if (r >= rp) break;
       uint4 u = make_uint4(0, 0, 0, 0);
       if (r < rank && c0 + n < N) u = *reinterpret_cast<const uint4*>(wg + r * N + c0 + n);
       const uint32_t to = sm + r * LDW + 2 * ((n & ~63) + (b >> 1 & 7) * 8 + (b >> 4) * 2);
@@ -544,7 +555,7 @@ __global__ void __launch_bounds__(LR_THREADS, LrExpandCfg<NQ, W_ROWS>::CTAS)
   float mult[2], inv[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const int64_t pos = t.y + (row[h] >= 0 ? r0 + 8 * h : 0);
+    const int64_t pos = t.y + min(r0 + 8 * h, t.z - 1);
     const T* hr = static_cast<const T*>(hid.h) + pos * rp;
     mult[h] = std::is_same_v<T, __half> ? hid.mult[pos] : 1.f;
     inv[h] = 1.f / mult[h];
@@ -558,6 +569,7 @@ __global__ void __launch_bounds__(LR_THREADS, LrExpandCfg<NQ, W_ROWS>::CTAS)
       a[q][h] = u.x, a[q][2 + h] = u.y;
     }
   }
+  ask();
   lr_copy_wait<0>();
   __syncthreads();
 #pragma unroll
@@ -576,7 +588,6 @@ __global__ void __launch_bounds__(LR_THREADS, LrExpandCfg<NQ, W_ROWS>::CTAS)
       for (int j = 0; j < 8; ++j)
 #pragma unroll
         for (int q = 0; q < NQ; ++q) {
-          if (16 * q >= rp) break;
           const uint2 u = *reinterpret_cast<const uint2*>(lr_smem + (64 * b + 8 * j + g) * LDW + 32 * q + 8 * q4);
           lr_mma<T>(d[j], a[q][0], a[q][1], a[q][2], a[q][3], u.x, u.y);
         }
@@ -585,7 +596,6 @@ __global__ void __launch_bounds__(LR_THREADS, LrExpandCfg<NQ, W_ROWS>::CTAS)
       for (int j = 0; j < 8; j += 2)
 #pragma unroll
         for (int q = 0; q < NQ; ++q) {
-          if (16 * q >= rp) break;
           uint32_t m[4];
           lr_ldmatrix_t(m, sm + (16 * q + (lane & 15)) * LDW + 2 * (64 * b + 8 * j) + (lane >> 4) * 16);
           lr_mma<T>(d[j], a[q][0], a[q][1], a[q][2], a[q][3], m[0], m[1]);
@@ -638,7 +648,7 @@ __global__ void __launch_bounds__(LR_FEW_THREADS) lr_few_down_kernel(const LrPla
   const int4 t = p.few[tile];
   if (t.z == 0 || t.x >= R) return;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q4 = lane & 3;
-  const int row = g < t.z ? p.order[t.y + g] : -1;  // this lane's row
+  const int row = g < t.z ? lr_row(p, t, g) : -1;  // this lane's row
   const T* ag = a + static_cast<int64_t>(t.x) * rank * K;
   float acc[RB][4];
 #pragma unroll
@@ -694,7 +704,7 @@ __global__ void __launch_bounds__(LR_FEW_THREADS) lr_few_up_kernel(const LrPlan 
     after_previous();
     return;
   }
-  const int row = g < t.z ? p.order[t.y + g] : -1;  // this lane's row
+  const int row = g < t.z ? lr_row(p, t, g) : -1;  // this lane's row
   const int64_t c0 = (static_cast<int64_t>(at) * (LR_FEW_THREADS / 32) + warp) * 64, c = c0 + 16 * q4, n0 = c0 + 16 * (g >> 1) + (g & 1);
   uint32_t v[8];
   lr_load16(base + row * ldb + c, base && row >= 0 ? N - c : 0, wide, v);
@@ -1067,7 +1077,7 @@ static int lr_expand_s(const LrPlan& p, const LrHidden& h, const T* w, int rank,
   static std::atomic<bool> ready[CA_DEVICES];
   const int parts = static_cast<int>((N + Cfg::COLS - 1) / Cfg::COLS);
   return lr_launch("lr_expand_kernel", lr_expand_kernel<T, W_ROWS, NQ>, ready, dim3(static_cast<unsigned>(p.n_tiles * parts)), LR_THREADS,
-                   Cfg::SMEM, 1, st, p, h, w, rank, rp, R, base, ldb, out, ldo, N, parts, lr_wide(base, ldb) && lr_wide(out, ldo));
+                   Cfg::SMEM, 1, st, p, h, w, rank, rp, R, base, ldb, out, ldo, N, parts, N % 16 == 0 && lr_wide(base, ldb) && lr_wide(out, ldo));
 }
 template <typename T, bool W_ROWS>
 static int lr_expand(const LrPlan& p, const LrHidden& h, const T* w, int rank, int R, const T* base, int64_t ldb, T* out, int64_t ldo,
@@ -1103,7 +1113,7 @@ static int lr_few_s(const LrPlan& p, const LrArgs& a, int rp, const LrHidden& h,
     return rc;
   return lr_launch("lr_few_up_kernel", lr_few_up_kernel<T, RB>, ready[1], dim3(static_cast<unsigned>(p.n_few * columns)), LR_FEW_THREADS, 0, 1,
                    st, p, static_cast<const T*>(a.b), a.rank, rp, R, a.scales, base, a.ldbase, out, a.ldo, a.N, columns,
-                   lr_wide(base, a.ldbase) && lr_wide(out, a.ldo), part, splits, h, a.hidden != nullptr);
+                   a.N % 16 == 0 && lr_wide(base, a.ldbase) && lr_wide(out, a.ldo), part, splits, h, a.hidden != nullptr);
 }
 template <typename T>
 static int lr_few(const LrPlan& p, const LrArgs& a, const LrHidden& h, float* part, cudaStream_t st) {
