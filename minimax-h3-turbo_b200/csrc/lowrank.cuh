@@ -483,19 +483,21 @@ __global__ void __launch_bounds__(LR_SHRINK_THREADS) lr_shrink_kernel(const LrPl
 //   block of 64 columns: lane t has columns 16 t .. 16 t + 15; 2 j, 2 j + 1 of these are product j's n = 2 t, 2 t + 1
 // Ranks are filled up with zeros to 16 NQ: leaving products out by the rank cost 13 instructions to a product.
 constexpr int LR_THREADS = 256;
-template <int NQ, bool W_ROWS>  // 16 NQ: the largest rp of this variant
+template <int NQ, bool W_ROWS, bool BASE>  // 16 NQ: the largest rp of this variant
 struct LrExpandCfg {
-  static constexpr int CB = 2, COLS = 64 * CB;
+  // Columns of a CTA: 128 with base, whose numbers wait in registers.  256 where that does not count (no base), or counts less than what W
+  // and H take of L2 (ranks from 33 on: 59440 rows 5120 -> 5120 of rank 64 in all 411 us, with 128 columns 430).
+  static constexpr int CB = BASE && NQ <= 2 ? 2 : 4, COLS = 64 * CB;
   // rows of W: [COLS][16 NQ], 32 bytes apart from a multiple of 64; or [16 NQ][COLS], 16 from a multiple of 128: no bank conflicts
   static constexpr int LDW = W_ROWS ? (32 * NQ + 31) / 64 * 64 + 32 : 2 * COLS + 16;
   static constexpr int SMEM = LDW * (W_ROWS ? COLS : 16 * NQ);
-  static constexpr int CTAS = NQ <= 4 ? 3 : 2;
+  static constexpr int CTAS = NQ <= (BASE ? 2 : 4) ? 3 : 2;
 };
-template <typename T, bool W_ROWS, int NQ>
-__global__ void __launch_bounds__(LR_THREADS, LrExpandCfg<NQ, W_ROWS>::CTAS)
+template <typename T, bool W_ROWS, bool BASE, int NQ>
+__global__ void __launch_bounds__(LR_THREADS, LrExpandCfg<NQ, W_ROWS, BASE>::CTAS)
     lr_expand_kernel(const LrPlan p, const LrHidden hid, const T* w, int rank, int rp, int R, const T* base, int64_t ldb, T* out,
                      int64_t ldo, int64_t N, int parts, bool wide) {
-  using Cfg = LrExpandCfg<NQ, W_ROWS>;
+  using Cfg = LrExpandCfg<NQ, W_ROWS, BASE>;
   constexpr int CB = Cfg::CB, COLS = Cfg::COLS, LDW = Cfg::LDW;
   extern __shared__ __align__(1024) unsigned char lr_smem[];
   after_previous();
@@ -509,19 +511,26 @@ __global__ void __launch_bounds__(LR_THREADS, LrExpandCfg<NQ, W_ROWS>::CTAS)
   int row[2];  // on their way while the small operands are asked for
 #pragma unroll
   for (int h = 0; h < 2; ++h) row[h] = r0 + 8 * h < t.z ? lr_row(p, t, r0 + 8 * h) : -1;
-  uint32_t v[CB][2][8];
+  uint32_t v[BASE ? CB : 1][2][8];
   auto ask = [&] {
+    if constexpr (BASE) {
 #pragma unroll
-    for (int b = 0; b < CB; ++b)
+      for (int b = 0; b < CB; ++b)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) lr_load16(base + row[h] * ldb + c + 64 * b, base && row[h] >= 0 ? N - c - 64 * b : 0, wide, v[b][h]);
+        for (int h = 0; h < 2; ++h) lr_load16(base + row[h] * ldb + c + 64 * b, row[h] >= 0 ? N - c - 64 * b : 0, wide, v[b][h]);
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[0][h][j] = 0u;
+    }
   };
   if (t.x >= R) {  // rows without an adapter
     ask();
 #pragma unroll
     for (int b = 0; b < CB; ++b)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) lr_store16(out + row[h] * ldo + c + 64 * b, row[h] >= 0 ? N - c - 64 * b : 0, wide, v[b][h]);
+      for (int h = 0; h < 2; ++h) lr_store16(out + row[h] * ldo + c + 64 * b, row[h] >= 0 ? N - c - 64 * b : 0, wide, v[BASE ? b : 0][h]);
     return;
   }
   const uint32_t sm = smem_u32(lr_smem);
@@ -579,7 +588,7 @@ __global__ void __launch_bounds__(LR_THREADS, LrExpandCfg<NQ, W_ROWS>::CTAS)
     for (int j = 0; j < 8; ++j)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float2 f = lr_unpack2<T>(v[b][h][j]);
+        const float2 f = BASE ? lr_unpack2<T>(v[BASE ? b : 0][h][j]) : make_float2(0.f, 0.f);
         d[j][2 * h] = std::is_same_v<T, __half> ? f.x * inv[h] : f.x;
         d[j][2 * h + 1] = std::is_same_v<T, __half> ? f.y * inv[h] : f.y;
       }
@@ -1070,23 +1079,32 @@ static int lr_shrink(const LrPlan& p, const T* x, int64_t ldx, int64_t C, const 
   if (rp <= 64) return lr_shrink_s<T, W_ROWS, 64>(p, x, ldx, C, w, rank, rp, R, scales, h, st);
   return lr_shrink_s<T, W_ROWS, 128>(p, x, ldx, C, w, rank, rp, R, scales, h, st);
 }
-template <typename T, bool W_ROWS, int NQ>
+template <typename T, bool W_ROWS, bool BASE, int NQ>
 static int lr_expand_s(const LrPlan& p, const LrHidden& h, const T* w, int rank, int rp, int R, const T* base, int64_t ldb, T* out,
                        int64_t ldo, int64_t N, cudaStream_t st) {
-  using Cfg = LrExpandCfg<NQ, W_ROWS>;
+  using Cfg = LrExpandCfg<NQ, W_ROWS, BASE>;
   static std::atomic<bool> ready[CA_DEVICES];
   const int parts = static_cast<int>((N + Cfg::COLS - 1) / Cfg::COLS);
-  return lr_launch("lr_expand_kernel", lr_expand_kernel<T, W_ROWS, NQ>, ready, dim3(static_cast<unsigned>(p.n_tiles * parts)), LR_THREADS,
-                   Cfg::SMEM, 1, st, p, h, w, rank, rp, R, base, ldb, out, ldo, N, parts, N % 16 == 0 && lr_wide(base, ldb) && lr_wide(out, ldo));
+  return lr_launch("lr_expand_kernel", lr_expand_kernel<T, W_ROWS, BASE, NQ>, ready, dim3(static_cast<unsigned>(p.n_tiles * parts)), LR_THREADS,
+                   Cfg::SMEM, 1, st, p, h, w, rank, rp, R, base, ldb, out, ldo, N, parts,
+                   N % 16 == 0 && lr_wide(base, ldb) && lr_wide(out, ldo));
+}
+// W_ROWS: with or without base; else (dx) without
+template <typename T, bool W_ROWS, int NQ>
+static int lr_expand_b(const LrPlan& p, const LrHidden& h, const T* w, int rank, int rp, int R, const T* base, int64_t ldb, T* out,
+                       int64_t ldo, int64_t N, cudaStream_t st) {
+  if constexpr (W_ROWS)
+    if (base) return lr_expand_s<T, W_ROWS, true, NQ>(p, h, w, rank, rp, R, base, ldb, out, ldo, N, st);
+  return lr_expand_s<T, W_ROWS, false, NQ>(p, h, w, rank, rp, R, nullptr, 0, out, ldo, N, st);
 }
 template <typename T, bool W_ROWS>
 static int lr_expand(const LrPlan& p, const LrHidden& h, const T* w, int rank, int R, const T* base, int64_t ldb, T* out, int64_t ldo,
                      int64_t N, cudaStream_t st) {
   const int rp = lr_rp(rank);
-  if (rp <= 16) return lr_expand_s<T, W_ROWS, 1>(p, h, w, rank, rp, R, base, ldb, out, ldo, N, st);
-  if (rp <= 32) return lr_expand_s<T, W_ROWS, 2>(p, h, w, rank, rp, R, base, ldb, out, ldo, N, st);
-  if (rp <= 64) return lr_expand_s<T, W_ROWS, 4>(p, h, w, rank, rp, R, base, ldb, out, ldo, N, st);
-  return lr_expand_s<T, W_ROWS, 8>(p, h, w, rank, rp, R, base, ldb, out, ldo, N, st);
+  if (rp <= 16) return lr_expand_b<T, W_ROWS, 1>(p, h, w, rank, rp, R, base, ldb, out, ldo, N, st);
+  if (rp <= 32) return lr_expand_b<T, W_ROWS, 2>(p, h, w, rank, rp, R, base, ldb, out, ldo, N, st);
+  if (rp <= 64) return lr_expand_b<T, W_ROWS, 4>(p, h, w, rank, rp, R, base, ldb, out, ldo, N, st);
+  return lr_expand_b<T, W_ROWS, 8>(p, h, w, rank, rp, R, base, ldb, out, ldo, N, st);
 }
 template <typename T, int RPM>
 static int lr_wgrad(const LrPlan& p, const LrWgradSide<T>& a, const LrWgradSide<T>& b, int rank, int R, cudaStream_t st) {
