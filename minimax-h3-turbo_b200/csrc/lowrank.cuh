@@ -305,11 +305,12 @@ __device__ __forceinline__ void lr_stage8(uint32_t dst, const T* row, int j, int
 // gathered.  Warps 0-3 copy, then read the accumulators; warp 4 issues the products.
 constexpr int LR_XPART = LR_TILE * 128;  // 64 channels of 128 rows
 constexpr int LR_SHRINK_THREADS = 160;
-template <int RPM>  // the largest rp of this variant: 64 or 128
+template <int RPM, bool W_ROWS>  // the largest rp of this variant: 64 or 128
 struct LrShrinkCfg {
-  static constexpr int STAGES = 3, CTAS = RPM == 128 ? 2 : 3;  // stages, CTAs to an SM
-  static constexpr int WBYTES = RPM == 128 ? 16384 : 8192;
-  static constexpr int STAGE = LR_XPART + WBYTES;
+  // A stage has PB parts of 64 channels: 256 bytes of every row at a time where they fit
+  static constexpr int PB = RPM == 64 ? 2 : 1, STAGES = RPM == 64 ? 2 : 3, CTAS = 2, KC = 64 * PB;
+  static constexpr int WPART = W_ROWS ? RPM * 128 : KC * 128;  // of W: [RPM ranks][64 channels], or [KC channels][64 ranks]
+  static constexpr int STAGE = PB * LR_XPART + (W_ROWS ? PB : RPM / 64) * WPART;
   static constexpr int SMEM = STAGES * STAGE + 1024;
 };
 // The power of two that brings a row whose largest magnitude is `top` into [1, 2), 2^-60 at least (rows below add nothing that
@@ -319,12 +320,33 @@ __device__ __forceinline__ float lr_power(float top) {
   return e >= 253 ? 1.f : __int_as_float(max(e, 127 - 60) << 23);
 }
 
+// This CTA's rows of a tile: the parts of the cluster's S CTAs added up in their order, into its own; by warps 0-3
+template <int S>
+__device__ __forceinline__ void lr_gather(float* red, int ld, int row0, int rp) {
+  const int n4 = rp / 4;
+#pragma unroll 2
+  for (int e = threadIdx.x; e < LR_TILE / S * n4; e += 128) {
+    const int r = e / n4;
+    float* const own = red + (row0 + r) * ld + (e - r * n4) * 4;
+    const uint32_t at = smem_u32(own);
+    float4 v[S];
+#pragma unroll
+    for (int k = 0; k < S; ++k)
+      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(v[k].x), "=f"(v[k].y), "=f"(v[k].z), "=f"(v[k].w) : "r"(mapa_rank(at, k)) : "memory");
+    float4 sum = v[0];
+#pragma unroll
+    for (int k = 1; k < S; ++k) sum.x += v[k].x, sum.y += v[k].y, sum.z += v[k].z, sum.w += v[k].w;
+    *reinterpret_cast<float4*>(own) = sum;  // read by this thread alone
+  }
+}
+
 template <typename T, bool W_ROWS, int RPM>
 __global__ void __launch_bounds__(LR_SHRINK_THREADS) lr_shrink_kernel(const LrPlan p, const T* x, int64_t ldx, int64_t C,
                                                                       const T* w, int rank, int rp, int R, const float* scales, const LrHidden out,
                                                                       int splits) {
-  using Cfg = LrShrinkCfg<RPM>;
-  constexpr int STAGES = Cfg::STAGES;
+  using Cfg = LrShrinkCfg<RPM, W_ROWS>;
+  constexpr int STAGES = Cfg::STAGES, PB = Cfg::PB, KC = Cfg::KC;
   extern __shared__ __align__(1024) unsigned char lr_smem[];
   __shared__ uint64_t full[STAGES], empty[STAGES], done;
   __shared__ uint32_t tmem_at;
@@ -336,7 +358,7 @@ __global__ void __launch_bounds__(LR_SHRINK_THREADS) lr_shrink_kernel(const LrPl
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   unsigned char* const base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(lr_smem) + 1023) & ~static_cast<uintptr_t>(1023));
   volatile int* abort = &abort_flag;
-  const int chunks = static_cast<int>((C + 63) / 64), per = (chunks + splits - 1) / splits;
+  const int chunks = static_cast<int>((C + KC - 1) / KC), per = (chunks + splits - 1) / splits;
   const int c0 = min(split * per, chunks), n = min(per, chunks - c0);
   if (warp == 4) {
     if (lane == 0) {
@@ -358,51 +380,56 @@ __global__ void __launch_bounds__(LR_SHRINK_THREADS) lr_shrink_kernel(const LrPl
       const int s = i % STAGES;
       warp_wait(&full[s], (i / STAGES) & 1, abort);
       tc_fence_after();
-      const uint32_t xs = smem_u32(base + s * Cfg::STAGE), ws = xs + LR_XPART;
+      const uint32_t xs = smem_u32(base + s * Cfg::STAGE), ws = xs + PB * LR_XPART;
       if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          mma_f16_ss(tmem, desc_rows(xs) + kk * 2, W_ROWS ? desc_rows(ws) + kk * 2 : lr_desc_mn(ws, 64 * 128) + kk * 128, idesc,
-                     i > 0 || kk > 0);
+        for (int kk = 0; kk < 4 * PB; ++kk)
+          mma_f16_ss(tmem, desc_rows(xs) + rows_step(kk),
+                     W_ROWS ? desc_rows(ws + kk / 4 * Cfg::WPART) + kk % 4 * 2 : lr_desc_mn(ws, Cfg::WPART) + kk * 128, idesc, i > 0 || kk > 0);
       }
       __syncwarp();
       commit_one(&empty[s]);
     }
     commit_one(&done);
   } else {
-    const int r0 = tid >> 3, ch = tid & 7;  // rows r0, r0 + 16, ...; 16-byte chunk of the part
-    const T* xr[8];
+    // 8 PB lanes have a row's 128 PB bytes; rows r0, r0 + RS, ...
+    constexpr int LANES = 8 * PB, RS = 128 / LANES, NR = LR_TILE / RS;
+    const int r0 = tid / LANES, ch = tid % LANES, part = ch >> 3, c8 = ch & 7;
+    int row[NR];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = r0 + 16 * i;
-      xr[i] = r < t.z ? x + static_cast<int64_t>(lr_row(p, t, r)) * ldx + ch * 8 : nullptr;
-    }
+    for (int i = 0; i < NR; ++i) row[i] = r0 + RS * i < t.z ? lr_row(p, t, r0 + RS * i) : -1;
     const T* wg = w + static_cast<int64_t>(t.x) * rank * C;
-    const uint32_t at = static_cast<uint32_t>(r0 * 128 + ((ch ^ (r0 & 7)) << 4));
+    const uint32_t at = static_cast<uint32_t>(r0 * 128 + ((c8 ^ (r0 & 7)) << 4));  // RS is 16 or 8: the same chunk in all rows
+    const T* const xc = x + ch * 8;
     for (int i = 0; i < n + STAGES - 1; ++i) {
       if (i < n) {
         const int s = i % STAGES;
         mbar_wait(&empty[s], ((i / STAGES) & 1) ^ 1, abort);
-        const uint32_t xs = smem_u32(base + s * Cfg::STAGE) + at, ws = xs + LR_XPART;
-        const int64_t c = static_cast<int64_t>(c0 + i) * 64;
+        const uint32_t xs = smem_u32(base + s * Cfg::STAGE), ws = xs + PB * LR_XPART;
+        const int64_t c = static_cast<int64_t>(c0 + i) * KC;
         const bool in = c + ch * 8 < C;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) lr_copy16(xs + j * 2048, xr[j] && in ? xr[j] + c : x, xr[j] && in);
+        for (int j = 0; j < NR; ++j) {
+          const bool ok = row[j] >= 0 && in;
+          lr_copy16(xs + part * LR_XPART + at + j * RS * 128, ok ? xc + row[j] * ldx + c : x, ok);
+        }
         if constexpr (W_ROWS) {
 #pragma unroll
-          for (int j = 0; j < RPM / 16; ++j) {
-            const int r = r0 + 16 * j;
-            if (16 * j < rp) lr_copy16(ws + j * 2048, r < rank && in ? wg + r * C + c + ch * 8 : w, r < rank && in);
+          for (int j = 0; j < RPM / RS; ++j) {
+            const int r = r0 + RS * j;
+            if (RS * j < rp) lr_copy16(ws + part * Cfg::WPART + at + j * RS * 128, r < rank && in ? wg + r * C + c + ch * 8 : w, r < rank && in);
           }
         } else {
+          const int k0 = tid >> 3, k8 = tid & 7;  // 16 channels at a time, eight lanes to 64 ranks of one
+          const uint32_t wat = ws + k0 * 128 + ((k8 ^ (k0 & 7)) << 4);
 #pragma unroll
-          for (int part = 0; part < (RPM + 63) / 64; ++part) {
-            const int k = part * 64 + ch * 8;
+          for (int q = 0; q < RPM / 64; ++q) {
+            const int k = q * 64 + k8 * 8;
             if (k < rp) {
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const int64_t r = c + r0 + 16 * j;
-                lr_stage8(ws + part * 8192 + j * 2048, r < C ? wg + r * rank : w, k, rank, r < C);
+              for (int j = 0; j < KC / 16; ++j) {
+                const int64_t r = c + k0 + 16 * j;
+                lr_stage8(wat + q * Cfg::WPART + j * 2048, r < C ? wg + r * rank : w, k, rank, r < C);
               }
             }
           }
@@ -443,35 +470,33 @@ __global__ void __launch_bounds__(LR_SHRINK_THREADS) lr_shrink_kernel(const LrPl
     tc_fence_after();
     tmem_dealloc(tmem, lr_tmem_cols(rp));
   } else {
-    // `splits` lanes to a row, rp / splits values each (an even number)
-    const int row = split * (LR_TILE / splits) + tid / splits, w0 = rp / splits, cols = tid % splits * w0;
-    float top = 0.f;
-    for (int c = cols; c < cols + w0; c += 2) {
-      float2 sum = make_float2(0.f, 0.f);
-      const uint32_t mine = smem_u32(red + row * ld + c);
-      for (int k = 0; k < splits; ++k) {
-        float2 v;
-        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(mapa_rank(mine, k)) : "memory");
-        sum.x += v.x, sum.y += v.y;
+    const int rows = LR_TILE / splits, row0 = split * rows;  // this CTA's share of the tile's rows
+    if (splits == 2) lr_gather<2>(red, ld, row0, rp);
+    if (splits == 4) lr_gather<4>(red, ld, row0, rp);
+    if (splits == 8) lr_gather<8>(red, ld, row0, rp);
+    if constexpr (std::is_same_v<T, __half>) {  // the rows' powers of two
+      group_sync(1, 128);
+      if (tid < rows) {
+        float top = 0.f;
+        for (int c = 0; c < rp; c += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(red + (row0 + tid) * ld + c);
+          top = fmaxf(fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+        }
+        const float mult = lr_power(fabsf(scale) * top);
+        red[(row0 + tid) * ld + rp] = mult;  // behind the row
       }
-      sum.x *= scale, sum.y *= scale;
-      top = fmaxf(top, fmaxf(fabsf(sum.x), fabsf(sum.y)));
-      *reinterpret_cast<float2*>(red + row * ld + c) = sum;  // read by this thread alone
     }
-    float mult = 1.f;
-    if constexpr (std::is_same_v<T, __half>) {
-      for (int o = splits / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      mult = lr_power(top);
-    }
-    if (row < t.z) {
-      const int64_t pos = t.y + row;
-      const float inv = 1.f / mult;  // a power of two
-      uint32_t* h = reinterpret_cast<uint32_t*>(static_cast<T*>(out.h) + pos * rp + cols);
-      for (int c = 0; c < w0; c += 2) {
-        const float2 v = *reinterpret_cast<const float2*>(red + row * ld + cols + c);
-        h[c / 2] = pack2<T>(v.x * inv, v.y * inv);
-      }
-      if (cols == 0) out.mult[pos] = mult;
+    group_sync(1, 128);
+    const int lanes = rp / 8;  // 8 numbers to a lane
+    for (int e = tid; e < rows * lanes; e += 128) {
+      const int r = e / lanes, c = (e - r * lanes) * 8, row = row0 + r;
+      if (row >= t.z) break;
+      const float* from = red + row * ld + c;
+      const float mult = std::is_same_v<T, __half> ? red[row * ld + rp] : 1.f, by = scale * (1.f / mult);  // a power of two
+      const float4 u = *reinterpret_cast<const float4*>(from), v = *reinterpret_cast<const float4*>(from + 4);
+      *reinterpret_cast<uint4*>(static_cast<T*>(out.h) + static_cast<int64_t>(t.y + row) * rp + c) =
+          make_uint4(pack2<T>(u.x * by, u.y * by), pack2<T>(u.z * by, u.w * by), pack2<T>(v.x * by, v.y * by), pack2<T>(v.z * by, v.w * by));
+      if (c == 0) out.mult[t.y + row] = mult;
     }
   }
   if (splits > 1) cluster_sync();  // the others have read this CTA's part
@@ -1032,15 +1057,16 @@ size_t lr_workspace(int64_t M, int64_t K, int64_t N, int rank, int64_t R, bool b
   return M == 0 ? 0 : lr_space(M, K, N, rank, R, backward).total;
 }
 // How many CTAs share a tile's steps, 1, 2, 4 or 8: the fewest rounds of resident CTAs times the steps that each takes, with what a
-// CTA's start and end cost (`extra` steps).
+// CTA's start and end cost (`extra` steps; about what 768 columns do: 97 tiles x 5120 columns go in two parts, 189 and 467 tiles whole,
+// up to 33 tiles in eight).
 static int64_t lr_cost(int64_t tiles, int64_t steps, int64_t parts, int64_t slots, int64_t extra) {
   return ((tiles * parts + slots - 1) / slots) * ((steps + parts - 1) / parts + extra);
 }
-static int lr_splits(int64_t tiles, int64_t chunks, int ctas) {
+static int lr_splits(int64_t tiles, int64_t chunks, int extra, int ctas) {
   const int64_t slots = static_cast<int64_t>(ctas) * cross_sms();
   int best = 1;
   for (int n = 2; n <= 8; n *= 2)
-    if (lr_cost(tiles, chunks, n, slots, 6) < lr_cost(tiles, chunks, best, slots, 6)) best = n;
+    if (lr_cost(tiles, chunks, n, slots, extra) < lr_cost(tiles, chunks, best, slots, extra)) best = n;
   return best;
 }
 template <typename... KA, typename... A>
@@ -1066,9 +1092,9 @@ static bool lr_wide(const void* p, int64_t ld) { return !p || (ld % 16 == 0 && r
 template <typename T, bool W_ROWS, int RPM>
 static int lr_shrink_s(const LrPlan& p, const T* x, int64_t ldx, int64_t C, const T* w, int rank, int rp, int R, const float* scales,
                        const LrHidden& h, cudaStream_t st) {
-  using Cfg = LrShrinkCfg<RPM>;
+  using Cfg = LrShrinkCfg<RPM, W_ROWS>;
   static std::atomic<bool> ready[CA_DEVICES];
-  const int splits = lr_splits(p.n_tiles, (C + 63) / 64, Cfg::CTAS);
+  const int splits = lr_splits(p.n_tiles, (C + Cfg::KC - 1) / Cfg::KC, 768 / Cfg::KC, Cfg::CTAS);
   return lr_launch("lr_shrink_kernel", lr_shrink_kernel<T, W_ROWS, RPM>, ready, dim3(static_cast<unsigned>(p.n_tiles * splits)),
                    LR_SHRINK_THREADS, Cfg::SMEM, splits, st, p, x, ldx, C, w, rank, rp, R, scales, h, splits);
 }
