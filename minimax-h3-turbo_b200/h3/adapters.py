@@ -225,19 +225,28 @@ def _forward(p: _Problem, base, out, want_hidden: bool):
 def _backward(do, x, a, b, pl, hidden, scales, need):
     p = _Problem(x, a, b, pl, scales)
     do = _readable(p.rows(do, p.n, "do"))
-    size = _sizes(p.m, p.k, p.n, p.rank, p.adapters, True)[1]
-    if hidden.shape != (size,) or hidden.dtype != torch.uint8 or hidden.device != p.dev or hidden.data_ptr() % 256 or \
+    m, k, dev = p.m, p.k, p.dev
+    size = _sizes(m, k, p.n, p.rank, p.adapters, True)[1]
+    at = hidden.data_ptr()
+    if at % 256 or hidden.dtype is not torch.uint8 or hidden.dim() != 1 or hidden.shape[0] != size or hidden.device != dev or \
             not hidden.is_contiguous():
-        raise ValueError(f"low_rank: hidden must be what low_rank(..., return_hidden=True) gave, {size} bytes on {p.dev}")
-    dx = torch.empty(p.m, p.k, dtype=p.dt, device=p.dev) if need[0] else None
-    da = torch.empty(p.a.shape, dtype=p.dt, device=p.dev) if need[1] else None
-    db = torch.empty(p.b.shape, dtype=p.dt, device=p.dev) if need[2] else None
-    if any(need):
+        raise ValueError(f"low_rank: hidden must be what low_rank(..., return_hidden=True) gave, {size} bytes on {dev}")
+    dx = da = db = None
+    if need[0]:
+        dx = torch.empty(m, k, dtype=p.dt, device=dev)
+    if need[1]:
+        da = torch.empty_like(p.a)
+    if need[2]:
+        db = torch.empty_like(p.b)
+    if need[0] or need[1] or need[2]:
         p.launch(_lib.lib().h3b_low_rank_backward,
-                 (do.data_ptr(), _ld(do), p.x.data_ptr(), _ld(p.x), p.a.data_ptr(), p.b.data_ptr(), hidden.data_ptr(), _lib.ptr(dx),
-                  p.k, _lib.ptr(da), _lib.ptr(db)), (), True, "low_rank_backward")
-    return (None if dx is None else dx.view(x.shape), None if da is None else da.view(a.shape),
-            None if db is None else db.view(b.shape))
+                 (do.data_ptr(), _ld(do), p.x.data_ptr(), _ld(p.x), p.a.data_ptr(), p.b.data_ptr(), at, _lib.ptr(dx), k,
+                  _lib.ptr(da), _lib.ptr(db)), (), True, "low_rank_backward")
+    if x.dim() != 2 and dx is not None:
+        dx = dx.view(x.shape)
+    if a.dim() != 3:
+        da, db = None if da is None else da[0], None if db is None else db[0]
+    return dx, da, db
 
 
 class _LowRankGrads(torch.autograd.Function):
@@ -320,10 +329,9 @@ def low_rank_backward(do: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: tor
     itself); hidden as low_rank(..., return_hidden=True) gave it for the same arguments; need: which of the three to compute.
     Adapters without rows get zeros.  The same call gives the same bits.  There are no second derivatives."""
     no_tangents("low_rank", do, x, a, b)
-    args = (do, x, a, b, plan, hidden, scales, need)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (do, x, a, b)):
-        return _LowRankGrads.apply(*args)
-    return _backward(*args)
+    if torch.is_grad_enabled() and (do.requires_grad or x.requires_grad or a.requires_grad or b.requires_grad):
+        return _LowRankGrads.apply(do, x, a, b, plan, hidden, scales, need)
+    return _backward(do, x, a, b, plan, hidden, scales, need)
 
 
 def linear(x: torch.Tensor, w: Weight, a: torch.Tensor, b: torch.Tensor, plan: Optional[AdapterPlan] = None,

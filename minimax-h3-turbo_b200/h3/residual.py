@@ -24,10 +24,10 @@ from .types import W4A8Weight, Weight
 
 
 class ResidualNorm(NamedTuple):
-    """What `residual_norm` gives: the stream t, the row factors rsqrt(mean t^2 + eps), and what was asked for (else None)."""
+    """What `residual_norm` gives: the stream t, and what was asked for (else None)."""
 
     x: torch.Tensor                   # [M, K] t
-    rstd: torch.Tensor                # [M] fp32
+    rstd: Optional[torch.Tensor]      # [M] fp32, with hidden: the row factors rsqrt(mean t^2 + eps), which the gradients take
     hidden: Optional[torch.Tensor]    # [M, K] h
     codes: Optional[torch.Tensor]     # [M, K] int8, of h rotated
     scales: Optional[torch.Tensor]    # [M, 1] fp32
@@ -86,6 +86,7 @@ class _Problem:
         if x.dim() != 2 or x.shape[1] % 8 or not 8 <= x.shape[1] <= _lib.MAX_RESIDUAL:
             raise ValueError(f"residual_norm: the stream must be [M, K] with K a multiple of 8 up to {_lib.MAX_RESIDUAL}, got "
                              f"{tuple(x.shape)}")
+        self.shape = x.shape
         self.m, self.k = x.shape
         self.dev, self.dt, self.code = x.device, x.dtype, _lib.act_code(x.dtype)
         if weight.shape != (self.k,) or weight.device != self.dev:
@@ -94,57 +95,67 @@ class _Problem:
         if self.w.data_ptr() % 16:
             self.w = self.w.clone()
         self.w_code = _lib.act_code(self.w.dtype)
-        mods = [t for t in (gate, shift, scale) if t is not None]
-        for t in mods:
-            if t.dim() != 2 or t.shape[1] != self.k or t.shape[0] != mods[0].shape[0] or t.device != self.dev:
+        self.gate, self.shift, self.scale = gate, shift, scale
+        first = gate if gate is not None else shift if shift is not None else scale
+        if first is None:
+            self.mod_args = (0, 0, _lib.BF16, None, 0, None)
+            return
+        n_rows, dt, ld = first.shape[0] if first.dim() == 2 else -1, first.dtype, _ld(first) if first.dim() == 2 else 0
+        alike = True  # read as they are
+        for t in (gate, shift, scale):
+            if t is None:
+                continue
+            if t.dim() != 2 or t.shape[1] != self.k or t.shape[0] != n_rows or t.device != self.dev:
                 raise ValueError(f"residual_norm: gate, shift and scale must be [rows, {self.k}] alike on {self.dev}")
-        self.table, self.n_seg, self.token_rows, self.n_rows = None, 0, None, 0
-        if mods:
-            self.n_rows = mods[0].shape[0]
-            self.table, self.n_seg, self.token_rows = _segments(segments or (), self.m, self.n_rows, self.dev)
-            dt = mods[0].dtype
+            alike = alike and t.dtype is dt and t.is_contiguous() and t.data_ptr() % 16 == 0
+        if not alike:
+            mods = [t for t in (gate, shift, scale) if t is not None]
             if any(t.dtype != dt for t in mods):
-                mods = [t.float() for t in mods]
+                dt, mods = torch.float32, [t.float() for t in mods]
             mods = [_rows(t) for t in mods]
             ld = _ld(mods[0])
             if any(_ld(t) != ld for t in mods):
-                mods = [t.contiguous() for t in mods]
-        it = iter(mods)
-        self.gate, self.shift, self.scale = (None if t is None else next(it) for t in (gate, shift, scale))
-        first = mods[0] if mods else None
-        self.mod_args = (_ld(first), self.n_rows, _code(first), self.table, self.n_seg, _lib.ptr(self.token_rows))
+                mods = [_rows(t.contiguous()) for t in mods]
+                ld = self.k
+            it = iter(mods)
+            self.gate, self.shift, self.scale = (None if t is None else next(it) for t in (gate, shift, scale))
+        table, n_seg, self.token_rows = _segments(segments or (), self.m, n_rows, self.dev)
+        self.mod_args = (ld, n_rows, _lib.act_code(dt), table, n_seg, _lib.ptr(self.token_rows))
 
     def rows(self, t: torch.Tensor, name: str) -> torch.Tensor:
-        if t.shape != (self.m, self.k) or t.dtype != self.dt or t.device != self.dev:
+        if t.shape != self.shape or t.dtype is not self.dt or t.device != self.dev:
             raise ValueError(f"residual_norm: {name} must be {(self.m, self.k)} {self.dt} on {self.dev}, got {tuple(t.shape)} "
                              f"{t.dtype} on {t.device}")
         return _rows(t)
 
     def launch(self, fn, args, backward: bool) -> None:
-        n = _workspace_bytes(self.m, self.k, backward)
+        n, index = _workspace_bytes(self.m, self.k, backward) if backward else 0, self.dev.index
         ws = torch.empty(n, dtype=torch.uint8, device=self.dev) if n else None
-        if self.dev.index == torch.cuda.current_device():
-            rc = fn(*args, _lib.ptr(ws), n, _lib.raw_stream(self.dev.index))
+        if index == torch.cuda.current_device():
+            rc = fn(*args, _lib.ptr(ws), n, _lib.raw_stream(index))
         else:
             with torch.cuda.device(self.dev):
-                rc = fn(*args, _lib.ptr(ws), n, _lib.raw_stream(self.dev.index))
+                rc = fn(*args, _lib.ptr(ws), n, _lib.raw_stream(index))
         if rc:
             _lib.check(rc, "residual_norm")
 
 
 def _forward(p: _Problem, x, y, eps, codes, hidden, out) -> ResidualNorm:
     x, y = p.rows(x, "x"), p.rows(y, "y")
-    m, k = p.m, p.k
-    t = torch.empty(m, k, dtype=p.dt, device=p.dev) if out is None else out
-    h = torch.empty(m, k, dtype=p.dt, device=p.dev) if hidden else None
-    rstd = torch.empty(m, dtype=torch.float32, device=p.dev)
-    q = torch.empty(m, k, dtype=torch.int8, device=p.dev) if codes else None
-    s = torch.empty(m, 1, dtype=torch.float32, device=p.dev) if codes else None
+    m, k, dev = p.m, p.k, p.dev
+    t, ldt = (torch.empty(m, k, dtype=p.dt, device=dev), k) if out is None else (out, _ld(out))
+    h = rstd = q = s = None
+    if hidden:
+        h = torch.empty_like(t, memory_format=torch.contiguous_format)
+        rstd = torch.empty(m, dtype=torch.float32, device=dev)
+    if codes:
+        q = torch.empty(m, k, dtype=torch.int8, device=dev)
+        s = torch.empty(m, 1, dtype=torch.float32, device=dev)
     if m:
+        ptr = _lib.ptr
         p.launch(_lib.lib().h3b_residual_norm,
-                 (x.data_ptr(), _ld(x), y.data_ptr(), _ld(y), p.code, m, k, p.w.data_ptr(), p.w_code, eps, _lib.ptr(p.gate),
-                  _lib.ptr(p.shift), _lib.ptr(p.scale), *p.mod_args, t.data_ptr(), _ld(t), _lib.ptr(h), k, _lib.ptr(q), k,
-                  _lib.ptr(s), rstd.data_ptr()), False)
+                 (x.data_ptr(), _ld(x), y.data_ptr(), _ld(y), p.code, m, k, p.w.data_ptr(), p.w_code, eps, ptr(p.gate),
+                  ptr(p.shift), ptr(p.scale), *p.mod_args, t.data_ptr(), ldt, ptr(h), k, ptr(q), k, ptr(s), ptr(rstd)), False)
     return ResidualNorm(t, rstd, h, q, s)
 
 
@@ -152,11 +163,11 @@ def _backward(dt, dh, t, rstd, weight, gate, scale, segments, need_w):
     p = _Problem(t, weight, gate, None, scale, segments)
     t, dh = p.rows(t, "x"), p.rows(dh, "dh")
     dt = None if dt is None else p.rows(dt, "dt")
-    if rstd.shape != (p.m,) or rstd.dtype != torch.float32 or rstd.device != p.dev:
-        raise ValueError(f"residual_norm: rstd must be fp32 [{p.m}] on {p.dev}")
+    if rstd is None or rstd.shape != (p.m,) or rstd.dtype != torch.float32 or rstd.device != p.dev:
+        raise ValueError(f"residual_norm: rstd must be fp32 [{p.m}] on {p.dev} (residual_norm gives it with hidden=True)")
     rstd = rstd.contiguous()
     dx = torch.empty(p.m, p.k, dtype=p.dt, device=p.dev)
-    dy = torch.empty_like(dx) if p.gate is not None else dx
+    dy = torch.empty_like(dx) if gate is not None else dx
     dw = torch.empty(p.k, dtype=p.w.dtype, device=p.dev) if need_w else None
     if p.m or need_w:
         p.launch(_lib.lib().h3b_residual_norm_backward,
@@ -201,7 +212,8 @@ class _ResidualNorm(torch.autograd.Function):
 
 
 def _constants(gate, shift, scale) -> None:
-    if any(t is not None and t.requires_grad for t in (gate, shift, scale)):
+    if (gate is not None and gate.requires_grad) or (shift is not None and shift.requires_grad) or \
+            (scale is not None and scale.requires_grad):
         raise ValueError("residual_norm: gate, shift and scale have no gradient; detach them")
 
 
@@ -258,12 +270,11 @@ def residual_norm_backward(dt: Optional[torch.Tensor], dh: torch.Tensor, t: torc
     """Gradients (dx, dy, dweight) of residual_norm from those of its x (dt, None: zeros) and hidden (dh); t and rstd as it gave
     them for the same arguments.  Without a gate dy is dx itself.  The same call gives the same bits.  No second derivatives."""
     no_tangents("residual_norm", dt, dh, t, weight, gate, scale)
-    args = (dt, dh, t, rstd, weight, gate, scale, segments, need_weight)
     if torch.is_grad_enabled():
         _constants(gate, None, scale)
-        if any(v is not None and v.requires_grad for v in (dt, dh, t, weight)):
-            return _ResidualNormGrads.apply(*args)
-    return _backward(*args)
+        if (dt is not None and dt.requires_grad) or dh.requires_grad or t.requires_grad or weight.requires_grad:
+            return _ResidualNormGrads.apply(dt, dh, t, rstd, weight, gate, scale, segments, need_weight)
+    return _backward(dt, dh, t, rstd, weight, gate, scale, segments, need_weight)
 
 
 def linear(r: ResidualNorm, w: Weight, bias: Optional[torch.Tensor] = None, *, quant_mode: str = "ck") -> torch.Tensor:

@@ -224,7 +224,7 @@ def test_refusals():
         rs.residual_norm(buf[:8192].view(16, 512), y, w, EPS, out=buf[512:].view(16, 512))
     with pytest.raises(ValueError, match="gradients"):
         rs.residual_norm(x.clone().requires_grad_(), y, w, EPS)
-    r = rs.residual_norm(x, y, w, EPS, codes=False)
+    r = rs.residual_norm(x, y, w, EPS, codes=False, hidden=True)
     with pytest.raises(ValueError, match="rstd"):
         rs.residual_norm_backward(x, y, r.x, r.rstd[:4], w)
     xr = x.clone().requires_grad_()
