@@ -10,33 +10,45 @@
 //
 // HBM-bound: x and y are read and t and the codes written once, 7 bytes a channel (9 with h; the gradients 8 or 10).  A thread has 16
 // channels of two rows (or 16 and 16 of one row, SPLIT, where a row is long), the halves of packed fp32 instructions, from their
-// arrival to their codes: the rotation's four butterfly digits are two in registers and two over the 16 threads of a block (through
-// shared memory, as in rotq.cuh).  CTAs are persistent; while rows are worked on, the next ones come into shared memory as bulk copies
-// of whole rows (held in registers instead, they left room for 10 warps to an SM: 763 us for 59440 x 5120 into codes).  w, gate,
-// scale and shift come from L1 every time: 4 bytes a channel and pair of rows.
+// arrival to their codes.  16 threads have a block of 256: four times 4 channels each, 64 apart, so that every access of theirs is 128
+// bytes in a row (16 channels in a row to a thread: 502 us where this takes 448, 59440 x 5120 into codes; the floor is 326).  The
+// rotation's four butterfly digits are then two in registers and two over the 16 threads, through shared memory as in rotq.cuh.  The
+// gradients need no rotation and have twice 8 channels, 128 apart (four times 4: 160 us where this takes 130, 12090 x 5376).  CTAs are
+// persistent; while rows are worked on, the next ones come into shared memory as bulk copies of whole rows (held in registers instead,
+// they left room for 10 warps to an SM: 763 us).  What is left above the floor is the work itself: some 29 instructions a channel at
+// 20 warps to an SM (30 warps of 64 registers spill: 580 us).  w, gate, scale and shift come from L1 every time: 4 bytes a channel
+// and pair of rows.
 #pragma once
 #include <atomic>
+#include <type_traits>
 
 #include "rotq.cuh"
 
 namespace h3b {
 
-template <int DT>
-__device__ __forceinline__ void rn_unpack(const uint4& u, float (&f)[8]) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+// W channels of the stream's type, 4 or 8, that one load brings
+template <int W>
+using RnWord = std::conditional_t<W == 4, uint2, uint4>;
+template <int DT, int W>
+__device__ __forceinline__ void rn_unpack(const RnWord<W>& u, float (&f)[W]) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(&u);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < W / 2; ++i) {
     const float2 v = unpack2<DT>(w[i]);
     f[2 * i] = v.x, f[2 * i + 1] = v.y;
   }
 }
-template <int DT>
-__device__ __forceinline__ uint4 rn_pack(const float (&f)[8]) {
-  return make_uint4(pack2<DT>(make_float2(f[0], f[1])), pack2<DT>(make_float2(f[2], f[3])), pack2<DT>(make_float2(f[4], f[5])),
-                    pack2<DT>(make_float2(f[6], f[7])));
+template <int DT, int W>
+__device__ __forceinline__ RnWord<W> rn_pack(const float (&f)[W]) {
+  RnWord<W> u;
+  uint32_t* w = reinterpret_cast<uint32_t*>(&u);
+#pragma unroll
+  for (int i = 0; i < W / 2; ++i) w[i] = pack2<DT>(make_float2(f[2 * i], f[2 * i + 1]));
+  return u;
 }
-__device__ __forceinline__ uint4 rn_load(const unsigned char* p, bool ok) {
-  return ok ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
+template <int W>
+__device__ __forceinline__ RnWord<W> rn_load(const unsigned char* p, bool ok) {
+  return ok ? *reinterpret_cast<const RnWord<W>*>(p) : RnWord<W>{};
 }
 __device__ __forceinline__ void rn_bulk(void* dst, const void* src, int bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
@@ -48,14 +60,23 @@ template <bool FAST>
 __device__ __forceinline__ const char* rn_param_at(const void* p, int64_t at, int dt) {
   return static_cast<const char*>(p) + (FAST || dt != H3B_FP32 ? 2 : 4) * at;
 }
-// 8 numbers, the k-th 8 from there
-template <int DT, bool FAST>
-__device__ __forceinline__ void rn_param(const char* p, int k, int dt, bool ok, float (&f)[8]) {
+// The k-th W numbers of a thread from there: 16 W apart
+template <int DT, bool FAST, int W>
+__device__ __forceinline__ void rn_param(const char* p, int k, int dt, bool ok, float (&f)[W]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = 0.f;
+  for (int i = 0; i < W; ++i) f[i] = 0.f;
   if (!ok) return;
-  if constexpr (FAST) load8(p, 8 * k, DT == DT_BF16 ? H3B_BF16 : H3B_FP16, f);
-  else load8(p, 8 * k, dt, f);
+  if (!FAST && dt == H3B_FP32) {
+#pragma unroll
+    for (int i = 0; i < W; i += 4) {
+      const float4 u = __ldg(reinterpret_cast<const float4*>(p + 64 * W * k) + i / 4);
+      f[i] = u.x, f[i + 1] = u.y, f[i + 2] = u.z, f[i + 3] = u.w;
+    }
+  } else {
+    const RnWord<W> u = __ldg(reinterpret_cast<const RnWord<W>*>(p + 32 * W * k));
+    if (FAST || dt == (DT == DT_BF16 ? H3B_BF16 : H3B_FP16)) rn_unpack<DT, W>(u, f);
+    else rn_unpack<DT == DT_BF16 ? DT_FP16 : DT_BF16, W>(u, f);
+  }
 }
 __device__ __forceinline__ int rn_mod_row(const ResNormArgs& a, int64_t row) {
   int m = -1;
@@ -73,20 +94,44 @@ __device__ __forceinline__ int rn_mod_row(const ResNormArgs& a, int64_t row) {
 __device__ __forceinline__ char* rn_at(const void* p, int64_t row, int64_t ld, int col) {
   return static_cast<char*>(const_cast<void*>(p)) + 2 * (row * ld + col);
 }
-// A row's sum: every 16 threads leave theirs in `part`; behind the barrier (the CTA's) every 16 threads add up the row's n <= 32.
 __device__ __forceinline__ float rn_sum16(float v) {
 #pragma unroll
   for (int o = 8; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-__device__ __forceinline__ float2 rn_sum(float2 v, float2* part, int mine, int first, int n) {
-  const int t = threadIdx.x & 15;
-  v = make_float2(rn_sum16(v.x), rn_sum16(v.y));
-  if (t == 0) part[mine] = v;
+// Sums (or largest numbers) of two rows: every 16 threads leave theirs in `part`; behind the barrier (the CTA's) every 16 threads add
+// up the rows' n <= 32.  Threads 0-7 of the 16 have the first row, 8-15 the second.
+template <typename N, typename N2, typename F>
+__device__ __forceinline__ N2 rn_over_rows(N2 v, N2* part, int mine, int first, int n, F&& f) {
+  const int t = threadIdx.x & 7, up = (threadIdx.x >> 3) & 1;
+  auto eight = [&](N w) {
+#pragma unroll
+    for (int o = 4; o; o >>= 1) w = f(w, __shfl_xor_sync(0xffffffffu, w, o));
+    return w;
+  };
+  N* const flat = reinterpret_cast<N*>(part);
+  const N s = eight(f(up ? v.y : v.x, __shfl_xor_sync(0xffffffffu, up ? v.x : v.y, 8)));
+  if (t == 0) flat[2 * mine + up] = s;
   __syncthreads();
-  const float2 lo = t < n ? part[first + t] : make_float2(0.f, 0.f);
-  const float2 hi = t + 16 < n ? part[first + 16 + t] : make_float2(0.f, 0.f);
-  return make_float2(rn_sum16(lo.x + hi.x), rn_sum16(lo.y + hi.y));
+  N w = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (t + 8 * i < n) w = f(w, flat[2 * (first + t + 8 * i) + up]);
+  w = eight(w);
+  const N other = __shfl_xor_sync(0xffffffffu, w, 8);
+  N2 out;
+  out.x = up ? other : w, out.y = up ? w : other;
+  return out;
+}
+
+// Four codes: rounded to the nearest, saturated, the first in the lowest byte
+__device__ __forceinline__ uint32_t rn_codes(float x0, float x1, float x2, float x3) {
+  uint32_t c;
+  asm("{\n\t.reg .s32 k0, k1, k2, k3;\n\t.reg .b32 up;\n\tcvt.rni.s32.f32 k0, %1;\n\tcvt.rni.s32.f32 k1, %2;\n\t"
+      "cvt.rni.s32.f32 k2, %3;\n\tcvt.rni.s32.f32 k3, %4;\n\tcvt.pack.sat.s8.s32.b32 up, k3, k2, 0;\n\t"
+      "cvt.pack.sat.s8.s32.b32 %0, k1, k0, up;\n\t}"
+      : "=r"(c) : "f"(x0), "f"(x1), "f"(x2), "f"(x3));
+  return c;
 }
 
 // What a launch is made of: groups of T threads, G to a CTA (rounded up to whole warps); a group has two rows, or one (SPLIT: its lanes'
@@ -105,10 +150,11 @@ __host__ __device__ inline int rn_group_bytes(int K, bool split) { return (split
 
 template <int DT, bool CODES, bool FAST, bool SPLIT, bool WIDE>
 __global__ void __launch_bounds__(WIDE ? 512 : RN_THREADS, WIDE ? 1 : 2) resnorm_kernel(const ResNormArgs a, const RnShape s) {
+  constexpr int W = 4, PIECES = 16 / W;  // with or without codes, so that the sums are the same
   extern __shared__ __align__(128) unsigned char rn_smem[];
   const int tid = threadIdx.x, T = s.T, G = s.G, unit = tid / T, tr = tid - unit * T, K = a.K;
   const int half = tid >> 4, halves = blockDim.x >> 4, t16 = tid & 15, parts = unit < G ? T >> 4 : 0, first = unit * parts;
-  const int col[2] = {16 * tr, 16 * tr + (SPLIT ? s.off : 0)};
+  const int col[2] = {(tr & ~15) * 16 + W * t16, (tr & ~15) * 16 + W * t16 + (SPLIT ? s.off : 0)};  // and PIECES times 16 W further
   uint64_t* const bar = reinterpret_cast<uint64_t*>(rn_smem);
   volatile int* const abort = reinterpret_cast<volatile int*>(rn_smem + 8);
   float2* const part = reinterpret_cast<float2*>(rn_smem + RN_HEAD);
@@ -146,7 +192,7 @@ __global__ void __launch_bounds__(WIDE ? 512 : RN_THREADS, WIDE ? 1 : 2) resnorm
       }
   };
   if (leads) bring(r0);
-  const bool mods = FAST && a.gate && a.scale;
+  const bool mods = FAST && a.gate && a.scale && K % 256 == 0 && unit < G;
   const float over_k = 1.f / static_cast<float>(K);
   uint32_t turn = 0;
   for (int64_t base = static_cast<int64_t>(blockIdx.x) * G; base < groups; base += step, r0 += ROWS * step, turn ^= 1) {
@@ -155,79 +201,59 @@ __global__ void __launch_bounds__(WIDE ? 512 : RN_THREADS, WIDE ? 1 : 2) resnorm
     const int2 both = *rows_of;
     const int mrow[2] = {both.x, both.y};
     const bool same = !SPLIT && mrow[0] == mrow[1];  // one load of a modulation row serves both lanes
-    // the ordinary case by itself, without a branch inside: rows of one segment (of codes: 16 channels to every thread that has any)
-    const bool plain = CODES && mods && same && mrow[0] >= 0 && unit < G;
-    const int64_t mod0 = 2 * (mrow[0] * a.ldm + col[0]);  // bytes into gate, scale and shift
+    // the ordinary case by itself, without a branch inside: modulation rows of the stream's type, 16 channels and 16 to every thread
+    const bool plain = mods && mrow[0] >= 0 && (SPLIT ? n[1] > 0 : same);
     mbar_wait(bar, turn, abort);
     // ---- the stream
     float2 v[16], ss = make_float2(0.f, 0.f);
-    if (plain) {
-      const unsigned char* at = mine + 2 * col[0];
-      char* const to = rn_at(a.t, row[0], a.ldt, col[0]);
-      const int64_t next = row[1] < a.M ? 2 * a.ldt : 0;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        float g[8], f[8], y[8];
-        load8(static_cast<const char*>(a.gate) + mod0, 8 * k, DT == DT_BF16 ? H3B_BF16 : H3B_FP16, g);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          rn_unpack<DT>(*reinterpret_cast<const uint4*>(at + h * 4 * K + 16 * k), f);
-          rn_unpack<DT>(*reinterpret_cast<const uint4*>(at + h * 4 * K + 2 * K + 16 * k), y);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = fmaf(y[i], g[i], f[i]);  // the product of two numbers of 16 bits is exact
-          const uint4 t = rn_pack<DT>(f);
-          if (h == 0 || next) *reinterpret_cast<uint4*>(to + h * next + 16 * k) = t;
-          rn_unpack<DT>(t, f);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if (h == 0) v[8 * k + i].x = f[i];
-            else v[8 * k + i].y = f[i];
-          }
-        }
-      }
-    } else {
+    auto stream = [&](auto is_plain) {
+      constexpr bool P = decltype(is_plain)::value;
+      const unsigned char* at[2];
       const char* pg[2];
       char* to[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
+        at[h] = mine + (SPLIT ? 0 : h) * 4 * K + 2 * col[h];
         pg[h] = rn_param_at<FAST>(a.gate, mrow[h] * a.ldm + col[h], a.m_dtype);
         to[h] = rn_at(a.t, row[h], a.ldt, col[h]);
       }
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {  // 8 channels at a time
-        float p[8];
+      for (int k = 0; k < PIECES; ++k) {  // W channels at a time
+        float p[W];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          float f[8], y[8];
-          const bool ok = n[h] > 8 * k;
-          const unsigned char* at = mine + (SPLIT ? 0 : h) * 4 * K + 2 * col[h] + 16 * k;
-          rn_unpack<DT>(rn_load(at, ok), f);
-          rn_unpack<DT>(rn_load(at + 2 * K, ok), y);
-          if (a.gate) {
-            if (mrow[h] >= 0) {
-              if (h == 0 || !same) rn_param<DT, FAST>(pg[h], k, a.m_dtype, ok, p);
+          float f[W], y[W];
+          const bool ok = P || n[h] > 16 * W * k;
+          rn_unpack<DT, W>(rn_load<W>(at[h] + 32 * W * k, ok), f);
+          rn_unpack<DT, W>(rn_load<W>(at[h] + 2 * K + 32 * W * k, ok), y);
+          if (P || a.gate) {
+            if (P || mrow[h] >= 0) {
+              if (h == 0 || SPLIT || !(P || same)) rn_param<DT, FAST, W>(pg[h], k, a.m_dtype, ok, p);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) f[i] = __fadd_rn(f[i], __fmul_rn(y[i], p[i]));
+              for (int i = 0; i < W; ++i)  // P: the product of two numbers of 16 bits is exact
+                f[i] = P ? fmaf(y[i], p[i], f[i]) : __fadd_rn(f[i], __fmul_rn(y[i], p[i]));
             }
           } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = __fadd_rn(f[i], y[i]);
+            for (int i = 0; i < W; ++i) f[i] = __fadd_rn(f[i], y[i]);
           }
-          const uint4 t = rn_pack<DT>(f);
-          if (ok) *reinterpret_cast<uint4*>(to[h] + 16 * k) = t;
-          rn_unpack<DT>(t, f);
+          const RnWord<W> t = rn_pack<DT, W>(f);
+          if (P ? n[h] > 0 : ok) *reinterpret_cast<RnWord<W>*>(to[h] + 32 * W * k) = t;
+          rn_unpack<DT, W>(t, f);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if (h == 0) v[8 * k + i].x = f[i];
-            else v[8 * k + i].y = f[i];
+          for (int i = 0; i < W; ++i) {
+            if (h == 0) v[W * k + i].x = f[i];
+            else v[W * k + i].y = f[i];
           }
         }
       }
-    }
+    };
+    if (plain) stream(std::true_type{});
+    else stream(std::false_type{});
 #pragma unroll
     for (int i = 0; i < 16; ++i) ss = __ffma2_rn(v[i], v[i], ss);
     if (SPLIT) ss.x = ss.y = ss.x + ss.y;
-    ss = rn_sum(ss, part, half, first, parts);
+    ss = rn_over_rows<float>(ss, part, half, first, parts, [](float b, float c) { return b + c; });
     // everyone has read the rows: the next ones may come
     if (leads && base + step < groups) bring(r0 + ROWS * step), find(r0 + ROWS * step);
     const float2 rs = make_float2(rsqrtf(fmaf(ss.x, over_k, a.eps)), rsqrtf(fmaf(ss.y, over_k, a.eps)));
@@ -236,58 +262,46 @@ __global__ void __launch_bounds__(WIDE ? 512 : RN_THREADS, WIDE ? 1 : 2) resnorm
       if (!SPLIT && row[1] < a.M) a.rstd[row[1]] = rs.y;
     }
     // ---- the norm and its modulation
-    if (plain && !a.h) {
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        float p[8], u[8], q[8];
-        load8(a.w, col[0] + 8 * k, DT == DT_BF16 ? H3B_BF16 : H3B_FP16, p);
-        load8(static_cast<const char*>(a.scale) + mod0, 8 * k, DT == DT_BF16 ? H3B_BF16 : H3B_FP16, u);
-        load8(static_cast<const char*>(a.shift) + mod0, 8 * k, DT == DT_BF16 ? H3B_BF16 : H3B_FP16, q);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float c = 1.f + u[i];
-          float2& z = v[8 * k + i];
-          z = __fmul2_rn(__fmul2_rn(z, rs), make_float2(p[i], p[i]));
-          z = __ffma2_rn(z, make_float2(c, c), make_float2(q[i], q[i]));
-        }
-      }
-    } else {
+    auto norm = [&](auto is_plain) {
+      constexpr bool P = decltype(is_plain)::value;
       const char *pw[2], *ps[2], *pt[2];
+      char* to[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         pw[h] = rn_param_at<FAST>(a.w, col[h], a.w_dtype);
         ps[h] = rn_param_at<FAST>(a.scale, mrow[h] * a.ldm + col[h], a.m_dtype);
         pt[h] = rn_param_at<FAST>(a.shift, mrow[h] * a.ldm + col[h], a.m_dtype);
+        to[h] = rn_at(a.h, row[h], a.ldh, col[h]);
       }
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        float p[8], q[8];
-        rn_param<DT, FAST>(pw[0], k, a.w_dtype, unit < G && K - col[0] > 8 * k, p);
-        if (SPLIT) rn_param<DT, FAST>(pw[1], k, a.w_dtype, unit < G && K - col[1] > 8 * k, q);
+      for (int k = 0; k < PIECES; ++k) {
+        float p[W], q[W];
+        rn_param<DT, FAST, W>(pw[0], k, a.w_dtype, P || (unit < G && K - col[0] > 16 * W * k), p);
+        if (SPLIT) rn_param<DT, FAST, W>(pw[1], k, a.w_dtype, P || (unit < G && K - col[1] > 16 * W * k), q);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          v[8 * k + i] = __fmul2_rn(__fmul2_rn(v[8 * k + i], rs), make_float2(p[i], SPLIT ? q[i] : p[i]));
-        if (a.scale) {
-          if (same) {
-            if (mrow[0] >= 0) {
-              rn_param<DT, FAST>(ps[0], k, a.m_dtype, n[0] > 8 * k, p);
-              rn_param<DT, FAST>(pt[0], k, a.m_dtype, n[0] > 8 * k, q);
+        for (int i = 0; i < W; ++i)
+          v[W * k + i] = __fmul2_rn(__fmul2_rn(v[W * k + i], rs), make_float2(p[i], SPLIT ? q[i] : p[i]));
+        if (P || a.scale) {
+          if (!SPLIT && (P || same)) {
+            if (P || mrow[0] >= 0) {
+              rn_param<DT, FAST, W>(ps[0], k, a.m_dtype, P || n[0] > 16 * W * k, p);
+              rn_param<DT, FAST, W>(pt[0], k, a.m_dtype, P || n[0] > 16 * W * k, q);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
+              for (int i = 0; i < W; ++i) {
                 const float u = 1.f + p[i];
-                v[8 * k + i] = __ffma2_rn(v[8 * k + i], make_float2(u, u), make_float2(q[i], q[i]));
+                v[W * k + i] = __ffma2_rn(v[W * k + i], make_float2(u, u), make_float2(q[i], q[i]));
               }
             }
           } else {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              if (mrow[h] < 0) continue;
-              rn_param<DT, FAST>(ps[h], k, a.m_dtype, n[h] > 8 * k, p);
-              rn_param<DT, FAST>(pt[h], k, a.m_dtype, n[h] > 8 * k, q);
+              if (!P && mrow[h] < 0) continue;
+              rn_param<DT, FAST, W>(ps[h], k, a.m_dtype, P || n[h] > 16 * W * k, p);
+              rn_param<DT, FAST, W>(pt[h], k, a.m_dtype, P || n[h] > 16 * W * k, q);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                if (h == 0) v[8 * k + i].x = fmaf(v[8 * k + i].x, 1.f + p[i], q[i]);
-                else v[8 * k + i].y = fmaf(v[8 * k + i].y, 1.f + p[i], q[i]);
+              for (int i = 0; i < W; ++i) {
+                if (h == 0) v[W * k + i].x = fmaf(v[W * k + i].x, 1.f + p[i], q[i]);
+                else v[W * k + i].y = fmaf(v[W * k + i].y, 1.f + p[i], q[i]);
               }
             }
           }
@@ -296,14 +310,16 @@ __global__ void __launch_bounds__(WIDE ? 512 : RN_THREADS, WIDE ? 1 : 2) resnorm
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) p[i] = h == 0 ? v[8 * k + i].x : v[8 * k + i].y;
-            if (n[h] > 8 * k) *reinterpret_cast<uint4*>(rn_at(a.h, row[h], a.ldh, col[h] + 8 * k)) = rn_pack<DT>(p);
+            for (int i = 0; i < W; ++i) p[i] = h == 0 ? v[W * k + i].x : v[W * k + i].y;
+            if (n[h] > (P ? 0 : 16 * W * k)) *reinterpret_cast<RnWord<W>*>(to[h] + 32 * W * k) = rn_pack<DT, W>(p);
           }
         }
       }
-    }
+    };
+    if (plain) norm(std::true_type{});
+    else norm(std::false_type{});
     if constexpr (CODES) {
-      // ---- the rotation: digits d0, d1 in registers, d2, d3 over the block's 16 threads
+      // ---- the rotation: digits d0, d3 in registers, d1, d2 over the block's 16 threads; then thread 4 d3 + d0 has number d1 + 4 d2
 #pragma unroll
       for (int i = 0; i < 4; ++i) h4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], 1.0f);
 #pragma unroll
@@ -326,23 +342,8 @@ __global__ void __launch_bounds__(WIDE ? 512 : RN_THREADS, WIDE ? 1 : 2) resnorm
       for (int i = 0; i < 16; i += 2) m.x = max3f(m.x, fabsf(v[i].x), fabsf(v[i + 1].x)), m.y = max3f(m.y, fabsf(v[i].y), fabsf(v[i + 1].y));
       uint2 top = make_uint2(max(__float_as_uint(m.x), __float_as_uint(v[0].x) & 0x7FFFFFFFu),
                              max(__float_as_uint(m.y), __float_as_uint(v[0].y) & 0x7FFFFFFFu));
-      if (SPLIT) top.x = max(top.x, top.y);
-      auto top16 = [&] {
-#pragma unroll
-        for (int o = 8; o; o >>= 1) {
-          top.x = max(top.x, __shfl_xor_sync(0xffffffffu, top.x, o));
-          if (!SPLIT) top.y = max(top.y, __shfl_xor_sync(0xffffffffu, top.y, o));
-        }
-      };
-      top16();
-      if (t16 == 0) tops[half] = top;
-      __syncthreads();
-      {
-        const uint2 lo = t16 < parts ? tops[first + t16] : make_uint2(0u, 0u), hi = t16 + 16 < parts ? tops[first + 16 + t16] : make_uint2(0u, 0u);
-        top = make_uint2(max(lo.x, hi.x), max(lo.y, hi.y));
-      }
-      top16();
-      if (SPLIT) top.y = top.x;
+      if (SPLIT) top.x = top.y = max(top.x, top.y);
+      top = rn_over_rows<uint32_t>(top, tops, half, first, parts, [](uint32_t b, uint32_t c) { return max(b, c); });
       const float2 amax = make_float2(__uint_as_float(top.x), __uint_as_float(top.y));
       if (leads) {
         if (row[0] < a.M) a.scales[row[0]] = __fdiv_rn(amax.x, 127.f);
@@ -351,30 +352,33 @@ __global__ void __launch_bounds__(WIDE ? 512 : RN_THREADS, WIDE ? 1 : 2) resnorm
       // ---- codes: 0 for rows of zeros and rows without a finite largest magnitude
       const float2 inv = make_float2(amax.x > 0.f && amax.x < INFINITY ? fminf(__fdiv_rn(127.f, amax.x), 3e38f) : 0.f,
                                      amax.y > 0.f && amax.y < INFINITY ? fminf(__fdiv_rn(127.f, amax.y), 3e38f) : 0.f);
-      unsigned char* const cbuf = reinterpret_cast<unsigned char*>(gbuf);  // 16 chunks of 16 byte pairs, CSTRIDE apart
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float2 q = __fmul2_rn(v[i], inv);
-        uint32_t c;
-        asm("{\n\t.reg .s32 k0, k1;\n\tcvt.rni.s32.f32 k0, %1;\n\tcvt.rni.s32.f32 k1, %2;\n\t"
-            "cvt.pack.sat.s8.s32.b32 %0, k1, k0, 0;\n\t}"
-            : "=r"(c) : "f"(q.x), "f"(q.y));
-        *reinterpret_cast<uint16_t*>(cbuf + i * CSTRIDE + 2 * t16) = static_cast<uint16_t>(c);  // element t + 16 i of the block
-      }
-      __syncwarp();
-      const uint4* rd = reinterpret_cast<const uint4*>(cbuf + t16 * CSTRIDE);
-      const uint4 u0 = rd[0], u1 = rd[1];
-      const uint32_t w8[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
-      uint32_t o[2][4];
+      // a thread's 16 codes of a row, channels 64 d3 + d0 + 4 i, as four words; every four threads change words to have 16 channels
+      // that follow one another (lines of 4 threads are 16 bytes further apart, which keeps the reads off each other's banks)
+      unsigned char* const cbuf = reinterpret_cast<unsigned char*>(gbuf);
+      uint32_t c[2][4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        o[0][i] = __byte_perm(w8[2 * i], w8[2 * i + 1], 0x6420);
-        o[1][i] = __byte_perm(w8[2 * i], w8[2 * i + 1], 0x7531);
+        float2 q[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) q[j] = __fmul2_rn(v[4 * i + j], inv);
+        c[0][i] = rn_codes(q[0].x, q[1].x, q[2].x, q[3].x), c[1][i] = rn_codes(q[0].y, q[1].y, q[2].y, q[3].y);
       }
-      __syncwarp();
+      const int line = 80 * (t16 >> 2);
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        if (n[h] > 0) *reinterpret_cast<uint4*>(a.codes + row[h] * a.ldc + col[h]) = make_uint4(o[h][0], o[h][1], o[h][2], o[h][3]);
+        *reinterpret_cast<uint4*>(cbuf + 320 * h + line + 16 * (t16 & 3)) = make_uint4(c[h][0], c[h][1], c[h][2], c[h][3]);
+      __syncwarp();
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c[h][j] = *reinterpret_cast<const uint32_t*>(cbuf + 320 * h + line + 16 * j + 4 * (t16 & 3));
+        const uint32_t a0 = __byte_perm(c[h][0], c[h][1], 0x5140), a1 = __byte_perm(c[h][0], c[h][1], 0x7362);
+        const uint32_t b0 = __byte_perm(c[h][2], c[h][3], 0x5140), b1 = __byte_perm(c[h][2], c[h][3], 0x7362);
+        if (n[h] > 0)
+          *reinterpret_cast<uint4*>(a.codes + row[h] * a.ldc + 16 * tr + (SPLIT && h ? s.off : 0)) =
+              make_uint4(__byte_perm(a0, b0, 0x5410), __byte_perm(a0, b0, 0x7632), __byte_perm(a1, b1, 0x5410), __byte_perm(a1, b1, 0x7632));
+      }
+      __syncwarp();
     } else {
       __syncthreads();  // the next rows' sums
     }
@@ -388,10 +392,11 @@ constexpr int RN_GRAD_THREADS = 384;  // of a row that is not split, with 80 reg
 template <int DT, bool FAST, bool SPLIT>
 __global__ void __launch_bounds__(SPLIT ? 512 : RN_GRAD_THREADS, SPLIT ? 1 : 2) resnorm_grad_kernel(const ResNormArgs a, const RnShape s,
                                                                                            float* dw) {
-  constexpr int L = SPLIT ? 2 : 1;
+  constexpr int L = SPLIT ? 2 : 1, W = 8, PIECES = 16 / W;
   extern __shared__ __align__(128) unsigned char rn_smem[];
   const int tid = threadIdx.x, T = s.T, G = s.G, unit = tid / T, tr = tid - unit * T, K = a.K;
   const int half = tid >> 4, halves = blockDim.x >> 4, parts = unit < G ? T >> 4 : 0, first = unit * parts;
+  const int col0 = (tr & ~15) * 16 + W * (tid & 15);
   uint64_t* const bars = reinterpret_cast<uint64_t*>(rn_smem);  // three
   volatile int* const abort = reinterpret_cast<volatile int*>(rn_smem + 24);
   float* const part = reinterpret_cast<float*>(rn_smem + RN_HEAD);  // two rows' sums in turn: one barrier a row
@@ -420,6 +425,7 @@ __global__ void __launch_bounds__(SPLIT ? 512 : RN_GRAD_THREADS, SPLIT ? 1 : 2) 
   if (leads)
     for (int i = 0; i < s.ahead - 1 && i < left; ++i) bring(r + i * step, i);
   const float over_k = 1.f / static_cast<float>(K);
+  const bool mods = FAST && a.dy && a.scale && K % 256 == 0 && unit < G;
   float sum[L][16];
 #pragma unroll
   for (int l = 0; l < L; ++l)
@@ -433,33 +439,42 @@ __global__ void __launch_bounds__(SPLIT ? 512 : RN_GRAD_THREADS, SPLIT ? 1 : 2) 
     mbar_wait(bars + buf, phase, abort);
     const unsigned char* const at = mine + buf * bytes;
     float g[L][16], x[L][16], dot = 0.f;
+    // the ordinary case by itself, as above
+    const bool plain = mods && mrow >= 0 && (!SPLIT || col0 + s.off < K);
+    auto dots = [&](auto is_plain) {
+      constexpr bool P = decltype(is_plain)::value;
 #pragma unroll
-    for (int l = 0; l < L; ++l) {
+      for (int l = 0; l < L; ++l) {
+        const int col = col0 + l * s.off;
+        const char* const ps = rn_param_at<FAST>(a.scale, mrow * a.ldm + col, a.m_dtype);
+        const char* const pw = rn_param_at<FAST>(a.w, col, a.w_dtype);
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int col = 16 * tr + l * s.off + 8 * k;
-        const bool ok = r < a.M && col < K;
-        float p[8], f[8];
-        rn_unpack<DT>(rn_load(at + 2 * col, ok), f);
-        if (a.scale && mrow >= 0) {
-          rn_param<DT, FAST>(rn_param_at<FAST>(a.scale, mrow * a.ldm + col, a.m_dtype), 0, a.m_dtype, ok, p);
+        for (int k = 0; k < PIECES; ++k) {
+          const bool ok = P || (r < a.M && col + 16 * W * k < K);
+          float p[W], f[W];
+          rn_unpack<DT, W>(rn_load<W>(at + 2 * col + 32 * W * k, ok), f);
+          if (P || (a.scale && mrow >= 0)) {
+            rn_param<DT, FAST, W>(ps, k, a.m_dtype, ok, p);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] *= 1.f + p[i];
-        }
+            for (int i = 0; i < W; ++i) f[i] *= 1.f + p[i];
+          }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) g[l][8 * k + i] = f[i];
-        rn_unpack<DT>(rn_load(at + 2 * K + 2 * col, ok), f);
-        rn_param<DT, FAST>(rn_param_at<FAST>(a.w, col, a.w_dtype), 0, a.w_dtype, ok, p);
+          for (int i = 0; i < W; ++i) g[l][W * k + i] = f[i];
+          rn_unpack<DT, W>(rn_load<W>(at + 2 * K + 2 * col + 32 * W * k, ok), f);
+          rn_param<DT, FAST, W>(pw, k, a.w_dtype, ok, p);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int e = 8 * k + i;
-          x[l][e] = f[i] * rs;
-          sum[l][e] = fmaf(g[l][e], x[l][e], sum[l][e]);
-          g[l][e] *= p[i];
-          dot = fmaf(g[l][e], x[l][e], dot);
+          for (int i = 0; i < W; ++i) {
+            const int e = W * k + i;
+            x[l][e] = f[i] * rs;
+            sum[l][e] = fmaf(g[l][e], x[l][e], sum[l][e]);
+            g[l][e] *= p[i];
+            dot = fmaf(g[l][e], x[l][e], dot);
+          }
         }
       }
-    }
+    };
+    if (plain) dots(std::true_type{});
+    else dots(std::false_type{});
     dot = rn_sum16(dot);
     float* const here = part + (k & 1) * halves;
     if ((tid & 15) == 0) here[half] = dot;
@@ -469,36 +484,46 @@ __global__ void __launch_bounds__(SPLIT ? 512 : RN_GRAD_THREADS, SPLIT ? 1 : 2) 
     if (leads && k + s.ahead - 1 < left) bring(r + (s.ahead - 1) * step, free);
     const int t16 = tid & 15;
     dot = rn_sum16((t16 < parts ? here[first + t16] : 0.f) + (t16 + 16 < parts ? here[first + 16 + t16] : 0.f)) * over_k;
+    auto write = [&](auto is_plain) {
+      constexpr bool P = decltype(is_plain)::value;
 #pragma unroll
-    for (int l = 0; l < L; ++l) {
+      for (int l = 0; l < L; ++l) {
+        const int col = col0 + l * s.off;
+        const char* const pg = rn_param_at<FAST>(a.gate, mrow * a.ldm + col, a.m_dtype);
+        char* const to_x = rn_at(a.dx, r, a.lddx, col);
+        char* const to_y = rn_at(a.dy, r, a.lddy, col);
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int col = 16 * tr + l * s.off + 8 * k;
-        const bool ok = r < a.M && col < K;
-        float d[8];
-        rn_unpack<DT>(rn_load(at + 4 * K + 2 * col, ok && a.dt), d);
+        for (int k = 0; k < PIECES; ++k) {
+          const bool ok = P || (r < a.M && col + 16 * W * k < K);
+          float d[W];
+          rn_unpack<DT, W>(rn_load<W>(at + 4 * K + 2 * col + 32 * W * k, ok && a.dt), d);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) d[i] = fmaf(rs, g[l][8 * k + i] - x[l][8 * k + i] * dot, d[i]);
-        if (ok) *reinterpret_cast<uint4*>(rn_at(a.dx, r, a.lddx, col)) = rn_pack<DT>(d);
-        if (a.dy) {
-          float p[8];
-          rn_param<DT, FAST>(rn_param_at<FAST>(a.gate, mrow * a.ldm + col, a.m_dtype), 0, a.m_dtype, ok && mrow >= 0, p);
+          for (int i = 0; i < W; ++i) d[i] = fmaf(rs, g[l][W * k + i] - x[l][W * k + i] * dot, d[i]);
+          if (ok) *reinterpret_cast<RnWord<W>*>(to_x + 32 * W * k) = rn_pack<DT, W>(d);
+          if (P || a.dy) {
+            float p[W];
+            rn_param<DT, FAST, W>(pg, k, a.m_dtype, ok && (P || mrow >= 0), p);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) d[i] = mrow >= 0 ? d[i] * p[i] : 0.f;
-          if (ok) *reinterpret_cast<uint4*>(rn_at(a.dy, r, a.lddy, col)) = rn_pack<DT>(d);
+            for (int i = 0; i < W; ++i) d[i] = P || mrow >= 0 ? d[i] * p[i] : 0.f;
+            if (ok) *reinterpret_cast<RnWord<W>*>(to_y + 32 * W * k) = rn_pack<DT, W>(d);
+          }
         }
       }
-    }
+    };
+    if (plain) write(std::true_type{});
+    else write(std::false_type{});
     if (++buf == s.ahead) buf = 0, phase ^= 1;
   }
   if (dw && unit < G) {
 #pragma unroll
     for (int l = 0; l < L; ++l) {
-      const int col = 16 * tr + l * s.off;
+      const int col = col0 + l * s.off;
       float* to = dw + (static_cast<int64_t>(blockIdx.x) * G + unit) * K + col;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (K - col > 4 * i) *reinterpret_cast<float4*>(to + 4 * i) = make_float4(sum[l][4 * i], sum[l][4 * i + 1], sum[l][4 * i + 2], sum[l][4 * i + 3]);
+      for (int i = 0; i < 4; ++i) {
+        const int e = i / (W / 4) * 16 * W + i % (W / 4) * 4;
+        if (K - col > e) *reinterpret_cast<float4*>(to + e) = make_float4(sum[l][4 * i], sum[l][4 * i + 1], sum[l][4 * i + 2], sum[l][4 * i + 3]);
+      }
     }
   }
 }
