@@ -199,6 +199,8 @@ def _whole(m: int, dev: torch.device) -> AdapterPlan:
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors share memory.  Rows with the same stride (columns of one wider tensor) are told apart; of other
+    strided tensors the stretches from their first to their last number count."""
     if a.numel() == 0 or b.numel() == 0:
         return False
 
@@ -206,7 +208,14 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
         return t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
 
     (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+    if a0 >= b1 or b0 >= a1:
+        return False
+    if a.dim() == b.dim() == 2 and a.dtype == b.dtype and a.stride() == b.stride() and a.stride(1) == 1:
+        size, width = a.element_size(), a.stride(0) * a.element_size()
+        if width >= max(a.shape[1], b.shape[1]) * size:
+            at = (b0 - a0) % width  # of b's rows behind a's
+            return at < a.shape[1] * size or at + b.shape[1] * size > width
+    return True
 
 
 def _forward(p: _Problem, base, out, want_hidden: bool):
@@ -227,9 +236,8 @@ def _backward(do, x, a, b, pl, hidden, scales, need):
     do = _readable(p.rows(do, p.n, "do"))
     m, k, dev = p.m, p.k, p.dev
     size = _sizes(m, k, p.n, p.rank, p.adapters, True)[1]
-    at = hidden.data_ptr()
-    if at % 256 or hidden.dtype is not torch.uint8 or hidden.dim() != 1 or hidden.shape[0] != size or hidden.device != dev or \
-            not hidden.is_contiguous():
+    if hidden is None or hidden.dtype is not torch.uint8 or hidden.dim() != 1 or hidden.shape[0] != size or \
+            hidden.device != dev or not hidden.is_contiguous() or hidden.data_ptr() % 256:
         raise ValueError(f"low_rank: hidden must be what low_rank(..., return_hidden=True) gave, {size} bytes on {dev}")
     dx = da = db = None
     if need[0]:
@@ -240,7 +248,7 @@ def _backward(do, x, a, b, pl, hidden, scales, need):
         db = torch.empty_like(p.b)
     if need[0] or need[1] or need[2]:
         p.launch(_lib.lib().h3b_low_rank_backward,
-                 (do.data_ptr(), _ld(do), p.x.data_ptr(), _ld(p.x), p.a.data_ptr(), p.b.data_ptr(), at, _lib.ptr(dx), k,
+                 (do.data_ptr(), _ld(do), p.x.data_ptr(), _ld(p.x), p.a.data_ptr(), p.b.data_ptr(), hidden.data_ptr(), _lib.ptr(dx), k,
                   _lib.ptr(da), _lib.ptr(db)), (), True, "low_rank_backward")
     if x.dim() != 2 and dx is not None:
         dx = dx.view(x.shape)

@@ -19,6 +19,7 @@ import torch
 from .. import _lib
 from . import block as blk
 from . import qlinear as ql
+from .adapters import _overlap
 from .rope import no_tangents
 from .types import W4A8Weight, Weight
 
@@ -225,10 +226,11 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, eps: f
 
     x, y: [M, K] bf16 or fp16, K a multiple of 8 up to 16384 (of 256 with codes).  gate, shift, scale: [rows, K] modulation rows
     that `segments` deals out to the tokens as `block.rms_modulate` takes them (ints, or per-token row tensors; numbers
-    outside the rows: none).  Without a gate y is added everywhere; with one a token outside every segment keeps x.  Without shift and scale (they go
-    together) h is the norm alone.  codes: int8 codes and scales of h rotated, as the W4A8 linears take them (`linear`);
-    hidden: h itself.  out: a [M, K] tensor for t, which may be x (not with gradients).  Differentiable in x, y and weight through
-    x and hidden of the result; with gradients the codes, which have none, are refused."""
+    outside the rows: none).  Without a gate y is added everywhere; with one a token outside every segment keeps x.  Without
+    shift and scale (they go together) h is the norm alone.  codes: int8 codes and scales of h rotated, as the W4A8 linears
+    take them (`linear`); hidden: h itself.  out: a [M, K] tensor for t, which may be x or y (not with gradients).
+    Differentiable in x, y and weight through x and hidden of the result; with gradients the codes, which have none, are
+    refused."""
     no_tangents("residual_norm", x, y, weight, gate, shift, scale)
     if (shift is None) != (scale is None):
         raise ValueError("residual_norm: shift and scale go together")
@@ -250,17 +252,6 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, eps: f
         if out.numel() and any(t.data_ptr() != out.data_ptr() or _ld(t) != _ld(out) for t in (x, y) if _overlap(t, out)):
             raise ValueError("residual_norm: out may be x or y, and overlaps them in no other way")
     return _forward(p, x, y, float(eps), codes, hidden, out)
-
-
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    if a.numel() == 0 or b.numel() == 0:
-        return False
-
-    def span(t):
-        return t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
-
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
 
 
 def residual_norm_backward(dt: Optional[torch.Tensor], dh: torch.Tensor, t: torch.Tensor, rstd: torch.Tensor,

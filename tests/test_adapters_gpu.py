@@ -261,3 +261,90 @@ def test_refusals():
     g, = torch.autograd.grad(ad.low_rank(xr, a, b, p).sum(), xr, create_graph=True)
     with pytest.raises(RuntimeError, match="second derivatives"):
         g.sum().backward()
+
+
+@pytest.mark.parametrize("r", [16, 128])  # rows by eights, rows by 128
+def test_offsets_beyond_32_bits(r):
+    x, a, b, base, scales = make(140, 256, 384, r, 3, torch.bfloat16)
+    p = ad.plan(mapped("mixed", 140, 3), 3)
+    want, hidden = ad.low_rank(x, a, b, p, base=base, scales=scales, return_hidden=True)
+    far = torch.empty(140, 1 << 24, dtype=x.dtype, device=DEV)  # the last row begins behind 2^31 numbers
+    xf, bf = far[:, :256], far[:, 512:896]
+    xf.copy_(x), bf.copy_(base)
+    assert torch.equal(ad.low_rank(xf, a, b, p, base=bf, scales=scales), want)
+    for u, v in zip(ad.low_rank_backward(bf, xf, a, b, p, hidden, scales=scales),
+                    ad.low_rank_backward(base, x, a, b, p, hidden, scales=scales)):
+        assert torch.equal(u, v)
+    assert ad.low_rank(x, a, b, p, base=bf, scales=scales, out=bf).data_ptr() == bf.data_ptr()
+    assert torch.equal(bf, want)
+
+
+@pytest.mark.parametrize("m,r", [(4, 64), (40, 16), (300, 64)])
+def test_calls_in_a_row(m, r):
+    """Each call reads what the one before wrote, and workspaces pass from call to call: as many as a decoder's layers, in a
+    stream, in two streams at once and captured, give what calls with a synchronisation behind each give."""
+    x, a, b, _, scales = make(m, 512, 512, r, 4, torch.bfloat16)
+    b, p = b / 8, ad.plan(mapped("mixed", m, 4), 4)
+
+    def run(x, sync=False):
+        out = []
+        for _ in range(24):
+            x = ad.low_rank(x, a, b, p, base=x, scales=scales)
+            y = x.clone()
+            out += [x, ad.low_rank(x, a, b, p, base=y, scales=scales, out=y)]
+            if sync:
+                torch.cuda.synchronize()
+        return torch.stack(out)
+
+    want, other = run(x, True), run(x.flip(0), True)
+    assert torch.isfinite(want).all()
+    assert torch.equal(run(x), want)
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for side, start in zip(sides, (x, x.flip(0))):
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got.append(run(start))
+    for side in sides:
+        torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got[0], want) and torch.equal(got[1], other)
+    graphs, xs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], x.clone()
+    got = []
+    for graph in graphs:  # of two in one pool, replayed in turn
+        with torch.cuda.graph(graph, pool=graphs[0].pool() if got else None):
+            got.append(run(xs))
+    for graph, y in zip(graphs, got):
+        graph.replay()
+        assert torch.equal(y, want)
+    xs.copy_(x.flip(0))
+    for graph, y in zip(graphs, got):
+        graph.replay()
+        assert torch.equal(y, other)
+
+
+def test_one_plan_for_many_projections_and_no_hidden_rows():
+    x, a, b, base, scales = make(50, 256, 384, 16, 3, torch.float16)
+    p = ad.plan(mapped("runs", 50, 3), 3)
+    first = ad.low_rank(x, a, b, p, base=base, scales=scales)
+    x2, a2, b2, base2, _ = make(50, 520, 136, 40, 3, torch.float16)
+    second = ad.low_rank(x2, a2, b2, p, base=base2)
+    assert torch.equal(first, ad.low_rank(x, a, b, p, base=base, scales=scales))
+    assert torch.equal(second, ad.low_rank(x2, a2, b2, ad.plan(mapped("runs", 50, 3), 3), base=base2))
+    with pytest.raises(ValueError, match="hidden"):
+        ad.low_rank_backward(base, x, a, b, p, None, scales=scales)
+
+
+def test_columns_of_one_tensor_as_input_and_output():
+    x, a, b, base, scales = make(30, 256, 384, 16, 3, torch.bfloat16)
+    p = ad.plan(mapped("mixed", 30, 3), 3)
+    both = torch.full((30, 648), 7.0, dtype=x.dtype, device=DEV)
+    both[:, :256] = x
+    ad.low_rank(both[:, :256], a, b, p, base=base, scales=scales, out=both[:, 256:640])
+    assert torch.equal(both[:, 256:640], ad.low_rank(x, a, b, p, base=base, scales=scales))
+    assert torch.equal(both[:, :256], x) and (both[:, 640:] == 7).all()
+    for out in (both[:, 248:632], both[:, 264:]):
+        with pytest.raises(ValueError, match="overlap"):
+            ad.low_rank(both[:, :256] if out.data_ptr() < both[:, 256:].data_ptr() else both[:, 392:], a, b, p, out=out)
+    with pytest.raises(ValueError, match="overlap"):  # a row further, half a row back
+        flat = torch.zeros(31 * 512, dtype=x.dtype, device=DEV)
+        ad.low_rank(flat[:30 * 512].view(30, 512)[:, :256], a, b, p, out=flat[384:384 + 30 * 512].view(30, 512)[:, :384])

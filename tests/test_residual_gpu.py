@@ -231,3 +231,58 @@ def test_refusals():
     g, = torch.autograd.grad(rs.residual_norm(xr, y, w, EPS, codes=False, hidden=True).hidden.sum(), xr, create_graph=True)
     with pytest.raises(RuntimeError, match="second derivatives"):
         g.sum().backward()
+
+
+def test_offsets_beyond_32_bits():
+    x, y, w, gate, shift, scale = make(140, 512, 2, torch.bfloat16, 12)
+    segs, _ = dealt("runs", 140, 2)
+    kw = dict(gate=gate, scale=scale, segments=segs)
+    want = rs.residual_norm(x, y, w, EPS, shift=shift, hidden=True, **kw)
+    far = torch.empty(140, 1 << 24, dtype=x.dtype, device=DEV)  # the last row begins behind 2^31 numbers
+    xf, yf, tf = far[:, :512], far[:, 1024:1536], far[:, 2048:2560]
+    xf.copy_(x), yf.copy_(y), tf.copy_(want.x)
+    got = rs.residual_norm(xf, yf, w, EPS, shift=shift, hidden=True, **kw)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for a, b in zip(rs.residual_norm_backward(yf, xf, tf, want.rstd, w, **kw),
+                    rs.residual_norm_backward(y, x, want.x, want.rstd, w, **kw)):
+        assert torch.equal(a, b)
+    assert rs.residual_norm(xf, yf, w, EPS, shift=shift, out=xf, **kw).x.data_ptr() == xf.data_ptr()
+    assert torch.equal(xf, want.x)
+
+
+@pytest.mark.parametrize("m,k", [(3, 1280), (700, 512), (300, 5376)])
+def test_calls_in_a_row(m, k):
+    """A stream carried through many layers in place (over x, or over y), in two streams at once and captured, against calls with
+    a synchronisation behind each."""
+    x, y, w, gate, shift, scale = make(m, k, 2, torch.bfloat16, 13)
+    segs, _ = dealt("runs", m, 2)
+    kw = dict(gate=gate, shift=shift, scale=scale, segments=segs, codes=k % 256 == 0, hidden=True)
+
+    def run(x, sync=False):
+        t, out = x.clone(), []
+        for i in range(12):
+            h = y.clone()
+            r = rs.residual_norm(t, h, w, EPS, out=(t, h)[i % 2], **kw)
+            t = r.x
+            out += [t.clone().float(), r.hidden.float(), r.codes.float()]
+            if sync:
+                torch.cuda.synchronize()
+        return torch.stack(out)
+
+    want, other = run(x, True), run(x.flip(0), True)
+    sides, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for side, start in zip(sides, (x, x.flip(0))):
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got.append(run(start))
+    for side in sides:
+        torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got[0], want) and torch.equal(got[1], other)
+    graph, xs = torch.cuda.CUDAGraph(), x.clone()
+    with torch.cuda.graph(graph):
+        z = run(xs)
+    graph.replay()
+    assert torch.equal(z, want)
+    xs.copy_(x.flip(0))
+    graph.replay()
+    assert torch.equal(z, other)
