@@ -15,11 +15,6 @@
 namespace h3b {
 
 template <typename T>
-__device__ __forceinline__ float lr_f(T v) {
-  if constexpr (std::is_same_v<T, __half>) return __half2float(v);
-  else return __bfloat162float(v);
-}
-template <typename T>
 __device__ __forceinline__ T lr_t(float v) {
   if constexpr (std::is_same_v<T, __half>) return __float2half_rn(v);
   else return __float2bfloat16_rn(v);
@@ -220,13 +215,12 @@ __device__ __forceinline__ void lr_arrive_full(uint64_t* bar) {
 }
 
 // ----------------------------------------------------------------------------------------------- rows through registers
-// The first two products have 2 rank flops to a byte of x, base or out and are HBM-bound, so what counts is how these bytes travel.
-// They go between global memory and the registers that feed mma.sync directly, 32 bytes to a lane and 128 to a row (four lanes)
-// an instruction.  Fragments of m16n8k16 would have a lane touch 4 bytes of a row; but which numbers a product calls its k (or
-// its n) is free as long as both operands agree, so lane t of a row takes 16 numbers in one piece and hands them out as the
-// fragments' k (n) 2 t, 2 t + 1 (and 2 t + 8, 2 t + 9) of several products; the small operand W is put in that order in shared memory.
-// (tcgen05 forms of both, X by cp.async or out by way of tensor memory, measured 2 to 3 times their floors: 37 us for X of 12090 x
-// 5120, 220 us for base and out of 12090 x 15360; they have too few bytes under way next to their buffers.)
+// The second product has 2 rank flops to a byte of base and out and is HBM-bound, so what counts is how these bytes travel.  They go
+// between global memory and the registers of mma.sync directly, 32 bytes to a lane and 128 to a row (four lanes) an instruction.
+// Fragments of m16n8k16 would have a lane touch 4 bytes of a row; but which numbers a product calls its n (or its k) is free as long
+// as all operands agree, so lane t of a row takes 16 numbers in one piece as the n = 2 t, 2 t + 1 of eight products; the small
+// operand W is put in that order in shared memory.  (tcgen05, out by way of tensor memory and shared memory: 220 us for base and out
+// of 12090 x 15360 where this takes 115 and their bytes 113.)  The same goes for the products of few rows.
 template <typename T>
 __device__ __forceinline__ void lr_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if constexpr (std::is_same_v<T, __half>)
@@ -245,7 +239,8 @@ __device__ __forceinline__ void lr_ldmatrix_t(uint32_t (&r)[4], uint32_t addr) {
                : "r"(addr)
                : "memory");
 }
-// 16 numbers of a row from p on, `left` of them there (a multiple of 8, also negative); wide: rows start on 32-byte boundaries and are multiples of 16 long
+// 16 numbers of a row from p on, `left` of them there (a multiple of 8, also negative); wide: rows start on 32-byte boundaries and are
+// multiples of 16 long
 template <typename T>
 __device__ __forceinline__ void lr_load16(const T* p, int64_t left, bool wide, uint32_t (&v)[8]) {
   if (wide && left >= 16) {
@@ -302,12 +297,16 @@ __device__ __forceinline__ void lr_stage8(uint32_t dst, const T* row, int j, int
 // H [128 rows, rp] of a tile = X [128, C] W, C the contraction: W is A_g [rank, C] (W_ROWS) or B_g [C, rank].  HBM-bound: X is read
 // once, 2 rank flops a byte.  The CTAs of a cluster share a tile's C (95 tiles of 12090 rows would leave a third of the SMs idle)
 // and add their parts up through distributed shared memory in a fixed order.  Copies are cp.async of 16 bytes, since rows are
-// gathered.  Warps 0-3 copy, then read the accumulators; warp 4 issues the products.
+// gathered.  Warps 0-3 copy, then read the accumulators; warp 4 issues the products.  12090 x 5120 of rank 16: 30 us, 4.1 TB/s (its
+// bytes take 19; the rest is the pipeline's start and the parts' way through the cluster); 59440 x 5120 of rank 64: 124 us, 4.9 TB/s.
+// Letting the second product's CTAs in early, to have base on the way at the end of this one, made both slower (together 150 -> 192
+// us for 12090 rows 5120 -> 15360).
 constexpr int LR_XPART = LR_TILE * 128;  // 64 channels of 128 rows
 constexpr int LR_SHRINK_THREADS = 160;
 template <int RPM, bool W_ROWS>  // the largest rp of this variant: 64 or 128
 struct LrShrinkCfg {
-  // A stage has PB parts of 64 channels: 256 bytes of every row at a time where they fit
+  // A stage has PB parts of 64 channels: 256 bytes of every row at a time where they fit (59440 rows 5120 -> 5120 of rank 64, both
+  // products: 356 us, with 128 bytes 404)
   static constexpr int PB = RPM == 64 ? 2 : 1, STAGES = RPM == 64 ? 2 : 3, CTAS = 2, KC = 64 * PB;
   static constexpr int WPART = W_ROWS ? RPM * 128 : KC * 128;  // of W: [RPM ranks][64 channels], or [KC channels][64 ranks]
   static constexpr int STAGE = PB * LR_XPART + (W_ROWS ? PB : RPM / 64) * WPART;
@@ -506,7 +505,8 @@ __global__ void __launch_bounds__(LR_SHRINK_THREADS) lr_shrink_kernel(const LrPl
 // out [128 rows, N] of a tile = base + H W^T: W is B_g [N, rank] (W_ROWS) or A_g [rank, N].  A CTA has 64 CB columns of a tile, a warp 16
 // rows of them: all of its base is asked for at once, then W goes to shared memory, then the products are added and stored.
 //   block of 64 columns: lane t has columns 16 t .. 16 t + 15; 2 j, 2 j + 1 of these are product j's n = 2 t, 2 t + 1
-// Ranks are filled up with zeros to 16 NQ: leaving products out by the rank cost 13 instructions to a product.
+// Ranks are filled up with zeros to 16 NQ: leaving products out by the rank cost 13 instructions to a product.  12090 x 15360 of
+// rank 16 with base: 115 us, 6.5 TB/s; 59440 x 5120 of rank 64: 241 us, 5.1 TB/s; dx of 12090 x 5120, rank 32: 26 us, its bytes 19.
 constexpr int LR_THREADS = 256;
 template <int NQ, bool W_ROWS, bool BASE>  // 16 NQ: the largest rp of this variant
 struct LrExpandCfg {
@@ -650,7 +650,8 @@ __global__ void __launch_bounds__(LR_THREADS, LrExpandCfg<NQ, W_ROWS, BASE>::CTA
 // ----------------------------------------------------------------------------------------------- few rows
 // Up to eight rows of one adapter, as single tokens of many requests have them: everything is the adapters' weights, read once, and
 // latency.  Weights go from memory straight to fragments; K is dealt out to `splits` CTAs of a tile, whose parts the second kernel adds
-// up in a fixed order.  The second kernel is let in when every CTA of the first has begun, and asks for its weights and base
+// up in a fixed order (4 rows of rank 16, 5120 -> 5120: 6.9 us; 64 rows of 64 adapters of rank 64, 5120 -> 15360: 33 us, 3.9 TB/s of the
+// weights in use, base and out).  The second kernel is let in when every CTA of the first has begun, and asks for its weights and base
 // before it waits for the parts: the two products' weights come in one stream.  (A cluster of eight CTAs for both products, its parts
 // in distributed shared memory: 16.2 us for one row of rank 64, 91 us for 64 rows of 64 adapters 5120 -> 15360.)
 //   32 columns (ranks) of a row: lane t has 8 t .. 8 t + 7, which are k = 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of two products
@@ -823,7 +824,9 @@ __global__ void __launch_bounds__(LR_FEW_THREADS) lr_few_up_kernel(const LrPlan 
 // D [128 channels, rp] = X^T H over the rows of a unit (a stretch of one adapter's rows): X's columns are M, H's are N, rows are K,
 // all read as they lie in memory.  HBM-bound: X is read once; H comes from L2.  Rows behind the last are zeros in both operands.  One
 // launch does dA (x with dh) and dB (grad_out with h).  fp16: a row's power of two is taken out against the largest of the unit.
-// Warps 0-3 copy, then read the accumulators; warp 4 issues the products.
+// Warps 0-3 copy, then read the accumulators; warp 4 issues the products.  12090 rows of 5120 and 5120, rank 32: 58 us, 4.3 TB/s (5.0
+// by itself; in a training step dx's way out of L2 is in it), and 7 to 11 us for the sum of the units' parts.  Fewer, longer units
+// took longer (two of these 16 in one CTA 58, four 60, eight 74).
 constexpr int LR_KROWS = 64;  // rows of a stage
 template <int RPM>
 struct LrWgradCfg {
@@ -1058,7 +1061,8 @@ size_t lr_workspace(int64_t M, int64_t K, int64_t N, int rank, int64_t R, bool b
 }
 // How many CTAs share a tile's steps, 1, 2, 4 or 8: the fewest rounds of resident CTAs times the steps that each takes, with what a
 // CTA's start and end cost (`extra` steps; about what 768 columns do: 97 tiles x 5120 columns go in two parts, 189 and 467 tiles whole,
-// up to 33 tiles in eight).
+// up to 33 tiles in eight).  Powers of two alone: a training step of
+// 12090 rows takes 204 us with two parts, 227 with three (and 214 with four, 211 with five).
 static int64_t lr_cost(int64_t tiles, int64_t steps, int64_t parts, int64_t slots, int64_t extra) {
   return ((tiles * parts + slots - 1) / slots) * ((steps + parts - 1) / parts + extra);
 }
