@@ -43,7 +43,8 @@ struct LrPlan {
 static int64_t lr_up4(int64_t v) { return (v + 3) / 4 * 4; }
 static int64_t lr_lines(int64_t M, int64_t R, int rows) { return M / rows + (R + 1 < M ? R + 1 : M); }
 static int lr_unit_tiles(int64_t M) { return static_cast<int>((M + LR_TILE * LR_SPLITS - 1) / (LR_TILE * LR_SPLITS)); }
-static int64_t lr_unit_lines(int64_t M, int64_t R) { return lr_lines(M, R, LR_TILE) / lr_unit_tiles(M) + (R < M ? R : M); }
+// n rows make at most (n - 1) / rows of a unit + 1 of them
+static int64_t lr_unit_lines(int64_t M, int64_t R) { return M / (LR_TILE * lr_unit_tiles(M)) + (R < M ? R : M); }
 // An adapter with several units has more than lr_unit_tiles(M) >= M / (LR_TILE LR_SPLITS) tiles, of which all but one are full: there
 // are at most LR_SPLITS of them, and their units are at most (M / LR_TILE + LR_SPLITS) / lr_unit_tiles(M) + LR_SPLITS.
 static int64_t lr_slots(int64_t M) { return (M / LR_TILE + LR_SPLITS) / lr_unit_tiles(M) + LR_SPLITS; }
@@ -828,11 +829,13 @@ __global__ void __launch_bounds__(LR_FEW_THREADS) lr_few_up_kernel(const LrPlan 
 // by itself; in a training step dx's way out of L2 is in it), and 7 to 11 us for the sum of the units' parts.  Fewer, longer units
 // took longer (two of these 16 in one CTA 58, four 60, eight 74).
 constexpr int LR_KROWS = 64;  // rows of a stage
-template <int RPM>
+// ST stages: three, or one where the adapters have no more rows than that on average, so that more CTAs fit an SM (training steps 5120
+// -> 5120: 512 rows of 64 adapters, rank 64, 171 us, with three 180; 61 rows of 24, rank 128, 102, with three 116)
+template <int RPM, int ST>
 struct LrWgradCfg {
-  static constexpr int PARTS = RPM / 64, STAGES = 3;
-  static constexpr int XBYTES = 2 * LR_KROWS * 128, STAGE = XBYTES + PARTS * LR_KROWS * 128;
-  static constexpr int SMEM = STAGES * STAGE + 1024;
+  static constexpr int PARTS = RPM / 64;
+  static constexpr int XBYTES = 2 * LR_KROWS * 128, STAGE = XBYTES + PARTS * LR_KROWS * 128, OUT = 128 * (RPM + 8) * 2 + 1024;
+  static constexpr int SMEM = (ST * STAGE > OUT ? ST * STAGE : OUT) + 1024;
 };
 template <typename T>
 struct LrWgradSide {
@@ -844,11 +847,10 @@ struct LrWgradSide {
   int blocks;    // of 128 channels
   bool by_rank;
 };
-template <typename T, int RPM>
+template <typename T, int RPM, int ST>
 __global__ void __launch_bounds__(160) lr_wgrad_kernel(const LrPlan p, const LrWgradSide<T> sa, const LrWgradSide<T> sb, int rank, int rp,
                                                        int R) {
-  using Cfg = LrWgradCfg<RPM>;
-  constexpr int ST = Cfg::STAGES;
+  using Cfg = LrWgradCfg<RPM, ST>;
   extern __shared__ __align__(1024) unsigned char lr_smem[];
   __shared__ uint64_t full[ST], empty[ST], done;
   __shared__ uint32_t tmem_at;
@@ -965,21 +967,59 @@ __global__ void __launch_bounds__(160) lr_wgrad_kernel(const LrPlan p, const LrW
     }
     warp_wait(&done, 0, abort);
     tc_fence_after();
-    const int64_t c = col + tid;  // a channel per lane
+    // a channel per lane.  A whole gradient goes out by way of shared memory (every product has read the stages), 16 bytes at a time
+    // in the order of memory: lanes that wrote their channel's ranks one by one took 223 us for 24 adapters of rank 128 beside 1112 ->
+    // 7680
+    const int64_t c = col + tid;
+    const bool eights = rank % 8 == 0;
+    const int ld = sd.by_rank ? 136 : rank + 8;
+    T* const out = reinterpret_cast<T*>(base);
     for (int j = 0; j < rp; j += 16) {
       uint32_t v[16];
       tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(warp * 32) << 16) + j, v);
       tmem_ld_wait();
-      if (c >= sd.C) {
-      } else if (u.w >= 0) {
-        store_cols_f32(sd.part + (u.w * sd.C + c) * rp + j, v, top, 16);
+      if (u.w >= 0) {
+        if (c < sd.C) store_cols_f32(sd.part + (u.w * sd.C + c) * rp + j, v, top, 16);
+      } else if (!sd.by_rank && eights) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] = pack2<T>(__uint_as_float(v[8 * h + 2 * k]) * top, __uint_as_float(v[8 * h + 2 * k + 1]) * top);
+          if (j + 8 * h < rank) *reinterpret_cast<uint4*>(out + tid * ld + j + 8 * h) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
       } else {
-        T* g = sd.grad + static_cast<int64_t>(u.x) * rank * sd.C;
 #pragma unroll
         for (int k = 0; k < 16; ++k)
-          if (j + k < rank) g[sd.by_rank ? (j + k) * sd.C + c : c * rank + j + k] = lr_t<T>(__uint_as_float(v[k]) * top);
+          if (j + k < rank) out[sd.by_rank ? (j + k) * ld + tid : tid * ld + j + k] = lr_t<T>(__uint_as_float(v[k]) * top);
       }
       __syncwarp();
+    }
+    if (u.w < 0) {
+      group_sync(1, 128);
+      T* const g = sd.grad + static_cast<int64_t>(u.x) * rank * sd.C + col * (sd.by_rank ? 1 : rank);
+      if (sd.by_rank) {
+        for (int e = tid; e < rank * 16; e += 128) {
+          const int j = e >> 4, i = (e & 15) * 8;
+          if (col + i < sd.C) *reinterpret_cast<uint4*>(g + j * sd.C + i) = *reinterpret_cast<const uint4*>(out + j * ld + i);
+        }
+      } else {
+        const int total = static_cast<int>(min(static_cast<int64_t>(128), sd.C - col)) * rank;
+        for (int i = tid * 8; i < total; i += 128 * 8) {
+          const int r = i / rank, k = i - r * rank;
+          if (eights) {
+            *reinterpret_cast<uint4*>(g + i) = *reinterpret_cast<const uint4*>(out + r * ld + k);
+          } else {
+            uint4 w;
+            T* const e = reinterpret_cast<T*>(&w);
+            for (int q = 0, rr = r, kk = k; q < 8; ++q) {
+              e[q] = out[rr * ld + kk];
+              if (++kk == rank) kk = 0, ++rr;
+            }
+            *reinterpret_cast<uint4*>(g + i) = w;
+          }
+        }
+      }
     }
     tc_fence_before();
   }
@@ -989,42 +1029,69 @@ __global__ void __launch_bounds__(160) lr_wgrad_kernel(const LrPlan p, const LrW
     tmem_dealloc(tmem, lr_tmem_cols(rp));
   }
 }
-// The parts of an adapter's units, added up in their order; zeros for adapters without rows.  A CTA: 1024 numbers (1024 / rp channels)
-// of one adapter, four to a thread, so that the loads of 16 parts are on the way at once.
+// The parts of an adapter's units, added up in their order; zeros for adapters without rows.  A CTA adds up to 1024 numbers (lr_chans(rp)
+// channels) of one adapter at a time, four to a thread, so that the loads of 16 parts are on the way at once, and stores them 16 bytes
+// at a time.  Most adapters of many have nothing to add up: they share so many CTAs as fill the SMs.
+__host__ __device__ inline int lr_chans(int rp) { return 1024 / rp / 8 * 8; }
 template <typename T>
 __global__ void __launch_bounds__(256) lr_join_kernel(const LrPlan p, const LrWgradSide<T> sa, const LrWgradSide<T> sb, int blocks_a,
-                                                      int rank, int rp) {
-  __shared__ float sums[1024 + 128];  // a line of rp + 1 numbers to a channel
+                                                      int blocks, int rank, int rp) {
+  __shared__ float sums[1024 + 64];  // a line of rp + 1 numbers to a channel
   after_previous();
-  const int g = blockIdx.y;
+  const int g = blockIdx.y, tid = threadIdx.x;
   const int s0 = p.slot[g], s1 = p.slot[g + 1];
-  const bool none = p.offset[g] == p.offset[g + 1];
-  if (s0 == s1 && !none) return;
-  const bool second = static_cast<int>(blockIdx.x) >= blocks_a;
-  const LrWgradSide<T>& sd = second ? sb : sa;
-  const int chans = 1024 / rp;
-  const int64_t col = static_cast<int64_t>(second ? blockIdx.x - blocks_a : blockIdx.x) * chans;
-  const int cols = static_cast<int>(min(static_cast<int64_t>(chans), sd.C - col));
-  const int e = threadIdx.x * 4, c = e / rp, j = e - c * rp;
-  if (c < cols) {
-    const float4* from = reinterpret_cast<const float4*>(sd.part + col * rp + e);
-    const int64_t step = sd.C * rp / 4;
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = s0; s < s1; s += 16) {
-      float4 v[16];
-#pragma unroll
-      for (int k = 0; k < 16; ++k) v[k] = s + k < s1 ? from[(s + k) * step] : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int k = 0; k < 16; ++k) sum.x += v[k].x, sum.y += v[k].y, sum.z += v[k].z, sum.w += v[k].w;
+  if (p.offset[g] == p.offset[g + 1]) {
+    for (const LrWgradSide<T>* sd : {&sa, &sb}) {
+      const int64_t size = static_cast<int64_t>(rank) * sd->C;  // a multiple of 8
+      if (sd->blocks)
+        for (int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + tid) * 8; i < size; i += static_cast<int64_t>(gridDim.x) * 256 * 8)
+          *reinterpret_cast<uint4*>(sd->grad + g * size + i) = make_uint4(0, 0, 0, 0);
     }
-    float* to = sums + c * (rp + 1) + j;
-    to[0] = sum.x, to[1] = sum.y, to[2] = sum.z, to[3] = sum.w;
+    return;
   }
-  __syncthreads();
-  T* out = sd.grad + static_cast<int64_t>(g) * rank * sd.C;
-  for (int i = threadIdx.x; i < cols * rank; i += 256) {
-    const int cc = sd.by_rank ? i % cols : i / rank, jj = sd.by_rank ? i / cols : i % rank;
-    out[sd.by_rank ? jj * sd.C + col + cc : (col + cc) * rank + jj] = lr_t<T>(sums[cc * (rp + 1) + jj]);
+  if (s0 == s1) return;
+  const int chans = lr_chans(rp), e = tid * 4, c = e / rp, j = e - c * rp;
+  for (int block = blockIdx.x; block < blocks; block += gridDim.x) {
+    const bool second = block >= blocks_a;
+    const LrWgradSide<T>& sd = second ? sb : sa;
+    const int64_t col = static_cast<int64_t>(second ? block - blocks_a : block) * chans;
+    const int cols = static_cast<int>(min(static_cast<int64_t>(chans), sd.C - col));  // a multiple of 8
+    if (c < cols) {
+      const float4* from = reinterpret_cast<const float4*>(sd.part + col * rp + e);
+      const int64_t step = sd.C * rp / 4;
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int s = s0; s < s1; s += 16) {
+        float4 v[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] = s + k < s1 ? from[(s + k) * step] : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) sum.x += v[k].x, sum.y += v[k].y, sum.z += v[k].z, sum.w += v[k].w;
+      }
+      float* to = sums + c * (rp + 1) + j;
+      to[0] = sum.x, to[1] = sum.y, to[2] = sum.z, to[3] = sum.w;
+    }
+    __syncthreads();
+    T* const out = sd.grad + static_cast<int64_t>(g) * rank * sd.C;
+    if (tid < rank * cols / 8) {
+      float w[8];
+      T* to;
+      if (sd.by_rank) {  // eight channels of a rank
+        const int jj = tid / (cols / 8), cc = (tid - jj * (cols / 8)) * 8;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) w[q] = sums[(cc + q) * (rp + 1) + jj];
+        to = out + jj * sd.C + col + cc;
+      } else {  // eight numbers in the order of memory
+        int cc = tid * 8 / rank, jj = tid * 8 - cc * rank;
+        to = out + (col + cc) * rank + jj;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          w[q] = sums[cc * (rp + 1) + jj];
+          if (++jj == rank) jj = 0, ++cc;
+        }
+      }
+      *reinterpret_cast<uint4*>(to) = make_uint4(pack2<T>(w[0], w[1]), pack2<T>(w[2], w[3]), pack2<T>(w[4], w[5]), pack2<T>(w[6], w[7]));
+    }
+    __syncthreads();
   }
 }
 
@@ -1136,17 +1203,23 @@ static int lr_expand(const LrPlan& p, const LrHidden& h, const T* w, int rank, i
   if (rp <= 64) return lr_expand_b<T, W_ROWS, 4>(p, h, w, rank, rp, R, base, ldb, out, ldo, N, st);
   return lr_expand_b<T, W_ROWS, 8>(p, h, w, rank, rp, R, base, ldb, out, ldo, N, st);
 }
+template <typename T, int RPM, int ST>
+static int lr_wgrad_s(const LrPlan& p, const LrWgradSide<T>& a, const LrWgradSide<T>& b, int rank, int R, cudaStream_t st) {
+  static std::atomic<bool> ready[CA_DEVICES];
+  return lr_launch("lr_wgrad_kernel", lr_wgrad_kernel<T, RPM, ST>, ready, dim3(static_cast<unsigned>(p.n_units * (a.blocks + b.blocks))), 160,
+                   LrWgradCfg<RPM, ST>::SMEM, 1, st, p, a, b, rank, lr_rp(rank), R);
+}
 template <typename T, int RPM>
-static int lr_wgrad(const LrPlan& p, const LrWgradSide<T>& a, const LrWgradSide<T>& b, int rank, int R, cudaStream_t st) {
-  static std::atomic<bool> ready[CA_DEVICES], joined[CA_DEVICES];
+static int lr_wgrad(const LrPlan& p, const LrWgradSide<T>& a, const LrWgradSide<T>& b, int rank, int64_t M, int R, cudaStream_t st) {
+  static std::atomic<bool> joined[CA_DEVICES];
   const int rp = lr_rp(rank);
-  const int64_t grid = p.n_units * (a.blocks + b.blocks);
-  if (int rc = lr_launch("lr_wgrad_kernel", lr_wgrad_kernel<T, RPM>, ready, dim3(static_cast<unsigned>(grid)), 160, LrWgradCfg<RPM>::SMEM,
-                         1, st, p, a, b, rank, rp, R))
-    return rc;
-  const int chans = 1024 / rp;
+  const bool one = M <= LR_KROWS * R;
+  if (int rc = one ? lr_wgrad_s<T, RPM, 1>(p, a, b, rank, R, st) : lr_wgrad_s<T, RPM, 3>(p, a, b, rank, R, st)) return rc;
+  const int chans = lr_chans(rp);
   const int ja = static_cast<int>((a.blocks ? a.C + chans - 1 : 0) / chans), jb = static_cast<int>((b.blocks ? b.C + chans - 1 : 0) / chans);
-  return lr_launch("lr_join_kernel", lr_join_kernel<T>, joined, dim3(ja + jb, R), 256, 0, 1, st, p, a, b, ja, rank, rp);
+  const int each = (8 * cross_sms() + R - 1) / R;
+  return lr_launch("lr_join_kernel", lr_join_kernel<T>, joined, dim3(ja + jb < each ? ja + jb : each, R), 256, 0, 1, st, p, a, b, ja, ja + jb,
+                   rank, rp);
 }
 template <typename T, int RB>
 static int lr_few_s(const LrPlan& p, const LrArgs& a, int rp, const LrHidden& h, float* part, cudaStream_t st) {
@@ -1200,7 +1273,7 @@ static int lr_backward_t(const LrArgs& a, cudaStream_t st) {
   const int blocks_k = static_cast<int>((a.K + 127) / 128), blocks_n = static_cast<int>((a.N + 127) / 128);
   const LrWgradSide<T> sa{x, a.ldx, a.K, dh, static_cast<T*>(a.da), reinterpret_cast<float*>(ws + s.part_a), a.da ? blocks_k : 0, true};
   const LrWgradSide<T> sb{go, a.ldgo, a.N, h, static_cast<T*>(a.db), reinterpret_cast<float*>(ws + s.part_b), a.db ? blocks_n : 0, false};
-  return lr_rp(a.rank) <= 64 ? lr_wgrad<T, 64>(p, sa, sb, a.rank, R, st) : lr_wgrad<T, 128>(p, sa, sb, a.rank, R, st);
+  return lr_rp(a.rank) <= 64 ? lr_wgrad<T, 64>(p, sa, sb, a.rank, a.M, R, st) : lr_wgrad<T, 128>(p, sa, sb, a.rank, a.M, R, st);
 }
 int lr_forward(const LrArgs& a, cudaStream_t st) {
   return a.dtype == H3B_FP16 ? lr_forward_t<__half>(a, st) : lr_forward_t<__nv_bfloat16>(a, st);
