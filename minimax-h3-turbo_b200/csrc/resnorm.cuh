@@ -138,23 +138,27 @@ __device__ __forceinline__ uint32_t rn_codes(float x0, float x1, float x2, float
 // columns are `off` apart, half the row rounded up to whole blocks of 256, so that both are at the same place of theirs).
 struct RnShape {
   int T, G, threads, blocks, off, smem, ahead;
-  bool split;
+  bool split, more;
 };
-constexpr int RN_THREADS = 320;  // a CTA's, with 96 registers each and 20 warps to an SM; groups of more (WIDE) are CTAs of up to 512
-                                 // with 128 registers and 16 warps
+// Threads of a CTA at most: 320 with 96 registers each and 20 warps to an SM; 384 with 80 and 24, for groups of more than 320 and,
+// without codes, where it lets more warps onto an SM (16000 x 4096: 88 us, with 96 registers 94; with codes 114 and 109); 512 with 128
+// and 16 for groups of more than 384.  Rows of up to 8192 channels are worked on in pairs, since the weight's and the modulation's
+// numbers then serve both (in halves of one row: 12090 x 5376 without codes 128 us where pairs take 106, with codes and h 177 and 148).
+constexpr int RN_THREADS = 320, RN_MORE = 384, RN_LARGE = 512;
 // Shared memory: barriers and abort flag (32 bytes), the groups' modulation rows (at most RN_GRAD_THREADS / 16 pairs of them), their
 // sums, their rows, the rotation's exchange
 constexpr int RN_HEAD = 256;
 __host__ __device__ inline int rn_rows_at(int threads) { return RN_HEAD + threads; }  // threads / 16 half-warps x (8 + 8) bytes
 __host__ __device__ inline int rn_group_bytes(int K, bool split) { return (split ? 2 : 4) * 2 * K; }
 
-template <int DT, bool CODES, bool FAST, bool SPLIT, bool WIDE>
-__global__ void __launch_bounds__(WIDE ? 512 : RN_THREADS, WIDE ? 1 : 2) resnorm_kernel(const ResNormArgs a, const RnShape s) {
+template <int DT, bool CODES, bool FAST, bool SPLIT, int MOST>
+__global__ void __launch_bounds__(MOST, MOST == RN_LARGE ? 1 : 2) resnorm_kernel(const ResNormArgs a, const RnShape s) {
   constexpr int W = 4, PIECES = 16 / W;  // with or without codes, so that the sums are the same
   extern __shared__ __align__(128) unsigned char rn_smem[];
   const int tid = threadIdx.x, T = s.T, G = s.G, unit = tid / T, tr = tid - unit * T, K = a.K;
   const int half = tid >> 4, halves = blockDim.x >> 4, t16 = tid & 15, parts = unit < G ? T >> 4 : 0, first = unit * parts;
   const int col[2] = {(tr & ~15) * 16 + W * t16, (tr & ~15) * 16 + W * t16 + (SPLIT ? s.off : 0)};  // and PIECES times 16 W further
+  const int from[2] = {col[0], SPLIT && col[1] >= K ? col[0] : col[1]};
   uint64_t* const bar = reinterpret_cast<uint64_t*>(rn_smem);
   volatile int* const abort = reinterpret_cast<volatile int*>(rn_smem + 8);
   float2* const part = reinterpret_cast<float2*>(rn_smem + RN_HEAD);
@@ -201,8 +205,9 @@ __global__ void __launch_bounds__(WIDE ? 512 : RN_THREADS, WIDE ? 1 : 2) resnorm
     const int2 both = *rows_of;
     const int mrow[2] = {both.x, both.y};
     const bool same = !SPLIT && mrow[0] == mrow[1];  // one load of a modulation row serves both lanes
-    // the ordinary case by itself, without a branch inside: modulation rows of the stream's type, 16 channels and 16 to every thread
-    const bool plain = mods && mrow[0] >= 0 && (SPLIT ? n[1] > 0 : same);
+    // the ordinary case by itself, without a branch inside: modulation rows of the stream's type, 16 channels to every thread.  Where a
+    // split row's second half ends before (off, above), its threads go through the first half's channels with zeros.
+    const bool plain = mods && mrow[0] >= 0 && (SPLIT || same);
     mbar_wait(bar, turn, abort);
     // ---- the stream
     float2 v[16], ss = make_float2(0.f, 0.f);
@@ -213,8 +218,8 @@ __global__ void __launch_bounds__(WIDE ? 512 : RN_THREADS, WIDE ? 1 : 2) resnorm
       char* to[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        at[h] = mine + (SPLIT ? 0 : h) * 4 * K + 2 * col[h];
-        pg[h] = rn_param_at<FAST>(a.gate, mrow[h] * a.ldm + col[h], a.m_dtype);
+        at[h] = mine + (SPLIT ? 0 : h) * 4 * K + 2 * from[h];
+        pg[h] = rn_param_at<FAST>(a.gate, mrow[h] * a.ldm + from[h], a.m_dtype);
         to[h] = rn_at(a.t, row[h], a.ldt, col[h]);
       }
 #pragma unroll
@@ -243,7 +248,7 @@ __global__ void __launch_bounds__(WIDE ? 512 : RN_THREADS, WIDE ? 1 : 2) resnorm
 #pragma unroll
           for (int i = 0; i < W; ++i) {
             if (h == 0) v[W * k + i].x = f[i];
-            else v[W * k + i].y = f[i];
+            else v[W * k + i].y = P && SPLIT && n[1] <= 0 ? 0.f : f[i];
           }
         }
       }
@@ -268,9 +273,9 @@ __global__ void __launch_bounds__(WIDE ? 512 : RN_THREADS, WIDE ? 1 : 2) resnorm
       char* to[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        pw[h] = rn_param_at<FAST>(a.w, col[h], a.w_dtype);
-        ps[h] = rn_param_at<FAST>(a.scale, mrow[h] * a.ldm + col[h], a.m_dtype);
-        pt[h] = rn_param_at<FAST>(a.shift, mrow[h] * a.ldm + col[h], a.m_dtype);
+        pw[h] = rn_param_at<FAST>(a.w, from[h], a.w_dtype);
+        ps[h] = rn_param_at<FAST>(a.scale, mrow[h] * a.ldm + from[h], a.m_dtype);
+        pt[h] = rn_param_at<FAST>(a.shift, mrow[h] * a.ldm + from[h], a.m_dtype);
         to[h] = rn_at(a.h, row[h], a.ldh, col[h]);
       }
 #pragma unroll
@@ -342,7 +347,7 @@ __global__ void __launch_bounds__(WIDE ? 512 : RN_THREADS, WIDE ? 1 : 2) resnorm
       for (int i = 0; i < 16; i += 2) m.x = max3f(m.x, fabsf(v[i].x), fabsf(v[i + 1].x)), m.y = max3f(m.y, fabsf(v[i].y), fabsf(v[i + 1].y));
       uint2 top = make_uint2(max(__float_as_uint(m.x), __float_as_uint(v[0].x) & 0x7FFFFFFFu),
                              max(__float_as_uint(m.y), __float_as_uint(v[0].y) & 0x7FFFFFFFu));
-      if (SPLIT) top.x = top.y = max(top.x, top.y);
+      if (SPLIT) top.x = top.y = n[1] > 0 ? max(top.x, top.y) : top.x;
       top = rn_over_rows<uint32_t>(top, tops, half, first, parts, [](uint32_t b, uint32_t c) { return max(b, c); });
       const float2 amax = make_float2(__uint_as_float(top.x), __uint_as_float(top.y));
       if (leads) {
@@ -425,7 +430,7 @@ __global__ void __launch_bounds__(SPLIT ? 512 : RN_GRAD_THREADS, SPLIT ? 1 : 2) 
   if (leads)
     for (int i = 0; i < s.ahead - 1 && i < left; ++i) bring(r + i * step, i);
   const float over_k = 1.f / static_cast<float>(K);
-  const bool mods = FAST && a.dy && a.scale && K % 256 == 0 && unit < G;
+  const bool mods = FAST && a.dy && a.scale && K % 256 == 0 && unit < G, second = SPLIT && col0 + s.off < K;
   float sum[L][16];
 #pragma unroll
   for (int l = 0; l < L; ++l)
@@ -440,12 +445,13 @@ __global__ void __launch_bounds__(SPLIT ? 512 : RN_GRAD_THREADS, SPLIT ? 1 : 2) 
     const unsigned char* const at = mine + buf * bytes;
     float g[L][16], x[L][16], dot = 0.f;
     // the ordinary case by itself, as above
-    const bool plain = mods && mrow >= 0 && (!SPLIT || col0 + s.off < K);
+    const bool plain = mods && mrow >= 0;
     auto dots = [&](auto is_plain) {
       constexpr bool P = decltype(is_plain)::value;
 #pragma unroll
       for (int l = 0; l < L; ++l) {
-        const int col = col0 + l * s.off;
+        const bool live = !P || l == 0 || second;
+        const int col = live ? col0 + l * s.off : col0;
         const char* const ps = rn_param_at<FAST>(a.scale, mrow * a.ldm + col, a.m_dtype);
         const char* const pw = rn_param_at<FAST>(a.w, col, a.w_dtype);
 #pragma unroll
@@ -459,7 +465,7 @@ __global__ void __launch_bounds__(SPLIT ? 512 : RN_GRAD_THREADS, SPLIT ? 1 : 2) 
             for (int i = 0; i < W; ++i) f[i] *= 1.f + p[i];
           }
 #pragma unroll
-          for (int i = 0; i < W; ++i) g[l][W * k + i] = f[i];
+          for (int i = 0; i < W; ++i) g[l][W * k + i] = live ? f[i] : 0.f;
           rn_unpack<DT, W>(rn_load<W>(at + 2 * K + 2 * col + 32 * W * k, ok), f);
           rn_param<DT, FAST, W>(pw, k, a.w_dtype, ok, p);
 #pragma unroll
@@ -488,7 +494,8 @@ __global__ void __launch_bounds__(SPLIT ? 512 : RN_GRAD_THREADS, SPLIT ? 1 : 2) 
       constexpr bool P = decltype(is_plain)::value;
 #pragma unroll
       for (int l = 0; l < L; ++l) {
-        const int col = col0 + l * s.off;
+        const bool live = !P || l == 0 || second;
+        const int col = live ? col0 + l * s.off : col0;
         const char* const pg = rn_param_at<FAST>(a.gate, mrow * a.ldm + col, a.m_dtype);
         char* const to_x = rn_at(a.dx, r, a.lddx, col);
         char* const to_y = rn_at(a.dy, r, a.lddy, col);
@@ -499,13 +506,13 @@ __global__ void __launch_bounds__(SPLIT ? 512 : RN_GRAD_THREADS, SPLIT ? 1 : 2) 
           rn_unpack<DT, W>(rn_load<W>(at + 4 * K + 2 * col + 32 * W * k, ok && a.dt), d);
 #pragma unroll
           for (int i = 0; i < W; ++i) d[i] = fmaf(rs, g[l][W * k + i] - x[l][W * k + i] * dot, d[i]);
-          if (ok) *reinterpret_cast<RnWord<W>*>(to_x + 32 * W * k) = rn_pack<DT, W>(d);
+          if (ok && live) *reinterpret_cast<RnWord<W>*>(to_x + 32 * W * k) = rn_pack<DT, W>(d);
           if (P || a.dy) {
             float p[W];
             rn_param<DT, FAST, W>(pg, k, a.m_dtype, ok && (P || mrow >= 0), p);
 #pragma unroll
             for (int i = 0; i < W; ++i) d[i] = P || mrow >= 0 ? d[i] * p[i] : 0.f;
-            if (ok) *reinterpret_cast<RnWord<W>*>(to_y + 32 * W * k) = rn_pack<DT, W>(d);
+            if (ok && live) *reinterpret_cast<RnWord<W>*>(to_y + 32 * W * k) = rn_pack<DT, W>(d);
           }
         }
       }
@@ -568,9 +575,9 @@ static int rn_sms() {
 static RnShape rn_shape(int64_t M, int K, bool codes, bool backward) {
   RnShape s{};
   s.T = (K + 255) / 256 * 16;
-  const int most = backward ? RN_GRAD_THREADS : RN_THREADS;
-  s.split = s.T > most;
+  s.split = s.T > (backward ? RN_GRAD_THREADS : RN_LARGE);
   if (s.split) s.off = (K + 511) / 512 * 256, s.T = s.off / 16;
+  const int most = backward ? RN_GRAD_THREADS : RN_THREADS;
   s.G = s.T > most ? 1 : most / s.T;
   const int64_t groups = backward || s.split ? M : (M + 1) / 2;
   if (groups < 2 * rn_sms() && s.G > 1) s.G = 1;  // few rows: spread over the SMs
@@ -578,7 +585,9 @@ static RnShape rn_shape(int64_t M, int K, bool codes, bool backward) {
   s.ahead = RN_AHEAD * 6 * K > 220 * 1024 ? 2 : RN_AHEAD;
   s.smem = rn_rows_at(s.threads) + s.G * (backward ? s.ahead * 6 * K : rn_group_bytes(K, s.split)) +
            (codes ? s.threads / 16 * xgrp(16) * 8 : 0);
-  int per = (backward ? (s.split ? 16 : 24) : s.threads > RN_THREADS ? 16 : 20) / (s.threads / 32);
+  const int w = s.threads / 32;
+  s.more = s.threads <= RN_MORE && (s.threads > RN_THREADS || (!codes && 24 / w * w > 20 / w * w));
+  int per = (backward ? (s.split ? 16 : 24) : s.threads > RN_MORE ? 16 : s.more ? 24 : 20) / w;
   if (per > 225 * 1024 / (s.smem + 1024)) per = 225 * 1024 / (s.smem + 1024);
   if (per < 1) per = 1;
   const int64_t want = (groups + s.G - 1) / s.G, cap = static_cast<int64_t>(rn_sms()) * per;
@@ -601,13 +610,18 @@ static int rn_ready(F* kernel, int smem, std::atomic<bool> (&done)[RN_DEVICES]) 
   return H3B_OK;
 }
 
-template <int DT, bool FAST, bool SPLIT, bool WIDE>
-static int resnorm_forward_t(const ResNormArgs& a, const RnShape& s, cudaStream_t st) {
-  auto kernel = a.codes ? resnorm_kernel<DT, true, FAST, SPLIT, WIDE> : resnorm_kernel<DT, false, FAST, SPLIT, WIDE>;
+template <int DT, bool FAST, bool SPLIT, int MOST>
+static int resnorm_forward_s(const ResNormArgs& a, const RnShape& s, cudaStream_t st) {
+  auto kernel = a.codes ? resnorm_kernel<DT, true, FAST, SPLIT, MOST> : resnorm_kernel<DT, false, FAST, SPLIT, MOST>;
   static std::atomic<bool> ready[2][RN_DEVICES];
   if (int rc = rn_ready(kernel, s.smem, ready[a.codes != nullptr])) return rc;
   kernel<<<s.blocks, s.threads, s.smem, st>>>(a, s);
   return check_launch("resnorm_kernel");
+}
+template <int DT, bool FAST, bool SPLIT>
+static int resnorm_forward_t(const ResNormArgs& a, const RnShape& s, cudaStream_t st) {
+  if (s.more) return resnorm_forward_s<DT, FAST, SPLIT, RN_MORE>(a, s, st);
+  return s.threads > RN_MORE ? resnorm_forward_s<DT, FAST, SPLIT, RN_LARGE>(a, s, st) : resnorm_forward_s<DT, FAST, SPLIT, RN_THREADS>(a, s, st);
 }
 template <int DT, bool FAST>
 static int resnorm_backward_t(const ResNormArgs& a, const RnShape& s, cudaStream_t st) {
@@ -626,12 +640,8 @@ static int resnorm_t(const ResNormArgs& a, bool backward, cudaStream_t st) {
   const bool fast = a.w_dtype == CODE && ((!a.gate && !a.scale) || a.m_dtype == CODE);
   const RnShape s = rn_shape(a.M, a.K, !backward && a.codes, backward);
   if (backward) return fast ? resnorm_backward_t<DT, true>(a, s, st) : resnorm_backward_t<DT, false>(a, s, st);
-  const bool wide = s.threads > RN_THREADS;  // only of split rows
-  if (fast)
-    return wide ? resnorm_forward_t<DT, true, true, true>(a, s, st)
-                : s.split ? resnorm_forward_t<DT, true, true, false>(a, s, st) : resnorm_forward_t<DT, true, false, false>(a, s, st);
-  return wide ? resnorm_forward_t<DT, false, true, true>(a, s, st)
-              : s.split ? resnorm_forward_t<DT, false, true, false>(a, s, st) : resnorm_forward_t<DT, false, false, false>(a, s, st);
+  if (fast) return s.split ? resnorm_forward_t<DT, true, true>(a, s, st) : resnorm_forward_t<DT, true, false>(a, s, st);
+  return s.split ? resnorm_forward_t<DT, false, true>(a, s, st) : resnorm_forward_t<DT, false, false>(a, s, st);
 }
 int resnorm_launch(const ResNormArgs& a, bool backward, cudaStream_t st) {
   if (backward && a.M == 0) {  // nothing to add up
