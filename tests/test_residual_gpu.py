@@ -45,7 +45,8 @@ def dealt(kind, m, mods):
 
 CASES = [(1, 256, 1, "runs"), (2, 512, 0, "none"), (7, 5120, 2, "runs"), (8, 5376, 3, "tokens"), (33, 1280, 4, "many"),
          (65, 16384, 2, "runs"), (130, 8448, 1, "tokens"), (257, 768, 2, "none"), (1031, 1280, 3, "runs"), (5000, 256, 2, "runs"),
-         (3, 14336, 0, "none"), (2100, 2560, 2, "tokens")]
+         (3, 14336, 0, "none"), (2100, 2560, 2, "tokens"), (70, 6144, 2, "runs"), (39, 8192, 2, "tokens"), (150, 4096, 3, "runs"),
+         (41, 8704, 2, "runs"), (29, 11264, 3, "many"), (150, 14080, 2, "runs"), (2, 7936, 0, "none")]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -78,7 +79,8 @@ def test_forward(m, k, mods, kind, dtype):
 
 
 GRADS = [(1, 8, 1, "runs"), (3, 136, 0, "none"), (17, 1288, 2, "runs"), (130, 5376, 3, "tokens"), (517, 1288, 0, "none"),
-         (600, 16384, 1, "runs"), (2050, 640, 4, "many"), (300, 8200, 2, "none"), (40, 264, 2, "tokens")]
+         (600, 16384, 1, "runs"), (2050, 640, 4, "many"), (300, 8200, 2, "none"), (40, 264, 2, "tokens"),
+         (70, 6400, 2, "runs"), (90, 6152, 3, "tokens"), (33, 13568, 2, "runs")]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
