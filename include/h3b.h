@@ -250,8 +250,8 @@ int h3b_low_rank(const void* x, int64_t ldx, const void* a, const void* b, const
                  int64_t ldo, int dtype, int64_t M, int64_t K, int64_t N, int rank, int64_t adapters, const float* scales,
                  const int32_t* plan, void* hidden, void* workspace, size_t ws_bytes, void* stream);
 /* Gradients with respect to x, a and b (each may be NULL: not asked for); that of base is grad_out itself.  hidden as
- * h3b_low_rank left it for the same arguments.  Adapters without rows and rows without an adapter get zeros.  Every sum has a
- * fixed order: the same call gives the same bits. */
+ * h3b_low_rank left it for the same arguments.  dx, da and db overlap no input and not one another.  Adapters without rows and rows
+ * without an adapter get zeros.  Every sum has a fixed order: the same call gives the same bits. */
 int h3b_low_rank_backward(const void* grad_out, int64_t ldgo, const void* x, int64_t ldx, const void* a, const void* b,
                           const void* hidden, void* dx, int64_t lddx, void* da, void* db, int dtype, int64_t M, int64_t K,
                           int64_t N, int rank, int64_t adapters, const float* scales, const int32_t* plan, void* workspace,

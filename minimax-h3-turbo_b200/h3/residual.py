@@ -106,8 +106,8 @@ class _Problem:
         for t in (gate, shift, scale):
             if t is None:
                 continue
-            if t.dim() != 2 or t.shape[1] != self.k or t.shape[0] != n_rows or t.device != self.dev:
-                raise ValueError(f"residual_norm: gate, shift and scale must be [rows, {self.k}] alike on {self.dev}")
+            if t.dim() != 2 or t.shape[1] != self.k or t.shape[0] != n_rows or n_rows < 1 or t.device != self.dev:
+                raise ValueError(f"residual_norm: gate, shift and scale must be [rows, {self.k}] alike on {self.dev}, of a row at least")
             alike = alike and t.dtype is dt and t.is_contiguous() and t.data_ptr() % 16 == 0
         if not alike:
             mods = [t for t in (gate, shift, scale) if t is not None]

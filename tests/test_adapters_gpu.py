@@ -348,3 +348,17 @@ def test_columns_of_one_tensor_as_input_and_output():
     with pytest.raises(ValueError, match="overlap"):  # a row further, half a row back
         flat = torch.zeros(31 * 512, dtype=x.dtype, device=DEV)
         ad.low_rank(flat[:30 * 512].view(30, 512)[:, :256], a, b, p, out=flat[384:384 + 30 * 512].view(30, 512)[:, :384])
+
+
+@pytest.mark.parametrize("r", [1, 7, 24, 127])
+def test_gradients_of_single_rows_and_of_none(r):
+    """An adapter of one row, one of none, one of some: the first's gradients are outer products, the second's zeros."""
+    x, a, b, base, scales = make(9, 136, 264, r, 3, torch.float16)
+    rows = torch.tensor([2, 0, 2, 2, -1, 2, 2, 5, 2], device=DEV)
+    p = ad.plan(rows, 3)
+    _, hidden = ad.low_rank(x, a, b, p, base=base, scales=scales, return_hidden=True)
+    dx, da, db = ad.low_rank_backward(base, x, a, b, p, hidden, scales=scales)
+    want, tol = ref.backward(base, x, a, b, rows, scales)
+    for name, u, v, t in zip(("dx", "da", "db"), (dx, da, db), want, tol):
+        ref.check(u, v, t, name)
+    assert not da[1].any() and not db[1].any() and not dx[4].any() and not dx[7].any()

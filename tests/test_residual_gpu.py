@@ -288,3 +288,23 @@ def test_calls_in_a_row(m, k):
     xs.copy_(x.flip(0))
     graph.replay()
     assert torch.equal(z, other)
+
+
+def test_modulation_of_no_rows_is_refused():
+    """An empty gate has no address, which would read as no gate at all: y added everywhere where it belongs nowhere."""
+    x, y, w, gate, shift, scale = make(4, 512, 2, torch.bfloat16, 14)
+    for kw in (dict(gate=gate[:0]), dict(shift=shift[:0], scale=scale[:0])):
+        with pytest.raises(ValueError, match="a row at least"):
+            rs.residual_norm(x, y, w, EPS, **kw)
+    with pytest.raises(ValueError, match="a row at least"):
+        rs.residual_norm_backward(x, x, x, torch.ones(4, device=DEV), w, gate=gate[:0])
+    assert torch.equal(rs.residual_norm(x, y, w, EPS, gate=gate, codes=False).x, x)  # a gate whose rows no token has
+
+
+def test_one_modulation_row_and_one_token():
+    x, y, w, gate, shift, scale = make(1, 256, 1, torch.float16, 15)
+    r = rs.residual_norm(x, y, w, EPS, gate=gate, shift=shift, scale=scale, segments=[(0, 1, 0)], hidden=True)
+    wide = [torch.stack([t[0], t[0]])[:1].expand(1, 256) for t in (gate, shift, scale)]
+    q = rs.residual_norm(x, y, w, EPS, gate=wide[0], shift=wide[1], scale=wide[2], segments=[(0, 1, 0)], hidden=True)
+    assert all(torch.equal(a, b) for a, b in zip(r, q))
+    ref.check(r.x, *ref.stream(x, y, gate, torch.zeros(1, dtype=torch.long, device=DEV)), "t")
