@@ -303,9 +303,9 @@ __device__ __forceinline__ void lr_stage8(uint32_t dst, const T* row, int j, int
 // Letting the second product's CTAs in early, to have base on the way at the end of this one, made both slower (together 150 -> 192
 // us for 12090 rows 5120 -> 15360).
 constexpr int LR_XPART = LR_TILE * 128;  // 64 channels of 128 rows
-constexpr int LR_SHRINK_THREADS = 160;
+constexpr int LR_FIRST_THREADS = 160;
 template <int RPM, bool W_ROWS>  // the largest rp of this variant: 64 or 128
-struct LrShrinkCfg {
+struct LrFirstCfg {
   // A stage has PB parts of 64 channels: 256 bytes of every row at a time where they fit (59440 rows 5120 -> 5120 of rank 64, both
   // products: 356 us, with 128 bytes 404)
   static constexpr int PB = RPM == 64 ? 2 : 1, STAGES = RPM == 64 ? 2 : 3, CTAS = 2, KC = 64 * PB;
@@ -342,10 +342,10 @@ __device__ __forceinline__ void lr_gather(float* red, int ld, int row0, int rp) 
 }
 
 template <typename T, bool W_ROWS, int RPM>
-__global__ void __launch_bounds__(LR_SHRINK_THREADS) lr_shrink_kernel(const LrPlan p, const T* x, int64_t ldx, int64_t C,
+__global__ void __launch_bounds__(LR_FIRST_THREADS) lr_first_kernel(const LrPlan p, const T* x, int64_t ldx, int64_t C,
                                                                       const T* w, int rank, int rp, int R, const float* scales, const LrHidden out,
                                                                       int splits) {
-  using Cfg = LrShrinkCfg<RPM, W_ROWS>;
+  using Cfg = LrFirstCfg<RPM, W_ROWS>;
   constexpr int STAGES = Cfg::STAGES, PB = Cfg::PB, KC = Cfg::KC;
   extern __shared__ __align__(1024) unsigned char lr_smem[];
   __shared__ uint64_t full[STAGES], empty[STAGES], done;
@@ -510,7 +510,7 @@ __global__ void __launch_bounds__(LR_SHRINK_THREADS) lr_shrink_kernel(const LrPl
 // rank 16 with base: 115 us, 6.5 TB/s; 59440 x 5120 of rank 64: 241 us, 5.1 TB/s; dx of 12090 x 5120, rank 32: 26 us, its bytes 19.
 constexpr int LR_THREADS = 256;
 template <int NQ, bool W_ROWS, bool BASE>  // 16 NQ: the largest rp of this variant
-struct LrExpandCfg {
+struct LrSecondCfg {
   // Columns of a CTA: 128 with base, whose numbers wait in registers.  256 where that does not count (no base), or counts less than what W
   // and H take of L2 (ranks from 33 on: 59440 rows 5120 -> 5120 of rank 64 in all 411 us, with 128 columns 430).
   static constexpr int CB = BASE && NQ <= 2 ? 2 : 4, COLS = 64 * CB;
@@ -520,10 +520,10 @@ struct LrExpandCfg {
   static constexpr int CTAS = NQ <= (BASE ? 2 : 4) ? 3 : 2;
 };
 template <typename T, bool W_ROWS, bool BASE, int NQ>
-__global__ void __launch_bounds__(LR_THREADS, LrExpandCfg<NQ, W_ROWS, BASE>::CTAS)
-    lr_expand_kernel(const LrPlan p, const LrHidden hid, const T* w, int rank, int rp, int R, const T* base, int64_t ldb, T* out,
+__global__ void __launch_bounds__(LR_THREADS, LrSecondCfg<NQ, W_ROWS, BASE>::CTAS)
+    lr_second_kernel(const LrPlan p, const LrHidden hid, const T* w, int rank, int rp, int R, const T* base, int64_t ldb, T* out,
                      int64_t ldo, int64_t N, int parts, bool wide) {
-  using Cfg = LrExpandCfg<NQ, W_ROWS, BASE>;
+  using Cfg = LrSecondCfg<NQ, W_ROWS, BASE>;
   constexpr int CB = Cfg::CB, COLS = Cfg::COLS, LDW = Cfg::LDW;
   extern __shared__ __align__(1024) unsigned char lr_smem[];
   after_previous();
@@ -1161,47 +1161,47 @@ static int lr_launch(const char* what, void (*kernel)(KA...), std::atomic<bool> 
 }
 static bool lr_wide(const void* p, int64_t ld) { return !p || (ld % 16 == 0 && reinterpret_cast<uintptr_t>(p) % 32 == 0); }
 template <typename T, bool W_ROWS, int RPM>
-static int lr_shrink_s(const LrPlan& p, const T* x, int64_t ldx, int64_t C, const T* w, int rank, int rp, int R, const float* scales,
+static int lr_first_s(const LrPlan& p, const T* x, int64_t ldx, int64_t C, const T* w, int rank, int rp, int R, const float* scales,
                        const LrHidden& h, cudaStream_t st) {
-  using Cfg = LrShrinkCfg<RPM, W_ROWS>;
+  using Cfg = LrFirstCfg<RPM, W_ROWS>;
   static std::atomic<bool> ready[CA_DEVICES];
   const int splits = lr_splits(p.n_tiles, (C + Cfg::KC - 1) / Cfg::KC, 768 / Cfg::KC, Cfg::CTAS);
-  return lr_launch("lr_shrink_kernel", lr_shrink_kernel<T, W_ROWS, RPM>, ready, dim3(static_cast<unsigned>(p.n_tiles * splits)),
-                   LR_SHRINK_THREADS, Cfg::SMEM, splits, st, p, x, ldx, C, w, rank, rp, R, scales, h, splits);
+  return lr_launch("lr_first_kernel", lr_first_kernel<T, W_ROWS, RPM>, ready, dim3(static_cast<unsigned>(p.n_tiles * splits)),
+                   LR_FIRST_THREADS, Cfg::SMEM, splits, st, p, x, ldx, C, w, rank, rp, R, scales, h, splits);
 }
 template <typename T, bool W_ROWS>
-static int lr_shrink(const LrPlan& p, const T* x, int64_t ldx, int64_t C, const T* w, int rank, int R, const float* scales,
+static int lr_first(const LrPlan& p, const T* x, int64_t ldx, int64_t C, const T* w, int rank, int R, const float* scales,
                      const LrHidden& h, cudaStream_t st) {
   const int rp = lr_rp(rank);
-  if (rp <= 64) return lr_shrink_s<T, W_ROWS, 64>(p, x, ldx, C, w, rank, rp, R, scales, h, st);
-  return lr_shrink_s<T, W_ROWS, 128>(p, x, ldx, C, w, rank, rp, R, scales, h, st);
+  if (rp <= 64) return lr_first_s<T, W_ROWS, 64>(p, x, ldx, C, w, rank, rp, R, scales, h, st);
+  return lr_first_s<T, W_ROWS, 128>(p, x, ldx, C, w, rank, rp, R, scales, h, st);
 }
 template <typename T, bool W_ROWS, bool BASE, int NQ>
-static int lr_expand_s(const LrPlan& p, const LrHidden& h, const T* w, int rank, int rp, int R, const T* base, int64_t ldb, T* out,
+static int lr_second_s(const LrPlan& p, const LrHidden& h, const T* w, int rank, int rp, int R, const T* base, int64_t ldb, T* out,
                        int64_t ldo, int64_t N, cudaStream_t st) {
-  using Cfg = LrExpandCfg<NQ, W_ROWS, BASE>;
+  using Cfg = LrSecondCfg<NQ, W_ROWS, BASE>;
   static std::atomic<bool> ready[CA_DEVICES];
   const int parts = static_cast<int>((N + Cfg::COLS - 1) / Cfg::COLS);
-  return lr_launch("lr_expand_kernel", lr_expand_kernel<T, W_ROWS, BASE, NQ>, ready, dim3(static_cast<unsigned>(p.n_tiles * parts)), LR_THREADS,
+  return lr_launch("lr_second_kernel", lr_second_kernel<T, W_ROWS, BASE, NQ>, ready, dim3(static_cast<unsigned>(p.n_tiles * parts)), LR_THREADS,
                    Cfg::SMEM, 1, st, p, h, w, rank, rp, R, base, ldb, out, ldo, N, parts,
                    N % 16 == 0 && lr_wide(base, ldb) && lr_wide(out, ldo));
 }
 // W_ROWS: with or without base; else (dx) without
 template <typename T, bool W_ROWS, int NQ>
-static int lr_expand_b(const LrPlan& p, const LrHidden& h, const T* w, int rank, int rp, int R, const T* base, int64_t ldb, T* out,
+static int lr_second_b(const LrPlan& p, const LrHidden& h, const T* w, int rank, int rp, int R, const T* base, int64_t ldb, T* out,
                        int64_t ldo, int64_t N, cudaStream_t st) {
   if constexpr (W_ROWS)
-    if (base) return lr_expand_s<T, W_ROWS, true, NQ>(p, h, w, rank, rp, R, base, ldb, out, ldo, N, st);
-  return lr_expand_s<T, W_ROWS, false, NQ>(p, h, w, rank, rp, R, nullptr, 0, out, ldo, N, st);
+    if (base) return lr_second_s<T, W_ROWS, true, NQ>(p, h, w, rank, rp, R, base, ldb, out, ldo, N, st);
+  return lr_second_s<T, W_ROWS, false, NQ>(p, h, w, rank, rp, R, nullptr, 0, out, ldo, N, st);
 }
 template <typename T, bool W_ROWS>
-static int lr_expand(const LrPlan& p, const LrHidden& h, const T* w, int rank, int R, const T* base, int64_t ldb, T* out, int64_t ldo,
+static int lr_second(const LrPlan& p, const LrHidden& h, const T* w, int rank, int R, const T* base, int64_t ldb, T* out, int64_t ldo,
                      int64_t N, cudaStream_t st) {
   const int rp = lr_rp(rank);
-  if (rp <= 16) return lr_expand_b<T, W_ROWS, 1>(p, h, w, rank, rp, R, base, ldb, out, ldo, N, st);
-  if (rp <= 32) return lr_expand_b<T, W_ROWS, 2>(p, h, w, rank, rp, R, base, ldb, out, ldo, N, st);
-  if (rp <= 64) return lr_expand_b<T, W_ROWS, 4>(p, h, w, rank, rp, R, base, ldb, out, ldo, N, st);
-  return lr_expand_b<T, W_ROWS, 8>(p, h, w, rank, rp, R, base, ldb, out, ldo, N, st);
+  if (rp <= 16) return lr_second_b<T, W_ROWS, 1>(p, h, w, rank, rp, R, base, ldb, out, ldo, N, st);
+  if (rp <= 32) return lr_second_b<T, W_ROWS, 2>(p, h, w, rank, rp, R, base, ldb, out, ldo, N, st);
+  if (rp <= 64) return lr_second_b<T, W_ROWS, 4>(p, h, w, rank, rp, R, base, ldb, out, ldo, N, st);
+  return lr_second_b<T, W_ROWS, 8>(p, h, w, rank, rp, R, base, ldb, out, ldo, N, st);
 }
 template <typename T, int RPM, int ST>
 static int lr_wgrad_s(const LrPlan& p, const LrWgradSide<T>& a, const LrWgradSide<T>& b, int rank, int R, cudaStream_t st) {
@@ -1251,9 +1251,9 @@ static int lr_forward_t(const LrArgs& a, cudaStream_t st) {
   const int R = static_cast<int>(a.R);
   if (lr_are_few(a.M, a.R, a.rank))
     return lr_few<T>(p, a, h, reinterpret_cast<float*>(static_cast<char*>(a.ws) + lr_space(a.M, a.K, a.N, a.rank, a.R, false).part_a), st);
-  if (int rc = lr_shrink<T, true>(p, static_cast<const T*>(a.x), a.ldx, a.K, static_cast<const T*>(a.a), a.rank, R, a.scales, h, st))
+  if (int rc = lr_first<T, true>(p, static_cast<const T*>(a.x), a.ldx, a.K, static_cast<const T*>(a.a), a.rank, R, a.scales, h, st))
     return rc;
-  return lr_expand<T, true>(p, h, static_cast<const T*>(a.b), a.rank, R, static_cast<const T*>(a.base), a.ldbase, static_cast<T*>(a.out),
+  return lr_second<T, true>(p, h, static_cast<const T*>(a.b), a.rank, R, static_cast<const T*>(a.base), a.ldbase, static_cast<T*>(a.out),
                             a.ldo, a.N, st);
 }
 template <typename T>
@@ -1264,9 +1264,9 @@ static int lr_backward_t(const LrArgs& a, cudaStream_t st) {
   const int R = static_cast<int>(a.R);
   const T *x = static_cast<const T*>(a.x), *go = static_cast<const T*>(a.go);
   if (a.dx || a.da)
-    if (int rc = lr_shrink<T, false>(p, go, a.ldgo, a.N, static_cast<const T*>(a.b), a.rank, R, a.scales, dh, st)) return rc;
+    if (int rc = lr_first<T, false>(p, go, a.ldgo, a.N, static_cast<const T*>(a.b), a.rank, R, a.scales, dh, st)) return rc;
   if (a.dx)
-    if (int rc = lr_expand<T, false>(p, dh, static_cast<const T*>(a.a), a.rank, R, nullptr, 0, static_cast<T*>(a.dx), a.lddx, a.K, st))
+    if (int rc = lr_second<T, false>(p, dh, static_cast<const T*>(a.a), a.rank, R, nullptr, 0, static_cast<T*>(a.dx), a.lddx, a.K, st))
       return rc;
   if (!a.da && !a.db) return H3B_OK;
   char* ws = static_cast<char*>(a.ws);
