@@ -1,8 +1,20 @@
 // Low-rank adapters of many requests beside a shared projection, and their gradients.
 //
 //   out_i = base_i + s_g (x_i A_g^T) B_g^T        g: the adapter of row i; rows without one keep base_i
-//   h_i = s_g x_i A_g^T                           [rank], held in 32 bits until it is an operand of the second product
+//   h_i = s_g x_i A_g^T                           [rank], summed in 32 bits; an operand of the second product
 //   dh_i = s_g go_i B_g,   dx_i = dh_i A_g,   dA_g = sum_i dh_i^T x_i,   dB_g = sum_i go_i^T h_i
+//
+// As operands, h and dh are rounded once: to bf16 where the others are bf16, to tf32 beside fp16 ones.  fp16 itself does not hold
+// them: its numbers span 2^40, products of two of them twice that, and rows, ranks and the other operand may each have a size of
+// their own, so that no power of two per row or rank keeps a number's digits in every sum that it is part of.  tf32 has fp16's 11
+// digits over fp32's range, and every fp16 number is one: the products of fp16 operands with h and dh are tf32 products.  (Operands
+// scaled into fp16 by a power of two per row lost what is 2^-25 of the row's largest number and below, and in the gradients of A and B
+// 2^-25 of the largest of all rows that are added up.  They took 301 us for 12090 rows 5120 -> 15360 of rank 128 where tf32 takes 451, at rank 16 167 and 164; training steps of 12090 rows
+// 5120 -> 5120 269 and 277 at rank 32, 597 and 671 at rank 128.)
+// In bf16 the rounding of h to 8 digits is a choice for speed, which results of 8 digits allow: 1.9e-3 to 2.3e-3 from the exact ones in
+// all, where their own rounding alone is 1.65e-3 and tf32 products come to 1.67e-3, but take 172 us instead of 148 for 12090 rows 5120
+// -> 15360 of rank 16, 570 instead of 359 for 59440 rows 5120 -> 5120 of rank 64, and 273 instead of 205 for a training step of 12090
+// rows 5120 -> 5120 of rank 32.
 //
 // The rows are gone through in the plan's order (by adapter, then by row), in tiles of one adapter's rows; rows are gathered by their
 // numbers, so a batch may hold its requests in any order.
@@ -174,19 +186,28 @@ int lr_plan_launch(const int32_t* rows, int64_t M, int64_t R, int32_t* plan, cud
 }
 
 // ----------------------------------------------------------------------------------------------- hidden rows
-// h (or dh) of every row in the plan's order: rows of rp = rank rounded up to 16 values of the operands' type, and a power of
-// two per row that they are to be multiplied by (1 in bf16): fp16 holds products of fp16 numbers only after scaling.
+// h (or dh) of every row in the plan's order: rows of rp = rank rounded up to 16 numbers, bf16, or tf32 in 32 bits (WIDE)
+template <typename T>
+constexpr bool LR_WIDE = std::is_same_v<T, __half>;
+template <typename T>
+using LrHid = std::conditional_t<LR_WIDE<T>, float, T>;
 static int lr_rp(int rank) { return (rank + 15) / 16 * 16; }
 static size_t lr_up256(size_t v) { return (v + 255) / 256 * 256; }
-size_t lr_hidden_bytes(int64_t M, int rank) {
-  return lr_up256(static_cast<size_t>(M) * lr_rp(rank) * 2) + lr_up256(static_cast<size_t>(M) * 4);
+size_t lr_hidden_bytes(int64_t M, int rank) { return lr_up256(static_cast<size_t>(M) * lr_rp(rank) * 4); }  // of the wider type
+__device__ __forceinline__ float lr_tf32(float v) {  // to the nearest; infinities and NaN stay
+  uint32_t r;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(v));
+  return __uint_as_float(r);
 }
-struct LrHidden {
-  void* h;      // [M][rp]
-  float* mult;  // [M]
-};
-static LrHidden lr_hidden(void* p, int64_t M, int rank) {
-  return LrHidden{p, reinterpret_cast<float*>(static_cast<char*>(p) + lr_up256(static_cast<size_t>(M) * lr_rp(rank) * 2))};
+// 8 numbers of a hidden row
+template <typename T>
+__device__ __forceinline__ void lr_store_hidden(LrHid<T>* to, const float4& u, const float4& v) {
+  if constexpr (LR_WIDE<T>) {
+    *reinterpret_cast<float4*>(to) = make_float4(lr_tf32(u.x), lr_tf32(u.y), lr_tf32(u.z), lr_tf32(u.w));
+    *reinterpret_cast<float4*>(to + 4) = make_float4(lr_tf32(v.x), lr_tf32(v.y), lr_tf32(v.z), lr_tf32(v.w));
+  } else {
+    *reinterpret_cast<uint4*>(to) = make_uint4(pack2<T>(u.x, u.y), pack2<T>(u.z, u.w), pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
+  }
 }
 // ----------------------------------------------------------------------------------------------- common parts of the tile kernels
 // 16 bytes from global to shared memory without passing through registers; zeros where ok is false (nothing is read then)
@@ -232,6 +253,14 @@ __device__ __forceinline__ void lr_mma(float (&d)[4], uint32_t a0, uint32_t a1, 
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// two numbers of each operand's row (k = t, t + 4 of the instruction; which numbers of the sum these are is free, as above): a0, a2 of
+// row g, a1, a3 of row g + 8
+__device__ __forceinline__ void lr_mma_tf32(float (&d)[4], float a0, float a1, float a2, float a3, float2 b) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(__float_as_uint(a0)), "r"(__float_as_uint(a1)), "r"(__float_as_uint(a2)), "r"(__float_as_uint(a3)),
+        "r"(__float_as_uint(b.x)), "r"(__float_as_uint(b.y)));
 }
 // four 8 x 8 matrices of 16-bit numbers, each transposed on the way: lane l gives the address of row l % 8 of matrix l / 8
 __device__ __forceinline__ void lr_ldmatrix_t(uint32_t (&r)[4], uint32_t addr) {
@@ -313,13 +342,6 @@ struct LrFirstCfg {
   static constexpr int STAGE = PB * LR_XPART + (W_ROWS ? PB : RPM / 64) * WPART;
   static constexpr int SMEM = STAGES * STAGE + 1024;
 };
-// The power of two that brings a row whose largest magnitude is `top` into [1, 2), 2^-60 at least (rows below add nothing that
-// fp16 holds; and a row of zeros has no say in the largest power of several rows); 1 for infinities and NaN.
-__device__ __forceinline__ float lr_power(float top) {
-  const int e = (__float_as_int(top) >> 23) & 0xFF;
-  return e >= 253 ? 1.f : __int_as_float(max(e, 127 - 60) << 23);
-}
-
 // This CTA's rows of a tile: the parts of the cluster's S CTAs added up in their order, into its own; by warps 0-3
 template <int S>
 __device__ __forceinline__ void lr_gather(float* red, int ld, int row0, int rp) {
@@ -343,7 +365,7 @@ __device__ __forceinline__ void lr_gather(float* red, int ld, int row0, int rp) 
 
 template <typename T, bool W_ROWS, int RPM>
 __global__ void __launch_bounds__(LR_FIRST_THREADS) lr_first_kernel(const LrPlan p, const T* x, int64_t ldx, int64_t C,
-                                                                      const T* w, int rank, int rp, int R, const float* scales, const LrHidden out,
+                                                                      const T* w, int rank, int rp, int R, const float* scales, LrHid<T>* out,
                                                                       int splits) {
   using Cfg = LrFirstCfg<RPM, W_ROWS>;
   constexpr int STAGES = Cfg::STAGES, PB = Cfg::PB, KC = Cfg::KC;
@@ -474,29 +496,15 @@ __global__ void __launch_bounds__(LR_FIRST_THREADS) lr_first_kernel(const LrPlan
     if (splits == 2) lr_gather<2>(red, ld, row0, rp);
     if (splits == 4) lr_gather<4>(red, ld, row0, rp);
     if (splits == 8) lr_gather<8>(red, ld, row0, rp);
-    if constexpr (std::is_same_v<T, __half>) {  // the rows' powers of two
-      group_sync(1, 128);
-      if (tid < rows) {
-        float top = 0.f;
-        for (int c = 0; c < rp; c += 4) {
-          const float4 v = *reinterpret_cast<const float4*>(red + (row0 + tid) * ld + c);
-          top = fmaxf(fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
-        }
-        const float mult = lr_power(fabsf(scale) * top);
-        red[(row0 + tid) * ld + rp] = mult;  // behind the row
-      }
-    }
     group_sync(1, 128);
     const int lanes = rp / 8;  // 8 numbers to a lane
     for (int e = tid; e < rows * lanes; e += 128) {
       const int r = e / lanes, c = (e - r * lanes) * 8, row = row0 + r;
       if (row >= t.z) break;
       const float* from = red + row * ld + c;
-      const float mult = std::is_same_v<T, __half> ? red[row * ld + rp] : 1.f, by = scale * (1.f / mult);  // a power of two
       const float4 u = *reinterpret_cast<const float4*>(from), v = *reinterpret_cast<const float4*>(from + 4);
-      *reinterpret_cast<uint4*>(static_cast<T*>(out.h) + static_cast<int64_t>(t.y + row) * rp + c) =
-          make_uint4(pack2<T>(u.x * by, u.y * by), pack2<T>(u.z * by, u.w * by), pack2<T>(v.x * by, v.y * by), pack2<T>(v.z * by, v.w * by));
-      if (c == 0) out.mult[t.y + row] = mult;
+      lr_store_hidden<T>(out + static_cast<int64_t>(t.y + row) * rp + c, make_float4(u.x * scale, u.y * scale, u.z * scale, u.w * scale),
+                         make_float4(v.x * scale, v.y * scale, v.z * scale, v.w * scale));
     }
   }
   if (splits > 1) cluster_sync();  // the others have read this CTA's part
@@ -509,22 +517,25 @@ __global__ void __launch_bounds__(LR_FIRST_THREADS) lr_first_kernel(const LrPlan
 // Ranks are filled up with zeros to 16 NQ: leaving products out by the rank cost 13 instructions to a product.  12090 x 15360 of
 // rank 16 with base: 115 us, 6.5 TB/s; 59440 x 5120 of rank 64: 241 us, 5.1 TB/s; dx of 12090 x 5120, rank 32: 26 us, its bytes 19.
 constexpr int LR_THREADS = 256;
-template <int NQ, bool W_ROWS, bool BASE>  // 16 NQ: the largest rp of this variant
+template <int NQ, bool W_ROWS, bool BASE, bool WIDE>  // 16 NQ: the largest rp of this variant
 struct LrSecondCfg {
   // Columns of a CTA: 128 with base, whose numbers wait in registers.  256 where that does not count (no base), or counts less than what W
-  // and H take of L2 (ranks from 33 on: 59440 rows 5120 -> 5120 of rank 64 in all 411 us, with 128 columns 430).
-  static constexpr int CB = BASE && NQ <= 2 ? 2 : 4, COLS = 64 * CB;
+  // and H take of L2 (ranks from 33 on: 59440 rows 5120 -> 5120 of rank 64 in all 411 us, with 128 columns 430).  WIDE with base: 256,
+  // and two CTAs to an SM instead of three, up to rank 64 (12090 rows 5120 -> 15360 of rank 16 164 us, with 128 and three 172; 59440 of
+  // rank 64 522 and 528), then 128 and three (12090 rows of rank 128 451 us, with 256 and two 488)
+  static constexpr int CB = !BASE ? 4 : WIDE ? (NQ <= 4 ? 4 : 2) : NQ <= 2 ? 2 : 4, COLS = 64 * CB;
   // rows of W: [COLS][16 NQ], 32 bytes apart from a multiple of 64; or [16 NQ][COLS], 16 from a multiple of 128: no bank conflicts
   static constexpr int LDW = W_ROWS ? (32 * NQ + 31) / 64 * 64 + 32 : 2 * COLS + 16;
   static constexpr int SMEM = LDW * (W_ROWS ? COLS : 16 * NQ);
-  static constexpr int CTAS = NQ <= (BASE ? 2 : 4) ? 3 : 2;
+  static constexpr int CTAS = !BASE ? (NQ <= 4 ? 3 : 2) : WIDE ? (NQ <= 4 ? 2 : 3) : NQ <= 2 ? 3 : 2;
 };
 template <typename T, bool W_ROWS, bool BASE, int NQ>
-__global__ void __launch_bounds__(LR_THREADS, LrSecondCfg<NQ, W_ROWS, BASE>::CTAS)
-    lr_second_kernel(const LrPlan p, const LrHidden hid, const T* w, int rank, int rp, int R, const T* base, int64_t ldb, T* out,
+__global__ void __launch_bounds__(LR_THREADS, LrSecondCfg<NQ, W_ROWS, BASE, LR_WIDE<T>>::CTAS)
+    lr_second_kernel(const LrPlan p, const LrHid<T>* hid, const T* w, int rank, int rp, int R, const T* base, int64_t ldb, T* out,
                      int64_t ldo, int64_t N, int parts, bool wide) {
-  using Cfg = LrSecondCfg<NQ, W_ROWS, BASE>;
+  using Cfg = LrSecondCfg<NQ, W_ROWS, BASE, LR_WIDE<T>>;
   constexpr int CB = Cfg::CB, COLS = Cfg::COLS, LDW = Cfg::LDW;
+  constexpr bool WIDE = LR_WIDE<T>;
   extern __shared__ __align__(1024) unsigned char lr_smem[];
   after_previous();
   const int tile = blockIdx.x / parts;
@@ -585,40 +596,74 @@ __global__ void __launch_bounds__(LR_THREADS, LrSecondCfg<NQ, W_ROWS, BASE>::CTA
       asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + 48), "r"(u.w) : "memory");
     }
   }
-  // H: this lane's k are 4 t .. 4 t + 3 of every 16 (W_ROWS), or 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+  // H: this lane's k are 4 t .. 4 t + 3 of every 16 (W_ROWS), or 2 t, 2 t + 1, 2 t + 8, 2 t + 9.  Beside fp16 they take twice the
+  // registers and come from L1 at their product instead.
+  const LrHid<T>* hr[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) hr[h] = hid + static_cast<int64_t>(t.y + min(r0 + 8 * h, t.z - 1)) * rp + (W_ROWS ? 4 : 2) * q4;
   uint32_t a[NQ][4];
-  float mult[2], inv[2];
+  if constexpr (!WIDE) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int64_t pos = t.y + min(r0 + 8 * h, t.z - 1);
-    const T* hr = static_cast<const T*>(hid.h) + pos * rp;
-    mult[h] = std::is_same_v<T, __half> ? hid.mult[pos] : 1.f;
-    inv[h] = 1.f / mult[h];
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-      uint2 u = make_uint2(0, 0);
-      if (16 * q < rp) {
-        if constexpr (W_ROWS) u = *reinterpret_cast<const uint2*>(hr + 16 * q + 4 * q4);
-        else u = make_uint2(*reinterpret_cast<const uint32_t*>(hr + 16 * q + 2 * q4), *reinterpret_cast<const uint32_t*>(hr + 16 * q + 2 * q4 + 8));
+      for (int q = 0; q < NQ; ++q) {
+        uint2 u = make_uint2(0, 0);
+        if (16 * q < rp) {
+          if constexpr (W_ROWS) u = *reinterpret_cast<const uint2*>(hr[h] + 16 * q);
+          else u = make_uint2(*reinterpret_cast<const uint32_t*>(hr[h] + 16 * q), *reinterpret_cast<const uint32_t*>(hr[h] + 16 * q + 8));
+        }
+        a[q][h] = u.x, a[q][2 + h] = u.y;
       }
-      a[q][h] = u.x, a[q][2 + h] = u.y;
-    }
   }
   ask();
   lr_copy_wait<0>();
   __syncthreads();
 #pragma unroll
   for (int b = 0; b < CB; ++b) {
-    float d[8][4];  // the sums begin with base (in fp16 over the row's power of two, which is exact)
+    float d[8][4];  // the sums begin with base
 #pragma unroll
     for (int j = 0; j < 8; ++j)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const float2 f = BASE ? lr_unpack2<T>(v[BASE ? b : 0][h][j]) : make_float2(0.f, 0.f);
-        d[j][2 * h] = std::is_same_v<T, __half> ? f.x * inv[h] : f.x;
-        d[j][2 * h + 1] = std::is_same_v<T, __half> ? f.y * inv[h] : f.y;
+        d[j][2 * h] = f.x, d[j][2 * h + 1] = f.y;
       }
-    if constexpr (W_ROWS) {
+    if constexpr (WIDE) {
+      constexpr int AT_ONCE = NQ <= 4 ? 4 : 2;
+#pragma unroll AT_ONCE
+      for (int q = 0; q < NQ; ++q) {
+        if (16 * q >= rp) break;
+        float4 f[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if constexpr (W_ROWS) {
+            f[h] = *reinterpret_cast<const float4*>(hr[h] + 16 * q);
+          } else {
+            const float2 lo = *reinterpret_cast<const float2*>(hr[h] + 16 * q), hi = *reinterpret_cast<const float2*>(hr[h] + 16 * q + 8);
+            f[h] = make_float4(lo.x, lo.y, hi.x, hi.y);
+          }
+        }
+        auto product = [&](float (&to)[4], uint32_t w0, uint32_t w1) {
+          lr_mma_tf32(to, f[0].x, f[1].x, f[0].y, f[1].y, lr_unpack2<T>(w0));
+          lr_mma_tf32(to, f[0].z, f[1].z, f[0].w, f[1].w, lr_unpack2<T>(w1));
+        };
+        if constexpr (W_ROWS) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const uint2 u = *reinterpret_cast<const uint2*>(lr_smem + (64 * b + 8 * j + g) * LDW + 32 * q + 8 * q4);
+            product(d[j], u.x, u.y);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; j += 2) {
+            uint32_t m[4];
+            lr_ldmatrix_t(m, sm + (16 * q + (lane & 15)) * LDW + 2 * (64 * b + 8 * j) + (lane >> 4) * 16);
+            product(d[j], m[0], m[1]);
+            product(d[j + 1], m[2], m[3]);
+          }
+        }
+      }
+    } else if constexpr (W_ROWS) {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
 #pragma unroll
@@ -641,8 +686,7 @@ __global__ void __launch_bounds__(LR_THREADS, LrSecondCfg<NQ, W_ROWS, BASE>::CTA
     for (int h = 0; h < 2; ++h) {
       uint32_t res[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        res[j] = std::is_same_v<T, __half> ? pack2<T>(d[j][2 * h] * mult[h], d[j][2 * h + 1] * mult[h]) : pack2<T>(d[j][2 * h], d[j][2 * h + 1]);
+      for (int j = 0; j < 8; ++j) res[j] = pack2<T>(d[j][2 * h], d[j][2 * h + 1]);
       lr_store16(out + row[h] * ldo + c + 64 * b, row[h] >= 0 ? N - c - 64 * b : 0, wide, res);
     }
   }
@@ -728,11 +772,9 @@ __global__ void __launch_bounds__(LR_FEW_THREADS) lr_few_down_kernel(const LrPla
 template <typename T, int RB>
 __global__ void __launch_bounds__(LR_FEW_THREADS) lr_few_up_kernel(const LrPlan p, const T* b, int rank, int rp, int R, const float* scales,
                                                                    const T* base, int64_t ldb, T* out, int64_t ldo, int64_t N, int columns,
-                                                                   bool wide, const float* part, int splits, const LrHidden hid, bool keep) {
+                                                                   bool wide, const float* part, int splits, LrHid<T>* hid, bool keep) {
   constexpr int KB = (RB + 1) / 2, AT_ONCE = KB > 2 ? 4 : 8;  // blocks of 32 ranks; products whose weights are held
-  __shared__ float h[8][16 * RB];
-  __shared__ __align__(16) T hs[8][32 * KB + 8];
-  __shared__ float mults[8];
+  __shared__ __align__(16) LrHid<T> hs[8][32 * KB + 8];
   const int tile = blockIdx.x / columns, at = blockIdx.x - tile * columns;
   const int4 t = p.few[tile];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q4 = lane & 3;
@@ -768,41 +810,30 @@ __global__ void __launch_bounds__(LR_FEW_THREADS) lr_few_up_kernel(const LrPlan 
       if (n0 + 2 * j < N && q4 * 64 < rank) lr_prefetch(bg + (n0 + 2 * j) * rank + q4 * 64);
   }
   after_previous();
-  // ---- h: the splits' parts; a row's power of two (fp16); the operand of this product
+  // ---- h: the splits' parts added up, rounded as an operand of this product; zeros for rows and ranks that are not there
   const float scale = scales ? scales[t.x] : 1.f;
-  for (int e = tid; e < t.z * rp; e += LR_FEW_THREADS) {
-    const float* from = part + static_cast<int64_t>(tile) * splits * 8 * rp + e;
-    float sum = 0.f;
-#pragma unroll 8
-    for (int s = 0; s < splits; ++s) sum += from[static_cast<int64_t>(s) * 8 * rp];
-    h[e / rp][e % rp] = sum * scale;
-  }
-  __syncthreads();
   const bool first = keep && at == 0;
-  for (int m = warp; m < 8; m += LR_FEW_THREADS / 32) {
-    float mult = 1.f;
-    if constexpr (std::is_same_v<T, __half>) {
-      float top = 0.f;
-      for (int j = lane; j < rp; j += 32) top = fmaxf(top, m < t.z ? fabsf(h[m][j]) : 0.f);
-      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      mult = lr_power(top);
+  for (int e = tid; e < 8 * 32 * KB; e += LR_FEW_THREADS) {
+    const int m = e / (32 * KB), j = e % (32 * KB);
+    const bool ok = m < t.z && j < rp;
+    float sum = 0.f;
+    if (ok) {
+      const float* from = part + static_cast<int64_t>(tile) * splits * 8 * rp + m * rp + j;
+#pragma unroll 8
+      for (int s = 0; s < splits; ++s) sum += from[static_cast<int64_t>(s) * 8 * rp];
     }
-    const float inv = 1.f / mult;
-    for (int j = lane; j < 32 * KB; j += 32) {
-      const T u = lr_t<T>(m < t.z && j < rp ? h[m][j] * inv : 0.f);
-      hs[m][j] = u;
-      if (first && j < rp && m < t.z) static_cast<T*>(hid.h)[static_cast<int64_t>(t.y + m) * rp + j] = u;
-    }
-    if (lane == 0) {
-      mults[m] = mult;
-      if (first && m < t.z) hid.mult[t.y + m] = mult;
-    }
+    LrHid<T> u;
+    if constexpr (LR_WIDE<T>) u = lr_tf32(sum * scale);
+    else u = lr_t<T>(sum * scale);
+    hs[m][j] = u;
+    if (first && ok) hid[static_cast<int64_t>(t.y + m) * rp + j] = u;
   }
   __syncthreads();
   uint4 ha[KB];
+  if constexpr (!LR_WIDE<T>) {
 #pragma unroll
-  for (int k = 0; k < KB; ++k) ha[k] = *reinterpret_cast<const uint4*>(&hs[g][32 * k + 8 * q4]);
-  const float mult = mults[g];
+    for (int k = 0; k < KB; ++k) ha[k] = *reinterpret_cast<const uint4*>(&hs[g][32 * k + 8 * q4]);
+  }
 #pragma unroll
   for (int j0 = 0; j0 < 8; j0 += AT_ONCE) {
     if (j0 > 0) weights(j0);
@@ -811,11 +842,19 @@ __global__ void __launch_bounds__(LR_FEW_THREADS) lr_few_up_kernel(const LrPlan 
       float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < KB; ++k) {
-        lr_mma<T>(d, ha[k].x, 0u, ha[k].y, 0u, w[j][k].x, w[j][k].y);
-        lr_mma<T>(d, ha[k].z, 0u, ha[k].w, 0u, w[j][k].z, w[j][k].w);
+        if constexpr (LR_WIDE<T>) {
+          const float4 lo = *reinterpret_cast<const float4*>(&hs[g][32 * k + 8 * q4]), hi = *reinterpret_cast<const float4*>(&hs[g][32 * k + 8 * q4 + 4]);
+          lr_mma_tf32(d, lo.x, 0.f, lo.y, 0.f, lr_unpack2<T>(w[j][k].x));
+          lr_mma_tf32(d, lo.z, 0.f, lo.w, 0.f, lr_unpack2<T>(w[j][k].y));
+          lr_mma_tf32(d, hi.x, 0.f, hi.y, 0.f, lr_unpack2<T>(w[j][k].z));
+          lr_mma_tf32(d, hi.z, 0.f, hi.w, 0.f, lr_unpack2<T>(w[j][k].w));
+        } else {
+          lr_mma<T>(d, ha[k].x, 0u, ha[k].y, 0u, w[j][k].x, w[j][k].y);
+          lr_mma<T>(d, ha[k].z, 0u, ha[k].w, 0u, w[j][k].z, w[j][k].w);
+        }
       }
       const float2 f = lr_unpack2<T>(v[j0 + j]);
-      v[j0 + j] = pack2<T>(fmaf(d[0], mult, f.x), fmaf(d[1], mult, f.y));
+      v[j0 + j] = pack2<T>(d[0] + f.x, d[1] + f.y);
     }
   }
   lr_store16(out + row * ldo + c, row >= 0 ? N - c : 0, wide, v);
@@ -824,8 +863,8 @@ __global__ void __launch_bounds__(LR_FEW_THREADS) lr_few_up_kernel(const LrPlan 
 // ----------------------------------------------------------------------------------------------- weight gradients
 // D [128 channels, rp] = X^T H over the rows of a unit (a stretch of one adapter's rows): X's columns are M, H's are N, rows are K,
 // all read as they lie in memory.  HBM-bound: X is read once; H comes from L2.  Rows behind the last are zeros in both operands.  One
-// launch does dA (x with dh) and dB (grad_out with h).  fp16: a row's power of two is taken out against the largest of the unit.
-// Warps 0-3 copy, then read the accumulators; warp 4 issues the products.  12090 rows of 5120 and 5120, rank 32: 58 us, 4.3 TB/s (5.0
+// launch does dA (x with dh) and dB (grad_out with h).
+// bf16: warps 0-3 copy, then read the accumulators; warp 4 issues the products.  12090 rows of 5120 and 5120, rank 32: 58 us, 4.3 TB/s (5.0
 // by itself; in a training step dx's way out of L2 is in it), and 7 to 11 us for the sum of the units' parts.  Fewer, longer units
 // took longer (two of these 16 in one CTA 58, four 60, eight 74).
 constexpr int LR_KROWS = 64;  // rows of a stage
@@ -841,12 +880,62 @@ template <typename T>
 struct LrWgradSide {
   const T* x;
   int64_t ldx, C;
-  LrHidden hid;
+  const LrHid<T>* hid;
   T* grad;       // [rank][C] (by_rank) or [C][rank] of every adapter
   float* part;   // [slots][C][rp]
   int blocks;    // of 128 channels
   bool by_rank;
 };
+// Where a CTA of the weight gradients works: its unit's rows (places in order), its side and its first channel
+template <typename T>
+struct LrWgradPart {
+  const LrWgradSide<T>* sd;
+  int64_t col;
+  int adapter, slot, p0, rows;
+  __device__ LrWgradPart(const LrPlan& p, const LrWgradSide<T>& sa, const LrWgradSide<T>& sb, int R) {
+    const int both = sa.blocks + sb.blocks, unit = blockIdx.x / both, block = blockIdx.x - unit * both;
+    const int4 u = p.units[unit];
+    const bool second = block >= sa.blocks;
+    sd = second ? &sb : &sa, col = static_cast<int64_t>(second ? block - sa.blocks : block) * 128;
+    adapter = u.x, slot = u.w, p0 = rows = 0;
+    if (u.z == 0 || u.x >= R) return;  // no rows
+    const int4 first = p.tiles[u.y], last = p.tiles[u.y + u.z - 1];
+    p0 = first.y, rows = last.y + last.z - p0;
+  }
+};
+// A whole gradient of 128 channels from shared memory (`out`: [rank][136] by rank, else [128][rank + 8])
+// to memory, 16 bytes at a time in the order of memory, by 128 threads.  Lanes that wrote their channel's ranks one by one took 223 us
+// for 24 adapters of rank 128 beside 1112 -> 7680.
+__device__ __forceinline__ int lr_grad_ld(bool by_rank, int rank) { return by_rank ? 136 : rank + 8; }
+template <typename T>
+__device__ __forceinline__ void lr_put_gradient(const LrWgradPart<T>& w, const T* out, int rank) {
+  const LrWgradSide<T>& sd = *w.sd;
+  const int tid = threadIdx.x, ld = lr_grad_ld(sd.by_rank, rank);
+  T* const g = sd.grad + static_cast<int64_t>(w.adapter) * rank * sd.C + w.col * (sd.by_rank ? 1 : rank);
+  if (sd.by_rank) {
+    for (int e = tid; e < rank * 16; e += 128) {
+      const int j = e >> 4, i = (e & 15) * 8;
+      if (w.col + i < sd.C) *reinterpret_cast<uint4*>(g + j * sd.C + i) = *reinterpret_cast<const uint4*>(out + j * ld + i);
+    }
+  } else {
+    const bool eights = rank % 8 == 0;
+    const int total = static_cast<int>(min(static_cast<int64_t>(128), sd.C - w.col)) * rank;
+    for (int i = tid * 8; i < total; i += 128 * 8) {
+      const int r = i / rank, k = i - r * rank;
+      if (eights) {
+        *reinterpret_cast<uint4*>(g + i) = *reinterpret_cast<const uint4*>(out + r * ld + k);
+      } else {
+        uint4 u;
+        T* const e = reinterpret_cast<T*>(&u);
+        for (int q = 0, rr = r, kk = k; q < 8; ++q) {
+          e[q] = out[rr * ld + kk];
+          if (++kk == rank) kk = 0, ++rr;
+        }
+        *reinterpret_cast<uint4*>(g + i) = u;
+      }
+    }
+  }
+}
 template <typename T, int RPM, int ST>
 __global__ void __launch_bounds__(160) lr_wgrad_kernel(const LrPlan p, const LrWgradSide<T> sa, const LrWgradSide<T> sb, int rank, int rp,
                                                        int R) {
@@ -855,17 +944,12 @@ __global__ void __launch_bounds__(160) lr_wgrad_kernel(const LrPlan p, const LrW
   __shared__ uint64_t full[ST], empty[ST], done;
   __shared__ uint32_t tmem_at;
   __shared__ int abort_flag;
-  __shared__ float tops[4];
   after_previous();
-  const int both = sa.blocks + sb.blocks, unit = blockIdx.x / both, block = blockIdx.x - unit * both;
-  const int4 u = p.units[unit];
-  if (u.z == 0 || u.x >= R) return;
-  const bool second = block >= sa.blocks;
-  const LrWgradSide<T>& sd = second ? sb : sa;
-  const int64_t col = static_cast<int64_t>(second ? block - sa.blocks : block) * 128;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int4 first = p.tiles[u.y], last = p.tiles[u.y + u.z - 1];
-  const int p0 = first.y, rows = last.y + last.z - p0, n = (rows + LR_KROWS - 1) / LR_KROWS;
+  const LrWgradPart<T> w(p, sa, sb, R);
+  if (w.rows == 0) return;
+  const LrWgradSide<T>& sd = *w.sd;
+  const int64_t col = w.col;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, p0 = w.p0, rows = w.rows, n = (rows + LR_KROWS - 1) / LR_KROWS;
   unsigned char* const base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(lr_smem) + 1023) & ~static_cast<uintptr_t>(1023));
   volatile int* abort = &abort_flag;
   if (warp == 4) {
@@ -877,11 +961,6 @@ __global__ void __launch_bounds__(160) lr_wgrad_kernel(const LrPlan p, const LrW
     }
     tmem_alloc(&tmem_at, lr_tmem_cols(rp));
     tmem_relinquish();
-  } else if (std::is_same_v<T, __half>) {
-    float top = 0.f;
-    for (int i = tid; i < rows; i += 128) top = fmaxf(top, sd.hid.mult[p0 + i]);
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lane == 0) tops[warp] = top;
   }
   tc_fence_before();
   __syncthreads();
@@ -904,10 +983,8 @@ __global__ void __launch_bounds__(160) lr_wgrad_kernel(const LrPlan p, const LrW
     }
     commit_one(&done);
   } else {
-    const float top = std::is_same_v<T, __half> ? fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) : 1.f;
     const int r0 = tid >> 3, ch = tid & 7;
     const uint32_t at = static_cast<uint32_t>(r0 * 128 + ((ch ^ (r0 & 7)) << 4));
-    const T* h = static_cast<const T*>(sd.hid.h);
     int next[4];  // numbers of the next stage's rows
     auto numbers = [&](int i) {
 #pragma unroll
@@ -941,20 +1018,7 @@ __global__ void __launch_bounds__(160) lr_wgrad_kernel(const LrPlan p, const LrW
             for (int j = 0; j < 4; ++j) {
               const int r = i * LR_KROWS + r0 + 16 * j;
               const uint32_t to = dst + Cfg::XBYTES + part * (LR_KROWS * 128) + j * 2048;
-              const T* src = h + static_cast<int64_t>(p0 + r) * rp + k;
-              if constexpr (std::is_same_v<T, __half>) {
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (r < rows) {
-                  v = *reinterpret_cast<const uint4*>(src);
-                  const __half2 f = __float2half2_rn(sd.hid.mult[p0 + r] / top);
-                  __half2* e = reinterpret_cast<__half2*>(&v);
-#pragma unroll
-                  for (int q = 0; q < 4; ++q) e[q] = __hmul2(e[q], f);
-                }
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-              } else {
-                lr_copy16(to, r < rows ? src : h, r < rows);
-              }
+              lr_copy16(to, r < rows ? sd.hid + static_cast<int64_t>(p0 + r) * rp + k : sd.hid, r < rows);
             }
           }
         }
@@ -967,59 +1031,34 @@ __global__ void __launch_bounds__(160) lr_wgrad_kernel(const LrPlan p, const LrW
     }
     warp_wait(&done, 0, abort);
     tc_fence_after();
-    // a channel per lane.  A whole gradient goes out by way of shared memory (every product has read the stages), 16 bytes at a time
-    // in the order of memory: lanes that wrote their channel's ranks one by one took 223 us for 24 adapters of rank 128 beside 1112 ->
-    // 7680
+    // a channel per lane; a whole gradient by way of shared memory (every product has read the stages)
     const int64_t c = col + tid;
-    const bool eights = rank % 8 == 0;
-    const int ld = sd.by_rank ? 136 : rank + 8;
+    const int ld = lr_grad_ld(sd.by_rank, rank);
     T* const out = reinterpret_cast<T*>(base);
     for (int j = 0; j < rp; j += 16) {
       uint32_t v[16];
       tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(warp * 32) << 16) + j, v);
       tmem_ld_wait();
-      if (u.w >= 0) {
-        if (c < sd.C) store_cols_f32(sd.part + (u.w * sd.C + c) * rp + j, v, top, 16);
-      } else if (!sd.by_rank && eights) {
+      if (w.slot >= 0) {
+        if (c < sd.C) store_cols_f32(sd.part + (w.slot * sd.C + c) * rp + j, v, 1.f, 16);
+      } else if (!sd.by_rank && rank % 8 == 0) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          uint32_t w[4];
+          uint32_t o[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) w[k] = pack2<T>(__uint_as_float(v[8 * h + 2 * k]) * top, __uint_as_float(v[8 * h + 2 * k + 1]) * top);
-          if (j + 8 * h < rank) *reinterpret_cast<uint4*>(out + tid * ld + j + 8 * h) = make_uint4(w[0], w[1], w[2], w[3]);
+          for (int k = 0; k < 4; ++k) o[k] = pack2<T>(__uint_as_float(v[8 * h + 2 * k]), __uint_as_float(v[8 * h + 2 * k + 1]));
+          if (j + 8 * h < rank) *reinterpret_cast<uint4*>(out + tid * ld + j + 8 * h) = make_uint4(o[0], o[1], o[2], o[3]);
         }
       } else {
 #pragma unroll
         for (int k = 0; k < 16; ++k)
-          if (j + k < rank) out[sd.by_rank ? (j + k) * ld + tid : tid * ld + j + k] = lr_t<T>(__uint_as_float(v[k]) * top);
+          if (j + k < rank) out[sd.by_rank ? (j + k) * ld + tid : tid * ld + j + k] = lr_t<T>(__uint_as_float(v[k]));
       }
       __syncwarp();
     }
-    if (u.w < 0) {
+    if (w.slot < 0) {
       group_sync(1, 128);
-      T* const g = sd.grad + static_cast<int64_t>(u.x) * rank * sd.C + col * (sd.by_rank ? 1 : rank);
-      if (sd.by_rank) {
-        for (int e = tid; e < rank * 16; e += 128) {
-          const int j = e >> 4, i = (e & 15) * 8;
-          if (col + i < sd.C) *reinterpret_cast<uint4*>(g + j * sd.C + i) = *reinterpret_cast<const uint4*>(out + j * ld + i);
-        }
-      } else {
-        const int total = static_cast<int>(min(static_cast<int64_t>(128), sd.C - col)) * rank;
-        for (int i = tid * 8; i < total; i += 128 * 8) {
-          const int r = i / rank, k = i - r * rank;
-          if (eights) {
-            *reinterpret_cast<uint4*>(g + i) = *reinterpret_cast<const uint4*>(out + r * ld + k);
-          } else {
-            uint4 w;
-            T* const e = reinterpret_cast<T*>(&w);
-            for (int q = 0, rr = r, kk = k; q < 8; ++q) {
-              e[q] = out[rr * ld + kk];
-              if (++kk == rank) kk = 0, ++rr;
-            }
-            *reinterpret_cast<uint4*>(g + i) = w;
-          }
-        }
-      }
+      lr_put_gradient(w, out, rank);
     }
     tc_fence_before();
   }
@@ -1028,6 +1067,129 @@ __global__ void __launch_bounds__(160) lr_wgrad_kernel(const LrPlan p, const LrW
     tc_fence_after();
     tmem_dealloc(tmem, lr_tmem_cols(rp));
   }
+}
+// fp16: H is tf32, which tcgen05 takes with the contraction contiguous alone; X and H lie the other way.  So the products are those of
+// mma.sync: a warp has 32 channels, ldmatrix turns X on the way to the fragments, its numbers become tf32 there (they all are), and a
+// lane takes two neighbouring ranks as the n of two products.  Rows in stages of 32, three of them, or one where the adapters have no
+// more rows than that on average.
+constexpr int LR_WROWS = 32;
+template <int RPM, int ST>
+struct LrWgradWideCfg {
+  static constexpr int LDX = 136 * 2;  // bytes of a row of X: 16 from a multiple of 128, no bank conflicts
+  static constexpr int XBYTES = LR_WROWS * LDX, STAGE = XBYTES + LR_WROWS * (RPM + 4) * 4, OUT = 128 * (RPM + 8) * 2 + 1024;
+  static constexpr int SMEM = ST * STAGE > OUT ? ST * STAGE : OUT;
+  static constexpr int CTAS = RPM == 64 ? 4 : 3;
+};
+template <typename T, int RPM, int ST>
+__global__ void __launch_bounds__(128, LrWgradWideCfg<RPM, ST>::CTAS)
+    lr_wgrad_wide_kernel(const LrPlan p, const LrWgradSide<T> sa, const LrWgradSide<T> sb, int rank, int rp, int R) {
+  using Cfg = LrWgradWideCfg<RPM, ST>;
+  extern __shared__ __align__(1024) unsigned char lr_smem[];
+  after_previous();
+  const LrWgradPart<T> w(p, sa, sb, R);
+  if (w.rows == 0) return;
+  const LrWgradSide<T>& sd = *w.sd;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q4 = lane & 3;
+  const int rows = w.rows, n = (rows + LR_WROWS - 1) / LR_WROWS, ldh = rp + 4;  // numbers of a row of H: its reads touch every bank once
+  const uint32_t sm = smem_u32(lr_smem);
+  float acc[2][RPM / 16][2][4];  // [16 channels][16 ranks][product]
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int b = 0; b < RPM / 16; ++b)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[m][b][e / 4][e % 4] = 0.f;
+  const int r0 = tid >> 4, ch = (tid & 15) * 8;  // 16 lanes have a row's 256 bytes; rows r0, r0 + 8, ...
+  const bool in = w.col + ch < sd.C;
+  int next[4];
+  auto numbers = [&](int i) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r = i * LR_WROWS + r0 + 8 * j;
+      next[j] = r < rows ? p.order[w.p0 + r] : -1;
+    }
+  };
+  auto bring = [&](int i) {  // stage i, and the numbers of the next one's rows
+    if (i < n) {
+      const uint32_t xs = sm + i % ST * Cfg::STAGE, hs = xs + Cfg::XBYTES;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool ok = next[j] >= 0 && in;
+        lr_copy16(xs + (r0 + 8 * j) * Cfg::LDX + ch * 2, ok ? sd.x + next[j] * sd.ldx + w.col + ch : sd.x, ok);
+      }
+      const int fours = rp / 4;
+      for (int e = tid; e < LR_WROWS * fours; e += 128) {
+        const int r = e / fours, k = (e - r * fours) * 4, at = i * LR_WROWS + r;
+        lr_copy16(hs + (r * ldh + k) * 4, at < rows ? sd.hid + static_cast<int64_t>(w.p0 + at) * rp + k : sd.hid, at < rows);
+      }
+      if (i + 1 < n) numbers(i + 1);
+    }
+    lr_copy_commit();
+  };
+  numbers(0);
+  for (int i = 0; i < ST - 1; ++i) bring(i);
+  for (int i = 0; i < n; ++i) {
+    if (ST == 1) bring(i);
+    lr_copy_wait<ST == 1 ? 0 : ST - 2>();
+    __syncthreads();  // stage i is there, and everyone is through with the one before
+    if (ST > 1) bring(i + ST - 1);
+    const uint32_t xs = sm + i % ST * Cfg::STAGE + (warp * 32) * 2;
+    const float* hs = reinterpret_cast<const float*>(lr_smem + i % ST * Cfg::STAGE + Cfg::XBYTES);
+#pragma unroll
+    for (int k = 0; k < LR_WROWS; k += 16) {
+      if (i * LR_WROWS + k >= rows) break;
+      float2 a[2][4];  // rows 2 t, 2 t + 1 of channel g; of g + 8; rows 2 t + 8, 2 t + 9 of both
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        uint32_t u[4];
+        lr_ldmatrix_t(u, xs + (k + (lane >> 4) * 8 + (lane & 7)) * Cfg::LDX + (16 * m + (lane >> 3 & 1) * 8) * 2);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[m][e] = lr_unpack2<T>(u[e]);
+      }
+      const float* const h = hs + (k + 2 * q4) * ldh + 2 * g;
+#pragma unroll
+      for (int b = 0; b < RPM / 16; ++b) {
+        if (16 * b >= rp) break;
+        const float2 h0 = *reinterpret_cast<const float2*>(h + 16 * b), h1 = *reinterpret_cast<const float2*>(h + ldh + 16 * b);
+        const float2 h8 = *reinterpret_cast<const float2*>(h + 8 * ldh + 16 * b), h9 = *reinterpret_cast<const float2*>(h + 9 * ldh + 16 * b);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          lr_mma_tf32(acc[m][b][0], a[m][0].x, a[m][1].x, a[m][0].y, a[m][1].y, make_float2(h0.x, h1.x));
+          lr_mma_tf32(acc[m][b][1], a[m][0].x, a[m][1].x, a[m][0].y, a[m][1].y, make_float2(h0.y, h1.y));
+          lr_mma_tf32(acc[m][b][0], a[m][2].x, a[m][3].x, a[m][2].y, a[m][3].y, make_float2(h8.x, h9.x));
+          lr_mma_tf32(acc[m][b][1], a[m][2].x, a[m][3].x, a[m][2].y, a[m][3].y, make_float2(h8.y, h9.y));
+        }
+      }
+    }
+    if (ST == 1) __syncthreads();
+  }
+  lr_copy_wait<0>();
+  __syncthreads();
+  // a lane has ranks 16 b + 4 t .. + 3 of channels g and g + 8: product 0 the even ones, 1 the odd ones
+  T* const out = reinterpret_cast<T*>(lr_smem);
+  const int ld = lr_grad_ld(sd.by_rank, rank);
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int b = 0; b < RPM / 16; ++b)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const float v[4] = {acc[m][b][0][2 * s], acc[m][b][1][2 * s], acc[m][b][0][2 * s + 1], acc[m][b][1][2 * s + 1]};
+        const int c = warp * 32 + 16 * m + 8 * s + g, j = 16 * b + 4 * q4;
+        if (w.slot >= 0) {
+          if (j < rp && w.col + c < sd.C)
+            *reinterpret_cast<float4*>(sd.part + (w.slot * sd.C + w.col + c) * rp + j) = make_float4(v[0], v[1], v[2], v[3]);
+        } else if (!sd.by_rank && rank % 8 == 0) {
+          if (j < rank) *reinterpret_cast<uint2*>(out + c * ld + j) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (j + e < rank) out[sd.by_rank ? (j + e) * ld + c : c * ld + j + e] = lr_t<T>(v[e]);
+        }
+      }
+  if (w.slot >= 0) return;
+  __syncthreads();
+  lr_put_gradient(w, out, rank);
 }
 // The parts of an adapter's units, added up in their order; zeros for adapters without rows.  A CTA adds up to 1024 numbers (lr_chans(rp)
 // channels) of one adapter at a time, four to a thread, so that the loads of 16 parts are on the way at once, and stores them 16 bytes
@@ -1162,7 +1324,7 @@ static int lr_launch(const char* what, void (*kernel)(KA...), std::atomic<bool> 
 static bool lr_wide(const void* p, int64_t ld) { return !p || (ld % 16 == 0 && reinterpret_cast<uintptr_t>(p) % 32 == 0); }
 template <typename T, bool W_ROWS, int RPM>
 static int lr_first_s(const LrPlan& p, const T* x, int64_t ldx, int64_t C, const T* w, int rank, int rp, int R, const float* scales,
-                       const LrHidden& h, cudaStream_t st) {
+                       LrHid<T>* h, cudaStream_t st) {
   using Cfg = LrFirstCfg<RPM, W_ROWS>;
   static std::atomic<bool> ready[CA_DEVICES];
   const int splits = lr_splits(p.n_tiles, (C + Cfg::KC - 1) / Cfg::KC, 768 / Cfg::KC, Cfg::CTAS);
@@ -1171,15 +1333,15 @@ static int lr_first_s(const LrPlan& p, const T* x, int64_t ldx, int64_t C, const
 }
 template <typename T, bool W_ROWS>
 static int lr_first(const LrPlan& p, const T* x, int64_t ldx, int64_t C, const T* w, int rank, int R, const float* scales,
-                     const LrHidden& h, cudaStream_t st) {
+                     LrHid<T>* h, cudaStream_t st) {
   const int rp = lr_rp(rank);
   if (rp <= 64) return lr_first_s<T, W_ROWS, 64>(p, x, ldx, C, w, rank, rp, R, scales, h, st);
   return lr_first_s<T, W_ROWS, 128>(p, x, ldx, C, w, rank, rp, R, scales, h, st);
 }
 template <typename T, bool W_ROWS, bool BASE, int NQ>
-static int lr_second_s(const LrPlan& p, const LrHidden& h, const T* w, int rank, int rp, int R, const T* base, int64_t ldb, T* out,
+static int lr_second_s(const LrPlan& p, const LrHid<T>* h, const T* w, int rank, int rp, int R, const T* base, int64_t ldb, T* out,
                        int64_t ldo, int64_t N, cudaStream_t st) {
-  using Cfg = LrSecondCfg<NQ, W_ROWS, BASE>;
+  using Cfg = LrSecondCfg<NQ, W_ROWS, BASE, LR_WIDE<T>>;
   static std::atomic<bool> ready[CA_DEVICES];
   const int parts = static_cast<int>((N + Cfg::COLS - 1) / Cfg::COLS);
   return lr_launch("lr_second_kernel", lr_second_kernel<T, W_ROWS, BASE, NQ>, ready, dim3(static_cast<unsigned>(p.n_tiles * parts)), LR_THREADS,
@@ -1188,14 +1350,14 @@ static int lr_second_s(const LrPlan& p, const LrHidden& h, const T* w, int rank,
 }
 // W_ROWS: with or without base; else (dx) without
 template <typename T, bool W_ROWS, int NQ>
-static int lr_second_b(const LrPlan& p, const LrHidden& h, const T* w, int rank, int rp, int R, const T* base, int64_t ldb, T* out,
+static int lr_second_b(const LrPlan& p, const LrHid<T>* h, const T* w, int rank, int rp, int R, const T* base, int64_t ldb, T* out,
                        int64_t ldo, int64_t N, cudaStream_t st) {
   if constexpr (W_ROWS)
     if (base) return lr_second_s<T, W_ROWS, true, NQ>(p, h, w, rank, rp, R, base, ldb, out, ldo, N, st);
   return lr_second_s<T, W_ROWS, false, NQ>(p, h, w, rank, rp, R, nullptr, 0, out, ldo, N, st);
 }
 template <typename T, bool W_ROWS>
-static int lr_second(const LrPlan& p, const LrHidden& h, const T* w, int rank, int R, const T* base, int64_t ldb, T* out, int64_t ldo,
+static int lr_second(const LrPlan& p, const LrHid<T>* h, const T* w, int rank, int R, const T* base, int64_t ldb, T* out, int64_t ldo,
                      int64_t N, cudaStream_t st) {
   const int rp = lr_rp(rank);
   if (rp <= 16) return lr_second_b<T, W_ROWS, 1>(p, h, w, rank, rp, R, base, ldb, out, ldo, N, st);
@@ -1206,14 +1368,19 @@ static int lr_second(const LrPlan& p, const LrHidden& h, const T* w, int rank, i
 template <typename T, int RPM, int ST>
 static int lr_wgrad_s(const LrPlan& p, const LrWgradSide<T>& a, const LrWgradSide<T>& b, int rank, int R, cudaStream_t st) {
   static std::atomic<bool> ready[CA_DEVICES];
-  return lr_launch("lr_wgrad_kernel", lr_wgrad_kernel<T, RPM, ST>, ready, dim3(static_cast<unsigned>(p.n_units * (a.blocks + b.blocks))), 160,
-                   LrWgradCfg<RPM, ST>::SMEM, 1, st, p, a, b, rank, lr_rp(rank), R);
+  const dim3 grid(static_cast<unsigned>(p.n_units * (a.blocks + b.blocks)));
+  if constexpr (LR_WIDE<T>)
+    return lr_launch("lr_wgrad_wide_kernel", lr_wgrad_wide_kernel<T, RPM, ST>, ready, grid, 128, LrWgradWideCfg<RPM, ST>::SMEM, 1, st, p, a, b,
+                     rank, lr_rp(rank), R);
+  else
+    return lr_launch("lr_wgrad_kernel", lr_wgrad_kernel<T, RPM, ST>, ready, grid, 160, LrWgradCfg<RPM, ST>::SMEM, 1, st, p, a, b, rank,
+                     lr_rp(rank), R);
 }
 template <typename T, int RPM>
 static int lr_wgrad(const LrPlan& p, const LrWgradSide<T>& a, const LrWgradSide<T>& b, int rank, int64_t M, int R, cudaStream_t st) {
   static std::atomic<bool> joined[CA_DEVICES];
   const int rp = lr_rp(rank);
-  const bool one = M <= LR_KROWS * R;
+  const bool one = M <= (LR_WIDE<T> ? LR_WROWS : LR_KROWS) * R;
   if (int rc = one ? lr_wgrad_s<T, RPM, 1>(p, a, b, rank, R, st) : lr_wgrad_s<T, RPM, 3>(p, a, b, rank, R, st)) return rc;
   const int chans = lr_chans(rp);
   const int ja = static_cast<int>((a.blocks ? a.C + chans - 1 : 0) / chans), jb = static_cast<int>((b.blocks ? b.C + chans - 1 : 0) / chans);
@@ -1222,7 +1389,7 @@ static int lr_wgrad(const LrPlan& p, const LrWgradSide<T>& a, const LrWgradSide<
                    rank, rp);
 }
 template <typename T, int RB>
-static int lr_few_s(const LrPlan& p, const LrArgs& a, int rp, const LrHidden& h, float* part, cudaStream_t st) {
+static int lr_few_s(const LrPlan& p, const LrArgs& a, int rp, LrHid<T>* h, float* part, cudaStream_t st) {
   static std::atomic<bool> ready[2][CA_DEVICES];
   const T* base = static_cast<const T*>(a.base);
   T* out = static_cast<T*>(a.out);
@@ -1237,7 +1404,7 @@ static int lr_few_s(const LrPlan& p, const LrArgs& a, int rp, const LrHidden& h,
                    a.N % 16 == 0 && lr_wide(base, a.ldbase) && lr_wide(out, a.ldo), part, splits, h, a.hidden != nullptr);
 }
 template <typename T>
-static int lr_few(const LrPlan& p, const LrArgs& a, const LrHidden& h, float* part, cudaStream_t st) {
+static int lr_few(const LrPlan& p, const LrArgs& a, LrHid<T>* h, float* part, cudaStream_t st) {
   const int rp = lr_rp(a.rank);
   if (rp <= 16) return lr_few_s<T, 1>(p, a, rp, h, part, st);
   if (rp <= 32) return lr_few_s<T, 2>(p, a, rp, h, part, st);
@@ -1247,7 +1414,7 @@ static int lr_few(const LrPlan& p, const LrArgs& a, const LrHidden& h, float* pa
 template <typename T>
 static int lr_forward_t(const LrArgs& a, cudaStream_t st) {
   const LrPlan p = lr_plan(a.plan, a.M, a.R);
-  const LrHidden h = lr_hidden(a.hidden ? a.hidden : a.ws, a.M, a.rank);
+  LrHid<T>* const h = static_cast<LrHid<T>*>(a.hidden ? a.hidden : a.ws);
   const int R = static_cast<int>(a.R);
   if (lr_are_few(a.M, a.R, a.rank))
     return lr_few<T>(p, a, h, reinterpret_cast<float*>(static_cast<char*>(a.ws) + lr_space(a.M, a.K, a.N, a.rank, a.R, false).part_a), st);
@@ -1260,7 +1427,7 @@ template <typename T>
 static int lr_backward_t(const LrArgs& a, cudaStream_t st) {
   const LrPlan p = lr_plan(a.plan, a.M, a.R);
   const LrSpace s = lr_space(a.M, a.K, a.N, a.rank, a.R, true);
-  const LrHidden h = lr_hidden(a.hidden, a.M, a.rank), dh = lr_hidden(a.ws, a.M, a.rank);
+  LrHid<T> *const h = static_cast<LrHid<T>*>(a.hidden), *const dh = static_cast<LrHid<T>*>(a.ws);
   const int R = static_cast<int>(a.R);
   const T *x = static_cast<const T*>(a.x), *go = static_cast<const T*>(a.go);
   if (a.dx || a.da)
