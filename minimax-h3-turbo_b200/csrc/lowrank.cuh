@@ -480,6 +480,10 @@ __global__ void __launch_bounds__(LR_FIRST_THREADS) lr_first_kernel(const LrPlan
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = 0;
       }
+      if (c + 16 > rank) {  // an infinity in X times a rank that is not there: NaN, which would reach every sum over the row
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = c + i < rank ? v[i] : 0u;
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         *reinterpret_cast<uint4*>(red + tid * ld + c + 4 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
@@ -815,9 +819,8 @@ __global__ void __launch_bounds__(LR_FEW_THREADS) lr_few_up_kernel(const LrPlan 
   const bool first = keep && at == 0;
   for (int e = tid; e < 8 * 32 * KB; e += LR_FEW_THREADS) {
     const int m = e / (32 * KB), j = e % (32 * KB);
-    const bool ok = m < t.z && j < rp;
     float sum = 0.f;
-    if (ok) {
+    if (m < t.z && j < rank) {
       const float* from = part + static_cast<int64_t>(tile) * splits * 8 * rp + m * rp + j;
 #pragma unroll 8
       for (int s = 0; s < splits; ++s) sum += from[static_cast<int64_t>(s) * 8 * rp];
@@ -826,7 +829,7 @@ __global__ void __launch_bounds__(LR_FEW_THREADS) lr_few_up_kernel(const LrPlan 
     if constexpr (LR_WIDE<T>) u = lr_tf32(sum * scale);
     else u = lr_t<T>(sum * scale);
     hs[m][j] = u;
-    if (first && ok) hid[static_cast<int64_t>(t.y + m) * rp + j] = u;
+    if (first && m < t.z && j < rp) hid[static_cast<int64_t>(t.y + m) * rp + j] = u;
   }
   __syncthreads();
   uint4 ha[KB];

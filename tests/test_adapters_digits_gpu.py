@@ -108,3 +108,29 @@ def test_small_ranks_beside_large_ones(m):
     a[0, 0, 0], a[0, 1, 1] = 2.0 ** -4, 2.0 ** 4
     dx, _, _ = ad.low_rank_backward(do, x, a, b, p, hidden)  # dh = 2^14, 2^-8
     assert (dx[:, 0] == 2.0 ** 10).all() and (dx[:, 1] == 2.0 ** -4).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("m", [3, 200])
+@pytest.mark.parametrize("r", [1, 8, 24, 33, 120])
+def test_infinities_of_positive_numbers(r, m, dtype):
+    """Sums of positive numbers of which one is infinite are infinite, whatever the rank is filled up to; other rows keep theirs."""
+    g = torch.Generator(device=DEV).manual_seed(r)
+    x, a, b, do = ((torch.rand(s, generator=g, device=DEV) + 0.5).to(dtype) for s in ((m, 40), (2, r, 40), (2, 72, r), (m, 72)))
+    rows = torch.arange(m, device=DEV) % 2
+    p = ad.plan(rows, 2)
+    inf = float("inf")
+    for first in (True, False):  # of x, then of the output's gradient, both in row 1
+        xi, doi = x.clone(), do.clone()
+        (xi if first else doi)[1, 5] = inf
+        out, hidden = ad.low_rank(xi, a, b, p, return_hidden=True)
+        assert torch.equal(ad.low_rank(xi, a, b, p), out)
+        dx, da, db = ad.low_rank_backward(doi, xi, a, b, p, hidden)
+        others = torch.arange(m, device=DEV) != 1
+        assert out[others].isfinite().all() and dx[others].isfinite().all() and da[0].isfinite().all() and db[0].isfinite().all()
+        if first:  # h is infinite, dh is not
+            assert (out[1] == inf).all() and dx.isfinite().all() and (db[1] == inf).all()
+            assert (da[1, :, 5] == inf).all() and da[1, :, :5].isfinite().all() and da[1, :, 6:].isfinite().all()
+        else:
+            assert out.isfinite().all() and (dx[1] == inf).all() and (da[1] == inf).all()
+            assert (db[1, 5] == inf).all() and db[1, :5].isfinite().all() and db[1, 6:].isfinite().all()
