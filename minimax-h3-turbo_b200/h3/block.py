@@ -427,7 +427,7 @@ class DiTBlock:
     host at the phase boundaries of the attention ("qk_ready", "local_done", "kv_ready", "attn_done") so a caller can
     record CUDA events there.  fuse_residual: between attention and MLP, the gated residual, the norm and fc1's quantiser are
     one pass (residual.residual_norm); it rounds once where the separate operators round after every step, so results differ
-    from theirs in the last bits (off by default)."""
+    from theirs in the last bits (off by default; streams of more than 16384 channels take the separate operators)."""
 
     def __init__(self, heads: int, head_dim: int, norm_eps: float = 1e-5, qk_norm_eps: float = 1e-5,
                  precision: str = "a8", attn_chunk: Optional[int] = None, linear=None, kv_exchange: str = "gather",
@@ -549,13 +549,14 @@ class DiTBlock:
 
     def _fused_mlp(self, x: torch.Tensor, att: torch.Tensor, w: BlockWeights, mod: Modulation, segments: Sequence[Segment],
                    adapters) -> torch.Tensor:
-        """x += gate_a att in place, then the MLP of the normalised x: one pass over the stream up to fc1's codes."""
+        """x += gate_a att in place, then the MLP of the normalised x: one pass over the stream up to fc1's codes (to its input
+        where it takes no codes of blocks of 256)."""
         from . import residual
 
         low = None if adapters is None else adapters.fc1
-        w4 = isinstance(w.fc1, ql.W4A8Weight)
+        codes = residual.reads_codes(w.fc1)
         r = residual.residual_norm(x, att, w.norm2, self.norm_eps, gate=mod.gate_a, shift=mod.shift_m, scale=mod.scale_m,
-                                   segments=segments, codes=w4, hidden=not w4 or low is not None, out=x)
+                                   segments=segments, codes=codes, hidden=not codes or low is not None, out=x)
         f = self._adapted(residual.linear(r, w.fc1), r.hidden, low, None if low is None else adapters.plan)
         return self._fc2(f, w, adapters)
 
@@ -563,10 +564,12 @@ class DiTBlock:
                  sin: torch.Tensor, spec: Optional[ShardSpec] = None, adapters=None) -> torch.Tensor:
         """x: [S_local, hidden] residual stream (updated in place and returned); cos/sin: [S_local, half] for these rows;
         adapters (adapters.BlockAdapters): the low-rank adapters beside the block's linears, their plan of these rows."""
+        from .. import _lib
+
         norm = Prenorm if self._fuse_norm else self.ops.rms_modulate
         h = norm(x, w.norm1, self.norm_eps, mod.shift_a, mod.scale_a, segments)
         att = self.attention(h, w, cos, sin, spec, adapters)
-        if self.fuse_residual:
+        if self.fuse_residual and x.shape[1] <= _lib.MAX_RESIDUAL:
             return self.ops.gate_(x, mod.gate_m, self._fused_mlp(x, att, w, mod, segments, adapters), segments)
         self.ops.gate_(x, mod.gate_a, att, segments)
         h = norm(x, w.norm2, self.norm_eps, mod.shift_m, mod.scale_m, segments)

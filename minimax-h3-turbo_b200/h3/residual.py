@@ -268,15 +268,19 @@ def residual_norm_backward(dt: Optional[torch.Tensor], dh: torch.Tensor, t: torc
     return _backward(dt, dh, t, rstd, weight, gate, scale, segments, need_weight)
 
 
+def reads_codes(w: Weight) -> bool:
+    """Whether `linear` takes this weight's input as codes (W4A8, ConvRot 256) or as hidden rows (any other)."""
+    return isinstance(w, W4A8Weight) and w.convrot == 256
+
+
 def linear(r: ResidualNorm, w: Weight, bias: Optional[torch.Tensor] = None, *, quant_mode: str = "ck") -> torch.Tensor:
-    """The linear that reads h: a W4A8 weight (ConvRot 256) from the codes, a dense one from hidden."""
-    if isinstance(w, W4A8Weight):
+    """The linear that reads h: a W4A8 weight of ConvRot 256 from the codes, any other from hidden."""
+    if reads_codes(w):
         if r.codes is None:
-            raise ValueError("residual.linear: a W4A8 weight reads the codes; ask residual_norm for them")
-        if w.convrot != 256 or w.q.shape[1] * 2 != r.codes.shape[1]:
-            raise ValueError(f"residual.linear: the codes are of {r.codes.shape[1]} channels rotated by blocks of 256, the weight "
-                             f"takes {w.q.shape[1] * 2} by blocks of {w.convrot}")
+            raise ValueError("residual.linear: a W4A8 weight of ConvRot 256 reads the codes; ask residual_norm for them")
+        if w.q.shape[1] * 2 != r.codes.shape[1]:
+            raise ValueError(f"residual.linear: the codes are of {r.codes.shape[1]} channels, the weight takes {w.q.shape[1] * 2}")
         return ql._gemm_codes(r.codes, r.scales, w, bias, out_dtype=r.x.dtype, quant_mode=quant_mode)
     if r.hidden is None:
-        raise ValueError("residual.linear: a dense weight reads hidden; ask residual_norm for it")
-    return ql.linear(r.hidden, w, bias)
+        raise ValueError("residual.linear: a dense weight, or one of another ConvRot than 256, reads hidden; ask residual_norm for it")
+    return ql.linear(r.hidden, w, bias, quant_mode=quant_mode)

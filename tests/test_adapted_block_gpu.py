@@ -8,6 +8,7 @@ from minimax_h3_turbo_b200.h3 import adapters as ad
 from minimax_h3_turbo_b200.h3 import block as blk
 from minimax_h3_turbo_b200.h3 import qlinear as ql
 from minimax_h3_turbo_b200.h3 import residual as rs
+from minimax_h3_turbo_b200.h3.synth import synthetic_w4a8
 
 pytestmark = pytest.mark.gpu
 DEV, HID, FFN, S = tb.DEV, tb.HID, tb.FFN, tb.S
@@ -120,3 +121,34 @@ def test_training_step_of_adapters_over_a_norm():
     torch.autograd.backward([o, t], [do.double(), dt.double()])
     for name, got, want in zip("x y w a b".split(), leaves, dd):
         assert tb._rel(got.grad, want.grad) < 6 * 2.0 ** -8, name
+
+
+@pytest.mark.parametrize("kind", [16, 64, "dense"])
+def test_one_pass_with_an_fc1_that_takes_no_codes(kind):
+    """An fc1 of another ConvRot block, or a dense one, reads the hidden rows of the same pass: the block still gives what the fp32 block on
+    the dequantized weights gives, and the stream is not left halfway."""
+    x, w, mod, seg, cos, sin = tb.make(5)
+    fc1 = synthetic_w4a8(2 * FFN, HID, seed=8, device=DEV, convrot=256 if kind == "dense" else kind)
+    w.fc1 = ql.dequantize(fc1, torch.bfloat16) if kind == "dense" else fc1
+    rows, low = make_adapters(5)
+    for adapters in (None, low):
+        y = blk.DiTBlock(tb.HEADS, tb.HD, fuse_residual=True)(x.clone(), w, mod, seg, cos, sin, adapters=adapters)
+        z = blk.DiTBlock(tb.HEADS, tb.HD)(x.clone(), w, mod, seg, cos, sin, adapters=adapters)
+        # the bound of test_one_pass_and_separate_operators_differ_by_roundings, whose two 8-bit roundings are here too (or none)
+        assert float((y.float() - z.float()).norm()) < 0.03 * float((z.float() - x.float()).norm()) + 2 * 2.0 ** -8 / 3 ** 0.5 * float(z.float().norm())
+    r = rs.residual_norm(x, x, w.norm2, 1e-5, codes=False, hidden=True)
+    assert torch.equal(rs.linear(r, w.fc1), ql.linear(r.hidden, w.fc1))
+    with pytest.raises(ValueError, match="hidden"):
+        rs.linear(rs.residual_norm(x, x, w.norm2, 1e-5), w.fc1)
+
+
+def test_streams_wider_than_the_one_pass_takes_go_separately():
+    wide = 16640
+    g = torch.Generator(device=DEV).manual_seed(3)
+    normal = lambda *s: torch.randn(*s, generator=g, device=DEV).bfloat16()  # noqa: E731
+    _, w, _, seg, cos, sin = tb.make(6)
+    w.qkv, w.out, w.fc1, w.fc2 = normal(3 * INNER, wide) / 128, normal(wide, INNER) / 16, normal(256, wide) / 128, normal(wide, 128) / 16
+    w.norm1, w.norm2 = normal(wide), normal(wide)
+    x, mod = normal(S, wide), blk.Modulation(*(normal(2, wide) for _ in range(6)))
+    a = blk.DiTBlock(tb.HEADS, tb.HD, fuse_residual=True)(x.clone(), w, mod, seg, cos, sin)
+    assert torch.equal(a, blk.DiTBlock(tb.HEADS, tb.HD)(x.clone(), w, mod, seg, cos, sin))
