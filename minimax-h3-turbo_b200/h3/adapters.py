@@ -40,20 +40,22 @@ def plan(rows: Rows, adapters: int, *, count: Optional[int] = None, device=None)
     """The plan of a batch for `adapters` adapters.  rows: an int32 or int64 CUDA tensor [M], the adapter of each row, any
     number outside 0 .. adapters - 1 for none; or segments [(first row, end row, adapter)] with the number of rows `count` and
     their device (rows outside every segment have none, later segments win).  Does not synchronise; the kernels that
-    build it run on the current stream."""
+    build it run on the current stream (a fill per segment; of hundreds of them, pass a tensor), and may be captured."""
     if not 1 <= adapters <= _lib.MAX_ADAPTERS:
         raise ValueError(f"adapters.plan: 1 to {_lib.MAX_ADAPTERS} adapters, got {adapters}")
     if not isinstance(rows, torch.Tensor):
         if count is None or device is None:
             raise ValueError("adapters.plan: segments need the number of rows and their device")
-        index = torch.full((count,), -1, dtype=torch.int32)
-        for first, end, g in rows:
+        segments = list(rows)
+        for first, end, g in segments:
             if not 0 <= first <= end <= count or not 0 <= g < adapters:
                 raise ValueError(f"adapters.plan: segment {(first, end, g)} is out of range for {count} rows and {adapters} adapters")
-            index[first:end] = g
         if torch.device(device).type != "cuda":
             raise RuntimeError("adapters.plan: CUDA tensors only (there is no CPU path)")
-        rows = index.to(device)
+        rows = torch.full((count,), -1, dtype=torch.int32, device=device)
+        for first, end, g in segments:  # filled on the device: a copy from the host would wait for the stream
+            if end > first:
+                rows[first:end].fill_(g)
     elif count is not None or device is not None:
         raise ValueError("adapters.plan: count and device go with segments, not with a tensor of rows")
     if rows.dim() != 1 or rows.dtype not in (torch.int32, torch.int64):

@@ -1,0 +1,49 @@
+"""Calls of the low-rank adapters and the residual's norm as programs make them around the kernels: captured plans, other devices'
+sizes, gradients that a call cannot give, tensors that autograd has kept."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+if torch.cuda.is_available():
+    from minimax_h3_turbo_b200.h3 import adapters as ad
+    from minimax_h3_turbo_b200.h3 import residual as rs
+DEV = "cuda"
+
+
+def make(m=50, k=128, n=64, r=8, adapters=3, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    normal = lambda *s: torch.randn(*s, generator=g, device=DEV).bfloat16()  # noqa: E731
+    return normal(m, k), normal(adapters, r, k) / k ** 0.5, normal(adapters, n, r) / r ** 0.5, normal(m, n)
+
+
+def test_plan_of_segments_is_captured():
+    """No copy from the host and no wait for the stream: both would end the capture with an error."""
+    x, a, b, base = make()
+    segments = [(5, 20, 2), (20, 33, 0), (40, 40, 1), (18, 22, 1)]  # later ones win
+    rows = torch.full((50,), -1, dtype=torch.int32, device=DEV)
+    rows[5:18], rows[18:22], rows[22:33] = 2, 1, 0
+    want = ad.low_rank(x, a, b, ad.plan(rows, 3), base=base)
+    assert torch.equal(ad.low_rank(x, a, b, ad.plan(iter(segments), 3, count=50, device=DEV), base=base), want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ad.low_rank(x, a, b, ad.plan(segments, 3, count=50, device=DEV), base=base)
+    out.zero_()
+    graph.replay()
+    assert torch.equal(out, want)
+    none = ad.plan([], 3, count=50, device=DEV)
+    assert torch.equal(ad.low_rank(x, a, b, none, base=base), base)
+
+
+def test_plan_of_segments_does_not_wait_for_the_stream():
+    done = torch.cuda.Event()
+    big = torch.zeros(1 << 28, device=DEV)
+    ad.plan([(0, 4, 0)], 1, count=8, device=DEV)  # the library is loaded, the memory there
+    torch.cuda.synchronize()
+    for _ in range(200):
+        big.add_(1)  # some 60 ms
+    done.record()
+    p = ad.plan([(0, 4, 0)], 1, count=8, device=DEV)
+    assert not done.query()
+    torch.cuda.synchronize()
+    assert p.rows == 8
