@@ -35,7 +35,8 @@ class ResidualNorm(NamedTuple):
 
 
 @lru_cache(maxsize=4096)
-def _workspace_bytes(m: int, k: int, backward: bool) -> int:
+def _workspace_bytes(m: int, k: int, backward: bool, device: int) -> int:
+    """Asked with `device` current: the number of SMs counts."""
     return _lib.lib().h3b_residual_norm_workspace_bytes(m, k, backward)
 
 
@@ -130,15 +131,19 @@ class _Problem:
         return _rows(t)
 
     def launch(self, fn, args, backward: bool) -> None:
-        n, index = _workspace_bytes(self.m, self.k, backward) if backward else 0, self.dev.index
-        ws = torch.empty(n, dtype=torch.uint8, device=self.dev) if n else None
-        if index == torch.cuda.current_device():
-            rc = fn(*args, _lib.ptr(ws), n, _lib.raw_stream(index))
+        if self.dev.index == torch.cuda.current_device():
+            rc = self._call(fn, args, backward)
         else:
             with torch.cuda.device(self.dev):
-                rc = fn(*args, _lib.ptr(ws), n, _lib.raw_stream(index))
+                rc = self._call(fn, args, backward)
         if rc:
             _lib.check(rc, "residual_norm")
+
+    def _call(self, fn, args, backward: bool) -> int:
+        index = self.dev.index
+        n = _workspace_bytes(self.m, self.k, backward, index) if backward else 0
+        ws = torch.empty(n, dtype=torch.uint8, device=self.dev) if n else None
+        return fn(*args, _lib.ptr(ws), n, _lib.raw_stream(index))
 
 
 def _forward(p: _Problem, x, y, eps, codes, hidden, out) -> ResidualNorm:

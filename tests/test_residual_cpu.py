@@ -78,3 +78,35 @@ def test_cpu_tensors_are_refused():
     x = torch.zeros(4, 256, dtype=torch.bfloat16)
     with pytest.raises(RuntimeError, match="CUDA"):
         rs.residual_norm(x, x, x[0], 1e-5)
+
+
+def test_workspace_is_of_the_device_that_the_call_runs_on(monkeypatch):
+    """GPUs with other numbers of SMs take other workspaces: the size is asked with the stream's device current, and kept for it alone."""
+    import contextlib
+    import types
+
+    current, asked, passed = [0], [], []
+
+    @contextlib.contextmanager
+    def device(d):
+        before, current[0] = current[0], d.index
+        yield
+        current[0] = before
+
+    def size(m, k, backward):
+        asked.append(current[0])
+        return 1000 * (current[0] + 1)
+
+    monkeypatch.setattr(rs._lib, "lib", lambda: types.SimpleNamespace(h3b_residual_norm_workspace_bytes=size))
+    monkeypatch.setattr(rs._lib, "raw_stream", lambda index: 0)
+    monkeypatch.setattr(rs.torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(rs.torch.cuda, "device", device)
+    empty = torch.empty
+    monkeypatch.setattr(rs.torch, "empty", lambda n, dtype, device: empty(n, dtype=dtype))
+    rs._workspace_bytes.cache_clear()
+    for index in (0, 1, 1, 0):
+        p = rs._Problem.__new__(rs._Problem)
+        p.m, p.k, p.dev = 16, 512, types.SimpleNamespace(index=index)
+        p.launch(lambda ws, n, stream: passed.append(n) or 0, (), True)
+    rs._workspace_bytes.cache_clear()
+    assert passed == [1000, 2000, 2000, 1000] and asked == [0, 1]
