@@ -348,11 +348,14 @@ def linear(x: torch.Tensor, w: Weight, a: torch.Tensor, b: torch.Tensor, plan: O
            bias: Optional[torch.Tensor] = None, *, scales: Scales = None, **kw) -> torch.Tensor:
     """The shared projection and its adapters: qlinear.linear(x, w, bias, **kw) + s_g (x A_g^T) B_g^T.  kw as qlinear.linear
     takes it, without input_act (the adapters read x as it is) and with outputs of x's type.  A W4A8 weight has no gradient
-    for x: where x requires one, that raises (a dense weight gives it)."""
+    for x and bias: where one of them requires it, that raises (a dense weight gives both)."""
     if kw.get("input_act") not in (None, "none") or kw.get("out_dtype") not in (None, x.dtype):
         raise ValueError("adapters.linear: input_act and another out_dtype are not taken; apply them outside")
-    if torch.is_grad_enabled() and x.requires_grad and isinstance(w, ql.W4A8Weight):
-        raise RuntimeError("adapters.linear: a W4A8 projection has no gradient for x; detach x, or use a dense weight")
+    if torch.is_grad_enabled() and isinstance(w, ql.W4A8Weight):
+        if x.requires_grad:
+            raise RuntimeError("adapters.linear: a W4A8 projection has no gradient for x; detach x, or use a dense weight")
+        if bias is not None and bias.requires_grad:
+            raise RuntimeError("adapters.linear: a W4A8 projection has no gradient for bias; add the bias outside, or use a dense weight")
     y = ql.linear(x, w, bias, **kw)
     if torch.is_grad_enabled() and (y.requires_grad or a.requires_grad or b.requires_grad):
         return low_rank(x, a, b, plan, base=y, scales=scales)

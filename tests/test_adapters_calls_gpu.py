@@ -47,3 +47,19 @@ def test_plan_of_segments_does_not_wait_for_the_stream():
     assert not done.query()
     torch.cuda.synchronize()
     assert p.rows == 8
+
+
+def test_bias_beside_a_w4a8_projection_gets_its_gradient_or_an_error():
+    from minimax_h3_turbo_b200.h3.synth import synthetic_w4a8
+
+    x, a, b, _ = make(20, 256, 64, 8, 1)
+    w = synthetic_w4a8(64, 256, device=DEV)
+    bias = torch.zeros(64, dtype=torch.bfloat16, device=DEV, requires_grad=True)
+    a.requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradient for bias"):
+        ad.linear(x, w, a, b, None, bias)
+    dense = torch.randn(64, 256, device=DEV).bfloat16()
+    ad.linear(x, dense, a, b, None, bias).sum().backward()
+    assert (bias.grad == 20).all() and a.grad is not None
+    with torch.no_grad():
+        assert torch.equal(ad.linear(x, w, a, b, None, bias), ad.linear(x, w, a, b))
