@@ -220,6 +220,13 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return True
 
 
+def _written(out: torch.Tensor) -> None:
+    """Tells autograd that a kernel has written out, as torch's own in-place operations do: a backward pass that kept its old values
+    then raises instead of using the new ones."""
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)
+
+
 def _forward(p: _Problem, base, out, want_hidden: bool):
     y = torch.empty(p.m, p.n, dtype=p.dt, device=p.dev) if out is None else out
     base = None if base is None else base if base is out else _readable(base)
@@ -301,12 +308,15 @@ def low_rank(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, plan: Optional[A
     a [adapters, rank, K] and b [adapters, N, rank] (or [rank, K] and [N, rank]: one adapter, which without a plan has every
     row); bf16 or fp16 as x, ranks up to 128, K and N multiples of 8.  plan: the batch's, from `plan`.  base [..., N]: what the
     shared projection gave (None: zeros).  scales: a number or fp32 [adapters].  out: a [..., N] tensor to write, which may be
-    base itself (its rows without an adapter are then not touched) and overlaps nothing else; not with gradients.
+    base itself (its rows without an adapter are then not touched) and overlaps nothing else; not with gradients, its own
+    included.
     Differentiable in x, a, b and base (not in scales, nor through hidden); hidden is what low_rank_backward takes."""
     no_tangents("low_rank", x, a, b, base, scales if isinstance(scales, torch.Tensor) else None)
     if torch.is_grad_enabled():
         if isinstance(scales, torch.Tensor) and scales.requires_grad:
             raise ValueError("low_rank: scales have no gradient; detach them")
+        if out is not None and out.requires_grad:
+            raise ValueError("low_rank: out requires a gradient, which what is written there does not have; detach it")
         if x.requires_grad or a.requires_grad or b.requires_grad or (base is not None and base.requires_grad):
             if out is not None:
                 raise ValueError("low_rank: out cannot be given where gradients are recorded")
@@ -328,6 +338,7 @@ def low_rank(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, plan: Optional[A
     if any(_overlap(y, t) for t in (p.x, p.a, p.b, *([] if base2 is None or base2 is y else [base2]))):
         raise ValueError("low_rank: out must not overlap x, a, b or a part of base")
     _, hidden = _forward(p, base2, y, return_hidden)
+    _written(out)
     return (out, hidden) if return_hidden else out
 
 

@@ -19,7 +19,7 @@ import torch
 from .. import _lib
 from . import block as blk
 from . import qlinear as ql
-from .adapters import _overlap
+from .adapters import _overlap, _written
 from .rope import no_tangents
 from .types import W4A8Weight, Weight
 
@@ -245,6 +245,8 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, eps: f
         raise ValueError(f"residual_norm: codes need a width that is a multiple of 256, got {x.shape[-1]}")
     if torch.is_grad_enabled():
         _constants(gate, shift, scale)
+        if out is not None and out.requires_grad:
+            raise ValueError("residual_norm: out requires a gradient, which what is written there does not have; detach it")
         if x.requires_grad or y.requires_grad or weight.requires_grad:
             if out is not None or codes:
                 raise ValueError("residual_norm: out and codes cannot be asked for where gradients are recorded")
@@ -256,7 +258,10 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, eps: f
             raise ValueError("residual_norm: out needs contiguous channels, a 16-byte aligned base and a row stride that is a multiple of 8")
         if out.numel() and any(t.data_ptr() != out.data_ptr() or _ld(t) != _ld(out) for t in (x, y) if _overlap(t, out)):
             raise ValueError("residual_norm: out may be x or y, and overlaps them in no other way")
-    return _forward(p, x, y, float(eps), codes, hidden, out)
+    r = _forward(p, x, y, float(eps), codes, hidden, out)
+    if out is not None:
+        _written(out)
+    return r
 
 
 def residual_norm_backward(dt: Optional[torch.Tensor], dh: torch.Tensor, t: torch.Tensor, rstd: torch.Tensor,

@@ -63,3 +63,45 @@ def test_bias_beside_a_w4a8_projection_gets_its_gradient_or_an_error():
     assert (bias.grad == 20).all() and a.grad is not None
     with torch.no_grad():
         assert torch.equal(ad.linear(x, w, a, b, None, bias), ad.linear(x, w, a, b))
+
+
+def norm_operands(m=8, k=256):
+    x, _, _, y = make(m, k, k)
+    return x, y, torch.ones(k, dtype=torch.bfloat16, device=DEV)
+
+
+def test_out_that_autograd_has_kept():
+    """A value that a backward pass still needs is overwritten: that pass raises, as behind any in-place operation of torch."""
+    x, a, b, base = make()
+    p = ad.plan(torch.zeros(50, dtype=torch.int32, device=DEV), 3)
+    factor = torch.ones(64, dtype=torch.bfloat16, device=DEV, requires_grad=True)
+    z = base * factor  # keeps base
+    ad.low_rank(x, a, b, p, base=base, out=base)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.sum().backward()
+    x, y, w = norm_operands()
+    factor = torch.ones(256, dtype=torch.bfloat16, device=DEV, requires_grad=True)
+    z = x * factor
+    with torch.no_grad():
+        rs.residual_norm(x, y, w, 1e-5, out=x[:])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.sum().backward()
+    with torch.inference_mode():  # has no such count
+        x, a, b, base = make()
+        ad.low_rank(x, a, b, p, base=base, out=base)
+        x, y, w = norm_operands()
+        rs.residual_norm(x, y, w, 1e-5, out=x)
+
+
+def test_out_that_requires_a_gradient_is_refused():
+    x, a, b, base = make()
+    p = ad.plan(torch.zeros(50, dtype=torch.int32, device=DEV), 3)
+    leaf = torch.zeros_like(base, requires_grad=True)
+    with pytest.raises(ValueError, match="out requires a gradient"):
+        ad.low_rank(x, a, b, p, base=base, out=leaf)
+    with torch.no_grad():
+        ad.low_rank(x, a, b, p, base=base, out=leaf)
+    x, y, w = norm_operands()
+    leaf = torch.zeros_like(x, requires_grad=True)
+    with pytest.raises(ValueError, match="out requires a gradient"):
+        rs.residual_norm(x, y, w, 1e-5, out=leaf)
