@@ -233,7 +233,8 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, eps: f
     that `segments` deals out to the tokens as `block.rms_modulate` takes them (ints, or per-token row tensors; numbers
     outside the rows: none).  Without a gate y is added everywhere; with one a token outside every segment keeps x.  Without
     shift and scale (they go together) h is the norm alone.  codes: int8 codes and scales of h rotated, as the W4A8 linears
-    take them (`linear`); hidden: h itself.  out: a [M, K] tensor for t, which may be x or y (not with gradients).
+    take them (`linear`); hidden: h itself.  out: a [M, K] tensor for t, which may be x or y and overlaps nothing else
+    (not with gradients).
     Differentiable in x, y and weight through x and hidden of the result; with gradients the codes, which have none, are
     refused."""
     no_tangents("residual_norm", x, y, weight, gate, shift, scale)
@@ -258,6 +259,10 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, eps: f
             raise ValueError("residual_norm: out needs contiguous channels, a 16-byte aligned base and a row stride that is a multiple of 8")
         if out.numel() and any(t.data_ptr() != out.data_ptr() or _ld(t) != _ld(out) for t in (x, y) if _overlap(t, out)):
             raise ValueError("residual_norm: out may be x or y, and overlaps them in no other way")
+        # the weight and the modulation are read for every row, also behind those that are written
+        w = p.w.as_strided((1, p.k), (_ld(out), 1))  # a row, told apart from columns beside it
+        if any(t is not None and _overlap(t, out) for t in (w, p.gate, p.shift, p.scale)):
+            raise ValueError("residual_norm: out must not overlap weight, gate, shift or scale")
     r = _forward(p, x, y, float(eps), codes, hidden, out)
     if out is not None:
         _written(out)

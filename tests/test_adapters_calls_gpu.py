@@ -105,3 +105,25 @@ def test_out_that_requires_a_gradient_is_refused():
     leaf = torch.zeros_like(x, requires_grad=True)
     with pytest.raises(ValueError, match="out requires a gradient"):
         rs.residual_norm(x, y, w, 1e-5, out=leaf)
+
+
+def test_out_over_what_every_row_reads_is_refused():
+    x, y, w = norm_operands()
+    mods = torch.randn(2, 256, device=DEV).bfloat16()
+    kw = dict(gate=mods, shift=mods, scale=mods, segments=[(0, 8, 1)])
+    flat = torch.cat([x.reshape(-1), w, mods.reshape(-1)])
+    t, wf, mf = flat[:2048].view(8, 256), flat[2048:2304], flat[2304:].view(2, 256)
+    want = rs.residual_norm(x, y, w, 1e-5, **kw)
+    for bad in (dict(gate=t[:2]), dict(shift=t[3:5], scale=mods), dict(shift=mods, scale=t[6:])):
+        with pytest.raises(ValueError, match="must not overlap"):
+            rs.residual_norm(x, y, w, 1e-5, out=t, segments=[(0, 8, 1)], **bad)
+    with pytest.raises(ValueError, match="must not overlap"):
+        rs.residual_norm(x, y, t[2], 1e-5, out=t)
+    # beside one another in one tensor, before it and behind it, and in columns of its own
+    got = rs.residual_norm(t, y, wf, 1e-5, out=t, gate=mf, shift=mf, scale=mf, segments=[(0, 8, 1)])
+    assert torch.equal(got.x, want.x) and torch.equal(got.codes, want.codes)
+    wide = torch.zeros(8, 1024, dtype=x.dtype, device=DEV)
+    wide[:, :256], wide[1, 256:512], wide[2:4, 512:768] = x, w, mods
+    m2 = wide[2:4, 512:768]
+    got = rs.residual_norm(wide[:, :256], y, wide[1, 256:512], 1e-5, out=wide[:, :256], gate=m2, shift=m2, scale=m2, segments=[(0, 8, 1)])
+    assert torch.equal(got.x, want.x) and torch.equal(got.codes, want.codes)
