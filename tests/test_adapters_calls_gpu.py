@@ -127,3 +127,16 @@ def test_out_over_what_every_row_reads_is_refused():
     m2 = wide[2:4, 512:768]
     got = rs.residual_norm(wide[:, :256], y, wide[1, 256:512], 1e-5, out=wide[:, :256], gate=m2, shift=m2, scale=m2, segments=[(0, 8, 1)])
     assert torch.equal(got.x, want.x) and torch.equal(got.codes, want.codes)
+
+
+def test_bias_behind_codes_gets_no_gradient_and_says_so():
+    from minimax_h3_turbo_b200.h3.synth import synthetic_w4a8
+
+    x, y, w = norm_operands()
+    q = synthetic_w4a8(64, 256, device=DEV)
+    bias = torch.zeros(64, dtype=torch.bfloat16, device=DEV, requires_grad=True)
+    r = rs.residual_norm(x, y, w, 1e-5)
+    with pytest.raises(RuntimeError, match="no gradient for bias"):
+        rs.linear(r, q, bias)
+    with torch.no_grad():
+        assert torch.equal(rs.linear(r, q, bias), rs.linear(r, q))
