@@ -134,3 +134,52 @@ def test_infinities_of_positive_numbers(r, m, dtype):
         else:
             assert out.isfinite().all() and (dx[1] == inf).all() and (da[1] == inf).all()
             assert (db[1, 5] == inf).all() and db[1, :5].isfinite().all() and db[1, 6:].isfinite().all()
+
+
+@pytest.mark.parametrize("r", [16, 128])  # rows by eights, rows by 128
+def test_offsets_beyond_32_bits(r):
+    x, a, b, do, rows = spread(140, 256, 384, r, 3, torch.float16, 5)
+    p = ad.plan(rows, 3)
+    want, hidden = ad.low_rank(x, a, b, p, base=do, return_hidden=True)
+    far = torch.empty(140, 1 << 24, dtype=x.dtype, device=DEV)  # the last row begins behind 2^31 numbers
+    xf, df = far[:, :256], far[:, 512:896]
+    xf.copy_(x), df.copy_(do)
+    assert torch.equal(ad.low_rank(xf, a, b, p, base=df), want)
+    for u, v in zip(ad.low_rank_backward(df, xf, a, b, p, hidden), ad.low_rank_backward(do, x, a, b, p, hidden)):
+        assert torch.equal(u, v)
+    assert ad.low_rank(x, a, b, p, base=df, out=df).data_ptr() == df.data_ptr() and torch.equal(df, want)
+
+
+@pytest.mark.parametrize("m,r,adapters", [(12, 40, 3), (300, 16, 4), (300, 128, 2), (2500, 72, 1)])
+def test_training_steps_captured_and_in_two_streams(m, r, adapters):
+    """The gradients of several steps, each on what the one before left, replayed and side by side, as they come one by one."""
+    x, a, b, do, rows = spread(m, 264, 264, r, adapters, torch.float16, 6)
+    p = ad.plan(rows, adapters)
+
+    def steps(x, sync=False):
+        results = []
+        for _ in range(6):
+            out, hidden = ad.low_rank(x, a, b, p, base=x, scales=0.5, return_hidden=True)
+            results += [out, *ad.low_rank_backward(do, x, a, b, p, hidden, scales=0.5)]
+            x = (x + out) / 2
+            if sync:
+                torch.cuda.synchronize()
+        return results
+
+    want, other = steps(x, True), steps(x.flip(0), True)
+    sides, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for side, start in zip(sides, (x, x.flip(0))):
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got.append(steps(start))
+    for side in sides:
+        torch.cuda.current_stream().wait_stream(side)
+    graph, xs = torch.cuda.CUDAGraph(), x.clone()
+    with torch.cuda.graph(graph):
+        captured = steps(xs)
+    graph.replay()
+    same = lambda u, v: all(torch.equal(s, t) for s, t in zip(u, v))  # noqa: E731
+    assert same(got[0], want) and same(got[1], other) and same(captured, want)
+    xs.copy_(x.flip(0))
+    graph.replay()
+    assert same(captured, other)
