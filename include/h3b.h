@@ -242,7 +242,7 @@ int h3b_adapter_plan(const int32_t* rows, int64_t M, int64_t adapters, int32_t* 
  * rank, K] and b [adapters, N, rank] of the same type, contiguous; scales [adapters] fp32 or NULL (1); base NULL: zeros; out may be
  * base (rows without an adapter are then left as they are), and otherwise overlaps nothing.  Sums are held in fp32; s x A^T
  * is rounded once for the second product and for the gradient of b (s grad_out B likewise for those of x and a): to bf16's 8 digits
- * beside bf16 operands, to fp16's 11 digits over fp32's range (tf32) beside fp16 ones.
+ * beside bf16 operands, to fp16's 11 digits over fp32's range (tf32) beside fp16 ones and in the second product of few rows.
  *   hidden     h3b_low_rank_hidden_bytes(M, rank) (256-byte aligned) for the gradients, or NULL
  *   workspace  h3b_low_rank_workspace_bytes(..., backward = 0), 256-byte aligned; the size queries give 0 for refused sizes. */
 size_t h3b_low_rank_hidden_bytes(int64_t M, int rank);

@@ -4,17 +4,17 @@
 //   h_i = s_g x_i A_g^T                           [rank], summed in 32 bits; an operand of the second product
 //   dh_i = s_g go_i B_g,   dx_i = dh_i A_g,   dA_g = sum_i dh_i^T x_i,   dB_g = sum_i go_i^T h_i
 //
-// As operands, h and dh are rounded once: to bf16 where the others are bf16, to tf32 beside fp16 ones.  fp16 itself does not hold
-// them: its numbers span 2^40, products of two of them twice that, and rows, ranks and the other operand may each have a size of
-// their own, so that no power of two per row or rank keeps a number's digits in every sum that it is part of.  tf32 has fp16's 11
-// digits over fp32's range, and every fp16 number is one: the products of fp16 operands with h and dh are tf32 products.  (Operands
-// scaled into fp16 by a power of two per row lost what is 2^-25 of the row's largest number and below, and in the gradients of A and B
-// 2^-25 of the largest of all rows that are added up.  They took 301 us for 12090 rows 5120 -> 15360 of rank 128 where tf32 takes 451, at rank 16 167 and 164; training steps of 12090 rows
-// 5120 -> 5120 269 and 277 at rank 32, 597 and 671 at rank 128.)
-// In bf16 the rounding of h to 8 digits is a choice for speed, which results of 8 digits allow: 1.9e-3 to 2.3e-3 from the exact ones in
-// all, where their own rounding alone is 1.65e-3 and tf32 products come to 1.67e-3, but take 172 us instead of 148 for 12090 rows 5120
-// -> 15360 of rank 16, 570 instead of 359 for 59440 rows 5120 -> 5120 of rank 64, and 273 instead of 205 for a training step of 12090
-// rows 5120 -> 5120 of rank 32.
+// As operands, h and dh are rounded once: to tf32 beside fp16 operands, to bf16 beside bf16 ones (few rows: to tf32).  fp16 itself does
+// not hold them: its numbers span 2^40, products of two of them twice that, and rows, ranks and the other operand may each have a size
+// of their own, so that no power of two per row or rank keeps a number's digits in every sum that it is part of.  tf32 has fp16's 11
+// digits over fp32's range, and every fp16 and bf16 number is one: the products of fp16 operands with h and dh are tf32 products.
+// (Operands scaled into fp16 by a power of two per row lost what is 2^-25 of the row's largest number and below, and in the gradients
+// of A and B 2^-25 of the largest of all rows that are added up.  They took 301 us for 12090 rows 5120 -> 15360 of rank 128 where tf32
+// takes 451, at rank 16 167 and 164; training steps of 12090 rows 5120 -> 5120 269 and 277 at rank 32, 597 and 671 at rank 128.)
+// bf16's 8 digits for h are a choice for speed, which results of 8 digits allow: these are 1.9e-3 to 2.3e-3 off in all, their own
+// rounding alone being 1.65e-3.  tf32 products come to 1.67e-3, but take 172 us instead of 148 for 12090 rows 5120 -> 15360 of rank 16, 570
+// instead of 359 for 59440 rows 5120 -> 5120 of rank 64, and 273 instead of 205 for a training step of 12090 rows 5120 -> 5120 of rank
+// 32.  Few rows wait for weights and cost the same either way (64 rows of 64 adapters of rank 64, 5120 -> 15360, 30 us and 33).
 //
 // The rows are gone through in the plan's order (by adapter, then by row), in tiles of one adapter's rows; rows are gathered by their
 // numbers, so a batch may hold its requests in any order.
@@ -778,7 +778,7 @@ __global__ void __launch_bounds__(LR_FEW_THREADS) lr_few_up_kernel(const LrPlan 
                                                                    const T* base, int64_t ldb, T* out, int64_t ldo, int64_t N, int columns,
                                                                    bool wide, const float* part, int splits, LrHid<T>* hid, bool keep) {
   constexpr int KB = (RB + 1) / 2, AT_ONCE = KB > 2 ? 4 : 8;  // blocks of 32 ranks; products whose weights are held
-  __shared__ __align__(16) LrHid<T> hs[8][32 * KB + 8];
+  __shared__ __align__(16) float hs[8][32 * KB + 8];
   const int tile = blockIdx.x / columns, at = blockIdx.x - tile * columns;
   const int4 t = p.few[tile];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q4 = lane & 3;
@@ -814,7 +814,7 @@ __global__ void __launch_bounds__(LR_FEW_THREADS) lr_few_up_kernel(const LrPlan 
       if (n0 + 2 * j < N && q4 * 64 < rank) lr_prefetch(bg + (n0 + 2 * j) * rank + q4 * 64);
   }
   after_previous();
-  // ---- h: the splits' parts added up, rounded as an operand of this product; zeros for rows and ranks that are not there
+  // ---- h: the splits' parts added up, in tf32 for this product; zeros for rows and ranks that are not there
   const float scale = scales ? scales[t.x] : 1.f;
   const bool first = keep && at == 0;
   for (int e = tid; e < 8 * 32 * KB; e += LR_FEW_THREADS) {
@@ -825,18 +825,15 @@ __global__ void __launch_bounds__(LR_FEW_THREADS) lr_few_up_kernel(const LrPlan 
 #pragma unroll 8
       for (int s = 0; s < splits; ++s) sum += from[static_cast<int64_t>(s) * 8 * rp];
     }
-    LrHid<T> u;
-    if constexpr (LR_WIDE<T>) u = lr_tf32(sum * scale);
-    else u = lr_t<T>(sum * scale);
+    const float u = lr_tf32(sum * scale);
     hs[m][j] = u;
-    if (first && m < t.z && j < rp) hid[static_cast<int64_t>(t.y + m) * rp + j] = u;
+    if (first && m < t.z && j < rp) {
+      LrHid<T>* const to = hid + static_cast<int64_t>(t.y + m) * rp + j;
+      if constexpr (LR_WIDE<T>) *to = u;
+      else *to = lr_t<T>(sum * scale);
+    }
   }
   __syncthreads();
-  uint4 ha[KB];
-  if constexpr (!LR_WIDE<T>) {
-#pragma unroll
-    for (int k = 0; k < KB; ++k) ha[k] = *reinterpret_cast<const uint4*>(&hs[g][32 * k + 8 * q4]);
-  }
 #pragma unroll
   for (int j0 = 0; j0 < 8; j0 += AT_ONCE) {
     if (j0 > 0) weights(j0);
@@ -845,16 +842,11 @@ __global__ void __launch_bounds__(LR_FEW_THREADS) lr_few_up_kernel(const LrPlan 
       float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < KB; ++k) {
-        if constexpr (LR_WIDE<T>) {
-          const float4 lo = *reinterpret_cast<const float4*>(&hs[g][32 * k + 8 * q4]), hi = *reinterpret_cast<const float4*>(&hs[g][32 * k + 8 * q4 + 4]);
-          lr_mma_tf32(d, lo.x, 0.f, lo.y, 0.f, lr_unpack2<T>(w[j][k].x));
-          lr_mma_tf32(d, lo.z, 0.f, lo.w, 0.f, lr_unpack2<T>(w[j][k].y));
-          lr_mma_tf32(d, hi.x, 0.f, hi.y, 0.f, lr_unpack2<T>(w[j][k].z));
-          lr_mma_tf32(d, hi.z, 0.f, hi.w, 0.f, lr_unpack2<T>(w[j][k].w));
-        } else {
-          lr_mma<T>(d, ha[k].x, 0u, ha[k].y, 0u, w[j][k].x, w[j][k].y);
-          lr_mma<T>(d, ha[k].z, 0u, ha[k].w, 0u, w[j][k].z, w[j][k].w);
-        }
+        const float4 lo = *reinterpret_cast<const float4*>(&hs[g][32 * k + 8 * q4]), hi = *reinterpret_cast<const float4*>(&hs[g][32 * k + 8 * q4 + 4]);
+        lr_mma_tf32(d, lo.x, 0.f, lo.y, 0.f, lr_unpack2<T>(w[j][k].x));
+        lr_mma_tf32(d, lo.z, 0.f, lo.w, 0.f, lr_unpack2<T>(w[j][k].y));
+        lr_mma_tf32(d, hi.x, 0.f, hi.y, 0.f, lr_unpack2<T>(w[j][k].z));
+        lr_mma_tf32(d, hi.z, 0.f, hi.w, 0.f, lr_unpack2<T>(w[j][k].w));
       }
       const float2 f = lr_unpack2<T>(v[j0 + j]);
       v[j0 + j] = pack2<T>(d[0] + f.x, d[1] + f.y);
