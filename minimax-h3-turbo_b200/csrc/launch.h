@@ -64,7 +64,6 @@ int qk_norm_rope_launch(void* q, int64_t ldq, void* k, int64_t ldk, int x_dtype,
 int attn_merge_launch(float* acc, float* acc_lse, const void* o, int64_t o_sh, int64_t o_sq, const float* lse, int64_t H,
                       int64_t Q, int D, int first, void* out, int64_t ldo, cudaStream_t st);
 
-// of h3b_residual_norm and h3b_residual_norm_backward
 struct ResNormArgs {  // of h3b_residual_norm and h3b_residual_norm_backward
   const void *x, *y, *w, *gate, *shift, *scale, *dt, *dh;
   void *t, *h, *dx, *dy, *dw;

@@ -520,6 +520,7 @@ __global__ void __launch_bounds__(LR_FIRST_THREADS) lr_first_kernel(const LrPlan
 //   block of 64 columns: lane t has columns 16 t .. 16 t + 15; 2 j, 2 j + 1 of these are product j's n = 2 t, 2 t + 1
 // Ranks are filled up with zeros to 16 NQ: leaving products out by the rank cost 13 instructions to a product.  12090 x 15360 of
 // rank 16 with base: 115 us, 6.5 TB/s; 59440 x 5120 of rank 64: 241 us, 5.1 TB/s; dx of 12090 x 5120, rank 32: 26 us, its bytes 19.
+// WIDE products take twice the tensor cores' time and H's fragments come from L1: 59440 x 5120 of rank 64 410 us, dx 43 us.
 constexpr int LR_THREADS = 256;
 template <int NQ, bool W_ROWS, bool BASE, bool WIDE>  // 16 NQ: the largest rp of this variant
 struct LrSecondCfg {
@@ -699,7 +700,7 @@ __global__ void __launch_bounds__(LR_THREADS, LrSecondCfg<NQ, W_ROWS, BASE, LR_W
 // ----------------------------------------------------------------------------------------------- few rows
 // Up to eight rows of one adapter, as single tokens of many requests have them: everything is the adapters' weights, read once, and
 // latency.  Weights go from memory straight to fragments; K is dealt out to `splits` CTAs of a tile, whose parts the second kernel adds
-// up in a fixed order (4 rows of rank 16, 5120 -> 5120: 6.9 us; 64 rows of 64 adapters of rank 64, 5120 -> 15360: 33 us, 3.9 TB/s of the
+// up in a fixed order (4 rows of rank 16, 5120 -> 5120: 4.3 us; 64 rows of 49 adapters of rank 64, 5120 -> 15360: 30 us, 4.3 TB/s of the
 // weights in use, base and out).  The second kernel is let in when every CTA of the first has begun, and asks for its weights and base
 // before it waits for the parts: the two products' weights come in one stream.  (A cluster of eight CTAs for both products, its parts
 // in distributed shared memory: 16.2 us for one row of rank 64, 91 us for 64 rows of 64 adapters 5120 -> 15360.)
@@ -842,7 +843,8 @@ __global__ void __launch_bounds__(LR_FEW_THREADS) lr_few_up_kernel(const LrPlan 
       float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < KB; ++k) {
-        const float4 lo = *reinterpret_cast<const float4*>(&hs[g][32 * k + 8 * q4]), hi = *reinterpret_cast<const float4*>(&hs[g][32 * k + 8 * q4 + 4]);
+        const float4* const hk = reinterpret_cast<const float4*>(&hs[g][32 * k + 8 * q4]);
+        const float4 lo = hk[0], hi = hk[1];
         lr_mma_tf32(d, lo.x, 0.f, lo.y, 0.f, lr_unpack2<T>(w[j][k].x));
         lr_mma_tf32(d, lo.z, 0.f, lo.w, 0.f, lr_unpack2<T>(w[j][k].y));
         lr_mma_tf32(d, hi.x, 0.f, hi.y, 0.f, lr_unpack2<T>(w[j][k].z));
@@ -1066,7 +1068,9 @@ __global__ void __launch_bounds__(160) lr_wgrad_kernel(const LrPlan p, const LrW
 // fp16: H is tf32, which tcgen05 takes with the contraction contiguous alone; X and H lie the other way.  So the products are those of
 // mma.sync: a warp has 32 channels, ldmatrix turns X on the way to the fragments, its numbers become tf32 there (they all are), and a
 // lane takes two neighbouring ranks as the n of two products.  Rows in stages of 32, three of them, or one where the adapters have no
-// more rows than that on average.
+// more rows than that on average.  12090 rows of 5120 and 5120, rank 32: 103 us (tcgen05 with bf16 operands 49, their bytes 38), by 16
+// warps to an SM that take turns at copies, conversions and products; training steps of 512 rows of 64 adapters, rank 64, 5120 -> 5120
+// take 153 us, bf16 144.
 constexpr int LR_WROWS = 32;
 template <int RPM, int ST>
 struct LrWgradWideCfg {
@@ -1145,8 +1149,8 @@ __global__ void __launch_bounds__(128, LrWgradWideCfg<RPM, ST>::CTAS)
 #pragma unroll
       for (int b = 0; b < RPM / 16; ++b) {
         if (16 * b >= rp) break;
-        const float2 h0 = *reinterpret_cast<const float2*>(h + 16 * b), h1 = *reinterpret_cast<const float2*>(h + ldh + 16 * b);
-        const float2 h8 = *reinterpret_cast<const float2*>(h + 8 * ldh + 16 * b), h9 = *reinterpret_cast<const float2*>(h + 9 * ldh + 16 * b);
+        auto ranks = [&](int row) { return *reinterpret_cast<const float2*>(h + row * ldh + 16 * b); };
+        const float2 h0 = ranks(0), h1 = ranks(1), h8 = ranks(8), h9 = ranks(9);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
           lr_mma_tf32(acc[m][b][0], a[m][0].x, a[m][1].x, a[m][0].y, a[m][1].y, make_float2(h0.x, h1.x));
@@ -1258,7 +1262,8 @@ __global__ void __launch_bounds__(256) lr_join_kernel(const LrPlan p, const LrWg
 // 512 rows 19.9, 20.8; rank 128 64 rows 23, 27, 256 rows 34, 28), and where most adapters have no more than eight rows anyway.
 static bool lr_are_few(int64_t M, int64_t R, int rank) { return M <= 8 * R || (M <= 512 && M * lr_rp(rank) <= 12288); }
 // CTAs that share the first product of a tile of few rows: some four to an SM in all, of four blocks of 32 columns at least,
-// and 16 at most (their parts are added up by every CTA of the second product)
+// and 16 at most (their parts are added up by every CTA of the second product).  The SMs are B200's number, not the device's: the
+// workspace goes by it, whose size is asked with any device current.
 static int lr_few_splits(int64_t tiles, int64_t K) {
   const int64_t most = K / 128 < 16 ? K / 128 : 16, want = 4 * 148 / tiles;
   return static_cast<int>(want > most ? (most < 1 ? 1 : most) : want < 1 ? 1 : want);

@@ -15,9 +15,9 @@
 // rotation's four butterfly digits are then two in registers and two over the 16 threads, through shared memory as in rotq.cuh.  The
 // gradients need no rotation and have twice 8 channels, 128 apart (four times 4: 160 us where this takes 130, 12090 x 5376).  CTAs are
 // persistent; while rows are worked on, the next ones come into shared memory as bulk copies of whole rows (held in registers instead,
-// they left room for 10 warps to an SM: 763 us).  What is left above the floor is the work itself: some 29 instructions a channel at
-// 20 warps to an SM (30 warps of 64 registers spill: 580 us).  w, gate, scale and shift come from L1 every time: 4 bytes a channel
-// and pair of rows.
+// they left room for 10 warps to an SM: 763 us).  What is left above the floor: some 29 instructions a channel take
+// 59 % of the issue slots, and the CTA's two barriers a round are the largest stall of its 20 warps to an SM (30 warps of 64 registers
+// spill: 580 us).  w, gate, scale and shift come from L1 every time: 4 bytes a channel and pair of rows.
 #pragma once
 #include <atomic>
 #include <type_traits>
@@ -571,7 +571,7 @@ static int rn_sms() {
   }
   return sms;
 }
-// CTAs of up to 320 threads, as many to an SM as its registers and its shared memory allow
+// CTAs of up to RN_THREADS, RN_MORE or RN_LARGE threads, as many to an SM as its registers and its shared memory allow
 static RnShape rn_shape(int64_t M, int K, bool codes, bool backward) {
   RnShape s{};
   s.T = (K + 255) / 256 * 16;

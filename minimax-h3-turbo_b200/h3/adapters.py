@@ -306,7 +306,8 @@ def low_rank(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, plan: Optional[A
     """out_i = base_i + s_g (x_i A_g^T) B_g^T for x [..., K] -> [..., N], or (out, hidden) with return_hidden.
 
     a [adapters, rank, K] and b [adapters, N, rank] (or [rank, K] and [N, rank]: one adapter, which without a plan has every
-    row); bf16 or fp16 as x, ranks up to 128, K and N multiples of 8.  plan: the batch's, from `plan`.  base [..., N]: what the
+    row); bf16 or fp16 as x, ranks up to 128, K and N multiples of 8.  Adapters of one call have one rank: lower ones are filled
+    up with zeros.  Adapters without rows are not read, but the launches allow for them: pass those in use where there are many.  plan: the batch's, from `plan`.  base [..., N]: what the
     shared projection gave (None: zeros).  scales: a number or fp32 [adapters].  out: a [..., N] tensor to write, which may be
     base itself (its rows without an adapter are then not touched) and overlaps nothing else; not with gradients, its own
     included.

@@ -292,7 +292,7 @@ def linear(r: ResidualNorm, w: Weight, bias: Optional[torch.Tensor] = None, *, q
     """The linear that reads h: a W4A8 weight of ConvRot 256 from the codes, any other from hidden."""
     if reads_codes(w):
         if torch.is_grad_enabled() and bias is not None and bias.requires_grad:
-            raise RuntimeError("residual.linear: a W4A8 projection has no gradient for bias; add the bias outside, or use a dense weight")
+            raise RuntimeError("residual.linear: a W4A8 projection has no gradient for bias; add it outside, or use a dense weight")
         if r.codes is None:
             raise ValueError("residual.linear: a W4A8 weight of ConvRot 256 reads the codes; ask residual_norm for them")
         if w.q.shape[1] * 2 != r.codes.shape[1]:

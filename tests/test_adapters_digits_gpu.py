@@ -185,8 +185,8 @@ def test_training_steps_captured_and_in_two_streams(m, r, adapters):
     assert same(captured, other)
 
 
-@pytest.mark.parametrize("m,k,n,r,adapters", [(1, 136, 264, 33, 1), (5, 136, 264, 8, 2), (8, 520, 136, 64, 8), (20, 264, 392, 24, 3), (60, 512, 136, 128, 8),
-                                              (200, 256, 264, 16, 2)])
+@pytest.mark.parametrize("m,k,n,r,adapters", [(1, 136, 264, 33, 1), (5, 136, 264, 8, 2), (8, 520, 136, 64, 8), (20, 264, 392, 24, 3),
+                                              (60, 512, 136, 128, 8), (200, 256, 264, 16, 2)])
 def test_few_bf16_rows_have_hidden_rows_of_11_digits(m, k, n, r, adapters):
     """Rows by eights: beside bf16 operands too, what is rounded to 8 digits is the result alone."""
     x, a, b, _, rows = spread(m, k, n, r, adapters, torch.bfloat16, m)

@@ -43,7 +43,8 @@ def test_stream_and_hidden_rows(m, k, mods, kind, dtype):
             assert torch.equal(xs[1 - target], (y, x)[target])
 
 
-@pytest.mark.parametrize("w_dtype,m_dtype", [(torch.float32, torch.float32), (torch.float16, torch.float32), (torch.float32, torch.bfloat16)])
+@pytest.mark.parametrize("w_dtype,m_dtype", [(torch.float32, torch.float32), (torch.float16, torch.float32),
+                                             (torch.float32, torch.bfloat16)])
 @pytest.mark.parametrize("k", [264, 1288, 8200])
 def test_types_of_weight_and_modulation(k, w_dtype, m_dtype):
     m = 19
